@@ -37,6 +37,9 @@ LIBRARIES: Dict[str, str] = {
     "gemm_stream": "gemm_stream.cu",
     "gemm_tc5": "gemm_tc5.cu",
     "gemm_pair": "gemm_pair.cu",
+    "gemm_fp8": "gemm_fp8.cu",
+    "rows_fp8": "rows_fp8.cu",
+    "logprobs": "logprobs.cu",
     "attention_generic": "attention_generic.cu",
     "attention_f32": "attention_f32.cu",
     "attention_flash": "attention_flash.cu",
@@ -63,6 +66,8 @@ EXTRA_DEPS: Dict[str, List[str]] = {
     "decode_attention_noalloc": ["attention_flash.cu", "decode_attention_noalloc.h"],
     "gemm_f32": ["tc5_ops.cuh"],
     "gemm_pair": ["tc5_ops.cuh"],
+    "gemm_fp8": ["tc5_ops.cuh", "fp8.cuh"],
+    "rows_fp8": ["fp8.cuh"],
     "gated_block": ["short_conv.cuh"],
     "attention_diff": ["short_conv.cuh", "mma_sync.cuh"],
     "qkv_prep": ["short_conv.cuh"],

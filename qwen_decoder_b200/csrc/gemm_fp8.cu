@@ -1,0 +1,725 @@
+// Contraction Y[T, N] = X[T, K] * W[N, K]^T of rows in 8 bits (fp8.cuh) on the tensor cores, which apply the scales themselves:
+//
+//   Y[t, n] = sum_b 2^(ex[t, b] + ew[n, b]) sum_{k in block b} x[t, k] w[n, k]
+//
+// tcgen05.mma kind::mxf8f6f4 with block scaling takes e4m3 operands from shared memory (TMA tensor copies, 128-byte swizzle, a block of
+// 128 k to a stage), float32 sums in tensor memory and the scales, bytes of exponents, from tensor memory too: lane l, column c of a
+// tile's scales holds the scales of row 32 c + l, the same in all four quarters of the lanes.  A column's word has four bytes and the
+// instruction says which one it takes, so a word is the scales of four blocks of 128 k: exactly four neighbouring bytes of a row of
+// scales.  Four warps of a CTA bring these words: one load to a word, one tcgen05.st to a quarter.
+//
+// One CTA to a tile of up to 128 tokens, or (``CG`` 2) two to a tile of up to 256: each brings its own tokens and half of the weights'
+// rows, the tensor cores of both read both halves.  A worker (a CTA or a pair) goes through its items one after the other with two
+// accumulators in turn, so that an item's epilogue runs under the next one's MMAs.  512 columns of tensor memory hold two buffers of
+// scales (32 columns) and two accumulators of up to 240 columns; two of 256 overlap in 32 columns, which the epilogue reads first, and
+// then lets the next item's MMAs begin.
+//
+// Warps: 0..7 epilogue (two for each quarter of the lanes, columns halved between them), 8 producer, 9 MMAs, 10..13 scales.
+//
+// Epilogues: whole sums (+ bias) as bfloat16 or float32; the same of a K shared by the CTAs of a cluster, joined over their shared
+// memories in the order of the shares; the gated activation in 8 bits, where a tile has 128 features of the gate matrix and the same of
+// the up matrix, a block of the result's rows, whose largest magnitude the two warps of a row exchange.
+//
+// Every mbarrier wait is bounded; after one that ran out all roles run on to their ends with void results and a status word says
+// which wait it was.
+//
+// The reference has 16-bit products only (cublasHgemm, gpu_kernels.cu:431-436).
+#include "fp8.cuh"
+#include "tc5_ops.cuh"
+
+#define G8_EPI_WARPS 8
+#define G8_THREADS (14 * 32)
+#define G8_MAX_STAGES 16
+#define G8_SMEM (208 * 1024)                  // of stages
+#define G8_STAGE_ROWS (32 * 64)               // of a warp's epilogue: 64 bytes of each of its rows
+#define G8_SCALES 480                         // columns of the scales' two buffers, 16 each: 4 of the tokens', up to 8 of the weights'
+#define G8_OVERLAP 32                         // columns that two accumulators of 256 share (the first that the epilogue reads)
+
+#define G8_STORE 0
+#define G8_SHARED 1                           // K shared by a cluster
+#define G8_GATED 2
+
+struct G8Params {
+  int act, T, N, K;
+  int bn;                  // rows of W of a tile, of both CTAs together
+  int mrows;               // tokens of a CTA
+  int n_ft, n_tt, splits;
+  int kb_total, stages;
+  int feats;               // columns of the result
+  int vec;                 // rows of the result take 16-byte stores
+  long long ldo;           // elements
+  const unsigned char *sx, *sw;
+  long long ldsx, ldsw;
+  unsigned char* s_out;    // of the gated product
+  long long lds_out;
+};
+
+// ---- what a pair needs beyond tc5_ops.cuh
+__device__ __forceinline__ unsigned g8_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// where the first CTA of the pair has what this one has at ``p``: bit 24 of a shared-memory address is the place in the pair
+__device__ __forceinline__ unsigned g8_leader(const void* p) { return tc_smem(p) & 0xFEFFFFFFu; }
+__device__ __forceinline__ void g8_arrive_at(unsigned bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void g8_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void g8_load_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(tc_smem(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void g8_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned sa, unsigned sb,
+                                       bool accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate ? 1u : 0u) : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate ? 1u : 0u) : "memory");
+}
+// e4m3 operands, both K-major, scales of 8 exponent bits; the scales' byte is added for each MMA
+__device__ __forceinline__ unsigned g8_idesc(int m, int n) { return (unsigned)(n >> 3) << 17 | 1u << 23 | (unsigned)(m >> 4) << 24; }
+__device__ __forceinline__ unsigned g8_idesc_byte(unsigned i) { return i << 4 | i << 29; }
+// arrives at the barrier of both CTAs once the MMAs so far are done
+template <int CG>
+__device__ __forceinline__ void g8_commit(unsigned long long* bar) {
+  if (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(tc_smem(bar)), "h"((unsigned short)3) : "memory");
+  else tc_commit(bar);
+}
+__device__ __forceinline__ void g8_ld16(unsigned addr, float (&v)[16]) {
+  unsigned r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void g8_st4(unsigned addr, const unsigned* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
+// a row's scales of ``there`` blocks of 128 k, up to four
+__device__ __forceinline__ unsigned g8_scales(const unsigned char* s, int there) {
+  if (there == 4) return *reinterpret_cast<const unsigned*>(s);
+  unsigned v = s[0];
+  if (there > 1) v |= s[1] << 8;
+  if (there > 2) v |= s[2] << 16;
+  return v;
+}
+
+// A worker's item
+struct G8Item { int tt, ft, kb0, kb1; };
+__device__ __forceinline__ G8Item g8_item(const G8Params& p, int item, int share) {
+  G8Item q;
+  q.tt = item % p.n_tt;
+  q.ft = item / p.n_tt;
+  q.kb0 = p.kb_total * share / p.splits;
+  q.kb1 = p.kb_total * (share + 1) / p.splits;
+  return q;
+}
+
+// The tensor cores cut a sum off at 24 bits with every addition, always towards zero: 4 additions to a block of 128 k, 2.7e-7 of the sum's
+// norm after 512 of k, 1.7e-6 after 3,584 (scales spread over 2^12).  A float32 result is therefore summed in pieces of 1,024 of k, which
+// the epilogue adds up with rounding (5e-7); what becomes bfloat16 is off by 1.7e-3 anyway and stays one sum.
+#define G8_PIECE 8
+#define G8_MAX_FLOAT_BN 128                   // of which a thread of the epilogue keeps half a row's sums
+template <typename TO>
+__device__ __forceinline__ int g8_piece_end(const G8Item& q, int kb) { return sizeof(TO) == 4 ? min(kb + G8_PIECE, q.kb1) : q.kb1; }
+
+__device__ __forceinline__ void g8_bias16(float (&v)[16], const float* bias, int col, int feats) {
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    if (col + i < feats) v[i] += bias[col + i];
+}
+// 16 numbers as pieces of 16 bytes of a row of 64 in a warp's part of shared memory.  Rows lie side by side, the pieces of rows
+// 2 i and 2 i + 1 turned by i: eight lanes that write or read together meet no bank twice.
+__device__ __forceinline__ uint4* g8_piece(unsigned char* rows, int row, int piece) {
+  return reinterpret_cast<uint4*>(rows + row * 64 + ((piece ^ (row >> 1 & 3)) << 4));
+}
+__device__ __forceinline__ unsigned g8_bf16x2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+template <typename TO>
+__device__ __forceinline__ void g8_stage16(unsigned char* rows, int row, int piece, const float (&v)[16]) {
+  if (sizeof(TO) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      *g8_piece(rows, row, piece + i) = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                                   __float_as_uint(v[4 * i + 3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      *g8_piece(rows, row, piece + i) = make_uint4(g8_bf16x2(v[8 * i], v[8 * i + 1]), g8_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                                                   g8_bf16x2(v[8 * i + 4], v[8 * i + 5]), g8_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+  }
+}
+// The first ``pieces`` of the four pieces of each of a warp's first ``n_rows`` rows to memory, ``left`` elements of a row from ``dst`` on
+template <typename TO>
+__device__ __forceinline__ void g8_store_rows(unsigned char* rows, TO* dst, long long ld, int n_rows, int pieces, int left, bool vec) {
+  constexpr int E = 16 / (int)sizeof(TO);
+  const int lane = threadIdx.x & 31, piece = lane & 3, e0 = piece * E;
+  if (piece >= pieces || e0 >= left) return;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = 8 * i + (lane >> 2);
+    if (r >= n_rows) break;
+    const uint4* src = g8_piece(rows, r, piece);
+    TO* to = dst + (size_t)r * ld + e0;
+    if (vec && e0 + E <= left) *reinterpret_cast<uint4*>(to) = *src;
+    else
+      for (int e = 0; e < E && e0 + e < left; e++) to[e] = reinterpret_cast<const TO*>(src)[e];
+  }
+}
+
+template <int EPI, typename TO, int CG>
+__global__ void __launch_bounds__(G8_THREADS, 1)
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ bias,
+                TO* __restrict__ out, const G8Params p, int* __restrict__ status) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_ready[2], acc_free[2], scales_full[2], scales_empty[2];
+  __shared__ unsigned tmem_slot, peaks[4][2][32];
+  __shared__ int dead;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)g8_rank() : 0;
+  const int share = EPI == G8_SHARED ? (int)g8_rank() : 0;
+  unsigned char* base = smem_raw + ((1024 - (tc_smem(smem_raw) & 1023)) & 1023);
+  // The stages' tokens lie before the stages' weights: an MMA reads 128 rows of tokens whatever a CTA has, and what lies behind
+  // them is then always there.
+  const int a_bytes = p.mrows * 128, b_bytes = p.bn / CG * 128;
+  unsigned char* a_s = base;
+  unsigned char* b_s = base + (size_t)p.stages * a_bytes;
+  if (threadIdx.x == 0) {
+    dead = 0;
+    for (int s = 0; s < p.stages; s++) { tc_bar_init(&full[s], 1); tc_bar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; b++) {
+      tc_bar_init(&acc_ready[b], 1);
+      tc_bar_init(&acc_free[b], CG * G8_EPI_WARPS);
+      tc_bar_init(&scales_full[b], CG * 4);
+      tc_bar_init(&scales_empty[b], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (CG == 2) g8_cluster_sync();
+
+  const int per = EPI == G8_SHARED ? p.splits : CG;
+  const int worker = blockIdx.x / per, n_workers = gridDim.x / per, n_items = p.n_ft * p.n_tt;
+  const int half = p.bn >> 1;
+  const bool overlap = p.bn > 240;
+  const unsigned acc_step = overlap ? 256 - G8_OVERLAP : 240;
+  auto row_x = [&](const G8Item& q) { return (CG * q.tt + rank) * p.mrows; };
+  // the first row of W of the part ``h`` (0: first half, 1: second) of an item's tile
+  auto row_w = [&](const G8Item& q, int h) { return EPI == G8_GATED ? q.ft * half + h * p.feats : q.ft * p.bn + h * half; };
+
+  if (warp == G8_EPI_WARPS) {
+    // ------------------------------------------------------------------ producer
+    // (the whole warp goes through the loop and one lane issues: addresses and coordinates are then known to be the same for all lanes)
+    const bool one = tc_elect();
+    const unsigned bytes = (unsigned)(CG * (a_bytes + b_bytes));
+    auto load = [&](unsigned char* dst, const CUtensorMap* map, int x, int y, int s) {
+      if (CG == 2) g8_load_2d(dst, map, x, y, g8_leader(&full[s]));
+      else tc_load_2d(dst, map, x, y, &full[s]);
+    };
+    auto tokens = [&](int s, const G8Item& q, int kb) { load(a_s + s * a_bytes, &map_x, kb * FP8_BLOCK, row_x(q), s); };
+    auto weights = [&](int s, const G8Item& q, int kb) {
+      if (CG == 1 || rank == 0) tc_expect_tx(&full[s], bytes);
+      load(b_s + s * b_bytes, &map_w, kb * FP8_BLOCK, row_w(q, rank), s);
+      if (CG == 1 && EPI == G8_GATED) load(b_s + s * b_bytes + half * 128, &map_w, kb * FP8_BLOCK, row_w(q, 1), s);
+    };
+    int item = worker, n = 0;
+    G8Item q = g8_item(p, item, share);
+    int kb = q.kb0;
+    auto next = [&](int& it, G8Item& i, int& k) {
+      if (++k < i.kb1) return;
+      it += n_workers;
+      if (it < n_items) i = g8_item(p, it, share);
+      k = i.kb0;
+    };
+    int item_t = item, kb_t = kb;
+    G8Item q_t = q;
+    for (; n < p.stages && item < n_items; n++, next(item, q, kb))
+      if (one) weights(n, q, kb);
+    pdl_wait();
+    for (int s = 0; s < n; s++, next(item_t, q_t, kb_t))
+      if (one) tokens(s, q_t, kb_t);
+    int s = n == p.stages ? 0 : n;
+    unsigned ph = 0;
+    for (; item < n_items; next(item, q, kb)) {
+      if (!tc_wait(&empty[s], ph, &dead)) atomicExch(status, 1);
+      if (one) {
+        weights(s, q, kb);
+        tokens(s, q, kb);
+      }
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+    // the commits' last arrivals at this CTA's barriers come before it may go
+    for (int i = 0; i < n; i++) {
+      if (n == p.stages) {
+        if (!tc_wait(&empty[s], ph, &dead)) atomicExch(status, 1);
+        if (++s == p.stages) { s = 0; ph ^= 1; }
+      } else if (!tc_wait(&empty[i], 0, &dead)) {
+        atomicExch(status, 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == G8_EPI_WARPS + 1) {
+    // ------------------------------------------------------------------ MMAs
+    if (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_slot)), "r"(512u) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tc_alloc(&tmem_slot, 512);
+    }
+    // (not before this CTA has its tensor memory: the next kernel's CTA beside it might take that, and then wait for this one)
+    pdl_launch_dependents();
+    tc_fence_before();
+    asm volatile("bar.sync 1, %0;" ::"n"(G8_EPI_WARPS * 32 + 160) : "memory");
+    tc_fence_after();
+    if (rank == 0) {
+      const bool one = tc_elect();
+      const unsigned tmem = tmem_slot;
+      const unsigned idesc = g8_idesc(128 * CG, p.bn);
+      const unsigned long long a0 = tc_desc_sw128(tc_smem(a_s)), b0 = tc_desc_sw128(tc_smem(b_s));
+      const unsigned a_step = (unsigned)a_bytes >> 4, b_step = (unsigned)b_bytes >> 4;
+      int s = 0, n = 0;
+      unsigned ph = 0, sc = 0, sc_ph = 0;
+      for (int item = worker; item < n_items; item += n_workers) {
+        const G8Item q = g8_item(p, item, share);
+        for (int k0 = q.kb0; k0 < q.kb1; n++) {
+          const int k1 = g8_piece_end<TO>(q, k0);
+          const unsigned buf = n & 1;
+          // accumulators apart: the sum before the last has been read; overlapping: of the last one the common columns have
+          const int of = overlap ? n - 1 : n - 2;
+          if (of >= 0 && !tc_wait(&acc_free[of & 1], of >> 1 & 1, &dead)) atomicExch(status, 3);
+          tc_fence_after();
+          const unsigned d = tmem + buf * acc_step;
+          for (int kb = k0; kb < k1; kb++) {
+            if ((kb == q.kb0 || !(kb & 3)) && !tc_wait(&scales_full[sc], sc_ph, &dead)) atomicExch(status, 5);
+            if (!tc_wait(&full[s], ph, &dead)) atomicExch(status, 2);
+            tc_fence_after();
+            const unsigned long long da = a0 + s * a_step, db = b0 + s * b_step;
+            const unsigned id = idesc | g8_idesc_byte(kb & 3), sa = tmem + G8_SCALES + 16 * sc;
+            const bool last = kb + 1 == q.kb1 || (kb & 3) == 3;
+            if (one) {
+#pragma unroll
+              for (int k = 0; k < FP8_BLOCK / 32; k++) g8_mma<CG>(d, da + 2 * k, db + 2 * k, id, sa, sa + 4, k > 0 || kb > k0);
+              g8_commit<CG>(&empty[s]);
+              if (last) g8_commit<CG>(&scales_empty[sc]);
+            }
+            if (last && ++sc == 2) { sc = 0; sc_ph ^= 1; }
+            if (++s == p.stages) { s = 0; ph ^= 1; }
+          }
+          if (one) g8_commit<CG>(&acc_ready[buf]);
+          k0 = k1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= G8_EPI_WARPS + 2) {
+    // ------------------------------------------------------------------ scales
+    asm volatile("bar.sync 1, %0;" ::"n"(G8_EPI_WARPS * 32 + 160) : "memory");
+    tc_fence_after();
+    const unsigned at = tmem_slot + ((unsigned)(warp & 3) << 21) + G8_SCALES;
+    const int wcols = p.bn >> 5;
+    pdl_wait();
+    unsigned sc = 0, ph = 1;
+    int words = 0;
+    for (int item = worker; item < n_items; item += n_workers) {
+      const G8Item q = g8_item(p, item, share);
+      const int x0 = row_x(q) + lane;
+      for (int kw = q.kb0 >> 2; kw <= (q.kb1 - 1) >> 2; kw++, words++) {
+        unsigned v[12];
+        const int there = min(4, p.kb_total - 4 * kw);       // a row's last word may not be whole
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int m = 32 * c + lane;
+          v[c] = m < p.mrows && x0 + 32 * c < p.T ? g8_scales(p.sx + (x0 + 32 * c) * p.ldsx + 4 * kw, there) : 0;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+          const int j = 32 * c + lane, h = j >= half, row = row_w(q, h) + j - (h ? half : 0);
+          v[4 + c] = c < wcols && row < p.N ? g8_scales(p.sw + row * p.ldsw + 4 * kw, there) : 0;
+        }
+        if (!tc_wait(&scales_empty[sc], ph, &dead)) atomicExch(status, 6);
+        tc_fence_after();
+        g8_st4(at + 16 * sc, v);
+        g8_st4(at + 16 * sc + 4, v + 4);
+        if (wcols > 4) g8_st4(at + 16 * sc + 8, v + 8);
+        tc_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) g8_arrive_at(g8_leader(&scales_full[sc]));
+          else tc_arrive(&scales_full[sc]);
+        }
+        if (++sc == 2) { sc = 0; ph ^= 1; }
+      }
+    }
+    // the commits' last arrivals at these barriers, too
+    for (int i = 0; i < min(words, 2); i++) {
+      if (words < 2) { sc = 0; ph = 0; }
+      if (!tc_wait(&scales_empty[sc], ph, &dead)) atomicExch(status, 6);
+      if (++sc == 2) { sc = 0; ph ^= 1; }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    asm volatile("bar.sync 1, %0;" ::"n"(G8_EPI_WARPS * 32 + 160) : "memory");
+    tc_fence_after();
+    const int quarter = (warp & 3) * 32, side = warp >> 2;
+    const unsigned tmem = tmem_slot + ((unsigned)quarter << 16);
+    unsigned char* rows = b_s + (size_t)p.stages * b_bytes + warp * G8_STAGE_ROWS;
+    auto release = [&](unsigned buf) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) g8_arrive_at(g8_leader(&acc_free[buf]));
+        else tc_arrive(&acc_free[buf]);
+      }
+    };
+    // 16 columns of a share of K as float32, a row's pieces turned by the row: what the cluster adds up
+    auto keep16 = [&](const float (&v)[16], int g) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        *reinterpret_cast<float4*>(base + (size_t)(quarter + lane) * p.bn * 4 + ((4 * g + e ^ (lane & 7)) << 4)) =
+            make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+    };
+    int n = 0;
+    auto wait_sum = [&]() {
+      if (!tc_wait(&acc_ready[n & 1], n >> 1 & 1, &dead, 64) && lane == 0) atomicExch(status, 4);
+      tc_fence_after();
+    };
+    for (int item = worker; item < n_items; item += n_workers) {
+      const G8Item q = g8_item(p, item, share);
+      const int tok0 = row_x(q) + quarter;                   // of this warp's rows the first, and how many there are
+      const int n_rows = min(32, min(p.mrows - quarter, p.T - tok0));
+      const int groups = p.bn / 16, g0 = groups * side / 2, g1 = groups * (side + 1) / 2;     // this side's 16s of columns
+      if constexpr (sizeof(TO) == 4) {
+        constexpr int MOST = G8_MAX_FLOAT_BN / 32;
+        float sum[MOST][16];
+        for (int k0 = q.kb0; k0 < q.kb1; k0 = g8_piece_end<TO>(q, k0), n++) {
+          wait_sum();
+          const unsigned acc = tmem + (n & 1) * acc_step;
+          if (n_rows > 0) {                                  // whole warps: the loads are collective
+#pragma unroll
+            for (int i = 0; i < MOST; i++)
+              if (i < g1 - g0) {
+                float v[16];
+                g8_ld16(acc + 16 * (g0 + i), v);
+                tc_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; e++) sum[i][e] = k0 == q.kb0 ? v[e] : sum[i][e] + v[e];
+              }
+          }
+          release(n & 1);
+        }
+        if (n_rows > 0) {
+#pragma unroll
+          for (int i = 0; i < MOST; i++)
+            if (i < g1 - g0) {
+              const int col = q.ft * p.bn + 16 * (g0 + i);
+              if constexpr (EPI == G8_SHARED) {
+                if (lane < n_rows) keep16(sum[i], g0 + i);
+              } else {
+                if (bias) g8_bias16(sum[i], bias, col, p.feats);
+                __syncwarp();
+                g8_stage16<TO>(rows, lane, 0, sum[i]);
+                __syncwarp();
+                g8_store_rows<TO>(rows, out + (size_t)tok0 * p.ldo + col, p.ldo, n_rows, 4, p.feats - col, p.vec);
+              }
+            }
+        }
+        continue;
+      }
+      const unsigned buf = n & 1;
+      wait_sum();
+      n++;
+      const unsigned acc = tmem + buf * acc_step;
+      // which side has the columns that overlap with the next item's: the first accumulator's last, the second's first
+      const bool owner = overlap && side == (buf == 0);
+      if (overlap && (!owner || n_rows <= 0)) release(buf);
+      if constexpr (EPI == G8_GATED) {
+        if (n_rows > 0) {                                    // whole warps: the loads are collective
+          float h[2][32];
+          unsigned peak = 0;
+          const bool back = side == 1;                       // the second side starts with its last 32 features
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const int f0 = 64 * side + 32 * (back ? 1 - c : c);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              float g[16], u[16];
+              g8_ld16(acc + f0 + 16 * i, g);
+              g8_ld16(acc + 128 + f0 + 16 * i, u);
+              tc_ld_wait();
+              if (c == 0 && i == 1 && owner) release(buf);
+              const int col = q.ft * 128 + f0 + 16 * i;
+              if (bias) {
+                g8_bias16(g, bias, col, p.feats);
+                g8_bias16(u, bias + p.feats, col, p.feats);
+              }
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const float a = col + e < p.feats ? fp8_gated(g[e], u[e], p.act) : 0.f;
+                h[c][16 * i + e] = a;
+                peak = max(peak, fp8_magnitude(a));
+              }
+            }
+          }
+          peaks[warp & 3][side][lane] = peak;
+          asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+          peak = max(peak, peaks[warp & 3][side ^ 1][lane]);
+          const unsigned byte = fp8_scale_byte(peak);
+          const float inv = fp8_inverse(byte);
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            unsigned w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              w[i] = fp8_pack4(h[c][4 * i] * inv, h[c][4 * i + 1] * inv, h[c][4 * i + 2] * inv, h[c][4 * i + 3] * inv);
+            const int piece = 2 * (back ? 1 - c : c);
+            *g8_piece(rows, lane, piece) = make_uint4(w[0], w[1], w[2], w[3]);
+            *g8_piece(rows, lane, piece + 1) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+          __syncwarp();
+          const int col = q.ft * 128 + 64 * side;
+          g8_store_rows<unsigned char>(rows, (unsigned char*)out + (size_t)tok0 * p.ldo + col, p.ldo, n_rows, 4, p.feats - col, p.vec);
+          if (side == 0 && lane < n_rows) p.s_out[(size_t)(tok0 + lane) * p.lds_out + q.ft] = (unsigned char)byte;
+          asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");        // the peaks have been read
+        }
+      } else if (n_rows > 0) {
+        const int passes = (g1 - g0 + 1) / 2;
+        for (int i = 0; i < passes; i++) {
+          const int g = owner && side ? g1 - 2 * (i + 1) : g0 + 2 * i;
+          const int w = min(2, g1 - g);                      // 64 bytes of every row, or what is left of the columns
+          float v[2][16];
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            if (j < w) g8_ld16(acc + 16 * (g + j), v[j]);
+          tc_ld_wait();
+          if (owner && i == 0) release(buf);
+          __syncwarp();
+          const int col = q.ft * p.bn + 16 * g;
+          if constexpr (EPI == G8_SHARED) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+              if (j < w && lane < n_rows) keep16(v[j], g + j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+              if (j < w) {
+                if (bias) g8_bias16(v[j], bias, col + 16 * j, p.feats);
+                g8_stage16<TO>(rows, lane, 2 * j, v[j]);
+              }
+            __syncwarp();
+            g8_store_rows<TO>(rows, out + (size_t)tok0 * p.ldo + col, p.ldo, n_rows, 2 * w, p.feats - col, p.vec);
+          }
+        }
+      }
+      if (!overlap) release(buf);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (EPI == G8_SHARED) {
+    g8_cluster_sync();
+    // this CTA's share of the tile's pieces of four features, summed in the order of the shares of K
+    const G8Item q = g8_item(p, worker, share);
+    const int tok0 = q.tt * p.mrows, n_rows = min(p.mrows, p.T - tok0), pieces = p.bn >> 2, total = n_rows * pieces;
+    const unsigned at = tc_smem(base);
+    const int e1 = (int)((long long)total * (share + 1) / p.splits);
+    for (int e = (int)((long long)total * share / p.splits) + threadIdx.x; e < e1; e += G8_THREADS) {
+      const int r = e / pieces, c = e - r * pieces, col = q.ft * p.bn + 4 * c;
+      const unsigned from = at + (r * pieces + (c ^ (r & 7))) * 16;
+      float4 v[8];
+#pragma unroll
+      for (int sp = 0; sp < 8; sp++)
+        if (sp < p.splits) {
+          unsigned remote;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(from), "r"(sp));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[sp].x), "=f"(v[sp].y), "=f"(v[sp].z), "=f"(v[sp].w) : "r"(remote) : "memory");
+        }
+      float4 t = v[0];
+#pragma unroll
+      for (int sp = 1; sp < 8; sp++)
+        if (sp < p.splits) { t.x += v[sp].x; t.y += v[sp].y; t.z += v[sp].z; t.w += v[sp].w; }
+      const float f[4] = {t.x, t.y, t.z, t.w};
+      TO* to = out + (size_t)(tok0 + r) * p.ldo + col;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (col + i < p.feats) to[i] = from_float<TO>(f[i] + (bias ? bias[col + i] : 0.f));
+    }
+  }
+  if (CG == 2 || EPI == G8_SHARED) g8_cluster_sync();
+  if (warp == G8_EPI_WARPS + 1) {
+    tc_fence_after();
+    if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(512u) : "memory");
+    else tc_dealloc(tmem_slot, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------ host
+static int* g_status[64];
+static int* status_word() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!g_status[dev]) {
+    int* ptr = nullptr;
+    if (cudaMalloc(&ptr, sizeof(int)) != cudaSuccess) return nullptr;
+    cudaMemset(ptr, 0, sizeof(int));
+    g_status[dev] = ptr;
+  }
+  return g_status[dev];
+}
+
+static int up(int a, int b) { return (a + b - 1) / b; }
+
+// How a product is cut: *cg CTAs to a tile of tokens, *bn rows of W to a tile, K in *splits shares (of a cluster).
+extern "C" int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out) {
+  epi &= 255;
+  const int most = epi == G8_STORE && out_dtype == QD_F32 ? G8_MAX_FLOAT_BN : 256;
+  if (T <= 0 || N <= 0 || K <= 0 || sms < 2) return 0;
+  const int kb = up(K, FP8_BLOCK);
+  const double dram = (double)N * K / 3300.0;          // clocks of 1.9 GHz
+  double best = 0;
+  for (int cg = T <= 128 ? 1 : 2; cg >= 1; cg--) {
+    const int workers = sms / cg, n_tt = up(T, 128 * cg), mrows = up(up(T, cg * n_tt), 8) * 8;
+    for (int bn = epi == G8_GATED ? 256 : 32; bn <= most; bn += 32) {
+      const long long tiles = (long long)up(epi == G8_GATED ? N / 2 : N, epi == G8_GATED ? bn / 2 : bn) * n_tt;
+      for (int splits = 1; splits <= (epi == G8_GATED || cg == 2 ? 1 : 8) && (splits == 1 || splits * 4 <= kb); splits++) {
+        if (splits > 1 && tiles * splits > sms) break;
+        const long long rounds = splits > 1 ? 1 : (tiles + workers - 1) / workers;
+        const double bytes = (mrows + bn / cg) * 128 / 60.0;
+        double block = 2.0 * bn;
+        if (block < bytes) block = bytes;
+        if (block < 350) block = 350;
+        const double work = (double)rounds * up(kb, splits) * block;
+        double cost = work > dram ? work + 0.15 * dram : dram + 0.15 * work;
+        cost += 12.0 * bn + (splits > 1 ? 1500.0 : 0.0);
+        if (best == 0 || cost < best) { best = cost; *cg_out = cg; *bn_out = bn; *splits_out = splits; }
+      }
+    }
+  }
+  return 1;
+}
+
+template <int EPI, typename TO, int CG>
+static int g8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const float* bias, void* out, const G8Params& p, int* status,
+                     int ctas, size_t smem, cudaStream_t stream) {
+  cudaFuncSetAttribute(gemm_fp8_kernel<EPI, TO, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(G8_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = EPI == G8_SHARED ? p.splits : CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = qd_pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<EPI, TO, CG>, map_w, map_x, bias, (TO*)out, p, status);
+  return qd_last_error();
+}
+
+// rows x cols bytes, rows ``ld`` bytes apart; boxes of box_rows rows of 128 bytes, 128-byte swizzle, zeros outside
+static bool g8_make_map(CUtensorMap* map, const void* base, long long rows, long long cols, int box_rows, long long ld) {
+  TcEncodeFn fn = tc_encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// X [T, K] and W [N, K] e4m3, rows ``ldx`` and ``ldw`` bytes apart (multiples of 16, as the addresses), with scales sx and sw, rows
+// ``ldsx`` and ``ldsw`` bytes apart (multiples of 4, as the addresses).  epi 0: out [T, N] = X W^T (+ bias
+// float32 [N]), bfloat16 or float32, rows ``ldo`` apart; ``splits`` > 1: K shared by clusters of so many CTAs (up to 8), a tile to each.
+// epi 2 (+ 256 * QD_ACT_*): W [2F, K] the gate's rows, then up's; out e4m3 [T, F] = act(X Wg^T) * (X Wu^T), rows ``ldo`` bytes apart
+// (a multiple of 4), and its scales s_out, rows ``lds_out`` apart.  ``cg``: CTAs to a tile of tokens, 1 (up to 128) or 2 (up to 256);
+// ``bn``: rows of W to a tile, a multiple of 32 up to 256 (256 for epi 2).
+extern "C" int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
+                           long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, void* s_out, long long lds_out,
+                           int T, int N, int K, int cg, int bn, int splits, int epi, int sms, cudaStream_t stream) {
+  if (T <= 0 || N <= 0) return 0;
+  const int act = epi >> 8;
+  epi &= 255;
+  if (K <= 0 || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) || bn < 32 || bn > 256 || bn % 32 || splits < 1 ||
+      splits > 8 || sms < 2 || !out)
+    return QD_ERR_UNSUPPORTED;
+  if ((((uintptr_t)W | (uintptr_t)X) & 15) || (((uintptr_t)sw | (uintptr_t)sx) & 3) || ldsw % 4 || ldsx % 4) return QD_ERR_UNSUPPORTED;
+  if (epi == G8_GATED ? ((N & 1) || bn != 256 || splits != 1 || !s_out || ldo % 4 || (act != QD_ACT_SILU && act != QD_ACT_GELU_TANH))
+                      : epi != G8_STORE)
+    return QD_ERR_UNSUPPORTED;
+  G8Params p;
+  p.act = act; p.T = T; p.N = N; p.K = K; p.bn = bn; p.splits = splits; p.ldo = ldo;
+  p.sx = (const unsigned char*)sx; p.sw = (const unsigned char*)sw; p.ldsx = ldsx; p.ldsw = ldsw;
+  p.s_out = (unsigned char*)s_out; p.lds_out = lds_out;
+  p.kb_total = up(K, FP8_BLOCK);
+  if (ldsx < p.kb_total || ldsw < p.kb_total) return QD_ERR_UNSUPPORTED;
+  if (splits > p.kb_total || (splits > 1 && cg != 1) || (epi == G8_STORE && out_dtype == QD_F32 && bn > G8_MAX_FLOAT_BN)) return QD_ERR_UNSUPPORTED;
+  p.feats = epi == G8_GATED ? N / 2 : N;
+  p.n_tt = up(T, 128 * cg);
+  p.mrows = up(up(T, cg * p.n_tt), 8) * 8;           // the tokens evenly over the token tiles and their CTAs
+  p.n_ft = up(p.feats, epi == G8_GATED ? bn / 2 : bn);
+  const long long items = (long long)p.n_ft * p.n_tt;
+  if (items * splits > (1ll << 30)) return QD_ERR_UNSUPPORTED;
+  const int workers = splits > 1 ? (int)items : (int)(items < sms / cg ? items : sms / cg);
+  const int stage_bytes = (p.mrows + bn / cg) * 128;
+  p.stages = G8_SMEM / stage_bytes;
+  if (p.stages > G8_MAX_STAGES) p.stages = G8_MAX_STAGES;
+  p.vec = !((uintptr_t)out & 15) && ldo % (epi == G8_GATED ? 16 : out_dtype == QD_F32 ? 4 : 8) == 0;
+  // An MMA reads 128 rows of the last stage's tokens.  With fewer there are more stages, and the weights' stages behind them
+  // hold at least 16 x 32 rows.
+  const size_t smem = (size_t)p.stages * stage_bytes + G8_EPI_WARPS * G8_STAGE_ROWS + 1024;
+  // (a share's sums lie where the stages were: at most 128 KB, and with few rows or features the stages are as many)
+  if (splits > 1 && (size_t)p.mrows * bn * 4 > (size_t)p.stages * stage_bytes) return QD_ERR_UNSUPPORTED;
+  int* status = status_word();
+  CUtensorMap map_w, map_x;
+  const int box = epi == G8_GATED || cg == 2 ? bn / 2 : bn;
+  if (!status || !g8_make_map(&map_w, W, N, K, box, ldw) || !g8_make_map(&map_x, X, T, K, p.mrows, ldx)) return QD_ERR_UNSUPPORTED;
+#define GO(E, TO)                                                                                                      \
+  return cg == 2 ? g8_launch<E, TO, 2>(map_w, map_x, bias, out, p, status, 2 * workers, smem, stream)                   \
+                 : g8_launch<E, TO, 1>(map_w, map_x, bias, out, p, status, workers, smem, stream)
+#define GO1(E, TO) return g8_launch<E, TO, 1>(map_w, map_x, bias, out, p, status, workers * splits, smem, stream)
+  if (epi == G8_GATED) GO(G8_GATED, unsigned char);
+  if (splits > 1 && out_dtype == QD_BF16) GO1(G8_SHARED, bf16);
+  if (splits > 1 && out_dtype == QD_F32) GO1(G8_SHARED, float);
+  if (out_dtype == QD_BF16) GO(G8_STORE, bf16);
+  if (out_dtype == QD_F32) GO(G8_STORE, float);
+#undef GO
+#undef GO1
+  return QD_ERR_UNSUPPORTED;
+}
+
+// 0 if no bounded wait of this library's kernel has run out on the current device (1: producer, for a free stage; 2: MMAs, for
+// data; 3: MMAs, for a drained accumulator; 4: epilogue; 5: MMAs, for scales; 6: scales, for a free buffer).  Synchronises the device.
+QD_DEFINE_WAIT_PROBE(qd_gemm_fp8_wait_probe, tc_wait(bar, 0, dead, 0, poll_limit), status_word, 99)
+
+extern "C" int qd_gemm_fp8_status() {
+  int* status = status_word();
+  if (!status) return -1;
+  int v = 0;
+  if (cudaMemcpy(&v, status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
+  if (v) cudaMemset(status, 0, sizeof(int));
+  return v;
+}

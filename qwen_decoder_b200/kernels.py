@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os as _os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -842,6 +842,31 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                                          _ptr(draws), _ptr(out), _stream()), "sample")
 
 
+LOGPROBS_MAX_TOP = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """Of each row of ``logits`` [R, V] (float32 or bfloat16, rows may lie apart): (log probability of tokens[r], int32 [R]; entropy of
+    the row's distribution; ids int32 [R, top] of the ``top`` (up to 32) most probable tokens, the largest first and of equal ones the
+    lowest index first; their log probabilities), float32.  Logits of minus infinity have probability 0; a row of nothing else gives
+    minus infinity, entropy 0.  A row with a NaN or an infinity has none: NaN, and its ids are of the numbers there are (-1: none).  A
+    token outside of the row gives NaN."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise KernelError("token_logprobs: logits must be float32 or bfloat16 [R, V] with contiguous rows")
+    R, V = logits.shape
+    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (R,) or not tokens.is_contiguous():
+        raise KernelError(f"token_logprobs: tokens must be contiguous int32 [{R}]")
+    if V < 1 or not 0 <= top <= min(LOGPROBS_MAX_TOP, V):
+        raise KernelError(f"token_logprobs: top must be between 0 and {min(LOGPROBS_MAX_TOP, V)}, got {top}")
+    both = torch.empty((2, R), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((R, top), dtype=torch.int32, device=logits.device)
+    lps = torch.empty((R, top), dtype=torch.float32, device=logits.device)
+    _check(library("logprobs").qd_token_logprobs(
+        _ptr(logits), _I(dtype_code(logits.dtype)), _LL(logits.stride(0)), _ptr(tokens), _ptr(both[0]), _ptr(both[1]), _ptr(ids), _ptr(lps),
+        _I(R), _I(V), _I(top), _I(sm_count()), _stream()), "token_logprobs")
+    return both[0], both[1], ids, lps
+
+
 def prefill_tc5_supported(dtype, H: int, G: int, d: int, page_size: int) -> bool:
     """What the tcgen05 prefill attention takes: bfloat16, head size 64 or 128, up to 16 query heads per KV
     head, pages of a multiple of 16 tokens."""
@@ -874,6 +899,7 @@ def prefill_attention_tc5_status() -> int:
 _STATUS = {"gemm_stream": ("qd_gemm_stream_status", "qd_gemm_stream_wait_probe"),
            "gemm_tc5": ("qd_gemm_tc5_status", "qd_gemm_tc5_wait_probe"),
            "gemm_pair": ("qd_gemm_pair_status", "qd_gemm_pair_wait_probe"),
+           "gemm_fp8": ("qd_gemm_fp8_status", "qd_gemm_fp8_wait_probe"),
            "gemm_f32": ("qd_gemm_f32_status", "qd_gemm_f32_wait_probe"),
            "attention_tc5": ("qd_prefill_attention_tc5_status", "qd_prefill_attention_tc5_wait_probe"),
            "attention_flash": ("qd_decode_attention_tma_status", "qd_decode_attention_tma_wait_probe")}
@@ -899,6 +925,165 @@ def wait_probe(name: str, poll_limit: int = 2048) -> None:
     function, on an mbarrier that nobody arrives at.  The wait runs out, the kernel ends, and the next
     ``check_status`` raises.  For tests of that chain; it harms nothing else."""
     _check(getattr(library(name), _STATUS[name][1])(ctypes.c_uint(poll_limit), _stream()), f"{name} wait probe")
+
+
+# ------------------------------------------------------------------ rows and products in 8 bits
+FP8_BLOCK = 128        # features to a scale
+
+
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits: ``q`` float8_e4m3fn [R, K], and the scales of every row's blocks of 128 features, ``s`` float8_e8m0fnu
+    [R, ceil(K / 128)] (powers of two): x[r, k] = q[r, k] * s[r, k // 128].  Rows of q begin on 16 bytes and lie a multiple of
+    16 apart, rows of s 4."""
+    q: torch.Tensor
+    s: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+
+def fp8_rows(R: int, K: int, device) -> Fp8Rows:
+    """Room for ``R`` rows of ``K`` features in 8 bits."""
+    kb = -(-K // FP8_BLOCK)
+    q = torch.empty((R, -(-K // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
+    s = torch.empty((R, -(-kb // 4) * 4), dtype=torch.float8_e8m0fnu, device=device)
+    return Fp8Rows(q if q.shape[1] == K else q[:, :K], s if s.shape[1] == kb else s[:, :kb])
+
+
+def _fp8_check(rows: Fp8Rows, name: str, R: Optional[int] = None, K: Optional[int] = None) -> None:
+    q, s = rows
+    kb = -(-q.shape[1] // FP8_BLOCK) if q.dim() == 2 else 0
+    if q.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu or q.dim() != 2 or s.dim() != 2:
+        raise KernelError(f"{name}: rows in 8 bits are q float8_e4m3fn [R, K] and s float8_e8m0fnu [R, ceil(K / 128)]")
+    if (R is not None and q.shape[0] != R) or (K is not None and q.shape[1] != K) or s.shape[0] != q.shape[0] or s.shape[1] != kb:
+        raise KernelError(f"{name}: q {tuple(q.shape)} and s {tuple(s.shape)} do not fit"
+                          f" {'any' if R is None else R} rows of {'any' if K is None else K} features")
+    if q.numel() == 0:
+        return
+    if q.stride(1) != 1 or q.stride(0) % 16 or q.stride(0) < q.shape[1] or q.data_ptr() % 16:
+        raise KernelError(f"{name}: rows of q must be contiguous, on 16 bytes and a multiple of 16 bytes apart")
+    if (s.stride(1) != 1 and kb > 1) or s.stride(0) % 4 or s.stride(0) < kb or s.data_ptr() % 4:
+        raise KernelError(f"{name}: rows of s must be contiguous, on 4 bytes and a multiple of 4 bytes apart")
+
+
+def _fp8_source(x: torch.Tensor, name: str, T: int, K: int):
+    """(distance of rows, number of parts, distance of parts) of a bfloat16 or float32 [T, K], or float32 parts [n, T, K]."""
+    if x.dtype not in (torch.float32, torch.bfloat16) or (x.dim() == 3 and x.dtype != torch.float32) \
+            or x.dim() not in (2, 3) or tuple(x.shape[-2:]) != (T, K) or (x.dim() == 3 and not x.shape[0]):
+        raise KernelError(f"{name}: bfloat16 or float32 [{T}, {K}], or float32 parts [n, {T}, {K}] expected, got {x.dtype} {tuple(x.shape)}")
+    if x.stride(-1) != 1 and K > 1:
+        raise KernelError(f"{name}: rows must be contiguous")
+    return x.stride(-2), (x.shape[0] if x.dim() == 3 else 1), (x.stride(0) if x.dim() == 3 else 0)
+
+
+def quantize_fp8(x: torch.Tensor, out: Fp8Rows) -> None:
+    """out = x in 8 bits: x bfloat16 or float32 [T, K] (rows may lie apart), or float32 partial sums [n, T, K], which are added first.
+    A block's scale is the smallest power of two with which its largest magnitude stays within 448; a block with an infinity or a NaN
+    gets the scale NaN."""
+    _fp8_check(out, "quantize_fp8: out")
+    T, K = out.shape
+    ld, n, step = _fp8_source(x, "quantize_fp8: x", T, K)
+    _check(library("rows_fp8").qd_rows_fp8(
+        _ptr(x), _I(dtype_code(x.dtype)), _LL(ld), _I(n), _LL(step), _I(0), _I(0), _ptr(None), _ptr(out.q), _LL(out.q.stride(0)),
+        _ptr(out.s), _LL(out.s.stride(0)), _I(T), _I(K), _stream()), "quantize_fp8")
+
+
+def gate_fp8(gate_up: torch.Tensor, out: Fp8Rows, bias: Optional[torch.Tensor] = None, act: int = ACT_SILU) -> None:
+    """out[t, f] = act(g) u in 8 bits, with g = gate_up[t, f] + bias[f] and u = gate_up[t, F + f] + bias[F + f]: gate_up bfloat16 or
+    float32 [T, 2F], or float32 partial sums [n, T, 2F]; ``bias`` float32 [2F] or None; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``."""
+    _fp8_check(out, "gate_fp8: out")
+    T, F = out.shape
+    ld, n, step = _fp8_source(gate_up, "gate_fp8: gate_up", T, 2 * F)
+    _fp8_bias(bias, 2 * F, "gate_fp8")
+    _fp8_act(act, "gate_fp8")
+    _check(library("rows_fp8").qd_rows_fp8(
+        _ptr(gate_up), _I(dtype_code(gate_up.dtype)), _LL(ld), _I(n), _LL(step), _I(1), _I(act), _ptr(bias), _ptr(out.q),
+        _LL(out.q.stride(0)), _ptr(out.s), _LL(out.s.stride(0)), _I(T), _I(F), _stream()), "gate_fp8")
+
+
+def _fp8_bias(bias: Optional[torch.Tensor], n: int, what: str) -> None:
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
+        raise KernelError(f"{what}: bias must be contiguous float32 [{n}]")
+
+
+def _fp8_act(act: int, what: str) -> None:
+    if act not in (ACT_SILU, ACT_GATED_GELU):
+        raise KernelError(f"{what}: act must be ACT_SILU or ACT_GATED_GELU, got {act}")
+
+
+def add_rmsnorm_fp8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, out: Fp8Rows, eps: float,
+                    rows: Optional[torch.Tensor] = None, write_back: bool = True, delta_scale: Optional[torch.Tensor] = None) -> None:
+    """``add_rmsnorm`` with its output in 8 bits: out[r] = rmsnorm(x[s] + delta[s]) * weight with s = rows[r] (or r), rounded once; x
+    float32 [T, D] is updated to x + delta when ``write_back``.  delta: bfloat16 or float32 [T, D], or float32 partial sums [n, T, D];
+    ``delta_scale`` float32 [D] or None multiplies it."""
+    _fp8_check(out, "add_rmsnorm_fp8: out")
+    R, D = out.shape
+    if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != D or not x.is_contiguous():
+        raise KernelError(f"add_rmsnorm_fp8: x must be contiguous float32 [T, {D}]")
+    for name, v in (("weight", weight), ("delta_scale", delta_scale)):
+        if v is not None and (v.dtype != torch.float32 or v.numel() != D or not v.is_contiguous()):
+            raise KernelError(f"add_rmsnorm_fp8: {name} must be contiguous float32 [{D}]")
+    if rows is None and R != x.shape[0] or rows is not None and (rows.dtype != torch.int32 or rows.numel() != R or not rows.is_contiguous()):
+        raise KernelError("add_rmsnorm_fp8: out has a row for every row of x, or for every one of rows (contiguous int32)")
+    n = 1
+    if delta is not None:
+        _, n, _ = _fp8_source(delta, "add_rmsnorm_fp8: delta", *x.shape)
+        if not delta.is_contiguous():
+            raise KernelError("add_rmsnorm_fp8: delta must be contiguous")
+    _check(library("rows_fp8").qd_add_rmsnorm_fp8(
+        _ptr(x), _ptr(delta), _I(dtype_code(delta.dtype) if delta is not None else F32), _ptr(delta_scale), _ptr(weight), _ptr(out.q),
+        _LL(out.q.stride(0)), _ptr(out.s), _LL(out.s.stride(0)), _ptr(rows), _I(R), _I(D), _F(eps), _I(1 if write_back else 0), _I(n),
+        _LL(x.numel()), _stream()), "add_rmsnorm_fp8")
+
+
+@functools.lru_cache(maxsize=4096)
+def gemm_fp8_plan(T: int, N: int, K: int, epi: int, out_code: int, sms: int):
+    """(CTAs to a tile of tokens, rows of w to a tile, shares of K) of a product in 8 bits; ``out_code``: ``dtype_code`` of the result
+    (of ``EPI_STORE``)."""
+    a, b, c = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
+    if not library("gemm_fp8").qd_gemm_fp8_plan(_I(T), _I(N), _I(K), _I(epi), _I(out_code), _I(sms), ctypes.byref(a), ctypes.byref(b), ctypes.byref(c)):
+        raise KernelError(f"gemm_fp8: no product of {T} x {K} by {N} x {K}")
+    return a.value, b.value, c.value
+
+
+def _gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias, out, ldo, s_out, lds_out, epi, plan, what):
+    T, K = x.shape
+    N = w.shape[0]
+    if T == 0 or N == 0:
+        return
+    code = dtype_code(out.dtype) if s_out is None else BF16
+    cg, bn, splits = plan or gemm_fp8_plan(T, N, K, epi, code, sm_count())
+    _check(library("gemm_fp8").qd_gemm_fp8(
+        _ptr(w.q), _LL(w.q.stride(0)), _ptr(w.s), _LL(w.s.stride(0)), _ptr(x.q), _LL(x.q.stride(0)), _ptr(x.s), _LL(x.s.stride(0)),
+        _ptr(bias), _ptr(out), _I(code), _LL(ldo), _ptr(s_out), _LL(lds_out), _I(T), _I(N), _I(K),
+        _I(cg), _I(bn), _I(splits), _I(epi), _I(sm_count()), _stream()), what)
+
+
+def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Tensor, plan=None) -> None:
+    """out[T, N] = x @ w^T (+ bias float32 [N]) of rows in 8 bits on the tensor cores, float32 sums; out bfloat16 or float32, rows may
+    lie apart.  ``plan``: as ``gemm_fp8_plan`` gives it."""
+    _fp8_check(x, "gemm_fp8: x")
+    _fp8_check(w, "gemm_fp8: w", K=x.shape[1])
+    T, N = x.shape[0], w.shape[0]
+    if out.dtype not in (torch.float32, torch.bfloat16) or tuple(out.shape) != (T, N) or (out.stride(1) != 1 and N > 1):
+        raise KernelError(f"gemm_fp8: out must be bfloat16 or float32 [{T}, {N}] with contiguous rows")
+    _fp8_bias(bias, N, "gemm_fp8")
+    _gemm_fp8(x, w, bias, out, out.stride(0), None, 0, EPI_STORE, plan, "gemm_fp8")
+
+
+def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None) -> None:
+    """out[T, F] = act(x @ wg^T + bg) * (x @ wu^T + bu) in 8 bits, for the product that follows: w [2F, K] holds the gate's rows, then
+    up's, ``bias`` float32 [2F] (or None) likewise; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``.  The sums and the activation are
+    float32, rounded once."""
+    _fp8_check(x, "gemm_fp8_gated: x")
+    _fp8_check(w, "gemm_fp8_gated: w", K=x.shape[1])
+    if w.shape[0] % 2:
+        raise KernelError("gemm_fp8_gated: w holds as many rows of up as of the gate")
+    _fp8_check(out, "gemm_fp8_gated: out", x.shape[0], w.shape[0] // 2)
+    _fp8_bias(bias, w.shape[0], "gemm_fp8_gated")
+    _fp8_act(act, "gemm_fp8_gated")
+    _gemm_fp8(x, w, bias, out.q, out.q.stride(0), out.s, out.s.stride(0), EPI_SWIGLU + 256 * act, plan, "gemm_fp8_gated")
 
 
 # ------------------------------------------------------------------ latent attention
