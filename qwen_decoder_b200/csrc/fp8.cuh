@@ -29,8 +29,15 @@ __device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return (unsigned)lo | (unsigned)hi << 16;
 }
-// act(g) u.  A gate of minus infinity goes as the largest finite one does, to zero.
+// act(g) u, the quotient and the exponential within 2^-20.  A gate of minus infinity goes as the largest finite one does, to zero.
 __device__ __forceinline__ float fp8_gated(float g, float u, int act) {
+  float r;
   asm("max.NaN.f32 %0, %0, 0fFF7FFFFF;" : "+f"(g));
-  return qd_gated(g, u, act);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-qd_gate_arg(g, act))));
+  return g * r * u;
+}
+// the larger magnitude, or no number where one is none
+__device__ __forceinline__ float fp8_peak(float a, float b) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(b)));
+  return a;
 }

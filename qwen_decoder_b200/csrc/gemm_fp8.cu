@@ -6,12 +6,12 @@
 // 128 k to a stage), float32 sums in tensor memory and the scales, bytes of exponents, from tensor memory too: lane l, column c of a
 // tile's scales holds the scales of row 32 c + l, the same in all four quarters of the lanes.  A column's word has four bytes and the
 // instruction says which one it takes, so a word is the scales of four blocks of 128 k: exactly four neighbouring bytes of a row of
-// scales.  Four warps of a CTA bring these words: one load to a word, one tcgen05.st to a quarter.
+// scales.  Four warps of a CTA bring these words, one for each quarter.
 //
 // One CTA to a tile of up to 128 tokens, or (``CG`` 2) two to a tile of up to 256: each brings its own tokens and half of the weights'
 // rows, the tensor cores of both read both halves.  A worker (a CTA or a pair) goes through its items one after the other with two
-// accumulators in turn, so that an item's epilogue runs under the next one's MMAs.  512 columns of tensor memory hold two buffers of
-// scales (32 columns) and two accumulators of up to 240 columns; two of 256 overlap in 32 columns, which the epilogue reads first, and
+// accumulators in turn, so that an item's epilogue runs under the next one's MMAs.  512 columns of tensor memory hold four buffers of
+// scales (64 columns) and two accumulators of up to 224 columns; two of 256 overlap in 64 columns, which the epilogue reads first, and
 // then lets the next item's MMAs begin.
 //
 // Warps: 0..7 epilogue (two for each quarter of the lanes, columns halved between them), 8 producer, 9 MMAs, 10..13 scales.
@@ -30,10 +30,15 @@
 #define G8_EPI_WARPS 8
 #define G8_THREADS (14 * 32)
 #define G8_MAX_STAGES 16
-#define G8_SMEM (208 * 1024)                  // of stages
+#define G8_SMEM (202 * 1024)                  // of stages
+#define G8_WORDS 4                            // of scales that are brought together
 #define G8_STAGE_ROWS (32 * 64)               // of a warp's epilogue: 64 bytes of each of its rows
-#define G8_SCALES 480                         // columns of the scales' two buffers, 16 each: 4 of the tokens', up to 8 of the weights'
-#define G8_OVERLAP 32                         // columns that two accumulators of 256 share (the first that the epilogue reads)
+#define G8_MAX_SMEM (G8_SMEM + G8_EPI_WARPS * G8_STAGE_ROWS + 1024)
+#define G8_COLS 512                           // of tensor memory, all
+#define G8_SCALES 448                         // columns of the scales' buffers, 16 each: 4 of the tokens', up to 8 of the weights'
+#define G8_BUFFERS 4
+#define G8_FEW 16                             // tokens of a gated product whose sums fit the epilogue's part of shared memory
+#define G8_OVERLAP 64                         // columns that two accumulators of 256 share (the first that the epilogue reads)
 
 #define G8_STORE 0
 #define G8_SHARED 1                           // K shared by a cluster
@@ -111,9 +116,9 @@ __device__ __forceinline__ void g8_st4(unsigned addr, const unsigned* v) {
                : "memory");
 }
 
-// a row's scales of ``there`` blocks of 128 k, up to four
+// a row's scales of the next four blocks of 128 k, or the ``there`` that there are
 __device__ __forceinline__ unsigned g8_scales(const unsigned char* s, int there) {
-  if (there == 4) return *reinterpret_cast<const unsigned*>(s);
+  if (there >= 4) return *reinterpret_cast<const unsigned*>(s);
   unsigned v = s[0];
   if (there > 1) v |= s[1] << 8;
   if (there > 2) v |= s[2] << 16;
@@ -185,13 +190,36 @@ __device__ __forceinline__ void g8_store_rows(unsigned char* rows, TO* dst, long
   }
 }
 
+// h = act(g) u of 64 features from ``col0`` on, zero from ``feats`` on: h holds the gate's sums (``gate``) or up's, the others lie in tensor
+// memory
+template <int ACT>
+__device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool gate, const float* bias, int col0, int feats) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float o[16];
+    float (&x)[16] = *reinterpret_cast<float (*)[16]>(h + 16 * i);
+    g8_ld16(other + 16 * i, o);
+    tc_ld_wait();
+    if (bias) {
+      g8_bias16(x, bias + (gate ? 0 : feats), col0 + 16 * i, feats);
+      g8_bias16(o, bias + (gate ? feats : 0), col0 + 16 * i, feats);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++) x[e] = fp8_gated(gate ? x[e] : o[e], gate ? o[e] : x[e], ACT);
+    if (col0 + 16 * i + 16 > feats)
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (col0 + 16 * i + e >= feats) x[e] = 0.f;
+  }
+}
+
 template <int EPI, typename TO, int CG>
 __global__ void __launch_bounds__(G8_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ bias,
                 TO* __restrict__ out, const G8Params p, int* __restrict__ status) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_ready[2], acc_free[2], scales_full[2], scales_empty[2];
-  __shared__ unsigned tmem_slot, peaks[4][2][32];
+  __shared__ unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_ready[2], acc_free[2], scales_full[G8_BUFFERS], scales_empty[G8_BUFFERS];
+  __shared__ unsigned tmem_slot, peaks[4][2][32], scales[G8_WORDS][384];
   __shared__ int dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)g8_rank() : 0;
@@ -208,9 +236,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     for (int b = 0; b < 2; b++) {
       tc_bar_init(&acc_ready[b], 1);
       tc_bar_init(&acc_free[b], CG * G8_EPI_WARPS);
-      tc_bar_init(&scales_full[b], CG * 4);
-      tc_bar_init(&scales_empty[b], 1);
     }
+    for (int b = 0; b < G8_BUFFERS; b++) { tc_bar_init(&scales_full[b], CG == 2 && rank == 0 ? 5 : 4); tc_bar_init(&scales_empty[b], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -219,8 +246,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   const int per = EPI == G8_SHARED ? p.splits : CG;
   const int worker = blockIdx.x / per, n_workers = gridDim.x / per, n_items = p.n_ft * p.n_tt;
   const int half = p.bn >> 1;
-  const bool overlap = p.bn > 240;
-  const unsigned acc_step = overlap ? 256 - G8_OVERLAP : 240;
+  const bool overlap = p.bn > G8_SCALES / 2;
+  const unsigned acc_step = overlap ? 256 - G8_OVERLAP : G8_SCALES / 2;
   auto row_x = [&](const G8Item& q) { return (CG * q.tt + rank) * p.mrows; };
   // the first row of W of the part ``h`` (0: first half, 1: second) of an item's tile
   auto row_w = [&](const G8Item& q, int h) { return EPI == G8_GATED ? q.ft * half + h * p.feats : q.ft * p.bn + h * half; };
@@ -279,15 +306,15 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   } else if (warp == G8_EPI_WARPS + 1) {
     // ------------------------------------------------------------------ MMAs
     if (CG == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_slot)), "r"(512u) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_slot)), "r"((unsigned)G8_COLS) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     } else {
-      tc_alloc(&tmem_slot, 512);
+      tc_alloc(&tmem_slot, G8_COLS);
     }
     // (not before this CTA has its tensor memory: the next kernel's CTA beside it might take that, and then wait for this one)
     pdl_launch_dependents();
     tc_fence_before();
-    asm volatile("bar.sync 1, %0;" ::"n"(G8_EPI_WARPS * 32 + 160) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(G8_THREADS - 32) : "memory");
     tc_fence_after();
     if (rank == 0) {
       const bool one = tc_elect();
@@ -320,64 +347,111 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
               g8_commit<CG>(&empty[s]);
               if (last) g8_commit<CG>(&scales_empty[sc]);
             }
-            if (last && ++sc == 2) { sc = 0; sc_ph ^= 1; }
+            if (last && ++sc == G8_BUFFERS) { sc = 0; sc_ph ^= 1; }
             if (++s == p.stages) { s = 0; ph ^= 1; }
           }
           if (one) g8_commit<CG>(&acc_ready[buf]);
           k0 = k1;
         }
       }
+    } else {
+      // The pair's second CTA: its scales are there, word by word.  An arrival at the first CTA's barrier waits for the loads before it;
+      // from the warps that load the scales it was the time of the whole (2,048 x 8,192 x 2,048 in tiles of 256 x 256 35.2 us, x 128 49.5;
+      // without the scales' loads 31.1 and 37.3), so this warp, which has none, hands them on.
+      int words = 0;
+      for (int item = worker; item < n_items; item += n_workers) {
+        const G8Item q = g8_item(p, item, share);
+        for (int kw = q.kb0 >> 2; kw <= (q.kb1 - 1) >> 2; kw++, words++) {
+          const int sc = words % G8_BUFFERS;
+          if (!tc_wait(&scales_full[sc], words / G8_BUFFERS & 1, &dead)) atomicExch(status, 5);
+          tc_fence_after();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) g8_arrive_at(g8_leader(&scales_full[sc]));
+        }
+      }
     }
     __syncwarp();
   } else if (warp >= G8_EPI_WARPS + 2) {
     // ------------------------------------------------------------------ scales
-    asm volatile("bar.sync 1, %0;" ::"n"(G8_EPI_WARPS * 32 + 160) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(G8_THREADS - 32) : "memory");
     tc_fence_after();
     const unsigned at = tmem_slot + ((unsigned)(warp & 3) << 21) + G8_SCALES;
-    const int wcols = p.bn >> 5;
-    pdl_wait();
-    unsigned sc = 0, ph = 1;
-    int words = 0;
-    for (int item = worker; item < n_items; item += n_workers) {
+    const int wcols = (p.bn + 31) >> 5;
+    // A thread brings three rows' words, a token's and two of W, G8_WORDS of each together and the next ones while the present ones are
+    // handed out; each warp then takes all 384 rows' from shared memory.  (With every warp loading all rows itself, word by word, the
+    // loads of rows 148 bytes apart were the time of 2,048 x 3,584 x 18,944 in pairs: 174 us, so 121.)
+    const int t = threadIdx.x - (G8_EPI_WARPS + 2) * 32;
+    const unsigned char* from[3];
+    unsigned v[3][G8_WORDS];
+    int item = worker, kw = 0, kw_end = 0, words = 0;
+    auto open = [&]() {
       const G8Item q = g8_item(p, item, share);
-      const int x0 = row_x(q) + lane;
-      for (int kw = q.kb0 >> 2; kw <= (q.kb1 - 1) >> 2; kw++, words++) {
-        unsigned v[12];
-        const int there = min(4, p.kb_total - 4 * kw);       // a row's last word may not be whole
+      kw = q.kb0 >> 2;
+      kw_end = ((q.kb1 - 1) >> 2) + 1;
+      const int row = row_x(q) + t;
+      from[0] = t < p.mrows && row < p.T ? p.sx + row * p.ldsx : nullptr;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const int m = 32 * c + lane;
-          v[c] = m < p.mrows && x0 + 32 * c < p.T ? g8_scales(p.sx + (x0 + 32 * c) * p.ldsx + 4 * kw, there) : 0;
-        }
+      for (int i = 0; i < 2; i++) {
+        const int j = t + 128 * i, h = j >= half, row_of_w = row_w(q, h) + j - (h ? half : 0);
+        from[1 + i] = j < p.bn && row_of_w < p.N ? p.sw + row_of_w * p.ldsw : nullptr;
+      }
+    };
+    auto load = [&](int i) {
+      const int n = min(G8_WORDS, kw_end - kw);
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-          const int j = 32 * c + lane, h = j >= half, row = row_w(q, h) + j - (h ? half : 0);
-          v[4 + c] = c < wcols && row < p.N ? g8_scales(p.sw + row * p.ldsw + 4 * kw, there) : 0;
-        }
-        if (!tc_wait(&scales_empty[sc], ph, &dead)) atomicExch(status, 6);
+      for (int k = 0; k < G8_WORDS; k++) v[i][k] = from[i] && k < n ? g8_scales(from[i] + 4 * (kw + k), p.kb_total - 4 * (kw + k)) : 0;
+    };
+    auto next = [&]() {                                      // how many words the loads before were of
+      const int n = min(G8_WORDS, kw_end - kw);
+      kw += n;
+      if (kw == kw_end) {
+        item += n_workers;
+        if (item < n_items) open();
+      }
+      return n;
+    };
+    open();
+    load(1);                                                 // (W's do not come from the kernel before)
+    load(2);
+    pdl_wait();
+    load(0);
+    for (int n = next(); n;) {
+      asm volatile("bar.sync 6, 128;" ::: "memory");         // the words before have been taken
+#pragma unroll
+      for (int i = 0; i < 3; i++)
+#pragma unroll
+        for (int k = 0; k < G8_WORDS; k++) scales[k][t + 128 * i] = v[i][k];
+      asm volatile("bar.sync 6, 128;" ::: "memory");
+      const int now = n;
+      n = 0;
+      if (item < n_items) {
+#pragma unroll
+        for (int i = 0; i < 3; i++) load(i);
+        n = next();
+      }
+      for (int k = 0; k < now; k++, words++) {
+        const int sc = words % G8_BUFFERS;
+        unsigned w[12];
+#pragma unroll
+        for (int c = 0; c < 12; c++) w[c] = scales[k][32 * c + lane];
+        if (!tc_wait(&scales_empty[sc], ~(words / G8_BUFFERS) & 1, &dead)) atomicExch(status, 6);
         tc_fence_after();
-        g8_st4(at + 16 * sc, v);
-        g8_st4(at + 16 * sc + 4, v + 4);
-        if (wcols > 4) g8_st4(at + 16 * sc + 8, v + 8);
+        g8_st4(at + 16 * sc, w);
+        g8_st4(at + 16 * sc + 4, w + 4);
+        if (wcols > 4) g8_st4(at + 16 * sc + 8, w + 8);
         tc_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (CG == 2) g8_arrive_at(g8_leader(&scales_full[sc]));
-          else tc_arrive(&scales_full[sc]);
-        }
-        if (++sc == 2) { sc = 0; ph ^= 1; }
+        if (lane == 0) tc_arrive(&scales_full[sc]);
       }
     }
     // the commits' last arrivals at these barriers, too
-    for (int i = 0; i < min(words, 2); i++) {
-      if (words < 2) { sc = 0; ph = 0; }
-      if (!tc_wait(&scales_empty[sc], ph, &dead)) atomicExch(status, 6);
-      if (++sc == 2) { sc = 0; ph ^= 1; }
-    }
+    for (int i = max(0, words - G8_BUFFERS); i < words; i++)
+      if (!tc_wait(&scales_empty[i % G8_BUFFERS], i / G8_BUFFERS & 1, &dead)) atomicExch(status, 6);
   } else {
     // ------------------------------------------------------------------ epilogue
-    asm volatile("bar.sync 1, %0;" ::"n"(G8_EPI_WARPS * 32 + 160) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(G8_THREADS - 32) : "memory");
     tc_fence_after();
     const int quarter = (warp & 3) * 32, side = warp >> 2;
     const unsigned tmem = tmem_slot + ((unsigned)quarter << 16);
@@ -452,48 +526,78 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const bool owner = overlap && side == (buf == 0);
       if (overlap && (!owner || n_rows <= 0)) release(buf);
       if constexpr (EPI == G8_GATED) {
-        if (n_rows > 0) {                                    // whole warps: the loads are collective
-          float h[2][32];
-          unsigned peak = 0;
-          const bool back = side == 1;                       // the second side starts with its last 32 features
-#pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const int f0 = 64 * side + 32 * (back ? 1 - c : c);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-              float g[16], u[16];
-              g8_ld16(acc + f0 + 16 * i, g);
-              g8_ld16(acc + 128 + f0 + 16 * i, u);
+        if (p.mrows <= G8_FEW) {
+          // The rows of few tokens lie in one quarter of the lanes, which two of the warps reach: they pass the sums on through shared
+          // memory, a row of 256 to a warp, four features to a lane (two warps alone took 16.3 us for 8 tokens of 2,048 by 2 x 11,008).
+          float* sums = reinterpret_cast<float*>(b_s + (size_t)p.stages * b_bytes);
+          if (quarter == 0) {
+#pragma unroll 1
+            for (int i = 0; i < 8; i++) {
+              const int g = owner && side ? 15 - i : 8 * side + i;
+              float v[16];
+              g8_ld16(acc + 16 * g, v);
               tc_ld_wait();
-              if (c == 0 && i == 1 && owner) release(buf);
-              const int col = q.ft * 128 + f0 + 16 * i;
-              if (bias) {
-                g8_bias16(g, bias, col, p.feats);
-                g8_bias16(u, bias + p.feats, col, p.feats);
-              }
+              if (owner && i == G8_OVERLAP / 16 - 1) release(buf);
+              if (lane < n_rows)
 #pragma unroll
-              for (int e = 0; e < 16; e++) {
-                const float a = col + e < p.feats ? fp8_gated(g[e], u[e], p.act) : 0.f;
-                h[c][16 * i + e] = a;
-                peak = max(peak, fp8_magnitude(a));
-              }
+                for (int e = 0; e < 4; e++)
+                  *reinterpret_cast<float4*>(sums + lane * 256 + ((4 * g + e ^ (lane & 7)) << 2)) =
+                      make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
             }
           }
-          peaks[warp & 3][side][lane] = peak;
+          asm volatile("bar.sync 7, 256;" ::: "memory");
+          const int tokens = min(p.mrows, p.T - row_x(q)), col = q.ft * 128 + 4 * lane;
+          for (int r = warp; r < tokens; r += G8_EPI_WARPS) {
+            const float4 g4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((lane ^ (r & 7)) << 2));
+            const float4 u4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((32 + lane ^ (r & 7)) << 2));
+            float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+            float peak = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              if (bias && col + e < p.feats) {
+                g[e] += bias[col + e];
+                u[e] += bias[p.feats + col + e];
+              }
+              g[e] = col + e < p.feats ? fp8_gated(g[e], u[e], p.act) : 0.f;
+              peak = fp8_peak(peak, g[e]);
+            }
+            const unsigned byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));
+            const float inv = fp8_inverse(byte);
+            const unsigned w = fp8_pack4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
+            unsigned char* to = (unsigned char*)out + (size_t)(row_x(q) + r) * p.ldo + col;
+            if (col + 4 <= p.feats) *reinterpret_cast<unsigned*>(to) = w;
+            else
+              for (int e = 0; e < 4 && col + e < p.feats; e++) to[e] = (unsigned char)(w >> 8 * e);
+            if (lane == 0) p.s_out[(size_t)(row_x(q) + r) * p.lds_out + q.ft] = (unsigned char)byte;
+          }
+          asm volatile("bar.sync 7, 256;" ::: "memory");     // the sums have been read
+        } else if (n_rows > 0) {                             // whole warps: the loads are collective
+          // First the 64 columns that the next item's MMAs may overwrite, of up in the first accumulator and of the gate in the second,
+          // then they may begin (with the loads in the activations' order they waited for those: 2,048 tokens of 2,048 by 2 x 11,008
+          // 114 us, 1,620 TFLOP/s).
+          float h[64], peak = 0.f;
+          const unsigned one = acc + 64 * side + (buf ? 0 : 128), two = acc + 64 * side + (buf ? 128 : 0);
+#pragma unroll
+          for (int i = 0; i < 4; i++) g8_ld16(one + 16 * i, *reinterpret_cast<float (*)[16]>(h + 16 * i));
+          tc_ld_wait();
+          if (owner) release(buf);
+          const int col0 = q.ft * 128 + 64 * side;
+          if (p.act == QD_ACT_GELU_TANH) g8_activate<QD_ACT_GELU_TANH>(h, two, buf, bias, col0, p.feats);
+          else g8_activate<QD_ACT_SILU>(h, two, buf, bias, col0, p.feats);
+#pragma unroll
+          for (int e = 0; e < 64; e++) peak = fp8_peak(peak, h[e]);
+          peaks[warp & 3][side][lane] = __float_as_uint(peak);
           asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
-          peak = max(peak, peaks[warp & 3][side ^ 1][lane]);
-          const unsigned byte = fp8_scale_byte(peak);
+          const unsigned byte = fp8_scale_byte(max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]));
           const float inv = fp8_inverse(byte);
           __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            unsigned w[8];
+          for (int c = 0; c < 4; c++) {
+            unsigned w[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-              w[i] = fp8_pack4(h[c][4 * i] * inv, h[c][4 * i + 1] * inv, h[c][4 * i + 2] * inv, h[c][4 * i + 3] * inv);
-            const int piece = 2 * (back ? 1 - c : c);
-            *g8_piece(rows, lane, piece) = make_uint4(w[0], w[1], w[2], w[3]);
-            *g8_piece(rows, lane, piece + 1) = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int i = 0; i < 4; i++)
+              w[i] = fp8_pack4(h[16 * c + 4 * i] * inv, h[16 * c + 4 * i + 1] * inv, h[16 * c + 4 * i + 2] * inv, h[16 * c + 4 * i + 3] * inv);
+            *g8_piece(rows, lane, c) = make_uint4(w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
           const int col = q.ft * 128 + 64 * side;
@@ -511,7 +615,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           for (int j = 0; j < 2; j++)
             if (j < w) g8_ld16(acc + 16 * (g + j), v[j]);
           tc_ld_wait();
-          if (owner && i == 0) release(buf);
+          if (owner && i == G8_OVERLAP / 32 - 1) release(buf);
           __syncwarp();
           const int col = q.ft * p.bn + 16 * g;
           if constexpr (EPI == G8_SHARED) {
@@ -568,8 +672,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (CG == 2 || EPI == G8_SHARED) g8_cluster_sync();
   if (warp == G8_EPI_WARPS + 1) {
     tc_fence_after();
-    if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(512u) : "memory");
-    else tc_dealloc(tmem_slot, 512);
+    if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"((unsigned)G8_COLS) : "memory");
+    else tc_dealloc(tmem_slot, G8_COLS);
   }
 }
 
@@ -589,39 +693,18 @@ static int* status_word() {
 
 static int up(int a, int b) { return (a + b - 1) / b; }
 
-// How a product is cut: *cg CTAs to a tile of tokens, *bn rows of W to a tile, K in *splits shares (of a cluster).
-extern "C" int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out) {
-  epi &= 255;
-  const int most = epi == G8_STORE && out_dtype == QD_F32 ? G8_MAX_FLOAT_BN : 256;
-  if (T <= 0 || N <= 0 || K <= 0 || sms < 2) return 0;
-  const int kb = up(K, FP8_BLOCK);
-  const double dram = (double)N * K / 3300.0;          // clocks of 1.9 GHz
-  double best = 0;
-  for (int cg = T <= 128 ? 1 : 2; cg >= 1; cg--) {
-    const int workers = sms / cg, n_tt = up(T, 128 * cg), mrows = up(up(T, cg * n_tt), 8) * 8;
-    for (int bn = epi == G8_GATED ? 256 : 32; bn <= most; bn += 32) {
-      const long long tiles = (long long)up(epi == G8_GATED ? N / 2 : N, epi == G8_GATED ? bn / 2 : bn) * n_tt;
-      for (int splits = 1; splits <= (epi == G8_GATED || cg == 2 ? 1 : 8) && (splits == 1 || splits * 4 <= kb); splits++) {
-        if (splits > 1 && tiles * splits > sms) break;
-        const long long rounds = splits > 1 ? 1 : (tiles + workers - 1) / workers;
-        const double bytes = (mrows + bn / cg) * 128 / 60.0;
-        double block = 2.0 * bn;
-        if (block < bytes) block = bytes;
-        if (block < 350) block = 350;
-        const double work = (double)rounds * up(kb, splits) * block;
-        double cost = work > dram ? work + 0.15 * dram : dram + 0.15 * work;
-        cost += 12.0 * bn + (splits > 1 ? 1500.0 : 0.0);
-        if (best == 0 || cost < best) { best = cost; *cg_out = cg; *bn_out = bn; *splits_out = splits; }
-      }
-    }
-  }
-  return 1;
-}
-
 template <int EPI, typename TO, int CG>
 static int g8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const float* bias, void* out, const G8Params& p, int* status,
                      int ctas, size_t smem, cudaStream_t stream) {
-  cudaFuncSetAttribute(gemm_fp8_kernel<EPI, TO, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static bool allowed[64];                     // by device; all shared memory that a launch may ask for
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QD_ERR_UNSUPPORTED;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(gemm_fp8_kernel<EPI, TO, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             G8_MAX_SMEM) != cudaSuccess)
+      return (int)cudaGetLastError();
+    allowed[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(G8_THREADS);
@@ -637,6 +720,61 @@ static int g8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const f
   cfg.numAttrs = qd_pdl_enabled() ? 2 : 1;
   cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<EPI, TO, CG>, map_w, map_x, bias, (TO*)out, p, status);
   return qd_last_error();
+}
+
+// How many clusters of ``n`` CTAs run at a time: they lie within a group of multiprocessors, whose sizes need not be a multiple of theirs
+// (of 148 multiprocessors 5 to a cluster leave some idle; a cluster too many doubles the time).
+static int g8_clusters(int n, int sms) {
+  static int known[9];
+  if (known[n]) return known[n];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n * 148);
+  cfg.blockDim = dim3(G8_THREADS);
+  cfg.dynamicSmemBytes = G8_MAX_SMEM;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = n;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int got = 0;
+  if (cudaFuncSetAttribute(gemm_fp8_kernel<G8_SHARED, bf16, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, G8_MAX_SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&got, gemm_fp8_kernel<G8_SHARED, bf16, 1>, &cfg) != cudaSuccess || got < 1) {
+    (void)cudaGetLastError();
+    got = sms / (n + 1);
+  }
+  return known[n] = got;
+}
+
+// How a product is cut: *cg CTAs to a tile of tokens, *bn rows of W to a tile, K in *splits shares (of a cluster).
+extern "C" int qd_gemm_fp8_clusters(int n, int sms) { return n >= 1 && n <= 8 ? g8_clusters(n, sms) : 0; }
+extern "C" int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out) {
+  epi &= 255;
+  const int most = epi == G8_STORE && out_dtype == QD_F32 ? G8_MAX_FLOAT_BN : 256;
+  if (T <= 0 || N <= 0 || K <= 0 || sms < 2) return 0;
+  const int kb = up(K, FP8_BLOCK);
+  const double dram = (double)N * K / 3300.0;          // clocks of 1.9 GHz
+  double best = 0;
+  for (int cg = T <= 128 ? 1 : 2; cg >= 1; cg--) {
+    const int workers = sms / cg, n_tt = up(T, 128 * cg), mrows = up(up(T, cg * n_tt), 8) * 8;
+    for (int bn = epi == G8_GATED ? 256 : 32; bn <= most; bn += 16) {
+      const long long tiles = (long long)up(epi == G8_GATED ? N / 2 : N, epi == G8_GATED ? bn / 2 : bn) * n_tt;
+      for (int splits = 1; splits <= (epi == G8_GATED || cg == 2 ? 1 : 8) && (splits == 1 || splits * 4 <= kb); splits++) {
+        if ((cg == 2 || splits > 1) && bn % 32) break;
+        if (splits > 1 && tiles > g8_clusters(splits, sms)) break;      // one round
+        const long long rounds = splits > 1 ? 1 : (tiles + workers - 1) / workers;
+        const double bytes = (mrows + bn / cg) * 128 / 60.0;
+        double block = 2.0 * bn;
+        if (block < bytes) block = bytes;
+        if (block < 350) block = 350;
+        const double work = (double)rounds * up(kb, splits) * block;
+        double cost = work > dram ? work + 0.15 * dram : dram + 0.15 * work;
+        cost += 12.0 * bn + (splits > 1 ? 1500.0 : 0.0);
+        if (best == 0 || cost < best) { best = cost; *cg_out = cg; *bn_out = bn; *splits_out = splits; }
+      }
+    }
+  }
+  return 1;
 }
 
 // rows x cols bytes, rows ``ld`` bytes apart; boxes of box_rows rows of 128 bytes, 128-byte swizzle, zeros outside
@@ -656,14 +794,14 @@ static bool g8_make_map(CUtensorMap* map, const void* base, long long rows, long
 // float32 [N]), bfloat16 or float32, rows ``ldo`` apart; ``splits`` > 1: K shared by clusters of so many CTAs (up to 8), a tile to each.
 // epi 2 (+ 256 * QD_ACT_*): W [2F, K] the gate's rows, then up's; out e4m3 [T, F] = act(X Wg^T) * (X Wu^T), rows ``ldo`` bytes apart
 // (a multiple of 4), and its scales s_out, rows ``lds_out`` apart.  ``cg``: CTAs to a tile of tokens, 1 (up to 128) or 2 (up to 256);
-// ``bn``: rows of W to a tile, a multiple of 32 up to 256 (256 for epi 2).
+// ``bn``: rows of W to a tile, a multiple of 16 (of 32 for pairs and clusters) from 32 to 256 (256 for epi 2).
 extern "C" int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
                            long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, void* s_out, long long lds_out,
                            int T, int N, int K, int cg, int bn, int splits, int epi, int sms, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
   const int act = epi >> 8;
   epi &= 255;
-  if (K <= 0 || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) || bn < 32 || bn > 256 || bn % 32 || splits < 1 ||
+  if (K <= 0 || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) || bn < 32 || bn > 256 || bn % (cg == 2 || splits > 1 ? 32 : 16) || splits < 1 ||
       splits > 8 || sms < 2 || !out)
     return QD_ERR_UNSUPPORTED;
   if ((((uintptr_t)W | (uintptr_t)X) & 15) || (((uintptr_t)sw | (uintptr_t)sx) & 3) || ldsw % 4 || ldsx % 4) return QD_ERR_UNSUPPORTED;

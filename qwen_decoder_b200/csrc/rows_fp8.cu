@@ -7,14 +7,17 @@
 // The reference rounds nothing below 16 bits (its norm and activation: gpu_kernels.cu:32-67, 136-160).
 #include "fp8.cuh"
 
-// four neighbouring features, zeros from ``K`` on; ``vec``: they lie on 16 (float32) or 8 bytes (bfloat16)
-__device__ __forceinline__ float4 load4(const float* row, int k, int K, bool vec) {
-  if (vec && k + 4 <= K) return *reinterpret_cast<const float4*>(row + k);
+// Four neighbouring features, zeros from ``K`` on.  VEC: K is a multiple of 4 and they lie on 16 (float32) or 8 bytes (bfloat16): one
+// load behind a predicate, of which as many are under way at a time as a thread has room for.
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float* row, int k, int K) {
+  if (VEC) return k < K ? *reinterpret_cast<const float4*>(row + k) : make_float4(0.f, 0.f, 0.f, 0.f);
   return make_float4(k < K ? row[k] : 0.f, k + 1 < K ? row[k + 1] : 0.f, k + 2 < K ? row[k + 2] : 0.f, k + 3 < K ? row[k + 3] : 0.f);
 }
-__device__ __forceinline__ float4 load4(const bf16* row, int k, int K, bool vec) {
-  if (vec && k + 4 <= K) {
-    const uint2 raw = *reinterpret_cast<const uint2*>(row + k);
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const bf16* row, int k, int K) {
+  if (VEC) {
+    const uint2 raw = k < K ? *reinterpret_cast<const uint2*>(row + k) : make_uint2(0, 0);
     return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
                        __uint_as_float(raw.y & 0xffff0000u));
   }
@@ -42,39 +45,57 @@ struct RowsArgs {
   const void* x;
   const float* bias;       // of the gate and the up product, [2 K], or null
   unsigned char *q, *s;
-  int T, K, blocks, n_parts, act, vec;
+  int T, K, blocks, n_parts, act;
   long long ldx, part_stride, ldq, lds;
 };
 
-template <typename TX>
-__device__ __forceinline__ float4 sum_parts(const RowsArgs& a, const TX* row, int k, int K) {
-  float4 v = load4(row, k, K, a.vec);
-  for (int p = 1; p < a.n_parts; p++) add4(v, load4(row + p * a.part_stride, k, K, a.vec));
-  return v;
+// A warp's EACH blocks, four features to a lane of each, of the sum of a row's parts in their order, four parts' loads together
+template <bool VEC, int EACH, typename TX>
+__device__ __forceinline__ void sum_parts(float4 (&v)[EACH], const TX* row, int k0, int step, int K, int n_parts, long long part_stride) {
+#pragma unroll
+  for (int i = 0; i < EACH; i++) v[i] = load4<VEC>(row, k0 + i * step, K);
+  if (sizeof(TX) == 2) return;
+  for (int p0 = 1; p0 < n_parts; p0 += 4) {
+    float4 d[4][EACH];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int i = 0; i < EACH; i++) d[j][i] = load4<VEC>(row + (p0 + j) * part_stride, k0 + i * step, p0 + j < n_parts ? K : 0);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int i = 0; i < EACH; i++) add4(v[i], d[j][i]);
+  }
 }
 
-template <typename TX, bool GATED>
+// A warp takes EACH neighbouring blocks of a row, all of their loads before the first is used
+template <typename TX, bool GATED, int EACH, bool VEC>
 __global__ void __launch_bounds__(256) rows_fp8_kernel(const RowsArgs a) {
   pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (long long)a.T * a.blocks) return;
-  const int t = (int)(item / a.blocks), block = (int)(item - (long long)t * a.blocks), k = block * FP8_BLOCK + 4 * lane;
+  const int lane = threadIdx.x & 31, runs = (a.blocks + EACH - 1) / EACH;
+  const unsigned item = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int t = item / runs, b0 = (item - t * runs) * EACH, k0 = b0 * FP8_BLOCK + 4 * lane;
+  if (t >= a.T) return;
   const TX* row = (const TX*)a.x + t * a.ldx;
-  float4 v = sum_parts(a, row, k, a.K);
-  if (GATED) {
-    float4 u = sum_parts(a, row + a.K, k, a.K);
-    if (a.bias) {
-      add4(v, load4(a.bias, k, a.K, false));
-      add4(u, load4(a.bias + a.K, k, a.K, false));
+  pdl_wait();
+  float4 v[EACH], u[EACH];
+  sum_parts<VEC>(v, row, k0, FP8_BLOCK, a.K, a.n_parts, a.part_stride);
+  if (GATED) sum_parts<VEC>(u, row + a.K, k0, FP8_BLOCK, a.K, a.n_parts, a.part_stride);
+#pragma unroll
+  for (int i = 0; i < EACH; i++) {
+    if (b0 + i >= a.blocks) break;
+    if (GATED) {
+      if (a.bias) {
+        add4(v[i], load4<false>(a.bias, k0 + i * FP8_BLOCK, a.K));
+        add4(u[i], load4<false>(a.bias + a.K, k0 + i * FP8_BLOCK, a.K));
+      }
+      v[i].x = fp8_gated(v[i].x, u[i].x, a.act);
+      v[i].y = fp8_gated(v[i].y, u[i].y, a.act);
+      v[i].z = fp8_gated(v[i].z, u[i].z, a.act);
+      v[i].w = fp8_gated(v[i].w, u[i].w, a.act);
     }
-    v.x = fp8_gated(v.x, u.x, a.act);
-    v.y = fp8_gated(v.y, u.y, a.act);
-    v.z = fp8_gated(v.z, u.z, a.act);
-    v.w = fp8_gated(v.w, u.w, a.act);
+    store_block(v[i], a.q + t * a.ldq, a.s + t * a.lds, b0 + i, a.K);
   }
-  store_block(v, a.q + t * a.ldq, a.s + t * a.lds, block, a.K);
 }
 
 // q [T, K] e4m3 and s [T, ceil(K / 128)], rows ``ldq`` and ``lds`` bytes apart (a multiple of 4), of
@@ -90,14 +111,19 @@ extern "C" int qd_rows_fp8(const void* x, int dtype, long long ldx, int n_parts,
   a.T = T; a.K = K; a.blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK; a.n_parts = n_parts; a.act = act;
   a.ldx = ldx; a.part_stride = part_stride; a.ldq = ldq; a.lds = lds;
   const int bytes = dtype == QD_F32 ? 16 : 8;
-  a.vec = !((uintptr_t)x & (bytes - 1)) && ldx % 4 == 0 && part_stride % 4 == 0 && (!gated || K % 4 == 0);
-  const long long items = (long long)T * a.blocks;
-  if (items > (1ll << 33)) return QD_ERR_UNSUPPORTED;
+  const bool vec = !((uintptr_t)x & (bytes - 1)) && ldx % 4 == 0 && part_stride % 4 == 0 && K % 4 == 0;
+  // few blocks: one to a warp, over as many multiprocessors as there are; many: four, for more bytes on their way
+  const int each = (long long)T * a.blocks > 4096 ? 4 : 1;
+  const long long items = (long long)T * ((a.blocks + each - 1) / each);
+  if (items > (1ll << 31)) return QD_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)((items + 7) / 8));
-#define GO(TX, G) qd_launch(rows_fp8_kernel<TX, G>, grid, dim3(256), 0, stream, a)
+#define GO2(TX, G, V) do { if (each == 4) qd_launch(rows_fp8_kernel<TX, G, 4, V>, grid, dim3(256), 0, stream, a);             \
+                           else qd_launch(rows_fp8_kernel<TX, G, 1, V>, grid, dim3(256), 0, stream, a); } while (0)
+#define GO(TX, G) do { if (vec) GO2(TX, G, true); else GO2(TX, G, false); } while (0)
   if (gated) { if (dtype == QD_F32) GO(float, true); else GO(bf16, true); }
   else { if (dtype == QD_F32) GO(float, false); else GO(bf16, false); }
 #undef GO
+#undef GO2
   return qd_last_error();
 }
 
@@ -108,59 +134,63 @@ struct NormArgs {
   const float *dscale, *w;
   unsigned char *q, *s;
   const int* rows;
-  int D, blocks, n_parts, write_back, vec;
+  int D, blocks, n_parts, write_back;
   float eps;
   long long part_stride, ldq, lds;
 };
 
 // One CTA to a row.  A warp holds up to VPT of the row's blocks in registers.
-template <typename TD, int VPT>
+template <typename TD, int VPT, bool VEC>
 __global__ void __launch_bounds__(1024) norm_fp8_kernel(const NormArgs a) {
   __shared__ float scratch[40];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = (blockDim.x >> 5) * FP8_BLOCK, k0 = warp * FP8_BLOCK + 4 * lane;
   pdl_launch_dependents();
+  // (the weights do not come from the kernel before: with few blocks to a warp they travel while that is waited for)
+  float4 w[VPT <= 4 ? VPT : 1];
+  if (VPT <= 4)
+#pragma unroll
+    for (int i = 0; i < VPT; i++) w[VPT <= 4 ? i : 0] = load4<VEC>(a.w, k0 + i * step, a.D);
   pdl_wait();
   const int r = blockIdx.x;
   const size_t at = (size_t)(a.rows ? a.rows[r] : r) * a.D;
   float4 v[VPT];
-  float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < VPT; i++) {
-    const int block = warp + i * warps, k = block * FP8_BLOCK + 4 * lane;
-    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (block < a.blocks) {
-      v[i] = load4(a.x + at, k, a.D, a.vec);
-      if (a.delta) {
-        const TD* dp = (const TD*)a.delta + at;
-        float4 d = load4(dp, k, a.D, a.vec);
-        for (int p = 1; p < a.n_parts; p++) add4(d, load4(dp + p * a.part_stride, k, a.D, a.vec));
-        if (a.dscale) {
-          const float4 f = load4(a.dscale, k, a.D, a.vec);
-          d.x *= f.x; d.y *= f.y; d.z *= f.z; d.w *= f.w;
-        }
-        add4(v[i], d);
-        if (a.write_back) {
-          float* to = a.x + at + k;
-          if (a.vec && k + 4 <= a.D) *reinterpret_cast<float4*>(to) = v[i];
-          else {
-            if (k < a.D) to[0] = v[i].x;
-            if (k + 1 < a.D) to[1] = v[i].y;
-            if (k + 2 < a.D) to[2] = v[i].z;
-            if (k + 3 < a.D) to[3] = v[i].w;
-          }
+  for (int i = 0; i < VPT; i++) v[i] = load4<VEC>(a.x + at, k0 + i * step, a.D);
+  if (a.delta) {
+    float4 d[VPT];
+    sum_parts<VEC>(d, (const TD*)a.delta + at, k0, step, a.D, a.n_parts, a.part_stride);
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+      const int k = k0 + i * step;
+      if (a.dscale) {
+        const float4 f = load4<VEC>(a.dscale, k, a.D);
+        d[i].x *= f.x; d[i].y *= f.y; d[i].z *= f.z; d[i].w *= f.w;
+      }
+      add4(v[i], d[i]);
+      if (a.write_back) {
+        float* to = a.x + at + k;
+        if (VEC) {
+          if (k < a.D) *reinterpret_cast<float4*>(to) = v[i];
+        } else {
+          if (k < a.D) to[0] = v[i].x;
+          if (k + 1 < a.D) to[1] = v[i].y;
+          if (k + 2 < a.D) to[2] = v[i].z;
+          if (k + 3 < a.D) to[3] = v[i].w;
         }
       }
-      ss += v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
     }
   }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) ss += v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
   ss = block_sum(ss, scratch);
   const float inv = 1.0f / sqrtf(ss / (float)a.D + a.eps);
 #pragma unroll
   for (int i = 0; i < VPT; i++) {
-    const int block = warp + i * warps, k = block * FP8_BLOCK + 4 * lane;
+    const int block = warp + i * (int)(blockDim.x >> 5);
     if (block < a.blocks) {
-      const float4 w = load4(a.w, k, a.D, a.vec);
-      v[i].x = v[i].x * inv * w.x; v[i].y = v[i].y * inv * w.y; v[i].z = v[i].z * inv * w.z; v[i].w = v[i].w * inv * w.w;
+      const float4 f = VPT <= 4 ? w[VPT <= 4 ? i : 0] : load4<VEC>(a.w, k0 + i * step, a.D);
+      v[i].x = v[i].x * inv * f.x; v[i].y = v[i].y * inv * f.y; v[i].z = v[i].z * inv * f.z; v[i].w = v[i].w * inv * f.w;
       store_block(v[i], a.q + (size_t)r * a.ldq, a.s + (size_t)r * a.lds, block, a.D);
     }
   }
@@ -179,12 +209,14 @@ extern "C" int qd_add_rmsnorm_fp8(float* x, const void* delta, int delta_dtype, 
   a.x = x; a.delta = delta; a.dscale = dscale; a.w = w; a.q = (unsigned char*)q; a.s = (unsigned char*)s; a.rows = rows;
   a.D = D; a.blocks = (D + FP8_BLOCK - 1) / FP8_BLOCK; a.n_parts = n_parts; a.write_back = write_back; a.eps = eps;
   a.part_stride = part_stride; a.ldq = ldq; a.lds = lds;
-  a.vec = D % 4 == 0 && part_stride % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)dscale) & 15) &&
+  const bool vec = D % 4 == 0 && part_stride % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)dscale) & 15) &&
           !((uintptr_t)delta & (delta_dtype == QD_BF16 ? 7 : 15));
   if (a.blocks > 32 * 16) return QD_ERR_UNSUPPORTED;       // 65,536 features
-  const int vpt = a.blocks <= 32 ? 1 : a.blocks <= 64 ? 2 : a.blocks <= 128 ? 4 : 16;
+  // few rows: a block to each warp, the shortest way; many: four, so that more rows are on their way at a time
+  const int vpt = a.blocks > 128 ? 16 : a.blocks > 64 || n_rows > 296 ? 4 : a.blocks > 32 ? 2 : 1;
   const dim3 grid(n_rows), block(32 * ((a.blocks + vpt - 1) / vpt));
-#define GO(TD, V) qd_launch(norm_fp8_kernel<TD, V>, grid, block, 0, stream, a)
+#define GO(TD, V) do { if (vec) qd_launch(norm_fp8_kernel<TD, V, true>, grid, block, 0, stream, a);                           \
+                       else qd_launch(norm_fp8_kernel<TD, V, false>, grid, block, 0, stream, a); } while (0)
 #define PICK(TD) do { if (vpt == 1) GO(TD, 1); else if (vpt == 2) GO(TD, 2); else if (vpt == 4) GO(TD, 4); else GO(TD, 16); } while (0)
   if (delta && delta_dtype == QD_BF16) PICK(bf16); else PICK(float);
 #undef PICK

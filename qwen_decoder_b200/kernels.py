@@ -72,7 +72,8 @@ class step_stream:
 def _stream():
     _launch_count[0] += 1          # every launcher fetches the stream exactly once
     s = _step_stream[0]
-    return s if s is not None else ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the stream's handle alone: the object that torch.cuda.current_stream() makes for it costs 3 us)
+    return s if s is not None else ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _check(code: int, what: str) -> None:
@@ -843,6 +844,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
 
 
 LOGPROBS_MAX_TOP = 32
+LOGPROBS_SHARES = 0
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
@@ -851,20 +853,21 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     lowest index first; their log probabilities), float32.  Logits of minus infinity have probability 0; a row of nothing else gives
     minus infinity, entropy 0.  A row with a NaN or an infinity has none: NaN, and its ids are of the numbers there are (-1: none).  A
     token outside of the row gives NaN."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    dt = logits.dtype
+    if logits.dim() != 2 or dt not in (torch.float32, torch.bfloat16) or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise KernelError("token_logprobs: logits must be float32 or bfloat16 [R, V] with contiguous rows")
     R, V = logits.shape
-    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (R,) or not tokens.is_contiguous():
+    if tokens.dtype != torch.int32 or tokens.shape != (R,) or not tokens.is_contiguous():
         raise KernelError(f"token_logprobs: tokens must be contiguous int32 [{R}]")
     if V < 1 or not 0 <= top <= min(LOGPROBS_MAX_TOP, V):
         raise KernelError(f"token_logprobs: top must be between 0 and {min(LOGPROBS_MAX_TOP, V)}, got {top}")
-    both = torch.empty((2, R), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((R, top), dtype=torch.int32, device=logits.device)
-    lps = torch.empty((R, top), dtype=torch.float32, device=logits.device)
-    _check(library("logprobs").qd_token_logprobs(
-        _ptr(logits), _I(dtype_code(logits.dtype)), _LL(logits.stride(0)), _ptr(tokens), _ptr(both[0]), _ptr(both[1]), _ptr(ids), _ptr(lps),
-        _I(R), _I(V), _I(top), _I(sm_count()), _stream()), "token_logprobs")
-    return both[0], both[1], ids, lps
+    new = lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=logits.device)      # noqa: E731
+    lp, entropy = new((R,), (1,), torch.float32), new((R,), (1,), torch.float32)
+    ids, lps = new((R, top), (top, 1), torch.int32), new((R, top), (top, 1), torch.float32)
+    _check(_entry("logprobs", "qd_token_logprobs", "pilpppppiiiiip")(
+        _raw_ptr(logits), F32 if dt == torch.float32 else BF16, logits.stride(0), _raw_ptr(tokens), lp.data_ptr(), entropy.data_ptr(),
+        ids.data_ptr(), lps.data_ptr(), R, V, top, sm_count(), LOGPROBS_SHARES, _stream()), "token_logprobs")
+    return lp, entropy, ids, lps
 
 
 def prefill_tc5_supported(dtype, H: int, G: int, d: int, page_size: int) -> bool:
@@ -946,60 +949,89 @@ class Fp8Rows(NamedTuple):
 def fp8_rows(R: int, K: int, device) -> Fp8Rows:
     """Room for ``R`` rows of ``K`` features in 8 bits."""
     kb = -(-K // FP8_BLOCK)
-    q = torch.empty((R, -(-K // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
-    s = torch.empty((R, -(-kb // 4) * 4), dtype=torch.float8_e8m0fnu, device=device)
-    return Fp8Rows(q if q.shape[1] == K else q[:, :K], s if s.shape[1] == kb else s[:, :kb])
+    return Fp8Rows(torch.empty_strided((R, K), ((K + 15) & -16, 1), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty_strided((R, kb), ((kb + 3) & -4, 1), dtype=torch.float8_e8m0fnu, device=device))
 
 
-def _fp8_check(rows: Fp8Rows, name: str, R: Optional[int] = None, K: Optional[int] = None) -> None:
+def _entry(name: str, function: str, kinds: str):
+    """A library's function with its arguments' types (i int, l long long, f float, p pointer), looked up once: arguments then go as they
+    are, which for some twenty of them is 4 us less a call."""
+    fn = _entries.get(function)
+    if fn is None:
+        fn = getattr(library(name), function)
+        fn.argtypes = [{"i": _I, "l": _LL, "f": _F, "p": ctypes.c_void_p}[k] for k in kinds]
+        _entries[function] = fn
+    return fn
+
+
+_entries = {}
+
+
+def _raw_ptr(t: Optional[torch.Tensor]):
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise KernelError("kernel argument is not on a CUDA device (there is no CPU path)")
+    return t.data_ptr()
+
+
+def _fp8_check(rows: Fp8Rows, name: str, R: Optional[int] = None, K: Optional[int] = None):
+    """(R, K, address and distance of q's rows, of s's rows), or ``KernelError``."""
     q, s = rows
-    kb = -(-q.shape[1] // FP8_BLOCK) if q.dim() == 2 else 0
     if q.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu or q.dim() != 2 or s.dim() != 2:
         raise KernelError(f"{name}: rows in 8 bits are q float8_e4m3fn [R, K] and s float8_e8m0fnu [R, ceil(K / 128)]")
-    if (R is not None and q.shape[0] != R) or (K is not None and q.shape[1] != K) or s.shape[0] != q.shape[0] or s.shape[1] != kb:
+    (r, k), at, (ldq, one), s_at, (lds, s_one) = q.shape, q.data_ptr(), q.stride(), s.data_ptr(), s.stride()
+    kb = -(-k // FP8_BLOCK)
+    if (R is not None and r != R) or (K is not None and k != K) or s.shape != (r, kb):
         raise KernelError(f"{name}: q {tuple(q.shape)} and s {tuple(s.shape)} do not fit"
                           f" {'any' if R is None else R} rows of {'any' if K is None else K} features")
-    if q.numel() == 0:
-        return
-    if q.stride(1) != 1 or q.stride(0) % 16 or q.stride(0) < q.shape[1] or q.data_ptr() % 16:
-        raise KernelError(f"{name}: rows of q must be contiguous, on 16 bytes and a multiple of 16 bytes apart")
-    if (s.stride(1) != 1 and kb > 1) or s.stride(0) % 4 or s.stride(0) < kb or s.data_ptr() % 4:
-        raise KernelError(f"{name}: rows of s must be contiguous, on 4 bytes and a multiple of 4 bytes apart")
+    if r and k:
+        if one != 1 or ldq % 16 or ldq < k or at % 16:
+            raise KernelError(f"{name}: rows of q must be contiguous, on 16 bytes and a multiple of 16 bytes apart")
+        if (s_one != 1 and kb > 1) or lds % 4 or lds < kb or s_at % 4:
+            raise KernelError(f"{name}: rows of s must be contiguous, on 4 bytes and a multiple of 4 bytes apart")
+    return r, k, at, ldq, s_at, lds
+
+
+def _on_device(rows: Fp8Rows) -> None:
+    if not (rows.q.is_cuda and rows.s.is_cuda):
+        raise KernelError("kernel argument is not on a CUDA device (there is no CPU path)")
 
 
 def _fp8_source(x: torch.Tensor, name: str, T: int, K: int):
-    """(distance of rows, number of parts, distance of parts) of a bfloat16 or float32 [T, K], or float32 parts [n, T, K]."""
-    if x.dtype not in (torch.float32, torch.bfloat16) or (x.dim() == 3 and x.dtype != torch.float32) \
-            or x.dim() not in (2, 3) or tuple(x.shape[-2:]) != (T, K) or (x.dim() == 3 and not x.shape[0]):
-        raise KernelError(f"{name}: bfloat16 or float32 [{T}, {K}], or float32 parts [n, {T}, {K}] expected, got {x.dtype} {tuple(x.shape)}")
-    if x.stride(-1) != 1 and K > 1:
+    """(dtype code, distance of rows, number of parts, distance of parts) of a bfloat16 or float32 [T, K], or float32 parts [n, T, K]."""
+    shape, stride, dt = x.shape, x.stride(), x.dtype
+    parts = len(shape) == 3
+    if dt not in (torch.float32, torch.bfloat16) or (parts and (dt != torch.float32 or not shape[0])) \
+            or len(shape) not in (2, 3) or shape[-2:] != (T, K):
+        raise KernelError(f"{name}: bfloat16 or float32 [{T}, {K}], or float32 parts [n, {T}, {K}] expected, got {dt} {tuple(shape)}")
+    if stride[-1] != 1 and K > 1:
         raise KernelError(f"{name}: rows must be contiguous")
-    return x.stride(-2), (x.shape[0] if x.dim() == 3 else 1), (x.stride(0) if x.dim() == 3 else 0)
+    return (F32 if dt == torch.float32 else BF16), stride[-2], (shape[0] if parts else 1), (stride[0] if parts else 0)
+
+
+def _rows_fp8(x, code, ld, n, step, gated, act, bias, out, q, ldq, s, lds, T, K, what):
+    _on_device(out)
+    _check(_entry("rows_fp8", "qd_rows_fp8", "pililiipplpliip")(
+        _raw_ptr(x), code, ld, n, step, gated, act, _raw_ptr(bias), q, ldq, s, lds, T, K, _stream()), what)
 
 
 def quantize_fp8(x: torch.Tensor, out: Fp8Rows) -> None:
     """out = x in 8 bits: x bfloat16 or float32 [T, K] (rows may lie apart), or float32 partial sums [n, T, K], which are added first.
     A block's scale is the smallest power of two with which its largest magnitude stays within 448; a block with an infinity or a NaN
     gets the scale NaN."""
-    _fp8_check(out, "quantize_fp8: out")
-    T, K = out.shape
-    ld, n, step = _fp8_source(x, "quantize_fp8: x", T, K)
-    _check(library("rows_fp8").qd_rows_fp8(
-        _ptr(x), _I(dtype_code(x.dtype)), _LL(ld), _I(n), _LL(step), _I(0), _I(0), _ptr(None), _ptr(out.q), _LL(out.q.stride(0)),
-        _ptr(out.s), _LL(out.s.stride(0)), _I(T), _I(K), _stream()), "quantize_fp8")
+    T, K, *at = _fp8_check(out, "quantize_fp8: out")
+    _rows_fp8(x, *_fp8_source(x, "quantize_fp8: x", T, K), 0, 0, None, out, *at, T, K, "quantize_fp8")
 
 
 def gate_fp8(gate_up: torch.Tensor, out: Fp8Rows, bias: Optional[torch.Tensor] = None, act: int = ACT_SILU) -> None:
     """out[t, f] = act(g) u in 8 bits, with g = gate_up[t, f] + bias[f] and u = gate_up[t, F + f] + bias[F + f]: gate_up bfloat16 or
     float32 [T, 2F], or float32 partial sums [n, T, 2F]; ``bias`` float32 [2F] or None; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``."""
-    _fp8_check(out, "gate_fp8: out")
-    T, F = out.shape
-    ld, n, step = _fp8_source(gate_up, "gate_fp8: gate_up", T, 2 * F)
+    T, F, *at = _fp8_check(out, "gate_fp8: out")
+    source = _fp8_source(gate_up, "gate_fp8: gate_up", T, 2 * F)
     _fp8_bias(bias, 2 * F, "gate_fp8")
     _fp8_act(act, "gate_fp8")
-    _check(library("rows_fp8").qd_rows_fp8(
-        _ptr(gate_up), _I(dtype_code(gate_up.dtype)), _LL(ld), _I(n), _LL(step), _I(1), _I(act), _ptr(bias), _ptr(out.q),
-        _LL(out.q.stride(0)), _ptr(out.s), _LL(out.s.stride(0)), _I(T), _I(F), _stream()), "gate_fp8")
+    _rows_fp8(gate_up, *source, 1, act, bias, out, *at, T, F, "gate_fp8")
 
 
 def _fp8_bias(bias: Optional[torch.Tensor], n: int, what: str) -> None:
@@ -1017,73 +1049,76 @@ def add_rmsnorm_fp8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
     """``add_rmsnorm`` with its output in 8 bits: out[r] = rmsnorm(x[s] + delta[s]) * weight with s = rows[r] (or r), rounded once; x
     float32 [T, D] is updated to x + delta when ``write_back``.  delta: bfloat16 or float32 [T, D], or float32 partial sums [n, T, D];
     ``delta_scale`` float32 [D] or None multiplies it."""
-    _fp8_check(out, "add_rmsnorm_fp8: out")
-    R, D = out.shape
+    R, D, q, ldq, s, lds = _fp8_check(out, "add_rmsnorm_fp8: out")
     if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != D or not x.is_contiguous():
         raise KernelError(f"add_rmsnorm_fp8: x must be contiguous float32 [T, {D}]")
-    for name, v in (("weight", weight), ("delta_scale", delta_scale)):
-        if v is not None and (v.dtype != torch.float32 or v.numel() != D or not v.is_contiguous()):
-            raise KernelError(f"add_rmsnorm_fp8: {name} must be contiguous float32 [{D}]")
-    if rows is None and R != x.shape[0] or rows is not None and (rows.dtype != torch.int32 or rows.numel() != R or not rows.is_contiguous()):
+    T = x.shape[0]
+    if weight.dtype != torch.float32 or weight.numel() != D or not weight.is_contiguous():
+        raise KernelError(f"add_rmsnorm_fp8: weight must be contiguous float32 [{D}]")
+    if delta_scale is not None and (delta_scale.dtype != torch.float32 or delta_scale.numel() != D or not delta_scale.is_contiguous()):
+        raise KernelError(f"add_rmsnorm_fp8: delta_scale must be contiguous float32 [{D}]")
+    if rows is None and R != T or rows is not None and (rows.dtype != torch.int32 or rows.numel() != R or not rows.is_contiguous()):
         raise KernelError("add_rmsnorm_fp8: out has a row for every row of x, or for every one of rows (contiguous int32)")
-    n = 1
+    code, n = F32, 1
     if delta is not None:
-        _, n, _ = _fp8_source(delta, "add_rmsnorm_fp8: delta", *x.shape)
+        code, _, n, _ = _fp8_source(delta, "add_rmsnorm_fp8: delta", T, D)
         if not delta.is_contiguous():
             raise KernelError("add_rmsnorm_fp8: delta must be contiguous")
-    _check(library("rows_fp8").qd_add_rmsnorm_fp8(
-        _ptr(x), _ptr(delta), _I(dtype_code(delta.dtype) if delta is not None else F32), _ptr(delta_scale), _ptr(weight), _ptr(out.q),
-        _LL(out.q.stride(0)), _ptr(out.s), _LL(out.s.stride(0)), _ptr(rows), _I(R), _I(D), _F(eps), _I(1 if write_back else 0), _I(n),
-        _LL(x.numel()), _stream()), "add_rmsnorm_fp8")
+    _on_device(out)
+    _check(_entry("rows_fp8", "qd_add_rmsnorm_fp8", "ppippplplpiifiilp")(
+        _raw_ptr(x), _raw_ptr(delta), code, _raw_ptr(delta_scale), _raw_ptr(weight), q, ldq, s, lds, _raw_ptr(rows), R, D, eps,
+        1 if write_back else 0, n, T * D, _stream()), "add_rmsnorm_fp8")
 
 
 @functools.lru_cache(maxsize=4096)
 def gemm_fp8_plan(T: int, N: int, K: int, epi: int, out_code: int, sms: int):
     """(CTAs to a tile of tokens, rows of w to a tile, shares of K) of a product in 8 bits; ``out_code``: ``dtype_code`` of the result
     (of ``EPI_STORE``)."""
-    a, b, c = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
-    if not library("gemm_fp8").qd_gemm_fp8_plan(_I(T), _I(N), _I(K), _I(epi), _I(out_code), _I(sms), ctypes.byref(a), ctypes.byref(b), ctypes.byref(c)):
+    v = [ctypes.c_int(0) for _ in range(3)]
+    if not library("gemm_fp8").qd_gemm_fp8_plan(_I(T), _I(N), _I(K), _I(epi), _I(out_code), _I(sms), *map(ctypes.byref, v)):
         raise KernelError(f"gemm_fp8: no product of {T} x {K} by {N} x {K}")
-    return a.value, b.value, c.value
+    return tuple(n.value for n in v)
 
 
-def _gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias, out, ldo, s_out, lds_out, epi, plan, what):
-    T, K = x.shape
-    N = w.shape[0]
+def _gemm_fp8(x_at, w_at, bias, out, code, ldo, s_out, lds_out, epi, plan, what):
+    T, K, x, ldx, sx, ldsx = x_at
+    N, _, w, ldw, sw, ldsw = w_at
     if T == 0 or N == 0:
         return
-    code = dtype_code(out.dtype) if s_out is None else BF16
-    cg, bn, splits = plan or gemm_fp8_plan(T, N, K, epi, code, sm_count())
-    _check(library("gemm_fp8").qd_gemm_fp8(
-        _ptr(w.q), _LL(w.q.stride(0)), _ptr(w.s), _LL(w.s.stride(0)), _ptr(x.q), _LL(x.q.stride(0)), _ptr(x.s), _LL(x.s.stride(0)),
-        _ptr(bias), _ptr(out), _I(code), _LL(ldo), _ptr(s_out), _LL(lds_out), _I(T), _I(N), _I(K),
-        _I(cg), _I(bn), _I(splits), _I(epi), _I(sm_count()), _stream()), what)
+    sms = sm_count()
+    cg, bn, splits = plan or gemm_fp8_plan(T, N, K, epi, code, sms)
+    _check(_entry("gemm_fp8", "qd_gemm_fp8", "plplplplppilpliiiiiiiip")(
+        w, ldw, sw, ldsw, x, ldx, sx, ldsx, _raw_ptr(bias), out, code, ldo, s_out, lds_out, T, N, K, cg, bn, splits, epi, sms, _stream()), what)
 
 
 def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Tensor, plan=None) -> None:
     """out[T, N] = x @ w^T (+ bias float32 [N]) of rows in 8 bits on the tensor cores, float32 sums; out bfloat16 or float32, rows may
     lie apart.  ``plan``: as ``gemm_fp8_plan`` gives it."""
-    _fp8_check(x, "gemm_fp8: x")
-    _fp8_check(w, "gemm_fp8: w", K=x.shape[1])
-    T, N = x.shape[0], w.shape[0]
-    if out.dtype not in (torch.float32, torch.bfloat16) or tuple(out.shape) != (T, N) or (out.stride(1) != 1 and N > 1):
+    x_at = _fp8_check(x, "gemm_fp8: x")
+    w_at = _fp8_check(w, "gemm_fp8: w", K=x_at[1])
+    T, N, dt = x_at[0], w_at[0], out.dtype
+    if dt not in (torch.float32, torch.bfloat16) or out.shape != (T, N) or (out.stride(1) != 1 and N > 1):
         raise KernelError(f"gemm_fp8: out must be bfloat16 or float32 [{T}, {N}] with contiguous rows")
     _fp8_bias(bias, N, "gemm_fp8")
-    _gemm_fp8(x, w, bias, out, out.stride(0), None, 0, EPI_STORE, plan, "gemm_fp8")
+    _on_device(x)
+    _on_device(w)
+    _gemm_fp8(x_at, w_at, bias, _raw_ptr(out), F32 if dt == torch.float32 else BF16, out.stride(0), None, 0, EPI_STORE, plan, "gemm_fp8")
 
 
 def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None) -> None:
     """out[T, F] = act(x @ wg^T + bg) * (x @ wu^T + bu) in 8 bits, for the product that follows: w [2F, K] holds the gate's rows, then
     up's, ``bias`` float32 [2F] (or None) likewise; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``.  The sums and the activation are
     float32, rounded once."""
-    _fp8_check(x, "gemm_fp8_gated: x")
-    _fp8_check(w, "gemm_fp8_gated: w", K=x.shape[1])
-    if w.shape[0] % 2:
+    x_at = _fp8_check(x, "gemm_fp8_gated: x")
+    w_at = _fp8_check(w, "gemm_fp8_gated: w", K=x_at[1])
+    if w_at[0] % 2:
         raise KernelError("gemm_fp8_gated: w holds as many rows of up as of the gate")
-    _fp8_check(out, "gemm_fp8_gated: out", x.shape[0], w.shape[0] // 2)
-    _fp8_bias(bias, w.shape[0], "gemm_fp8_gated")
+    _, _, q, ldq, s, lds = _fp8_check(out, "gemm_fp8_gated: out", x_at[0], w_at[0] // 2)
+    _fp8_bias(bias, w_at[0], "gemm_fp8_gated")
     _fp8_act(act, "gemm_fp8_gated")
-    _gemm_fp8(x, w, bias, out.q, out.q.stride(0), out.s, out.s.stride(0), EPI_SWIGLU + 256 * act, plan, "gemm_fp8_gated")
+    for rows in (x, w, out):
+        _on_device(rows)
+    _gemm_fp8(x_at, w_at, bias, q, BF16, ldq, s, lds, EPI_SWIGLU + 256 * act, plan, "gemm_fp8_gated")
 
 
 # ------------------------------------------------------------------ latent attention

@@ -205,9 +205,9 @@ def test_product(T, N, K, dtype):
     want, off = value(x) @ value(w).T, sums_off(x, w)
     plans = {None}
     for cg in (1, 2):
-        for bn in (32, 64, 96, 128, 192, 224, 256):
+        for bn in (32, 48, 64, 96, 128, 192, 208, 224, 240, 256):
             for splits in (1, 2, 3, 8):
-                if (cg == 1 or splits == 1) and splits <= -(-K // 128) and not (dtype == torch.float32 and bn > 128):
+                if (cg == 1 or splits == 1) and (bn % 32 == 0 or cg * splits == 1) and splits <= -(-K // 128) and not (dtype == torch.float32 and bn > 128):
                     plans.add((cg, bn, splits))
     for plan in sorted(plans, key=str):
         for b in (None, bias):
@@ -246,7 +246,7 @@ def test_products_of_several_tiles_to_a_worker():
     from qwen_decoder_b200 import kernels
     x, w, _ = operands(520, 19000, 256)
     want, off = value(x) @ value(w).T, sums_off(x, w)
-    for plan in ((1, 256, 1), (2, 256, 1), (1, 32, 1), (2, 224, 1)):
+    for plan in ((1, 256, 1), (2, 256, 1), (1, 32, 1), (2, 224, 1), (1, 240, 1)):
         out = torch.empty(520, 19000, dtype=torch.bfloat16, device=DEV)
         kernels.gemm_fp8(x, w, None, out, plan)
         assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + off).all(), plan
