@@ -9,13 +9,14 @@
 // memories, so that a call is one launch without scratch memory of its own.
 //
 // The most probable ``top``: a token is a 64-bit key, its logit's bits in their order above the complement of its index, so that of equal
-// logits the lowest index is the largest key.  Every warp keeps a list of keys in shared memory and a threshold that at least ``top`` logits
-// of the list reach; only larger ones join it (a warp's later tiles have higher indices: equal ones lose), and it is cut back to its first
-// ``top`` when it has LP_CUT: no barrier of the CTA holds the reading up (with one list to a CTA and a barrier to every tile 509 rows of
-// 152,064 took 80 us, without a list 52).  For the first tile the threshold is the ``top``-th of the lanes' maxima.  Where a tile brings more
-// than the list holds (rows in rising order, a thousand equal logits), its largest ``top`` are taken one by one.  Of L sorted lists the
-// keys that count are those not below the least of the lists' ceil(top / L)-th keys, which ``top`` keys reach: few, and put in order by
-// counting for each how many are larger.
+// logits the lowest index is the largest key.  While a row is read only the maximum of every 512 neighbouring logits (a warp's of a tile) is
+// kept.  Then the ``top`` largest maxima are found, of equal ones the first: no other 512 hold one of the ``top`` logits, for each of those
+// chosen has one that comes before all of theirs.  They are read again (20 of 2 KB of a row of 600), and what reaches the least of the chosen
+// maxima is put in order by counting for each key how many are larger.  Where more than LP_HITS of 512 do (a thousand equal logits, a mask that
+// leaves fewer than ``top``), their largest ``top`` are taken one by one.  (With lists that grew while the row was read, 509 rows of 152,064
+// took 80 us with one to a CTA and a barrier to every tile, 131 with one to a warp; 52 without any.)
+// Of sorted lists of several CTAs the keys that count are those not below the least of the L lists' ceil(top / L)-th keys, which ``top`` keys
+// reach.
 //
 // The reference has no log probabilities; its sampler's softmax is common.cpp:576-629.
 #include "common.cuh"
@@ -25,9 +26,12 @@
 #define LP_EACH 16                           // logits of a thread's tile
 #define LP_TILE (LP_THREADS * LP_EACH)
 #define LP_MAX_TOP 32
-#define LP_LIST 96                           // of a warp
-#define LP_CUT 64
 #define LP_MAX_SHARES 16
+#define LP_CHUNK 512                         // a warp's logits of a tile
+#define LP_HITS 64                           // logits of a chunk that join without being chosen one by one
+#define LP_LANE 16                           // chunks to a lane of the warp that chooses
+#define LP_MAX_CHUNKS (32 * LP_LANE)         // of a CTA
+#define LP_MAX_VOCABULARY (LP_MAX_SHARES * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE)
 #define LP_LOWEST (-3.402823466e38f)
 
 struct LpArgs {
@@ -78,34 +82,39 @@ __device__ __forceinline__ unsigned long long lp_warp_max(unsigned long long k) 
 }
 
 struct LpShared {
-  unsigned long long list[LP_WARPS][LP_LIST], joined[LP_MAX_SHARES * LP_MAX_TOP], sorted[LP_MAX_TOP];
+  unsigned long long joined[LP_MAX_TOP * LP_HITS], sorted[LP_MAX_TOP];
+  unsigned peaks[LP_MAX_CHUNKS], least;
   LpSum sum[LP_WARPS], whole;
-  int n[LP_WARPS], n_joined, n_sorted;
+  int chosen[LP_MAX_TOP], n_chosen, n_joined, n_sorted;
 };
 
-// A warp's list of ``n`` keys in order, cut to the first ``top``; their number
-__device__ __forceinline__ int lp_cut(unsigned long long* list, int n, int top) {
+// Which logit a lane's i-th of 512 from ``at`` on is: whole 16 bytes of a lane side by side, or one by one
+template <typename TX>
+__device__ __forceinline__ int lp_index(int at, int i, bool vec) {
+  constexpr int E = 16 / (int)sizeof(TX);
   const int lane = threadIdx.x & 31;
-  unsigned long long mine[LP_LIST / 32];
-  int before[LP_LIST / 32];
-  __syncwarp();
+  return vec ? at + (i / E) * 32 * E + lane * E + i % E : at + i * 32 + lane;
+}
+// A lane's 16 of them, minus infinity behind the row's end
+template <typename TX>
+__device__ __forceinline__ void lp_load(float (&v)[LP_EACH], const TX* z, int at, int V, bool vec) {
+  constexpr int E = 16 / (int)sizeof(TX);
+  if (vec && at + LP_CHUNK <= V) {
 #pragma unroll
-  for (int i = 0; i < LP_LIST / 32; i++) {
-    mine[i] = lane + 32 * i < n ? list[lane + 32 * i] : 0ull;
-    before[i] = 0;
+    for (int i = 0; i < LP_EACH / E; i++) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(z + lp_index<TX>(at, i * E, true));
+      const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int j = 0; j < E; j++)
+        v[i * E + j] = __uint_as_float(sizeof(TX) == 4 ? w[j & 3] : j & 1 ? w[j >> 1 & 3] & 0xffff0000u : w[j >> 1 & 3] << 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < LP_EACH; i++) {
+      const int k = lp_index<TX>(at, i, vec);
+      v[i] = k < V ? to_float(z[k]) : -INFINITY;
+    }
   }
-#pragma unroll 4
-  for (int j = 0; j < n; j++) {
-    const unsigned long long k = list[j];
-#pragma unroll
-    for (int i = 0; i < LP_LIST / 32; i++) before[i] += k > mine[i];
-  }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < LP_LIST / 32; i++)
-    if (mine[i] && before[i] < top) list[before[i]] = mine[i];
-  __syncwarp();
-  return min(n, top);
 }
 
 template <typename TX>
@@ -113,36 +122,16 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   __shared__ LpShared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x / a.shares, share = blockIdx.x - row * a.shares;
-  unsigned long long* list = sh.list[warp];
   if (threadIdx.x == 0) sh.n_joined = 0;
   pdl_launch_dependents();
   pdl_wait();
   const TX* z = (const TX*)a.logits + row * a.ld;
   const int tiles = (a.V + LP_TILE - 1) / LP_TILE;
   const int lo = (int)((long long)tiles * share / a.shares), hi = (int)((long long)tiles * (share + 1) / a.shares);
-  constexpr int E = 16 / (int)sizeof(TX);                            // of a load
   LpSum sum = {LP_LOWEST, 0.f, 0.f};
-  float least = 0.f;                                                 // a logit joins the warp's list above this, ...
-  bool any = true;                                                   // ... or any does
-  int n = 0;                                                         // of the list, the same to all lanes
   for (int tile = lo; tile < hi; tile++) {
-    const int t0 = tile * LP_TILE;
-    // which logit a thread's i-th is: whole 16 bytes of a thread side by side, or one by one
-    auto index = [&](int i) { return a.vec ? t0 + (i / E) * LP_THREADS * E + (int)threadIdx.x * E + i % E : t0 + i * LP_THREADS + (int)threadIdx.x; };
     float v[LP_EACH];
-    if (a.vec && t0 + LP_TILE <= a.V) {
-#pragma unroll
-      for (int i = 0; i < LP_EACH / E; i++) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(z + index(i * E));
-        const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int j = 0; j < E; j++)
-          v[i * E + j] = __uint_as_float(sizeof(TX) == 4 ? w[j & 3] : j & 1 ? w[j >> 1 & 3] & 0xffff0000u : w[j >> 1 & 3] << 16);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < LP_EACH; i++) v[i] = index(i) < a.V ? to_float(z[index(i)]) : -INFINITY;
-    }
+    lp_load(v, z, tile * LP_TILE + warp * LP_CHUNK, a.V, a.vec);
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < LP_EACH; i++) m = fmaxf(m, v[i]);
@@ -153,67 +142,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
       sum.s += e;                                                    // (NaN comes this way)
       sum.d = fmaf(fmaxf(d, -256.f), e, sum.d);
     }
-    if (!a.top) continue;
-    const bool first = tile == lo;
-    if (first) {
-      unsigned left = lp_order(m), o = 0;
-      for (int i = 0; i < a.top; i++) {
-        o = __reduce_max_sync(0xffffffffu, left);
-        if ((int)__ffs(__ballot_sync(0xffffffffu, left == o)) - 1 == lane) left = 0;
-      }
-      any = o == 0;                                                  // (a lane with no number at all: no bound)
-      least = any ? 0.f : lp_value(o);
-    }
-    if (!__any_sync(0xffffffffu, any || m > least || (first && m == least))) continue;
-    unsigned hits = 0;
-    int more = 0;
-    auto count = [&]() {
-      hits = 0;
-#pragma unroll
-      for (int i = 0; i < LP_EACH; i++)
-        if ((any ? v[i] == v[i] : v[i] > least || (first && v[i] == least)) && index(i) < a.V) hits |= 1u << i;
-      more = __reduce_add_sync(0xffffffffu, __popc(hits));
-    };
-    auto cut = [&]() {
-      n = lp_cut(list, n, a.top);
-      any = n < a.top;
-      least = any ? 0.f : lp_value((unsigned)(list[a.top - 1] >> 32));
-    };
-    count();
-    if (n + more > LP_LIST && n > a.top) {
-      cut();
-      count();
-    }
-    if (n + more > LP_LIST) {
-      // the tile's largest ones, one after the other
-      unsigned long long last = ~0ull;
-      for (int k = 0; k < a.top; k++) {
-        unsigned long long mine = 0;
-#pragma unroll 1
-        for (int i = 0; i < LP_EACH; i++) {                          // (read again: kept numbers would cost every tile registers)
-          const int at = index(i);
-          const unsigned long long key = at < a.V ? lp_key(to_float(z[at]), at) : 0ull;
-          if (key < last && key > mine) mine = key;
-        }
-        last = lp_warp_max(mine);
-        if (!last) break;
-        if (lane == 0) list[n] = last;
-        n++;
-      }
-      cut();
-    } else {
-      int at = __popc(hits);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += x;
-      }
-      at += n - __popc(hits);
-#pragma unroll
-      for (int i = 0; i < LP_EACH; i++)
-        if (hits >> i & 1) list[at++] = lp_key(v[i], index(i));
-      n += more;
-      if (n >= LP_CUT || first) cut();
+    if (a.top) {
+      const unsigned peak = __reduce_max_sync(0xffffffffu, lp_order(m));
+      if (lane == 0) sh.peaks[(tile - lo) * LP_WARPS + warp] = peak;
     }
   }
   // ---- the CTA's sums and its list
@@ -221,18 +152,14 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   lp_to(sum, m);
   sum.s = warp_sum(sum.s);
   sum.d = warp_sum(sum.d);
-  if (a.top) n = lp_cut(list, n, a.top);
-  if (lane == 0) {
-    sh.sum[warp] = sum;
-    sh.n[warp] = n;
-  }
+  if (lane == 0) sh.sum[warp] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     LpSum w = sh.sum[0];
     for (int i = 1; i < LP_WARPS; i++) lp_join(w, sh.sum[i]);
     sh.whole = w;
   }
-  // keys of sorted lists that are not below ``least`` (of the lists' ``nth`` keys, 0 where one has fewer) join, and are put in order
+  // the joined keys in order
   auto order = [&]() {
     __syncthreads();
     const int total = sh.n_joined;
@@ -246,11 +173,94 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
     __syncthreads();
   };
   if (a.top) {
-    const int nth = (a.top + LP_WARPS - 1) / LP_WARPS - 1;
-    unsigned long long bound = ~0ull;
+    if (warp == 0) {
+      // the ``top`` largest of the chunks' maxima, a lane's chunks beside one another
+      const int chunks = (hi - lo) * LP_WARPS;
+      unsigned peak[LP_LANE], mine = 0, o = 0;
 #pragma unroll
-    for (int i = 0; i < LP_WARPS; i++) bound = min(bound, nth < sh.n[i] ? sh.list[i][nth] : 0ull);
-    if (lane < n && list[lane] >= bound) sh.joined[atomicAdd(&sh.n_joined, 1)] = list[lane];
+      for (int i = 0; i < LP_LANE; i++) {
+        peak[i] = lane * LP_LANE + i < chunks ? sh.peaks[lane * LP_LANE + i] : 0u;
+        mine = max(mine, peak[i]);
+      }
+      int k = 0;
+      for (; k < a.top; k++) {
+        const unsigned next = __reduce_max_sync(0xffffffffu, mine);
+        if (!next) break;                                            // (no number in any of the others)
+        o = next;
+        if ((int)__ffs(__ballot_sync(0xffffffffu, mine == o)) - 1 == lane) {
+          int at = LP_LANE;
+#pragma unroll
+          for (int i = LP_LANE - 1; i >= 0; i--)
+            if (peak[i] == o) at = i;
+          mine = 0;
+#pragma unroll
+          for (int i = 0; i < LP_LANE; i++) {
+            if (i == at) peak[i] = 0;
+            mine = max(mine, peak[i]);
+          }
+          sh.chosen[k] = lane * LP_LANE + at;
+        }
+      }
+      if (lane == 0) {
+        sh.n_chosen = k;
+        sh.least = k == a.top ? o : 1u;
+      }
+    }
+    __syncthreads();
+    if (sh.n_chosen < a.top) {
+      // Fewer chunks than tokens: of each chunk the maxima of 64 times 8 logits, of which the ``top``-th is reached by ``top`` logits
+      for (int c = warp; c < sh.n_chosen; c += LP_WARPS) {
+        float v[LP_EACH];
+        lp_load(v, z, lo * LP_TILE + sh.chosen[c] * LP_CHUNK, a.V, a.vec);
+        float x = v[0], y = v[LP_EACH / 2];
+#pragma unroll
+        for (int i = 1; i < LP_EACH / 2; i++) {
+          x = fmaxf(x, v[i]);
+          y = fmaxf(y, v[LP_EACH / 2 + i]);
+        }
+        unsigned one = lp_order(x), two = lp_order(y), o = 0;
+        for (int k = 0; k < a.top; k++) {
+          o = __reduce_max_sync(0xffffffffu, max(one, two));
+          if ((int)__ffs(__ballot_sync(0xffffffffu, max(one, two) == o)) - 1 == lane) {
+            if (one == o) one = 0;
+            else two = 0;
+          }
+        }
+        if (lane == 0 && o) atomicMax(&sh.least, o);
+      }
+      __syncthreads();
+    }
+    const unsigned least = sh.least;
+    for (int c = warp; c < sh.n_chosen; c += LP_WARPS) {
+      const int at = lo * LP_TILE + sh.chosen[c] * LP_CHUNK;
+      float v[LP_EACH];
+      lp_load(v, z, at, a.V, a.vec);
+      unsigned hits = 0;
+#pragma unroll
+      for (int i = 0; i < LP_EACH; i++)
+        if (lp_order(v[i]) >= least && lp_index<TX>(at, i, a.vec) < a.V) hits |= 1u << i;
+      if (__reduce_add_sync(0xffffffffu, __popc(hits)) <= LP_HITS) {
+        while (hits) {
+          const int i = __ffs(hits) - 1, k = lp_index<TX>(at, i, a.vec);
+          hits &= hits - 1;
+          sh.joined[atomicAdd(&sh.n_joined, 1)] = lp_key(to_float(z[k]), k);
+        }
+      } else {
+        // their largest ones, one after the other
+        unsigned long long last = ~0ull;
+        for (int k = 0; k < a.top; k++) {
+          unsigned long long mine = 0;
+#pragma unroll
+          for (int i = 0; i < LP_EACH; i++) {
+            const unsigned long long key = hits >> i & 1 ? lp_key(v[i], lp_index<TX>(at, i, a.vec)) : 0ull;
+            if (key < last && key > mine) mine = key;
+          }
+          last = lp_warp_max(mine);
+          if (!last) break;
+          if (lane == 0) sh.joined[atomicAdd(&sh.n_joined, 1)] = last;
+        }
+      }
+    }
     order();
   } else {
     __syncthreads();
@@ -315,7 +325,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
     if (share) return;
   }
   if (warp) return;
-  n = a.top ? sh.n_sorted : 0;
+  const int n = a.top ? sh.n_sorted : 0;
   const float log_s = logf(whole.s);
   // (a row of minus infinities alone has no probabilities: none is above 0)
   auto log_p = [&](float x) { return whole.s == 0.f ? -INFINITY : x - whole.m - log_s; };
@@ -337,15 +347,21 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
 extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob, float* entropy,
                                  int* top_ids, float* top_logprobs, int R, int V, int top, int sms, int shares, cudaStream_t stream) {
   if (R <= 0) return 0;
-  if ((dtype != QD_F32 && dtype != QD_BF16) || V <= 0 || V > (1 << 30) || top < 0 || top > LP_MAX_TOP || top > V || sms < 1 || shares > LP_MAX_SHARES)
+  if ((dtype != QD_F32 && dtype != QD_BF16) || V <= 0 || V > LP_MAX_VOCABULARY || top < 0 || top > LP_MAX_TOP || top > V || sms < 1 || shares > LP_MAX_SHARES)
     return QD_ERR_UNSUPPORTED;
   LpArgs a;
   a.logits = logits; a.tokens = tokens; a.logprob = logprob; a.entropy = entropy; a.top_ids = top_ids; a.top_logprobs = top_logprobs;
   a.R = R; a.V = V; a.top = top; a.ld = ld;
   const int size = dtype == QD_F32 ? 4 : 2;
   a.vec = !((uintptr_t)logits & 15) && ld * size % 16 == 0;
+  // As many CTAs to a row as run at a time, four to a multiprocessor, with four tiles and half again as many chunks as ``top`` to each.
+  // Measured, us: 64 rows of 152,064 with 4, 8 and 16 17.3, 14.3 and 27.6, 148 rows of 32,000 with 1, 2 and 4 11.2, 10.9 and 16.0.
+  const int tiles = (V + LP_TILE - 1) / LP_TILE;
   a.shares = shares > 0 ? shares : 1;
-  while (shares <= 0 && a.shares < LP_MAX_SHARES && (long long)R * a.shares * 2 <= 4ll * sms && a.shares * 2 * LP_TILE <= V) a.shares *= 2;
+  while (shares <= 0 && a.shares < LP_MAX_SHARES && (long long)R * a.shares * 2 <= 4ll * sms && tiles / (a.shares * 2) >= 4 &&
+         2 * (tiles / (a.shares * 2)) * LP_WARPS >= 3 * top)
+    a.shares *= 2;
+  while (a.shares * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE < V) a.shares++;      // a CTA keeps so many maxima
   if ((long long)R * a.shares > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(R * a.shares));

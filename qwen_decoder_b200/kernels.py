@@ -843,7 +843,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                                          _ptr(draws), _ptr(out), _stream()), "sample")
 
 
-LOGPROBS_MAX_TOP = 32
+LOGPROBS_MAX_TOP, LOGPROBS_MAX_VOCABULARY = 32, 1 << 22
 LOGPROBS_SHARES = 0
 
 
@@ -859,6 +859,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     R, V = logits.shape
     if tokens.dtype != torch.int32 or tokens.shape != (R,) or not tokens.is_contiguous():
         raise KernelError(f"token_logprobs: tokens must be contiguous int32 [{R}]")
+    if V > LOGPROBS_MAX_VOCABULARY:
+        raise KernelError(f"token_logprobs: rows of at most {LOGPROBS_MAX_VOCABULARY} logits, got {V}")
     if V < 1 or not 0 <= top <= min(LOGPROBS_MAX_TOP, V):
         raise KernelError(f"token_logprobs: top must be between 0 and {min(LOGPROBS_MAX_TOP, V)}, got {top}")
     new = lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=logits.device)      # noqa: E731
