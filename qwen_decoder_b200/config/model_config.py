@@ -11,7 +11,7 @@ from __future__ import annotations
 import json
 import os
 from dataclasses import dataclass, field, asdict
-from typing import Any, Mapping
+from typing import Any, Mapping, Optional
 
 
 class ConfigError(ValueError):
@@ -79,6 +79,10 @@ class Qwen2Config:
     # cpu_decoder.cpp:135-146); the optional key ``rope_pairing`` selects it.
     rope_pairing: str = "half"
     attention_bias: bool = True  # q, k, v carry a bias (gpu_decoder.cu:347-349)
+    # What the layers' four projections, and the one over the vocabulary, compute in: None, the engine's dtype, or "float8_e4m3", 8 bits
+    # with a scale to each 128 features (the reference has 16-bit weights only).  The stored tensors are the same.
+    projection_dtype: Optional[str] = None
+    output_projection_dtype: Optional[str] = None
     eos_token_ids: tuple = ()
     torch_dtype: str = "bfloat16"
     extra: dict = field(default_factory=dict, compare=False, hash=False)
@@ -131,6 +135,10 @@ class Qwen2Config:
         pairing = _get(d, "rope_pairing", str, "half")
         if pairing not in ("adjacent", "half"):
             raise ConfigError(f"config.json: 'rope_pairing' must be 'adjacent' or 'half', got {pairing!r}")
+        projections = {key: _get(d, key, str, None) for key in ("projection_dtype", "output_projection_dtype")}
+        for key, value in projections.items():
+            if value not in (None, "float8_e4m3"):
+                raise ConfigError(f"config.json: '{key}' must be 'float8_e4m3' if given, got {value!r}")
         eos = d.get("eos_token_id")
         if eos is None:
             eos_ids: tuple = ()
@@ -158,6 +166,7 @@ class Qwen2Config:
             attention_bias=_get(d, "attention_bias", bool, True),
             eos_token_ids=eos_ids,
             torch_dtype=_get(d, "torch_dtype", str, "bfloat16"),
+            **projections,
         )
         for name in ("hidden_size", "intermediate_size", "num_hidden_layers", "vocab_size",
                      "max_position_embeddings"):
@@ -193,6 +202,9 @@ class Qwen2Config:
         }
         if self.eos_token_ids:
             d["eos_token_id"] = list(self.eos_token_ids)
+        for key in ("projection_dtype", "output_projection_dtype"):
+            if getattr(self, key) is not None:
+                d[key] = getattr(self, key)
         return d
 
 

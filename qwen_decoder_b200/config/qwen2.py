@@ -5,7 +5,8 @@ cpu_decoder.cpp:111-220): embedding; per layer pre-norm -> grouped-query
 attention with q/k/v bias and rotary positions -> residual -> pre-norm -> SwiGLU
 feed-forward -> residual; final norm; output projection (tied to the embedding
 when ``tie_word_embeddings`` is set, which the reference cannot do:
-common.cpp:119 requires ``output.weight``).
+common.cpp:119 requires ``output.weight``).  With ``projection_dtype`` the same layers of
+parts whose products take 8 bits.
 """
 from __future__ import annotations
 
@@ -16,12 +17,14 @@ from .spec import LayerSpec, ModelSpec, PartSpec, ScheduleEntry
 
 def describe_qwen2(cfg: Qwen2Config) -> ModelSpec:
     norm = PartSpec("rmsnorm", {"size": cfg.hidden_size, "eps": cfg.rms_norm_eps})
+    in_8_bits = "_fp8" if cfg.projection_dtype is not None else ""
+    out_8_bits = "_fp8" if cfg.output_projection_dtype is not None else ""
     layers = []
     for i in range(cfg.num_hidden_layers):
         layers.append(LayerSpec(
             prefix=f"model.layers.{i}.",
             block="pre_norm",
-            mixer=PartSpec("gq_attention", {
+            mixer=PartSpec("gq_attention" + in_8_bits, {
                 "hidden_size": cfg.hidden_size,
                 "num_heads": cfg.num_attention_heads,
                 "num_kv_heads": cfg.num_key_value_heads,
@@ -32,14 +35,14 @@ def describe_qwen2(cfg: Qwen2Config) -> ModelSpec:
                 "window": None,
                 "prefix": "self_attn.",
             }),
-            feed_forward=PartSpec("swiglu", {
+            feed_forward=PartSpec("swiglu" + in_8_bits, {
                 "hidden_size": cfg.hidden_size,
                 "intermediate_size": cfg.intermediate_size,
                 "prefix": "mlp.",
             }),
             norms={
-                "input": PartSpec("rmsnorm", dict(norm.params, prefix="input_layernorm.")),
-                "post_mixer": PartSpec("rmsnorm", dict(norm.params, prefix="post_attention_layernorm.")),
+                "input": PartSpec("rmsnorm" + in_8_bits, dict(norm.params, prefix="input_layernorm.")),
+                "post_mixer": PartSpec("rmsnorm" + in_8_bits, dict(norm.params, prefix="post_attention_layernorm.")),
             },
         ))
     return ModelSpec(
@@ -55,9 +58,10 @@ def describe_qwen2(cfg: Qwen2Config) -> ModelSpec:
         })},
         layers=layers,
         schedule=[ScheduleEntry(layer=i) for i in range(cfg.num_hidden_layers)],
-        final_norm=PartSpec("rmsnorm", dict(norm.params, prefix="")),
+        final_norm=PartSpec("rmsnorm" + out_8_bits, dict(norm.params, prefix="")),
         final_norm_prefix="model.norm.",
         lm_head_tensor=None if cfg.tie_word_embeddings else "lm_head.weight",
+        lm_head_in_8_bits=bool(out_8_bits),
     )
 
 

@@ -64,3 +64,4 @@ class ModelSpec:
     lm_head_tensor: Optional[str]           # None: tied to the embedding
     embedding_scale: float = 1.0            # the embedding row is multiplied by this constant
     logit_softcap: Optional[float] = None   # c: logits z leave as c tanh(z / c)
+    lm_head_in_8_bits: bool = False         # the output projection takes rows in 8 bits, which the final norm must leave

@@ -176,17 +176,20 @@ __device__ __forceinline__ void g8_stage16(unsigned char* rows, int row, int pie
 template <typename TO>
 __device__ __forceinline__ void g8_store_rows(unsigned char* rows, TO* dst, long long ld, int n_rows, int pieces, int left, bool vec) {
   constexpr int E = 16 / (int)sizeof(TO);
-  const int lane = threadIdx.x & 31, piece = lane & 3, e0 = piece * E;
-  if (piece >= pieces || e0 >= left) return;
+  const int lane = threadIdx.x & 31;
+  if (vec && left >= pieces * E) {
+    const int piece = lane & 3;
+    if (piece >= pieces) return;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int r = 8 * i + (lane >> 2);
-    if (r >= n_rows) break;
-    const uint4* src = g8_piece(rows, r, piece);
-    TO* to = dst + (size_t)r * ld + e0;
-    if (vec && e0 + E <= left) *reinterpret_cast<uint4*>(to) = *src;
-    else
-      for (int e = 0; e < E && e0 + e < left; e++) to[e] = reinterpret_cast<const TO*>(src)[e];
+    for (int i = 0; i < 4; i++) {
+      const int r = 8 * i + (lane >> 2);
+      if (r < n_rows) *reinterpret_cast<uint4*>(dst + (size_t)r * ld + piece * E) = *g8_piece(rows, r, piece);
+    }
+  } else {
+    // a row at a time, its elements side by side
+    const int n = min(left, pieces * E);
+    for (int r = 0; r < n_rows; r++)
+      for (int e = lane; e < n; e += 32) dst[(size_t)r * ld + e] = reinterpret_cast<const TO*>(g8_piece(rows, r, e / E))[e % E];
   }
 }
 
@@ -746,30 +749,37 @@ static int g8_clusters(int n, int sms) {
   return known[n] = got;
 }
 
-// How a product is cut: *cg CTAs to a tile of tokens, *bn rows of W to a tile, K in *splits shares (of a cluster).
 extern "C" int qd_gemm_fp8_clusters(int n, int sms) { return n >= 1 && n <= 8 ? g8_clusters(n, sms) : 0; }
+
+// How a product is cut: *cg CTAs to a tile of tokens, *bn rows of W to a tile, K in *splits shares (of a cluster).
+//
+// The one of the least estimate, in clocks of 1.9 GHz: a worker's rounds over its tiles times its blocks of 128 k, a block being the longest of
+// its MMAs, its bytes into shared memory (70 a clock) and what one costs anyway; W's way from memory, the longer of both and half of the other;
+// an epilogue; a cluster's joining and its CTAs.  Fitted to 6,866 times of 154 shapes (1 to 2,048 tokens, 102 to 20,000 features, 111 to 18,944 of
+// k) in captured graphs on a B200, 6 % rms; the choices take 2.4 % longer than the best of all cuts on average.  Some of them, us, the chosen
+// one and the best of the other kind (without shares where it has some, one CTA where it has two, and the other way round):
+//   1 x 2,048 x 11,008      1 CTA, 192 rows, 8 shares   9.7   96 rows, 1 share   23.0
+//   23 x 4,608 x 3,584      1 CTA, 192 rows, 4 shares   9.0   64 rows, 1 share    9.9
+//   256 x 3,584 x 18,944    1 CTA, 224 rows, 4 shares  23.8   128 rows, 1 share  35.0
+//   2,048 x 3,584 x 3,584   2 CTAs, 224 rows           23.5   1 CTA, 208 rows    24.2
+//   2,048 x 3,584 x 18,944  2 CTAs, 224 rows          128.2   1 CTA, 208 rows   134.8   (under the power limit; alone 106.9 and 113.1)
 extern "C" int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out) {
   epi &= 255;
-  const int most = epi == G8_STORE && out_dtype == QD_F32 ? G8_MAX_FLOAT_BN : 256;
   if (T <= 0 || N <= 0 || K <= 0 || sms < 2) return 0;
-  const int kb = up(K, FP8_BLOCK);
-  const double dram = (double)N * K / 3300.0;          // clocks of 1.9 GHz
+  const int kb = up(K, FP8_BLOCK), most = epi == G8_STORE && out_dtype == QD_F32 ? G8_MAX_FLOAT_BN : 256, feats = epi == G8_GATED ? N / 2 : N;
+  const double dram = (double)N * K / 5400.0;
   double best = 0;
-  for (int cg = T <= 128 ? 1 : 2; cg >= 1; cg--) {
-    const int workers = sms / cg, n_tt = up(T, 128 * cg), mrows = up(up(T, cg * n_tt), 8) * 8;
-    for (int bn = epi == G8_GATED ? 256 : 32; bn <= most; bn += 16) {
-      const long long tiles = (long long)up(epi == G8_GATED ? N / 2 : N, epi == G8_GATED ? bn / 2 : bn) * n_tt;
-      for (int splits = 1; splits <= (epi == G8_GATED || cg == 2 ? 1 : 8) && (splits == 1 || splits * 4 <= kb); splits++) {
-        if ((cg == 2 || splits > 1) && bn % 32) break;
-        if (splits > 1 && tiles > g8_clusters(splits, sms)) break;      // one round
-        const long long rounds = splits > 1 ? 1 : (tiles + workers - 1) / workers;
-        const double bytes = (mrows + bn / cg) * 128 / 60.0;
-        double block = 2.0 * bn;
-        if (block < bytes) block = bytes;
-        if (block < 350) block = 350;
-        const double work = (double)rounds * up(kb, splits) * block;
-        double cost = work > dram ? work + 0.15 * dram : dram + 0.15 * work;
-        cost += 12.0 * bn + (splits > 1 ? 1500.0 : 0.0);
+  for (int cg = 1; cg <= (T > 128 ? 2 : 1); cg++) {
+    const int n_tt = up(T, 128 * cg), mrows = up(up(T, cg * n_tt), 8) * 8;
+    for (int bn = epi == G8_GATED ? 256 : 32; bn <= most; bn += cg == 2 ? 32 : 16) {
+      const long long tiles = (long long)up(feats, epi == G8_GATED ? bn / 2 : bn) * n_tt;
+      const double block = fmax(fmax(2.4 * bn, (mrows + bn / cg) * 128 / 70.0), cg == 2 ? 560.0 : 490.0);
+      for (int splits = 1; splits <= (epi == G8_GATED || cg == 2 || bn % 32 ? 1 : 8) && splits <= kb; splits++) {
+        if (splits > 1 && tiles > g8_clusters(splits, sms)) break;
+        const long long workers = sms / cg, rounds = splits > 1 ? 1 : (tiles + workers - 1) / workers;
+        const double work = (double)rounds * up(kb, splits) * block + (rounds - 1) * 7.7 * bn;
+        double cost = fmax(work, dram) + 0.55 * fmin(work, dram) + (0.18 * mrows + 7.7) * bn;
+        if (splits > 1) cost += 1000.0 + 170.0 * splits + 5100.0 * tiles * splits / sms;
         if (best == 0 || cost < best) { best = cost; *cg_out = cg; *bn_out = bn; *splits_out = splits; }
       }
     }

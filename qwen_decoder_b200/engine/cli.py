@@ -13,7 +13,7 @@ folder needs config.json only; weights N(0, 0.02) from ``--weights-seed`` are ma
 ``--prompt-ids`` / ``--prompt-file`` / ``--random-prompts`` instead of standard input, and ``--stats``:
 one line per step as the reference prints it (decoder.cpp:178-185: tokens, decoding and prefilling
 requests, prompt tokens) with the step's device time and the free pages, and prompt and decode
-tokens per second apart at the end.
+tokens per second apart at the end; ``--projection-dtype float8_e4m3`` (8-bit products) and ``--logprobs K``.
 """
 from __future__ import annotations
 
@@ -66,6 +66,11 @@ def main(argv=None) -> int:
     ap.add_argument("--len", dest="length", default="128", metavar="A[:B]",
                     help="length of the random prompts, or a range to draw each from")
     ap.add_argument("--stats", action="store_true", help="a line per step, and prompt / decode tokens per second")
+    ap.add_argument("--projection-dtype", choices=["float8_e4m3"], default=None,
+                    help="the layers' products in 8 bits, with a scale to each 128 features")
+    ap.add_argument("--output-projection-dtype", choices=["float8_e4m3"], default=None, help="the product over the vocabulary, too")
+    ap.add_argument("--logprobs", type=int, default=None, metavar="K",
+                    help="each output token's log probability, and the K (0 to 32) most probable tokens in its place")
     args = ap.parse_args(argv)
 
     print(f"max_batch={args.max_batch} max_total_tokens={args.max_total_tokens} "
@@ -99,13 +104,15 @@ def main(argv=None) -> int:
                    max_prefill_len=args.max_prefill_len, max_prefill_tokens_per_step=args.max_prefill_step,
                    max_total_tokens=args.max_total_tokens, page_size=args.page_size, num_pages=args.num_pages,
                    enable_prefix_cache=bool(args.enable_prefix_cache), run_ahead=not args.no_run_ahead,
-                   record_steps=args.stats)
+                   record_steps=args.stats, projection_dtype=args.projection_dtype,
+                   output_projection_dtype=args.output_projection_dtype)
     if args.random_weights:
         engine = Engine(config=load_config(args.model), random_seed=args.weights_seed, **options)
     else:
         engine = Engine(args.model, **options)
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k,
-                            max_new_tokens=args.max_new_tokens, seed=args.seed, ignore_eos=args.ignore_eos)
+                            max_new_tokens=args.max_new_tokens, seed=args.seed, ignore_eos=args.ignore_eos,
+                            logprobs=args.logprobs)
     t0 = time.time()
     reqs = [engine.add_request(p, params) for p in prompts]
     while engine.has_work():
@@ -114,6 +121,8 @@ def main(argv=None) -> int:
     total = 0
     for i, r in enumerate(reqs):
         print(f"[{i}] ({r.finish_reason}) " + " ".join(map(str, r.output)))
+        for p in r.logprobs:
+            print(f"    {p.token} {p.logprob:.4f} entropy {p.entropy:.4f}" + "".join(f" {t}:{lp:.4f}" for t, lp in p.top))
         total += len(r.output)
     print(f"total tokens: {total}, time: {dt:.2f}s, speed: {total / max(dt, 1e-9):.2f} tokens/s", file=sys.stderr)
     if args.stats:

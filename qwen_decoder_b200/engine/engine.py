@@ -10,15 +10,17 @@ common.cpp:229-562, is outside it).
 """
 from __future__ import annotations
 
+import dataclasses
 from typing import Dict, Iterable, List, Optional, Sequence
 
 import torch
 
+from .. import kernels
 from ..cache import CacheManager
 from ..sampling import Sampler, uniform_draw
-from .batch import StepEntry
+from .batch import StepEntry, StepError
 from .runner import ModelRunner, resolve_dtype
-from .scheduler import Request, SamplingParams, Scheduler, StepPlan
+from .scheduler import Request, SamplingParams, Scheduler, StepPlan, TokenLogprob
 
 
 class Engine:
@@ -27,7 +29,8 @@ class Engine:
                  max_prefill_tokens_per_step: int = 512, max_total_tokens: int = 4096,
                  page_size: int = 16, num_pages: Optional[int] = None, kv_memory_fraction: float = 0.8,
                  max_positions: Optional[int] = None, use_graphs: bool = True,
-                 enable_prefix_cache: bool = False, run_ahead: bool = True, record_steps: bool = False):
+                 enable_prefix_cache: bool = False, run_ahead: bool = True, record_steps: bool = False,
+                 projection_dtype: Optional[str] = None, output_projection_dtype: Optional[str] = None):
         """``model``: a folder with config.json and model.safetensors; or give ``config`` (a typed
         configuration) and ``random_seed`` for random weights made on the device.
 
@@ -44,10 +47,13 @@ class Engine:
         step late.  The tokens are the same; a request that ends on a stop token costs one wasted row.
         ``record_steps``: keep one record per step (``step_records()``): tokens, how many of them prompt and
         decoded tokens, requests, device time by CUDA events, free pages, queue lengths -- what the reference
-        prints per step (decoder.cpp:178-185) and more; each step is also an NVTX range then."""
+        prints per step (decoder.cpp:178-185) and more; each step is also an NVTX range then.
+        ``projection_dtype``, ``output_projection_dtype``: "float8_e4m3" has the layers' products, and the one over the
+        vocabulary, in 8 bits where the configuration does not say so."""
         self.max_prefill_len = max_prefill_len
         make = dict(dtype=dtype, device=device, page_size=page_size, max_requests=max_batch,
-                    max_positions=max_positions, use_graphs=use_graphs, prefix_cache=enable_prefix_cache)
+                    max_positions=max_positions, use_graphs=use_graphs, prefix_cache=enable_prefix_cache,
+                    projections={"projection_dtype": projection_dtype, "output_projection_dtype": output_projection_dtype})
         sizing = _PageSizing(num_pages, kv_memory_fraction, page_size, resolve_dtype(dtype))
         if model is not None:
             self.runner = ModelRunner.from_folder(model, num_pages=sizing, **make)
@@ -76,6 +82,8 @@ class Engine:
     def add_request(self, prompt: Sequence[int], params: Optional[SamplingParams] = None,
                     request_id=None) -> Request:
         rid = self._next_id if request_id is None else request_id
+        if params is not None and params.logprobs is not None:
+            self._check_top(params.logprobs)
         self._next_id += 1
         req = Request(rid, [int(t) for t in prompt], params or SamplingParams())
         req.sample_key = self._next_id - 1
@@ -100,7 +108,7 @@ class Engine:
             self._end_record(rec)
             return flight
         ahead = 1 if device_tokens is not None else 0       # a step planned ahead samples one token later
-        _, ids = self.runner.step(entries, ensure_pages=False, device_tokens=device_tokens, sampling=(
+        logits, ids = self.runner.step(entries, ensure_pages=False, device_tokens=device_tokens, sampling=(
             [r.params.temperature for r in sampling], [r.params.top_k for r in sampling],
             [uniform_draw(r.params.seed, r.sample_key, len(r.output) + ahead) if r.params.temperature else 0.0
              for r in sampling]))
@@ -108,6 +116,9 @@ class Engine:
         self._turn ^= 1
         flight.host = self._host_tokens[self._turn][:len(sampling)]
         flight.host.copy_(ids, non_blocking=True)
+        wanted = [r.params.logprobs for r in sampling if r.params.logprobs is not None]
+        if wanted:
+            flight.logprobs = [t.to("cpu", non_blocking=True) for t in kernels.token_logprobs(logits, ids, max(wanted))]
         flight.event = torch.cuda.Event()
         flight.event.record()
         flight.device = ids
@@ -141,7 +152,13 @@ class Engine:
             for e, t in zip(cur.plan.entries, tokens):
                 if e.request.cache is not None:
                     self.runner.cache.log_tokens(e.request.cache, [t])
+        lengths = [len(e.request.output) for e in cur.plan.entries]
         finished += self.scheduler.update(cur.plan, tokens)
+        if cur.logprobs is not None:
+            sampled = [(e.request, n) for e, n in zip(cur.plan.entries, lengths) if e.samples]
+            for (r, n), entry in zip(sampled, _token_logprobs(tokens, *cur.logprobs)):
+                if r.params.logprobs is not None and len(r.output) > n:      # (a token that ends the request is no output)
+                    r.logprobs.append(dataclasses.replace(entry, top=entry.top[:r.params.logprobs]))
         if finished:
             self.runner.check_status()       # before results leave: no kernel's wait ran out on the way
         return finished
@@ -157,6 +174,37 @@ class Engine:
             self.step()
         self.runner.check_status()
         return [r.output for r in reqs]
+
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenLogprob]]:
+        """What the model gives to every prompt's tokens: of each but the first its log probability behind those before it, the
+        distribution's entropy and the ``top`` (0 to 32) most probable tokens.  Prompts run one after the other, in portions of
+        ``max_prefill_tokens_per_step``, on pages that the requests at work leave (``OutOfPages`` otherwise)."""
+        self._check_top(top)
+        out = []
+        for i, prompt in enumerate(prompts):
+            prompt = [int(t) for t in prompt]
+            found: List[TokenLogprob] = []
+            rc = self.runner.open(("score", i))
+            try:
+                step = self.scheduler.max_prefill_tokens_per_step
+                for at in range(0, len(prompt) - 1, step):         # (the last token is only looked up)
+                    portion, after = prompt[at:min(at + step, len(prompt) - 1)], prompt[at + 1:min(at + step, len(prompt) - 1) + 1]
+                    logits = self.runner.step([StepEntry(rc, portion, list(range(len(portion))))])
+                    tokens = torch.tensor(after, dtype=torch.int32).to(self.device, non_blocking=True)
+                    found += _token_logprobs(after, *(t.cpu() for t in kernels.token_logprobs(logits, tokens, top)))
+            finally:
+                self.runner.close(rc)
+            for t in prompt[-1:]:
+                if not 0 <= t < self.runner.model.vocab_size:
+                    raise StepError(f"token {t} is outside of the vocabulary")
+            out.append(found)
+        self.runner.check_status()
+        return out
+
+    def _check_top(self, top: int) -> None:
+        most = min(kernels.LOGPROBS_MAX_TOP, self.runner.model.vocab_size)
+        if not 0 <= top <= most:
+            raise ValueError(f"logprobs: between 0 and {most} most probable tokens, got {top}")
 
     # ---- per-step records ------------------------------------------------------
     def _begin_record(self, plan: StepPlan, ahead: bool) -> Optional[dict]:
@@ -196,6 +244,12 @@ class Engine:
         return dict(self.scheduler.stats, model_steps=self.runner.steps, model_tokens=self.runner.tokens_run)
 
 
+def _token_logprobs(tokens, logprob, entropy, ids, tops) -> List[TokenLogprob]:
+    """The results of ``kernels.token_logprobs``, on the host, as one record for each token."""
+    return [TokenLogprob(int(t), lp, h, tuple(zip(i, p)))
+            for t, lp, h, i, p in zip(tokens, logprob.tolist(), entropy.tolist(), ids.tolist(), tops.tolist())]
+
+
 class _InFlight:
     """A launched step: its plan, and where its sampled tokens arrive."""
 
@@ -206,6 +260,7 @@ class _InFlight:
         self.host: Optional[torch.Tensor] = None       # pinned; valid once ``event`` has passed
         self.event: Optional[torch.cuda.Event] = None
         self.device: Optional[torch.Tensor] = None     # the same tokens on the device
+        self.logprobs: Optional[list] = None           # of the tokens, where a request asks for them; valid with ``host``
 
 
 class _PageSizing:

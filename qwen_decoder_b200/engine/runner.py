@@ -9,6 +9,7 @@ one function.
 """
 from __future__ import annotations
 
+import dataclasses
 from typing import Optional, Sequence
 
 import torch
@@ -42,6 +43,17 @@ def require_cuda(device) -> torch.device:
     return device
 
 
+def with_projections(config, projections: Optional[dict]):
+    """``config`` with what ``projections`` gives of ``projection_dtype`` and ``output_projection_dtype`` (not None)."""
+    given = {k: v for k, v in (projections or {}).items() if v is not None}
+    for key, value in given.items():
+        if key not in ("projection_dtype", "output_projection_dtype") or value != "float8_e4m3":
+            raise ValueError(f"projections: 'projection_dtype' and 'output_projection_dtype' may be 'float8_e4m3', got {key!r}: {value!r}")
+        if not hasattr(config, key):
+            raise ValueError(f"projections in 8 bits: {type(config).__name__} has no {key!r}")
+    return dataclasses.replace(config, **given) if given else config
+
+
 class ModelRunner:
     """A bound model, its cache, and ``step``."""
 
@@ -73,19 +85,21 @@ class ModelRunner:
 
     # ---- construction ----------------------------------------------------
     @classmethod
-    def from_folder(cls, model_dir: str, dtype="bfloat16", device="cuda:0", **kw) -> "ModelRunner":
+    def from_folder(cls, model_dir: str, dtype="bfloat16", device="cuda:0", projections: Optional[dict] = None, **kw) -> "ModelRunner":
+        """``projections``: ``projection_dtype`` and ``output_projection_dtype`` in place of the configuration's."""
         device = require_cuda(device)
         dt = resolve_dtype(dtype)
-        config = load_config(model_dir)
+        config = with_projections(load_config(model_dir), projections)
         model = build_model(describe_model(config))
         load_into(model, TensorSource.from_folder(model_dir), dt, device)
         return cls(model, config, **kw)
 
     @classmethod
-    def from_random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", **kw) -> "ModelRunner":
+    def from_random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", projections: Optional[dict] = None, **kw) -> "ModelRunner":
         """Random weights made on the device (no folder); same distributions as ``write_random_model``."""
         device = require_cuda(device)
         dt = resolve_dtype(dtype)
+        config = with_projections(config, projections)
         model = build_model(describe_model(config))
         specs = {s.name: s for s in model.tensor_specs()}
         from ..weights.random_init import random_tensor

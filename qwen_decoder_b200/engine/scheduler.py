@@ -24,7 +24,7 @@ from __future__ import annotations
 
 from collections import deque
 from dataclasses import dataclass, field
-from typing import Deque, List, Optional, Sequence
+from typing import Deque, List, Optional, Sequence, Tuple
 
 from ..cache import CacheManager, OutOfPages, RequestCache
 
@@ -38,6 +38,17 @@ class SamplingParams:
     seed: int = 0
     stop_ids: Sequence[int] = ()
     ignore_eos: bool = False
+    # with every output token its log probability, the distribution's entropy and so many most probable tokens (0 to 32); None: none of it
+    logprobs: Optional[int] = None
+
+
+@dataclass(frozen=True)
+class TokenLogprob:
+    """What a model gave to a token, by its logits as they are (before temperature and top-k)."""
+    token: int
+    logprob: float
+    entropy: float
+    top: Tuple[Tuple[int, float], ...] = ()        # (token, log probability), the most probable first
 
 
 @dataclass
@@ -46,6 +57,7 @@ class Request:
     prompt: List[int]
     params: SamplingParams = field(default_factory=SamplingParams)
     output: List[int] = field(default_factory=list)
+    logprobs: List[TokenLogprob] = field(default_factory=list)     # of the output's tokens, if the parameters ask for them
     cache: Optional[RequestCache] = None
     num_computed: int = 0             # tokens of prompt + output whose cache entries exist
     finished: bool = False

@@ -948,11 +948,15 @@ class Fp8Rows(NamedTuple):
         return self.q.shape
 
 
+_E4M3, _E8M0, _F32, _BF16, _I32 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float32, torch.bfloat16, torch.int32
+_device_of = functools.lru_cache(maxsize=64)(torch.device)
+
+
 def fp8_rows(R: int, K: int, device) -> Fp8Rows:
     """Room for ``R`` rows of ``K`` features in 8 bits."""
-    kb = -(-K // FP8_BLOCK)
-    return Fp8Rows(torch.empty_strided((R, K), ((K + 15) & -16, 1), dtype=torch.float8_e4m3fn, device=device),
-                   torch.empty_strided((R, kb), ((kb + 3) & -4, 1), dtype=torch.float8_e8m0fnu, device=device))
+    kb, device = -(-K // FP8_BLOCK), _device_of(device)
+    return Fp8Rows(torch.empty_strided((R, K), ((K + 15) & -16, 1), dtype=_E4M3, device=device),
+                   torch.empty_strided((R, kb), ((kb + 3) & -4, 1), dtype=_E8M0, device=device))
 
 
 def _entry(name: str, function: str, kinds: str):
@@ -980,15 +984,19 @@ def _raw_ptr(t: Optional[torch.Tensor]):
 def _fp8_check(rows: Fp8Rows, name: str, R: Optional[int] = None, K: Optional[int] = None):
     """(R, K, address and distance of q's rows, of s's rows), or ``KernelError``."""
     q, s = rows
-    if q.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu or q.dim() != 2 or s.dim() != 2:
+    shape, s_shape = q.shape, s.shape
+    if q.dtype is not _E4M3 or s.dtype is not _E8M0 or len(shape) != 2 or len(s_shape) != 2:
         raise KernelError(f"{name}: rows in 8 bits are q float8_e4m3fn [R, K] and s float8_e8m0fnu [R, ceil(K / 128)]")
-    (r, k), at, (ldq, one), s_at, (lds, s_one) = q.shape, q.data_ptr(), q.stride(), s.data_ptr(), s.stride()
-    kb = -(-k // FP8_BLOCK)
-    if (R is not None and r != R) or (K is not None and k != K) or s.shape != (r, kb):
-        raise KernelError(f"{name}: q {tuple(q.shape)} and s {tuple(s.shape)} do not fit"
+    r, k = shape
+    kb = (k + FP8_BLOCK - 1) // FP8_BLOCK
+    if (R is not None and r != R) or (K is not None and k != K) or s_shape[0] != r or s_shape[1] != kb:
+        raise KernelError(f"{name}: q {tuple(shape)} and s {tuple(s_shape)} do not fit"
                           f" {'any' if R is None else R} rows of {'any' if K is None else K} features")
+    (ldq, one), (lds, s_one), at, s_at = q.stride(), s.stride(), q.data_ptr(), s.data_ptr()
+    if r == 1:                       # (one row is nowhere from the next)
+        ldq, lds = (k + 15) & -16, (kb + 3) & -4
     if r and k:
-        if one != 1 or ldq % 16 or ldq < k or at % 16:
+        if (one != 1 and k > 1) or ldq % 16 or ldq < k or at % 16:
             raise KernelError(f"{name}: rows of q must be contiguous, on 16 bytes and a multiple of 16 bytes apart")
         if (s_one != 1 and kb > 1) or lds % 4 or lds < kb or s_at % 4:
             raise KernelError(f"{name}: rows of s must be contiguous, on 4 bytes and a multiple of 4 bytes apart")
@@ -1004,12 +1012,12 @@ def _fp8_source(x: torch.Tensor, name: str, T: int, K: int):
     """(dtype code, distance of rows, number of parts, distance of parts) of a bfloat16 or float32 [T, K], or float32 parts [n, T, K]."""
     shape, stride, dt = x.shape, x.stride(), x.dtype
     parts = len(shape) == 3
-    if dt not in (torch.float32, torch.bfloat16) or (parts and (dt != torch.float32 or not shape[0])) \
-            or len(shape) not in (2, 3) or shape[-2:] != (T, K):
+    if not (dt is _F32 or dt is _BF16) or (parts and (dt is not _F32 or not shape[0])) \
+            or len(shape) not in (2, 3) or shape[-2] != T or shape[-1] != K:
         raise KernelError(f"{name}: bfloat16 or float32 [{T}, {K}], or float32 parts [n, {T}, {K}] expected, got {dt} {tuple(shape)}")
     if stride[-1] != 1 and K > 1:
         raise KernelError(f"{name}: rows must be contiguous")
-    return (F32 if dt == torch.float32 else BF16), stride[-2], (shape[0] if parts else 1), (stride[0] if parts else 0)
+    return (F32 if dt is _F32 else BF16), stride[-2], (shape[0] if parts else 1), (stride[0] if parts else 0)
 
 
 def _rows_fp8(x, code, ld, n, step, gated, act, bias, out, q, ldq, s, lds, T, K, what):
@@ -1052,10 +1060,11 @@ def add_rmsnorm_fp8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
     float32 [T, D] is updated to x + delta when ``write_back``.  delta: bfloat16 or float32 [T, D], or float32 partial sums [n, T, D];
     ``delta_scale`` float32 [D] or None multiplies it."""
     R, D, q, ldq, s, lds = _fp8_check(out, "add_rmsnorm_fp8: out")
-    if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != D or not x.is_contiguous():
+    shape = x.shape
+    if x.dtype is not _F32 or len(shape) != 2 or shape[1] != D or not x.is_contiguous():
         raise KernelError(f"add_rmsnorm_fp8: x must be contiguous float32 [T, {D}]")
-    T = x.shape[0]
-    if weight.dtype != torch.float32 or weight.numel() != D or not weight.is_contiguous():
+    T = shape[0]
+    if weight.dtype is not _F32 or weight.numel() != D or not weight.is_contiguous():
         raise KernelError(f"add_rmsnorm_fp8: weight must be contiguous float32 [{D}]")
     if delta_scale is not None and (delta_scale.dtype != torch.float32 or delta_scale.numel() != D or not delta_scale.is_contiguous()):
         raise KernelError(f"add_rmsnorm_fp8: delta_scale must be contiguous float32 [{D}]")
@@ -1099,12 +1108,13 @@ def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Te
     x_at = _fp8_check(x, "gemm_fp8: x")
     w_at = _fp8_check(w, "gemm_fp8: w", K=x_at[1])
     T, N, dt = x_at[0], w_at[0], out.dtype
-    if dt not in (torch.float32, torch.bfloat16) or out.shape != (T, N) or (out.stride(1) != 1 and N > 1):
+    shape, stride = out.shape, out.stride()
+    if not (dt is _F32 or dt is _BF16) or len(shape) != 2 or shape[0] != T or shape[1] != N or (stride[1] != 1 and N > 1):
         raise KernelError(f"gemm_fp8: out must be bfloat16 or float32 [{T}, {N}] with contiguous rows")
     _fp8_bias(bias, N, "gemm_fp8")
     _on_device(x)
     _on_device(w)
-    _gemm_fp8(x_at, w_at, bias, _raw_ptr(out), F32 if dt == torch.float32 else BF16, out.stride(0), None, 0, EPI_STORE, plan, "gemm_fp8")
+    _gemm_fp8(x_at, w_at, bias, _raw_ptr(out), F32 if dt is _F32 else BF16, stride[0], None, 0, EPI_STORE, plan, "gemm_fp8")
 
 
 def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None) -> None:

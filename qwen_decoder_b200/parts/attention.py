@@ -52,6 +52,7 @@ class GQAttention(Mixer):
         return self.qkv.tensor_specs() + self.out.tensor_specs()
 
     def bind(self, source: TensorSource, dtype: torch.dtype, device: torch.device) -> None:
+        self.dtype = dtype
         self.qkv.bind(source, dtype, device)
         self.out.bind(source, dtype, device)
 
@@ -66,37 +67,46 @@ class GQAttention(Mixer):
                 "pairing": pos.pairing_code if pos is not None else 0,
                 "wqkv": self.qkv.weight, "bqkv": self.qkv.bias, "wo": self.out.weight}
 
+    def _few_token_sums(self, x: torch.Tensor) -> Optional[torch.Tensor]:
+        """q, k and v of few tokens as float32 partial sums [n_parts, T, (H + 2G) d] without their bias, or None where the product
+        takes another way."""
+        if not matmul_backend.use_skinny(x, self.qkv.weight):
+            return None
+        matmul_backend.counters["own"] += 1
+        return kernels.gemm_skinny_partial(x, self.qkv.weight, kernels.skinny_splits(self.qkv.out_features, self.hidden_size, x.shape[0]))
+
+    def _out_product(self, attn: torch.Tensor) -> torch.Tensor:
+        return self.out.forward_partial(attn)
+
     def forward(self, x: torch.Tensor, ctx, cache: PagedCacheView) -> torch.Tensor:
         H, G, d = self.num_heads, self.num_kv_heads, self.head_dim
-        pos = self.position
+        pos, dtype = self.position, self.dtype
         rope = (pos.rotary_dim if pos is not None else 0, pos.pairing_code if pos is not None else 0,
                 pos.cos if pos is not None else None, pos.sin if pos is not None else None)
-        if matmul_backend.use_skinny(x, self.qkv.weight):
+        part = self._few_token_sums(x)
+        if part is not None:
             # few tokens: the product leaves float32 partial sums; bias, rotation and cache write take them
-            part = kernels.gemm_skinny_partial(x, self.qkv.weight,
-                                               kernels.skinny_splits(self.qkv.out_features, self.hidden_size, x.shape[0]))
-            matmul_backend.counters["own"] += 1
             ps, window = cache.group.page_size, self.window or 0
-            if ctx.all_decode and _DECODE_ROPE and kernels.decode_rope_supported(x.dtype, H, G, d, ps):
+            if ctx.all_decode and _DECODE_ROPE and kernels.decode_rope_supported(dtype, H, G, d, ps):
                 # ... and so does attention itself: one kernel from the partial sums to the attention output
-                attn = torch.empty((x.shape[0], H * d), dtype=x.dtype, device=x.device)
+                attn = torch.empty((x.shape[0], H * d), dtype=dtype, device=ctx.positions.device)
                 kernels.decode_attention_rope(
                     part, self.qkv.bias, attn, cache.kv, cache.group.block_table, ctx.token_request, ctx.positions,
                     cache.group.slot_map, H, G, d, ps, self.scale, window,
                     decode_rope_splits(ctx.num_tokens * G, min(ctx.max_context, window or ctx.max_context)),
                     cache.write, *rope)
-                return self.out.forward_partial(attn)
-            qkv = torch.empty((x.shape[0], H * d), dtype=x.dtype, device=x.device)       # q only
+                return self._out_product(attn)
+            qkv = torch.empty((x.shape[0], H * d), dtype=dtype, device=ctx.positions.device)       # q only
             kernels.rope_kv_write_partial(part, self.qkv.bias, qkv, H, G, d, *rope, ctx.positions, cache.kv,
                                           cache.group.slot_map, cache.group.page_size, cache.write)
         else:
             qkv = self.qkv.forward(x)
             kernels.rope_kv_write(qkv, H, G, d, *rope, ctx.positions, cache.kv, cache.group.slot_map,
                                   cache.group.page_size, cache.write)
-        shares = step_decode_shares(ctx, cache, H, G, d, self.window, x.dtype)
-        attn = torch.empty((x.shape[0], H * d), dtype=x.dtype, device=x.device)
+        shares = step_decode_shares(ctx, cache, H, G, d, self.window, dtype)
+        attn = torch.empty((x.shape[0], H * d), dtype=dtype, device=ctx.positions.device)
         ps, window = cache.group.page_size, self.window or 0
-        if ctx.all_decode and kernels.flash_decode_supported(x.dtype, H, G, d, ps):
+        if ctx.all_decode and kernels.flash_decode_supported(dtype, H, G, d, ps):
             if shares is not None:
                 kernels.decode_attention_shares(qkv, qkv.stride(0), attn, cache.kv, cache.group.block_table, ctx.num_tokens, H, G, d,
                                                 ps, self.scale, *shares)
@@ -105,12 +115,12 @@ class GQAttention(Mixer):
                     qkv, qkv.stride(0), attn, cache.kv, cache.group.block_table, ctx.token_request,
                     ctx.positions, ctx.num_tokens, H, G, d, ps, self.scale, window,
                     decode_splits(ctx.num_tokens * G, min(ctx.max_context, window or ctx.max_context), kernels.decode_ctas(d)))
-        elif kernels.flash_prefill_supported(x.dtype, H, G, d, ps) or \
-                (_PREFILL_TC5 and kernels.prefill_tc5_supported(x.dtype, H, G, d, ps)):
+        elif kernels.flash_prefill_supported(dtype, H, G, d, ps) or \
+                (_PREFILL_TC5 and kernels.prefill_tc5_supported(dtype, H, G, d, ps)):
             # a mixed step: its single tokens (first in the batch) go to the decode kernel, which shares
             # a request's keys among CTAs; a prompt kernel would walk them with one CTA per request
             nd = getattr(ctx, "num_decode", 0)
-            if nd and not kernels.flash_decode_supported(x.dtype, H, G, d, ps):
+            if nd and not kernels.flash_decode_supported(dtype, H, G, d, ps):
                 nd = 0
             if nd and shares is not None:
                 kernels.decode_attention_shares(qkv, qkv.stride(0), attn[:nd], cache.kv, cache.group.block_table, nd, H, G, d, ps,
@@ -121,10 +131,10 @@ class GQAttention(Mixer):
                     ctx.positions[:nd], nd, H, G, d, ps, self.scale, window,
                     decode_splits(nd * G, min(ctx.decode_max_context, window or ctx.decode_max_context), kernels.decode_ctas(d)))
             fn = kernels.prefill_attention_tc5 \
-                if _PREFILL_TC5 and kernels.prefill_tc5_supported(x.dtype, H, G, d, ps) else kernels.prefill_attention
+                if _PREFILL_TC5 and kernels.prefill_tc5_supported(dtype, H, G, d, ps) else kernels.prefill_attention
             fn(qkv, qkv.stride(0), attn, cache.kv, cache.group.block_table[nd:], ctx.cu_tokens[nd:],
                ctx.start_pos[nd:], ctx.num_requests - nd, ctx.num_tokens - nd, H, G, d, ps, self.scale, window)
-        elif kernels.attention_f32_supported(x.dtype, H, G, d):
+        elif kernels.attention_f32_supported(dtype, H, G, d):
             kernels.attention_f32(
                 qkv, qkv.stride(0), attn, cache.kv, cache.group.block_table, ctx.token_request, ctx.positions,
                 ctx.num_tokens, H, G, d, ps, self.scale, window,
@@ -133,7 +143,7 @@ class GQAttention(Mixer):
             kernels.paged_attention_generic(
                 qkv, qkv.stride(0), attn, cache.kv, cache.group.block_table, ctx.token_request,
                 ctx.positions, ctx.num_tokens, H, G, d, ps, self.scale, window)
-        return self.out.forward_partial(attn)
+        return self._out_product(attn)
 
 
 import os as _os

@@ -24,7 +24,7 @@ from .linear import Linear
 from . import attention as _attention, block as _block, mlp as _mlp, norm as _norm, rotary as _rotary  # noqa: F401
 from . import latent_attention as _latent, mamba2 as _mamba2, moe as _moe, sink_attention as _sink  # noqa: F401
 from . import diff_attention as _diff, masked_attention as _masked, side_by_side as _side, time_mix as _tmix  # noqa: F401
-from . import linear_attention as _linear_attention  # noqa: F401
+from . import linear_attention as _linear_attention, fp8 as _fp8  # noqa: F401
 
 
 class DecoderModel:
@@ -66,12 +66,13 @@ class DecoderModel:
         fn["prefix"] = spec.final_norm_prefix + fn.get("prefix", "")
         self.final_norm = create_part("norm", spec.final_norm.name, **fn)
         head = spec.lm_head_tensor
+        linear = _fp8.Fp8Linear if spec.lm_head_in_8_bits else Linear
         if head is None:
-            self.lm_head = Linear(spec.hidden_size, [("lm_head", spec.vocab_size)], bias=False)
+            self.lm_head = linear(spec.hidden_size, [("lm_head", spec.vocab_size)], bias=False)
         elif head.endswith(".weight"):
-            self.lm_head = Linear(spec.hidden_size, [(head[:-len(".weight")], spec.vocab_size)], bias=False)
+            self.lm_head = linear(spec.hidden_size, [(head[:-len(".weight")], spec.vocab_size)], bias=False)
         else:           # a model that names its output matrix without the suffix
-            self.lm_head = Linear(spec.hidden_size, [(head, spec.vocab_size)], bias=False, weight_suffix="")
+            self.lm_head = linear(spec.hidden_size, [(head, spec.vocab_size)], bias=False, weight_suffix="")
         self.embedding_scale = float(spec.embedding_scale)
         self.logit_softcap = spec.logit_softcap
         self.embedding: Optional[torch.Tensor] = None

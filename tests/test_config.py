@@ -74,3 +74,20 @@ def test_model_description_follows_the_configuration():
     assert spec.positions["rope"].params["base"] == 1e6
     assert spec.lm_head_tensor == "lm_head.weight"
     assert describe_model(Qwen2Config.from_dict(TINY_A)).lm_head_tensor is None
+
+
+def test_projection_dtypes():
+    """The keys that have products in 8 bits: kept, checked, and described as the parts that take them."""
+    from qwen_decoder_b200.config import ConfigError, Qwen2Config, describe_model
+    from tiny_configs import TINY
+    plain = Qwen2Config.from_dict(TINY["A"])
+    assert plain.projection_dtype is None and "projection_dtype" not in plain.to_dict()
+    cfg = Qwen2Config.from_dict(dict(TINY["A"], projection_dtype="float8_e4m3"))
+    assert Qwen2Config.from_dict(cfg.to_dict()) == cfg
+    spec = describe_model(cfg)
+    assert spec.layers[0].mixer.name == "gq_attention_fp8" and spec.layers[0].feed_forward.name == "swiglu_fp8"
+    assert spec.layers[0].norms["input"].name == "rmsnorm_fp8" and spec.final_norm.name == "rmsnorm" and not spec.lm_head_in_8_bits
+    spec = describe_model(Qwen2Config.from_dict(dict(TINY["A"], output_projection_dtype="float8_e4m3")))
+    assert spec.layers[0].mixer.name == "gq_attention" and spec.final_norm.name == "rmsnorm_fp8" and spec.lm_head_in_8_bits
+    with pytest.raises(ConfigError, match="projection_dtype"):
+        Qwen2Config.from_dict(dict(TINY["A"], projection_dtype="int4"))
