@@ -38,6 +38,7 @@ LIBRARIES: Dict[str, str] = {
     "gemm_tc5": "gemm_tc5.cu",
     "gemm_pair": "gemm_pair.cu",
     "gemm_fp8": "gemm_fp8.cu",
+    "gemm_fp8_few": "gemm_fp8_few.cu",
     "rows_fp8": "rows_fp8.cu",
     "logprobs": "logprobs.cu",
     "attention_generic": "attention_generic.cu",
@@ -67,6 +68,7 @@ EXTRA_DEPS: Dict[str, List[str]] = {
     "gemm_f32": ["tc5_ops.cuh"],
     "gemm_pair": ["tc5_ops.cuh"],
     "gemm_fp8": ["tc5_ops.cuh", "fp8.cuh"],
+    "gemm_fp8_few": ["fp8.cuh"],
     "rows_fp8": ["fp8.cuh"],
     "gated_block": ["short_conv.cuh"],
     "attention_diff": ["short_conv.cuh", "mma_sync.cuh"],

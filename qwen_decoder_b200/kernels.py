@@ -1091,12 +1091,26 @@ def gemm_fp8_plan(T: int, N: int, K: int, epi: int, out_code: int, sms: int):
     return tuple(n.value for n in v)
 
 
+FP8_FEW = (0, 0, 0)      # as a plan: the kernel of few tokens
+FP8_FEW_TOKENS = 16      # what it takes
+
+
+def gemm_fp8_few_wanted(T: int, N: int, K: int) -> bool:
+    """Whether ``csrc/gemm_fp8_few.cu`` is the faster one: up to 8 tokens and 20 MB of weights, up to 16 and 10 MB (times beside its
+    kernel)."""
+    return T <= 8 and N * K <= 20_000_000 or T <= FP8_FEW_TOKENS and N * K <= 10_000_000
+
+
 def _gemm_fp8(x_at, w_at, bias, out, code, ldo, s_out, lds_out, epi, plan, what):
     T, K, x, ldx, sx, ldsx = x_at
     N, _, w, ldw, sw, ldsw = w_at
     if T == 0 or N == 0:
         return
     sms = sm_count()
+    if epi == EPI_STORE and (plan == FP8_FEW or plan is None and gemm_fp8_few_wanted(T, N, K)):
+        _check(_entry("gemm_fp8_few", "qd_gemm_fp8_few", "plplplplppiliiiip")(
+            w, ldw, sw, ldsw, x, ldx, sx, ldsx, _raw_ptr(bias), out, code, ldo, T, N, K, sms, _stream()), what)
+        return
     cg, bn, splits = plan or gemm_fp8_plan(T, N, K, epi, code, sms)
     _check(_entry("gemm_fp8", "qd_gemm_fp8", "plplplplppilpliiiiiiiip")(
         w, ldw, sw, ldsw, x, ldx, sx, ldsx, _raw_ptr(bias), out, code, ldo, s_out, lds_out, T, N, K, cg, bn, splits, epi, sms, _stream()), what)
@@ -1104,7 +1118,7 @@ def _gemm_fp8(x_at, w_at, bias, out, code, ldo, s_out, lds_out, epi, plan, what)
 
 def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Tensor, plan=None) -> None:
     """out[T, N] = x @ w^T (+ bias float32 [N]) of rows in 8 bits on the tensor cores, float32 sums; out bfloat16 or float32, rows may
-    lie apart.  ``plan``: as ``gemm_fp8_plan`` gives it."""
+    lie apart.  ``plan``: as ``gemm_fp8_plan`` gives it, or ``FP8_FEW`` (up to 16 tokens); None: the faster one."""
     x_at = _fp8_check(x, "gemm_fp8: x")
     w_at = _fp8_check(w, "gemm_fp8: w", K=x_at[1])
     T, N, dt = x_at[0], w_at[0], out.dtype

@@ -193,7 +193,7 @@ def operands(T, N, K):
     return rows_of(numbers((T, K), g, spread=6)), rows_of(numbers((N, K), g, spread=6) * K ** -0.5), numbers((N,), g)
 
 
-PRODUCTS = [(1, 1, 1), (1, 64, 128), (5, 200, 1000), (17, 33, 129), (127, 130, 512), (128, 2049, 640), (129, 96, 2056), (257, 264, 1024),
+PRODUCTS = [(1, 1, 1), (1, 64, 128), (5, 200, 1000), (8, 97, 5000), (9, 530, 1601), (16, 40, 4500), (17, 33, 129), (127, 130, 512), (128, 2049, 640), (129, 96, 2056), (257, 264, 1024),
             (300, 1000, 1500), (700, 514, 300)]
 
 
@@ -203,7 +203,7 @@ def test_product(T, N, K, dtype):
     from qwen_decoder_b200 import kernels
     x, w, bias = operands(T, N, K)
     want, off = value(x) @ value(w).T, sums_off(x, w)
-    plans = {None}
+    plans = {None} | ({kernels.FP8_FEW} if T <= kernels.FP8_FEW_TOKENS else set())
     for cg in (1, 2):
         for bn in (32, 48, 64, 96, 128, 192, 208, 224, 240, 256):
             for splits in (1, 2, 3, 8):
@@ -241,6 +241,28 @@ def test_gated_product(T, F, K, bias, act):
     kernels.check_status()
 
 
+def test_few_tokens_and_several_tiles_to_a_cta():
+    from qwen_decoder_b200 import kernels
+    for T in (1, 8, 13):
+        x, w, bias = operands(T, 12345, 700)
+        out = torch.empty(T, 12345, device=DEV)
+        kernels.gemm_fp8(x, w, bias, out, kernels.FP8_FEW)
+        want = value(x) @ value(w).T + bias.double()
+        assert ((out.double() - want).abs() <= 2.0 ** -23 * want.abs() + sums_off(x, w)).all()
+
+
+def test_rows_behind_the_end_are_not_taken():
+    """Numbers that end within 16 bytes, and rows of a larger matrix: what lies behind them, here no numbers, is in no sum."""
+    from qwen_decoder_b200 import kernels
+    x, w, _ = operands(7, 40, 389)
+    wide = lambda r: kernels.Fp8Rows(torch.nn.functional.pad(r.q.view(torch.uint8), (0, 400 - 389), value=0x7f)[:, :389].view(torch.float8_e4m3fn), r.s)  # noqa: E731
+    want = value(x) @ value(w).T
+    for plan in (kernels.FP8_FEW, (1, 64, 1), (1, 32, 2)):
+        out = torch.empty(7, 40, device=DEV)
+        kernels.gemm_fp8(wide(x), wide(w), None, out, plan)
+        assert ((out.double() - want).abs() <= 2.0 ** -23 * want.abs() + sums_off(x, w)).all(), plan
+
+
 def test_products_of_several_tiles_to_a_worker():
     """More tiles than multiprocessors: accumulators in turn, with whole and with overlapping columns, in both forms."""
     from qwen_decoder_b200 import kernels
@@ -262,25 +284,27 @@ def test_products_of_several_tiles_to_a_worker():
     kernels.check_status()
 
 
-def test_a_block_of_no_numbers_reaches_its_rows_sums_alone():
+@pytest.mark.parametrize("plan", [None, (0, 0, 0), (1, 64, 1), (1, 96, 3)])
+def test_a_block_of_no_numbers_reaches_its_rows_sums_alone(plan):
     from qwen_decoder_b200 import kernels
     x, w, _ = operands(5, 70, 384)
     x.s.view(torch.uint8)[2, 1] = 255
     w.s.view(torch.uint8)[64, 0] = 255
     out = torch.empty(5, 70, device=DEV)
-    kernels.gemm_fp8(x, w, None, out)
+    kernels.gemm_fp8(x, w, None, out, plan)
     none = torch.zeros(5, 70, dtype=torch.bool, device=DEV)
     none[2], none[:, 64] = True, True
     assert torch.equal(out.isnan(), none)
 
 
-def test_rows_apart_and_scales_apart():
+@pytest.mark.parametrize("plan", [(0, 0, 0), (1, 64, 1), (1, 96, 3)])
+def test_rows_apart_and_scales_apart(plan):
     from qwen_decoder_b200 import kernels
     x, w, _ = operands(9, 100, 384)
     apart = lambda t, n: torch.cat([t.view(torch.uint8), torch.full((t.shape[0], n), 0x7f, dtype=torch.uint8, device=DEV)], 1)[:, :t.shape[1]].view(t.dtype)  # noqa: E731
     a, b = torch.empty(9, 100, device=DEV), torch.empty(9, 100, device=DEV)
-    kernels.gemm_fp8(x, w, None, a)
-    kernels.gemm_fp8(kernels.Fp8Rows(apart(x.q, 16), apart(x.s, 5)), kernels.Fp8Rows(apart(w.q, 48), apart(w.s, 1)), None, b)
+    kernels.gemm_fp8(x, w, None, a, plan)
+    kernels.gemm_fp8(kernels.Fp8Rows(apart(x.q, 16), apart(x.s, 5)), kernels.Fp8Rows(apart(w.q, 48), apart(w.s, 1)), None, b, plan)
     assert torch.equal(a, b)
 
 

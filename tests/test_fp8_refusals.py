@@ -61,6 +61,11 @@ def test_products():
         kernels.gemm_fp8(x, w, None, torch.empty(3, 8), (1, 64, 1))
 
 
+def test_which_kernel_takes_few_tokens():
+    wanted = kernels.gemm_fp8_few_wanted
+    assert wanted(1, 2048, 2048) and wanted(8, 4608, 3584) and not wanted(8, 2048, 11008) and wanted(16, 2560, 2048) and not wanted(17, 64, 128)
+
+
 def test_sources():
     out = rows(3, 256)
     for x in (torch.zeros(3, 255), torch.zeros(3, 256, dtype=torch.float16), torch.zeros(2, 3, 256, dtype=torch.bfloat16), torch.zeros(256, 3).t(),
