@@ -1,7 +1,8 @@
 """Compiling and loading the CUDA libraries.
 
 Each ``.cu`` file under ``csrc/`` becomes one shared library of ``extern "C"``
-launchers, compiled for sm_100a with nvcc and loaded with ctypes.  A library is
+launchers, compiled for sm_100a with nvcc and loaded with ctypes; a ``.cpp`` file becomes a Python module
+(``extension``), compiled with g++ against torch's headers.  A library is
 built the first time an operation needs it (so a run compiles what its model and
 dtype use, nothing else) and kept under ``csrc/_build/`` (or, if the package
 folder is read-only, a per-user folder under the temporary directory), keyed by a
@@ -12,10 +13,12 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 import threading
 import time
@@ -41,6 +44,7 @@ LIBRARIES: Dict[str, str] = {
     "gemm_fp8_few": "gemm_fp8_few.cu",
     "rows_fp8": "rows_fp8.cu",
     "logprobs": "logprobs.cu",
+    "host_calls": "host_calls.cpp",
     "attention_generic": "attention_generic.cu",
     "attention_f32": "attention_f32.cu",
     "attention_flash": "attention_flash.cu",
@@ -78,6 +82,7 @@ EXTRA_DEPS: Dict[str, List[str]] = {
 }
 
 _loaded: Dict[str, ctypes.CDLL] = {}
+_extensions: Dict[str, object] = {}
 _lock = threading.Lock()
 _dir_lock = threading.Lock()
 
@@ -131,8 +136,26 @@ def _build_dir() -> str:
         return d
 
 
+def _torch_folder() -> str:
+    return list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+
+
+def _extension_command(src: str, out: str) -> List[str]:
+    """The Python module ``qd_<name>`` of a ``.cpp`` file, against the interpreter's and torch's headers and libraries."""
+    torch_dir, lib = _torch_folder(), os.path.join(_torch_folder(), "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(find_nvcc())), "include")
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(torch_dir, "include"), "-I", cuda, "-o", out, src, "-L", lib,
+            f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
 def _key(name: str, nvcc: str) -> str:
     h = hashlib.sha256()
+    if LIBRARIES[name].endswith(".cpp"):
+        with open(os.path.join(CSRC, LIBRARIES[name]), "rb") as fh, open(os.path.join(_torch_folder(), "version.py"), "rb") as version:
+            h.update(fh.read() + b"\0" + version.read() + sys.version.encode())
+        h.update(" ".join(_extension_command("", "")).encode())
+        return h.hexdigest()[:16]
     for f in [LIBRARIES[name]] + HEADERS + EXTRA_DEPS.get(name, []):
         with open(os.path.join(CSRC, f), "rb") as fh:
             h.update(f.encode() + b"\0" + fh.read() + b"\0")
@@ -156,9 +179,10 @@ def build_library(name: str, verbose: bool = True, extra_flags=()) -> str:
         return path
     src = os.path.join(CSRC, LIBRARIES[name])
     tmp = f"{path}.tmp{os.getpid()}"
-    cmd = [nvcc] + NVCC_FLAGS + list(extra_flags) + ["-I", CSRC, "-o", tmp, src]
+    host = src.endswith(".cpp")
+    cmd = _extension_command(src, tmp) if host else [nvcc] + NVCC_FLAGS + list(extra_flags) + ["-I", CSRC, "-o", tmp, src]
     if verbose:
-        _log(f"compiling {LIBRARIES[name]} for sm_100a (first use) ...")
+        _log(f"compiling {LIBRARIES[name]} {'with g++' if host else 'for sm_100a'} (first use) ...")
     t0 = time.time()
     proc = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     out_chunks: List[str] = []
@@ -178,7 +202,7 @@ def build_library(name: str, verbose: bool = True, extra_flags=()) -> str:
             os.unlink(tmp)
         except OSError:
             pass
-        raise BuildError(f"nvcc failed on {LIBRARIES[name]} (exit {proc.returncode}):\n{out}")
+        raise BuildError(f"{cmd[0]} failed on {LIBRARIES[name]} (exit {proc.returncode}):\n{out}")
     os.replace(tmp, path)
     # builds of older sources of this library are of no use any more (a process that still has one mapped keeps it)
     prefix = f"libqd_{name}-"
@@ -205,6 +229,22 @@ def library(name: str) -> ctypes.CDLL:
                 raise BuildError(f"cannot load {path}: {e}") from None
             _loaded[name] = lib
         return lib
+
+
+def extension(name: str):
+    """The Python module of the library ``name`` (a ``.cpp`` file; built first if needed)."""
+    with _lock:
+        mod = _extensions.get(name)
+        if mod is None:
+            path = build_library(name)
+            spec = importlib.util.spec_from_file_location(f"qd_{name}", path)
+            try:
+                mod = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+            except ImportError as e:
+                raise BuildError(f"cannot load {path}: {e}") from None
+            _extensions[name] = mod
+        return mod
 
 
 def build_all(verbose: bool = True, jobs: int = 0) -> Dict[str, str]:

@@ -129,6 +129,11 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   const int tiles = (a.V + LP_TILE - 1) / LP_TILE;
   const int lo = (int)((long long)tiles * share / a.shares), hi = (int)((long long)tiles * (share + 1) / a.shares);
   LpSum sum = {LP_LOWEST, 0.f, 0.f};
+  // (one thread asks for the token, and behind the first tile for its logit: at the end both would be waited for, 2 us)
+  const bool writes = share == 0 && threadIdx.x == 0;
+  int token = -1;
+  float its = __uint_as_float(0x7fc00000u);
+  if (writes) token = __ldg(a.tokens + row);
   for (int tile = lo; tile < hi; tile++) {
     float v[LP_EACH];
     lp_load(v, z, tile * LP_TILE + warp * LP_CHUNK, a.V, a.vec);
@@ -146,6 +151,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
       const unsigned peak = __reduce_max_sync(0xffffffffu, lp_order(m));
       if (lane == 0) sh.peaks[(tile - lo) * LP_WARPS + warp] = peak;
     }
+    if (writes && tile == lo && token >= 0 && token < a.V) its = to_float(z[token]);
   }
   // ---- the CTA's sums and its list
   const float m = lp_value(__reduce_max_sync(0xffffffffu, lp_order(sum.m)));
@@ -330,8 +336,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   // (a row of minus infinities alone has no probabilities: none is above 0)
   auto log_p = [&](float x) { return whole.s == 0.f ? -INFINITY : x - whole.m - log_s; };
   if (threadIdx.x == 0) {
-    const int t = a.tokens[row];
-    a.logprob[row] = t >= 0 && t < a.V ? log_p(to_float(z[t])) : __uint_as_float(0x7fc00000u);
+    a.logprob[row] = token >= 0 && token < a.V ? log_p(its) : its;
     a.entropy[row] = whole.s == 0.f ? 0.f : log_s - LP_LN2 * (whole.d / whole.s);
   }
   if ((int)threadIdx.x < a.top) {
@@ -345,9 +350,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
 // logits [R, V] float32 or bfloat16, rows ``ld`` elements apart; tokens int32 [R] (outside of [0, V): the log probability NaN); logprob and
 // entropy float32 [R]; top_ids int32 and top_logprobs float32 [R, top], top up to 32, of rows with fewer numbers -1 and NaN.
 extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob, float* entropy,
-                                 int* top_ids, float* top_logprobs, int R, int V, int top, int sms, int shares, cudaStream_t stream) {
+                                 int* top_ids, float* top_logprobs, int R, int V, int top, int sms, cudaStream_t stream) {
   if (R <= 0) return 0;
-  if ((dtype != QD_F32 && dtype != QD_BF16) || V <= 0 || V > LP_MAX_VOCABULARY || top < 0 || top > LP_MAX_TOP || top > V || sms < 1 || shares > LP_MAX_SHARES)
+  if ((dtype != QD_F32 && dtype != QD_BF16) || V <= 0 || V > LP_MAX_VOCABULARY || top < 0 || top > LP_MAX_TOP || top > V || sms < 1)
     return QD_ERR_UNSUPPORTED;
   LpArgs a;
   a.logits = logits; a.tokens = tokens; a.logprob = logprob; a.entropy = entropy; a.top_ids = top_ids; a.top_logprobs = top_logprobs;
@@ -357,8 +362,8 @@ extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, co
   // As many CTAs to a row as run at a time, four to a multiprocessor, with four tiles and half again as many chunks as ``top`` to each.
   // Measured, us: 64 rows of 152,064 with 4, 8 and 16 17.3, 14.3 and 27.6, 148 rows of 32,000 with 1, 2 and 4 11.2, 10.9 and 16.0.
   const int tiles = (V + LP_TILE - 1) / LP_TILE;
-  a.shares = shares > 0 ? shares : 1;
-  while (shares <= 0 && a.shares < LP_MAX_SHARES && (long long)R * a.shares * 2 <= 4ll * sms && tiles / (a.shares * 2) >= 4 &&
+  a.shares = 1;
+  while (a.shares < LP_MAX_SHARES && (long long)R * a.shares * 2 <= 4ll * sms && tiles / (a.shares * 2) >= 4 &&
          2 * (tiles / (a.shares * 2)) * LP_WARPS >= 3 * top)
     a.shares *= 2;
   while (a.shares * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE < V) a.shares++;      // a CTA keeps so many maxima

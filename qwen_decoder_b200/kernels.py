@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .csrc.build import library, loaded as _library_loaded
+from .csrc.build import extension, library, loaded as _library_loaded
 
 F32, BF16 = 0, 1
 ERR_UNSUPPORTED = 10001
@@ -844,7 +844,6 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
 
 
 LOGPROBS_MAX_TOP, LOGPROBS_MAX_VOCABULARY = 32, 1 << 22
-LOGPROBS_SHARES = 0
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
@@ -853,23 +852,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     lowest index first; their log probabilities), float32.  Logits of minus infinity have probability 0; a row of nothing else gives
     minus infinity, entropy 0.  A row with a NaN or an infinity has none: NaN, and its ids are of the numbers there are (-1: none).  A
     token outside of the row gives NaN."""
-    dt = logits.dtype
-    if logits.dim() != 2 or dt not in (torch.float32, torch.bfloat16) or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise KernelError("token_logprobs: logits must be float32 or bfloat16 [R, V] with contiguous rows")
-    R, V = logits.shape
-    if tokens.dtype != torch.int32 or tokens.shape != (R,) or not tokens.is_contiguous():
-        raise KernelError(f"token_logprobs: tokens must be contiguous int32 [{R}]")
-    if V > LOGPROBS_MAX_VOCABULARY:
-        raise KernelError(f"token_logprobs: rows of at most {LOGPROBS_MAX_VOCABULARY} logits, got {V}")
-    if V < 1 or not 0 <= top <= min(LOGPROBS_MAX_TOP, V):
-        raise KernelError(f"token_logprobs: top must be between 0 and {min(LOGPROBS_MAX_TOP, V)}, got {top}")
-    new = lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=logits.device)      # noqa: E731
-    lp, entropy = new((R,), (1,), torch.float32), new((R,), (1,), torch.float32)
-    ids, lps = new((R, top), (top, 1), torch.int32), new((R, top), (top, 1), torch.float32)
-    _check(_entry("logprobs", "qd_token_logprobs", "pilpppppiiiiip")(
-        _raw_ptr(logits), F32 if dt == torch.float32 else BF16, logits.stride(0), _raw_ptr(tokens), lp.data_ptr(), entropy.data_ptr(),
-        ids.data_ptr(), lps.data_ptr(), R, V, top, sm_count(), LOGPROBS_SHARES, _stream()), "token_logprobs")
-    return lp, entropy, ids, lps
+    _launch_count[0] += 1
+    return (_host or _host_calls()).token_logprobs(logits, tokens, top)
 
 
 def prefill_tc5_supported(dtype, H: int, G: int, d: int, page_size: int) -> bool:
@@ -948,110 +932,44 @@ class Fp8Rows(NamedTuple):
         return self.q.shape
 
 
-_E4M3, _E8M0, _F32, _BF16, _I32 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float32, torch.bfloat16, torch.int32
+_host = None            # the module of csrc/host_calls.cpp, which checks the arguments of what follows and launches it
 _device_of = functools.lru_cache(maxsize=64)(torch.device)
+
+
+def _host_calls():
+    global _host
+    if _host is None:
+        mod = extension("host_calls")
+        mod.start(KernelError, _resolve, Fp8Rows)
+        _host = mod
+    return _host
+
+
+def _resolve(name: str, function: str) -> int:
+    """For ``csrc/host_calls.cpp``: a launcher's address, or the multiprocessors of device ``function`` ("sms")."""
+    if name == "sms":
+        return torch.cuda.get_device_properties(int(function)).multi_processor_count
+    return ctypes.cast(getattr(library(name), function), ctypes.c_void_p).value
 
 
 def fp8_rows(R: int, K: int, device) -> Fp8Rows:
     """Room for ``R`` rows of ``K`` features in 8 bits."""
-    kb, device = -(-K // FP8_BLOCK), _device_of(device)
-    return Fp8Rows(torch.empty_strided((R, K), ((K + 15) & -16, 1), dtype=_E4M3, device=device),
-                   torch.empty_strided((R, kb), ((kb + 3) & -4, 1), dtype=_E8M0, device=device))
-
-
-def _entry(name: str, function: str, kinds: str):
-    """A library's function with its arguments' types (i int, l long long, f float, p pointer), looked up once: arguments then go as they
-    are, which for some twenty of them is 4 us less a call."""
-    fn = _entries.get(function)
-    if fn is None:
-        fn = getattr(library(name), function)
-        fn.argtypes = [{"i": _I, "l": _LL, "f": _F, "p": ctypes.c_void_p}[k] for k in kinds]
-        _entries[function] = fn
-    return fn
-
-
-_entries = {}
-
-
-def _raw_ptr(t: Optional[torch.Tensor]):
-    if t is None:
-        return None
-    if not t.is_cuda:
-        raise KernelError("kernel argument is not on a CUDA device (there is no CPU path)")
-    return t.data_ptr()
-
-
-def _fp8_check(rows: Fp8Rows, name: str, R: Optional[int] = None, K: Optional[int] = None):
-    """(R, K, address and distance of q's rows, of s's rows), or ``KernelError``."""
-    q, s = rows
-    shape, s_shape = q.shape, s.shape
-    if q.dtype is not _E4M3 or s.dtype is not _E8M0 or len(shape) != 2 or len(s_shape) != 2:
-        raise KernelError(f"{name}: rows in 8 bits are q float8_e4m3fn [R, K] and s float8_e8m0fnu [R, ceil(K / 128)]")
-    r, k = shape
-    kb = (k + FP8_BLOCK - 1) // FP8_BLOCK
-    if (R is not None and r != R) or (K is not None and k != K) or s_shape[0] != r or s_shape[1] != kb:
-        raise KernelError(f"{name}: q {tuple(shape)} and s {tuple(s_shape)} do not fit"
-                          f" {'any' if R is None else R} rows of {'any' if K is None else K} features")
-    (ldq, one), (lds, s_one), at, s_at = q.stride(), s.stride(), q.data_ptr(), s.data_ptr()
-    if r == 1:                       # (one row is nowhere from the next)
-        ldq, lds = (k + 15) & -16, (kb + 3) & -4
-    if r and k:
-        if (one != 1 and k > 1) or ldq % 16 or ldq < k or at % 16:
-            raise KernelError(f"{name}: rows of q must be contiguous, on 16 bytes and a multiple of 16 bytes apart")
-        if (s_one != 1 and kb > 1) or lds % 4 or lds < kb or s_at % 4:
-            raise KernelError(f"{name}: rows of s must be contiguous, on 4 bytes and a multiple of 4 bytes apart")
-    return r, k, at, ldq, s_at, lds
-
-
-def _on_device(rows: Fp8Rows) -> None:
-    if not (rows.q.is_cuda and rows.s.is_cuda):
-        raise KernelError("kernel argument is not on a CUDA device (there is no CPU path)")
-
-
-def _fp8_source(x: torch.Tensor, name: str, T: int, K: int):
-    """(dtype code, distance of rows, number of parts, distance of parts) of a bfloat16 or float32 [T, K], or float32 parts [n, T, K]."""
-    shape, stride, dt = x.shape, x.stride(), x.dtype
-    parts = len(shape) == 3
-    if not (dt is _F32 or dt is _BF16) or (parts and (dt is not _F32 or not shape[0])) \
-            or len(shape) not in (2, 3) or shape[-2] != T or shape[-1] != K:
-        raise KernelError(f"{name}: bfloat16 or float32 [{T}, {K}], or float32 parts [n, {T}, {K}] expected, got {dt} {tuple(shape)}")
-    if stride[-1] != 1 and K > 1:
-        raise KernelError(f"{name}: rows must be contiguous")
-    return (F32 if dt is _F32 else BF16), stride[-2], (shape[0] if parts else 1), (stride[0] if parts else 0)
-
-
-def _rows_fp8(x, code, ld, n, step, gated, act, bias, out, q, ldq, s, lds, T, K, what):
-    _on_device(out)
-    _check(_entry("rows_fp8", "qd_rows_fp8", "pililiipplpliip")(
-        _raw_ptr(x), code, ld, n, step, gated, act, _raw_ptr(bias), q, ldq, s, lds, T, K, _stream()), what)
+    return (_host or _host_calls()).fp8_rows(R, K, _device_of(device))
 
 
 def quantize_fp8(x: torch.Tensor, out: Fp8Rows) -> None:
     """out = x in 8 bits: x bfloat16 or float32 [T, K] (rows may lie apart), or float32 partial sums [n, T, K], which are added first.
     A block's scale is the smallest power of two with which its largest magnitude stays within 448; a block with an infinity or a NaN
     gets the scale NaN."""
-    T, K, *at = _fp8_check(out, "quantize_fp8: out")
-    _rows_fp8(x, *_fp8_source(x, "quantize_fp8: x", T, K), 0, 0, None, out, *at, T, K, "quantize_fp8")
+    _launch_count[0] += 1
+    (_host or _host_calls()).quantize_fp8(x, out)
 
 
 def gate_fp8(gate_up: torch.Tensor, out: Fp8Rows, bias: Optional[torch.Tensor] = None, act: int = ACT_SILU) -> None:
     """out[t, f] = act(g) u in 8 bits, with g = gate_up[t, f] + bias[f] and u = gate_up[t, F + f] + bias[F + f]: gate_up bfloat16 or
     float32 [T, 2F], or float32 partial sums [n, T, 2F]; ``bias`` float32 [2F] or None; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``."""
-    T, F, *at = _fp8_check(out, "gate_fp8: out")
-    source = _fp8_source(gate_up, "gate_fp8: gate_up", T, 2 * F)
-    _fp8_bias(bias, 2 * F, "gate_fp8")
-    _fp8_act(act, "gate_fp8")
-    _rows_fp8(gate_up, *source, 1, act, bias, out, *at, T, F, "gate_fp8")
-
-
-def _fp8_bias(bias: Optional[torch.Tensor], n: int, what: str) -> None:
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
-        raise KernelError(f"{what}: bias must be contiguous float32 [{n}]")
-
-
-def _fp8_act(act: int, what: str) -> None:
-    if act not in (ACT_SILU, ACT_GATED_GELU):
-        raise KernelError(f"{what}: act must be ACT_SILU or ACT_GATED_GELU, got {act}")
+    _launch_count[0] += 1
+    (_host or _host_calls()).gate_fp8(gate_up, out, bias, act)
 
 
 def add_rmsnorm_fp8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, out: Fp8Rows, eps: float,
@@ -1059,92 +977,27 @@ def add_rmsnorm_fp8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
     """``add_rmsnorm`` with its output in 8 bits: out[r] = rmsnorm(x[s] + delta[s]) * weight with s = rows[r] (or r), rounded once; x
     float32 [T, D] is updated to x + delta when ``write_back``.  delta: bfloat16 or float32 [T, D], or float32 partial sums [n, T, D];
     ``delta_scale`` float32 [D] or None multiplies it."""
-    R, D, q, ldq, s, lds = _fp8_check(out, "add_rmsnorm_fp8: out")
-    shape = x.shape
-    if x.dtype is not _F32 or len(shape) != 2 or shape[1] != D or not x.is_contiguous():
-        raise KernelError(f"add_rmsnorm_fp8: x must be contiguous float32 [T, {D}]")
-    T = shape[0]
-    if weight.dtype is not _F32 or weight.numel() != D or not weight.is_contiguous():
-        raise KernelError(f"add_rmsnorm_fp8: weight must be contiguous float32 [{D}]")
-    if delta_scale is not None and (delta_scale.dtype != torch.float32 or delta_scale.numel() != D or not delta_scale.is_contiguous()):
-        raise KernelError(f"add_rmsnorm_fp8: delta_scale must be contiguous float32 [{D}]")
-    if rows is None and R != T or rows is not None and (rows.dtype != torch.int32 or rows.numel() != R or not rows.is_contiguous()):
-        raise KernelError("add_rmsnorm_fp8: out has a row for every row of x, or for every one of rows (contiguous int32)")
-    code, n = F32, 1
-    if delta is not None:
-        code, _, n, _ = _fp8_source(delta, "add_rmsnorm_fp8: delta", T, D)
-        if not delta.is_contiguous():
-            raise KernelError("add_rmsnorm_fp8: delta must be contiguous")
-    _on_device(out)
-    _check(_entry("rows_fp8", "qd_add_rmsnorm_fp8", "ppippplplpiifiilp")(
-        _raw_ptr(x), _raw_ptr(delta), code, _raw_ptr(delta_scale), _raw_ptr(weight), q, ldq, s, lds, _raw_ptr(rows), R, D, eps,
-        1 if write_back else 0, n, T * D, _stream()), "add_rmsnorm_fp8")
+    _launch_count[0] += 1
+    (_host or _host_calls()).add_rmsnorm_fp8(x, delta, weight, out, eps, rows, write_back, delta_scale)
 
 
-@functools.lru_cache(maxsize=4096)
-def gemm_fp8_plan(T: int, N: int, K: int, epi: int, out_code: int, sms: int):
-    """(CTAs to a tile of tokens, rows of w to a tile, shares of K) of a product in 8 bits; ``out_code``: ``dtype_code`` of the result
-    (of ``EPI_STORE``)."""
-    v = [ctypes.c_int(0) for _ in range(3)]
-    if not library("gemm_fp8").qd_gemm_fp8_plan(_I(T), _I(N), _I(K), _I(epi), _I(out_code), _I(sms), *map(ctypes.byref, v)):
-        raise KernelError(f"gemm_fp8: no product of {T} x {K} by {N} x {K}")
-    return tuple(n.value for n in v)
-
-
-FP8_FEW = (0, 0, 0)      # as a plan: the kernel of few tokens
-FP8_FEW_TOKENS = 16      # what it takes
-
-
-def gemm_fp8_few_wanted(T: int, N: int, K: int) -> bool:
-    """Whether ``csrc/gemm_fp8_few.cu`` is the faster one: up to 8 tokens and 20 MB of weights, up to 16 and 10 MB (times beside its
-    kernel)."""
-    return T <= 8 and N * K <= 20_000_000 or T <= FP8_FEW_TOKENS and N * K <= 10_000_000
-
-
-def _gemm_fp8(x_at, w_at, bias, out, code, ldo, s_out, lds_out, epi, plan, what):
-    T, K, x, ldx, sx, ldsx = x_at
-    N, _, w, ldw, sw, ldsw = w_at
-    if T == 0 or N == 0:
-        return
-    sms = sm_count()
-    if epi == EPI_STORE and (plan == FP8_FEW or plan is None and gemm_fp8_few_wanted(T, N, K)):
-        _check(_entry("gemm_fp8_few", "qd_gemm_fp8_few", "plplplplppiliiiip")(
-            w, ldw, sw, ldsw, x, ldx, sx, ldsx, _raw_ptr(bias), out, code, ldo, T, N, K, sms, _stream()), what)
-        return
-    cg, bn, splits = plan or gemm_fp8_plan(T, N, K, epi, code, sms)
-    _check(_entry("gemm_fp8", "qd_gemm_fp8", "plplplplppilpliiiiiiiip")(
-        w, ldw, sw, ldsw, x, ldx, sx, ldsx, _raw_ptr(bias), out, code, ldo, s_out, lds_out, T, N, K, cg, bn, splits, epi, sms, _stream()), what)
+FP8_FEW = (0, 0, 0)      # as a plan: the kernel of up to FP8_FEW_TOKENS tokens
+FP8_FEW_TOKENS = 16
 
 
 def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Tensor, plan=None) -> None:
     """out[T, N] = x @ w^T (+ bias float32 [N]) of rows in 8 bits on the tensor cores, float32 sums; out bfloat16 or float32, rows may
-    lie apart.  ``plan``: as ``gemm_fp8_plan`` gives it, or ``FP8_FEW`` (up to 16 tokens); None: the faster one."""
-    x_at = _fp8_check(x, "gemm_fp8: x")
-    w_at = _fp8_check(w, "gemm_fp8: w", K=x_at[1])
-    T, N, dt = x_at[0], w_at[0], out.dtype
-    shape, stride = out.shape, out.stride()
-    if not (dt is _F32 or dt is _BF16) or len(shape) != 2 or shape[0] != T or shape[1] != N or (stride[1] != 1 and N > 1):
-        raise KernelError(f"gemm_fp8: out must be bfloat16 or float32 [{T}, {N}] with contiguous rows")
-    _fp8_bias(bias, N, "gemm_fp8")
-    _on_device(x)
-    _on_device(w)
-    _gemm_fp8(x_at, w_at, bias, _raw_ptr(out), F32 if dt is _F32 else BF16, stride[0], None, 0, EPI_STORE, plan, "gemm_fp8")
+    lie apart.  ``plan``: (CTAs to a tile of tokens, rows of w to a tile, shares of K), or ``FP8_FEW``; None: the fastest by its sizes."""
+    _launch_count[0] += 1
+    (_host or _host_calls()).gemm_fp8(x, w, bias, out, plan)
 
 
 def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None) -> None:
     """out[T, F] = act(x @ wg^T + bg) * (x @ wu^T + bu) in 8 bits, for the product that follows: w [2F, K] holds the gate's rows, then
     up's, ``bias`` float32 [2F] (or None) likewise; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``.  The sums and the activation are
     float32, rounded once."""
-    x_at = _fp8_check(x, "gemm_fp8_gated: x")
-    w_at = _fp8_check(w, "gemm_fp8_gated: w", K=x_at[1])
-    if w_at[0] % 2:
-        raise KernelError("gemm_fp8_gated: w holds as many rows of up as of the gate")
-    _, _, q, ldq, s, lds = _fp8_check(out, "gemm_fp8_gated: out", x_at[0], w_at[0] // 2)
-    _fp8_bias(bias, w_at[0], "gemm_fp8_gated")
-    _fp8_act(act, "gemm_fp8_gated")
-    for rows in (x, w, out):
-        _on_device(rows)
-    _gemm_fp8(x_at, w_at, bias, q, BF16, ldq, s, lds, EPI_SWIGLU + 256 * act, plan, "gemm_fp8_gated")
+    _launch_count[0] += 1
+    (_host or _host_calls()).gemm_fp8_gated(x, w, bias, out, act, plan)
 
 
 # ------------------------------------------------------------------ latent attention

@@ -14,7 +14,7 @@ def rows(R, K):
 def test_room_for_rows(R, K, q, s):
     out = rows(R, K)
     assert tuple(out.q.shape) == (R, K) and out.q.stride() == q and tuple(out.s.shape) == (R, -(-K // 128)) and out.s.stride()[:1] == s[:1]
-    kernels._fp8_check(out, "out", R, K)
+    assert kernels._host_calls().check_rows(out, "out") == (R, K)
 
 
 BAD_ROWS = {
@@ -59,11 +59,6 @@ def test_products():
         kernels.gemm_fp8_gated(x, w, None, rows(3, 4), kernels.ACT_CLAMPED)
     with pytest.raises(KernelError, match="CUDA"):
         kernels.gemm_fp8(x, w, None, torch.empty(3, 8), (1, 64, 1))
-
-
-def test_which_kernel_takes_few_tokens():
-    wanted = kernels.gemm_fp8_few_wanted
-    assert wanted(1, 2048, 2048) and wanted(8, 4608, 3584) and not wanted(8, 2048, 11008) and wanted(16, 2560, 2048) and not wanted(17, 64, 128)
 
 
 def test_sources():
