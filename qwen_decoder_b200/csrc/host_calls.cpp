@@ -162,8 +162,8 @@ Plan plan_of(int T, int N, int K, int epi, int code, int sms) {
   if (kept.size() >= 4096) kept.clear();
   return kept[key] = p;
 }
-// The few-token kernel is the faster one up to 8 tokens and 20 MB of weights, up to 16 and 10 MB (times beside it)
-bool few_wanted(int64_t T, int64_t N, int64_t K) { return (T <= 8 && N * K <= 20000000) || (T <= FEW_TOKENS && N * K <= 10000000); }
+// The few-token kernel is the faster one up to 8 tokens and 23 MB of weights, up to 16 and 10 MB (times beside it)
+bool few_wanted(int64_t T, int64_t N, int64_t K) { return (T <= 8 && N * K <= 23000000) || (T <= FEW_TOKENS && N * K <= 10000000); }
 
 void product(const Rows& x, const Rows& w, const at::Tensor* bias, void* out, int code, int64_t ldo, void* s_out, int64_t lds_out, int epi, PyObject* plan,
              const char* what) {
