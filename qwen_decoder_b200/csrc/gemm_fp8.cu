@@ -811,7 +811,7 @@ extern "C" int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long lo
   if (T <= 0 || N <= 0) return 0;
   const int act = epi >> 8;
   epi &= 255;
-  if (K <= 0 || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) || bn < 32 || bn > 256 || bn % (cg == 2 || splits > 1 ? 32 : 16) || splits < 1 ||
+  if (T > (1 << 30) || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) || bn < 32 || bn > 256 || bn % (cg == 2 || splits > 1 ? 32 : 16) || splits < 1 ||
       splits > 8 || sms < 2 || !out)
     return QD_ERR_UNSUPPORTED;
   if ((((uintptr_t)W | (uintptr_t)X) & 15) || (((uintptr_t)sw | (uintptr_t)sx) & 3) || ldsw % 4 || ldsx % 4) return QD_ERR_UNSUPPORTED;

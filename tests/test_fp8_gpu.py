@@ -23,6 +23,14 @@ def numbers(shape, g, spread=0):
     return x
 
 
+def room(R, K):
+    """``kernels.fp8_rows`` between margins that are looked at when a test ends (its own room does not go through torch.empty)."""
+    from qwen_decoder_b200 import kernels
+    kb = -(-K // 128)
+    return kernels.Fp8Rows(torch.empty((R, -(-K // 16) * 16), dtype=torch.float8_e4m3fn, device=DEV)[:, :K],
+                           torch.empty((R, -(-kb // 4) * 4), dtype=torch.float8_e8m0fnu, device=DEV)[:, :kb])
+
+
 def scales_of(peak):
     """The scale of a block by its definition: the smallest power of two with peak <= 448 * scale, 1 of zeros, 2^-126 at least."""
     e = torch.ceil(torch.log2(peak / 448.0))
@@ -54,7 +62,7 @@ def check_rows(rows, y, off):
 
 def rows_of(x):
     from qwen_decoder_b200 import kernels
-    out = kernels.fp8_rows(*x.shape, DEV)
+    out = room(*x.shape)
     kernels.quantize_fp8(x, out)
     return out
 
@@ -106,7 +114,7 @@ def test_parts_are_added_first(n, K):
 
 def rows_of_parts(parts):
     from qwen_decoder_b200 import kernels
-    out = kernels.fp8_rows(*parts.shape[1:], DEV)
+    out = room(*parts.shape[1:])
     kernels.quantize_fp8(parts, out)
     return out
 
@@ -123,7 +131,7 @@ def test_gate(T, F, n, bias, act):
     from qwen_decoder_b200 import kernels
     g = generator(T, F, n)
     parts, b = numbers((n, T, 2 * F), g), numbers((2 * F,), g) if bias else None
-    out = kernels.fp8_rows(T, F, DEV)
+    out = room(T, F)
     kernels.gate_fp8(parts, out, b, act)
     z = parts.double().sum(0) + (b.double() if bias else 0)
     # n + 1 roundings of 2^-24 of what is added; the activation's slope is below 1.2, its exponential and quotient within 2^-20
@@ -137,7 +145,7 @@ def test_gate_of_infinities():
     from qwen_decoder_b200 import kernels
     z = torch.ones(3, 256, device=DEV)
     z[0, 0], z[1, 0], z[2, 0] = -float("inf"), float("inf"), float("nan")
-    out = kernels.fp8_rows(3, 128, DEV)
+    out = room(3, 128)
     kernels.gate_fp8(z, out)
     assert out.q[0, 0].float() == 0 and not out.s[0].float().isnan().any() and out.s[1:].float().isnan().all()
 
@@ -155,7 +163,7 @@ def test_norm(T, D, parts, scaled):
         d, size = d * f.double(), size * f.double().abs()
     sums, off = x.double() + d, (parts + 3) * 2.0 ** -24 * (x.double().abs() + size)
     y = sums * torch.rsqrt(sums.square().mean(1, keepdim=True) + 1e-6) * w.double()
-    out, kept = kernels.fp8_rows(T, D, DEV), x.clone()
+    out, kept = room(T, D), x.clone()
     kernels.add_rmsnorm_fp8(x, delta, w, out, 1e-6, delta_scale=f)
     assert ((x.double() - sums).abs() <= off).all()
     # a thread's up to 64 squares and a tree of 10 levels, a quotient, a root and three products: below 2^-17; the sums' own error apart
@@ -165,7 +173,7 @@ def test_norm(T, D, parts, scaled):
     check_rows(out, y, own)
     # chosen rows, the sum left as it was
     rows = torch.tensor([T - 1, 0], dtype=torch.int32, device=DEV)
-    again, few = kept.clone(), kernels.fp8_rows(2, D, DEV)
+    again, few = kept.clone(), room(2, D)
     kernels.add_rmsnorm_fp8(again, delta, w, few, 1e-6, rows=rows, write_back=False, delta_scale=f)
     assert torch.equal(again, kept) and torch.equal(few.q.view(torch.uint8), out.q[rows.long()].view(torch.uint8))
     assert torch.equal(few.s.view(torch.uint8), out.s.view(torch.uint8)[rows.long()])
@@ -175,7 +183,7 @@ def test_norm_of_zeros_and_without_delta():
     from qwen_decoder_b200 import kernels
     x = torch.zeros(2, 300, device=DEV)
     x[1, 7] = 3.0
-    out = kernels.fp8_rows(2, 300, DEV)
+    out = room(2, 300)
     kernels.add_rmsnorm_fp8(x, None, torch.ones(300, device=DEV), out, 1e-6)
     assert out.q[0].float().abs().max() == 0 and (out.s[0].float() == 1).all()
     assert float(value(out)[1, 7]) == pytest.approx(300 ** 0.5, rel=2.0 ** -4) and (out.q[1].float() != 0).sum() == 1
@@ -235,7 +243,7 @@ def test_gated_product(T, F, K, bias, act):
     h = gated(z[:, :F], z[:, F:], act)
     wide = 1.2 * off[:, :F] * z[:, F:].abs() + (z[:, :F].abs() + off[:, :F]) * off[:, F:] + 2.0 ** -20 * (z[:, :F] * z[:, F:]).abs()
     for plan in (None, (1, 256, 1), (2, 256, 1)):
-        out = kernels.fp8_rows(T, F, DEV)
+        out = room(T, F)
         kernels.gemm_fp8_gated(x, w, b if bias else None, out, act, plan)
         check_rows(out, h, wide)
     kernels.check_status()
@@ -249,6 +257,30 @@ def test_few_tokens_and_several_tiles_to_a_cta():
         kernels.gemm_fp8(x, w, bias, out, kernels.FP8_FEW)
         want = value(x) @ value(w).T + bias.double()
         assert ((out.double() - want).abs() <= 2.0 ** -23 * want.abs() + sums_off(x, w)).all()
+
+
+@pytest.mark.parametrize("T,plan", [(5, (1, 256, 1)), (40, (1, 256, 1)), (140, (2, 256, 1)), (140, (1, 256, 1))])
+def test_no_numbers_and_infinities_in_a_gated_product(T, plan):
+    """A block that holds one makes its rows' sums none and the result's whole blocks with them; sums that are infinite do the same, but for
+    gates of minus infinity, which close."""
+    from qwen_decoder_b200 import kernels
+    F = 300
+    x, w, _ = operands(T, 2 * F, 384)
+    clean = room(T, F)
+    kernels.gemm_fp8_gated(x, w, None, clean, 0, plan)
+    x.s.view(torch.uint8)[2, 1] = 255
+    w.s.view(torch.uint8)[130, 0] = 255                    # a row of the gate, of the second block of features
+    bias = torch.zeros(2 * F, device=DEV)
+    bias[299] = -float("inf")                              # a closed gate, of the third
+    out = room(T, F)
+    kernels.gemm_fp8_gated(x, w, bias, out, 0, plan)
+    none = torch.zeros(T, 3, dtype=torch.bool, device=DEV)
+    none[2], none[:, 1] = True, True
+    assert torch.equal(out.s.float().isnan(), none)
+    rows = [r for r in range(T) if r != 2]
+    assert torch.equal(out.q[rows, :128].view(torch.uint8), clean.q[rows, :128].view(torch.uint8))
+    assert (out.q[rows, 299].float() == 0).all() and out.q[2].float().isnan().all()
+    kernels.check_status()
 
 
 def test_rows_behind_the_end_are_not_taken():
@@ -278,7 +310,7 @@ def test_products_of_several_tiles_to_a_worker():
     h = gated(want[:, :9500], want[:, 9500:], 0)
     wide = 1.2 * off[:, :9500] * want[:, 9500:].abs() + (want[:, :9500].abs() + off[:, :9500]) * off[:, 9500:] + 2.0 ** -20 * (want[:, :9500] * want[:, 9500:]).abs()
     for plan in ((1, 256, 1), (2, 256, 1)):
-        rows = kernels.fp8_rows(520, 9500, DEV)
+        rows = room(520, 9500)
         kernels.gemm_fp8_gated(x, w, None, rows, 0, plan)
         check_rows(rows, h, wide)
     kernels.check_status()
@@ -312,7 +344,7 @@ def test_on_another_stream_and_in_a_graph():
     from qwen_decoder_b200 import kernels
     g = generator(3)
     x, w, gu = numbers((40, 512), g), operands(40, 256, 512)[1], operands(40, 600, 512)[1]
-    first, second, out = kernels.fp8_rows(40, 512, DEV), kernels.fp8_rows(40, 300, DEV), torch.empty(40, 256, device=DEV)
+    first, second, out = room(40, 512), room(40, 300), torch.empty(40, 256, device=DEV)
 
     def chain():
         kernels.add_rmsnorm_fp8(x, None, torch.ones(512, device=DEV), first, 1e-6)
@@ -341,9 +373,9 @@ def test_on_another_stream_and_in_a_graph():
 def test_nothing_to_do():
     from qwen_decoder_b200 import kernels
     w = operands(1, 64, 256)[1]
-    none = kernels.fp8_rows(0, 256, DEV)
+    none = room(0, 256)
     kernels.quantize_fp8(torch.empty(0, 256, device=DEV), none)
     kernels.gemm_fp8(none, w, None, torch.empty(0, 64, device=DEV))
-    kernels.gemm_fp8_gated(none, w, None, kernels.fp8_rows(0, 32, DEV))
+    kernels.gemm_fp8_gated(none, w, None, room(0, 32))
     kernels.add_rmsnorm_fp8(torch.empty(0, 256, device=DEV), None, torch.ones(256, device=DEV), none, 1e-6)
     torch.cuda.synchronize()
