@@ -52,6 +52,7 @@ struct G8Params {
   int kb_total, stages;
   int feats;               // columns of the result
   int vec;                 // rows of the result take 16-byte stores
+  int resident;            // no kernel before this one writes W or its scales
   long long ldo;           // elements
   const unsigned char *sx, *sw;
   long long ldsx, ldsw;
@@ -281,6 +282,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     };
     int item_t = item, kb_t = kb;
     G8Item q_t = q;
+    if (!p.resident) pdl_wait();
     for (; n < p.stages && item < n_items; n++, next(item, q, kb))
       if (one) weights(n, q, kb);
     pdl_wait();
@@ -415,7 +417,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       return n;
     };
     open();
-    load(1);                                                 // (W's do not come from the kernel before)
+    if (!p.resident) pdl_wait();
+    load(1);
     load(2);
     pdl_wait();
     load(0);
@@ -804,22 +807,23 @@ static bool g8_make_map(CUtensorMap* map, const void* base, long long rows, long
 // float32 [N]), bfloat16 or float32, rows ``ldo`` apart; ``splits`` > 1: K shared by clusters of so many CTAs (up to 8), a tile to each.
 // epi 2 (+ 256 * QD_ACT_*): W [2F, K] the gate's rows, then up's; out e4m3 [T, F] = act(X Wg^T) * (X Wu^T), rows ``ldo`` bytes apart
 // (a multiple of 4), and its scales s_out, rows ``lds_out`` apart.  ``cg``: CTAs to a tile of tokens, 1 (up to 128) or 2 (up to 256);
-// ``bn``: rows of W to a tile, a multiple of 16 (of 32 for pairs and clusters) from 32 to 256 (256 for epi 2).
+// ``bn``: rows of W to a tile, a multiple of 16 (of 32 for pairs and clusters) from 32 to 256 (256 for epi 2).  ``resident``: W and sw are
+// written by nothing that may still run on the stream; they are then asked for before the kernels before this one have ended.
 extern "C" int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
                            long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, void* s_out, long long lds_out,
-                           int T, int N, int K, int cg, int bn, int splits, int epi, int sms, cudaStream_t stream) {
+                           int T, int N, int K, int cg, int bn, int splits, int epi, int resident, int sms, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
   const int act = epi >> 8;
   epi &= 255;
-  if (T > (1 << 30) || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) || bn < 32 || bn > 256 || bn % (cg == 2 || splits > 1 ? 32 : 16) || splits < 1 ||
-      splits > 8 || sms < 2 || !out)
+  if (T > (1 << 30) || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || (cg != 1 && cg != 2) ||
+      bn < 32 || bn > 256 || bn % (cg == 2 || splits > 1 ? 32 : 16) || splits < 1 || splits > 8 || sms < 2 || !out)
     return QD_ERR_UNSUPPORTED;
   if ((((uintptr_t)W | (uintptr_t)X) & 15) || (((uintptr_t)sw | (uintptr_t)sx) & 3) || ldsw % 4 || ldsx % 4) return QD_ERR_UNSUPPORTED;
   if (epi == G8_GATED ? ((N & 1) || bn != 256 || splits != 1 || !s_out || ldo % 4 || (act != QD_ACT_SILU && act != QD_ACT_GELU_TANH))
                       : epi != G8_STORE)
     return QD_ERR_UNSUPPORTED;
   G8Params p;
-  p.act = act; p.T = T; p.N = N; p.K = K; p.bn = bn; p.splits = splits; p.ldo = ldo;
+  p.act = act; p.resident = resident; p.T = T; p.N = N; p.K = K; p.bn = bn; p.splits = splits; p.ldo = ldo;
   p.sx = (const unsigned char*)sx; p.sw = (const unsigned char*)sw; p.ldsx = ldsx; p.ldsw = ldsw;
   p.s_out = (unsigned char*)s_out; p.lds_out = lds_out;
   p.kb_total = up(K, FP8_BLOCK);

@@ -33,6 +33,7 @@ struct FwParams {
   const float* bias;
   void* out;
   int T, N, K, blocks, tiles, shares;      // CTAs that share a tile's K
+  int resident;                            // no kernel before this one writes W or its scales
 };
 
 // 16 bytes, of which ``there`` (0 to 16) come from memory and the others are zero
@@ -93,6 +94,7 @@ __global__ void __launch_bounds__(FW_WARPS * 32, 2) gemm_fp8_few_kernel(const Fw
   auto commit = [&]() { asm volatile("cp.async.commit_group;" ::: "memory"); };
   const Place first = {b0 < b1 ? worker : p.tiles, b0};       // (a warp without blocks asks for none)
   Place ask = first;
+  if (!p.resident) pdl_wait();
 #pragma unroll 1
   for (int i = 0; i < DEPTH; i++) {
     if (ask.tile < p.tiles) {
@@ -236,16 +238,18 @@ static int fw_launch(const FwParams& p, int ctas, cudaStream_t stream) {
 
 // X [T, K] and W [N, K] e4m3, rows ``ldx`` and ``ldw`` bytes apart (multiples of 16, as the addresses), with scales sx and sw, rows ``ldsx``
 // and ``ldsw`` bytes apart; out [T, N] = X W^T (+ bias float32 [N]), bfloat16 or float32, rows ``ldo`` apart.  T up to 16.
+// ``resident``: W and sw are written by nothing that may still run on the stream (they are asked for before that has ended).
 extern "C" int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
-                               long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, int T, int N, int K, int sms,
-                               cudaStream_t stream) {
+                               long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, int T, int N, int K, int resident,
+                               int sms, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
-  if (T > 16 || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || ((((uintptr_t)W | (uintptr_t)X) & 15)) || sms < 1 || !out)
+  if (T > 16 || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || ((((uintptr_t)W | (uintptr_t)X) & 15)) ||
+      sms < 1 || !out)
     return QD_ERR_UNSUPPORTED;
   FwParams p;
   p.w = (const unsigned char*)W; p.sw = (const unsigned char*)sw; p.x = (const unsigned char*)X; p.sx = (const unsigned char*)sx;
   p.ldw = ldw; p.ldsw = ldsw; p.ldx = ldx; p.ldsx = ldsx; p.ldo = ldo; p.bias = bias; p.out = out;
-  p.T = T; p.N = N; p.K = K;
+  p.T = T; p.N = N; p.K = K; p.resident = resident;
   p.blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
   p.tiles = (N + FW_ROWS - 1) / FW_ROWS;
   if (ldsx < p.blocks || ldsw < p.blocks) return QD_ERR_UNSUPPORTED;

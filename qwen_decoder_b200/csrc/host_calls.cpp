@@ -138,9 +138,9 @@ typedef int NormFn(void*, const void*, int, const void*, const void*, void*, lon
                    cudaStream_t);
 typedef int PlanFn(int, int, int, int, int, int, int*, int*, int*);
 typedef int ProductFn(const void*, long long, const void*, long long, const void*, long long, const void*, long long, const void*, void*, int, long long,
-                      void*, long long, int, int, int, int, int, int, int, int, cudaStream_t);
+                      void*, long long, int, int, int, int, int, int, int, int, int, cudaStream_t);
 typedef int FewFn(const void*, long long, const void*, long long, const void*, long long, const void*, long long, const void*, void*, int, long long, int,
-                  int, int, int, cudaStream_t);
+                  int, int, int, int, cudaStream_t);
 typedef int LogprobsFn(const void*, int, long long, const void*, void*, void*, void*, void*, int, int, int, int, cudaStream_t);
 RowsFn* g_rows;
 NormFn* g_norm;
@@ -166,7 +166,9 @@ Plan plan_of(int T, int N, int K, int epi, int code, int sms) {
 bool few_wanted(int64_t T, int64_t N, int64_t K) { return (T <= 8 && N * K <= 23000000) || (T <= FEW_TOKENS && N * K <= 10000000); }
 
 void product(const Rows& x, const Rows& w, const at::Tensor* bias, void* out, int code, int64_t ldo, void* s_out, int64_t lds_out, int epi, PyObject* plan,
-             const char* what) {
+             PyObject* resident_o, const char* what) {
+  const int resident = PyObject_IsTrue(resident_o);
+  if (resident < 0) throw PythonError{};
   const int T = (int)x.R, N = (int)w.R, K = (int)x.K;
   on_device(x);
   on_device(w);
@@ -184,10 +186,10 @@ void product(const Rows& x, const Rows& w, const at::Tensor* bias, void* out, in
   }
   if (few)
     done(entry(g_few, "gemm_fp8_few", "qd_gemm_fp8_few")(w.q_at, w.ldq, w.s_at, w.lds, x.q_at, x.ldq, x.s_at, x.lds, address(bias), out, code, ldo, T, N, K,
-                                                        sms, stream), what);
+                                                        resident, sms, stream), what);
   else
     done(entry(g_product, "gemm_fp8", "qd_gemm_fp8")(w.q_at, w.ldq, w.s_at, w.lds, x.q_at, x.ldq, x.s_at, x.lds, address(bias), out, code, ldo, s_out, lds_out,
-                                                    T, N, K, p.cg, p.bn, p.splits, epi, sms, stream), what);
+                                                    T, N, K, p.cg, p.bn, p.splits, epi, resident, sms, stream), what);
 }
 
 // ---- the module's functions
@@ -282,8 +284,8 @@ CALL(add_rmsnorm_fp8, 8)
   Py_RETURN_NONE;
 END
 
-// (x, w, bias, out, plan)
-CALL(gemm_fp8, 5)
+// (x, w, bias, out, plan, resident)
+CALL(gemm_fp8, 6)
   const Rows x = rows_of(a[0], "gemm_fp8: x"), w = rows_of(a[1], "gemm_fp8: w", -1, x.K);
   const at::Tensor& out = tensor(a[3], "gemm_fp8: out");
   const at::Tensor* bias = tensor_or_none(a[2], "gemm_fp8: bias");
@@ -292,12 +294,12 @@ CALL(gemm_fp8, 5)
     refuse("gemm_fp8: out must be bfloat16 or float32 [", x.R, ", ", w.R, "] with contiguous rows");
   vector_of(bias, w.R, "gemm_fp8", "bias");
   on_device(x);
-  product(x, w, bias, address(out), dt == at::kFloat ? F32 : BF16, out.stride(0), nullptr, 0, STORE, a[4], "gemm_fp8");
+  product(x, w, bias, address(out), dt == at::kFloat ? F32 : BF16, out.stride(0), nullptr, 0, STORE, a[4], a[5], "gemm_fp8");
   Py_RETURN_NONE;
 END
 
-// (x, w, bias, out, act, plan)
-CALL(gemm_fp8_gated, 6)
+// (x, w, bias, out, act, plan, resident)
+CALL(gemm_fp8_gated, 7)
   const Rows x = rows_of(a[0], "gemm_fp8_gated: x"), w = rows_of(a[1], "gemm_fp8_gated: w", -1, x.K);
   if (w.R % 2) refuse("gemm_fp8_gated: w holds as many rows of up as of the gate");
   const Rows out = rows_of(a[3], "gemm_fp8_gated: out", x.R, w.R / 2);
@@ -305,7 +307,7 @@ CALL(gemm_fp8_gated, 6)
   vector_of(bias, w.R, "gemm_fp8_gated", "bias");
   const int act = act_of(a[4], "gemm_fp8_gated");
   on_device(out);
-  product(x, w, bias, out.q_at, BF16, out.ldq, out.s_at, out.lds, GATED + 256 * act, a[5], "gemm_fp8_gated");
+  product(x, w, bias, out.q_at, BF16, out.ldq, out.s_at, out.lds, GATED + 256 * act, a[5], a[6], "gemm_fp8_gated");
   Py_RETURN_NONE;
 END
 

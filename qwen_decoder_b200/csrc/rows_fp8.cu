@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(1024) norm_fp8_kernel(const NormArgs a) {
   __shared__ float scratch[40];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = (blockDim.x >> 5) * FP8_BLOCK, k0 = warp * FP8_BLOCK + 4 * lane;
   pdl_launch_dependents();
-  // (the weights do not come from the kernel before: with few blocks to a warp they travel while that is waited for)
+  // (no kernel of the package writes a norm's weights: with few blocks to a warp they travel while that is waited for)
   float4 w[VPT <= 4 ? VPT : 1];
   if (VPT <= 4)
 #pragma unroll

@@ -985,19 +985,22 @@ FP8_FEW = (0, 0, 0)      # as a plan: the kernel of up to FP8_FEW_TOKENS tokens
 FP8_FEW_TOKENS = 16
 
 
-def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Tensor, plan=None) -> None:
+def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Tensor, plan=None, resident: bool = False) -> None:
     """out[T, N] = x @ w^T (+ bias float32 [N]) of rows in 8 bits on the tensor cores, float32 sums; out bfloat16 or float32, rows may
-    lie apart.  ``plan``: (CTAs to a tile of tokens, rows of w to a tile, shares of K), or ``FP8_FEW``; None: the fastest by its sizes."""
+    lie apart.  ``plan``: (CTAs to a tile of tokens, rows of w to a tile, shares of K), or ``FP8_FEW``; None: the fastest by its sizes.
+    ``resident``: ``w`` is written by nothing that may still run on the stream, as a model's weights; they are then on their way before the
+    kernel before has ended."""
     _launch_count[0] += 1
-    (_host or _host_calls()).gemm_fp8(x, w, bias, out, plan)
+    (_host or _host_calls()).gemm_fp8(x, w, bias, out, plan, resident)
 
 
-def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None) -> None:
+def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None,
+                   resident: bool = False) -> None:
     """out[T, F] = act(x @ wg^T + bg) * (x @ wu^T + bu) in 8 bits, for the product that follows: w [2F, K] holds the gate's rows, then
     up's, ``bias`` float32 [2F] (or None) likewise; ``act``: ``ACT_SILU`` or ``ACT_GATED_GELU``.  The sums and the activation are
-    float32, rounded once."""
+    float32, rounded once.  ``resident``: as in ``gemm_fp8``."""
     _launch_count[0] += 1
-    (_host or _host_calls()).gemm_fp8_gated(x, w, bias, out, act, plan)
+    (_host or _host_calls()).gemm_fp8_gated(x, w, bias, out, act, plan, resident)
 
 
 # ------------------------------------------------------------------ latent attention

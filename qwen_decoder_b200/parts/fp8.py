@@ -65,6 +65,7 @@ class Fp8Linear(Linear):
             weight = weight.float()                # (float16 as it is stored)
         n = weight.shape[0]
         kernels.quantize_fp8(weight.contiguous(), kernels.Fp8Rows(self.rows.q[at:at + n], self.rows.s[at:at + n]))
+        torch.cuda.current_stream(weight.device).synchronize()      # the products read them ahead of what is before them on the stream
 
     def forward(self, x: kernels.Fp8Rows, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return self._product(x, self.bias, out_dtype or torch.bfloat16)
@@ -78,7 +79,7 @@ class Fp8Linear(Linear):
 
     def _product(self, x: kernels.Fp8Rows, bias: Optional[torch.Tensor], dtype: torch.dtype) -> torch.Tensor:
         out = torch.empty((x.q.shape[0], self.out_features), dtype=dtype, device=x.q.device)
-        kernels.gemm_fp8(x, self.rows, bias, out)
+        kernels.gemm_fp8(x, self.rows, bias, out, resident=True)
         matmul_backend.counters["own"] += 1
         return out
 
@@ -138,6 +139,6 @@ class SwiGLUFp8(SwiGLU):
 
     def _products(self, x: kernels.Fp8Rows) -> torch.Tensor:
         h = kernels.fp8_rows(x.q.shape[0], self.intermediate_size, x.q.device)
-        kernels.gemm_fp8_gated(x, self.gate_up.rows, self.gate_up.bias, h, ACTIVATIONS[self.activation])
+        kernels.gemm_fp8_gated(x, self.gate_up.rows, self.gate_up.bias, h, ACTIVATIONS[self.activation], resident=True)
         matmul_backend.counters["own"] += 1
         return self._down(h)

@@ -72,15 +72,15 @@ class Watch:
         kernel_tests.check_rows(out, x.double(), torch.zeros_like(x, dtype=torch.float64))
         self.calls.append(("rows", x.data_ptr(), out.q.data_ptr()))
 
-    def gemm_fp8(self, real, x, w, bias, out, plan=None):
-        real(x, w, bias, out, plan)
+    def gemm_fp8(self, real, x, w, bias, out, plan=None, resident=False):
+        real(x, w, bias, out, plan, resident)
         want = kernel_tests.value(x) @ kernel_tests.value(w).T + (0 if bias is None else bias.double())
         close = (2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -23) * want.abs() + kernel_tests.sums_off(x, w)
         assert ((out.double() - want).abs() <= close).all()
         self.calls.append(("product", x.q.data_ptr(), out.data_ptr()))
 
-    def gemm_fp8_gated(self, real, x, w, bias, out, act=0, plan=None):
-        real(x, w, bias, out, act, plan)
+    def gemm_fp8_gated(self, real, x, w, bias, out, act=0, plan=None, resident=False):
+        real(x, w, bias, out, act, plan, resident)
         z, F = kernel_tests.value(x) @ kernel_tests.value(w).T, out.shape[1]
         off = kernel_tests.sums_off(x, w) + 2.0 ** -23 * z.abs()
         g, u = z[:, :F], z[:, F:]

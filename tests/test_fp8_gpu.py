@@ -329,6 +329,41 @@ def test_a_block_of_no_numbers_reaches_its_rows_sums_alone(plan):
     assert torch.equal(out.isnan(), none)
 
 
+@pytest.mark.parametrize("gated_one", [False, True])
+@pytest.mark.parametrize("T, plan", [(4, None), (64, None), (300, None), (4, (1, 128, 4)), (12, (0, 0, 0))])
+def test_weights_that_the_launches_before_write(T, plan, gated_one):
+    """Both operands rounded right before the product, which must not read either earlier: results as of the same operands at rest."""
+    from qwen_decoder_b200 import kernels
+    N, K = 4096, 4096
+    if gated_one and plan is not None:
+        pytest.skip("a gated product has one cut")
+    g = generator(T, 7)
+    x, w = numbers((T, K), g).bfloat16(), numbers((N, K), g).bfloat16()
+    xr, wr = room(T, K), room(N, K)
+
+    def product():
+        if gated_one:
+            out = room(T, N // 2)
+            kernels.gemm_fp8_gated(xr, wr, None, out)
+            return out.q.view(torch.uint8), out.s.view(torch.uint8)
+        out = torch.empty((T, N), device="cuda")
+        kernels.gemm_fp8(xr, wr, None, out, plan)
+        return (out,)
+
+    kernels.quantize_fp8(x, xr)
+    kernels.quantize_fp8(w, wr)
+    torch.cuda.synchronize()
+    want = product()
+    zeros = torch.zeros_like(w)
+    for order in range(8):
+        kernels.quantize_fp8(zeros, wr)
+        torch.cuda.synchronize()
+        for rows, source in ((wr, w), (xr, x))[::-1 if order % 2 else 1]:
+            kernels.quantize_fp8(source, rows)
+        for got, wanted in zip(product(), want):
+            assert torch.equal(got, wanted)
+
+
 @pytest.mark.parametrize("plan", [(0, 0, 0), (1, 64, 1), (1, 96, 3)])
 def test_rows_apart_and_scales_apart(plan):
     from qwen_decoder_b200 import kernels
