@@ -11,6 +11,20 @@ int qd_add_rmsnorm(float* x, const void* delta, int delta_dtype, const float* w,
 int qd_rope_kv_write_biased(void* qkv, const float* bias, int T, int H, int G, int d, int rotary_dim, int pairing,
                             const float* cos_t, const float* sin_t, const int* positions, void* kv,
                             const int* slot_map, int page_size, int write_kv, cudaStream_t stream);
+int qd_rope_kv_write_partial(const float* part, int n_parts, const float* bias, void* q_out, int T, int H, int G, int d, int rotary_dim,
+                             int pairing, const float* cos_t, const float* sin_t, const int* positions, void* kv, const int* slot_map,
+                             int page_size, int write_kv, cudaStream_t stream);
+int qd_rows_fp8(const void* x, int dtype, long long ldx, int n_parts, long long part_stride, int gated, int act, const float* bias, void* q,
+                long long ldq, void* s, long long lds, int T, int K, cudaStream_t stream);
+int qd_add_rmsnorm_fp8(float* x, const void* delta, int delta_dtype, const float* dscale, const float* w, void* q, long long ldq, void* s,
+                       long long lds, const int* rows, int n_rows, int D, float eps, int write_back, int n_parts, long long part_stride,
+                       cudaStream_t stream);
+int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx, long long ldsx,
+                const float* bias, void* out, int out_dtype, long long ldo, void* s_out, long long lds_out, int T, int N, int K, int cg,
+                int bn, int splits, int epi, int resident, int sms, cudaStream_t stream);
+int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
+                    long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, int T, int N, int K, int resident,
+                    int sms, cudaStream_t stream);
 int qd_gemm_pair(const void* W, const void* X, long long ldx, const float* bias, void* out, int out_dtype, long long ldo, int T,
                  int N, int K, int cg, int bn, int splits, int epi, int sms, cudaStream_t stream);
 int qd_gemm_pair_plan(int T, int N, int K, int epi, int sms, int* cg_out, int* bn_out, int* splits_out);

@@ -24,6 +24,7 @@
 // which wait it was.
 //
 // The reference has 16-bit products only (cublasHgemm, gpu_kernels.cu:431-436).
+#include "entry_points.h"
 #include "fp8.cuh"
 #include "tc5_ops.cuh"
 

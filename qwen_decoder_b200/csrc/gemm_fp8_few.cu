@@ -17,6 +17,7 @@
 //   1,000 x 1,000    2.4 /  4.5    3.1 / 5.2      22,016 x 2,048   13.3 / 10.5   19.6 / 11.8
 //
 // The reference has 16-bit products only (cublasHgemm, gpu_kernels.cu:431-436).
+#include "entry_points.h"
 #include "fp8.cuh"
 
 #define FW_WARPS 8

@@ -311,6 +311,17 @@ CALL(gemm_fp8_gated, 7)
   Py_RETURN_NONE;
 END
 
+// (T, N, K, gated, float32, device) -> (CTAs to a tile of tokens, rows of w to a tile, shares of K), three zeros: the few-token kernel
+CALL(gemm_fp8_plan, 6)
+  const long T = PyLong_AsLong(a[0]), N = PyLong_AsLong(a[1]), K = PyLong_AsLong(a[2]);
+  const int gated = PyObject_IsTrue(a[3]), f32 = PyObject_IsTrue(a[4]), device = (int)PyLong_AsLong(a[5]);
+  if (PyErr_Occurred()) throw PythonError{};
+  if (T < 1 || N < 1 || K < 1 || T > INT32_MAX || N > INT32_MAX || K > INT32_MAX) refuse("gemm_fp8_plan: no product of ", T, " x ", K, " by ", N, " x ", K);
+  Plan p = {0, 0, 0};
+  if (gated || !few_wanted(T, N, K)) p = plan_of((int)T, (int)N, (int)K, gated ? GATED : STORE, f32 ? F32 : BF16, multiprocessors(device));
+  return Py_BuildValue("iii", p.cg, p.bn, p.splits);
+END
+
 // (logits, tokens, top) -> (logprob, entropy, ids, logprobs of the ids)
 CALL(token_logprobs, 3)
   const at::Tensor &z = tensor(a[0], "token_logprobs: logits"), &tokens = tensor(a[1], "token_logprobs: tokens");
@@ -356,7 +367,7 @@ END
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(start), ENTRY(fp8_rows), ENTRY(check_rows), ENTRY(quantize_fp8), ENTRY(gate_fp8), ENTRY(add_rmsnorm_fp8), ENTRY(gemm_fp8),
-                         ENTRY(gemm_fp8_gated), ENTRY(token_logprobs), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(gemm_fp8_gated), ENTRY(gemm_fp8_plan), ENTRY(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qd_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

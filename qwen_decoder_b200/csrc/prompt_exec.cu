@@ -13,6 +13,10 @@
 //               where gemm_pair.cu takes it) ; delta = act Wd^T
 //   at the end: hrows = rmsnorm(x += delta) at the wanted rows          (the output projection stays outside)
 //
+// With ``layers8`` the same layers with their products in 8 bits: both norms leave such rows, attention's output is rounded by a launch
+// of its own, gate, up and the activation are one product, and q, k and v come with their bias (of up to ``few8`` tokens as float32 sums,
+// which the rotation takes with it).  ``final8``: the output projection takes such rows, whatever the layers do.
+//
 // It holds no kernel of its own.  The launchers live in the other libraries of this directory and the matrix
 // products that gemm_pair.cu does not take in cuBLAS (as the reference's do, gpu_kernels.cu:431-436); the caller hands over their
 // addresses, so this library links against none of them and uses whatever cuBLAS the process has loaded.
@@ -57,7 +61,18 @@ struct PeFns {
   decltype(&qd_decode_attention_shares) attention_shares;       // the single tokens' attention with shares by length
 };
 
-// How a product is cut (``qd_gemm_pair_plan``); cg 0: the library's product
+// Rows in 8 bits and their scales, rows so many bytes apart
+struct PeRows8 { void* q; long long ldq; void* s; long long lds; };
+struct PeLayer8 { PeRows8 wqkv, wo, wgu, wd; };
+struct PeFns8 {
+  decltype(&qd_rope_kv_write_partial) rope_partial;
+  decltype(&qd_rows_fp8) rows;
+  decltype(&qd_add_rmsnorm_fp8) add_rmsnorm;
+  decltype(&qd_gemm_fp8) gemm;
+  decltype(&qd_gemm_fp8_few) gemm_few;
+};
+
+// How a product is cut (``qd_gemm_pair_plan``; in 8 bits ``qd_gemm_fp8_plan``); cg 0: the library's product (in 8 bits ``gemm_few``)
 struct PePlan { int cg, bn, splits; };
 
 struct PeParams {
@@ -88,10 +103,18 @@ struct PeParams {
   // the single tokens' shares of decode attention (null: ``decode_splits`` for each); ``part_o`` and ``part_ml`` are theirs then
   void* shares;
   int n_shares, scratch_row;
+  // products in 8 bits (null ``layers8``: none)
+  PeFns8 fn8;
+  const PeLayer8* layers8;         // of the same layers, for their weights
+  PeRows8 h8, attn8, act8, hrows8; // [T, D] [T, Hd] [T, F] [n_wanted, D]
+  PePlan qkv_plan8, wo_plan8, wgu_plan8, wd_plan8;
+  float* qkv32;                    // [T, (H+2G)d], up to ``few8`` tokens
+  int few8, final8;
 };
 
-extern "C" int qd_prompt_exec_struct_sizes(int* layer_bytes, int* params_bytes) {
+extern "C" int qd_prompt_exec_struct_sizes(int* layer_bytes, int* layer8_bytes, int* params_bytes) {
   *layer_bytes = (int)sizeof(PeLayer);
+  *layer8_bytes = (int)sizeof(PeLayer8);
   *params_bytes = (int)sizeof(PeParams);
   return 0;
 }
@@ -124,6 +147,18 @@ static int product_for_norm(const PeParams& p, const PePlan& plan, const void* W
   return p.fn.gemm_pair(W, X, K, nullptr, part, QD_F32, N, T, N, K, plan.cg, plan.bn, plan.splits, 1, p.sms, stream);
 }
 
+// Y[T, N] = X W^T (+ bias) of rows in 8 bits; ``out8``: Y is act(gate) * up in such rows, W's N rows the gate's and then up's
+static int product8(const PeParams& p, const PePlan& plan, const PeRows8& W, const PeRows8& X, const float* bias, void* Y, int dtype, int N,
+                    int K, cudaStream_t stream, const PeRows8* out8 = nullptr) {
+  if (out8)
+    return p.fn8.gemm(W.q, W.ldq, W.s, W.lds, X.q, X.ldq, X.s, X.lds, bias, out8->q, QD_BF16, out8->ldq, out8->s, out8->lds, p.T, N, K, plan.cg,
+                      plan.bn, plan.splits, 2 + 256 * QD_ACT_SILU, 1, p.sms, stream);
+  if (!plan.cg)
+    return p.fn8.gemm_few(W.q, W.ldq, W.s, W.lds, X.q, X.ldq, X.s, X.lds, bias, Y, dtype, N, p.T, N, K, 1, p.sms, stream);
+  return p.fn8.gemm(W.q, W.ldq, W.s, W.lds, X.q, X.ldq, X.s, X.lds, bias, Y, dtype, N, nullptr, 0, p.T, N, K, plan.cg, plan.bn, plan.splits, 0, 1,
+                    p.sms, stream);
+}
+
 #define PE_TRY(call)            \
   do {                          \
     int rc_ = (call);           \
@@ -147,35 +182,63 @@ extern "C" int qd_prompt_exec(const PeParams* pp, cudaStream_t stream) {
   int delta_dtype = QD_BF16, delta_parts = 1;          // what the previous layer's down projection left
   const void* o;
   int o_dtype, o_parts;
+  const PeLayer8* layers8 = p.layers8;
+  if ((layers8 || p.final8) && !p.fn8.add_rmsnorm) return QD_ERR_UNSUPPORTED;
+  if (layers8 && (shares || !p.fn8.rows || !p.fn8.gemm || !p.fn8.gemm_few || !p.fn8.rope_partial || (T <= p.few8 && !p.qkv32))) return QD_ERR_UNSUPPORTED;
+  const int ldq = layers8 && T <= p.few8 ? H * d : n_qkv;         // elements from a token's q to the next one's
   for (int l = 0; l < p.n_layers; l++) {
     const PeLayer& L = p.layers[l];
-    if (shares > 1 && delta_parts > 1) p.fn.plain_next();     // the norm that reads the batched product waits for all of it
-    PE_TRY(p.fn.add_rmsnorm(p.x, delta, delta ? delta_dtype : -1, L.norm1_w, p.h, QD_BF16, nullptr, T, D, L.eps1, 1,
-                            delta_parts, xn, stream));
-    PE_TRY(product(p, L.wqkv, p.h, p.qkv, T, n_qkv, D));
-    PE_TRY(p.fn.rope_kv_write(p.qkv, L.bqkv, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv,
-                              p.slot_map, p.page_size, L.write_kv, stream));
+    if (layers8) {
+      const PeLayer8& W = layers8[l];
+      PE_TRY(p.fn8.add_rmsnorm(p.x, delta, QD_BF16, nullptr, L.norm1_w, p.h8.q, p.h8.ldq, p.h8.s, p.h8.lds, nullptr, T, D, L.eps1, 1, 1, xn, stream));
+      if (T <= p.few8) {
+        PE_TRY(product8(p, p.qkv_plan8, W.wqkv, p.h8, nullptr, p.qkv32, QD_F32, n_qkv, D, stream));
+        PE_TRY(p.fn8.rope_partial(p.qkv32, 1, L.bqkv, p.qkv, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv, p.slot_map,
+                                  p.page_size, L.write_kv, stream));
+      } else {
+        PE_TRY(product8(p, p.qkv_plan8, W.wqkv, p.h8, L.bqkv, p.qkv, QD_BF16, n_qkv, D, stream));
+        PE_TRY(p.fn.rope_kv_write(p.qkv, nullptr, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv, p.slot_map, p.page_size,
+                                  L.write_kv, stream));
+      }
+    } else {
+      if (shares > 1 && delta_parts > 1) p.fn.plain_next();     // the norm that reads the batched product waits for all of it
+      PE_TRY(p.fn.add_rmsnorm(p.x, delta, delta ? delta_dtype : -1, L.norm1_w, p.h, QD_BF16, nullptr, T, D, L.eps1, 1,
+                              delta_parts, xn, stream));
+      PE_TRY(product(p, L.wqkv, p.h, p.qkv, T, n_qkv, D));
+      PE_TRY(p.fn.rope_kv_write(p.qkv, L.bqkv, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv,
+                                p.slot_map, p.page_size, L.write_kv, stream));
+    }
     const int nd = p.n_decode;
     if (nd > 0 && p.shares && l == 0) PE_TRY(p.fn.decode_shares(p.positions, p.slot_map, p.scratch_row, nd, p.n_shares, p.shares, stream));
     if (nd > 0 && p.shares)
-      PE_TRY(p.fn.attention_shares(p.qkv, n_qkv, p.attn, L.kv, p.n_pages, p.block_table, p.max_blocks, nd, H, G, d, p.page_size,
+      PE_TRY(p.fn.attention_shares(p.qkv, ldq, p.attn, L.kv, p.n_pages, p.block_table, p.max_blocks, nd, H, G, d, p.page_size,
                                    p.scale, p.shares, p.n_shares, l == 0, p.part_o, p.part_ml, p.tickets, stream));
     else if (nd > 0 && p.fn.attention_decode_tma && (p.decode_splits == 1 || p.tickets))
-      PE_TRY(p.fn.attention_decode_tma(p.qkv, n_qkv, p.attn, L.kv, p.n_pages, p.block_table, p.max_blocks, p.token_req,
+      PE_TRY(p.fn.attention_decode_tma(p.qkv, ldq, p.attn, L.kv, p.n_pages, p.block_table, p.max_blocks, p.token_req,
                                        p.positions, nd, H, G, d, p.page_size, p.scale, p.window, p.decode_splits, p.part_o,
                                        p.part_ml, p.tickets, stream));
     else if (nd > 0)
-      PE_TRY(p.fn.attention_decode(p.qkv, n_qkv, p.attn, L.kv, p.block_table, p.max_blocks, p.token_req, p.positions,
+      PE_TRY(p.fn.attention_decode(p.qkv, ldq, p.attn, L.kv, p.block_table, p.max_blocks, p.token_req, p.positions,
                                    nd, H, G, d, p.page_size, p.scale, p.window, p.decode_splits, p.part_o, p.part_ml,
                                    p.tickets, stream));
     const int* bt = p.block_table + (size_t)nd * p.max_blocks;
     if (p.use_tc5)
-      PE_TRY(p.fn.attention_tc5(p.qkv, n_qkv, p.attn, L.kv, p.n_pages, bt, p.max_blocks, p.cu_tokens + nd,
+      PE_TRY(p.fn.attention_tc5(p.qkv, ldq, p.attn, L.kv, p.n_pages, bt, p.max_blocks, p.cu_tokens + nd,
                                 p.start_pos + nd, p.R - nd, T - nd, H, G, d, p.page_size, p.scale, p.window, nullptr,
                                 stream));
     else
-      PE_TRY(p.fn.attention_regs(p.qkv, n_qkv, p.attn, L.kv, bt, p.max_blocks, p.cu_tokens + nd, p.start_pos + nd,
+      PE_TRY(p.fn.attention_regs(p.qkv, ldq, p.attn, L.kv, bt, p.max_blocks, p.cu_tokens + nd, p.start_pos + nd,
                                  p.R - nd, T - nd, H, G, d, p.page_size, p.scale, p.window, stream));
+    if (layers8) {
+      const PeLayer8& W = layers8[l];
+      PE_TRY(p.fn8.rows(p.attn, QD_BF16, H * d, 1, 0, 0, 0, nullptr, p.attn8.q, p.attn8.ldq, p.attn8.s, p.attn8.lds, T, H * d, stream));
+      PE_TRY(product8(p, p.wo_plan8, W.wo, p.attn8, nullptr, p.delta, QD_BF16, D, H * d, stream));
+      PE_TRY(p.fn8.add_rmsnorm(p.x, p.delta, QD_BF16, nullptr, L.norm2_w, p.h8.q, p.h8.ldq, p.h8.s, p.h8.lds, nullptr, T, D, L.eps2, 1, 1, xn, stream));
+      PE_TRY(product8(p, p.wgu_plan8, W.wgu, p.h8, nullptr, nullptr, QD_BF16, 2 * F, D, stream, &p.act8));
+      PE_TRY(product8(p, p.wd_plan8, W.wd, p.act8, nullptr, p.delta, QD_BF16, D, F, stream));
+      delta = p.delta;
+      continue;
+    }
     PE_TRY(product_for_norm(p, p.wo_plan, L.wo, p.attn, p.delta, p.o_part, T, D, H * d, &o, &o_dtype, &o_parts, stream));
     PE_TRY(p.fn.add_rmsnorm(p.x, o, o_dtype, L.norm2_w, p.h, QD_BF16, nullptr, T, D, L.eps2, 1, o_parts, xn, stream));
     if (p.wgu_plan.cg) {
@@ -191,6 +254,9 @@ extern "C" int qd_prompt_exec(const PeParams* pp, cudaStream_t stream) {
       PE_TRY(product_for_norm(p, p.wd_plan, L.wd, p.act, p.delta, p.down_part, T, D, F, &delta, &delta_dtype, &delta_parts, stream));
     }
   }
+  if (p.n_wanted > 0 && p.final8)
+    return p.fn8.add_rmsnorm(p.x, delta, delta_dtype, nullptr, p.final_w, p.hrows8.q, p.hrows8.ldq, p.hrows8.s, p.hrows8.lds, p.logit_rows, p.n_wanted, D,
+                             p.final_eps, 0, delta_parts, xn, stream);
   if (p.n_wanted > 0 && shares > 1 && delta_parts > 1) p.fn.plain_next();
   if (p.n_wanted > 0)
     PE_TRY(p.fn.add_rmsnorm(p.x, delta, delta ? delta_dtype : -1, p.final_w, p.hrows, QD_BF16, p.logit_rows, p.n_wanted,

@@ -5,6 +5,7 @@
 // to 8 bits.
 //
 // The reference rounds nothing below 16 bits (its norm and activation: gpu_kernels.cu:32-67, 136-160).
+#include "entry_points.h"
 #include "fp8.cuh"
 
 // Four neighbouring features, zeros from ``K`` on.  VEC: K is a multiple of 4 and they lie on 16 (float32) or 8 bytes (bfloat16): one

@@ -994,6 +994,12 @@ def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Te
     (_host or _host_calls()).gemm_fp8(x, w, bias, out, plan, resident)
 
 
+def gemm_fp8_plan(T: int, N: int, K: int, gated: bool = False, dtype: torch.dtype = torch.bfloat16, device=None) -> tuple:
+    """The plan that ``gemm_fp8`` (or ``gemm_fp8_gated``) takes by itself for T rows of x and N of w, results of ``dtype``."""
+    index = torch.cuda.current_device() if device is None else _device_of(device).index
+    return (_host or _host_calls()).gemm_fp8_plan(T, N, K, gated, dtype == torch.float32, index)
+
+
 def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp8Rows, act: int = ACT_SILU, plan=None,
                    resident: bool = False) -> None:
     """out[T, F] = act(x @ wg^T + bg) * (x @ wu^T + bu) in 8 bits, for the product that follows: w [2F, K] holds the gate's rows, then
@@ -1993,6 +1999,25 @@ class PromptLayer(ctypes.Structure):
         [("eps1", ctypes.c_float), ("eps2", ctypes.c_float), ("write_kv", ctypes.c_int), ("pad", ctypes.c_int)]
 
 
+class PromptRows8(ctypes.Structure):
+    """Rows in 8 bits of the native prompt step (PeRows8 in csrc/prompt_exec.cu)."""
+    _fields_ = [("q", ctypes.c_void_p), ("ldq", ctypes.c_longlong), ("s", ctypes.c_void_p), ("lds", ctypes.c_longlong)]
+
+    @classmethod
+    def of(cls, rows: Fp8Rows) -> "PromptRows8":
+        return cls(rows.q.data_ptr(), rows.q.stride(0), rows.s.data_ptr(), rows.s.stride(0))
+
+
+class PromptLayer8(ctypes.Structure):
+    """The weights in 8 bits of one schedule entry (PeLayer8 in csrc/prompt_exec.cu)."""
+    _fields_ = [(n, PromptRows8) for n in ("wqkv", "wo", "wgu", "wd")]
+
+
+class PromptFns8(ctypes.Structure):
+    """Addresses of the launchers that the native prompt step calls for products in 8 bits."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("rope_partial", "rows", "add_rmsnorm", "gemm", "gemm_few")]
+
+
 class PromptFns(ctypes.Structure):
     """Addresses of the launchers and of the library product that the native prompt step calls."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("add_rmsnorm", "rope_kv_write", "swiglu", "attention_regs",
@@ -2019,13 +2044,16 @@ class PromptParams(ctypes.Structure):
         [(n, ctypes.c_void_p) for n in ("token_req", "part_o", "part_ml", "tickets", "down_part")] + \
         [("down_shares", ctypes.c_int), ("pad2", ctypes.c_int)] + \
         [(n, PromptPlan) for n in ("wo_plan", "wgu_plan", "wd_plan")] + [("sms", ctypes.c_int), ("o_part", ctypes.c_void_p)] + \
-        [("shares", ctypes.c_void_p), ("n_shares", ctypes.c_int), ("scratch_row", ctypes.c_int)]
+        [("shares", ctypes.c_void_p), ("n_shares", ctypes.c_int), ("scratch_row", ctypes.c_int)] + \
+        [("fn8", PromptFns8), ("layers8", ctypes.c_void_p)] + [(n, PromptRows8) for n in ("h8", "attn8", "act8", "hrows8")] + \
+        [(n, PromptPlan) for n in ("qkv_plan8", "wo_plan8", "wgu_plan8", "wd_plan8")] + \
+        [("qkv32", ctypes.c_void_p), ("few8", ctypes.c_int), ("final8", ctypes.c_int)]
 
 
 def prompt_exec_struct_sizes_match() -> bool:
-    a, b = ctypes.c_int(0), ctypes.c_int(0)
-    library("prompt_exec").qd_prompt_exec_struct_sizes(ctypes.byref(a), ctypes.byref(b))
-    return a.value == ctypes.sizeof(PromptLayer) and b.value == ctypes.sizeof(PromptParams)
+    sizes = [ctypes.c_int(0) for _ in range(3)]
+    library("prompt_exec").qd_prompt_exec_struct_sizes(*(ctypes.byref(s) for s in sizes))
+    return [s.value for s in sizes] == [ctypes.sizeof(t) for t in (PromptLayer, PromptLayer8, PromptParams)]
 
 
 def _loaded_cublas() -> ctypes.CDLL:
@@ -2069,6 +2097,17 @@ def prompt_fns(use_tc5: bool, with_decode: bool = False, decode_tma: bool = Fals
         fns.plain_next = addr(ew.qd_elementwise_plain_next)
         fns.gemm_pair = addr(library("gemm_pair").qd_gemm_pair)
         _prompt_fns[(use_tc5, with_decode, decode_tma)] = fns
+    return fns
+
+
+def prompt_fns8() -> PromptFns8:
+    """The launchers' addresses for products in 8 bits."""
+    fns = _prompt_fns.get("fp8")
+    if fns is None:
+        addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+        rows = library("rows_fp8")
+        fns = _prompt_fns["fp8"] = PromptFns8(addr(library("elementwise").qd_rope_kv_write_partial), addr(rows.qd_rows_fp8), addr(rows.qd_add_rmsnorm_fp8),
+                                              addr(library("gemm_fp8").qd_gemm_fp8), addr(library("gemm_fp8_few").qd_gemm_fp8_few))
     return fns
 
 

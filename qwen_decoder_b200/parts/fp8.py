@@ -89,7 +89,7 @@ class RMSNormFp8(RMSNorm):
     """``rmsnorm`` whose output leaves as rows in 8 bits, for products that take them."""
 
     def native_params(self):
-        return None
+        return dict(super().native_params(), kind="rmsnorm_fp8")
 
     def forward(self, stream: ResidualStream, out_dtype: torch.dtype, rows: Optional[torch.Tensor] = None) -> kernels.Fp8Rows:
         stream.settle()
@@ -111,7 +111,8 @@ class GQAttentionFp8(GQAttention):
         self.out = Fp8Linear(self.out.in_features, self.out.pieces, bias=self.out.has_bias)
 
     def native_params(self):
-        return None
+        answer = super().native_params()
+        return answer and dict(answer, kind="gq_attention_fp8", wqkv=self.qkv.rows, wo=self.out.rows)
 
     def _few_token_sums(self, x: kernels.Fp8Rows) -> Optional[torch.Tensor]:
         return self.qkv.sums(x) if x.q.shape[0] <= FEW_TOKENS else None
@@ -135,7 +136,8 @@ class SwiGLUFp8(SwiGLU):
                               bias_suffix=self.down.bias_suffix)
 
     def native_params(self):
-        return None
+        answer = super().native_params()
+        return answer and dict(answer, kind="swiglu_fp8", wgu=self.gate_up.rows, wd=self.down.rows)
 
     def _products(self, x: kernels.Fp8Rows) -> torch.Tensor:
         h = kernels.fp8_rows(x.q.shape[0], self.intermediate_size, x.q.device)

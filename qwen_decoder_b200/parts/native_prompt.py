@@ -4,7 +4,7 @@ A step with a prompt portion is launched kernel by kernel.  From Python that is 
 15 us of host time per launch, 5 ms for 36 layers, while the device needs 3 ms for a
 portion of 512 tokens: the device waits for the interpreter.  When every layer of the
 schedule is the common composition -- pre-norm block, grouped-query attention with one
-rotary table, SwiGLU, RMSNorm, bfloat16 -- the same launchers are called,
+rotary table, SwiGLU, RMSNorm, bfloat16 or with its products in 8 bits -- the same launchers are called,
 in the same order and with the same arguments, from one C++ loop instead.  The embedding
 before it and the output projection after it stay with the model.
 
@@ -14,7 +14,7 @@ collects the answers.  A model with any other part or another dtype keeps the pa
 path, and so does a step of single tokens (it replays as a CUDA graph); so does everything
 when ``QD_NATIVE_PROMPT=0`` is set.
 
-One difference in arithmetic: the parts' q/k/v product adds its bias in the product's
+One difference in arithmetic (not of products in 8 bits, which are the parts' own): the parts' q/k/v product adds its bias in the product's
 epilogue, here the rotation kernel adds it to the product's bfloat16 output (one more
 rounding to bfloat16 of q, k and v).
 """
@@ -34,6 +34,8 @@ _MIN_TOKENS = 1       # measured faster at every length: 4 tokens 3.2 against 4.
 # the one arrangement of parts whose order of kernels csrc/prompt_exec.cu restates: a block that answers
 # ``native_params()`` with any other ``composition`` (another order, another part) keeps the parts' own path
 COMPOSITION = "pre_norm/gq_attention/swiglu/rmsnorm/rmsnorm"
+COMPOSITION_8 = "pre_norm/gq_attention_fp8/swiglu_fp8/rmsnorm_fp8/rmsnorm_fp8"      # the same with its products in 8 bits
+LAUNCHES_PER_LAYER_8 = 9
 OWN_LAUNCHES_PER_LAYER = 4    # norm, rotation, attention, norm; SwiGLU or a product with it; products as ``_plans`` says
 
 
@@ -48,6 +50,8 @@ class NativePrompt:
         self.schedule = [e.cache_of is None for e in model.schedule]
         self._cache_id = None
         self._layers = None               # host array of PromptLayer, kept alive here
+        self.in_8_bits = common["composition"] == COMPOSITION_8
+        self._layers8 = None              # of PromptLayer8
         self.steps = 0                    # steps run here (tests look at it)
 
     # ---- eligibility ---------------------------------------------------------
@@ -59,9 +63,9 @@ class NativePrompt:
         entries, common = [], None
         for e in model.schedule:
             answer = getattr(model.layers[e.layer], "native_params", lambda: None)()
-            if answer is None or answer.get("composition") != COMPOSITION:
+            if answer is None or answer.get("composition") not in (COMPOSITION, COMPOSITION_8):
                 return None
-            key = {k: answer[k] for k in ("D", "H", "G", "d", "F", "window", "scale", "rotary_dim", "pairing")}
+            key = {k: answer[k] for k in ("composition", "D", "H", "G", "d", "F", "window", "scale", "rotary_dim", "pairing")}
             key["position"] = id(answer["position"])
             if common is None:
                 common = dict(key, position_obj=answer["position"])
@@ -71,7 +75,7 @@ class NativePrompt:
         if common is None or model.hidden_size != common["D"]:
             return None
         final = getattr(model.final_norm, "native_params", lambda: None)()
-        if final is None or final.get("kind") != "rmsnorm" or "weight" not in final:
+        if final is None or final.get("kind") not in ("rmsnorm", "rmsnorm_fp8") or "weight" not in final:
             return None
         c = common
         n_qkv = (c["H"] + 2 * c["G"]) * c["d"]
@@ -106,7 +110,7 @@ class NativePrompt:
         """(output projection, gate and up, down projection): how ``csrc/gemm_pair.cu`` cuts them at ``T`` tokens, None: the
         library's product."""
         c = self.common
-        if matmul_backend.mode != "auto" or any(a[n].data_ptr() % 16 for a in self.entries for n in ("wo", "wgu", "wd")):
+        if self.in_8_bits or matmul_backend.mode != "auto" or any(a[n].data_ptr() % 16 for a in self.entries for n in ("wo", "wgu", "wd")):
             return None, None, None
         plan = lambda N, K, epi: kernels.gemm_pair_sizes_plan(T, N, K, epi, kernels.sm_count())
         return (plan(c["D"], c["H"] * c["d"], kernels.EPI_PARTIAL), plan(2 * c["F"], c["D"], kernels.EPI_SWIGLU),
@@ -119,19 +123,43 @@ class NativePrompt:
             for i, a in enumerate(self.entries):
                 arr[i].norm1_w = a["norm1_w"].data_ptr(); arr[i].eps1 = a["eps1"]
                 arr[i].norm2_w = a["norm2_w"].data_ptr(); arr[i].eps2 = a["eps2"]
-                arr[i].wqkv = a["wqkv"].data_ptr()
+                arr[i].kv = cache.layer_kv(i).data_ptr()
+                arr[i].write_kv = 1 if self.schedule[i] else 0
                 arr[i].bqkv = a["bqkv"].data_ptr() if a["bqkv"] is not None else None
+                if self.in_8_bits:
+                    continue
+                arr[i].wqkv = a["wqkv"].data_ptr()
                 arr[i].wo = a["wo"].data_ptr()
                 arr[i].wgu = a["wgu"].data_ptr()
                 arr[i].wd = a["wd"].data_ptr()
-                arr[i].kv = cache.layer_kv(i).data_ptr()
-                arr[i].write_kv = 1 if self.schedule[i] else 0
+            if self.in_8_bits:
+                self._layers8 = (kernels.PromptLayer8 * len(self.entries))(*(
+                    kernels.PromptLayer8(*(kernels.PromptRows8.of(a[n]) for n in ("wqkv", "wo", "wgu", "wd"))) for a in self.entries))
             self._layers, self._cache_id = arr, id(cache)
         return self._layers
 
-    def forward(self, ctx, x: torch.Tensor) -> Optional[torch.Tensor]:
+    def _in_8_bits(self, p, T: int) -> list:
+        """Fills in what products in 8 bits take; what has to stay alive."""
+        from .fp8 import FEW_TOKENS
+        c, dev = self.common, self.device
+        D, F, attended, n_qkv = c["D"], c["F"], c["H"] * c["d"], (c["H"] + 2 * c["G"]) * c["d"]
+        few = T <= FEW_TOKENS
+        rows = [kernels.fp8_rows(T, n, dev) for n in (D, attended, F)]
+        p.h8, p.attn8, p.act8 = map(kernels.PromptRows8.of, rows)
+        plan = lambda N, K, gated=False, dtype=torch.bfloat16: kernels.PromptPlan(*kernels.gemm_fp8_plan(T, N, K, gated, dtype, dev))
+        p.qkv_plan8 = plan(n_qkv, D, dtype=torch.float32 if few else torch.bfloat16)
+        p.wo_plan8, p.wgu_plan8, p.wd_plan8 = plan(D, attended), plan(2 * F, D, True), plan(D, F)
+        p.layers8 = ctypes.cast(self._layers8, ctypes.c_void_p)
+        p.few8 = FEW_TOKENS
+        if few:
+            rows.append(torch.empty((T, n_qkv), dtype=torch.float32, device=dev))
+            p.qkv32 = rows[-1].data_ptr()
+        return rows
+
+    def forward(self, ctx, x: torch.Tensor):
         """Runs every layer on the residual sum ``x`` (float32 [T, D], the embeddings on entry) and returns
-        the normalised rows at the wanted places (bfloat16 [n_wanted, D]; None if nothing is wanted)."""
+        the normalised rows at the wanted places (bfloat16 [n_wanted, D], or rows in 8 bits where the final norm leaves such; None if
+        nothing is wanted)."""
         c, dev = self.common, self.device
         T, D, H, G, d, F = ctx.num_tokens, c["D"], c["H"], c["G"], c["d"], c["F"]
         bf = torch.bfloat16
@@ -139,13 +167,18 @@ class NativePrompt:
         wo_plan, wgu_plan, wd_plan = plans = self._plans(T)
         # one scratch buffer for the step, carved into the six activations (all offsets 16-byte aligned)
         sizes = [T * D, T * n_qkv, T * H * d, T * D, 0 if wgu_plan else T * 2 * F, T * F]
+        if self.in_8_bits:
+            sizes[0] = sizes[4] = sizes[5] = 0
+        final8 = c["final"]["kind"] == "rmsnorm_fp8"
         offs, total = [], 0
         for n in sizes:
             offs.append(total)
             total += (n + 7) // 8 * 8
         scratch = torch.empty(total, dtype=bf, device=dev)
         base = scratch.data_ptr()
-        hrows = torch.empty((ctx.num_wanted, D), dtype=bf, device=dev) if ctx.num_wanted else None
+        hrows = None
+        if ctx.num_wanted:
+            hrows = kernels.fp8_rows(ctx.num_wanted, D, dev) if final8 else torch.empty((ctx.num_wanted, D), dtype=bf, device=dev)
         group = ctx.groups[0]
         pos = c["position_obj"]
         p = kernels.PromptParams()
@@ -188,8 +221,14 @@ class NativePrompt:
         p.final_w = c["final"]["weight"].data_ptr()
         p.x, p.delta0 = x.data_ptr(), None
         p.h, p.qkv, p.attn, p.delta, p.gu, p.act = (base + 2 * o for o in offs)
-        p.hrows = hrows.data_ptr() if hrows is not None else None
-        shares = matmul_backend.library_shares(T, D, F)
+        if final8 or self.in_8_bits:
+            p.fn8 = kernels.prompt_fns8()
+        if hrows is not None and final8:
+            p.final8, p.hrows8 = 1, kernels.PromptRows8.of(hrows)
+        elif hrows is not None:
+            p.hrows = hrows.data_ptr()
+        keep8 = self._in_8_bits(p, T) if self.in_8_bits else None
+        shares = 0 if self.in_8_bits or final8 else matmul_backend.library_shares(T, D, F)
         p.down_shares = shares
         for field, plan in zip((p.wo_plan, p.wgu_plan, p.wd_plan), plans):
             field.cg, field.bn, field.splits = plan or (0, 0, 0)
@@ -199,9 +238,9 @@ class NativePrompt:
         o_part = parts(wo_plan[2] if wo_plan else 0)
         p.down_part = down_part.data_ptr() if down_part is not None else None
         p.o_part = o_part.data_ptr() if o_part is not None else None
-        own = sum(1 for plan in plans if plan)
-        n_launches = len(self.entries) * (OWN_LAUNCHES_PER_LAYER + own + (0 if wgu_plan else 1) + (1 if nd else 0)) \
-            + (1 if ctx.num_wanted else 0)
+        own = 4 if self.in_8_bits else sum(1 for plan in plans if plan)
+        per_layer = LAUNCHES_PER_LAYER_8 if self.in_8_bits else OWN_LAUNCHES_PER_LAYER + own + (0 if wgu_plan else 1)
+        n_launches = len(self.entries) * (per_layer + (1 if nd else 0)) + (1 if ctx.num_wanted else 0)
         kernels.prompt_exec(p, n_launches)
         self.steps += 1
         matmul_backend.counters["library"] += (4 - own) * len(self.entries)

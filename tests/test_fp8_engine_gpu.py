@@ -93,6 +93,7 @@ class Watch:
 @pytest.mark.parametrize("name", ["A", "B", "C", "D"])
 def test_every_product_and_norm_of_a_step(name, output, tmp_path, monkeypatch):
     runner = runner_of(folder(name, tmp_path, **(BOTH if output else {"projection_dtype": "float8_e4m3"})), use_graphs=False)
+    runner.model.native_prompt = None                      # (the entry points stand between the parts alone)
     watch = Watch(monkeypatch)
     for cuts in ([100], [40, 1, 59], [17, 3, 16, 64], [96] + [1] * 4):
         logits_of(runner, PROMPT[:100], cuts)
@@ -114,6 +115,7 @@ def test_attention_behind_products_in_8_bits(tmp_path, monkeypatch):
     from qwen_decoder_b200.parts.fp8 import GQAttentionFp8
     path = folder("D", tmp_path, projection_dtype="float8_e4m3")
     runner = runner_of(path, use_graphs=False)
+    runner.model.native_prompt = None
     cfg, w = plain_model.read_folder(path)
     mixer = runner.model.layers[0].mixer
     qkv, attn = [], []
@@ -146,6 +148,49 @@ def test_attention_behind_products_in_8_bits(tmp_path, monkeypatch):
         # at most, a weight by e^(2 * that)
         sizes = torch.einsum("thd,shd->tsh", q.view(100, H, d).abs(), k.view(100, G, d).abs().repeat_interleave(H // G, 1)).amax() / d ** 0.5
         assert float((got - want).abs().max()) <= (2 * 2.0 ** -7 * float(sizes) + 3 * 2.0 ** -9) * float(v.abs().max())
+
+
+@pytest.mark.parametrize("output", [False, True])
+@pytest.mark.parametrize("name", ["A", "B", "C", "D"])
+def test_prompt_steps_from_native_code_are_the_parts(name, output, tmp_path):
+    """The same launches: the same bits, of few and of many tokens, beside single tokens of other requests, with nothing wanted."""
+    from qwen_decoder_b200.engine import StepEntry
+    path = folder(name, tmp_path, **(BOTH if output else {"projection_dtype": "float8_e4m3"}))
+    got = []
+    for native in (True, False):
+        runner = runner_of(path, use_graphs=False)
+        assert runner.model.native_prompt is not None
+        if not native:
+            runner.model.native_prompt = None
+        out = [logits_of(runner, PROMPT[:n], cuts) for n, cuts in ((100, [100]), (74, [40, 17, 3, 1, 13]), (2, [2]), (16, [16]))]
+        a, b = runner.open("a"), runner.open("b")
+        runner.step([StepEntry(a, PROMPT[:30], [])])
+        for n in (1, 9, 33):
+            out.append(runner.step([StepEntry(a, [7], [0]), StepEntry(b, PROMPT[:n + 1], [0, n])]).double().cpu())
+        if native:
+            assert runner.model.native_prompt.steps >= 10
+        got.append(out)
+    for x, y in zip(*got):
+        assert torch.isfinite(x).all() and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("tokens", [5, 100])
+def test_only_the_output_projection_in_8_bits(tokens, tmp_path):
+    """Layers in 16 bits launched from native code, whose last norm leaves rows in 8 bits: those that the model in 16 bits takes."""
+    from qwen_decoder_b200.engine import StepEntry
+    path = folder("B", tmp_path)
+    rows = []
+    for projections in (None, {"output_projection_dtype": "float8_e4m3"}):
+        runner = runner_of(path, projections=projections)
+        real = runner.model._logits
+        runner.model._logits = lambda h: (rows.append(h), real(h))[1]
+        assert runner.model.native_prompt is not None
+        rc = runner.open("r")
+        runner.step([StepEntry(rc, PROMPT[:tokens], [0, tokens - 1])])
+        assert runner.model.native_prompt.steps == 1
+    plain, rounded = rows
+    y = plain.double()
+    kernel_tests.check_rows(rounded, y, 2.0 ** -8 * y.abs())          # (y is rounded to bfloat16 itself)
 
 
 def test_weights_in_8_bits_are_near_the_ones_in_16(tmp_path):
