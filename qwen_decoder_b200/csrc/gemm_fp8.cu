@@ -220,7 +220,7 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
 
 template <int EPI, typename TO, int CG>
 __global__ void __launch_bounds__(G8_THREADS, 1)
-gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ bias,
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* bias,
                 TO* __restrict__ out, const G8Params p, int* __restrict__ status) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_ready[2], acc_free[2], scales_full[G8_BUFFERS], scales_empty[G8_BUFFERS];

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(FW_WARPS * 32, 2) gemm_fp8_few_kernel(const Fw
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const int row = scales.tile * FW_ROWS + g + 8 * i;
-      sw[i] = row < p.N ? __ldg(p.sw + row * p.ldsw + scales.b) : 0;
+      sw[i] = row < p.N ? p.sw[row * p.ldsw + scales.b] : 0;
     }
 #pragma unroll
     for (int j = 0; j < NT; j++)

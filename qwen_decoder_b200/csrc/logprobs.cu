@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   const bool writes = share == 0 && threadIdx.x == 0;
   int token = -1;
   float its = __uint_as_float(0x7fc00000u);
-  if (writes) token = __ldg(a.tokens + row);
+  if (writes) token = a.tokens[row];
   for (int tile = lo; tile < hi; tile++) {
     float v[LP_EACH];
     lp_load(v, z, tile * LP_TILE + warp * LP_CHUNK, a.V, a.vec);
