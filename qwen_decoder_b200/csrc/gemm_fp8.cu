@@ -218,6 +218,9 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
   }
 }
 
+template <int ACT>
+struct G8Act { static constexpr int value = ACT; };
+
 template <int EPI, typename TO, int CG>
 __global__ void __launch_bounds__(G8_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* bias,
@@ -533,10 +536,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const bool owner = overlap && side == (buf == 0);
       if (overlap && (!owner || n_rows <= 0)) release(buf);
       if constexpr (EPI == G8_GATED) {
-        if (p.mrows <= G8_FEW) {
+        const bool only = CG == 1 && n_items <= n_workers;   // (its stages have all been read)
+        if (p.mrows <= G8_FEW || (only && p.mrows <= 32)) {
           // The rows of few tokens lie in one quarter of the lanes, which two of the warps reach: they pass the sums on through shared
           // memory, a row of 256 to a warp, four features to a lane (two warps alone took 16.3 us for 8 tokens of 2,048 by 2 x 11,008).
-          float* sums = reinterpret_cast<float*>(b_s + (size_t)p.stages * b_bytes);
+          float* sums = reinterpret_cast<float*>(only ? base : b_s + (size_t)p.stages * b_bytes);
           if (quarter == 0) {
 #pragma unroll 1
             for (int i = 0; i < 8; i++) {
@@ -554,30 +558,92 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           }
           asm volatile("bar.sync 7, 256;" ::: "memory");
           const int tokens = min(p.mrows, p.T - row_x(q)), col = q.ft * 128 + 4 * lane;
-          for (int r = warp; r < tokens; r += G8_EPI_WARPS) {
-            const float4 g4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((lane ^ (r & 7)) << 2));
-            const float4 u4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((32 + lane ^ (r & 7)) << 2));
-            float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-            float peak = 0.f;
+          const auto gate = [&](auto act) {
+#pragma unroll 1
+            for (int r = warp; r < tokens; r += G8_EPI_WARPS) {
+              const float4 g4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((lane ^ (r & 7)) << 2));
+              const float4 u4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((32 + lane ^ (r & 7)) << 2));
+              float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+              float peak = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              if (bias && col + e < p.feats) {
-                g[e] += bias[col + e];
-                u[e] += bias[p.feats + col + e];
+              for (int e = 0; e < 4; e++) {
+                if (bias && col + e < p.feats) {
+                  g[e] += bias[col + e];
+                  u[e] += bias[p.feats + col + e];
+                }
+                g[e] = fp8_gated(g[e], u[e], decltype(act)::value);
               }
-              g[e] = col + e < p.feats ? fp8_gated(g[e], u[e], p.act) : 0.f;
-              peak = fp8_peak(peak, g[e]);
+              if (col + 4 > p.feats)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  if (col + e >= p.feats) g[e] = 0.f;
+#pragma unroll
+              for (int e = 0; e < 4; e++) peak = fp8_peak(peak, g[e]);
+              const unsigned byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));
+              const float inv = fp8_inverse(byte);
+              const unsigned w = fp8_pack4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
+              unsigned char* to = (unsigned char*)out + (size_t)(row_x(q) + r) * p.ldo + col;
+              if (col + 4 <= p.feats) *reinterpret_cast<unsigned*>(to) = w;
+              else
+                for (int e = 0; e < 4 && col + e < p.feats; e++) to[e] = (unsigned char)(w >> 8 * e);
+              if (lane == 0) p.s_out[(size_t)(row_x(q) + r) * p.lds_out + q.ft] = (unsigned char)byte;
             }
-            const unsigned byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));
-            const float inv = fp8_inverse(byte);
-            const unsigned w = fp8_pack4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
-            unsigned char* to = (unsigned char*)out + (size_t)(row_x(q) + r) * p.ldo + col;
-            if (col + 4 <= p.feats) *reinterpret_cast<unsigned*>(to) = w;
-            else
-              for (int e = 0; e < 4 && col + e < p.feats; e++) to[e] = (unsigned char)(w >> 8 * e);
-            if (lane == 0) p.s_out[(size_t)(row_x(q) + r) * p.lds_out + q.ft] = (unsigned char)byte;
-          }
+          };
+          if (p.act == QD_ACT_GELU_TANH) gate(G8Act<QD_ACT_GELU_TANH>());
+          else gate(G8Act<QD_ACT_SILU>());
           asm volatile("bar.sync 7, 256;" ::: "memory");     // the sums have been read
+        } else if (only) {
+          // 16 features at a time, the activations by way of shared memory: the code below, which keeps 64 in registers, is long, and after
+          // other launches the wait for it hides behind nothing here (64 tokens, 2,048 by 2 x 11,008 between the launches of a layer: 18.4 us,
+          // so 13.6; alone, over and over, 13.3 and 13.1).
+          if (n_rows > 0) {
+            float4* mine = reinterpret_cast<float4*>(base) + threadIdx.x;
+            const int col0 = q.ft * 128 + 64 * side;
+            float peak = 0.f;
+            const auto gate = [&](auto act) {
+#pragma unroll 1
+              for (int i = 0; i < 4; i++) {
+                float g[16], u[16];
+                g8_ld16(acc + 64 * side + 16 * i, g);
+                g8_ld16(acc + 128 + 64 * side + 16 * i, u);
+                tc_ld_wait();
+                const int col = col0 + 16 * i;
+                if (bias) {
+                  g8_bias16(g, bias, col, p.feats);
+                  g8_bias16(u, bias + p.feats, col, p.feats);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++) g[e] = fp8_gated(g[e], u[e], decltype(act)::value);
+                if (col + 16 > p.feats)                      // (asked for each feature by itself it was a jump for each, 2.5 us)
+#pragma unroll
+                  for (int e = 0; e < 16; e++)
+                    if (col + e >= p.feats) g[e] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) peak = fp8_peak(peak, g[e]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) mine[(4 * i + e) * 32 * G8_EPI_WARPS] = make_float4(g[4 * e], g[4 * e + 1], g[4 * e + 2], g[4 * e + 3]);
+              }
+            };
+            if (p.act == QD_ACT_GELU_TANH) gate(G8Act<QD_ACT_GELU_TANH>());
+            else gate(G8Act<QD_ACT_SILU>());
+            peaks[warp & 3][side][lane] = __float_as_uint(peak);
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+            const unsigned byte = fp8_scale_byte(max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]));
+            const float inv = fp8_inverse(byte);
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+              unsigned w[4];
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float4 h = mine[(4 * c + e) * 32 * G8_EPI_WARPS];
+                w[e] = fp8_pack4(h.x * inv, h.y * inv, h.z * inv, h.w * inv);
+              }
+              *g8_piece(rows, lane, c) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+            g8_store_rows<unsigned char>(rows, (unsigned char*)out + (size_t)tok0 * p.ldo + col0, p.ldo, n_rows, 4, p.feats - col0, p.vec);
+            if (side == 0 && lane < n_rows) p.s_out[(size_t)(tok0 + lane) * p.lds_out + q.ft] = (unsigned char)byte;
+          }
         } else if (n_rows > 0) {                             // whole warps: the loads are collective
           // First the 64 columns that the next item's MMAs may overwrite, of up in the first accumulator and of the gate in the second,
           // then they may begin (with the loads in the activations' order they waited for those: 2,048 tokens of 2,048 by 2 x 11,008
