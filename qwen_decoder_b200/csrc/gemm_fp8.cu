@@ -714,35 +714,51 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   __syncthreads();
   if constexpr (EPI == G8_SHARED) {
     g8_cluster_sync();
-    // this CTA's share of the tile's pieces of four features, summed in the order of the shares of K
+    // this CTA's share of the tile's rows, summed in the order of the shares of K: up to 32 pieces of four features of a row to a warp, two
+    // times that on their way together
     const G8Item q = g8_item(p, worker, share);
-    const int tok0 = q.tt * p.mrows, n_rows = min(p.mrows, p.T - tok0), pieces = p.bn >> 2, total = n_rows * pieces;
+    const int tok0 = q.tt * p.mrows, n_rows = min(p.mrows, p.T - tok0), pieces = p.bn >> 2, wide = pieces > 32;
+    const int r0 = n_rows * share / p.splits, units = (n_rows * (share + 1) / p.splits - r0) << wide;
     const unsigned at = tc_smem(base);
-    const int e1 = (int)((long long)total * (share + 1) / p.splits);
-    for (int e = (int)((long long)total * share / p.splits) + threadIdx.x; e < e1; e += G8_THREADS) {
-      const int r = e / pieces, c = e - r * pieces, col = q.ft * p.bn + 4 * c;
-      const unsigned from = at + (r * pieces + (c ^ (r & 7))) * 16;
-      float4 v[8];
+    constexpr int WARPS = G8_THREADS / 32;
+#pragma unroll 1
+    for (int u0 = warp; u0 < units; u0 += 2 * WARPS) {
+      float4 v[2][8];
+      int r[2], c[2];
 #pragma unroll
-      for (int sp = 0; sp < 8; sp++)
-        if (sp < p.splits) {
-          unsigned remote;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(from), "r"(sp));
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[sp].x), "=f"(v[sp].y), "=f"(v[sp].z), "=f"(v[sp].w) : "r"(remote) : "memory");
-        }
-      float4 t = v[0];
+      for (int h = 0; h < 2; h++) {
+        const int u = u0 + h * WARPS;
+        r[h] = r0 + (u >> wide);
+        c[h] = u < units ? (wide ? (u & 1) * 32 : 0) + lane : pieces;
+        const unsigned from = at + (r[h] * pieces + (c[h] ^ (r[h] & 7))) * 16;
 #pragma unroll
-      for (int sp = 1; sp < 8; sp++)
-        if (sp < p.splits) { t.x += v[sp].x; t.y += v[sp].y; t.z += v[sp].z; t.w += v[sp].w; }
-      const float f[4] = {t.x, t.y, t.z, t.w};
-      TO* to = out + (size_t)(tok0 + r) * p.ldo + col;
+        for (int sp = 0; sp < 8; sp++)
+          if (sp < p.splits && c[h] < pieces) {
+            unsigned remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(from), "r"(sp));
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[h][sp].x), "=f"(v[h][sp].y), "=f"(v[h][sp].z), "=f"(v[h][sp].w) : "r"(remote) : "memory");
+          }
+      }
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (col + i < p.feats) to[i] = from_float<TO>(f[i] + (bias ? bias[col + i] : 0.f));
+      for (int h = 0; h < 2; h++) {
+        if (c[h] >= pieces) break;
+        float4 t = v[h][0];
+#pragma unroll
+        for (int sp = 1; sp < 8; sp++)
+          if (sp < p.splits) { t.x += v[h][sp].x; t.y += v[h][sp].y; t.z += v[h][sp].z; t.w += v[h][sp].w; }
+        const int col = q.ft * p.bn + 4 * c[h];
+        const float f[4] = {t.x, t.y, t.z, t.w};
+        TO* to = out + (size_t)(tok0 + r[h]) * p.ldo + col;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (col + i < p.feats) to[i] = from_float<TO>(f[i] + (bias ? bias[col + i] : 0.f));
+      }
     }
+    // (what the others have here has been read before it is used; the stores need not have arrived)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  if (CG == 2 || EPI == G8_SHARED) g8_cluster_sync();
+  if (CG == 2) g8_cluster_sync();
   if (warp == G8_EPI_WARPS + 1) {
     tc_fence_after();
     if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"((unsigned)G8_COLS) : "memory");
