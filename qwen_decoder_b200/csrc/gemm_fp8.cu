@@ -842,30 +842,30 @@ extern "C" int qd_gemm_fp8_clusters(int n, int sms) { return n >= 1 && n <= 8 ? 
 // The one of the least estimate, in clocks of 1.9 GHz: a worker's rounds over its tiles times its blocks of 128 k, a block being the longest of
 // its MMAs, its bytes into shared memory (70 a clock) and what one costs anyway; W's way from memory, the longer of both and half of the other;
 // an epilogue; a cluster's joining and its CTAs.  Fitted to 6,866 times of 154 shapes (1 to 2,048 tokens, 102 to 20,000 features, 111 to 18,944 of
-// k) in captured graphs on a B200, 6 % rms; the choices take 2.4 % longer than the best of all cuts on average.  Some of them, us, the chosen
+// k) in captured graphs on a B200, 5 % rms; the choices take 2.5 % longer than the best of all cuts on average.  Some of them, us, the chosen
 // one and the best of the other kind (without shares where it has some, one CTA where it has two, and the other way round):
-//   1 x 2,048 x 11,008      1 CTA, 192 rows, 8 shares   9.7   96 rows, 1 share   23.0
-//   23 x 4,608 x 3,584      1 CTA, 192 rows, 4 shares   9.0   64 rows, 1 share    9.9
-//   256 x 3,584 x 18,944    1 CTA, 224 rows, 4 shares  23.8   128 rows, 1 share  35.0
-//   2,048 x 3,584 x 3,584   2 CTAs, 224 rows           23.5   1 CTA, 208 rows    24.2
+//   1 x 2,048 x 11,008      1 CTA, 192 rows, 8 shares   9.2   32 rows, 1 share   23.2
+//   23 x 4,608 x 3,584      1 CTA, 192 rows, 4 shares   8.1   64 rows, 1 share   10.4
+//   256 x 3,584 x 18,944    1 CTA, 224 rows, 4 shares  23.9   64 rows, 1 share   39.4
+//   2,048 x 3,584 x 3,584   2 CTAs, 224 rows           23.6   1 CTA, 224 rows    24.4
 //   2,048 x 3,584 x 18,944  2 CTAs, 224 rows          128.2   1 CTA, 208 rows   134.8   (under the power limit; alone 106.9 and 113.1)
 extern "C" int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out) {
   epi &= 255;
   if (T <= 0 || N <= 0 || K <= 0 || sms < 2) return 0;
   const int kb = up(K, FP8_BLOCK), most = epi == G8_STORE && out_dtype == QD_F32 ? G8_MAX_FLOAT_BN : 256, feats = epi == G8_GATED ? N / 2 : N;
-  const double dram = (double)N * K / 5400.0;
+  const double dram = (double)N * K / 5290.0;
   double best = 0;
   for (int cg = 1; cg <= (T > 128 ? 2 : 1); cg++) {
     const int n_tt = up(T, 128 * cg), mrows = up(up(T, cg * n_tt), 8) * 8;
     for (int bn = epi == G8_GATED ? 256 : 32; bn <= most; bn += cg == 2 ? 32 : 16) {
       const long long tiles = (long long)up(feats, epi == G8_GATED ? bn / 2 : bn) * n_tt;
-      const double block = fmax(fmax(2.4 * bn, (mrows + bn / cg) * 128 / 70.0), cg == 2 ? 560.0 : 490.0);
+      const double block = fmax(fmax(2.37 * bn, (mrows + bn / cg) * 128 / 70.0), cg == 2 ? 542.0 : 486.0);
       for (int splits = 1; splits <= (epi == G8_GATED || cg == 2 || bn % 32 ? 1 : 8) && splits <= kb; splits++) {
         if (splits > 1 && tiles > g8_clusters(splits, sms)) break;
         const long long workers = sms / cg, rounds = splits > 1 ? 1 : (tiles + workers - 1) / workers;
         const double work = (double)rounds * up(kb, splits) * block + (rounds - 1) * 7.7 * bn;
-        double cost = fmax(work, dram) + 0.55 * fmin(work, dram) + (0.18 * mrows + 7.7) * bn;
-        if (splits > 1) cost += 1000.0 + 170.0 * splits + 5100.0 * tiles * splits / sms;
+        double cost = fmax(work, dram) + 0.505 * fmin(work, dram) + (0.214 * mrows + 7.7) * bn;
+        if (splits > 1) cost += 70.0 * splits + 4830.0 * tiles * splits / sms;
         if (best == 0 || cost < best) { best = cost; *cg_out = cg; *bn_out = bn; *splits_out = splits; }
       }
     }

@@ -11,10 +11,10 @@
 // What bounds it: a multiprocessor's 60 clocks to a block for the MMAs and as many for the rest, 4 TB/s; the product on tcgen05
 // (gemm_fp8.cu) reads large matrices at 6 TB/s but has a longer way through barriers, tensor memory and a cluster's joining.  Measured
 // here / there, us, in captured graphs, 1 and 16 tokens:
-//   2,048 x 2,048    2.7 /  5.3    4.0 / 5.8       3,584 x 3,584    5.3 /  7.1    7.6 /  7.6
-//   2,560 x 2,048    3.2 /  5.4    4.3 / 5.9       4,608 x 3,584    5.9 /  7.7    8.0 /  8.2
-//   2,048 x 5,120    5.6 /  7.0    7.7 / 7.6       2,048 x 11,008   8.6 /  9.2   12.2 /  9.8
-//   1,000 x 1,000    2.4 /  4.5    3.1 / 5.2      22,016 x 2,048   13.3 / 10.5   19.6 / 11.8
+//   2,048 x 2,048    3.4 /  4.9    4.2 / 5.1       3,584 x 3,584    5.1 /  6.7    7.0 /  7.0
+//   2,560 x 2,048    3.5 /  5.1    4.5 / 5.4       4,608 x 3,584    5.8 /  7.3    7.3 /  7.5
+//   2,048 x 5,120    5.3 /  6.7    7.3 / 6.9       2,048 x 11,008   8.6 /  9.1   11.8 /  9.4
+//   1,000 x 1,000    2.1 /  4.1    2.6 / 4.3      22,016 x 2,048   13.1 / 10.3   19.2 / 11.3
 //
 // The reference has 16-bit products only (cublasHgemm, gpu_kernels.cu:431-436).
 #include "entry_points.h"
