@@ -82,10 +82,10 @@ __device__ __forceinline__ unsigned long long lp_warp_max(unsigned long long k) 
 }
 
 struct LpShared {
-  unsigned long long joined[LP_MAX_TOP * LP_HITS], sorted[LP_MAX_TOP];
+  unsigned long long joined[LP_MAX_TOP * LP_HITS], sorted[LP_MAX_TOP], nth[LP_MAX_SHARES];
   unsigned peaks[LP_MAX_CHUNKS], least;
   LpSum sum[LP_WARPS], whole;
-  int chosen[LP_MAX_TOP], n_chosen, n_joined, n_sorted;
+  int chosen[LP_MAX_TOP], n_chosen, n_joined;
 };
 
 // Which logit a lane's i-th of 512 from ``at`` on is: whole 16 bytes of a lane side by side, or one by one
@@ -134,9 +134,13 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   int token = -1;
   float its = __uint_as_float(0x7fc00000u);
   if (writes) token = a.tokens[row];
+  float next[LP_EACH];
+  lp_load(next, z, lo * LP_TILE + warp * LP_CHUNK, a.V, a.vec);
   for (int tile = lo; tile < hi; tile++) {
     float v[LP_EACH];
-    lp_load(v, z, tile * LP_TILE + warp * LP_CHUNK, a.V, a.vec);
+#pragma unroll
+    for (int i = 0; i < LP_EACH; i++) v[i] = next[i];
+    if (tile + 1 < hi) lp_load(next, z, (tile + 1) * LP_TILE + warp * LP_CHUNK, a.V, a.vec);
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < LP_EACH; i++) m = fmaxf(m, v[i]);
@@ -175,41 +179,80 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
       for (int j = 0; j < total; j++) before += sh.joined[j] > mine;
       if (before < a.top) sh.sorted[before] = mine;
     }
-    if (threadIdx.x == 0) sh.n_sorted = min(total, a.top);
+    if ((int)threadIdx.x >= total && (int)threadIdx.x < a.top) sh.sorted[threadIdx.x] = 0;
     __syncthreads();
   };
   if (a.top) {
     if (warp == 0) {
-      // the ``top`` largest of the chunks' maxima, a lane's chunks beside one another
+      // the ``top`` largest of the chunks' maxima, a lane's chunks beside one another: bit by bit the largest bound that ``top`` of them reach
       const int chunks = (hi - lo) * LP_WARPS;
-      unsigned peak[LP_LANE], mine = 0, o = 0;
+      unsigned peak[LP_LANE];
+#pragma unroll
+      for (int i = 0; i < LP_LANE; i++) peak[i] = lane * LP_LANE + i < chunks ? sh.peaks[lane * LP_LANE + i] : 0u;
+      const auto reach = [&](unsigned bound) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < LP_LANE; i++) n += peak[i] >= bound;
+        return n;
+      };
+      unsigned high = 0, low = 0xffffffffu;                          // the largest and the least (0: no number)
 #pragma unroll
       for (int i = 0; i < LP_LANE; i++) {
-        peak[i] = lane * LP_LANE + i < chunks ? sh.peaks[lane * LP_LANE + i] : 0u;
-        mine = max(mine, peak[i]);
+        high = max(high, peak[i]);
+        low = min(low, peak[i] - 1u);
       }
-      int k = 0;
-      for (; k < a.top; k++) {
-        const unsigned next = __reduce_max_sync(0xffffffffu, mine);
-        if (!next) break;                                            // (no number in any of the others)
-        o = next;
-        if ((int)__ffs(__ballot_sync(0xffffffffu, mine == o)) - 1 == lane) {
-          int at = LP_LANE;
-#pragma unroll
-          for (int i = LP_LANE - 1; i >= 0; i--)
-            if (peak[i] == o) at = i;
-          mine = 0;
-#pragma unroll
-          for (int i = 0; i < LP_LANE; i++) {
-            if (i == at) peak[i] = 0;
-            mine = max(mine, peak[i]);
-          }
-          sh.chosen[k] = lane * LP_LANE + at;
+      high = __reduce_max_sync(0xffffffffu, high);
+      low = __reduce_min_sync(0xffffffffu, low) + 1u;
+      unsigned bound = low;
+      int all = high ? __reduce_add_sync(0xffffffffu, reach(bound)) : 0, bit = 31 - __clz(high ^ low);
+      if (all > a.top) bound = bit < 0 ? high : high & ~0u << bit << 1;        // (what they begin with alike)
+#pragma unroll 1
+      for (; bit >= 0 && all > a.top; bit--) {
+        const unsigned higher = bound | 1u << bit;
+        const int n = __reduce_add_sync(0xffffffffu, reach(higher));
+        if (n >= a.top) {
+          bound = higher;
+          all = n;
         }
       }
+      // more of them than ``top`` only where some are equal to the bound: the first ones
+      int mine = high ? reach(bound) : 0, spare = all > a.top ? all - a.top : 0, equal = 0;
+      if (spare) {
+#pragma unroll
+        for (int i = 0; i < LP_LANE; i++) equal += peak[i] == bound;
+        int behind = 0;                                              // equal ones of the lanes behind
+        for (int l = 31; l > 0; l--) {
+          const int e = __shfl_sync(0xffffffffu, equal, l);
+          if (lane < l) behind += e;
+        }
+        equal = max(0, min(equal, spare - behind));                  // of this lane's the last so many are not taken
+        mine -= equal;
+      }
+      int at = mine;
+      for (int d = 1; d < 32; d *= 2) {
+        const int n = __shfl_up_sync(0xffffffffu, at, d);
+        if (lane >= d) at += n;
+      }
+      const int n_chosen = __shfl_sync(0xffffffffu, at, 31);
+      at -= mine;
+      unsigned least = 0xffffffffu;
+      int left = equal;
+#pragma unroll
+      for (int i = LP_LANE - 1; i >= 0; i--) {
+        bool take = high && peak[i] >= bound;
+        if (take && left && peak[i] == bound) {
+          left--;
+          take = false;
+        }
+        if (take) {
+          sh.chosen[at++] = lane * LP_LANE + i;
+          least = min(least, peak[i]);
+        }
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
       if (lane == 0) {
-        sh.n_chosen = k;
-        sh.least = k == a.top ? o : 1u;
+        sh.n_chosen = n_chosen;
+        sh.least = n_chosen == a.top ? least : 1u;
       }
     }
     __syncthreads();
@@ -247,9 +290,13 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
         if (lp_order(v[i]) >= least && lp_index<TX>(at, i, a.vec) < a.V) hits |= 1u << i;
       if (__reduce_add_sync(0xffffffffu, __popc(hits)) <= LP_HITS) {
         while (hits) {
-          const int i = __ffs(hits) - 1, k = lp_index<TX>(at, i, a.vec);
+          const int i = __ffs(hits) - 1;
           hits &= hits - 1;
-          sh.joined[atomicAdd(&sh.n_joined, 1)] = lp_key(to_float(z[k]), k);
+          float x = v[0];
+#pragma unroll
+          for (int j = 1; j < LP_EACH; j++)
+            if (j == i) x = v[j];
+          sh.joined[atomicAdd(&sh.n_joined, 1)] = lp_key(x, lp_index<TX>(at, i, a.vec));
         }
       } else {
         // their largest ones, one after the other
@@ -282,19 +329,24 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(base + (unsigned)((const char*)p - (const char*)&sh)), "r"(cta));
         return r;
       };
-      // (a lane to a share: all of their words are on their way together)
-      unsigned long long nth_key = 0;
-      int have = 0;
-      if (warp == 0 && lane < a.shares) {
-        LpSum x;
-        const unsigned from = at(&sh.whole, lane);
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.m) : "r"(from) : "memory");
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.s) : "r"(from + 4) : "memory");
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.d) : "r"(from + 8) : "memory");
-        sum = x;
+      // (a lane to a share, and of the lists warp w those of shares w and w + 8: all that is far is on its way together)
+      unsigned long long key[LP_MAX_SHARES / LP_WARPS];
+#pragma unroll
+      for (int i = 0; i < LP_MAX_SHARES / LP_WARPS; i++) {
+        const int c = warp + i * LP_WARPS;
+        key[i] = 0;
+        if (c < a.shares && lane < a.top) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key[i]) : "r"(at(&sh.sorted[lane], c)) : "memory");
       }
       if (warp == 0) {
-        if (lane >= a.shares) sum = {LP_LOWEST, 0.f, 0.f};
+        sum = {LP_LOWEST, 0.f, 0.f};
+        if (lane < a.shares) {
+          LpSum x;
+          const unsigned from = at(&sh.whole, lane);
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.m) : "r"(from) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.s) : "r"(from + 4) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.d) : "r"(from + 8) : "memory");
+          sum = x;
+        }
         lp_to(sum, lp_value(__reduce_max_sync(0xffffffffu, lp_order(sum.m))));
         whole.m = sum.m;
         whole.s = warp_sum(sum.s);
@@ -302,25 +354,15 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
       }
       if (a.top) {
         const int nth = (a.top + a.shares - 1) / a.shares - 1;
-        if (lane < a.shares) {
-          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(have) : "r"(at(&sh.n_sorted, lane)) : "memory");
-          asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(nth_key) : "r"(at(&sh.sorted[nth], lane)) : "memory");
-          if (nth >= have) nth_key = 0;
-        } else {
-          nth_key = ~0ull;
-        }
-        const unsigned long long bound = ~lp_warp_max(~nth_key);
-        // warp w brings the lists of shares w, w + 8
-        unsigned long long key[LP_MAX_SHARES / LP_WARPS];
 #pragma unroll
         for (int i = 0; i < LP_MAX_SHARES / LP_WARPS; i++) {
-          const int c = warp + i * LP_WARPS, its = __shfl_sync(0xffffffffu, have, c & 31);
-          key[i] = 0;
-          if (c < a.shares && lane < its) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key[i]) : "r"(at(&sh.sorted[lane], c)) : "memory");
+          const int c = warp + i * LP_WARPS;
+          const unsigned long long of = __shfl_sync(0xffffffffu, key[i], nth);
+          if (lane == 0) sh.nth[c] = c < a.shares ? of : ~0ull;
         }
-        __syncthreads();
         if (threadIdx.x == 0) sh.n_joined = 0;
         __syncthreads();
+        const unsigned long long bound = ~lp_warp_max(lane < LP_MAX_SHARES ? ~sh.nth[lane] : 0ull);
 #pragma unroll
         for (int i = 0; i < LP_MAX_SHARES / LP_WARPS; i++)
           if (key[i] && key[i] >= bound) sh.joined[atomicAdd(&sh.n_joined, 1)] = key[i];
@@ -331,7 +373,6 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
     if (share) return;
   }
   if (warp) return;
-  const int n = a.top ? sh.n_sorted : 0;
   const float log_s = logf(whole.s);
   // (a row of minus infinities alone has no probabilities: none is above 0)
   auto log_p = [&](float x) { return whole.s == 0.f ? -INFINITY : x - whole.m - log_s; };
@@ -340,8 +381,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
     a.entropy[row] = whole.s == 0.f ? 0.f : log_s - LP_LN2 * (whole.d / whole.s);
   }
   if ((int)threadIdx.x < a.top) {
-    const bool there = (int)threadIdx.x < n;
-    const unsigned long long key = there ? sh.sorted[threadIdx.x] : 0;
+    const unsigned long long key = sh.sorted[threadIdx.x];
+    const bool there = key != 0;
     a.top_ids[(size_t)row * a.top + threadIdx.x] = there ? (int)(0xffffffffu - (unsigned)key) : -1;
     a.top_logprobs[(size_t)row * a.top + threadIdx.x] = there ? log_p(lp_value((unsigned)(key >> 32))) : __uint_as_float(0x7fc00000u);
   }
