@@ -117,6 +117,65 @@ __device__ __forceinline__ void lp_load(float (&v)[LP_EACH], const TX* z, int at
   }
 }
 
+// A warp finds the ``top`` largest of up to 32 N chunks' maxima, of equal ones the first: bit by bit the largest bound that ``top`` of
+// them reach
+template <int N>
+__device__ __forceinline__ void lp_choose(LpShared& sh, int chunks, int top) {
+  const int lane = threadIdx.x & 31;
+  unsigned peak[N], high = 0, low = 0xffffffffu;                     // the largest and the least (0: no number)
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    peak[i] = 32 * i + lane < chunks ? sh.peaks[32 * i + lane] : 0u;
+    high = max(high, peak[i]);
+    low = min(low, peak[i] - 1u);
+  }
+  high = __reduce_max_sync(0xffffffffu, high);
+  low = __reduce_min_sync(0xffffffffu, low) + 1u;
+  const auto reach = [&](unsigned bound) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) n += peak[i] >= bound;
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  unsigned bound = high ? low : 1u;
+  int all = reach(bound), bit = 31 - __clz(high ^ low);
+  if (all > top) bound = bit < 0 ? high : high & ~0u << bit << 1;    // (what they begin with alike)
+#pragma unroll 1
+  for (; bit >= 0 && all > top; bit--) {
+    const unsigned higher = bound | 1u << bit;
+    const int n = reach(higher);
+    if (n >= top) {
+      bound = higher;
+      all = n;
+    }
+  }
+  // (more of them than ``top`` only where some are equal to the bound)
+  int taken = 0, above = 0;
+  if (all > top) above = reach(bound + 1u);
+  unsigned least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const bool over = peak[i] > bound, equal = peak[i] == bound;
+    unsigned take = __ballot_sync(0xffffffffu, over || equal);
+    if (all > top) {
+      const unsigned equals = __ballot_sync(0xffffffffu, equal);
+      const int before = __popc(equals & ((1u << lane) - 1u));
+      take = __ballot_sync(0xffffffffu, over || (equal && above + before < top));
+      above += __popc(equals);
+    }
+    if (take >> lane & 1) {
+      sh.chosen[taken + __popc(take & ((1u << lane) - 1u))] = 32 * i + lane;
+      least = min(least, peak[i]);
+    }
+    taken += __popc(take);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (lane == 0) {
+    sh.n_chosen = taken;
+    sh.least = taken == top ? least : 1u;
+  }
+}
+
 template <typename TX>
 __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a) {
   __shared__ LpShared sh;
@@ -184,76 +243,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   };
   if (a.top) {
     if (warp == 0) {
-      // the ``top`` largest of the chunks' maxima, a lane's chunks beside one another: bit by bit the largest bound that ``top`` of them reach
-      const int chunks = (hi - lo) * LP_WARPS;
-      unsigned peak[LP_LANE];
-#pragma unroll
-      for (int i = 0; i < LP_LANE; i++) peak[i] = lane * LP_LANE + i < chunks ? sh.peaks[lane * LP_LANE + i] : 0u;
-      const auto reach = [&](unsigned bound) {
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < LP_LANE; i++) n += peak[i] >= bound;
-        return n;
-      };
-      unsigned high = 0, low = 0xffffffffu;                          // the largest and the least (0: no number)
-#pragma unroll
-      for (int i = 0; i < LP_LANE; i++) {
-        high = max(high, peak[i]);
-        low = min(low, peak[i] - 1u);
-      }
-      high = __reduce_max_sync(0xffffffffu, high);
-      low = __reduce_min_sync(0xffffffffu, low) + 1u;
-      unsigned bound = low;
-      int all = high ? __reduce_add_sync(0xffffffffu, reach(bound)) : 0, bit = 31 - __clz(high ^ low);
-      if (all > a.top) bound = bit < 0 ? high : high & ~0u << bit << 1;        // (what they begin with alike)
-#pragma unroll 1
-      for (; bit >= 0 && all > a.top; bit--) {
-        const unsigned higher = bound | 1u << bit;
-        const int n = __reduce_add_sync(0xffffffffu, reach(higher));
-        if (n >= a.top) {
-          bound = higher;
-          all = n;
-        }
-      }
-      // more of them than ``top`` only where some are equal to the bound: the first ones
-      int mine = high ? reach(bound) : 0, spare = all > a.top ? all - a.top : 0, equal = 0;
-      if (spare) {
-#pragma unroll
-        for (int i = 0; i < LP_LANE; i++) equal += peak[i] == bound;
-        int behind = 0;                                              // equal ones of the lanes behind
-        for (int l = 31; l > 0; l--) {
-          const int e = __shfl_sync(0xffffffffu, equal, l);
-          if (lane < l) behind += e;
-        }
-        equal = max(0, min(equal, spare - behind));                  // of this lane's the last so many are not taken
-        mine -= equal;
-      }
-      int at = mine;
-      for (int d = 1; d < 32; d *= 2) {
-        const int n = __shfl_up_sync(0xffffffffu, at, d);
-        if (lane >= d) at += n;
-      }
-      const int n_chosen = __shfl_sync(0xffffffffu, at, 31);
-      at -= mine;
-      unsigned least = 0xffffffffu;
-      int left = equal;
-#pragma unroll
-      for (int i = LP_LANE - 1; i >= 0; i--) {
-        bool take = high && peak[i] >= bound;
-        if (take && left && peak[i] == bound) {
-          left--;
-          take = false;
-        }
-        if (take) {
-          sh.chosen[at++] = lane * LP_LANE + i;
-          least = min(least, peak[i]);
-        }
-      }
-      least = __reduce_min_sync(0xffffffffu, least);
-      if (lane == 0) {
-        sh.n_chosen = n_chosen;
-        sh.least = n_chosen == a.top ? least : 1u;
-      }
+      if ((hi - lo) * LP_WARPS <= 128) lp_choose<4>(sh, (hi - lo) * LP_WARPS, a.top);
+      else lp_choose<LP_LANE>(sh, (hi - lo) * LP_WARPS, a.top);
     }
     __syncthreads();
     if (sh.n_chosen < a.top) {
