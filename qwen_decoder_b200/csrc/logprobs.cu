@@ -270,15 +270,19 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
       }
       __syncthreads();
     }
-    const unsigned least = sh.least;
-    for (int c = warp; c < sh.n_chosen; c += LP_WARPS) {
+    const float least = sh.least > lp_order(-INFINITY) ? lp_value(sh.least) : -INFINITY;
+    const int n_chosen = sh.n_chosen;
+    if (warp < n_chosen) lp_load(next, z, lo * LP_TILE + sh.chosen[warp] * LP_CHUNK, a.V, a.vec);
+    for (int c = warp; c < n_chosen; c += LP_WARPS) {
       const int at = lo * LP_TILE + sh.chosen[c] * LP_CHUNK;
       float v[LP_EACH];
-      lp_load(v, z, at, a.V, a.vec);
+#pragma unroll
+      for (int i = 0; i < LP_EACH; i++) v[i] = next[i];
+      if (c + LP_WARPS < n_chosen) lp_load(next, z, lo * LP_TILE + sh.chosen[c + LP_WARPS] * LP_CHUNK, a.V, a.vec);
       unsigned hits = 0;
 #pragma unroll
       for (int i = 0; i < LP_EACH; i++)
-        if (lp_order(v[i]) >= least && lp_index<TX>(at, i, a.vec) < a.V) hits |= 1u << i;
+        if (v[i] >= least && lp_index<TX>(at, i, a.vec) < a.V) hits |= 1u << i;
       if (__reduce_add_sync(0xffffffffu, __popc(hits)) <= LP_HITS) {
         while (hits) {
           const int i = __ffs(hits) - 1;
