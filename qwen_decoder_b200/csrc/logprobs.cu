@@ -383,6 +383,27 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   }
 }
 
+// How many clusters of ``n`` CTAs run at a time
+static int lp_clusters(int n, int sms) {
+  static int known[LP_MAX_SHARES + 1];
+  if (known[n]) return known[n];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n * 1024);
+  cfg.blockDim = dim3(LP_THREADS);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = n;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int got = 0;
+  if (cudaOccupancyMaxActiveClusters(&got, logprobs_kernel<float>, &cfg) != cudaSuccess || got < 1) {
+    (void)cudaGetLastError();
+    got = 3 * sms / n;
+  }
+  return known[n] = got;
+}
+
 // logits [R, V] float32 or bfloat16, rows ``ld`` elements apart; tokens int32 [R] (outside of [0, V): the log probability NaN); logprob and
 // entropy float32 [R]; top_ids int32 and top_logprobs float32 [R, top], top up to 32, of rows with fewer numbers -1 and NaN.
 extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob, float* entropy,
@@ -395,13 +416,25 @@ extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, co
   a.R = R; a.V = V; a.top = top; a.ld = ld;
   const int size = dtype == QD_F32 ? 4 : 2;
   a.vec = !((uintptr_t)logits & 15) && ld * size % 16 == 0;
-  // As many CTAs to a row as run at a time, four to a multiprocessor, with four tiles and half again as many chunks as ``top`` to each.
-  // Measured, us: 64 rows of 152,064 with 4, 8 and 16 17.3, 14.3 and 27.6, 148 rows of 32,000 with 1, 2 and 4 11.2, 10.9 and 16.0.
+  // clusters of more than 8 are asked for once
+  static bool allowed[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QD_ERR_UNSUPPORTED;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(logprobs_kernel<float>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaFuncSetAttribute(logprobs_kernel<bf16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return (int)cudaGetLastError();
+    allowed[dev] = true;
+  }
+  // As many CTAs to a row as run at a time, with four tiles and half again as many chunks as ``top`` to each, or two tiles where they leave a third
+  // of the places free.  Measured, us, top 5: 64 rows of 152,064 with 4 and 8 16.8 and 13.4, 148 rows with 2 and 4 (some of whose clusters
+  // wait) 24.7 and 30.9; 8 rows of 32,000 with 2 and 4 7.2 and 6.4, 110 rows 9.5 and 11.1.
   const int tiles = (V + LP_TILE - 1) / LP_TILE;
   a.shares = 1;
-  while (a.shares < LP_MAX_SHARES && (long long)R * a.shares * 2 <= 4ll * sms && tiles / (a.shares * 2) >= 4 &&
-         2 * (tiles / (a.shares * 2)) * LP_WARPS >= 3 * top)
-    a.shares *= 2;
+  for (int n = 2; n <= LP_MAX_SHARES && tiles / n >= 2 && 2 * (tiles / n) * LP_WARPS >= 3 * top; n *= 2) {
+    if (tiles / n >= 4 ? R > lp_clusters(n, sms) : 2ll * R * n > 5ll * sms) break;
+    a.shares = n;
+  }
   while (a.shares * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE < V) a.shares++;      // a CTA keeps so many maxima
   if ((long long)R * a.shares > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
@@ -416,16 +449,6 @@ extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, co
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = qd_pdl_enabled() ? 2 : 1;
-  // clusters of more than 8 are asked for once
-  static bool allowed[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QD_ERR_UNSUPPORTED;
-  if (!allowed[dev]) {
-    if (cudaFuncSetAttribute(logprobs_kernel<float>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-        cudaFuncSetAttribute(logprobs_kernel<bf16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return (int)cudaGetLastError();
-    allowed[dev] = true;
-  }
   if (dtype == QD_F32) cudaLaunchKernelEx(&cfg, logprobs_kernel<float>, a);
   else cudaLaunchKernelEx(&cfg, logprobs_kernel<bf16>, a);
   return qd_last_error();
