@@ -14,7 +14,7 @@
 // chosen has one that comes before all of theirs.  They are read again (20 of 2 KB of a row of 600), and what reaches the least of the chosen
 // maxima is put in order by counting for each key how many are larger.  Where more than LP_HITS of 512 do (a thousand equal logits, a mask that
 // leaves fewer than ``top``), their largest ``top`` are taken one by one.  (With lists that grew while the row was read, 509 rows of 152,064
-// took 80 us with one to a CTA and a barrier to every tile, 131 with one to a warp; 52 without any.)
+// took 80 us with one to a CTA and a barrier to every tile, 131 with one to a warp; so they take 56, and 48 without any.)
 // Of sorted lists of several CTAs the keys that count are those not below the least of the L lists' ceil(top / L)-th keys, which ``top`` keys
 // reach.
 //
