@@ -428,11 +428,12 @@ extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, co
   }
   // As many CTAs to a row as run at a time, with four tiles and half again as many chunks as ``top`` to each, or two tiles where they leave a third
   // of the places free.  Measured, us, top 5: 64 rows of 152,064 with 4 and 8 16.8 and 13.4, 148 rows with 2 and 4 (some of whose clusters
-  // wait) 24.7 and 30.9; 8 rows of 32,000 with 2 and 4 7.2 and 6.4, 110 rows 9.5 and 11.1.
+  // wait) 24.7 and 30.9; 8 rows of 32,000 with 2 and 4 7.2 and 6.4, 110 rows 9.5 and 11.1; 8 rows of 151,936 with 8 and 16 7.9 and 8.6 in L2,
+  // as the product over the vocabulary leaves them, 9.1 and 9.2 from memory.
   const int tiles = (V + LP_TILE - 1) / LP_TILE;
   a.shares = 1;
   for (int n = 2; n <= LP_MAX_SHARES && tiles / n >= 2 && 2 * (tiles / n) * LP_WARPS >= 3 * top; n *= 2) {
-    if (tiles / n >= 4 ? R > lp_clusters(n, sms) : 2ll * R * n > 5ll * sms) break;
+    if (tiles / n >= 4 ? R > lp_clusters(n, sms) : n > 8 || 2ll * R * n > 5ll * sms) break;
     a.shares = n;
   }
   while (a.shares * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE < V) a.shares++;      // a CTA keeps so many maxima
