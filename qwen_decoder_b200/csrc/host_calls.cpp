@@ -1,6 +1,6 @@
 // The host's side of the operators in 8 bits and of the log probabilities: their arguments' checks, room for their results and the call of
-// their launchers, as a Python module.  A decode step replays as a graph, but a prompt's step is launched call by call, and from Python a
-// call's checks, two torch.empty and some twenty arguments through ctypes took 13 to 17 us where the device needs 2 to 10; so it takes 5 to 7.
+// their launchers, as a Python module.  Decode steps replay as graphs and prompts' are launched by prompt_exec.cu, but any other call has its checks,
+// two torch.empty and some twenty arguments through ctypes: from Python 13 to 17 us where the device needs 2 to 10, so 5 to 7.
 //
 // The launchers are those of the kernel libraries, whose addresses ``resolve`` gives (a library is built and loaded when the first call needs
 // it); refusals are raised as the package's KernelError before anything is launched.
