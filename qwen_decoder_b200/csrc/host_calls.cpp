@@ -272,7 +272,8 @@ CALL(add_rmsnorm_fp8, 8)
   const double eps = PyFloat_AsDouble(a[4]);
   const int write_back = PyObject_IsTrue(a[6]);
   if (PyErr_Occurred()) throw PythonError{};
-  if (x.scalar_type() != at::kFloat || x.dim() != 2 || x.size(1) != r.K || !x.is_contiguous()) refuse("add_rmsnorm_fp8: x must be contiguous float32 [T, ", r.K, "]");
+  if (x.scalar_type() != at::kFloat || x.dim() != 2 || x.size(1) != r.K || !x.is_contiguous())
+    refuse("add_rmsnorm_fp8: x must be contiguous float32 [T, ", r.K, "]");
   const int64_t T = x.size(0);
   vector_of(&weight, r.K, "add_rmsnorm_fp8", "weight");
   vector_of(scale, r.K, "add_rmsnorm_fp8", "delta_scale");
