@@ -29,6 +29,12 @@ __device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return (unsigned)lo | (unsigned)hi << 16;
 }
+// an e4m3 number
+__device__ __forceinline__ float fp8_value(unsigned byte) {
+  unsigned h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)byte));
+  return __half2float(__ushort_as_half((unsigned short)h));
+}
 // act(g) u, the quotient and the exponential within 2^-20.  A gate of minus infinity goes as the largest finite one does, to zero.
 __device__ __forceinline__ float fp8_gated(float g, float u, int act) {
   float r;

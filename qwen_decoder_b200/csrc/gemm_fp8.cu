@@ -57,7 +57,9 @@ struct G8Params {
   long long ldo;           // elements
   const unsigned char *sx, *sw;
   long long ldsx, ldsw;
-  unsigned char* s_out;    // of the gated product
+  const unsigned char *x, *w;      // of the gated product, as what follows
+  long long ldx, ldw;
+  unsigned char* s_out;
   long long lds_out;
 };
 
@@ -218,6 +220,38 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
   }
 }
 
+// Where a block's largest magnitude is so near the last one of a scale that the sums' cut-off decides, its sums are made again at the kernel's
+// end: a scale is then that of the sums as they are, not of the order of their additions.  (Without it 1 to 4 of a million blocks had the
+// other scale, K 2,048 to 11,008; some 35 of a million are looked at for K 3,584, 1 to 2 us each where the kernel ends with one.  Looked at in
+// the epilogue itself they made its code so long that products of 8 to 512 tokens took 3 to 15 % more; this way 0 to 3.)  How near is in units of
+// the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by 0.36 in sums of numbers of one sign, in the
+// gate's sum and in up's, and the activation's own error.
+#define G8_NEAR 128                           // blocks of a CTA that are looked at; with more of them none is
+__device__ __forceinline__ bool g8_near(unsigned peak, int K) {
+  const int off = (int)(peak & 0x7fffffu) - 0x600000;
+  return peak >= 10u << 23 && peak < 0x7f800000u && abs(off) <= min((int)(3ll * K >> 6) + 16, 0xfffff);
+}
+// 8 e4m3 numbers of a row, zeros behind its end
+__device__ __forceinline__ void g8_eight(float (&v)[8], const unsigned char* from, int there) {
+  uint2 raw = make_uint2(0, 0);
+  if (there >= 8) {
+    raw = *reinterpret_cast<const uint2*>(from);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < there; i++) (i < 4 ? raw.x : raw.y) |= (unsigned)from[i] << 8 * (i & 3);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    unsigned h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)((i < 2 ? raw.x : raw.y) >> 16 * (i & 1))));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+// 2^(a + b) of two scales' bytes
+__device__ __forceinline__ double g8_scaled(unsigned a, unsigned b) { return __longlong_as_double((long long)(a + b - 254 + 1023) << 52); }
+
 template <int ACT>
 struct G8Act { static constexpr int value = ACT; };
 
@@ -228,7 +262,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_ready[2], acc_free[2], scales_full[G8_BUFFERS], scales_empty[G8_BUFFERS];
   __shared__ unsigned tmem_slot, peaks[4][2][32], scales[G8_WORDS][384];
-  __shared__ int dead;
+  __shared__ int dead, n_near;
+  __shared__ unsigned near_rows[EPI == G8_GATED ? G8_NEAR : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)g8_rank() : 0;
   const int share = EPI == G8_SHARED ? (int)g8_rank() : 0;
@@ -239,7 +274,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   unsigned char* a_s = base;
   unsigned char* b_s = base + (size_t)p.stages * a_bytes;
   if (threadIdx.x == 0) {
-    dead = 0;
+    dead = n_near = 0;
     for (int s = 0; s < p.stages; s++) { tc_bar_init(&full[s], 1); tc_bar_init(&empty[s], 1); }
     for (int b = 0; b < 2; b++) {
       tc_bar_init(&acc_ready[b], 1);
@@ -481,6 +516,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         *reinterpret_cast<float4*>(base + (size_t)(quarter + lane) * p.bn * 4 + ((4 * g + e ^ (lane & 7)) << 4)) =
             make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
     };
+    // a row of the item's tile whose scale is to be looked at
+    auto look_at = [&](int item, int r) {
+      const int at = atomicAdd(&n_near, 1);
+      if (at < G8_NEAR) near_rows[at] = (unsigned)item << 7 | r;
+    };
     int n = 0;
     auto wait_sum = [&]() {
       if (!tc_wait(&acc_ready[n & 1], n >> 1 & 1, &dead, 64) && lane == 0) atomicExch(status, 4);
@@ -579,7 +619,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                   if (col + e >= p.feats) g[e] = 0.f;
 #pragma unroll
               for (int e = 0; e < 4; e++) peak = fp8_peak(peak, g[e]);
-              const unsigned byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));
+              const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(peak)), byte = fp8_scale_byte(most);
+              if (lane == 0 && g8_near(most, p.K)) look_at(item, r);
               const float inv = fp8_inverse(byte);
               const unsigned w = fp8_pack4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
               unsigned char* to = (unsigned char*)out + (size_t)(row_x(q) + r) * p.ldo + col;
@@ -628,7 +669,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             else gate(G8Act<QD_ACT_SILU>());
             peaks[warp & 3][side][lane] = __float_as_uint(peak);
             asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
-            const unsigned byte = fp8_scale_byte(max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]));
+            const unsigned most = max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]), byte = fp8_scale_byte(most);
+            if (side == 0 && lane < n_rows && g8_near(most, p.K)) look_at(item, quarter + lane);
             const float inv = fp8_inverse(byte);
 #pragma unroll 1
             for (int c = 0; c < 4; c++) {
@@ -661,7 +703,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           for (int e = 0; e < 64; e++) peak = fp8_peak(peak, h[e]);
           peaks[warp & 3][side][lane] = __float_as_uint(peak);
           asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
-          const unsigned byte = fp8_scale_byte(max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]));
+          const unsigned most = max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]), byte = fp8_scale_byte(most);
+          if (side == 0 && lane < n_rows && g8_near(most, p.K)) look_at(item, quarter + lane);
           const float inv = fp8_inverse(byte);
           __syncwarp();
 #pragma unroll
@@ -712,6 +755,80 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (EPI == G8_GATED) {
+    // (the whole CTA: a thread to 8 of k)
+    double (*sums)[2] = reinterpret_cast<double (*)[2]>(base);
+    const int looked = n_near <= G8_NEAR && n_items <= 1 << 25 ? n_near : 0;
+#pragma unroll 1
+    for (int i = 0; i < looked; i++) {
+      const G8Item q = g8_item(p, near_rows[i] >> 7, 0);
+      const long long row = row_x(q) + (int)(near_rows[i] & 127);
+      const int col = q.ft * 128 + 4 * lane, there = min(4, p.feats - col);
+      unsigned char *to = (unsigned char*)out + row * p.ldo + col, *scale = p.s_out + row * p.lds_out + q.ft;
+      float v[4];
+      unsigned most = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        v[e] = e < there ? fp8_value(to[e]) : 0.f;
+        most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      // The scale is the one of at most 448, or twice that.  Those that count are the largest of the rounded ones; the edge is 448 of the lower.
+      const bool higher = most < __float_as_uint(400.f);
+      const unsigned low = *scale - higher, edge = (low + 8) << 23 | 0x600000u;
+      bool over = false;
+#pragma unroll 1
+      for (int e = 0; e < 4 && !over; e++) {
+        const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+#pragma unroll 1
+        for (unsigned c = __ballot_sync(0xffffffffu, (__float_as_uint(of) & 0x7fffffffu) == most); c && !over; c &= c - 1) {
+          const long long g = q.ft * 128 + 4 * (__ffs(c) - 1) + e, u = p.feats + g;
+          double tg = 0.0, tu = 0.0;
+#pragma unroll 1
+          for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
+            float a[8], b[8], d[8], sg = 0.f, su = 0.f;
+            g8_eight(a, p.x + row * p.ldx + k, p.K - k);
+            g8_eight(b, p.w + g * p.ldw + k, p.K - k);
+            g8_eight(d, p.w + u * p.ldw + k, p.K - k);
+            const int block = k >> 7;
+            const unsigned sx = p.sx[row * p.ldsx + block];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              sg = fmaf(a[j], b[j], sg);
+              su = fmaf(a[j], d[j], su);
+            }
+            tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
+            tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
+          }
+          for (int d = 16; d; d >>= 1) {
+            tg += __shfl_xor_sync(0xffffffffu, tg, d);
+            tu += __shfl_xor_sync(0xffffffffu, tu, d);
+          }
+          __syncthreads();                                   // (what the sums before were is no longer read)
+          if (lane == 0) {
+            sums[warp][0] = tg;
+            sums[warp][1] = tu;
+          }
+          __syncthreads();
+          tg = bias ? bias[g] : 0.f;
+          tu = bias ? bias[u] : 0.f;
+#pragma unroll 1
+          for (int j = 0; j < G8_THREADS / 32; j++) {
+            tg += sums[j][0];
+            tu += sums[j][1];
+          }
+          over = (__float_as_uint(fp8_gated((float)tg, (float)tu, p.act)) & 0x7fffffffu) > edge;
+        }
+      }
+      __syncthreads();                                       // all have read the row
+      if (warp == 0 && over != higher) {
+        const float by = over ? 0.5f : 2.f;
+        const unsigned w = fp8_pack4(v[0] * by, v[1] * by, v[2] * by, v[3] * by);
+        for (int e = 0; e < there; e++) to[e] = (unsigned char)(w >> 8 * e);
+        if (lane == 0) *scale = (unsigned char)(low + over);
+      }
+    }
+  }
   if constexpr (EPI == G8_SHARED) {
     g8_cluster_sync();
     // this CTA's share of the tile's rows, summed in the order of the shares of K: up to 32 pieces of four features of a row to a warp, two
@@ -908,6 +1025,7 @@ extern "C" int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long lo
   G8Params p;
   p.act = act; p.resident = resident; p.T = T; p.N = N; p.K = K; p.bn = bn; p.splits = splits; p.ldo = ldo;
   p.sx = (const unsigned char*)sx; p.sw = (const unsigned char*)sw; p.ldsx = ldsx; p.ldsw = ldsw;
+  p.x = (const unsigned char*)X; p.w = (const unsigned char*)W; p.ldx = ldx; p.ldw = ldw;
   p.s_out = (unsigned char*)s_out; p.lds_out = lds_out;
   p.kb_total = up(K, FP8_BLOCK);
   if (ldsx < p.kb_total || ldsw < p.kb_total) return QD_ERR_UNSUPPORTED;

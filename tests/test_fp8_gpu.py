@@ -249,6 +249,40 @@ def test_gated_product(T, F, K, bias, act):
     kernels.check_status()
 
 
+@pytest.mark.parametrize("act", [0, 2])
+@pytest.mark.parametrize("T,plan", [(1, None), (9, None), (30, (1, 256, 1)), (90, (1, 256, 1)), (200, (1, 256, 1)), (200, (2, 256, 1))])
+def test_gated_scales_are_of_the_sums_as_they_are(T, plan, act):
+    """Largest magnitudes a few millionths off where the scale doubles, of sums that the tensor cores cut off by as much.  The activation of a
+    large gate is the gate; roundings of the gate, of up, of their product and of the quotient are 5 times 2^-24 at most."""
+    from qwen_decoder_b200 import kernels
+    K, blocks = 8192, 40
+    F = 128 * blocks
+    g = generator(T, K, act)
+    x = rows_of(numbers((1, K), g, spread=5).abs().expand(T, K).contiguous())
+    w = torch.zeros((2 * F, K), device=DEV)
+    at = torch.randint(0, 128, (blocks,), generator=g, device=DEV) + 128 * torch.arange(blocks, device=DEV)      # the feature that counts
+    w[at] = numbers((blocks, K), g, spread=5).abs() * 64 / K
+    w[at + F] = numbers((blocks, K), g, spread=5).abs() * 64 / K
+    w = rows_of(w)
+    z = (value(x)[:1] @ value(w).T)[0]
+    gate, up = z[at], z[at + F]
+    # biases that bring up to where the product is so many millionths beyond 1.75 times a power of two
+    off = torch.linspace(-4e-6, 4e-6, blocks, device=DEV, dtype=torch.float64)
+    bias = torch.zeros(2 * F, device=DEV)
+    bias[at] = torch.clamp(30 - gate, min=0).float()
+    gate = gate + bias[at].double()
+    edge = 1.75 * torch.exp2(torch.floor(torch.log2(gate * up / 1.75)))
+    bias[at + F] = (edge * (1 + off) / gate - up).float()
+    h = gate * (up + bias[at + F].double())
+    far = (h / edge - 1).abs() > 5 * 2.0 ** -24
+    assert far.sum() > 30
+    out = room(T, F)
+    kernels.gemm_fp8_gated(x, w, bias, out, act, plan)
+    s = out.s.float().double()
+    assert (s == torch.where(h > edge, 2 * edge / 448, edge / 448))[:, far].all()
+    kernels.check_status()
+
+
 def test_few_tokens_and_several_tiles_to_a_cta():
     from qwen_decoder_b200 import kernels
     for T in (1, 8, 13):
