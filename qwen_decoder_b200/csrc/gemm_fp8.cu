@@ -57,7 +57,8 @@ struct G8Params {
   long long ldo;           // elements
   const unsigned char *sx, *sw;
   long long ldsx, ldsw;
-  const unsigned char *x, *w;      // of the gated product, as what follows
+  int doubt;               // of the gated product, as what follows
+  const unsigned char *x, *w;
   long long ldx, ldw;
   unsigned char* s_out;
   long long lds_out;
@@ -222,14 +223,15 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
 
 // Where a block's largest magnitude is so near the last one of a scale that the sums' cut-off decides, its sums are made again at the kernel's
 // end: a scale is then that of the sums as they are, not of the order of their additions.  (Without it 1 to 4 of a million blocks had the
-// other scale, K 2,048 to 11,008; some 35 of a million are looked at for K 3,584, 1 to 2 us each where the kernel ends with one.  Looked at in
-// the epilogue itself they made its code so long that products of 8 to 512 tokens took 3 to 15 % more; this way 0 to 3.)  How near is in units of
-// the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by 0.36 in sums of numbers of one sign, in the
-// gate's sum and in up's, and the activation's own error.
+// other scale, K 2,048 to 11,008; some 25 of a million are looked at for K 3,584, 1 to 2 us each where the kernel ends with one: a layer of 8
+// tokens of the 7B sizes 56.6 -> 57.3 us.  Looked at in the epilogue itself they made its code so long that products of 8 to 512 tokens took 3
+// to 15 % more.)  How near is in units of the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by up to 0.2
+// in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error.
 #define G8_NEAR 128                           // blocks of a CTA that are looked at; with more of them none is
-__device__ __forceinline__ bool g8_near(unsigned peak, int K) {
+static int g8_doubt(int K) { return K < 1 << 24 ? (K >> 5) + 16 : 0xfffff; }
+__device__ __forceinline__ bool g8_near(unsigned peak, int doubt) {
   const int off = (int)(peak & 0x7fffffu) - 0x600000;
-  return peak >= 10u << 23 && peak < 0x7f800000u && abs(off) <= min((int)(3ll * K >> 6) + 16, 0xfffff);
+  return peak >= 10u << 23 && peak < 0x7f800000u && abs(off) <= doubt;
 }
 // 8 e4m3 numbers of a row, zeros behind its end
 __device__ __forceinline__ void g8_eight(float (&v)[8], const unsigned char* from, int there) {
@@ -620,7 +622,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
               for (int e = 0; e < 4; e++) peak = fp8_peak(peak, g[e]);
               const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(peak)), byte = fp8_scale_byte(most);
-              if (lane == 0 && g8_near(most, p.K)) look_at(item, r);
+              if (lane == 0 && g8_near(most, p.doubt)) look_at(item, r);
               const float inv = fp8_inverse(byte);
               const unsigned w = fp8_pack4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
               unsigned char* to = (unsigned char*)out + (size_t)(row_x(q) + r) * p.ldo + col;
@@ -670,7 +672,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             peaks[warp & 3][side][lane] = __float_as_uint(peak);
             asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
             const unsigned most = max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]), byte = fp8_scale_byte(most);
-            if (side == 0 && lane < n_rows && g8_near(most, p.K)) look_at(item, quarter + lane);
+            if (side == 0 && lane < n_rows && g8_near(most, p.doubt)) look_at(item, quarter + lane);
             const float inv = fp8_inverse(byte);
 #pragma unroll 1
             for (int c = 0; c < 4; c++) {
@@ -704,7 +706,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           peaks[warp & 3][side][lane] = __float_as_uint(peak);
           asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
           const unsigned most = max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]), byte = fp8_scale_byte(most);
-          if (side == 0 && lane < n_rows && g8_near(most, p.K)) look_at(item, quarter + lane);
+          if (side == 0 && lane < n_rows && g8_near(most, p.doubt)) look_at(item, quarter + lane);
           const float inv = fp8_inverse(byte);
           __syncwarp();
 #pragma unroll
@@ -755,6 +757,58 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (EPI == G8_SHARED) {
+    g8_cluster_sync();
+    // this CTA's share of the tile's rows, summed in the order of the shares of K: up to 32 pieces of four features of a row to a warp, two
+    // times that on their way together
+    const G8Item q = g8_item(p, worker, share);
+    const int tok0 = q.tt * p.mrows, n_rows = min(p.mrows, p.T - tok0), pieces = p.bn >> 2, wide = pieces > 32;
+    const int r0 = n_rows * share / p.splits, units = (n_rows * (share + 1) / p.splits - r0) << wide;
+    const unsigned at = tc_smem(base);
+    constexpr int WARPS = G8_THREADS / 32;
+#pragma unroll 1
+    for (int u0 = warp; u0 < units; u0 += 2 * WARPS) {
+      float4 v[2][8];
+      int r[2], c[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int u = u0 + h * WARPS;
+        r[h] = r0 + (u >> wide);
+        c[h] = u < units ? (wide ? (u & 1) * 32 : 0) + lane : pieces;
+        const unsigned from = at + (r[h] * pieces + (c[h] ^ (r[h] & 7))) * 16;
+#pragma unroll
+        for (int sp = 0; sp < 8; sp++)
+          if (sp < p.splits && c[h] < pieces) {
+            unsigned remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(from), "r"(sp));
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[h][sp].x), "=f"(v[h][sp].y), "=f"(v[h][sp].z), "=f"(v[h][sp].w) : "r"(remote) : "memory");
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (c[h] >= pieces) break;
+        float4 t = v[h][0];
+#pragma unroll
+        for (int sp = 1; sp < 8; sp++)
+          if (sp < p.splits) { t.x += v[h][sp].x; t.y += v[h][sp].y; t.z += v[h][sp].z; t.w += v[h][sp].w; }
+        const int col = q.ft * p.bn + 4 * c[h];
+        const float f[4] = {t.x, t.y, t.z, t.w};
+        TO* to = out + (size_t)(tok0 + r[h]) * p.ldo + col;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (col + i < p.feats) to[i] = from_float<TO>(f[i] + (bias ? bias[col + i] : 0.f));
+      }
+    }
+    // (what the others have here has been read before it is used; the stores need not have arrived)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (CG == 2) g8_cluster_sync();
+  if (warp == G8_EPI_WARPS + 1) {
+    tc_fence_after();
+    if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"((unsigned)G8_COLS) : "memory");
+    else tc_dealloc(tmem_slot, G8_COLS);
+  }
   if constexpr (EPI == G8_GATED) {
     // (the whole CTA: a thread to 8 of k)
     double (*sums)[2] = reinterpret_cast<double (*)[2]>(base);
@@ -828,58 +882,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (lane == 0) *scale = (unsigned char)(low + over);
       }
     }
-  }
-  if constexpr (EPI == G8_SHARED) {
-    g8_cluster_sync();
-    // this CTA's share of the tile's rows, summed in the order of the shares of K: up to 32 pieces of four features of a row to a warp, two
-    // times that on their way together
-    const G8Item q = g8_item(p, worker, share);
-    const int tok0 = q.tt * p.mrows, n_rows = min(p.mrows, p.T - tok0), pieces = p.bn >> 2, wide = pieces > 32;
-    const int r0 = n_rows * share / p.splits, units = (n_rows * (share + 1) / p.splits - r0) << wide;
-    const unsigned at = tc_smem(base);
-    constexpr int WARPS = G8_THREADS / 32;
-#pragma unroll 1
-    for (int u0 = warp; u0 < units; u0 += 2 * WARPS) {
-      float4 v[2][8];
-      int r[2], c[2];
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int u = u0 + h * WARPS;
-        r[h] = r0 + (u >> wide);
-        c[h] = u < units ? (wide ? (u & 1) * 32 : 0) + lane : pieces;
-        const unsigned from = at + (r[h] * pieces + (c[h] ^ (r[h] & 7))) * 16;
-#pragma unroll
-        for (int sp = 0; sp < 8; sp++)
-          if (sp < p.splits && c[h] < pieces) {
-            unsigned remote;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(from), "r"(sp));
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(v[h][sp].x), "=f"(v[h][sp].y), "=f"(v[h][sp].z), "=f"(v[h][sp].w) : "r"(remote) : "memory");
-          }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (c[h] >= pieces) break;
-        float4 t = v[h][0];
-#pragma unroll
-        for (int sp = 1; sp < 8; sp++)
-          if (sp < p.splits) { t.x += v[h][sp].x; t.y += v[h][sp].y; t.z += v[h][sp].z; t.w += v[h][sp].w; }
-        const int col = q.ft * p.bn + 4 * c[h];
-        const float f[4] = {t.x, t.y, t.z, t.w};
-        TO* to = out + (size_t)(tok0 + r[h]) * p.ldo + col;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (col + i < p.feats) to[i] = from_float<TO>(f[i] + (bias ? bias[col + i] : 0.f));
-      }
-    }
-    // (what the others have here has been read before it is used; the stores need not have arrived)
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-  if (CG == 2) g8_cluster_sync();
-  if (warp == G8_EPI_WARPS + 1) {
-    tc_fence_after();
-    if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"((unsigned)G8_COLS) : "memory");
-    else tc_dealloc(tmem_slot, G8_COLS);
   }
 }
 
@@ -1025,7 +1027,7 @@ extern "C" int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long lo
   G8Params p;
   p.act = act; p.resident = resident; p.T = T; p.N = N; p.K = K; p.bn = bn; p.splits = splits; p.ldo = ldo;
   p.sx = (const unsigned char*)sx; p.sw = (const unsigned char*)sw; p.ldsx = ldsx; p.ldsw = ldsw;
-  p.x = (const unsigned char*)X; p.w = (const unsigned char*)W; p.ldx = ldx; p.ldw = ldw;
+  p.doubt = g8_doubt(K); p.x = (const unsigned char*)X; p.w = (const unsigned char*)W; p.ldx = ldx; p.ldw = ldw;
   p.s_out = (unsigned char*)s_out; p.lds_out = lds_out;
   p.kb_total = up(K, FP8_BLOCK);
   if (ldsx < p.kb_total || ldsw < p.kb_total) return QD_ERR_UNSUPPORTED;
