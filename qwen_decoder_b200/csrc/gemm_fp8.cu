@@ -590,7 +590,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
               float v[16];
               g8_ld16(acc + 16 * g, v);
               tc_ld_wait();
-              if (owner && i == G8_OVERLAP / 16 - 1) release(buf);
+              if (owner && n_rows > 0 && i == G8_OVERLAP / 16 - 1) release(buf);       // (a CTA without rows has done so above)
               if (lane < n_rows)
 #pragma unroll
                 for (int e = 0; e < 4; e++)

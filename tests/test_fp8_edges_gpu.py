@@ -1,0 +1,27 @@
+"""Operators in 8 bits where their calls are unusual: pairs of which one CTA has no rows, operands that the launch before writes, a row alone
+and among others, scales and numbers of blocks whose largest magnitude lies where the scale doubles, deep gates."""
+import pytest
+import torch
+
+from test_fp8_gpu import DEV, check_rows, gated, operands, room, sums_off, value
+
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("guard_regions")]
+
+
+@pytest.mark.parametrize("T", [1, 8, 13])
+def test_gated_products_of_few_tokens_in_pairs_with_several_tiles(T):
+    """Pairs of which the second CTA has no rows (up to 8 tokens) or few, and more tiles than pairs: a tile's sums stay until they have been
+    read, whichever CTA has them."""
+    from qwen_decoder_b200 import kernels
+    F, K = 40000, 384
+    x, w, b = operands(T, 2 * F, K)
+    z = value(x) @ value(w).T + b.double()
+    off = sums_off(x, w) + 2.0 ** -23 * z.abs()
+    wide = 1.2 * off[:, :F] * z[:, F:].abs() + (z[:, :F].abs() + off[:, :F]) * off[:, F:] + 2.0 ** -20 * (z[:, :F] * z[:, F:]).abs()
+    h = gated(z[:, :F], z[:, F:], 0)
+    for _ in range(3):
+        for plan in ((2, 256, 1), (1, 256, 1)):
+            out = room(T, F)
+            kernels.gemm_fp8_gated(x, w, b, out, 0, plan)
+            check_rows(out, h, wide)
+    kernels.check_status()
