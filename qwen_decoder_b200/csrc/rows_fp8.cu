@@ -146,12 +146,12 @@ __global__ void __launch_bounds__(1024) norm_fp8_kernel(const NormArgs a) {
   __shared__ float scratch[40];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = (blockDim.x >> 5) * FP8_BLOCK, k0 = warp * FP8_BLOCK + 4 * lane;
   pdl_launch_dependents();
-  // (no kernel of the package writes a norm's weights: with few blocks to a warp they travel while that is waited for)
+  pdl_wait();
+  // (after the wait, as all that is read: the launch before may have written the weights; with few blocks to a warp they travel beside the row)
   float4 w[VPT <= 4 ? VPT : 1];
   if (VPT <= 4)
 #pragma unroll
     for (int i = 0; i < VPT; i++) w[VPT <= 4 ? i : 0] = load4<VEC>(a.w, k0 + i * step, a.D);
-  pdl_wait();
   const int r = blockIdx.x;
   const size_t at = (size_t)(a.rows ? a.rows[r] : r) * a.D;
   float4 v[VPT];

@@ -25,3 +25,22 @@ def test_gated_products_of_few_tokens_in_pairs_with_several_tiles(T):
             kernels.gemm_fp8_gated(x, w, b, out, 0, plan)
             check_rows(out, h, wide)
     kernels.check_status()
+
+
+@pytest.mark.parametrize("rows,D", [(1, 2048), (3, 8192), (400, 4096), (2, 20000)])
+def test_norm_weights_that_the_launch_before_writes(rows, D):
+    """A norm whose weights are the sums of the product right before it: as with the same weights at rest."""
+    from qwen_decoder_b200 import kernels
+    x, gains, _ = operands(1, D, 8192)
+    weight = torch.zeros(1, D, device=DEV)
+    stream = torch.empty(rows, D, device=DEV).normal_()
+    want, out = room(rows, D), room(rows, D)
+    kernels.gemm_fp8(x, gains, None, weight)
+    torch.cuda.synchronize()
+    kernels.add_rmsnorm_fp8(stream, None, weight[0], want, 1e-6)
+    for _ in range(8):
+        weight.zero_()
+        torch.cuda.synchronize()
+        kernels.gemm_fp8(x, gains, None, weight)
+        kernels.add_rmsnorm_fp8(stream, None, weight[0], out, 1e-6)
+        assert torch.equal(out.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(out.s.view(torch.uint8), want.s.view(torch.uint8))
