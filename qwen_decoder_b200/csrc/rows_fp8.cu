@@ -129,6 +129,7 @@ extern "C" int qd_rows_fp8(const void* x, int dtype, long long ldx, int n_parts,
 }
 
 // ------------------------------------------------------------------------------ the residual sum's norm
+#define NORM_MAX_BLOCKS (32 * 16)             // 65,536 features
 struct NormArgs {
   float* x;
   const void* delta;
@@ -140,10 +141,12 @@ struct NormArgs {
   long long part_stride, ldq, lds;
 };
 
-// One CTA to a row.  A warp holds up to VPT of the row's blocks in registers.
+// One CTA to a row.  A warp holds up to VPT of the row's blocks in registers.  The squares are summed block by block, a block in the order of
+// a warp's butterfly, the blocks' sums by lanes and then such a butterfly: an order that depends only on D, whatever VPT the number of rows
+// leads to, so that a row's result does not depend on what else is in the batch.
 template <typename TD, int VPT, bool VEC>
 __global__ void __launch_bounds__(1024) norm_fp8_kernel(const NormArgs a) {
-  __shared__ float scratch[40];
+  __shared__ float squares[32 * VPT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = (blockDim.x >> 5) * FP8_BLOCK, k0 = warp * FP8_BLOCK + 4 * lane;
   pdl_launch_dependents();
   pdl_wait();
@@ -165,9 +168,10 @@ __global__ void __launch_bounds__(1024) norm_fp8_kernel(const NormArgs a) {
       const int k = k0 + i * step;
       if (a.dscale) {
         const float4 f = load4<VEC>(a.dscale, k, a.D);
-        d[i].x *= f.x; d[i].y *= f.y; d[i].z *= f.z; d[i].w *= f.w;
+        v[i].x = fmaf(d[i].x, f.x, v[i].x); v[i].y = fmaf(d[i].y, f.y, v[i].y); v[i].z = fmaf(d[i].z, f.z, v[i].z); v[i].w = fmaf(d[i].w, f.w, v[i].w);
+      } else {
+        add4(v[i], d[i]);
       }
-      add4(v[i], d[i]);
       if (a.write_back) {
         float* to = a.x + at + k;
         if (VEC) {
@@ -181,10 +185,27 @@ __global__ void __launch_bounds__(1024) norm_fp8_kernel(const NormArgs a) {
       }
     }
   }
+  // The butterflies of VPT blocks as one: of two sums a lane keeps one, and gives the other to the lane that keeps that
+  float sq[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; i++) sq[i] = fmaf(v[i].w, v[i].w, fmaf(v[i].z, v[i].z, fmaf(v[i].y, v[i].y, v[i].x * v[i].x)));
+#pragma unroll
+  for (int o = 16, n = VPT / 2; o; o >>= 1, n >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < (n ? n : 1); i++) {
+      const float next = sq[(i + n) % VPT], other = n && !upper ? next : sq[i];
+      if (n && upper) sq[i] = next;
+      sq[i] += __shfl_xor_sync(0xffffffffu, other, o);
+    }
+  }
+  const int of = warp + lane / (32 / VPT) * (int)(blockDim.x >> 5);
+  if (lane % (32 / VPT) == 0 && of < a.blocks) squares[of] = sq[0];
+  __syncthreads();
   float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < VPT; i++) ss += v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
-  ss = block_sum(ss, scratch);
+  for (int i = 0; i < VPT; i++) ss += lane + 32 * i < a.blocks ? squares[lane + 32 * i] : 0.f;
+  ss = warp_sum(ss);
   const float inv = 1.0f / sqrtf(ss / (float)a.D + a.eps);
 #pragma unroll
   for (int i = 0; i < VPT; i++) {
@@ -212,7 +233,7 @@ extern "C" int qd_add_rmsnorm_fp8(float* x, const void* delta, int delta_dtype, 
   a.part_stride = part_stride; a.ldq = ldq; a.lds = lds;
   const bool vec = D % 4 == 0 && part_stride % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)dscale) & 15) &&
           !((uintptr_t)delta & (delta_dtype == QD_BF16 ? 7 : 15));
-  if (a.blocks > 32 * 16) return QD_ERR_UNSUPPORTED;       // 65,536 features
+  if (a.blocks > NORM_MAX_BLOCKS) return QD_ERR_UNSUPPORTED;
   // As many rows as run at a time (64 warps to a multiprocessor): a block to each warp, the shortest way; more: four, so that more rows are
   // on their way at a time (512 and 2,048 rows of 2,048 features, us: 3.1 and 10.9 with one, 4.5 and 10.0 with four)
   const int vpt = a.blocks > 128 ? 16 : a.blocks > 64 ? 4 : a.blocks > 32 ? (n_rows > 296 ? 4 : 2) : n_rows > 148 * (64 / a.blocks) ? 4 : 1;

@@ -976,7 +976,7 @@ def add_rmsnorm_fp8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
                     rows: Optional[torch.Tensor] = None, write_back: bool = True, delta_scale: Optional[torch.Tensor] = None) -> None:
     """``add_rmsnorm`` with its output in 8 bits: out[r] = rmsnorm(x[s] + delta[s]) * weight with s = rows[r] (or r), rounded once; x
     float32 [T, D] is updated to x + delta when ``write_back``.  delta: bfloat16 or float32 [T, D], or float32 partial sums [n, T, D];
-    ``delta_scale`` float32 [D] or None multiplies it."""
+    ``delta_scale`` float32 [D] or None multiplies it.  A row's result does not depend on the rows beside it."""
     _launch_count[0] += 1
     (_host or _host_calls()).add_rmsnorm_fp8(x, delta, weight, out, eps, rows, write_back, delta_scale)
 

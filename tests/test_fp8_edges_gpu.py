@@ -44,3 +44,22 @@ def test_norm_weights_that_the_launch_before_writes(rows, D):
         kernels.gemm_fp8(x, gains, None, weight)
         kernels.add_rmsnorm_fp8(stream, None, weight[0], out, 1e-6)
         assert torch.equal(out.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(out.s.view(torch.uint8), want.s.view(torch.uint8))
+
+
+@pytest.mark.parametrize("D,parts,scaled", [(1, 0, False), (517, 3, False), (2048, 0, False), (2048, 4, True), (3584, 0, True), (5000, 0, False),
+                                            (8192, 2, False), (20000, 0, True)])
+def test_a_row_of_the_norm_alone_and_among_others(D, parts, scaled):
+    """Whatever number of rows is normed with it, a row's sum and its 8 bits are the same."""
+    from qwen_decoder_b200 import kernels
+    T = 700
+    x, w = torch.empty(T, D, device=DEV).normal_() * 3, 1 + 0.1 * torch.empty(D, device=DEV).normal_()
+    delta = torch.empty(parts, T, D, device=DEV).normal_() if parts else torch.empty(T, D, device=DEV).normal_().bfloat16()
+    scale = torch.empty(D, device=DEV).normal_() if scaled else None
+    kept, whole = x.clone(), room(T, D)
+    kernels.add_rmsnorm_fp8(x, delta, w, whole, 1e-6, delta_scale=scale)
+    for at, n in ((0, 1), (5, 1), (699, 1), (100, 148), (100, 300), (200, 500)):
+        some, out = kept[at:at + n].clone(), room(n, D)
+        kernels.add_rmsnorm_fp8(some, delta[..., at:at + n, :].contiguous(), w, out, 1e-6, delta_scale=scale)
+        assert torch.equal(some, x[at:at + n])
+        assert torch.equal(out.q.view(torch.uint8), whole.q[at:at + n].view(torch.uint8))
+        assert torch.equal(out.s.view(torch.uint8), whole.s[at:at + n].view(torch.uint8))
