@@ -227,8 +227,10 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
 // tokens of the 7B sizes 56.6 -> 57.3 us.  Looked at in the epilogue itself they made its code so long that products of 8 to 512 tokens took 3
 // to 15 % more.)  How near is in units of the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by up to 0.2
 // in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error.
-#define G8_NEAR 128                           // blocks of a CTA that are looked at; with more of them none is
+#define G8_NEAR 128                           // blocks that a CTA keeps for that; with more of them it goes through all that it has written, a tile's at a time
 static int g8_doubt(int K) { return K < 1 << 24 ? (K >> 5) + 16 : 0xfffff; }
+#define G8_448 0x7e                           // as e4m3
+#define G8_224 0x76
 __device__ __forceinline__ bool g8_near(unsigned peak, int doubt) {
   const int off = (int)(peak & 0x7fffffu) - 0x600000;
   return peak >= 10u << 23 && peak < 0x7f800000u && abs(off) <= doubt;
@@ -812,75 +814,101 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if constexpr (EPI == G8_GATED) {
     // (the whole CTA: a thread to 8 of k)
     double (*sums)[2] = reinterpret_cast<double (*)[2]>(base);
-    const int looked = n_near <= G8_NEAR && n_items <= 1 << 25 ? n_near : 0;
+    int looked = n_near;
+    const bool all = looked > G8_NEAR || n_items > 1 << 25;
 #pragma unroll 1
-    for (int i = 0; i < looked; i++) {
-      const G8Item q = g8_item(p, near_rows[i] >> 7, 0);
-      const long long row = row_x(q) + (int)(near_rows[i] & 127);
-      const int col = q.ft * 128 + 4 * lane, there = min(4, p.feats - col);
-      unsigned char *to = (unsigned char*)out + row * p.ldo + col, *scale = p.s_out + row * p.lds_out + q.ft;
-      float v[4];
-      unsigned most = 0;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        v[e] = e < there ? fp8_value(to[e]) : 0.f;
-        most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+    for (int item = worker; item < n_items; item += n_workers) {
+      if (all) {
+        // Rounded numbers say where a scale may be that of a peak near the edge: 448 is then the largest one, or 224 of the higher scale.  One
+        // block in ten is such and is looked at; what is far from the edge stays as it is.
+        const G8Item q = g8_item(p, item, 0);
+        const int row0 = row_x(q), col = q.ft * 128 + 4 * lane, n_rows = min(p.mrows, p.T - row0);
+        __syncthreads();
+        if (threadIdx.x == 0) n_near = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int r = warp; r < n_rows; r += G8_THREADS / 32) {
+          const unsigned char* of = (const unsigned char*)out + (size_t)(row0 + r) * p.ldo + col;
+          unsigned most = 0;
+#pragma unroll 1
+          for (int e = 0; e < 4 && col + e < p.feats; e++) most = max(most, of[e] & 0x7fu);
+          most = __reduce_max_sync(0xffffffffu, most);
+          const unsigned byte = p.s_out[(size_t)(row0 + r) * p.lds_out + q.ft];
+          if (lane == 0 && byte != 255u && (most == G8_448 ? byte >= 2 : most == G8_224 && byte >= 3)) near_rows[atomicAdd(&n_near, 1)] = r;
+        }
+        __syncthreads();
+        looked = n_near;
       }
-      most = __reduce_max_sync(0xffffffffu, most);
-      // The scale is the one of at most 448, or twice that.  Those that count are the largest of the rounded ones; the edge is 448 of the lower.
-      const bool higher = most < __float_as_uint(400.f);
-      const unsigned low = *scale - higher, edge = (low + 8) << 23 | 0x600000u;
-      bool over = false;
 #pragma unroll 1
-      for (int e = 0; e < 4 && !over; e++) {
-        const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
-#pragma unroll 1
-        for (unsigned c = __ballot_sync(0xffffffffu, (__float_as_uint(of) & 0x7fffffffu) == most); c && !over; c &= c - 1) {
-          const long long g = q.ft * 128 + 4 * (__ffs(c) - 1) + e, u = p.feats + g;
-          double tg = 0.0, tu = 0.0;
-#pragma unroll 1
-          for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
-            float a[8], b[8], d[8], sg = 0.f, su = 0.f;
-            g8_eight(a, p.x + row * p.ldx + k, p.K - k);
-            g8_eight(b, p.w + g * p.ldw + k, p.K - k);
-            g8_eight(d, p.w + u * p.ldw + k, p.K - k);
-            const int block = k >> 7;
-            const unsigned sx = p.sx[row * p.ldsx + block];
+      for (int i = 0; i < looked; i++) {
+        const G8Item q = g8_item(p, all ? item : near_rows[i] >> 7, 0);
+        const long long row = row_x(q) + (int)(near_rows[i] & 127);
+        const int col = q.ft * 128 + 4 * lane, there = min(4, p.feats - col);
+        unsigned char *to = (unsigned char*)out + row * p.ldo + col, *scale = p.s_out + row * p.lds_out + q.ft;
+        float v[4];
+        unsigned most = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              sg = fmaf(a[j], b[j], sg);
-              su = fmaf(a[j], d[j], su);
-            }
-            tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
-            tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
-          }
-          for (int d = 16; d; d >>= 1) {
-            tg += __shfl_xor_sync(0xffffffffu, tg, d);
-            tu += __shfl_xor_sync(0xffffffffu, tu, d);
-          }
-          __syncthreads();                                   // (what the sums before were is no longer read)
-          if (lane == 0) {
-            sums[warp][0] = tg;
-            sums[warp][1] = tu;
-          }
-          __syncthreads();
-          tg = bias ? bias[g] : 0.f;
-          tu = bias ? bias[u] : 0.f;
+        for (int e = 0; e < 4; e++) {
+          v[e] = e < there ? fp8_value(to[e]) : 0.f;
+          most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        // The scale is the one of at most 448, or twice that.  Those that count are the largest of the rounded ones; the edge is 448 of the lower.
+        const bool higher = most < __float_as_uint(400.f);
+        const unsigned low = *scale - higher, edge = (low + 8) << 23 | 0x600000u;
+        bool over = false;
 #pragma unroll 1
-          for (int j = 0; j < G8_THREADS / 32; j++) {
-            tg += sums[j][0];
-            tu += sums[j][1];
+        for (int e = 0; e < 4 && !over; e++) {
+          const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+#pragma unroll 1
+          for (unsigned c = __ballot_sync(0xffffffffu, (__float_as_uint(of) & 0x7fffffffu) == most); c && !over; c &= c - 1) {
+            const long long g = q.ft * 128 + 4 * (__ffs(c) - 1) + e, u = p.feats + g;
+            double tg = 0.0, tu = 0.0;
+#pragma unroll 1
+            for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
+              float a[8], b[8], d[8], sg = 0.f, su = 0.f;
+              g8_eight(a, p.x + row * p.ldx + k, p.K - k);
+              g8_eight(b, p.w + g * p.ldw + k, p.K - k);
+              g8_eight(d, p.w + u * p.ldw + k, p.K - k);
+              const int block = k >> 7;
+              const unsigned sx = p.sx[row * p.ldsx + block];
+#pragma unroll
+              for (int j = 0; j < 8; j++) {
+                sg = fmaf(a[j], b[j], sg);
+                su = fmaf(a[j], d[j], su);
+              }
+              tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
+              tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
+            }
+            for (int d = 16; d; d >>= 1) {
+              tg += __shfl_xor_sync(0xffffffffu, tg, d);
+              tu += __shfl_xor_sync(0xffffffffu, tu, d);
+            }
+            __syncthreads();                                   // (what the sums before were is no longer read)
+            if (lane == 0) {
+              sums[warp][0] = tg;
+              sums[warp][1] = tu;
+            }
+            __syncthreads();
+            tg = bias ? bias[g] : 0.f;
+            tu = bias ? bias[u] : 0.f;
+#pragma unroll 1
+            for (int j = 0; j < G8_THREADS / 32; j++) {
+              tg += sums[j][0];
+              tu += sums[j][1];
+            }
+            over = (__float_as_uint(fp8_gated((float)tg, (float)tu, p.act)) & 0x7fffffffu) > edge;
           }
-          over = (__float_as_uint(fp8_gated((float)tg, (float)tu, p.act)) & 0x7fffffffu) > edge;
+        }
+        __syncthreads();                                       // all have read the row
+        if (warp == 0 && over != higher) {
+          const float by = over ? 0.5f : 2.f;
+          const unsigned w = fp8_pack4(v[0] * by, v[1] * by, v[2] * by, v[3] * by);
+          for (int e = 0; e < there; e++) to[e] = (unsigned char)(w >> 8 * e);
+          if (lane == 0) *scale = (unsigned char)(low + over);
         }
       }
-      __syncthreads();                                       // all have read the row
-      if (warp == 0 && over != higher) {
-        const float by = over ? 0.5f : 2.f;
-        const unsigned w = fp8_pack4(v[0] * by, v[1] * by, v[2] * by, v[3] * by);
-        for (int e = 0; e < there; e++) to[e] = (unsigned char)(w >> 8 * e);
-        if (lane == 0) *scale = (unsigned char)(low + over);
-      }
+      if (!all) break;
     }
   }
 }

@@ -3,7 +3,7 @@ and among others, scales and numbers of blocks whose largest magnitude lies wher
 import pytest
 import torch
 
-from test_fp8_gpu import DEV, check_rows, gated, operands, room, sums_off, value
+from test_fp8_gpu import DEV, check_rows, gated, operands, room, rows_of, sums_off, value
 
 pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("guard_regions")]
 
@@ -63,3 +63,38 @@ def test_a_row_of_the_norm_alone_and_among_others(D, parts, scaled):
         assert torch.equal(some, x[at:at + n])
         assert torch.equal(out.q.view(torch.uint8), whole.q[at:at + n].view(torch.uint8))
         assert torch.equal(out.s.view(torch.uint8), whole.s[at:at + n].view(torch.uint8))
+
+
+@pytest.mark.parametrize("T,plan", [(9, (1, 256, 1)), (200, (1, 256, 1)), (200, (2, 256, 1)), (200, None)])
+def test_gated_scales_where_all_blocks_are_near_the_edge(T, plan):
+    """More blocks to a CTA whose largest magnitude lies where the scale doubles than it keeps: equal rows, hundreds of such blocks in each.
+    The activation of a large gate is the gate; roundings of the gate, of up, of their product and of the quotient are 5 times 2^-24 at most."""
+    from qwen_decoder_b200 import kernels
+    K, blocks = 8192, 3000 if T == 9 else 400
+    F = 128 * blocks
+    x = rows_of(torch.empty(1, K, device=DEV).normal_().abs().expand(T, K).contiguous())
+    some = rows_of(torch.empty(2 * blocks, K, device=DEV).normal_().abs() * 64 / K)       # the features that count: gates, then ups
+    at = 128 * torch.arange(blocks, device=DEV) + torch.arange(blocks, device=DEV) * 37 % 128
+    w = room(2 * F, K)
+    w.q.view(torch.uint8).zero_()
+    w.s.view(torch.uint8).fill_(127)
+    for part, to in ((slice(0, blocks), at), (slice(blocks, None), at + F)):
+        w.q.view(torch.uint8)[to] = some.q.view(torch.uint8)[part]
+        w.s.view(torch.uint8)[to] = some.s.view(torch.uint8)[part]
+    z = (value(x)[:1] @ value(some).T)[0]
+    gate, up = z[:blocks], z[blocks:]
+    off = torch.linspace(-3e-6, 3e-6, blocks, device=DEV, dtype=torch.float64)[torch.randperm(blocks, device=DEV)]
+    bias = torch.zeros(2 * F, device=DEV)
+    bias[at] = torch.clamp(30 - gate, min=0).float()
+    gate = gate + bias[at].double()
+    edge = 1.75 * torch.exp2(torch.floor(torch.log2(gate * up / 1.75)))
+    bias[at + F] = (edge * (1 + off) / gate - up).float()
+    h = gate * (up + bias[at + F].double())
+    far = (h / edge - 1).abs() > 5 * 2.0 ** -24
+    assert far.sum() > 0.8 * blocks
+    out = room(T, F)
+    kernels.gemm_fp8_gated(x, w, bias, out, 0, plan)
+    s = out.s.float().double()
+    assert (s == torch.where(h > edge, 2 * edge / 448, edge / 448))[:, far].all()
+    assert (out.q[:, at].float() == torch.where(s > (edge / 448)[None], 224.0, 448.0)).all()
+    kernels.check_status()
