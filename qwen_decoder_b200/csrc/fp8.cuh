@@ -35,12 +35,36 @@ __device__ __forceinline__ float fp8_value(unsigned byte) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)byte));
   return __half2float(__ushort_as_half((unsigned short)h));
 }
-// act(g) u, the quotient and the exponential within 2^-20.  A gate of minus infinity goes as the largest finite one does, to zero.
+// act(g) u = g / (1 + e^-a) u, a = ``qd_gate_arg(g, act)``, within 6 2^-23 of itself: 2^-22 for the power of two, 2^-23 for the reciprocal, half
+// a unit or less for each rounding besides.  An exponent as one float32 would be off by |a| 2^-24 and more (a = -87: 2^-17 of the result, a of
+// gelu 2^-15), so what -a / log 2 loses in its rounding goes on as a factor 1 + r (Cody and Waite's reduction), and gelu's a is kept with what
+// its own roundings lose.  From a of -87.3 down the result is zero (1 + e^-a has no reciprocal that is a normal number), as of a gate of
+// minus infinity.
 __device__ __forceinline__ float fp8_gated(float g, float u, int act) {
-  float r;
-  asm("max.NaN.f32 %0, %0, 0fFF7FFFFF;" : "+f"(g));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-qd_gate_arg(g, act))));
-  return g * r * u;
+  const bool gelu = act == QD_ACT_GELU_TANH;
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(gelu ? -11.f : -88.f));       // (below: zero; products of infinities are none)
+  float a = fminf(g, gelu ? 16.f : 128.f), rest = 0.f;                       // (above: e^-a is nothing beside 1)
+  if (gelu) {
+    // a = g (c + c 0.044715 g^2); c in two parts, the first a multiple of 2^-15, so that the difference from it is exact
+    const float t = a * a, s = fmaf(0.071354814f, t, 1.5957642f);
+    float lost = fmaf(0.071354814f, t, -(s - 1.5957642f));
+    lost = fmaf(0.071354814f, fmaf(a, a, -t), lost);
+    lost = fmaf(2.3988325e-9f, t, lost) + 4.9614496e-6f;
+    const float whole = a * s;
+    rest = fmaf(a, lost, fmaf(a, s, -whole));
+    a = fmaxf(whole, -88.f);
+  }
+  const float p = -1.4426950408889634f * a;                                  // up to 127: a power that is finite
+  float r = fmaf(p, 1.9046542e-9f, fmaf(p, -0.69314718f, -a)) - rest, e, inv;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p));
+  e = fmaf(e, r, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.0f + e));
+  return g * inv * u;
+}
+// the same in float64, of which the rounding to 32 bits is no part
+__device__ __forceinline__ double fp8_gated_64(double g, double u, int act) {
+  const double a = act == QD_ACT_GELU_TANH ? 1.5957691216057308 * fma(0.044715 * g * g, g, g) : g;
+  return fmax(g, -3.4028234663852886e38) / (1.0 + exp(-a)) * u;
 }
 // the larger magnitude, or no number where one is none
 __device__ __forceinline__ float fp8_peak(float a, float b) {

@@ -226,7 +226,8 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
 // other scale, K 2,048 to 11,008; some 25 of a million are looked at for K 3,584, 1 to 2 us each where the kernel ends with one: a layer of 8
 // tokens of the 7B sizes 56.6 -> 57.3 us.  Looked at in the epilogue itself they made its code so long that products of 8 to 512 tokens took 3
 // to 15 % more.)  How near is in units of the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by up to 0.2
-// in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error.
+// in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error (1.75 times 6), which
+// the look itself does not have: it goes on in float64 to the end.
 #define G8_NEAR 128                           // blocks that a CTA keeps for that; with more of them it goes through all that it has written, a tile's at a time
 static int g8_doubt(int K) { return K < 1 << 24 ? (K >> 5) + 16 : 0xfffff; }
 #define G8_448 0x7e                           // as e4m3
@@ -855,7 +856,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         most = __reduce_max_sync(0xffffffffu, most);
         // The scale is the one of at most 448, or twice that.  Those that count are the largest of the rounded ones; the edge is 448 of the lower.
         const bool higher = most < __float_as_uint(400.f);
-        const unsigned low = *scale - higher, edge = (low + 8) << 23 | 0x600000u;
+        const unsigned low = *scale - higher;
+        const double edge = 448.0 * g8_scaled(low, 127);
         bool over = false;
 #pragma unroll 1
         for (int e = 0; e < 4 && !over; e++) {
@@ -866,7 +868,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             double tg = 0.0, tu = 0.0;
 #pragma unroll 1
             for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
-              float a[8], b[8], d[8], sg = 0.f, su = 0.f;
+              float a[8], b[8], d[8];
+              double sg = 0.0, su = 0.0;
               g8_eight(a, p.x + row * p.ldx + k, p.K - k);
               g8_eight(b, p.w + g * p.ldw + k, p.K - k);
               g8_eight(d, p.w + u * p.ldw + k, p.K - k);
@@ -874,8 +877,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
               const unsigned sx = p.sx[row * p.ldsx + block];
 #pragma unroll
               for (int j = 0; j < 8; j++) {
-                sg = fmaf(a[j], b[j], sg);
-                su = fmaf(a[j], d[j], su);
+                sg += a[j] * b[j];                           // (a product of two such numbers has 8 bits)
+                su += a[j] * d[j];
               }
               tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
               tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
@@ -897,7 +900,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
               tg += sums[j][0];
               tu += sums[j][1];
             }
-            over = (__float_as_uint(fp8_gated((float)tg, (float)tu, p.act)) & 0x7fffffffu) > edge;
+            over = fabs(fp8_gated_64(tg, tu, p.act)) > edge;
           }
         }
         __syncthreads();                                       // all have read the row

@@ -98,3 +98,48 @@ def test_gated_scales_where_all_blocks_are_near_the_edge(T, plan):
     assert (s == torch.where(h > edge, 2 * edge / 448, edge / 448))[:, far].all()
     assert (out.q[:, at].float() == torch.where(s > (edge / 448)[None], 224.0, 448.0)).all()
     kernels.check_status()
+
+
+def deep(g, u, act):
+    """``gated`` without the cancellation of 1 + tanh."""
+    return g * torch.sigmoid(1.5957691216057308 * (g + 0.044715 * g ** 3) if act else g) * u
+
+
+@pytest.mark.parametrize("act", [0, 2])
+def test_deep_gates(act):
+    """Gates far below zero, relative to the activation itself, which is tiny beside gate and up: within 6 units of 2^-23 of itself."""
+    from qwen_decoder_b200 import kernels
+    T, F = 40, 1000
+    z = torch.empty(T, 2 * F, device=DEV).normal_()
+    low = torch.tensor([10, 20, 40, 60] if act == 0 else [3, 5, 7, 8.5], device=DEV).repeat(T // 4)[:, None]
+    z[:, :F] = -low * (1 + 0.2 * torch.rand(T, F, device=DEV))
+    out = room(T, F)
+    kernels.gate_fp8(z, out, None, act)
+    g, u = z[:, :F].double(), z[:, F:].double()
+    h = deep(g, u, act)
+    check_rows(out, h, 6 * 2.0 ** -23 * h.abs())
+
+
+@pytest.mark.parametrize("act", [0, 2])
+@pytest.mark.parametrize("T,plan", [(3, None), (60, (1, 256, 1)), (200, (2, 256, 1))])
+def test_gated_scales_of_deep_gates(T, plan, act):
+    """Largest magnitudes of deep gates some ten millionths off where the scale doubles: the activation's own error does not decide."""
+    from qwen_decoder_b200 import kernels
+    K, blocks = 128, 400
+    F = 128 * blocks
+    x, w, _ = operands(T, 2 * F, K)
+    w.q.zero_()                                            # gate and up are their biases
+    at = 128 * torch.arange(blocks, device=DEV) + torch.arange(blocks, device=DEV) % 128
+    bias = torch.zeros(2 * F, device=DEV)
+    bias[at] = -torch.linspace(10, 80, blocks, device=DEV) if act == 0 else -torch.linspace(2.5, 9, blocks, device=DEV)
+    gate = bias[at].double()
+    off = torch.linspace(-1e-6, 1e-6, blocks, device=DEV, dtype=torch.float64)[torch.randperm(blocks, device=DEV)]
+    bias[at + F] = (1.75 * (1 + off) / deep(gate, 1.0, act)).float()
+    h = deep(gate, bias[at + F].double(), act).abs()
+    far = (h / 1.75 - 1).abs() > 1e-12
+    assert far.sum() > blocks - 10
+    out = room(T, F)
+    kernels.gemm_fp8_gated(x, w, bias, out, act, plan)
+    s = out.s.float().double()
+    assert (s == torch.where(h > 1.75, 2.0 ** -7, 2.0 ** -8))[:, far].all()
+    kernels.check_status()
