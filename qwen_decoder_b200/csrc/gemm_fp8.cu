@@ -223,11 +223,12 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
 
 // Where a block's largest magnitude is so near the last one of a scale that the sums' cut-off decides, its sums are made again at the kernel's
 // end: a scale is then that of the sums as they are, not of the order of their additions.  (Without it 1 to 4 of a million blocks had the
-// other scale, K 2,048 to 11,008; some 25 of a million are looked at for K 3,584, 1 to 2 us each where the kernel ends with one: a layer of 8
+// other scale, K 2,048 to 11,008; some 25 of a million are looked at for K 3,584, 2.4 us each where the kernel ends with one: a layer of 8
 // tokens of the 7B sizes 56.6 -> 57.3 us.  Looked at in the epilogue itself they made its code so long that products of 8 to 512 tokens took 3
 // to 15 % more.)  How near is in units of the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by up to 0.2
 // in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error (1.75 times 6), which
-// the look itself does not have: it goes on in float64 to the end.
+// the look itself does not have: it goes on in float64 to the end.  (A gate of -g < -2 makes g - 1 times its sum's error of it: where every gate of a
+// block lies far below -10, sums of one sign may leave the other scale, which holds the block as well but for half a step.)
 #define G8_NEAR 128                           // blocks that a CTA keeps for that; with more of them it goes through all that it has written, a tile's at a time
 static int g8_doubt(int K) { return K < 1 << 24 ? (K >> 5) + 16 : 0xfffff; }
 #define G8_448 0x7e                           // as e4m3
@@ -858,49 +859,58 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         const bool higher = most < __float_as_uint(400.f);
         const unsigned low = *scale - higher;
         const double edge = 448.0 * g8_scaled(low, 127);
+        // First whether the block is over the edge; if its scale changes then also the numbers that are among e4m3's smallest, 2^-9 apart, at one
+        // of the scales: their rounded ones have lost, or would be rounded twice.  (Others are as far apart for their size at both scales.)
         bool over = false;
 #pragma unroll 1
-        for (int e = 0; e < 4 && !over; e++) {
-          const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+        for (int pass = 0; pass < (over == higher ? 1 : 2); pass++) {
+          const double unit = g8_scaled(254 - low - over, 127) * (over ? 2.0 : 0.5);       // (of the scale before)
 #pragma unroll 1
-          for (unsigned c = __ballot_sync(0xffffffffu, (__float_as_uint(of) & 0x7fffffffu) == most); c && !over; c &= c - 1) {
-            const long long g = q.ft * 128 + 4 * (__ffs(c) - 1) + e, u = p.feats + g;
-            double tg = 0.0, tu = 0.0;
+          for (int e = 0; e < 4 && (pass || !over); e++) {
+            const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+            const bool taken = pass ? e < there && fabsf(of) < 0.03125f : (__float_as_uint(of) & 0x7fffffffu) == most;
 #pragma unroll 1
-            for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
-              float a[8], b[8], d[8];
-              double sg = 0.0, su = 0.0;
-              g8_eight(a, p.x + row * p.ldx + k, p.K - k);
-              g8_eight(b, p.w + g * p.ldw + k, p.K - k);
-              g8_eight(d, p.w + u * p.ldw + k, p.K - k);
-              const int block = k >> 7;
-              const unsigned sx = p.sx[row * p.ldsx + block];
+            for (unsigned c = __ballot_sync(0xffffffffu, taken); c && (pass || !over); c &= c - 1) {
+              const long long g = q.ft * 128 + 4 * (__ffs(c) - 1) + e, u = p.feats + g;
+              double tg = 0.0, tu = 0.0;
+#pragma unroll 1
+              for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
+                float a[8], b[8], d[8];
+                double sg = 0.0, su = 0.0;
+                g8_eight(a, p.x + row * p.ldx + k, p.K - k);
+                g8_eight(b, p.w + g * p.ldw + k, p.K - k);
+                g8_eight(d, p.w + u * p.ldw + k, p.K - k);
+                const int block = k >> 7;
+                const unsigned sx = p.sx[row * p.ldsx + block];
 #pragma unroll
-              for (int j = 0; j < 8; j++) {
-                sg += a[j] * b[j];                           // (a product of two such numbers has 8 bits)
-                su += a[j] * d[j];
+                for (int j = 0; j < 8; j++) {
+                  sg += a[j] * b[j];                           // (a product of two such numbers has 8 bits)
+                  su += a[j] * d[j];
+                }
+                tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
+                tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
               }
-              tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
-              tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
-            }
-            for (int d = 16; d; d >>= 1) {
-              tg += __shfl_xor_sync(0xffffffffu, tg, d);
-              tu += __shfl_xor_sync(0xffffffffu, tu, d);
-            }
-            __syncthreads();                                   // (what the sums before were is no longer read)
-            if (lane == 0) {
-              sums[warp][0] = tg;
-              sums[warp][1] = tu;
-            }
-            __syncthreads();
-            tg = bias ? bias[g] : 0.f;
-            tu = bias ? bias[u] : 0.f;
+              for (int d = 16; d; d >>= 1) {
+                tg += __shfl_xor_sync(0xffffffffu, tg, d);
+                tu += __shfl_xor_sync(0xffffffffu, tu, d);
+              }
+              __syncthreads();                                   // (what the sums before were is no longer read)
+              if (lane == 0) {
+                sums[warp][0] = tg;
+                sums[warp][1] = tu;
+              }
+              __syncthreads();
+              tg = bias ? bias[g] : 0.f;
+              tu = bias ? bias[u] : 0.f;
 #pragma unroll 1
-            for (int j = 0; j < G8_THREADS / 32; j++) {
-              tg += sums[j][0];
-              tu += sums[j][1];
+              for (int j = 0; j < G8_THREADS / 32; j++) {
+                tg += sums[j][0];
+                tu += sums[j][1];
+              }
+              const double h = fp8_gated_64(tg, tu, p.act);
+              if (!pass) over = fabs(h) > edge;
+              else if (lane == __ffs(c) - 1) (e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3]) = (float)(h * unit);
             }
-            over = fabs(fp8_gated_64(tg, tu, p.act)) > edge;
           }
         }
         __syncthreads();                                       // all have read the row

@@ -143,3 +143,50 @@ def test_gated_scales_of_deep_gates(T, plan, act):
     s = out.s.float().double()
     assert (s == torch.where(h > 1.75, 2.0 ** -7, 2.0 ** -8))[:, far].all()
     kernels.check_status()
+
+
+@pytest.mark.parametrize("T,plan", [(3, None), (30, (1, 256, 1)), (90, (1, 256, 1)), (200, (2, 256, 1))])
+@pytest.mark.parametrize("lower", [False, True])
+def test_numbers_of_blocks_whose_scale_is_looked_at_again(lower, T, plan):
+    """Beside the largest magnitude near the edge lie some among e4m3's smallest numbers: whichever scale it comes to be, they are rounded once,
+    to it.  The tensor cores cut sums off towards zero: a product of sums seems smaller, and ``lower`` one of a gate about -3 larger."""
+    from qwen_decoder_b200 import kernels
+    K, blocks = 8192, 64
+    F = 128 * blocks
+    x = rows_of(torch.empty(1, K, device=DEV).normal_().abs().expand(T, K).contiguous())
+    some = torch.empty(2 * blocks, K, device=DEV).normal_().abs() * 64 / K       # the features that count: gates, then ups
+    if lower:
+        some[:blocks] *= -3 / 26
+        some[blocks:] = 0
+    some = rows_of(some)
+    at = 128 * torch.arange(blocks, device=DEV) + torch.arange(blocks, device=DEV) * 37 % 128
+    w = room(2 * F, K)
+    w.q.view(torch.uint8).zero_()
+    w.s.view(torch.uint8).fill_(127)
+    for part, to in ((slice(0, blocks), at), (slice(blocks, None), at + F)):
+        w.q.view(torch.uint8)[to] = some.q.view(torch.uint8)[part]
+        w.s.view(torch.uint8)[to] = some.s.view(torch.uint8)[part]
+    z = (value(x)[:1] @ value(some).T)[0]
+    gate, up = z[:blocks], z[blocks:]
+    # the others: gates of 30, the activation of which is 30, and ups that bring them to 2^-11 to 2^-4 of the scale
+    bias = torch.zeros(2 * F, device=DEV)
+    bias[:F] = 30
+    bias[at] = 0 if lower else torch.clamp(30 - gate, min=0).float()
+    closed = gated(gate + bias[at].double(), 1.0, 0)
+    edge = 1.75 * torch.exp2(torch.floor(torch.log2(closed.abs() * (1 if lower else up) / 1.75)))
+    small = torch.exp2(-11 + 7 * torch.rand(F, device=DEV)) * (1 - 2 * torch.randint(0, 2, (F,), device=DEV))
+    bias[F:] = small * (edge / 448).float().repeat_interleave(128) / 30
+    off = torch.linspace(-3e-6, 3e-6, blocks, device=DEV, dtype=torch.float64)[torch.randperm(blocks, device=DEV)]
+    bias[at + F] = (edge * (1 + off) / closed - up).float()
+    g = torch.zeros(2 * F, dtype=torch.float64, device=DEV)
+    g[at], g[at + F] = gate, up
+    h = gated((g + bias.double())[:F], (g + bias.double())[F:], 0)
+    peak = h[at].abs()
+    far = (peak / edge - 1).abs() > 1e-10
+    assert far.sum() > blocks - 4
+    out = room(T, F)
+    kernels.gemm_fp8_gated(x, w, bias, out, 0, plan)
+    assert (out.s.float().double() == torch.where(peak > edge, 2 * edge / 448, edge / 448))[:, far].all()
+    # of the largest the sums' error, of the others the activation's
+    check_rows(out, h.expand(T, F), (6 * 2.0 ** -23 * h.abs()).scatter(0, at, 1e-5 * peak).expand(T, F))
+    kernels.check_status()
