@@ -144,7 +144,7 @@ def _extension_command(src: str, out: str) -> List[str]:
     """The Python module ``qd_<name>`` of a ``.cpp`` file, against the interpreter's and torch's headers and libraries."""
     torch_dir, lib = _torch_folder(), os.path.join(_torch_folder(), "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(find_nvcc())), "include")
-    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", CSRC,
             "-I", sysconfig.get_paths()["include"], "-I", os.path.join(torch_dir, "include"), "-I", cuda, "-o", out, src, "-L", lib,
             f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
@@ -152,9 +152,12 @@ def _extension_command(src: str, out: str) -> List[str]:
 def _key(name: str, nvcc: str) -> str:
     h = hashlib.sha256()
     if LIBRARIES[name].endswith(".cpp"):
-        with open(os.path.join(CSRC, LIBRARIES[name]), "rb") as fh, open(os.path.join(_torch_folder(), "version.py"), "rb") as version:
-            h.update(fh.read() + b"\0" + version.read() + sys.version.encode())
-        h.update(" ".join(_extension_command("", "")).encode())
+        with open(os.path.join(_torch_folder(), "version.py"), "rb") as version:
+            h.update(version.read() + sys.version.encode())
+        h.update(" ".join(a for a in _extension_command("", "") if a != CSRC).encode())
+        for f in [LIBRARIES[name], "entry_points.h"]:
+            with open(os.path.join(CSRC, f), "rb") as fh:
+                h.update(f.encode() + b"\0" + fh.read() + b"\0")
         return h.hexdigest()[:16]
     for f in [LIBRARIES[name]] + HEADERS + EXTRA_DEPS.get(name, []):
         with open(os.path.join(CSRC, f), "rb") as fh:

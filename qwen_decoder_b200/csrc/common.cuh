@@ -8,11 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#define QD_F32 0
-#define QD_BF16 1
-
-// Returned by launchers for arguments a kernel refuses (never a wrong result).
-#define QD_ERR_UNSUPPORTED 10001
+#include "entry_points.h"
 
 typedef __nv_bfloat16 bf16;
 
@@ -36,8 +32,6 @@ __device__ __forceinline__ float warp_max(float v) {
 
 // Gated activations, by code: silu(g) * u, or gelu(g) * u with gelu(z) = 0.5 z (1 + tanh(c (z + 0.044715 z^3))), c =
 // sqrt(2 / pi).  Since (1 + tanh(y)) / 2 = 1 / (1 + exp(-2 y)), both are g / (1 + exp(-a)) * u with another a.
-#define QD_ACT_SILU 0
-#define QD_ACT_GELU_TANH 2
 __device__ __forceinline__ float qd_gate_arg(float g, int act) {
   return act == QD_ACT_GELU_TANH ? 1.5957691216057308f * fmaf(0.044715f * g * g, g, g) : g;
 }

@@ -1,8 +1,25 @@
-// Prototypes of the kernel launchers that the native prompt-step executor (prompt_exec.cu) calls
-// through pointers.  The libraries that define them include this file as well, so that a definition
-// that drifts from its prototype does not compile.
+// Prototypes of the kernel launchers that the native prompt-step executor (prompt_exec.cu) and the host's
+// calls (host_calls.cpp) call through pointers, and the codes that launchers take.  The libraries that define them
+// include this file as well, so that a definition that drifts from its prototype does not compile.
 #pragma once
 #include <cuda_runtime.h>
+
+// element types
+#define QD_F32 0
+#define QD_BF16 1
+// returned by launchers for arguments a kernel refuses (never a wrong result)
+#define QD_ERR_UNSUPPORTED 10001
+// gated activations
+#define QD_ACT_SILU 0
+#define QD_ACT_GELU_TANH 2
+// rows in 8 bits: features to a scale; what becomes of a product's sums; tokens that ``qd_gemm_fp8_few`` takes
+#define QD_FP8_BLOCK 128
+#define QD_FP8_STORE 0
+#define QD_FP8_GATED 2
+#define QD_FP8_FEW_TOKENS 16
+// log probabilities
+#define QD_LOGPROBS_MAX_TOP 32
+#define QD_LOGPROBS_MAX_VOCABULARY (1 << 22)
 
 extern "C" {
 int qd_add_rmsnorm(float* x, const void* delta, int delta_dtype, const float* w, void* out, int out_dtype,
@@ -22,6 +39,9 @@ int qd_add_rmsnorm_fp8(float* x, const void* delta, int delta_dtype, const float
 int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx, long long ldsx,
                 const float* bias, void* out, int out_dtype, long long ldo, void* s_out, long long lds_out, int T, int N, int K, int cg,
                 int bn, int splits, int epi, int resident, int sms, cudaStream_t stream);
+int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out);
+int qd_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob, float* entropy, int* top_ids,
+                      float* top_logprobs, int R, int V, int top, int sms, cudaStream_t stream);
 int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
                     long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, int T, int N, int K, int resident,
                     int sms, cudaStream_t stream);

@@ -8,7 +8,7 @@
 #pragma once
 #include "common.cuh"
 
-#define FP8_BLOCK 128
+#define FP8_BLOCK QD_FP8_BLOCK
 
 // ``m``: the bits of the largest magnitude of a block (magnitudes order as their bits do, infinities and NaN above all numbers)
 __device__ __forceinline__ unsigned fp8_scale_byte(unsigned m) {

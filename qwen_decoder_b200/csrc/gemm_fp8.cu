@@ -41,9 +41,9 @@
 #define G8_FEW 16                             // tokens of a gated product whose sums fit the epilogue's part of shared memory
 #define G8_OVERLAP 64                         // columns that two accumulators of 256 share (the first that the epilogue reads)
 
-#define G8_STORE 0
+#define G8_STORE QD_FP8_STORE
 #define G8_SHARED 1                           // K shared by a cluster
-#define G8_GATED 2
+#define G8_GATED QD_FP8_GATED
 
 struct G8Params {
   int act, T, N, K;

@@ -244,7 +244,7 @@ extern "C" int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, lon
                                long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, int T, int N, int K, int resident,
                                int sms, cudaStream_t stream) {
   if (T <= 0 || N <= 0) return 0;
-  if (T > 16 || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || ((((uintptr_t)W | (uintptr_t)X) & 15)) ||
+  if (T > QD_FP8_FEW_TOKENS || N > (1 << 30) || K <= 0 || K > (1 << 30) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || ((((uintptr_t)W | (uintptr_t)X) & 15)) ||
       sms < 1 || !out)
     return QD_ERR_UNSUPPORTED;
   FwParams p;

@@ -12,6 +12,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "entry_points.h"
+
 #include <map>
 #include <sstream>
 #include <string>
@@ -19,8 +21,9 @@
 
 namespace {
 
-constexpr int F32 = 0, BF16 = 1, BLOCK = 128, UNSUPPORTED = 10001, STORE = 0, GATED = 2, ACT_SILU = 0, ACT_GELU = 2, FEW_TOKENS = 16, MOST_TOP = 32;
-constexpr int64_t MOST_VOCABULARY = 1 << 22;
+constexpr int F32 = QD_F32, BF16 = QD_BF16, BLOCK = QD_FP8_BLOCK, STORE = QD_FP8_STORE, GATED = QD_FP8_GATED, ACT_SILU = QD_ACT_SILU;
+constexpr int ACT_GELU = QD_ACT_GELU_TANH, FEW_TOKENS = QD_FP8_FEW_TOKENS, MOST_TOP = QD_LOGPROBS_MAX_TOP;
+constexpr int64_t MOST_VOCABULARY = QD_LOGPROBS_MAX_VOCABULARY;
 
 PyObject *g_error, *g_resolve, *g_rows_type;        // KernelError; (library, function) -> address, ("sms", device) -> multiprocessors; Fp8Rows
 
@@ -59,11 +62,17 @@ const at::Tensor& tensor(PyObject* o, const char* what) {
   return THPVariable_Unpack(o);
 }
 const at::Tensor* tensor_or_none(PyObject* o, const char* what) { return o == Py_None ? nullptr : &tensor(o, what); }
-void* address(const at::Tensor& t) {
+// of whatever a launcher takes there
+struct Address {
+  void* at;
+  template <typename T>
+  operator T*() const { return static_cast<T*>(at); }
+};
+Address address(const at::Tensor& t) {
   if (!t.is_cuda()) refuse("kernel argument is not on a CUDA device (there is no CPU path)");
-  return t.data_ptr();
+  return {t.data_ptr()};
 }
-void* address(const at::Tensor* t) { return t ? address(*t) : nullptr; }
+Address address(const at::Tensor* t) { return t ? address(*t) : Address{nullptr}; }
 std::string sizes(const at::Tensor& t) {
   std::ostringstream s;
   s << t.sizes();
@@ -71,7 +80,7 @@ std::string sizes(const at::Tensor& t) {
 }
 void done(int code, const char* what) {
   if (code == 0) return;
-  if (code == UNSUPPORTED) refuse(what, ": the kernel refuses these sizes or types");
+  if (code == QD_ERR_UNSUPPORTED) refuse(what, ": the kernel refuses these sizes or types");
   refuse(what, ": CUDA error ", code);
 }
 
@@ -133,21 +142,12 @@ int act_of(PyObject* o, const char* what) {
 cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // ---- the launchers
-typedef int RowsFn(const void*, int, long long, int, long long, int, int, const void*, void*, long long, void*, long long, int, int, cudaStream_t);
-typedef int NormFn(void*, const void*, int, const void*, const void*, void*, long long, void*, long long, const void*, int, int, float, int, int, long long,
-                   cudaStream_t);
-typedef int PlanFn(int, int, int, int, int, int, int*, int*, int*);
-typedef int ProductFn(const void*, long long, const void*, long long, const void*, long long, const void*, long long, const void*, void*, int, long long,
-                      void*, long long, int, int, int, int, int, int, int, int, int, cudaStream_t);
-typedef int FewFn(const void*, long long, const void*, long long, const void*, long long, const void*, long long, const void*, void*, int, long long, int,
-                  int, int, int, int, cudaStream_t);
-typedef int LogprobsFn(const void*, int, long long, const void*, void*, void*, void*, void*, int, int, int, int, cudaStream_t);
-RowsFn* g_rows;
-NormFn* g_norm;
-PlanFn* g_plan;
-ProductFn* g_product;
-FewFn* g_few;
-LogprobsFn* g_logprobs;
+decltype(qd_rows_fp8)* g_rows;
+decltype(qd_add_rmsnorm_fp8)* g_norm;
+decltype(qd_gemm_fp8_plan)* g_plan;
+decltype(qd_gemm_fp8)* g_product;
+decltype(qd_gemm_fp8_few)* g_few;
+decltype(qd_token_logprobs)* g_logprobs;
 
 struct Plan { int cg, bn, splits; };
 // (kept by sizes: a few microseconds of estimates)
@@ -345,13 +345,13 @@ CALL(token_logprobs, 3)
   const int64_t most = std::min<int64_t>(MOST_TOP, V);
   if (V < 1 || top < 0 || top > most) refuse("token_logprobs: top must be between 0 and ", most, ", got ", top);
   if (R > INT32_MAX / 16) refuse("token_logprobs: ", R, " rows");
-  void *z_at = address(z), *t_at = address(tokens);
+  const Address z_at = address(z), t_at = address(tokens);
   const auto options = z.options();
   const auto f32 = options.dtype(at::kFloat), i32 = options.dtype(at::kInt);
   at::Tensor lp = at::empty_strided({R}, {1}, f32), entropy = at::empty_strided({R}, {1}, f32);
   at::Tensor ids = at::empty_strided({R, top}, {top, 1}, i32), lps = at::empty_strided({R, top}, {top, 1}, f32);
-  done(entry(g_logprobs, "logprobs", "qd_token_logprobs")(z_at, dt == at::kFloat ? F32 : BF16, z.stride(0), t_at, lp.data_ptr(), entropy.data_ptr(),
-                                                         ids.data_ptr(), lps.data_ptr(), (int)R, (int)V, (int)top, multiprocessors(z.get_device()),
+  done(entry(g_logprobs, "logprobs", "qd_token_logprobs")(z_at, dt == at::kFloat ? F32 : BF16, z.stride(0), t_at, address(lp), address(entropy),
+                                                         address(ids), address(lps), (int)R, (int)V, (int)top, multiprocessors(z.get_device()),
                                                          stream_of(z)), "token_logprobs");
   PyObject* out = PyTuple_New(4);
   if (!out) throw PythonError{};

@@ -25,13 +25,14 @@
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_EACH 16                           // logits of a thread's tile
 #define LP_TILE (LP_THREADS * LP_EACH)
-#define LP_MAX_TOP 32
+#define LP_MAX_TOP QD_LOGPROBS_MAX_TOP
 #define LP_MAX_SHARES 16
 #define LP_CHUNK 512                         // a warp's logits of a tile
 #define LP_HITS 64                           // logits of a chunk that join without being chosen one by one
 #define LP_LANE 16                           // chunks to a lane of the warp that chooses
 #define LP_MAX_CHUNKS (32 * LP_LANE)         // of a CTA
 #define LP_MAX_VOCABULARY (LP_MAX_SHARES * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE)
+static_assert(LP_MAX_VOCABULARY == QD_LOGPROBS_MAX_VOCABULARY, "what the host's side refuses");
 #define LP_LOWEST (-3.402823466e38f)
 
 struct LpArgs {
