@@ -974,8 +974,13 @@ static int g8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const f
 // How many clusters of ``n`` CTAs run at a time: they lie within a group of multiprocessors, whose sizes need not be a multiple of theirs
 // (of 148 multiprocessors 5 to a cluster leave some idle; a cluster too many doubles the time).
 static int g8_clusters(int n, int sms) {
-  static int known[9];
-  if (known[n]) return known[n];
+  static int known[64][9];                     // by device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    (void)cudaGetLastError();
+    return sms / (n + 1);
+  }
+  if (known[dev][n]) return known[dev][n];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n * 148);
   cfg.blockDim = dim3(G8_THREADS);
@@ -992,7 +997,7 @@ static int g8_clusters(int n, int sms) {
     (void)cudaGetLastError();
     got = sms / (n + 1);
   }
-  return known[n] = got;
+  return known[dev][n] = got;
 }
 
 extern "C" int qd_gemm_fp8_clusters(int n, int sms) { return n >= 1 && n <= 8 ? g8_clusters(n, sms) : 0; }

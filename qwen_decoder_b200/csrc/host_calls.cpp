@@ -150,14 +150,14 @@ decltype(qd_gemm_fp8_few)* g_few;
 decltype(qd_token_logprobs)* g_logprobs;
 
 struct Plan { int cg, bn, splits; };
-// (kept by sizes: a few microseconds of estimates)
-Plan plan_of(int T, int N, int K, int epi, int code, int sms) {
+// (kept by sizes and device: a few microseconds of estimates)
+Plan plan_of(int T, int N, int K, int epi, int code, int device) {
   static std::map<std::tuple<int, int, int, int, int, int>, Plan> kept;
-  const auto key = std::make_tuple(T, N, K, epi & 255, code, sms);
+  const auto key = std::make_tuple(T, N, K, epi & 255, code, device);
   const auto at = kept.find(key);
   if (at != kept.end()) return at->second;
   Plan p;
-  if (!entry(g_plan, "gemm_fp8", "qd_gemm_fp8_plan")(T, N, K, epi, code, sms, &p.cg, &p.bn, &p.splits))
+  if (!entry(g_plan, "gemm_fp8", "qd_gemm_fp8_plan")(T, N, K, epi, code, multiprocessors(device), &p.cg, &p.bn, &p.splits))
     refuse("gemm_fp8: no product of ", T, " x ", K, " by ", N, " x ", K);
   if (kept.size() >= 4096) kept.clear();
   return kept[key] = p;
@@ -185,7 +185,7 @@ void product(const Rows& x, const Rows& w, const at::Tensor* bias, void* out, in
   bool few = false;
   if (plan == Py_None) {
     few = (epi & 255) == STORE && few_wanted(T, N, K, sms);
-    if (!few) p = plan_of(T, N, K, epi, code, sms);
+    if (!few) p = plan_of(T, N, K, epi, code, x.q->get_device());
   } else {
     if (!PyArg_ParseTuple(plan, "iii", &p.cg, &p.bn, &p.splits)) throw PythonError{};
     few = p.cg == 0 && (epi & 255) == STORE;
@@ -326,7 +326,7 @@ CALL(gemm_fp8_plan, 6)
   if (T < 1 || N < 1 || K < 1 || T > INT32_MAX || N > INT32_MAX || K > INT32_MAX) refuse("gemm_fp8_plan: no product of ", T, " x ", K, " by ", N, " x ", K);
   Plan p = {0, 0, 0};
   const int sms = multiprocessors(device);
-  if (gated || !few_wanted(T, N, K, sms)) p = plan_of((int)T, (int)N, (int)K, gated ? GATED : STORE, f32 ? F32 : BF16, sms);
+  if (gated || !few_wanted(T, N, K, sms)) p = plan_of((int)T, (int)N, (int)K, gated ? GATED : STORE, f32 ? F32 : BF16, device);
   return Py_BuildValue("iii", p.cg, p.bn, p.splits);
 END
 

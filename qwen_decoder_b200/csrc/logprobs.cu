@@ -384,10 +384,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
   }
 }
 
-// How many clusters of ``n`` CTAs run at a time
-static int lp_clusters(int n, int sms) {
-  static int known[LP_MAX_SHARES + 1];
-  if (known[n]) return known[n];
+// How many clusters of ``n`` CTAs run at a time on device ``dev``, the current one
+static int lp_clusters(int n, int sms, int dev) {
+  static int known[64][LP_MAX_SHARES + 1];
+  if (known[dev][n]) return known[dev][n];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n * 1024);
   cfg.blockDim = dim3(LP_THREADS);
@@ -402,7 +402,7 @@ static int lp_clusters(int n, int sms) {
     (void)cudaGetLastError();
     got = 3 * sms / n;
   }
-  return known[n] = got;
+  return known[dev][n] = got;
 }
 
 // logits [R, V] float32 or bfloat16, rows ``ld`` elements apart; tokens int32 [R] (outside of [0, V): the log probability NaN); logprob and
@@ -434,7 +434,7 @@ extern "C" int qd_token_logprobs(const void* logits, int dtype, long long ld, co
   const int tiles = (V + LP_TILE - 1) / LP_TILE;
   a.shares = 1;
   for (int n = 2; n <= LP_MAX_SHARES && tiles / n >= 2 && 2 * (tiles / n) * LP_WARPS >= 3 * top; n *= 2) {
-    if (tiles / n >= 4 ? R > lp_clusters(n, sms) : n > 8 || 2ll * R * n > 5ll * sms) break;
+    if (tiles / n >= 4 ? R > lp_clusters(n, sms, dev) : n > 8 || 2ll * R * n > 5ll * sms) break;
     a.shares = n;
   }
   while (a.shares * (LP_MAX_CHUNKS / LP_WARPS) * LP_TILE < V) a.shares++;      // a CTA keeps so many maxima
