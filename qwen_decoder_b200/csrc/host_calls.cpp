@@ -187,7 +187,10 @@ void product(const Rows& x, const Rows& w, const at::Tensor* bias, void* out, in
     few = (epi & 255) == STORE && few_wanted(T, N, K, sms);
     if (!few) p = plan_of(T, N, K, epi, code, x.q->get_device());
   } else {
-    if (!PyArg_ParseTuple(plan, "iii", &p.cg, &p.bn, &p.splits)) throw PythonError{};
+    if (!PyTuple_Check(plan) || !PyArg_ParseTuple(plan, "iii", &p.cg, &p.bn, &p.splits)) {
+      PyErr_Clear();
+      refuse(what, ": plan must be a tuple of three whole numbers or None");
+    }
     few = p.cg == 0 && (epi & 255) == STORE;
   }
   if (few)

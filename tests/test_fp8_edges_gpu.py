@@ -190,3 +190,13 @@ def test_numbers_of_blocks_whose_scale_is_looked_at_again(lower, T, plan):
     # of the largest the sums' error, of the others the activation's
     check_rows(out, h.expand(T, F), (6 * 2.0 ** -23 * h.abs()).scatter(0, at, 1e-5 * peak).expand(T, F))
     kernels.check_status()
+
+
+@pytest.mark.parametrize("plan", [[1, 64, 1], (1, 64), (1, 64, 1, 1), (1, "64", 1), (1, 64, 2 ** 40), 64, "plan"])
+def test_plans_that_are_none(plan):
+    from qwen_decoder_b200 import kernels
+    x, w, _ = operands(3, 64, 256)
+    with pytest.raises(kernels.KernelError, match="plan"):
+        kernels.gemm_fp8(x, w, None, torch.empty(3, 64, device=DEV), plan)
+    with pytest.raises(kernels.KernelError, match="plan"):
+        kernels.gemm_fp8_gated(x, w, None, room(3, 32), 0, plan)
