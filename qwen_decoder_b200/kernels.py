@@ -996,7 +996,8 @@ def gemm_fp8(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: torch.Te
 
 def gemm_fp8_plan(T: int, N: int, K: int, gated: bool = False, dtype: torch.dtype = torch.bfloat16, device=None) -> tuple:
     """The plan that ``gemm_fp8`` (or ``gemm_fp8_gated``) takes by itself for T rows of x and N of w, results of ``dtype``."""
-    index = torch.cuda.current_device() if device is None else _device_of(device).index
+    index = None if device is None else _device_of(device).index
+    index = torch.cuda.current_device() if index is None else index        # (a device without a number is the current one)
     return (_host or _host_calls()).gemm_fp8_plan(T, N, K, gated, dtype == torch.float32, index)
 
 

@@ -200,3 +200,9 @@ def test_plans_that_are_none(plan):
         kernels.gemm_fp8(x, w, None, torch.empty(3, 64, device=DEV), plan)
     with pytest.raises(kernels.KernelError, match="plan"):
         kernels.gemm_fp8_gated(x, w, None, room(3, 32), 0, plan)
+
+
+def test_plans_of_the_current_device():
+    from qwen_decoder_b200 import kernels
+    for sizes in ((4, 2048, 2048), (40, 4608, 3584), (500, 3584, 18944)):
+        assert kernels.gemm_fp8_plan(*sizes) == kernels.gemm_fp8_plan(*sizes, device="cuda") == kernels.gemm_fp8_plan(*sizes, device=torch.device(DEV))
