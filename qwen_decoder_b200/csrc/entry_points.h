@@ -40,6 +40,7 @@ int qd_gemm_fp8(const void* W, long long ldw, const void* sw, long long ldsw, co
                 const float* bias, void* out, int out_dtype, long long ldo, void* s_out, long long lds_out, int T, int N, int K, int cg,
                 int bn, int splits, int epi, int resident, int sms, cudaStream_t stream);
 int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* cg_out, int* bn_out, int* splits_out);
+int qd_gemm_fp8_few_wanted(int T, int N, int K, int sms);
 int qd_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob, float* entropy, int* top_ids,
                       float* top_logprobs, int R, int V, int top, int sms, cudaStream_t stream);
 int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,

@@ -237,6 +237,35 @@ static int fw_launch(const FwParams& p, int ctas, cudaStream_t stream) {
   return qd_last_error();
 }
 
+// Few tiles of a long K: K shared by as many CTAs as run beside one another, two to a multiprocessor, two blocks to a warp at least
+// (us with 1, 2 and 4 of them: 2,048 x 11,008 12.8, 8.6 and 9.9, 2,048 x 2,048 3.1, 3.7 and 5.4, 200 x 12,000 8.9, 5.8 and 4.3); else the
+// tiles evenly over these, in rounds.
+struct FwCut { int blocks, tiles, shares, rounds; };
+static FwCut fw_cut(int N, int K, int sms) {
+  const int most = 2 * sms;
+  FwCut c = {(K + FP8_BLOCK - 1) / FP8_BLOCK, (N + FW_ROWS - 1) / FW_ROWS, 1, 0};
+  while (c.shares < 8 && c.tiles * c.shares * 2 <= most && c.blocks >= c.shares * 4 * FW_WARPS) c.shares *= 2;
+  c.rounds = (c.tiles * c.shares + most - 1) / most;
+  return c;
+}
+
+// Whether this kernel is the faster one for T tokens, or the one on tcgen05 is.  Its time goes by the steps that a CTA makes one after the other, each a
+// block to each of its warps, and an end to each tile; the other's by bytes, from 4 us on.  Measured in captured graphs at 274 sizes of 0.5 to
+// 50 MB, K 256 to 18,944, with 1 to 16 tokens, us less here on average:
+//   steps                1     2     3     4     5     6     7     8    10
+//   up to 8 tokens      1.7   1.4   1.4   0.7   0.0  -0.4  -1.2  -1.3  -2.9
+//   9 to 16             1.4   0.6   0.0  -0.9  -1.9  -2.9  -4.0  -4.6  -6.9
+// Between other launches it is ahead by 1 to 4 us more (the other's code has to be fetched again): among the layers of ten widths, products of up
+// to 6 steps and 8 tokens took 1.0 to 6.5 us less here, of up to 4 steps and 16 tokens 0.7 to 4.7 less but for two (0.6 and 1.1 more), of 5
+// and more steps and 16 tokens 0.9 to 21 more.  In a graph of nothing else the rule's choices take 0.5 % longer than the best of both up to 8
+// tokens, 1.3 % up to 16.
+extern "C" int qd_gemm_fp8_few_wanted(int T, int N, int K, int sms) {
+  if (T > QD_FP8_FEW_TOKENS || N > (1 << 30) || K <= 0 || K > (1 << 30) || sms < 1) return 0;
+  const FwCut c = fw_cut(N, K, sms);
+  const long long steps = ((c.blocks + c.shares - 1) / c.shares + FW_WARPS - 1) / FW_WARPS, all = c.rounds * (steps + 1);
+  return T <= 8 ? all <= 7 : all + (c.shares > 1) <= 5;
+}
+
 // X [T, K] and W [N, K] e4m3, rows ``ldx`` and ``ldw`` bytes apart (multiples of 16, as the addresses), with scales sx and sw, rows ``ldsx``
 // and ``ldsw`` bytes apart; out [T, N] = X W^T (+ bias float32 [N]), bfloat16 or float32, rows ``ldo`` apart.  T up to 16.
 // ``resident``: W and sw are written by nothing that may still run on the stream (they are asked for before that has ended).
@@ -251,16 +280,10 @@ extern "C" int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, lon
   p.w = (const unsigned char*)W; p.sw = (const unsigned char*)sw; p.x = (const unsigned char*)X; p.sx = (const unsigned char*)sx;
   p.ldw = ldw; p.ldsw = ldsw; p.ldx = ldx; p.ldsx = ldsx; p.ldo = ldo; p.bias = bias; p.out = out;
   p.T = T; p.N = N; p.K = K; p.resident = resident;
-  p.blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
-  p.tiles = (N + FW_ROWS - 1) / FW_ROWS;
+  const FwCut c = fw_cut(N, K, sms);
+  p.blocks = c.blocks; p.tiles = c.tiles; p.shares = c.shares;
   if (ldsx < p.blocks || ldsw < p.blocks) return QD_ERR_UNSUPPORTED;
-  // Few tiles of a long K: K shared by as many CTAs as run beside one another, two to a multiprocessor, two blocks to a warp at least
-  // (us with 1, 2 and 4 of them: 2,048 x 11,008 12.8, 8.6 and 9.9, 2,048 x 2,048 3.1, 3.7 and 5.4, 200 x 12,000 8.9, 5.8 and 4.3); else the
-  // tiles evenly over these.
-  const int most = 2 * sms;
-  p.shares = 1;
-  while (p.shares < 8 && p.tiles * p.shares * 2 <= most && p.blocks >= p.shares * 4 * FW_WARPS) p.shares *= 2;
-  const int rounds = (p.tiles * p.shares + most - 1) / most, workers = (p.tiles + rounds - 1) / rounds, ctas = workers * p.shares;
+  const int workers = (c.tiles + c.rounds - 1) / c.rounds, ctas = workers * c.shares;
 #define GO(NT, TO) return p.shares > 1 ? fw_launch<NT, TO, true>(p, ctas, stream) : fw_launch<NT, TO, false>(p, ctas, stream)
   if (out_dtype == QD_BF16) { if (T <= 8) GO(1, bf16); else GO(2, bf16); }
   if (out_dtype == QD_F32) { if (T <= 8) GO(1, float); else GO(2, float); }

@@ -147,6 +147,7 @@ decltype(qd_add_rmsnorm_fp8)* g_norm;
 decltype(qd_gemm_fp8_plan)* g_plan;
 decltype(qd_gemm_fp8)* g_product;
 decltype(qd_gemm_fp8_few)* g_few;
+decltype(qd_gemm_fp8_few_wanted)* g_few_wanted;
 decltype(qd_token_logprobs)* g_logprobs;
 
 struct Plan { int cg, bn, splits; };
@@ -162,13 +163,9 @@ Plan plan_of(int T, int N, int K, int epi, int code, int device) {
   if (kept.size() >= 4096) kept.clear();
   return kept[key] = p;
 }
-// The few-token kernel is the faster one up to 8 tokens and 23 MB of weights, up to 16 and 10 MB (times beside it), or 17 MB whose tiles of 16
-// rows nearly fill its two CTAs to a multiprocessor at once (16 tokens between other launches, us less than the other one: 3,584 x 3,584 0.6,
-// 4,608 x 3,584 3.6; but 2,560 x 6,144 in 160 CTAs 1.7 more, 5,120 x 3,584 in two rounds 3.5).
+// (no kernel is asked for sizes that it does not take)
 bool few_wanted(int64_t T, int64_t N, int64_t K, int sms) {
-  if (T > FEW_TOKENS) return false;
-  const int64_t tiles = (N + 15) / 16, most = 2 * sms;
-  return N * K <= (T <= 8 ? 23000000 : tiles <= most && 4 * tiles >= 3 * most ? 17000000 : 10000000);
+  return T <= FEW_TOKENS && entry(g_few_wanted, "gemm_fp8_few", "qd_gemm_fp8_few_wanted")((int)T, (int)N, (int)K, sms);
 }
 
 void product(const Rows& x, const Rows& w, const at::Tensor* bias, void* out, int code, int64_t ldo, void* s_out, int64_t lds_out, int epi, PyObject* plan,
