@@ -201,7 +201,7 @@ __device__ __forceinline__ void g8_store_rows(unsigned char* rows, TO* dst, long
 // h = act(g) u of 64 features from ``col0`` on, zero from ``feats`` on: h holds the gate's sums (``gate``) or up's, the others lie in tensor
 // memory
 template <int ACT>
-__device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool gate, const float* bias, int col0, int feats) {
+__device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool gate, const float* bias, int col0, int feats, float& deepest) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     float o[16];
@@ -213,7 +213,10 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
       g8_bias16(o, bias + (gate ? feats : 0), col0 + 16 * i, feats);
     }
 #pragma unroll
-    for (int e = 0; e < 16; e++) x[e] = fp8_gated(gate ? x[e] : o[e], gate ? o[e] : x[e], ACT);
+    for (int e = 0; e < 16; e++) {
+      deepest = fminf(deepest, gate ? x[e] : o[e]);
+      x[e] = fp8_gated_short(gate ? x[e] : o[e], gate ? o[e] : x[e], ACT);
+    }
     if (col0 + 16 * i + 16 > feats)
 #pragma unroll
       for (int e = 0; e < 16; e++)
@@ -223,19 +226,26 @@ __device__ __forceinline__ void g8_activate(float (&h)[64], unsigned other, bool
 
 // Where a block's largest magnitude is so near the last one of a scale that the sums' cut-off decides, its sums are made again at the kernel's
 // end: a scale is then that of the sums as they are, not of the order of their additions.  (Without it 1 to 4 of a million blocks had the
-// other scale, K 2,048 to 11,008; some 25 of a million are looked at for K 3,584, 2.4 us each where the kernel ends with one: a layer of 8
+// other scale, K 2,048 to 11,008; some 25 of a million are looked at for K 3,584, 2 to 3 us each where the kernel ends with one: a layer of 8
 // tokens of the 7B sizes 56.6 -> 57.3 us.  Looked at in the epilogue itself they made its code so long that products of 8 to 512 tokens took 3
 // to 15 % more.)  How near is in units of the last place at 1.75: K / 32 additions, cut off by 0.02 to 0.09 of a unit each, by up to 0.2
-// in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error (1.75 times 6), which
-// the look itself does not have: it goes on in float64 to the end.  (A gate of -g < -2 makes g - 1 times its sum's error of it: where every gate of a
-// block lies far below -10, sums of one sign may leave the other scale, which holds the block as well but for half a step.)
-#define G8_NEAR 128                           // blocks that a CTA keeps for that; with more of them it goes through all that it has written, a tile's at a time
+// in most sums of numbers of one sign, in the gate's sum and in up's, and the activation's own error (1.75 times 5, and what the deepest gate
+// adds), which the look itself does not have: where it counts it goes on in float64 to the end.  Each thread tells of its own features, so that
+// a block may come twice; the second look finds it as it has to be.  (A gate of -g < -2 makes g - 1 times its sum's error of it: where every
+// gate of a block lies far below -10, sums of one sign may leave the other scale, which holds the block as well but for half a step.)
+// blocks that a CTA keeps for that; with more of them it goes through all that it has written, a tile's at a time
+#define G8_NEAR 128
 static int g8_doubt(int K) { return K < 1 << 24 ? (K >> 5) + 16 : 0xfffff; }
 #define G8_448 0x7e                           // as e4m3
 #define G8_224 0x76
-__device__ __forceinline__ bool g8_near(unsigned peak, int doubt) {
-  const int off = (int)(peak & 0x7fffffu) - 0x600000;
-  return peak >= 10u << 23 && peak < 0x7f800000u && abs(off) <= doubt;
+// ``most``: the largest magnitude of a block; ``peak``: that of some of its features, the lowest of whose gates is ``deepest`` (0, or below).  (Where
+// the activation is zero it has no error.)
+__device__ __forceinline__ bool g8_near(unsigned most, float peak, float deepest, int doubt, int act) {
+  const bool gelu = act == QD_ACT_GELU_TANH;
+  const int off = (int)(most & 0x7fffffu) - 0x600000;
+  if (most < 10u << 23 || most >= 0x7f800000u || abs(off) > doubt + (gelu ? 570 : 185)) return false;
+  const int margin = doubt - (int)(qd_gate_arg(fmaxf(deepest, gelu ? -10.f : -88.f), act) * (gelu ? 6.5f : 2.1f));
+  return abs((int)__float_as_uint(peak) - (int)most + off) <= margin;
 }
 // 8 e4m3 numbers of a row, zeros behind its end
 __device__ __forceinline__ void g8_eight(float (&v)[8], const unsigned char* from, int there) {
@@ -610,14 +620,15 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
               const float4 g4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((lane ^ (r & 7)) << 2));
               const float4 u4 = *reinterpret_cast<const float4*>(sums + r * 256 + ((32 + lane ^ (r & 7)) << 2));
               float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-              float peak = 0.f;
+              float peak = 0.f, deepest = 0.f;
 #pragma unroll
               for (int e = 0; e < 4; e++) {
                 if (bias && col + e < p.feats) {
                   g[e] += bias[col + e];
                   u[e] += bias[p.feats + col + e];
                 }
-                g[e] = fp8_gated(g[e], u[e], decltype(act)::value);
+                deepest = fminf(deepest, g[e]);
+                g[e] = fp8_gated_short(g[e], u[e], decltype(act)::value);
               }
               if (col + 4 > p.feats)
 #pragma unroll
@@ -626,7 +637,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
               for (int e = 0; e < 4; e++) peak = fp8_peak(peak, g[e]);
               const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(peak)), byte = fp8_scale_byte(most);
-              if (lane == 0 && g8_near(most, p.doubt)) look_at(item, r);
+              if (g8_near(most, peak, deepest, p.doubt, decltype(act)::value)) look_at(item, r);
               const float inv = fp8_inverse(byte);
               const unsigned w = fp8_pack4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
               unsigned char* to = (unsigned char*)out + (size_t)(row_x(q) + r) * p.ldo + col;
@@ -646,7 +657,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           if (n_rows > 0) {
             float4* mine = reinterpret_cast<float4*>(base) + threadIdx.x;
             const int col0 = q.ft * 128 + 64 * side;
-            float peak = 0.f;
+            float peak = 0.f, deepest = 0.f;
             const auto gate = [&](auto act) {
 #pragma unroll 1
               for (int i = 0; i < 4; i++) {
@@ -660,7 +671,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                   g8_bias16(u, bias + p.feats, col, p.feats);
                 }
 #pragma unroll
-                for (int e = 0; e < 16; e++) g[e] = fp8_gated(g[e], u[e], decltype(act)::value);
+                for (int e = 0; e < 16; e++) {
+                  deepest = fminf(deepest, g[e]);
+                  g[e] = fp8_gated_short(g[e], u[e], decltype(act)::value);
+                }
                 if (col + 16 > p.feats)                      // (asked for each feature by itself it was a jump for each, 2.5 us)
 #pragma unroll
                   for (int e = 0; e < 16; e++)
@@ -676,7 +690,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             peaks[warp & 3][side][lane] = __float_as_uint(peak);
             asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
             const unsigned most = max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]), byte = fp8_scale_byte(most);
-            if (side == 0 && lane < n_rows && g8_near(most, p.doubt)) look_at(item, quarter + lane);
+            if (lane < n_rows && g8_near(most, peak, deepest, p.doubt, p.act)) look_at(item, quarter + lane);
             const float inv = fp8_inverse(byte);
 #pragma unroll 1
             for (int c = 0; c < 4; c++) {
@@ -696,21 +710,21 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           // First the 64 columns that the next item's MMAs may overwrite, of up in the first accumulator and of the gate in the second,
           // then they may begin (with the loads in the activations' order they waited for those: 2,048 tokens of 2,048 by 2 x 11,008
           // 114 us, 1,620 TFLOP/s).
-          float h[64], peak = 0.f;
+          float h[64], peak = 0.f, deepest = 0.f;
           const unsigned one = acc + 64 * side + (buf ? 0 : 128), two = acc + 64 * side + (buf ? 128 : 0);
 #pragma unroll
           for (int i = 0; i < 4; i++) g8_ld16(one + 16 * i, *reinterpret_cast<float (*)[16]>(h + 16 * i));
           tc_ld_wait();
           if (owner) release(buf);
           const int col0 = q.ft * 128 + 64 * side;
-          if (p.act == QD_ACT_GELU_TANH) g8_activate<QD_ACT_GELU_TANH>(h, two, buf, bias, col0, p.feats);
-          else g8_activate<QD_ACT_SILU>(h, two, buf, bias, col0, p.feats);
+          if (p.act == QD_ACT_GELU_TANH) g8_activate<QD_ACT_GELU_TANH>(h, two, buf, bias, col0, p.feats, deepest);
+          else g8_activate<QD_ACT_SILU>(h, two, buf, bias, col0, p.feats, deepest);
 #pragma unroll
           for (int e = 0; e < 64; e++) peak = fp8_peak(peak, h[e]);
           peaks[warp & 3][side][lane] = __float_as_uint(peak);
           asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
           const unsigned most = max(__float_as_uint(peak), peaks[warp & 3][side ^ 1][lane]), byte = fp8_scale_byte(most);
-          if (side == 0 && lane < n_rows && g8_near(most, p.doubt)) look_at(item, quarter + lane);
+          if (lane < n_rows && g8_near(most, peak, deepest, p.doubt, p.act)) look_at(item, quarter + lane);
           const float inv = fp8_inverse(byte);
           __syncwarp();
 #pragma unroll
@@ -815,9 +829,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   }
   if constexpr (EPI == G8_GATED) {
     // (the whole CTA: a thread to 8 of k)
-    double (*sums)[2] = reinterpret_cast<double (*)[2]>(base);
     int looked = n_near;
     const bool all = looked > G8_NEAR || n_items > 1 << 25;
+    // (out from here: between other launches the way over what follows, code that has to be fetched, was 0.3 to 1.0 us of each)
+    if (looked == 0 && !all) return;
+    double (*sums)[2] = reinterpret_cast<double (*)[2]>(base);
 #pragma unroll 1
     for (int item = worker; item < n_items; item += n_workers) {
       if (all) {
@@ -858,65 +874,90 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         // The scale is the one of at most 448, or twice that.  Those that count are the largest of the rounded ones; the edge is 448 of the lower.
         const bool higher = most < __float_as_uint(400.f);
         const unsigned low = *scale - higher;
-        const double edge = 448.0 * g8_scaled(low, 127);
-        // First whether the block is over the edge; if its scale changes then also the numbers that are among e4m3's smallest, 2^-9 apart, at one
-        // of the scales: their rounded ones have lost, or would be rounded twice.  (Others are as far apart for their size at both scales.)
+        const unsigned edge = (low + 8) << 23 | 0x600000u;     // as float32
+        // the gate's and up's sums of feature ``f`` in float64, as far as this warp has them
+        const auto sums_of = [&](long long f, int first, int step, double& tg, double& tu) {
+          tg = tu = 0.0;
+#pragma unroll 1
+          for (int k = first; k < p.K; k += step) {
+            float a[8], b[8], d[8];
+            double sg = 0.0, su = 0.0;
+            g8_eight(a, p.x + row * p.ldx + k, p.K - k);
+            g8_eight(b, p.w + f * p.ldw + k, p.K - k);
+            g8_eight(d, p.w + (p.feats + f) * p.ldw + k, p.K - k);
+            const int block = k >> 7;
+            const unsigned sx = p.sx[row * p.ldsx + block];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              sg += a[j] * b[j];                               // (a product of two such numbers has 8 bits)
+              su += a[j] * d[j];
+            }
+            tg += sg * g8_scaled(sx, p.sw[f * p.ldsw + block]);
+            tu += su * g8_scaled(sx, p.sw[(p.feats + f) * p.ldsw + block]);
+          }
+          for (int d = 16; d; d >>= 1) {
+            tg += __shfl_xor_sync(0xffffffffu, tg, d);
+            tu += __shfl_xor_sync(0xffffffffu, tu, d);
+          }
+        };
+        const auto bias_of = [&](long long f) { return bias ? (double)bias[f] : 0.0; };
+        // First whether the block is over the edge, the whole CTA for each feature that may say so
         bool over = false;
 #pragma unroll 1
-        for (int pass = 0; pass < (over == higher ? 1 : 2); pass++) {
-          const double unit = g8_scaled(254 - low - over, 127) * (over ? 2.0 : 0.5);       // (of the scale before)
+        for (int e = 0; e < 4 && !over; e++) {
+          const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
 #pragma unroll 1
-          for (int e = 0; e < 4 && (pass || !over); e++) {
-            const float of = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
-            const bool taken = pass ? e < there && fabsf(of) < 0.03125f : (__float_as_uint(of) & 0x7fffffffu) == most;
-#pragma unroll 1
-            for (unsigned c = __ballot_sync(0xffffffffu, taken); c && (pass || !over); c &= c - 1) {
-              const long long g = q.ft * 128 + 4 * (__ffs(c) - 1) + e, u = p.feats + g;
-              double tg = 0.0, tu = 0.0;
-#pragma unroll 1
-              for (int k = 8 * threadIdx.x; k < p.K; k += 8 * G8_THREADS) {
-                float a[8], b[8], d[8];
-                double sg = 0.0, su = 0.0;
-                g8_eight(a, p.x + row * p.ldx + k, p.K - k);
-                g8_eight(b, p.w + g * p.ldw + k, p.K - k);
-                g8_eight(d, p.w + u * p.ldw + k, p.K - k);
-                const int block = k >> 7;
-                const unsigned sx = p.sx[row * p.ldsx + block];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                  sg += a[j] * b[j];                           // (a product of two such numbers has 8 bits)
-                  su += a[j] * d[j];
-                }
-                tg += sg * g8_scaled(sx, p.sw[g * p.ldsw + block]);
-                tu += su * g8_scaled(sx, p.sw[u * p.ldsw + block]);
-              }
-              for (int d = 16; d; d >>= 1) {
-                tg += __shfl_xor_sync(0xffffffffu, tg, d);
-                tu += __shfl_xor_sync(0xffffffffu, tu, d);
-              }
-              __syncthreads();                                   // (what the sums before were is no longer read)
-              if (lane == 0) {
-                sums[warp][0] = tg;
-                sums[warp][1] = tu;
-              }
-              __syncthreads();
-              tg = bias ? bias[g] : 0.f;
-              tu = bias ? bias[u] : 0.f;
-#pragma unroll 1
-              for (int j = 0; j < G8_THREADS / 32; j++) {
-                tg += sums[j][0];
-                tu += sums[j][1];
-              }
-              const double h = fp8_gated_64(tg, tu, p.act);
-              if (!pass) over = fabs(h) > edge;
-              else if (lane == __ffs(c) - 1) (e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3]) = (float)(h * unit);
+          for (unsigned c = __ballot_sync(0xffffffffu, (__float_as_uint(of) & 0x7fffffffu) == most); c && !over; c &= c - 1) {
+            const long long f = q.ft * 128 + 4 * (__ffs(c) - 1) + e;
+            double tg, tu;
+            sums_of(f, 8 * threadIdx.x, 8 * G8_THREADS, tg, tu);
+            __syncthreads();                                   // (what the sums before were is no longer read)
+            if (lane == 0) {
+              sums[warp][0] = tg;
+              sums[warp][1] = tu;
             }
+            __syncthreads();
+            tg = bias_of(f);
+            tu = bias_of(p.feats + f);
+#pragma unroll 1
+            for (int j = 0; j < G8_THREADS / 32; j++) {
+              tg += sums[j][0];
+              tu += sums[j][1];
+            }
+            // (the float32 activation and its arguments' rounding are 10 units off at most; only nearer than that float64 has to say, 0.5 us)
+            const int off = (int)(__float_as_uint(fp8_gated((float)tg, (float)tu, p.act)) & 0x7fffffffu) - (int)edge;
+            over = abs(off) > 32 ? off > 0 : fabs(fp8_gated_64(tg, tu, p.act)) > (double)__uint_as_float(edge);
+          }
+        }
+        if (over == higher) continue;
+        // Its scale changes.  Numbers that are among e4m3's smallest, 2^-9 apart, at one of the scales are made again, a warp to each: the rounded
+        // ones have lost, or would be rounded twice.  (Zeros of the lower scale stay; others are as far apart for their size at both.)
+        float* fresh = reinterpret_cast<float*>(sums + G8_THREADS / 32);
+        const double unit = g8_scaled(254 - low - over, 127);
+        const float by = over ? 0.5f : 2.f;
+        int turn = warp;
+        bool made[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          made[e] = e < there && fabsf(v[e]) < 0.03125f && (!over || v[e] != 0.f);
+          v[e] *= by;
+#pragma unroll 1
+          for (unsigned c = __ballot_sync(0xffffffffu, made[e]); c; c &= c - 1) {
+            if (turn-- != 0) continue;
+            turn = G8_THREADS / 32 - 1;
+            const int at = 4 * (__ffs(c) - 1) + e;
+            const long long f = q.ft * 128 + at;
+            double tg, tu;
+            sums_of(f, 8 * lane, 8 * 32, tg, tu);
+            if (lane == 0) fresh[at] = (float)(fp8_gated_64(tg + bias_of(f), tu + bias_of(p.feats + f), p.act) * unit);
           }
         }
         __syncthreads();                                       // all have read the row
-        if (warp == 0 && over != higher) {
-          const float by = over ? 0.5f : 2.f;
-          const unsigned w = fp8_pack4(v[0] * by, v[1] * by, v[2] * by, v[3] * by);
+        if (warp == 0) {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (made[e]) v[e] = fresh[4 * lane + e];
+          const unsigned w = fp8_pack4(v[0], v[1], v[2], v[3]);
           for (int e = 0; e < there; e++) to[e] = (unsigned char)(w >> 8 * e);
           if (lane == 0) *scale = (unsigned char)(low + over);
         }
