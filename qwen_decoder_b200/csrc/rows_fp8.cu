@@ -235,7 +235,7 @@ extern "C" int qd_add_rmsnorm_fp8(float* x, const void* delta, int delta_dtype, 
           !((uintptr_t)delta & (delta_dtype == QD_BF16 ? 7 : 15));
   if (a.blocks > NORM_MAX_BLOCKS) return QD_ERR_UNSUPPORTED;
   // As many rows as run at a time (64 warps to a multiprocessor): a block to each warp, the shortest way; more: four, so that more rows are
-  // on their way at a time (512 and 2,048 rows of 2,048 features, us: 3.1 and 10.9 with one, 4.5 and 10.0 with four)
+  // on their way at a time (512 and 2,048 rows of 2,048 features, us: 3.3 and 11.0 with one, 4.6 and 9.8 with four)
   const int vpt = a.blocks > 128 ? 16 : a.blocks > 64 ? 4 : a.blocks > 32 ? (n_rows > 296 ? 4 : 2) : n_rows > 148 * (64 / a.blocks) ? 4 : 1;
   const dim3 grid(n_rows), block(32 * ((a.blocks + vpt - 1) / vpt));
 #define GO(TD, V) do { if (vec) qd_launch(norm_fp8_kernel<TD, V, true>, grid, block, 0, stream, a);                           \
