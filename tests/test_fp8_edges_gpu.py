@@ -206,3 +206,39 @@ def test_plans_of_the_current_device():
     from qwen_decoder_b200 import kernels
     for sizes in ((4, 2048, 2048), (40, 4608, 3584), (500, 3584, 18944)):
         assert kernels.gemm_fp8_plan(*sizes) == kernels.gemm_fp8_plan(*sizes, device="cuda") == kernels.gemm_fp8_plan(*sizes, device=torch.device(DEV))
+
+
+@pytest.mark.parametrize("T,plan", [(3, None), (16, (1, 256, 1)), (30, (1, 256, 1)), (90, (1, 256, 1)), (200, (2, 256, 1))])
+def test_blocks_that_several_threads_tell_of(T, plan):
+    """Four equal largest magnitudes near the edge in every block, in all quarters of its features: it is looked at again and again, and stays."""
+    from qwen_decoder_b200 import kernels
+    K, blocks, four = 8192, 90, 4
+    F = 128 * blocks
+    x = rows_of(torch.empty(1, K, device=DEV).normal_().abs().expand(T, K).contiguous())
+    some = rows_of(torch.empty(2 * blocks, K, device=DEV).normal_().abs() * 64 / K)
+    at = 128 * torch.arange(blocks, device=DEV)[:, None] + torch.tensor([3, 40, 77, 126], device=DEV)
+    w = room(2 * F, K)
+    w.q.view(torch.uint8).zero_()
+    w.s.view(torch.uint8).fill_(127)
+    for part, to in ((slice(0, blocks), at), (slice(blocks, None), at + F)):
+        w.q.view(torch.uint8)[to.flatten()] = some.q.view(torch.uint8)[part].repeat_interleave(four, 0)
+        w.s.view(torch.uint8)[to.flatten()] = some.s.view(torch.uint8)[part].repeat_interleave(four, 0)
+    z = (value(x)[:1] @ value(some).T)[0]
+    gate, up = z[:blocks], z[blocks:]
+    bias = torch.zeros(2 * F, device=DEV)
+    bias[at] = torch.clamp(30 - gate, min=0).float()[:, None]
+    gate = gate + bias[at[:, 0]].double()
+    edge = 1.75 * torch.exp2(torch.floor(torch.log2(gate * up / 1.75)))
+    off = torch.linspace(-2e-6, 2e-6, blocks, device=DEV, dtype=torch.float64)[torch.randperm(blocks, device=DEV)]
+    bias[at + F] = (edge * (1 + off) / gate - up).float()[:, None]
+    h = gated(gate, up + bias[at[:, 0] + F].double(), 0)
+    far = (h / edge - 1).abs() > 1e-10
+    assert far.sum() > blocks - 4
+    for _ in range(3):
+        out = room(T, F)
+        kernels.gemm_fp8_gated(x, w, bias, out, 0, plan)
+        s = out.s.float().double()
+        assert (s == torch.where(h > edge, 2 * edge / 448, edge / 448))[:, far].all()
+        assert (out.q[:, at.flatten()].float() == torch.where(s > (edge / 448)[None], 224.0, 448.0).repeat_interleave(four, 1)).all()
+        assert (out.q.float() != 0).sum() == T * blocks * four
+    kernels.check_status()
