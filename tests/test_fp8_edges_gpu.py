@@ -242,3 +242,20 @@ def test_blocks_that_several_threads_tell_of(T, plan):
         assert (out.q[:, at.flatten()].float() == torch.where(s > (edge / 448)[None], 224.0, 448.0).repeat_interleave(four, 1)).all()
         assert (out.q.float() != 0).sum() == T * blocks * four
     kernels.check_status()
+
+
+@pytest.mark.parametrize("T", [1, 7, 16, 40, 300])
+def test_weights_that_rest(T):
+    """``resident`` says when weights are read, not what is made of them."""
+    from qwen_decoder_b200 import kernels
+    x, w, bias = operands(T, 1200, 1000)
+    torch.cuda.synchronize()
+    for dtype in (torch.bfloat16, torch.float32):
+        a, b = torch.empty(T, 1200, dtype=dtype, device=DEV), torch.empty(T, 1200, dtype=dtype, device=DEV)
+        kernels.gemm_fp8(x, w, bias, a)
+        kernels.gemm_fp8(x, w, bias, b, resident=True)
+        assert torch.equal(a, b)
+    a, b = room(T, 600), room(T, 600)
+    kernels.gemm_fp8_gated(x, w, bias, a)
+    kernels.gemm_fp8_gated(x, w, bias, b, resident=True)
+    assert torch.equal(a.q.view(torch.uint8), b.q.view(torch.uint8)) and torch.equal(a.s.view(torch.uint8), b.s.view(torch.uint8))
