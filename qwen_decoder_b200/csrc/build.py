@@ -44,6 +44,9 @@ LIBRARIES: Dict[str, str] = {
     "gemm_fp8_few": "gemm_fp8_few.cu",
     "rows_fp8": "rows_fp8.cu",
     "logprobs": "logprobs.cu",
+    "cache_fp8": "cache_fp8.cu",
+    "attention_fp8_decode": "attention_fp8_decode.cu",
+    "sampling_nucleus": "sampling_nucleus.cu",
     "host_calls": "host_calls.cpp",
     "attention_generic": "attention_generic.cu",
     "attention_f32": "attention_f32.cu",
@@ -74,6 +77,8 @@ EXTRA_DEPS: Dict[str, List[str]] = {
     "gemm_fp8": ["tc5_ops.cuh", "fp8.cuh"],
     "gemm_fp8_few": ["fp8.cuh"],
     "rows_fp8": ["fp8.cuh"],
+    "cache_fp8": ["fp8.cuh", "cache_fp8.cuh"],
+    "attention_fp8_decode": ["fp8.cuh", "cache_fp8.cuh"],
     "gated_block": ["short_conv.cuh"],
     "attention_diff": ["short_conv.cuh", "mma_sync.cuh"],
     "qkv_prep": ["short_conv.cuh"],

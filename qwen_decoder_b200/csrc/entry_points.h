@@ -20,6 +20,8 @@
 // log probabilities
 #define QD_LOGPROBS_MAX_TOP 32
 #define QD_LOGPROBS_MAX_VOCABULARY (1 << 22)
+// tokens from the nucleus of a distribution
+#define QD_NUCLEUS_MAX_VOCABULARY (1 << 22)
 
 extern "C" {
 int qd_add_rmsnorm(float* x, const void* delta, int delta_dtype, const float* w, void* out, int out_dtype,
@@ -43,6 +45,15 @@ int qd_gemm_fp8_plan(int T, int N, int K, int epi, int out_dtype, int sms, int* 
 int qd_gemm_fp8_few_wanted(int T, int N, int K, int sms);
 int qd_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob, float* entropy, int* top_ids,
                       float* top_logprobs, int R, int V, int top, int sms, cudaStream_t stream);
+int qd_sample_nucleus(const float* logits, long long ld, int R, int V, const float* temperature, const int* top_k, const float* top_p,
+                      const float* min_p, const float* draws, int* out, int only, int sms, cudaStream_t stream);
+int qd_rope_kv_write_fp8(const void* x, int dtype, long long ld, int parts, long long part_step, const float* bias, void* q, int T, int H, int G,
+                         int d, int rot, int half, const float* cos_t, const float* sin_t, int n_pos, const int* positions, void* pages,
+                         long long n_pages, const int* slots, int ps, int write, int sms, cudaStream_t stream);
+long long qd_decode_attention_fp8_scratch(int T, int H, int G, int d, int window, int max_keys, int sms);
+int qd_decode_attention_fp8(const void* q, long long ldq, void* out, long long ldo, const void* pages, long long n_pages, const int* table,
+                            int max_blocks, int table_rows, const int* token_req, const int* positions, int T, int H, int G, int d, int ps, float scale,
+                            int window, int max_keys, float* scratch, int sms, cudaStream_t stream);
 int qd_gemm_fp8_few(const void* W, long long ldw, const void* sw, long long ldsw, const void* X, long long ldx, const void* sx,
                     long long ldsx, const float* bias, void* out, int out_dtype, long long ldo, int T, int N, int K, int resident,
                     int sms, cudaStream_t stream);

@@ -1,4 +1,4 @@
-// The host's side of the operators in 8 bits and of the log probabilities: their arguments' checks, room for their results and the call of
+// The host's side of the operators in 8 bits, of the log probabilities and of tokens from the nucleus: their arguments' checks, room for their results and the call of
 // their launchers, as a Python module.  Decode steps replay as graphs and prompts' are launched by prompt_exec.cu, but any other call has its checks,
 // two torch.empty and some twenty arguments through ctypes: from Python 13 to 17 us where the device needs 2 to 10, so 5 to 7.
 //
@@ -7,6 +7,7 @@
 #include <Python.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Device.h>
 #include <torch/csrc/Exceptions.h>
@@ -149,6 +150,10 @@ decltype(qd_gemm_fp8)* g_product;
 decltype(qd_gemm_fp8_few)* g_few;
 decltype(qd_gemm_fp8_few_wanted)* g_few_wanted;
 decltype(qd_token_logprobs)* g_logprobs;
+decltype(qd_sample_nucleus)* g_nucleus;
+decltype(qd_rope_kv_write_fp8)* g_write;
+decltype(qd_decode_attention_fp8)* g_decode;
+decltype(qd_decode_attention_fp8_scratch)* g_decode_scratch;
 
 struct Plan { int cg, bn, splits; };
 // (kept by sizes and device: a few microseconds of estimates)
@@ -362,6 +367,151 @@ CALL(token_logprobs, 3)
   return out;
 END
 
+// ---- a cache in 8 bits
+int whole(PyObject* o, const char* what) {
+  const long v = PyLong_AsLong(o);
+  if (PyErr_Occurred()) throw PythonError{};
+  if (v < INT32_MIN || v > INT32_MAX) refuse(what, " must fit 32 bits, got ", v);
+  return (int)v;
+}
+// ``t`` on the device of the call, of ``dt`` and contiguous; n: numbers, or -1
+void* plain(const at::Tensor& t, at::ScalarType dt, int64_t n, int device, const char* what) {
+  if (t.scalar_type() != dt || !t.is_contiguous() || (n >= 0 && t.numel() != n))
+    refuse(what, " must be contiguous ", toString(dt), n >= 0 ? " [" + std::to_string(n) + "]" : std::string(), ", got ", toString(t.scalar_type()), " ", sizes(t));
+  void* at = address(t).at;
+  if (t.get_device() != device) refuse(what, " is on another device");
+  return at;
+}
+struct Heads { int H, G, d, ps; };
+Heads heads_of(PyObject* const* a, int at_ps, const char* what) {
+  const Heads h = {whole(a[0], what), whole(a[1], what), whole(a[2], what), whole(a[at_ps], what)};
+  if (h.G < 1 || h.H < 1 || h.H % h.G || h.H / h.G > 16 || (h.d != 64 && h.d != 128) || h.ps < 16 || h.ps % 16)
+    refuse(what, ": up to 16 query heads to each of ", h.G, " kv heads of 64 or 128 features and pages of a multiple of 16 tokens, got ", h.H, " heads of ",
+           h.d, ", pages of ", h.ps);
+  return h;
+}
+// uint8 [pages, G ps (2 d + 2)]; how many
+int64_t pages_of(const at::Tensor& p, const Heads& h, const char* what) {
+  const int64_t bytes = (int64_t)h.G * h.ps * (2 * h.d + 2);
+  if (p.scalar_type() != at::kByte || p.dim() != 2 || p.size(1) != bytes || p.size(0) < 1 || !p.is_contiguous())
+    refuse(what, ": pages must be contiguous uint8 [n, ", bytes, "], got ", toString(p.scalar_type()), " ", sizes(p));
+  if (p.size(0) > INT32_MAX / h.ps) refuse(what, ": more than 2^31 tokens of cache");
+  return p.size(0);
+}
+// bfloat16 [T, n], rows 16 bytes apart
+int64_t heads_rows(const at::Tensor& t, int64_t n, const char* what) {
+  if (t.scalar_type() != at::kBFloat16 || t.dim() != 2 || t.size(1) != n || t.stride(1) != 1 || t.stride(0) % 8 || (t.size(0) > 1 && t.stride(0) < n) ||
+      (uintptr_t)t.data_ptr() % 16 || t.size(0) > INT32_MAX)
+    refuse(what, " must be bfloat16 [T, ", n, "], rows contiguous, on 16 bytes and a multiple of 16 bytes apart, got ", toString(t.scalar_type()), " ", sizes(t));
+  return t.size(0);
+}
+
+// (qkv, bias, q_out, H, G, d, rotary_dim, pairing, cos, sin, positions, pages, slot_map, page_size, write_kv)
+CALL(rope_kv_write_fp8, 15)
+  const char* what = "rope_kv_write_fp8";
+  const at::Tensor &x = tensor(a[0], "rope_kv_write_fp8: qkv"), &q = tensor(a[2], "rope_kv_write_fp8: q_out"), &pos = tensor(a[10], "rope_kv_write_fp8: positions");
+  const at::Tensor *bias = tensor_or_none(a[1], "rope_kv_write_fp8: bias"), *cos = tensor_or_none(a[8], "rope_kv_write_fp8: cos");
+  const at::Tensor *sin = tensor_or_none(a[9], "rope_kv_write_fp8: sin"), *pages = tensor_or_none(a[11], "rope_kv_write_fp8: pages");
+  const at::Tensor* slots = tensor_or_none(a[12], "rope_kv_write_fp8: slot_map");
+  const Heads h = heads_of(a + 3, 10, what);
+  const int rot = whole(a[6], what), half = whole(a[7], what), write = PyObject_IsTrue(a[14]);
+  if (PyErr_Occurred()) throw PythonError{};
+  const int64_t W = (int64_t)(h.H + 2 * h.G) * h.d, T = heads_rows(q, (int64_t)h.H * h.d, "rope_kv_write_fp8: q_out");
+  if (!q.is_contiguous()) refuse(what, ": q_out must be contiguous");
+  const Source f = source_of(x, "rope_kv_write_fp8: qkv", T, W);
+  if (!x.is_contiguous()) refuse(what, ": qkv must be contiguous");
+  vector_of(bias, W, what, "bias");
+  if (half != 0 && half != 1) refuse(what, ": pairing must be 0 (neighbours) or 1 (halves), got ", half);
+  if (rot < 0 || rot > h.d || rot % (half ? 16 : 8)) refuse(what, ": rotary_dim must be a multiple of ", half ? 16 : 8, " up to ", h.d, ", got ", rot);
+  const at::Tensor* same[] = {bias, cos, sin, pages, slots};
+  const int device = x.is_cuda() ? x.get_device() : -1;
+  int64_t n_pos = 0, n_pages = 0;
+  if (rot) {
+    if (!cos || !sin || cos->dim() != 2 || cos->size(1) != rot / 2 || cos->size(0) < 1 || cos->sizes() != sin->sizes() || cos->size(0) > INT32_MAX)
+      refuse(what, ": cos and sin must be float32 [positions, ", rot / 2, "]");
+    n_pos = cos->size(0);
+    for (const at::Tensor* t : {cos, sin})
+      if (t->scalar_type() != at::kFloat || !t->is_contiguous()) refuse(what, ": cos and sin must be contiguous float32");
+  }
+  if (write) {
+    if (!pages || !slots) refuse(what, ": pages and slot_map are needed to write");
+    n_pages = pages_of(*pages, h, what);
+  }
+  void* x_at = address(x).at;
+  for (const at::Tensor* t : same)
+    if (t && (!t->is_cuda() || t->get_device() != device)) refuse(what, ": a tensor is on another device");
+  if (T == 0) Py_RETURN_NONE;
+  void *q_at = plain(q, at::kBFloat16, -1, device, "rope_kv_write_fp8: q_out"), *pos_at = plain(pos, at::kInt, T, device, "rope_kv_write_fp8: positions");
+  void* slots_at = write ? plain(*slots, at::kInt, T, device, "rope_kv_write_fp8: slot_map") : nullptr;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  done(entry(g_write, "cache_fp8", "qd_rope_kv_write_fp8")(x_at, f.code, f.ld, f.parts, f.step, address(bias), q_at, (int)T, h.H, h.G, h.d, rot, half,
+                                                          rot ? address(cos) : Address{nullptr}, rot ? address(sin) : Address{nullptr}, (int)n_pos,
+                                                          (const int*)pos_at, write ? address(pages) : Address{nullptr}, n_pages, (const int*)slots_at, h.ps, write,
+                                                          multiprocessors(device), stream_of(x)), what);
+  Py_RETURN_NONE;
+END
+
+// (q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys)
+CALL(decode_attention_fp8, 13)
+  const char* what = "decode_attention_fp8";
+  const at::Tensor &q = tensor(a[0], "decode_attention_fp8: q"), &out = tensor(a[1], "decode_attention_fp8: out"), &pages = tensor(a[2], "decode_attention_fp8: pages");
+  const at::Tensor &table = tensor(a[3], "decode_attention_fp8: block_table"), &req = tensor(a[4], "decode_attention_fp8: token_req");
+  const at::Tensor& pos = tensor(a[5], "decode_attention_fp8: positions");
+  const Heads h = heads_of(a + 6, 3, what);
+  const double scale = PyFloat_AsDouble(a[10]);
+  const int window = whole(a[11], what);
+  int64_t max_keys = a[12] == Py_None ? -1 : PyLong_AsLongLong(a[12]);
+  if (PyErr_Occurred()) throw PythonError{};
+  const int64_t T = heads_rows(q, (int64_t)h.H * h.d, "decode_attention_fp8: q"), n_pages = pages_of(pages, h, what);
+  if (heads_rows(out, (int64_t)h.H * h.d, "decode_attention_fp8: out") != T) refuse(what, ": q and out have ", T, " and ", out.size(0), " rows");
+  if (table.dim() != 2 || table.size(0) < 1 || table.size(1) < 1) refuse(what, ": block_table must be int32 [requests, pages], got ", sizes(table));
+  if (window < 0) refuse(what, ": window must not be negative");
+  const int64_t held = table.size(1) * h.ps;
+  if (max_keys < 0 || max_keys > held) max_keys = held;
+  if (max_keys > INT32_MAX) refuse(what, ": more than 2^31 keys");
+  address(q);
+  const int device = q.get_device();
+  if (!out.is_cuda() || out.get_device() != device) refuse(what, ": out is on another device");
+  void *pages_at = plain(pages, at::kByte, -1, device, "decode_attention_fp8: pages"), *table_at = plain(table, at::kInt, -1, device, "decode_attention_fp8: block_table");
+  void *req_at = plain(req, at::kInt, T, device, "decode_attention_fp8: token_req"), *pos_at = plain(pos, at::kInt, T, device, "decode_attention_fp8: positions");
+  if (T == 0) Py_RETURN_NONE;
+  if (max_keys == 0) max_keys = 1;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  const int sms = multiprocessors(device);
+  const int64_t floats = entry(g_decode_scratch, "attention_fp8_decode", "qd_decode_attention_fp8_scratch")((int)T, h.H, h.G, h.d, window, (int)max_keys, sms);
+  const at::Tensor scratch = at::empty_strided({floats}, {1}, q.options().dtype(at::kFloat));
+  done(entry(g_decode, "attention_fp8_decode", "qd_decode_attention_fp8")(address(q), q.stride(0), address(out), out.stride(0), pages_at, n_pages,
+                                                                         (const int*)table_at, (int)table.size(1), (int)table.size(0), (const int*)req_at,
+                                                                         (const int*)pos_at, (int)T, h.H, h.G, h.d, h.ps, (float)scale, window, (int)max_keys,
+                                                                         address(scratch), sms, stream_of(q)), what);
+  Py_RETURN_NONE;
+END
+
+// (logits, temperature, top_k, top_p, min_p, draws, out, only)
+CALL(sample_nucleus, 8)
+  const char* what = "sample_nucleus";
+  const at::Tensor &z = tensor(a[0], "sample_nucleus: logits"), &temperature = tensor(a[1], "sample_nucleus: temperature"), &k = tensor(a[2], "sample_nucleus: top_k");
+  const at::Tensor &p = tensor(a[3], "sample_nucleus: top_p"), &m = tensor(a[4], "sample_nucleus: min_p"), &u = tensor(a[5], "sample_nucleus: draws");
+  const at::Tensor& out = tensor(a[6], "sample_nucleus: out");
+  const int only = PyObject_IsTrue(a[7]);
+  if (PyErr_Occurred()) throw PythonError{};
+  if (z.scalar_type() != at::kFloat || z.dim() != 2 || (z.stride(1) != 1 && z.size(1) > 1)) refuse("sample_nucleus: logits must be float32 [R, V] with contiguous rows");
+  const int64_t R = z.size(0), V = z.size(1);
+  if (V < 1 || V > QD_NUCLEUS_MAX_VOCABULARY) refuse(what, ": rows of 1 to ", QD_NUCLEUS_MAX_VOCABULARY, " logits, got ", V);
+  if (R > INT32_MAX / 16) refuse(what, ": ", R, " rows");
+  for (const auto& [t, name, dt] : {std::make_tuple(&temperature, "temperature", at::kFloat), std::make_tuple(&k, "top_k", at::kInt), std::make_tuple(&p, "top_p", at::kFloat),
+                                    std::make_tuple(&m, "min_p", at::kFloat), std::make_tuple(&u, "draws", at::kFloat), std::make_tuple(&out, "out", at::kInt)})
+    if (t->scalar_type() != dt || t->dim() != 1 || t->size(0) != R || !t->is_contiguous()) refuse(what, ": ", name, " must be contiguous ", toString(dt), " [", R, "]");
+  address(z);
+  const int device = z.get_device();
+  for (const at::Tensor* t : {&temperature, &k, &p, &m, &u, &out})
+    if (!t->is_cuda() || t->get_device() != device) refuse(what, ": a tensor is on another device");
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  done(entry(g_nucleus, "sampling_nucleus", "qd_sample_nucleus")(address(z), z.stride(0), (int)R, (int)V, address(temperature), address(k), address(p), address(m),
+                                                                 address(u), address(out), only, multiprocessors(device), stream_of(z)), what);
+  Py_RETURN_NONE;
+END
+
 // (KernelError, resolve, Fp8Rows)
 CALL(start, 3)
   Py_INCREF(a[0]);
@@ -375,7 +525,8 @@ END
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(start), ENTRY(fp8_rows), ENTRY(check_rows), ENTRY(quantize_fp8), ENTRY(gate_fp8), ENTRY(add_rmsnorm_fp8), ENTRY(gemm_fp8),
-                         ENTRY(gemm_fp8_gated), ENTRY(gemm_fp8_plan), ENTRY(token_logprobs), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(gemm_fp8_gated), ENTRY(gemm_fp8_plan), ENTRY(token_logprobs), ENTRY(rope_kv_write_fp8),
+                         ENTRY(decode_attention_fp8), ENTRY(sample_nucleus), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qd_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -843,6 +843,18 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                                          _ptr(draws), _ptr(out), _stream()), "sample")
 
 
+def sample_nucleus(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
+                   draws: torch.Tensor, out: torch.Tensor, only: bool = False) -> None:
+    """out[r] (int32 [R]) = a token of logits[r] (float32 [R, V], rows may lie apart) by ``temperature``, ``top_k``, ``top_p``, ``min_p`` and
+    the number ``draws`` in [0, 1) (float32 [R], top_k int32).  With w_i = exp((z_i - max z) / temperature): the top_k largest logits stay
+    (0: all), of those the most probable that make up ``top_p`` of their weight together (1: all), of those the ones of w_i >= ``min_p``
+    (0: all; the largest always), logits that are equal in or out together; the token is the first of them whose running sum of weights reaches draws times
+    their sum.  Temperature 0 is argmax, the lowest index first.  Weights below 2^-45 (of rows of more than 2^18 logits 2^-41) count for
+    nothing; a logit that is no number is none.  ``only``: rows with neither top_p below 1 nor min_p above 0 keep what out holds."""
+    _launch_count[0] += 1
+    (_host or _host_calls()).sample_nucleus(logits, temperature, top_k, top_p, min_p, draws, out, only)
+
+
 LOGPROBS_MAX_TOP, LOGPROBS_MAX_VOCABULARY = 32, 1 << 22
 
 
@@ -1008,6 +1020,55 @@ def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp
     float32, rounded once.  ``resident``: as in ``gemm_fp8``."""
     _launch_count[0] += 1
     (_host or _host_calls()).gemm_fp8_gated(x, w, bias, out, act, plan, resident)
+
+
+# ------------------------------------------------------------------ a paged cache in 8 bits
+def fp8_cache_supported(H: int, G: int, d: int, page_size: int) -> bool:
+    """What the attention over a cache in 8 bits takes: heads of 64 or 128 features, up to 16 query heads per KV head, pages of a multiple
+    of 16 tokens."""
+    return d in (64, 128) and G >= 1 and H % G == 0 and 1 <= H // G <= 16 and page_size % 16 == 0 and page_size > 0
+
+
+def fp8_page_bytes(G: int, page_size: int, d: int) -> int:
+    """Bytes of a page of a cache in 8 bits: the keys [G, page_size, d], the values, float8_e4m3fn numbers, then the scales
+    [G, page_size, 2] of every token's key and value, float8_e8m0fnu (powers of two)."""
+    return G * page_size * (2 * d + 2)
+
+
+def fp8_pages(n_pages: int, G: int, page_size: int, d: int, device) -> torch.Tensor:
+    """An empty cache in 8 bits, uint8 [n_pages, ``fp8_page_bytes``]."""
+    return torch.zeros((n_pages, fp8_page_bytes(G, page_size, d)), dtype=torch.uint8, device=device)
+
+
+def fp8_page_views(pages: torch.Tensor, G: int, page_size: int, d: int):
+    """(numbers float8_e4m3fn [n_pages, 2, G, page_size, d], scales float8_e8m0fnu [n_pages, G, page_size, 2]) of such a cache: key and
+    value are numbers[:, 0] * scales[..., 0] and numbers[:, 1] * scales[..., 1]."""
+    n = 2 * G * page_size * d
+    return (pages[:, :n].view(torch.float8_e4m3fn).view(-1, 2, G, page_size, d),
+            pages[:, n:].view(torch.float8_e8m0fnu).view(-1, G, page_size, 2))
+
+
+def rope_kv_write_fp8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tensor, H: int, G: int, d: int, rotary_dim: int,
+                      pairing: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
+                      pages: Optional[torch.Tensor], slot_map: Optional[torch.Tensor], page_size: int, write_kv: bool = True) -> None:
+    """``rope_kv_write`` with a cache in 8 bits: qkv bfloat16 or float32 [T, (H + 2G) d], or float32 partial sums [n, T, (H + 2G) d], plus
+    ``bias`` (float32 [(H + 2G) d] or None); q and k turned by the table rows of ``positions``, q to q_out bfloat16 [T, H d], k and v to
+    their slots of ``pages`` (``fp8_pages``).  A row's scale is the smallest power of two with which its largest magnitude stays within 448,
+    of the numbers before any rounding; a row with an infinity or a NaN gets the scale NaN.  A token whose slot is negative is not
+    written."""
+    _launch_count[0] += 1
+    (_host or _host_calls()).rope_kv_write_fp8(qkv, bias, q_out, H, G, d, rotary_dim, pairing, cos, sin, positions, pages, slot_map, page_size, write_kv)
+
+
+def decode_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, token_req: torch.Tensor,
+                         positions: torch.Tensor, H: int, G: int, d: int, page_size: int, scale: float, window: int = 0,
+                         max_keys: Optional[int] = None) -> None:
+    """Attention of tokens one by one over a cache in 8 bits: q and out bfloat16 [T, H d] (rows may lie apart), token t sees the keys up to
+    positions[t] of the request whose pages are row token_req[t] of ``block_table``, the last ``window`` of them if that is not 0; with a
+    negative position none, and its row of out is zeros.  ``max_keys``: no position lies beyond max_keys - 1 (None: what the table
+    holds); the launch is cut by it."""
+    _launch_count[0] += 2
+    (_host or _host_calls()).decode_attention_fp8(q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys)
 
 
 # ------------------------------------------------------------------ latent attention
