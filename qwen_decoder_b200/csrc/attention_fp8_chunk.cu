@@ -1,0 +1,586 @@
+// Attention of portions of several requests' tokens over a paged cache in 8 bits (cache_fp8.cuh), causal, on the fifth-generation tensor cores:
+//
+//   z_k = scale 2^(s_k) (q . n_k),   p = softmax z over lo <= k <= pos,   out = sum_k p_k 2^(s_v) n_v
+//
+// A CTA takes 128 rows = (128 / gs) tokens x the gs query heads of one KV head, as attention_tc5.cu, and walks tiles of 128 keys.  The
+// softmax, the weights P that go over the scores in tensor memory and the sums that stay there are that kernel's.  What 8 bits change:
+//
+// * Scores by kind::mxf8f6f4 with block scaling: the keys' numbers are the operand as they lie in the cache, the tensor cores apply a key's scale,
+//   and nothing is converted.  Both operands have to be of 8 bits then, so a row of q is two of them: e4m3 numbers of q over the row's scale,
+//   and of what their rounding left, over a sixteenth of it.  Together they are the bfloat16 number itself where it is above 2^-14 of the row's
+//   largest, and off by 2^-23 of that below.  Two products of 128 features in 8 bits take the tensor cores as long as one of bfloat16.
+// * Values become bfloat16, scale included, which is exact: four warps take tiles from where the copies leave them to where the product reads
+//   them (P and sums as ever).  P in 8 bits would be two numbers as q is, for every weight; this is 16 KB of values to a tile for all 128 rows.
+//   They also bring the keys' scales to tensor memory.
+// * A key or value that is no number has the scale 255.  The value becomes zeros, its key's scale 255, so that the score is none and
+//   every row that sees it, and no other, is none.  Values behind the last row's position, which may be anything, become zeros.
+// * Few tiles of rows (a short portion behind a long history) share their keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
+//
+// Warps: 0..7 softmax (two threads to a row: halves of the keys and of the columns), 8 and 9 copies of keys and values, 10 MMAs, 12..15 values.
+// Slot i (i = -2 .. n - 1; stage (i + 2) % 3) holds the keys of tile i + 2 with their scales and the values of tile i: what the MMA warp
+// reads in its step i, behind one barrier.  Every wait on an mbarrier is bounded, as in attention_tc5.cu.
+#include "attention_tc5.cuh"
+#include "cache_fp8.cuh"
+#include "entry_points.h"
+#include "tc5_ops.cuh"
+
+#include <cuda_fp16.h>
+
+#define AC_SOFTMAX 256                 // threads
+#define AC_THREADS 512
+#define AC_STAGES 3
+#define AC_META 256                    // requests whose token ranges are staged in shared memory
+#define AC_ROWS 128
+#define AC_KEYS 128
+#define AC_GROW 8.0f                   // powers of two by which a row's maximum grows before it is followed
+#define AC_REGS_SOFTMAX 184            // 2 x 184 + 56 + 88 = 512: what 4 x 128 at the launch add up to
+#define AC_REGS_ISSUE 56
+#define AC_REGS_VALUES 88
+
+struct AcParams {
+  const bf16* q; long long ldq;
+  bf16* out; long long ldo;
+  const unsigned char* pages; long long page_bytes; int n_pages;
+  const int* table; int max_blocks;
+  const int *cu, *start;
+  int R, H, G, ps, window, tok_tile, rows;
+  float scale_log2e;
+  float *part_o, *part_s;              // [share][rows][H][HD]; [share][rows][H][2]: maximum, sum
+  int* status;
+};
+
+__device__ __forceinline__ int ac_key_lo(const AcParams& p, int pos) { return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0; }
+// x: byte of a row, y: row of a page, z: page
+__device__ __forceinline__ void ac_load_3d(void* dst, const CUtensorMap* map, int y, int z, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(tc_smem(dst)), "l"(map), "r"(tc_smem(bar)), "r"(0), "r"(y), "r"(z) : "memory");
+}
+// D[128 x 128] (+)= A[128 x 32] B[128 x 32]^T of e4m3 numbers with a scale to each row of A and of B: A in tensor memory, four neighbouring k a column
+__device__ __forceinline__ void ac_mma_scaled(unsigned d, unsigned a, unsigned desc_lo, unsigned desc_hi, unsigned idesc, unsigned sa, unsigned sb,
+                                              unsigned accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 d;\n setp.ne.b32 p, %7, 0;\n mov.b64 d, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], [%1], d, %4, [%5], [%6], p;\n}\n"
+      ::"r"(d), "r"(a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void ac_st4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// two e4m3 numbers times f as bfloat16
+__device__ __forceinline__ unsigned ac_bf16x2(unsigned short two, float f) {
+  unsigned h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return at_pack(v.x * f, v.y * f);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_constant__ CUtensorMap map, const AcParams p) {
+  constexpr int KQ = AC_KEYS / 2, DH = HD / 2, NS = AC_STAGES;
+  constexpr int TILE8 = AC_KEYS * HD, TILE16 = 2 * TILE8;           // bytes of a tile in 8 bits, in bfloat16
+  constexpr int BOX = 16 * HD;
+  // tensor memory: two buffers of scores and weights, the sums, q's two operands of HD / 4 columns, their scales, the keys' scales
+  constexpr unsigned TMEM_COLS = 512, T_O = 2 * AC_KEYS, T_Q = 3 * AC_KEYS, T_SA = 448, T_SB = 456;
+  // rows of 128 (64) bytes with the 128-byte (64-byte) swizzle, groups of 8 rows 1024 (512) bytes apart
+  constexpr unsigned K_DESC_HI = HD == 128 ? AT_DESC_HI : (unsigned)(512 >> 4) | (1u << 14) | (4u << 29);
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  unsigned char* base = smem_raw + ((1024 - (tc_smem(smem_raw) & 1023)) & 1023);
+  unsigned char* k_s = base;                        // NS stages of keys
+  unsigned char* v8_s = k_s + NS * TILE8;           // NS stages of values as they come
+  unsigned char* v_s = v8_s + NS * TILE8;           // NS stages of values in bfloat16
+  __shared__ unsigned long long full[NS], empty[NS], v8_full[NS], v8_empty[NS], s_full[2], p_full[2], o_done, o_last, q_full;
+  __shared__ float mx_s[2][2][AC_ROWS], l_s[2][AC_ROWS];
+  __shared__ unsigned sa_s[AC_ROWS];
+  __shared__ unsigned short sc_s[4][AC_KEYS];       // of a tile's keys: both scales
+  __shared__ unsigned tmem_slot;
+  __shared__ int dead;
+  __shared__ int cu_s[AC_META + 1], sp_s[AC_META + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    dead = 0;
+    for (int s = 0; s < NS; s++) {
+      tc_bar_init(&full[s], 1 + 128);
+      tc_bar_init(&empty[s], 1);
+      tc_bar_init(&v8_full[s], 1);
+      tc_bar_init(&v8_empty[s], 128);
+    }
+    for (int s = 0; s < 2; s++) { tc_bar_init(&s_full[s], 1); tc_bar_init(&p_full[s], AC_SOFTMAX); }
+    // (o_last: the last product has no scores behind it by which its phase of o_done would be known)
+    tc_bar_init(&o_done, 1); tc_bar_init(&o_last, 1);
+    tc_bar_init(&q_full, AC_SOFTMAX);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 10) tc_alloc(&tmem_slot, TMEM_COLS);
+  pdl_wait();
+  const bool staged = p.R < AC_META;
+  if (staged)
+    for (int i = threadIdx.x; i <= p.R; i += AC_THREADS) {
+      cu_s[i] = p.cu[i];
+      sp_s[i] = i < p.R ? p.start[i] : 0;
+    }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = tmem_slot;
+
+  // ---- which request and which tokens (tiles numbered request by request, the longest histories first)
+  const int g = blockIdx.y, gs = p.H / p.G;
+  const int* cu = staged ? cu_s : p.cu;
+  const int* sp = staged ? sp_s : p.start;
+  const int b = gridDim.x - 1 - blockIdx.x;
+  int r = 0, before = 0;
+  for (; r < p.R; r++) {
+    const int nt = (cu[r + 1] - cu[r] + p.tok_tile - 1) / p.tok_tile;
+    if (b < before + nt) break;
+    before += nt;
+  }
+  const bool idle = r == p.R;
+  int tok0 = 0, n_tok = 0, pos0 = 0;
+  if (!idle) {
+    tok0 = cu[r] + (b - before) * p.tok_tile;
+    n_tok = min(p.tok_tile, cu[r + 1] - tok0);
+    pos0 = sp[r] + (tok0 - cu[r]);
+  }
+  const int key_hi = pos0 + n_tok, key_lo = ac_key_lo(p, pos0);
+  // of the tiles from the first row's first key to the last row's last, this share's
+  const int t0 = key_lo / AC_KEYS, tn = idle ? 0 : (key_hi + AC_KEYS - 1) / AC_KEYS - t0;
+  const int kt_lo = t0 + (int)((long long)tn * blockIdx.z / gridDim.z), n_kt = t0 + (int)((long long)tn * (blockIdx.z + 1) / gridDim.z) - kt_lo;
+  const int* table = p.table + (long long)(idle ? 0 : r) * p.max_blocks;
+  auto page_at = [&](int key) {                       // keys that are none: any page will do
+    if (key >= key_hi || key / p.ps >= p.max_blocks) return 0;
+    return min(max(table[key / p.ps], 0), p.n_pages - 1);
+  };
+
+  if (warp < AC_SOFTMAX / 32) {
+    // ------------------------------------------------------------------ softmax: two threads to a row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AC_REGS_SOFTMAX));
+    const int row = (warp & 3) * 32 + lane, h = warp >> 2;          // row: also the lane of tensor memory
+    const int t = row / gs, hh = row - t * gs;
+    const bool ok = !idle && t < n_tok;
+    const int pos = pos0 + t, lo = ac_key_lo(p, pos);
+    const unsigned t_lane = tmem + ((unsigned)((warp & 3) * 32) << 16);
+    {
+      // this thread's half of the row of q as e4m3 numbers over the row's scale, and what that left over a sixteenth of it
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(tok0 + t) * p.ldq + (long long)(g * gs + hh) * HD + h * DH);
+      uint4 w[DH / 8];
+      unsigned peak = 0;                             // (magnitudes order as their bits do)
+#pragma unroll
+      for (int i = 0; i < DH / 8; i++) {
+        w[i] = ok ? src[i] : make_uint4(0, 0, 0, 0);
+        const unsigned x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) peak = max(peak, max(x[j] << 16 & 0x7fffffffu, x[j] & 0x7fff0000u));
+      }
+      mx_s[0][h][row] = __uint_as_float(peak);
+      asm volatile("bar.sync 1, %0;" ::"n"(AC_SOFTMAX) : "memory");
+      unsigned byte = fp8_scale_byte(max(peak, __float_as_uint(mx_s[0][h ^ 1][row])));
+      byte = max(byte, 5u);                          // (a sixteenth of it is a scale as well)
+      const float inv = fp8_inverse(byte);
+      unsigned big[DH / 4], small[DH / 4];
+#pragma unroll
+      for (int i = 0; i < DH / 4; i++) {
+        const unsigned* x = &w[i / 2].x + 2 * (i & 1);
+        const float v0 = __uint_as_float(x[0] << 16) * inv, v1 = __uint_as_float(x[0] & 0xffff0000u) * inv;
+        const float v2 = __uint_as_float(x[1] << 16) * inv, v3 = __uint_as_float(x[1] & 0xffff0000u) * inv;
+        big[i] = fp8_pack4(v0, v1, v2, v3);
+        small[i] = fp8_pack4((v0 - fp8_value(big[i] & 255u)) * 16.f, (v1 - fp8_value(big[i] >> 8 & 255u)) * 16.f,
+                             (v2 - fp8_value(big[i] >> 16 & 255u)) * 16.f, (v3 - fp8_value(big[i] >> 24)) * 16.f);
+      }
+#pragma unroll
+      for (int i = 0; i < DH / 4; i += 8) {
+        unsigned x[8], y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) { x[j] = big[i + j]; y[j] = small[i + j]; }
+        tc_st8(t_lane + T_Q + h * (DH / 4) + i, x);
+        tc_st8(t_lane + T_Q + HD / 4 + h * (DH / 4) + i, y);
+      }
+      if (h == 0) sa_s[row] = byte;
+      asm volatile("bar.sync 1, %0;" ::"n"(AC_SOFTMAX) : "memory");
+      if (h == 0) {                                  // lane l, column c: the scale of row 32 c + l, in every quarter of the lanes
+        unsigned a[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) a[c] = sa_s[32 * c + lane];
+        ac_st4(t_lane + T_SA, a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int c = 0; c < 4; c++) a[c] = a[c] == 255u ? 255u : a[c] - 4u;
+        ac_st4(t_lane + T_SA + 4, a[0], a[1], a[2], a[3]);
+      }
+      tc_st_wait();
+      tc_fence_before();
+      tc_arrive(&q_full);
+    }
+    float m = -INFINITY, l = 0.f;        // m: the maximum that this row's exponentials, sum and output refer to
+    const int free_hi = pos0 + 1, free_lo = ac_key_lo(p, key_hi - 1);       // keys that every row sees need no test
+    for (int j = 0; j < n_kt; j++) {
+      const int tile_base = (kt_lo + j) * AC_KEYS, key_base = tile_base + h * KQ;
+      if (!tc_wait_inline(&s_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 7);
+      tc_fence_after();
+      float sv[KQ];
+      at_tmem_ld<KQ>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * KQ, sv);
+      const bool interior = tile_base >= free_lo && tile_base + AC_KEYS <= free_hi && p.scale_log2e > 0.f;
+      float mx = -INFINITY;
+      if (interior) {
+#pragma unroll
+        for (int i = 0; i < KQ; i++) mx = fmaxf(mx, sv[i]);
+        mx *= p.scale_log2e;
+      } else {
+#pragma unroll
+        for (int i = 0; i < KQ; i++) {
+          const int key = key_base + i;
+          sv[i] = ok && key <= pos && key >= lo ? sv[i] * p.scale_log2e : -INFINITY;
+          mx = fmaxf(mx, sv[i]);
+        }
+      }
+      mx_s[j & 1][h][row] = mx;
+      asm volatile("bar.sync 1, %0;" ::"n"(AC_SOFTMAX) : "memory");
+      const float m_tile = fmaxf(mx, mx_s[j & 1][h ^ 1][row]);
+      // the row moves to a new reference only when its maximum has grown by more than AC_GROW (always from "no key yet"); both threads of a
+      // row decide alike, and the warp acts together
+      const bool grow = m_tile > m + AC_GROW;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float alpha = grow ? at_exp2(m - m_tile) : 1.0f;
+        if (grow) m = m_tile;
+        l *= alpha;
+        if (j > 0) {
+          if (!tc_wait_inline(&o_done, (j - 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 8);
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < DH; c += 32) {
+            float ov[32];
+            at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);
+            unsigned ob[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) ob[i] = __float_as_uint(ov[i] * alpha);
+            at_tmem_st<32>(t_lane + T_O + h * DH + c, ob);
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      unsigned pk[KQ / 2];
+      float sum = 0.f;
+      const float mul = interior ? p.scale_log2e : 1.0f;
+#pragma unroll
+      for (int i = 0; i < KQ / 2; i++) {
+        const float p0 = at_exp2(fmaf(sv[2 * i], mul, -ref)), p1 = at_exp2(fmaf(sv[2 * i + 1], mul, -ref));
+        sum += p0 + p1;
+        pk[i] = at_pack(p0, p1);
+      }
+      l += sum;
+      // over the first half of this tile's own scores, which every thread of the row has in registers since the barrier above
+      at_tmem_st<KQ / 2>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * (KQ / 2), pk);
+      tc_fence_before();
+      tc_arrive(&p_full[j & 1]);
+    }
+    if (n_kt > 0) {
+      if (!tc_wait_inline(&o_last, 0, &dead) && lane == 0) atomicCAS(p.status, 0, 9);
+      tc_fence_after();
+    }
+    l_s[h][row] = l;
+    asm volatile("bar.sync 1, %0;" ::"n"(AC_SOFTMAX) : "memory");
+    const float l_all = l + l_s[h ^ 1][row];
+    if (gridDim.z > 1) {
+      const long long at = ((long long)blockIdx.z * p.rows + tok0 + t) * p.H + g * gs + hh;
+      if (ok && h == 0) *reinterpret_cast<float2*>(p.part_s + 2 * at) = make_float2(m, l_all);
+      if (n_kt > 0) {
+#pragma unroll
+        for (int c = 0; c < DH; c += 32) {
+          float ov[32];
+          at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);      // the warp's access: rows without a token take part too
+          if (ok) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(p.part_o + at * HD + h * DH + c + i) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+          }
+        }
+      }
+    } else if (n_kt > 0) {
+      const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+      bf16* d = p.out + (long long)(tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + h * DH;
+#pragma unroll
+      for (int c = 0; c < DH; c += 32) {
+        float ov[32];
+        at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);
+        if (ok) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            v.x = at_pack(ov[i] * inv, ov[i + 1] * inv);
+            v.y = at_pack(ov[i + 2] * inv, ov[i + 3] * inv);
+            v.z = at_pack(ov[i + 4] * inv, ov[i + 5] * inv);
+            v.w = at_pack(ov[i + 6] * inv, ov[i + 7] * inv);
+            *reinterpret_cast<uint4*>(d + c + i) = v;
+          }
+        }
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------ the keys' scales, and values to bfloat16
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AC_REGS_VALUES));
+    const int ct = threadIdx.x - 384;
+    const unsigned t_sb = tmem + ((unsigned)((warp & 3) * 32) << 16) + T_SB;
+    auto key_of = [&](int j) { return (kt_lo + j) * AC_KEYS + ct; };
+    auto scales_at = [&](int j, int page) {           // of this thread's key of tile j
+      const int key = key_of(j);
+      if (j >= n_kt || key >= key_hi) return (unsigned short)0x7f7f;
+      const unsigned char* s = p.pages + page * p.page_bytes + (long long)2 * p.G * p.ps * HD + ((long long)g * p.ps + key % p.ps) * 2;
+      return *reinterpret_cast<const volatile unsigned short*>(s);
+    };
+    unsigned short sc = n_kt > 0 ? scales_at(0, page_at(key_of(0))) : 0;
+    int page = n_kt > 1 ? page_at(key_of(1)) : 0;
+    for (int i = -2; i < n_kt; i++) {
+      const int s = (i + 2) % NS, j = i + 2;
+      if (j < n_kt) {
+        sc_s[j & 3][ct] = sc;
+        sc = scales_at(j + 1, page);
+        page = j + 2 < n_kt ? page_at(key_of(j + 2)) : 0;
+      }
+      if (!tc_wait_inline(&empty[s], ((i + 2) / NS & 1) ^ 1, &dead)) atomicCAS(p.status, 0, 5);
+      tc_fence_after();
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+      if (j < n_kt) {
+        unsigned w[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const unsigned both = sc_s[j & 3][32 * c + lane];
+          w[c] = both >> 8 == 255u ? 255u : both & 255u;
+        }
+        ac_st4(t_sb + 4 * s, w[0], w[1], w[2], w[3]);
+      }
+      if (i >= 0) {
+        if (!tc_wait_inline(&v8_full[i % NS], i / NS & 1, &dead)) atomicCAS(p.status, 0, 6);
+        const unsigned char* from = v8_s + (i % NS) * TILE8;
+        unsigned char* to = v_s + s * TILE16;
+        constexpr int PIECES = HD / 16;               // of 16 features
+#pragma unroll
+        for (int e = 0; e < PIECES; e++) {
+          const int at = ct + 128 * e, key = at / PIECES, c = at % PIECES, k = (kt_lo + i) * AC_KEYS + key;
+          const int place = HD == 128 ? c ^ (key & 7) : c ^ (key >> 1 & 3);
+          uint4 v = *reinterpret_cast<const uint4*>(from + key * HD + 16 * place);
+          const unsigned byte = sc_s[i & 3][key] >> 8;
+          const bool none = byte == 255u || k >= key_hi || k < key_lo;
+          if (none) v = make_uint4(0, 0, 0, 0);
+          const float f = none ? 0.f : c8_power(byte);
+          const uint4 a = make_uint4(ac_bf16x2((unsigned short)v.x, f), ac_bf16x2((unsigned short)(v.x >> 16), f),
+                                     ac_bf16x2((unsigned short)v.y, f), ac_bf16x2((unsigned short)(v.y >> 16), f));
+          const uint4 b = make_uint4(ac_bf16x2((unsigned short)v.z, f), ac_bf16x2((unsigned short)(v.z >> 16), f),
+                                     ac_bf16x2((unsigned short)v.w, f), ac_bf16x2((unsigned short)(v.w >> 16), f));
+          // chunks 2 c and 2 c + 1 of 8 features, in blocks of 64; the second half of a row's threads begins with the other one, against conflicts
+          unsigned char* block = to + (c >> 2) * (AC_KEYS * 128) + key * 128;
+          const int chunk = 2 * (c & 3), x = key & 7;
+          const bool swap = HD == 128 && c >= 4;
+          *reinterpret_cast<uint4*>(block + (((chunk + swap) ^ x) << 4)) = swap ? b : a;
+          *reinterpret_cast<uint4*>(block + (((chunk + !swap) ^ x) << 4)) = swap ? a : b;
+        }
+        tc_arrive(&v8_empty[i % NS]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tc_st_wait();
+      tc_fence_before();
+      tc_arrive(&full[s]);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AC_REGS_ISSUE));
+    if (warp < 10) {
+      // ---------------------------------------------------------------- copies: a tile is eight boxes of 16 keys, each from its page
+      const int which = warp - 8;                     // 0 keys, 1 values
+      auto page_of = [&](int j) { return lane < 8 && j < n_kt ? page_at((kt_lo + j) * AC_KEYS + 16 * lane) : 0; };
+      int page_next = page_of(0);
+      for (int j = 0; j < n_kt + (which ? 0 : 2); j++) {       // (the last two slots have no keys)
+        const int page = page_next, s = j % NS;
+        page_next = page_of(j + 1);
+        unsigned long long* bar = which ? &v8_full[s] : &full[s];
+        if (!tc_wait_inline(which ? &v8_empty[s] : &empty[s], (j / NS & 1) ^ 1, &dead)) {
+          if (lane == 0) atomicCAS(p.status, 0, 1);
+          break;                                      // (nobody waits any more, and no more copies are to arrive)
+        }
+        if (lane == 0) {
+          if (j < n_kt) tc_expect_tx(bar, TILE8);
+          else tc_arrive(bar);
+        }
+        __syncwarp();
+        if (j < n_kt && lane < 8) {
+          const int key = (kt_lo + j) * AC_KEYS + 16 * lane;
+          ac_load_3d((which ? v8_s : k_s) + s * TILE8 + lane * BOX, &map, (which * p.G + g) * p.ps + key % p.ps, page, bar);
+        }
+      }
+    } else if (warp == 10 && !idle) {
+      // ---------------------------------------------------------------- MMAs: the whole warp goes through the tiles, one lane issues
+      const bool one = tc_elect();
+      const unsigned idesc_qk = (unsigned)(AC_KEYS >> 3) << 17 | 1u << 23 | (unsigned)(AC_ROWS >> 4) << 24;
+      const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(HD >> 3) << 17) | ((unsigned)(AC_ROWS >> 4) << 24);
+      const unsigned k_lo0 = at_desc_lo(tc_smem(k_s), 0), v_lo0 = at_desc_lo(tc_smem(v_s), AC_KEYS * 128);
+      auto slot_ready = [&](int i) {
+        if (!tc_wait_inline(&full[(i + 2) % NS], ((i + 2) / NS) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 2);
+      };
+      auto scores = [&](int j) {
+        const unsigned k_lo = k_lo0 + (unsigned)(j % NS) * (TILE8 >> 4);
+#pragma unroll
+        for (int part = 0; part < 2; part++)
+#pragma unroll
+          for (int k = 0; k < HD / 32; k++)
+            ac_mma_scaled(tmem + (unsigned)(j & 1) * AC_KEYS, tmem + T_Q + part * (HD / 4) + k * 8, k_lo + k * 2, K_DESC_HI, idesc_qk,
+                          tmem + T_SA + 4 * part, tmem + T_SB + 4 * (j % NS), part || k ? 1u : 0u);
+      };
+      if (n_kt > 0) {
+        if (!tc_wait_inline(&q_full, 0, &dead) && lane == 0) atomicCAS(p.status, 0, 3);
+        for (int j = 0; j < 2; j++) {                   // slots -2 and -1: the first two tiles' scores
+          slot_ready(j - 2);
+          tc_fence_after();
+          if (one) {
+            if (j < n_kt) scores(j);
+            tc_commit(&empty[j % NS]);
+            if (j < n_kt) tc_commit(&s_full[j & 1]);
+          }
+        }
+        for (int j = 0; j < n_kt; j++) {
+          const int s = (j + 2) % NS;
+          if (!tc_wait_inline(&p_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 4);
+          slot_ready(j);
+          tc_fence_after();
+          const unsigned v_lo = v_lo0 + (unsigned)s * (TILE16 >> 4);
+          if (one) {
+#pragma unroll
+            for (int k = 0; k < AC_KEYS / 16; k++)
+              at_umma_ta(tmem + T_O, tmem + (unsigned)(j & 1) * AC_KEYS + (unsigned)k * 8, v_lo + (unsigned)k * (2048 >> 4), AT_DESC_HI, idesc_pv,
+                         (j > 0 || k > 0) ? 1u : 0u);
+            tc_commit(j + 1 < n_kt ? &o_done : &o_last);
+            if (j + 2 < n_kt) scores(j + 2);
+            tc_commit(&empty[s]);
+            if (j + 2 < n_kt) tc_commit(&s_full[j & 1]);
+          }
+        }
+        // the last commit's arrival, and with it all before it
+        if (!tc_wait_inline(&empty[(n_kt + 1) % NS], (n_kt + 1) / NS & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 10);
+      }
+      __syncwarp();
+    }
+  }
+  pdl_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if (dead)
+    for (int i = 0; i < 1000; i++) __nanosleep(1000);        // copies on their way land in what is still this CTA's
+  if (warp == 10) {
+    tc_fence_after();
+    tc_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// The shares of every row together: a thread takes four features of a head.
+template <int HD>
+__global__ void __launch_bounds__(256) chunk_fp8_join_kernel(const AcParams p, int shares) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int f = (int)(i % (HD / 4)) * 4;
+  const long long at = i / (HD / 4), per = (long long)p.rows * p.H;
+  if (at >= per) return;
+  const int row = (int)(at / p.H), head = (int)(at % p.H);
+  if (row < p.cu[0] || row >= p.cu[p.R]) return;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < shares; s++) m = fmaxf(m, __ldcg(p.part_s + 2 * (s * per + at)));
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < shares; s++) {
+    const float2 st = __ldcg(reinterpret_cast<const float2*>(p.part_s + 2 * (s * per + at)));
+    if (st.x == -INFINITY) { l += st.y; continue; }           // (no key, whose sums were not written, or no numbers)
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * per + at) * HD + f));
+    const float x = at_exp2(st.x - m);
+    l = fmaf(st.y, x, l);
+    o.x = fmaf(v.x, x, o.x); o.y = fmaf(v.y, x, o.y); o.z = fmaf(v.z, x, o.z); o.w = fmaf(v.w, x, o.w);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.out + row * p.ldo + (long long)head * HD + f) = make_uint2(at_pack(o.x * inv, o.y * inv), at_pack(o.z * inv, o.w * inv));
+}
+
+// ------------------------------------------------------------------------------------ host
+static int* ac_status_word() {
+  static int* words[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!words[dev]) {
+    int* w = nullptr;
+    if (cudaMalloc(&w, sizeof(int)) != cudaSuccess) return nullptr;
+    cudaMemset(w, 0, sizeof(int));
+    words[dev] = w;
+  }
+  return words[dev];
+}
+
+// Shares of the keys: as many as fill the multiprocessors, and none of fewer than four tiles
+static int ac_shares(int T, int R, int H, int G, int window, int max_keys, int sms) {
+  const int tok_tile = AC_ROWS / (H / G);
+  const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0);
+  const long long keys = window > 0 && window + tok_tile < max_keys ? window + tok_tile : max_keys;
+  const long long by_fill = sms / (tiles * G), by_work = keys / (4 * AC_KEYS);
+  const long long n = by_fill < by_work ? by_fill : by_work;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
+// float32 numbers of scratch memory that a launch over ``rows`` rows of q takes
+extern "C" long long qd_prefill_attention_fp8_scratch(int rows, int T, int R, int H, int G, int d, int window, int max_keys, int sms) {
+  if (T < 1 || R < 1 || G < 1 || H < G) return 0;
+  const int n = ac_shares(T, R, H, G, window, max_keys, sms);
+  return n > 1 ? (long long)n * rows * H * (d + 2) : 0;
+}
+
+template <int HD>
+static int ac_launch(const CUtensorMap& map, const AcParams& p, int tiles, int shares, cudaStream_t stream) {
+  const size_t smem = 1024 + (size_t)AC_STAGES * 4 * AC_KEYS * HD;
+  if (cudaFuncSetAttribute(chunk_fp8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return QD_ERR_UNSUPPORTED;
+  }
+  qd_launch(chunk_fp8_kernel<HD>, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)shares), dim3(AC_THREADS), smem, stream, map, p);
+  if (shares > 1) {
+    const long long threads = (long long)p.rows * p.H * (HD / 4);
+    qd_launch(chunk_fp8_join_kernel<HD>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p, shares);
+  }
+  return qd_last_error();
+}
+
+// q, out: bfloat16 [rows, H d], ``ldq`` and ``ldo`` apart; request r's tokens are rows cu[r] .. cu[r + 1] - 1, at most T of them in all, at the
+// positions from start[r] on, its pages row r of table [R, max_blocks]; they see the keys up to their own, the last ``window`` of them if that is
+// positive.  ``max_keys``: no request has more keys; only how the launch is cut goes by it.
+extern "C" int qd_prefill_attention_fp8(const void* q, long long ldq, void* out, long long ldo, const void* pages, long long n_pages, const int* table,
+                                        int max_blocks, const int* cu, const int* start, int R, int T, int rows, int H, int G, int d, int ps,
+                                        float scale, int window, int max_keys, float* scratch, int sms, cudaStream_t stream) {
+  if (T <= 0 || R <= 0) return 0;
+  if (G < 1 || H < 1 || H % G || H / G > 16 || (d != 64 && d != 128) || ps < 16 || ps % 16 || n_pages < 1 || n_pages > 0x7fffffffll || max_blocks < 1 ||
+      window < 0 || T > rows || G > 65535)
+    return QD_ERR_UNSUPPORTED;
+  if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages) & 15) || ldq % 8 || ldo % 8) return QD_ERR_UNSUPPORTED;
+  TcEncodeFn fn = tc_encode_fn();
+  int* status = ac_status_word();
+  if (!fn || !status) return QD_ERR_UNSUPPORTED;
+  const long long page_bytes = c8_page_bytes(G, ps, d);
+  // pages of rows of d bytes (the scales behind a page's rows are no part of it); a box is 16 rows
+  CUtensorMap map;
+  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)2 * G * ps, (cuuint64_t)n_pages};
+  cuuint64_t strides[2] = {(cuuint64_t)d, (cuuint64_t)page_bytes};
+  cuuint32_t box[3] = {(cuuint32_t)d, 16, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  if (fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pages), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return QD_ERR_UNSUPPORTED;
+  const int shares = ac_shares(T, R, H, G, window, max_keys, sms), tok_tile = AC_ROWS / (H / G);
+  AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, page_bytes, (int)n_pages, table, max_blocks, cu, start, R, H, G, ps,
+                window, tok_tile, rows, scale * 1.4426950408889634f, scratch, scratch + (long long)shares * rows * H * d, status};
+  const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0);      // of R requests at most
+  if (tiles > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
+  return d == 64 ? ac_launch<64>(map, p, (int)tiles, shares, stream) : ac_launch<128>(map, p, (int)tiles, shares, stream);
+}
+
+QD_DEFINE_WAIT_PROBE(qd_prefill_attention_fp8_wait_probe, tc_wait(bar, 0, dead, 0, poll_limit), ac_status_word, 99)
+
+// 0 if no kernel of this library has recorded a wait that ran out on the current device.  Synchronises.
+extern "C" int qd_prefill_attention_fp8_status() {
+  int* status = ac_status_word();
+  if (!status) return -1;
+  int v = 0;
+  if (cudaMemcpy(&v, status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
+  if (v) cudaMemset(status, 0, sizeof(int));
+  return v;
+}

@@ -46,6 +46,7 @@ LIBRARIES: Dict[str, str] = {
     "logprobs": "logprobs.cu",
     "cache_fp8": "cache_fp8.cu",
     "attention_fp8_decode": "attention_fp8_decode.cu",
+    "attention_fp8_chunk": "attention_fp8_chunk.cu",
     "sampling_nucleus": "sampling_nucleus.cu",
     "host_calls": "host_calls.cpp",
     "attention_generic": "attention_generic.cu",
@@ -84,6 +85,8 @@ EXTRA_DEPS: Dict[str, List[str]] = {
     "qkv_prep": ["short_conv.cuh"],
     "linear_scan": ["short_conv.cuh", "linear_chunk.cuh", "mma_sync.cuh"],
     "attention_sink": ["mma_sync.cuh"],
+    "attention_tc5": ["attention_tc5.cuh"],
+    "attention_fp8_chunk": ["attention_tc5.cuh", "tc5_ops.cuh", "fp8.cuh", "cache_fp8.cuh"],
 }
 
 _loaded: Dict[str, ctypes.CDLL] = {}

@@ -154,6 +154,8 @@ decltype(qd_sample_nucleus)* g_nucleus;
 decltype(qd_rope_kv_write_fp8)* g_write;
 decltype(qd_decode_attention_fp8)* g_decode;
 decltype(qd_decode_attention_fp8_scratch)* g_decode_scratch;
+decltype(qd_prefill_attention_fp8)* g_prefill;
+decltype(qd_prefill_attention_fp8_scratch)* g_prefill_scratch;
 
 struct Plan { int cg, bn, splits; };
 // (kept by sizes and device: a few microseconds of estimates)
@@ -487,6 +489,45 @@ CALL(decode_attention_fp8, 13)
   Py_RETURN_NONE;
 END
 
+// (q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window, max_keys, n_tokens)
+CALL(prefill_attention_fp8, 14)
+  const char* what = "prefill_attention_fp8";
+  const at::Tensor &q = tensor(a[0], "prefill_attention_fp8: q"), &out = tensor(a[1], "prefill_attention_fp8: out"), &pages = tensor(a[2], "prefill_attention_fp8: pages");
+  const at::Tensor &table = tensor(a[3], "prefill_attention_fp8: block_table"), &cu = tensor(a[4], "prefill_attention_fp8: cu_tokens");
+  const at::Tensor& start = tensor(a[5], "prefill_attention_fp8: start_pos");
+  const Heads h = heads_of(a + 6, 3, what);
+  const double scale = PyFloat_AsDouble(a[10]);
+  const int window = whole(a[11], what);
+  int64_t max_keys = a[12] == Py_None ? -1 : PyLong_AsLongLong(a[12]), T = a[13] == Py_None ? -1 : PyLong_AsLongLong(a[13]);
+  if (PyErr_Occurred()) throw PythonError{};
+  const int64_t rows = heads_rows(q, (int64_t)h.H * h.d, "prefill_attention_fp8: q"), n_pages = pages_of(pages, h, what);
+  if (heads_rows(out, (int64_t)h.H * h.d, "prefill_attention_fp8: out") != rows) refuse(what, ": q and out have ", rows, " and ", out.size(0), " rows");
+  if (table.dim() != 2 || table.size(1) < 1) refuse(what, ": block_table must be int32 [requests, pages], got ", sizes(table));
+  const int64_t R = table.size(0);
+  if (T > rows) refuse(what, ": ", T, " tokens in ", rows, " rows");
+  if (T < 0) T = rows;
+  if (window < 0) refuse(what, ": window must not be negative");
+  const int64_t held = table.size(1) * h.ps;
+  if (max_keys < 0 || max_keys > held) max_keys = held;
+  if (max_keys > INT32_MAX || R > INT32_MAX - rows) refuse(what, ": more than 2^31 keys or requests");
+  address(q);
+  const int device = q.get_device();
+  if (!out.is_cuda() || out.get_device() != device) refuse(what, ": out is on another device");
+  void *pages_at = plain(pages, at::kByte, -1, device, "prefill_attention_fp8: pages"), *table_at = plain(table, at::kInt, -1, device, "prefill_attention_fp8: block_table");
+  void *cu_at = plain(cu, at::kInt, R + 1, device, "prefill_attention_fp8: cu_tokens"), *start_at = plain(start, at::kInt, R, device, "prefill_attention_fp8: start_pos");
+  if (T == 0 || R == 0) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  const int sms = multiprocessors(device);
+  const int64_t floats = entry(g_prefill_scratch, "attention_fp8_chunk", "qd_prefill_attention_fp8_scratch")((int)rows, (int)T, (int)R, h.H, h.G, h.d, window,
+                                                                                                         (int)max_keys, sms);
+  const at::Tensor scratch = at::empty_strided({floats}, {1}, q.options().dtype(at::kFloat));
+  done(entry(g_prefill, "attention_fp8_chunk", "qd_prefill_attention_fp8")(address(q), q.stride(0), address(out), out.stride(0), pages_at, n_pages,
+                                                                          (const int*)table_at, (int)table.size(1), (const int*)cu_at, (const int*)start_at,
+                                                                          (int)R, (int)T, (int)rows, h.H, h.G, h.d, h.ps, (float)scale, window, (int)max_keys,
+                                                                          address(scratch), sms, stream_of(q)), what);
+  return PyBool_FromLong(floats > 0);
+END
+
 // (logits, temperature, top_k, top_p, min_p, draws, out, only)
 CALL(sample_nucleus, 8)
   const char* what = "sample_nucleus";
@@ -526,7 +567,7 @@ END
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(start), ENTRY(fp8_rows), ENTRY(check_rows), ENTRY(quantize_fp8), ENTRY(gate_fp8), ENTRY(add_rmsnorm_fp8), ENTRY(gemm_fp8),
                          ENTRY(gemm_fp8_gated), ENTRY(gemm_fp8_plan), ENTRY(token_logprobs), ENTRY(rope_kv_write_fp8),
-                         ENTRY(decode_attention_fp8), ENTRY(sample_nucleus), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(decode_attention_fp8), ENTRY(prefill_attention_fp8), ENTRY(sample_nucleus), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qd_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -903,6 +903,7 @@ _STATUS = {"gemm_stream": ("qd_gemm_stream_status", "qd_gemm_stream_wait_probe")
            "gemm_fp8": ("qd_gemm_fp8_status", "qd_gemm_fp8_wait_probe"),
            "gemm_f32": ("qd_gemm_f32_status", "qd_gemm_f32_wait_probe"),
            "attention_tc5": ("qd_prefill_attention_tc5_status", "qd_prefill_attention_tc5_wait_probe"),
+           "attention_fp8_chunk": ("qd_prefill_attention_fp8_status", "qd_prefill_attention_fp8_wait_probe"),
            "attention_flash": ("qd_decode_attention_tma_status", "qd_decode_attention_tma_wait_probe")}
 
 
@@ -1069,6 +1070,18 @@ def decode_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor
     holds); the launch is cut by it."""
     _launch_count[0] += 2
     (_host or _host_calls()).decode_attention_fp8(q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys)
+
+
+def prefill_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Tensor,
+                          start_pos: torch.Tensor, H: int, G: int, d: int, page_size: int, scale: float, window: int = 0,
+                          max_keys: Optional[int] = None, n_tokens: Optional[int] = None) -> None:
+    """Attention of portions over a cache in 8 bits, causal: request r's tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1 of q and out
+    (bfloat16 [T, H d], rows may lie apart; rows of no request stay as they are), at the positions from start_pos[r] on, and its pages are
+    row r of ``block_table``; a token sees the keys up to its own, the last ``window`` of them if that is not 0.  ``max_keys``: no request
+    has more (None: what the table holds), ``n_tokens``: nor all of them together more tokens (None: T); the launch is cut by both."""
+    joined = (_host or _host_calls()).prefill_attention_fp8(q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window, max_keys,
+                                                            n_tokens)
+    _launch_count[0] += 2 if joined else 1
 
 
 # ------------------------------------------------------------------ latent attention

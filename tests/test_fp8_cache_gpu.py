@@ -294,3 +294,140 @@ def test_write_then_decode_behind_other_work():
         torch.cuda.synchronize()
         outs.append(out.clone())
     assert torch.equal(*outs)
+
+
+# ---- attention of portions ---------------------------------------------------------------------------------------
+
+def check_prefill(tokens, before, H, G, d, ps=16, window=0, spread=1.0, seed=0, q_scale=1.0, spoil=None, extra_rows=(0, 0), **kw):
+    """Portions of so many tokens behind so many cached ones; ``extra_rows`` of q and out before and behind them stay as they are."""
+    gen = torch.Generator().manual_seed(seed)
+    lengths = [b + t for b, t in zip(before, tokens)]
+    pages, table = a_cache(gen, lengths, G, ps, d, spread)
+    T, (ahead, behind) = sum(tokens), extra_rows
+    q = (torch.randn((T, H * d), generator=gen) * q_scale).bfloat16()
+    reqs = [r for r, t in enumerate(tokens) for _ in range(t)]
+    positions = [b + i for b, t in zip(before, tokens) for i in range(t)]
+    want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, window, plain.BF16_HALF_STEP)
+    if spoil is not None:
+        spoil(pages, table, lengths)
+    wide = torch.zeros((ahead + T + behind, H * d), dtype=torch.bfloat16)
+    wide[ahead:ahead + T] = q
+    out = torch.full(wide.shape, 7.0, dtype=torch.bfloat16, device=DEV)
+    cu = [ahead]
+    for t in tokens:
+        cu.append(cu[-1] + t)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    args = (wide.to(DEV), out, pages.to(DEV), table.to(DEV), i32(cu), i32(before), H, G, d, ps, d ** -0.5, window)
+    kernels.prefill_attention_fp8(*args, **kw)
+    kernels.check_status()
+    got = out.cpu()
+    assert bool((got[:ahead] == 7).all()) and bool((got[ahead + T:] == 7).all())
+    off = (got[ahead:ahead + T].double() - want).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), divmod(int((off / bound).argmax()), H * d))
+    return args
+
+
+@pytest.mark.parametrize("H,G,d", [(16, 2, 128), (28, 4, 128), (14, 2, 64), (5, 1, 128), (3, 3, 64), (16, 1, 128), (11, 1, 64)])
+@pytest.mark.parametrize("tokens,before", [([1], [0]), ([5], [0]), ([130], [0]), ([20, 1, 37], [0, 200, 3]), ([129], [127]), ([300, 2], [100, 511])])
+def test_prefill(guard_regions, H, G, d, tokens, before):
+    check_prefill(tokens, before, H, G, d)
+
+
+@pytest.mark.parametrize("ps", [32, 48, 64])
+def test_prefill_page_sizes(guard_regions, ps):
+    check_prefill([ps, ps + 1, 3], [0, 77, 2 * ps - 1], 14, 2, 64, ps=ps)
+    check_prefill([ps, ps + 1, 3], [0, 77, 2 * ps - 1], 4, 2, 128, ps=ps)
+
+
+@pytest.mark.parametrize("window", [1, 16, 100, 128, 129, 5000])
+def test_prefill_window(guard_regions, window):
+    check_prefill([140, 1, 33], [0, 300, 250], 12, 2, 128, window=window)
+    check_prefill([20], [3000], 8, 1, 64, window=window)
+
+
+@pytest.mark.parametrize("tokens,before", [([1], [5000]), ([37], [4000]), ([3, 40], [9000, 10]), ([17], [1100])])
+@pytest.mark.parametrize("H,G,d", [(7, 1, 128), (4, 2, 64)])
+def test_prefill_shares_of_keys(guard_regions, tokens, before, H, G, d):
+    """Few rows behind many keys: several CTAs have a share of them, some of which a request's rows do not reach."""
+    check_prefill(tokens, before, H, G, d, extra_rows=(2, 3), n_tokens=sum(tokens))
+
+
+def test_prefill_rows_around(guard_regions):
+    check_prefill([33, 150], [70, 0], 8, 2, 128, extra_rows=(9, 4))
+    check_prefill([0, 33, 0, 5], [0, 70, 0, 2], 8, 2, 128, extra_rows=(0, 1))
+
+
+def test_prefill_many_requests(guard_regions):
+    gen = torch.Generator().manual_seed(11)
+    tokens = torch.randint(1, 4, (300,), generator=gen).tolist()
+    before = torch.randint(0, 40, (300,), generator=gen).tolist()
+    check_prefill(tokens, before, 4, 2, 64)
+
+
+def test_prefill_scales_far_apart(guard_regions):
+    check_prefill([60, 9], [200, 40], 8, 2, 128, spread=8.0, q_scale=0.01)
+    check_prefill([60, 9], [200, 40], 8, 2, 128, spread=2.0, q_scale=8.0)
+    check_prefill([60, 9], [200, 40], 8, 2, 64, q_scale=1e-20)
+
+
+def test_prefill_what_nobody_sees(guard_regions):
+    """Rows behind a request's last token, pages of nobody and keys before every row's window that are no numbers."""
+    def spoil(pages, table, lengths):
+        numbers, scales = kernels.fp8_page_views(pages, 2, 16, 128)
+        used = set()
+        for r, n in enumerate(lengths):
+            used |= {int(p) for p in table[r] if p >= 0}
+            for key in list(range(n, table.shape[1] * 16)) + list(range(0, max(0, n - 41 - 100))):
+                page = int(table[r, key // 16])
+                if page >= 0:
+                    numbers.view(torch.uint8)[page, :, :, key % 16] = 0x7f
+                    scales.view(torch.uint8)[page, :, key % 16] = 255
+        for page in range(len(pages)):
+            if page not in used:
+                pages[page] = 255
+    check_prefill([41, 7, 100], [300, 0, 13], 8, 2, 128, window=100, spoil=spoil)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_prefill_no_number_that_some_see(which):
+    """A key or value that is no number: the rows from its own on are none, in its head alone; a window past it is not."""
+    gen = torch.Generator().manual_seed(2)
+    H, G, d, ps = 4, 2, 64, 16
+    pages, table = a_cache(gen, [300], G, ps, d)
+    kernels.fp8_page_views(pages, G, ps, d)[1].view(torch.uint8)[int(table[0, 3]), 1, 5, which] = 255        # key 53 of kv head 1
+    q = torch.randn((300, H * d), generator=gen).bfloat16().to(DEV)
+    for window, last in ((0, 300), (20, 73)):
+        out = torch.empty_like(q)
+        kernels.prefill_attention_fp8(q, out, pages.to(DEV), table.to(DEV), torch.tensor([0, 300], dtype=torch.int32, device=DEV),
+                                      torch.zeros(1, dtype=torch.int32, device=DEV), H, G, d, ps, 0.1, window)
+        none = out.isnan().view(300, H, d).cpu()
+        want = torch.zeros((300, H, d), dtype=torch.bool)
+        want[53:last, 2:] = True
+        assert torch.equal(none, want)
+
+
+def test_prefill_is_decode(guard_regions):
+    """Single tokens through both kernels, within both bounds; the same bits again, in a graph on another stream."""
+    args = check_prefill([1, 1, 1], [0, 400, 77], 8, 2, 128)
+    q, out, pages, table, cu, start, H, G, d, ps, scale, window = args
+    first, other = out.clone(), torch.empty_like(out)
+    kernels.decode_attention_fp8(q, other, pages, table, torch.arange(3, dtype=torch.int32, device=DEV), start, H, G, d, ps, scale)
+    assert float((other.double() - first.double()).abs().max()) < 2.0 ** -5 * float(first.double().abs().max())
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        kernels.prefill_attention_fp8(*args)
+    out.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+
+
+def test_prefill_wait_that_runs_out():
+    kernels.check_status()
+    check_prefill([5], [0], 2, 1, 64)
+    kernels.wait_probe("attention_fp8_chunk")
+    with pytest.raises(kernels.KernelError, match="attention_fp8_chunk"):
+        kernels.check_status()
+    check_prefill([5], [0], 2, 1, 64)

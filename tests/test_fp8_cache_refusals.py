@@ -78,3 +78,15 @@ def test_sample():
             kernels.sample_nucleus(**{**good, **bad})
     with pytest.raises(KernelError, match="CUDA"):
         kernels.sample_nucleus(**good)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=torch.zeros(3, 256)), dict(q=bf16(3, 255)), dict(out=bf16(2, 256)), dict(H=34), dict(d=32), dict(page_size=24), dict(pages=torch.zeros(2, 4160)),
+    dict(block_table=i32(10)), dict(block_table=i32(2, 0)), dict(window=-1), dict(n_tokens=4)])
+def test_prefill(bad):
+    a = dict(q=bf16(3, 256), out=bf16(3, 256), pages=kernels.fp8_pages(2, 2, 16, 64, "cpu"), block_table=i32(2, 5), cu_tokens=i32(3), start_pos=i32(2), H=4, G=2, d=64,
+             page_size=16, scale=0.1)
+    with pytest.raises(KernelError):
+        kernels.prefill_attention_fp8(**{**a, **bad})
+    with pytest.raises(KernelError, match="CUDA"):
+        kernels.prefill_attention_fp8(**a)
