@@ -12,7 +12,8 @@ while a full group keeps them.  Pages are taken lazily, as the reference's
 (scheduler.cpp:43-52) or when a window has passed them.
 
 Device layout of a group: ``[layer in group, page, K|V, kv head, offset in page,
-head_dim]``, so that one (layer, page, K or V, kv head) tile is contiguous.
+head_dim]``, so that one (layer, page, K or V, kv head) tile is contiguous; in 8 bits the same numbers, and
+behind a page's the scales ``[kv head, offset in page, K|V]``.
 """
 from __future__ import annotations
 
@@ -31,13 +32,28 @@ class PagedKV:
     all of them, an integer keeps the last ``window`` positions readable.  ``v_dim``: the size of a
     value where it differs from a key's; a page is then one flat row, the keys
     [kv heads, offset in page, head_dim] followed by the values [kv heads, offset in page, v_dim]
-    (with equal sizes this is the same memory as [K|V, kv heads, offset in page, head_dim])."""
+    (with equal sizes this is the same memory as [K|V, kv heads, offset in page, head_dim]).  ``numbers`` =
+    "float8_e4m3": 8 bits with a scale to each row, a page is a row of bytes (``kernels.fp8_page_views``)."""
     num_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     v_dim: Optional[int] = None
+    numbers: Optional[str] = None
+
+    def __post_init__(self):
+        if self.numbers not in (None, "float8_e4m3") or (self.numbers and self.v_dim not in (None, self.head_dim)):
+            raise ValueError(f"a cache of keys and values in {self.numbers!r}, values of {self.v_dim}: 'float8_e4m3' with values of a key's size, or None")
+
+    @property
+    def dtype(self) -> Optional[torch.dtype]:
+        """Of the pages' tensor; None: the cache's."""
+        return torch.uint8 if self.numbers else None
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        if self.numbers:
+            if page_size % 16:
+                raise ValueError(f"a cache in 8 bits takes pages of a multiple of 16 tokens, got {page_size}")
+            return (self.num_kv_heads * page_size * (2 * self.head_dim + 2),)
         if self.v_dim is None or self.v_dim == self.head_dim:
             return (2, self.num_kv_heads, page_size, self.head_dim)
         return (self.num_kv_heads * page_size * (self.head_dim + self.v_dim),)
@@ -50,6 +66,7 @@ class PagedRows:
     ``[offset in page, width]``, contiguous."""
     width: int
     window: Optional[int] = None
+    dtype = None
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
         return (page_size, self.width)
@@ -173,7 +190,7 @@ class CacheManager:
             for g, grp in enumerate(layout.groups):
                 self.kv[g] = torch.zeros(
                     (len(grp.entries), num_pages + 1) + tuple(grp.need.page_shape(page_size)),
-                    dtype=dtype, device=self.device)
+                    dtype=grp.need.dtype or dtype, device=self.device)
             # one slot more than requests: the padding rows of a padded decode batch update that one
             for i, need in enumerate(layout.fixed_needs):
                 self.states[i] = torch.zeros((max_requests + 1,) + tuple(need.shape), dtype=need.dtype,
@@ -193,9 +210,9 @@ class CacheManager:
     @staticmethod
     def bytes_per_page(layout: CacheLayout, page_size: int, dtype: torch.dtype) -> int:
         """Device bytes one page id costs over all groups and layers."""
-        es = torch.empty((), dtype=dtype).element_size()
         import math
-        return sum(len(g.entries) * math.prod(g.need.page_shape(page_size)) * es for g in layout.groups)
+        size = lambda g: torch.empty((), dtype=g.need.dtype or dtype).element_size()
+        return sum(len(g.entries) * math.prod(g.need.page_shape(page_size)) * size(g) for g in layout.groups)
 
     def _pages_for(self, g: int, first_token: int, total_tokens: int) -> range:
         """Logical pages of group g that tokens [first_token, total_tokens) touch."""

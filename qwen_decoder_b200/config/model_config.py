@@ -83,6 +83,9 @@ class Qwen2Config:
     # with a scale to each 128 features (the reference has 16-bit weights only).  The stored tensors are the same.
     projection_dtype: Optional[str] = None
     output_projection_dtype: Optional[str] = None
+    # What keys and values are cached in: None, the engine's dtype, or "float8_e4m3", 8 bits with a scale to each head's row (the
+    # reference caches 16 bits, gpu_decoder.cu:208-216).
+    cache_dtype: Optional[str] = None
     eos_token_ids: tuple = ()
     torch_dtype: str = "bfloat16"
     extra: dict = field(default_factory=dict, compare=False, hash=False)
@@ -135,7 +138,7 @@ class Qwen2Config:
         pairing = _get(d, "rope_pairing", str, "half")
         if pairing not in ("adjacent", "half"):
             raise ConfigError(f"config.json: 'rope_pairing' must be 'adjacent' or 'half', got {pairing!r}")
-        projections = {key: _get(d, key, str, None) for key in ("projection_dtype", "output_projection_dtype")}
+        projections = {key: _get(d, key, str, None) for key in ("projection_dtype", "output_projection_dtype", "cache_dtype")}
         for key, value in projections.items():
             if value not in (None, "float8_e4m3"):
                 raise ConfigError(f"config.json: '{key}' must be 'float8_e4m3' if given, got {value!r}")
@@ -202,7 +205,7 @@ class Qwen2Config:
         }
         if self.eos_token_ids:
             d["eos_token_id"] = list(self.eos_token_ids)
-        for key in ("projection_dtype", "output_projection_dtype"):
+        for key in ("projection_dtype", "output_projection_dtype", "cache_dtype"):
             if getattr(self, key) is not None:
                 d[key] = getattr(self, key)
         return d

@@ -6,7 +6,7 @@ attention with q/k/v bias and rotary positions -> residual -> pre-norm -> SwiGLU
 feed-forward -> residual; final norm; output projection (tied to the embedding
 when ``tie_word_embeddings`` is set, which the reference cannot do:
 common.cpp:119 requires ``output.weight``).  With ``projection_dtype`` the same layers of
-parts whose products take 8 bits.
+parts whose products take 8 bits, with ``cache_dtype`` of mixers that cache 8 bits.
 """
 from __future__ import annotations
 
@@ -34,6 +34,7 @@ def describe_qwen2(cfg: Qwen2Config) -> ModelSpec:
                 "position": "rope",
                 "window": None,
                 "prefix": "self_attn.",
+                **({} if cfg.cache_dtype is None else {"cache_dtype": cfg.cache_dtype}),
             }),
             feed_forward=PartSpec("swiglu" + in_8_bits, {
                 "hidden_size": cfg.hidden_size,

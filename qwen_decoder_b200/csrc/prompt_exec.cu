@@ -72,6 +72,16 @@ struct PeFns8 {
   decltype(&qd_gemm_fp8_few) gemm_few;
 };
 
+// A cache in 8 bits (null ``write``: none): its launchers, room for the rotated q [T, Hd] and for attention's scratch, which the single tokens' and the
+// portions' take one after the other; most keys of the two kinds' requests
+struct PeCache8 {
+  decltype(&qd_rope_kv_write_fp8) write;
+  decltype(&qd_decode_attention_fp8) decode;
+  decltype(&qd_prefill_attention_fp8) prefill;
+  void* q; float* scratch;
+  int n_pos, table_rows, decode_keys, prefill_keys;
+};
+
 // How a product is cut (``qd_gemm_pair_plan``; in 8 bits ``qd_gemm_fp8_plan``); cg 0: the library's product (in 8 bits ``gemm_few``)
 struct PePlan { int cg, bn, splits; };
 
@@ -110,6 +120,7 @@ struct PeParams {
   PePlan qkv_plan8, wo_plan8, wgu_plan8, wd_plan8;
   float* qkv32;                    // [T, (H+2G)d], up to ``few8`` tokens
   int few8, final8;
+  PeCache8 cache8;
 };
 
 extern "C" int qd_prompt_exec_struct_sizes(int* layer_bytes, int* layer8_bytes, int* params_bytes) {
@@ -159,6 +170,21 @@ static int product8(const PeParams& p, const PePlan& plan, const PeRows8& W, con
                     p.sms, stream);
 }
 
+// A layer's rotation and cache write from rows of q, k and v, and its attention, with a cache in 8 bits
+static int attend8(const PeParams& p, const PeLayer& L, const void* rows, int dtype, const float* bias, cudaStream_t stream) {
+  const PeCache8& c = p.cache8;
+  const int T = p.T, H = p.H, G = p.G, d = p.d, nd = p.n_decode, n_qkv = (H + 2 * G) * d;
+  int rc = c.write(rows, dtype, n_qkv, 1, 0, bias, c.q, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, c.n_pos, p.positions, L.kv, p.n_pages, p.slot_map,
+                   p.page_size, L.write_kv, p.sms, stream);
+  if (rc == 0 && nd > 0)
+    rc = c.decode(c.q, H * d, p.attn, H * d, L.kv, p.n_pages, p.block_table, p.max_blocks, c.table_rows, p.token_req, p.positions, nd, H, G, d, p.page_size,
+                  p.scale, p.window, c.decode_keys, c.scratch, p.sms, stream);
+  if (rc == 0)
+    rc = c.prefill(c.q, H * d, p.attn, H * d, L.kv, p.n_pages, p.block_table + (size_t)nd * p.max_blocks, p.max_blocks, p.cu_tokens + nd, p.start_pos + nd,
+                   p.R - nd, T - nd, T, H, G, d, p.page_size, p.scale, p.window, c.prefill_keys, c.scratch, p.sms, stream);
+  return rc;
+}
+
 #define PE_TRY(call)            \
   do {                          \
     int rc_ = (call);           \
@@ -172,6 +198,7 @@ extern "C" int qd_prompt_exec(const PeParams* pp, cudaStream_t stream) {
   if (shares < 0 || shares == 1 ||
       (shares > 1 && (!p.down_part || !p.fn.gemm_batched || !p.fn.plain_next || p.F % (8 * shares))))
     return QD_ERR_UNSUPPORTED;
+  if (p.cache8.write && (!p.cache8.decode || !p.cache8.prefill || !p.cache8.q)) return QD_ERR_UNSUPPORTED;
   if (p.shares && (!p.fn.attention_shares || !p.fn.decode_shares)) return QD_ERR_UNSUPPORTED;
   if ((p.wo_plan.cg || p.wgu_plan.cg || p.wd_plan.cg) && !p.fn.gemm_pair) return QD_ERR_UNSUPPORTED;
   if ((p.wo_plan.cg && p.wo_plan.splits > 1 && !p.o_part) || (p.wd_plan.cg && p.wd_plan.splits > 1 && !p.down_part)) return QD_ERR_UNSUPPORTED;
@@ -191,7 +218,11 @@ extern "C" int qd_prompt_exec(const PeParams* pp, cudaStream_t stream) {
     if (layers8) {
       const PeLayer8& W = layers8[l];
       PE_TRY(p.fn8.add_rmsnorm(p.x, delta, QD_BF16, nullptr, L.norm1_w, p.h8.q, p.h8.ldq, p.h8.s, p.h8.lds, nullptr, T, D, L.eps1, 1, 1, xn, stream));
-      if (T <= p.few8) {
+      const bool few = T <= p.few8;
+      if (p.cache8.write) {
+        PE_TRY(product8(p, p.qkv_plan8, W.wqkv, p.h8, few ? nullptr : L.bqkv, few ? p.qkv32 : p.qkv, few ? QD_F32 : QD_BF16, n_qkv, D, stream));
+        PE_TRY(attend8(p, L, few ? p.qkv32 : p.qkv, few ? QD_F32 : QD_BF16, few ? L.bqkv : nullptr, stream));
+      } else if (few) {
         PE_TRY(product8(p, p.qkv_plan8, W.wqkv, p.h8, nullptr, p.qkv32, QD_F32, n_qkv, D, stream));
         PE_TRY(p.fn8.rope_partial(p.qkv32, 1, L.bqkv, p.qkv, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv, p.slot_map,
                                   p.page_size, L.write_kv, stream));
@@ -205,10 +236,11 @@ extern "C" int qd_prompt_exec(const PeParams* pp, cudaStream_t stream) {
       PE_TRY(p.fn.add_rmsnorm(p.x, delta, delta ? delta_dtype : -1, L.norm1_w, p.h, QD_BF16, nullptr, T, D, L.eps1, 1,
                               delta_parts, xn, stream));
       PE_TRY(product(p, L.wqkv, p.h, p.qkv, T, n_qkv, D));
-      PE_TRY(p.fn.rope_kv_write(p.qkv, L.bqkv, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv,
-                                p.slot_map, p.page_size, L.write_kv, stream));
+      if (p.cache8.write) PE_TRY(attend8(p, L, p.qkv, QD_BF16, L.bqkv, stream));
+      else PE_TRY(p.fn.rope_kv_write(p.qkv, L.bqkv, T, H, G, d, p.rotary_dim, p.pairing, p.cos_t, p.sin_t, p.positions, L.kv,
+                                     p.slot_map, p.page_size, L.write_kv, stream));
     }
-    const int nd = p.n_decode;
+    const int nd = p.cache8.write ? 0 : p.n_decode;
     if (nd > 0 && p.shares && l == 0) PE_TRY(p.fn.decode_shares(p.positions, p.slot_map, p.scratch_row, nd, p.n_shares, p.shares, stream));
     if (nd > 0 && p.shares)
       PE_TRY(p.fn.attention_shares(p.qkv, ldq, p.attn, L.kv, p.n_pages, p.block_table, p.max_blocks, nd, H, G, d, p.page_size,
@@ -222,7 +254,8 @@ extern "C" int qd_prompt_exec(const PeParams* pp, cudaStream_t stream) {
                                    nd, H, G, d, p.page_size, p.scale, p.window, p.decode_splits, p.part_o, p.part_ml,
                                    p.tickets, stream));
     const int* bt = p.block_table + (size_t)nd * p.max_blocks;
-    if (p.use_tc5)
+    if (p.cache8.write) {
+    } else if (p.use_tc5)
       PE_TRY(p.fn.attention_tc5(p.qkv, ldq, p.attn, L.kv, p.n_pages, bt, p.max_blocks, p.cu_tokens + nd,
                                 p.start_pos + nd, p.R - nd, T - nd, H, G, d, p.page_size, p.scale, p.window, nullptr,
                                 stream));

@@ -13,7 +13,8 @@ folder needs config.json only; weights N(0, 0.02) from ``--weights-seed`` are ma
 ``--prompt-ids`` / ``--prompt-file`` / ``--random-prompts`` instead of standard input, and ``--stats``:
 one line per step as the reference prints it (decoder.cpp:178-185: tokens, decoding and prefilling
 requests, prompt tokens) with the step's device time and the free pages, and prompt and decode
-tokens per second apart at the end; ``--projection-dtype float8_e4m3`` (8-bit products) and ``--logprobs K``.
+tokens per second apart at the end; ``--projection-dtype float8_e4m3`` (8-bit products), ``--cache-dtype float8_e4m3`` (8-bit
+cache), ``--logprobs K``, ``--top-p P`` and ``--min-p P``.
 """
 from __future__ import annotations
 
@@ -48,6 +49,8 @@ def main(argv=None) -> int:
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=30)
+    ap.add_argument("--top-p", type=float, default=1.0, help="the most probable tokens that make up this much of what --top-k leaves")
+    ap.add_argument("--min-p", type=float, default=0.0, help="tokens of at least this times the largest probability")
     ap.add_argument("--max-new-tokens", type=int, default=256)
     ap.add_argument("--seed", type=int, default=42)
     ap.add_argument("--ignore-eos", action="store_true")
@@ -69,6 +72,7 @@ def main(argv=None) -> int:
     ap.add_argument("--projection-dtype", choices=["float8_e4m3"], default=None,
                     help="the layers' products in 8 bits, with a scale to each 128 features")
     ap.add_argument("--output-projection-dtype", choices=["float8_e4m3"], default=None, help="the product over the vocabulary, too")
+    ap.add_argument("--cache-dtype", choices=["float8_e4m3"], default=None, help="keys and values cached in 8 bits, with a scale to each row")
     ap.add_argument("--logprobs", type=int, default=None, metavar="K",
                     help="each output token's log probability, and the K (0 to 32) most probable tokens in its place")
     args = ap.parse_args(argv)
@@ -105,12 +109,12 @@ def main(argv=None) -> int:
                    max_total_tokens=args.max_total_tokens, page_size=args.page_size, num_pages=args.num_pages,
                    enable_prefix_cache=bool(args.enable_prefix_cache), run_ahead=not args.no_run_ahead,
                    record_steps=args.stats, projection_dtype=args.projection_dtype,
-                   output_projection_dtype=args.output_projection_dtype)
+                   output_projection_dtype=args.output_projection_dtype, cache_dtype=args.cache_dtype)
     if args.random_weights:
         engine = Engine(config=load_config(args.model), random_seed=args.weights_seed, **options)
     else:
         engine = Engine(args.model, **options)
-    params = SamplingParams(temperature=args.temperature, top_k=args.top_k,
+    params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
                             max_new_tokens=args.max_new_tokens, seed=args.seed, ignore_eos=args.ignore_eos,
                             logprobs=args.logprobs)
     t0 = time.time()

@@ -30,7 +30,8 @@ class Engine:
                  page_size: int = 16, num_pages: Optional[int] = None, kv_memory_fraction: float = 0.8,
                  max_positions: Optional[int] = None, use_graphs: bool = True,
                  enable_prefix_cache: bool = False, run_ahead: bool = True, record_steps: bool = False,
-                 projection_dtype: Optional[str] = None, output_projection_dtype: Optional[str] = None):
+                 projection_dtype: Optional[str] = None, output_projection_dtype: Optional[str] = None,
+                 cache_dtype: Optional[str] = None):
         """``model``: a folder with config.json and model.safetensors; or give ``config`` (a typed
         configuration) and ``random_seed`` for random weights made on the device.
 
@@ -49,11 +50,13 @@ class Engine:
         decoded tokens, requests, device time by CUDA events, free pages, queue lengths -- what the reference
         prints per step (decoder.cpp:178-185) and more; each step is also an NVTX range then.
         ``projection_dtype``, ``output_projection_dtype``: "float8_e4m3" has the layers' products, and the one over the
-        vocabulary, in 8 bits where the configuration does not say so."""
+        vocabulary, in 8 bits where the configuration does not say so; ``cache_dtype``: likewise the cache of keys and values, which then
+        holds nearly twice the tokens in the same memory."""
         self.max_prefill_len = max_prefill_len
         make = dict(dtype=dtype, device=device, page_size=page_size, max_requests=max_batch,
                     max_positions=max_positions, use_graphs=use_graphs, prefix_cache=enable_prefix_cache,
-                    projections={"projection_dtype": projection_dtype, "output_projection_dtype": output_projection_dtype})
+                    projections={"projection_dtype": projection_dtype, "output_projection_dtype": output_projection_dtype,
+                                 "cache_dtype": cache_dtype})
         sizing = _PageSizing(num_pages, kv_memory_fraction, page_size, resolve_dtype(dtype))
         if model is not None:
             self.runner = ModelRunner.from_folder(model, num_pages=sizing, **make)
@@ -84,6 +87,8 @@ class Engine:
         rid = self._next_id if request_id is None else request_id
         if params is not None and params.logprobs is not None:
             self._check_top(params.logprobs)
+        if params is not None and not (0.0 < params.top_p <= 1.0 and 0.0 <= params.min_p <= 1.0):
+            raise ValueError(f"top_p must be above 0 and at most 1, min_p between 0 and 1, got {params.top_p} and {params.min_p}")
         self._next_id += 1
         req = Request(rid, [int(t) for t in prompt], params or SamplingParams())
         req.sample_key = self._next_id - 1
@@ -108,10 +113,11 @@ class Engine:
             self._end_record(rec)
             return flight
         ahead = 1 if device_tokens is not None else 0       # a step planned ahead samples one token later
-        logits, ids = self.runner.step(entries, ensure_pages=False, device_tokens=device_tokens, sampling=(
-            [r.params.temperature for r in sampling], [r.params.top_k for r in sampling],
-            [uniform_draw(r.params.seed, r.sample_key, len(r.output) + ahead) if r.params.temperature else 0.0
-             for r in sampling]))
+        how = ([r.params.temperature for r in sampling], [r.params.top_k for r in sampling],
+               [uniform_draw(r.params.seed, r.sample_key, len(r.output) + ahead) if r.params.temperature else 0.0 for r in sampling])
+        if any(r.params.temperature and (r.params.top_p < 1.0 or r.params.min_p > 0.0) for r in sampling):
+            how += ([r.params.top_p for r in sampling], [r.params.min_p for r in sampling])
+        logits, ids = self.runner.step(entries, ensure_pages=False, device_tokens=device_tokens, sampling=how)
         self._end_record(rec)
         self._turn ^= 1
         flight.host = self._host_tokens[self._turn][:len(sampling)]

@@ -17,6 +17,7 @@ import torch
 from ..cache import CacheManager, RequestCache
 from ..config import describe_model, load_config
 from ..parts.model import DecoderModel, build_model
+from ..sampling import without_nucleus
 from ..weights import TensorSource, load_into, random_tensors
 from .batch import MetaLayout, StepEntry, StepError, build_context, fill, uneven_contexts, validate
 
@@ -44,13 +45,13 @@ def require_cuda(device) -> torch.device:
 
 
 def with_projections(config, projections: Optional[dict]):
-    """``config`` with what ``projections`` gives of ``projection_dtype`` and ``output_projection_dtype`` (not None)."""
+    """``config`` with what ``projections`` gives of ``projection_dtype``, ``output_projection_dtype`` and ``cache_dtype`` (not None)."""
     given = {k: v for k, v in (projections or {}).items() if v is not None}
     for key, value in given.items():
-        if key not in ("projection_dtype", "output_projection_dtype") or value != "float8_e4m3":
-            raise ValueError(f"projections: 'projection_dtype' and 'output_projection_dtype' may be 'float8_e4m3', got {key!r}: {value!r}")
+        if key not in ("projection_dtype", "output_projection_dtype", "cache_dtype") or value != "float8_e4m3":
+            raise ValueError(f"projections: 'projection_dtype', 'output_projection_dtype' and 'cache_dtype' may be 'float8_e4m3', got {key!r}: {value!r}")
         if not hasattr(config, key):
-            raise ValueError(f"projections in 8 bits: {type(config).__name__} has no {key!r}")
+            raise ValueError(f"{'a cache' if key == 'cache_dtype' else 'projections'} in 8 bits: {type(config).__name__} has no {key!r}")
     return dataclasses.replace(config, **given) if given else config
 
 
@@ -86,7 +87,7 @@ class ModelRunner:
     # ---- construction ----------------------------------------------------
     @classmethod
     def from_folder(cls, model_dir: str, dtype="bfloat16", device="cuda:0", projections: Optional[dict] = None, **kw) -> "ModelRunner":
-        """``projections``: ``projection_dtype`` and ``output_projection_dtype`` in place of the configuration's."""
+        """``projections``: ``projection_dtype``, ``output_projection_dtype`` and ``cache_dtype`` in place of the configuration's."""
         device = require_cuda(device)
         dt = resolve_dtype(dtype)
         config = with_projections(load_config(model_dir), projections)
@@ -137,7 +138,7 @@ class ModelRunner:
         With ``ensure_pages`` the pages the new tokens need are taken first (``OutOfPages`` if the
         pool cannot give them; nothing is taken then).  Afterwards each request's cached length has
         grown by its tokens.  With ``sampling`` = (temperatures, top_ks, draws), one per wanted
-        place, returns (logits, sampled int32 tokens on the device).
+        place, or (temperatures, top_ks, draws, top_ps, min_ps), returns (logits, sampled int32 tokens on the device).
 
         ``device_tokens`` (int32 on the device, one per entry): the entries' single tokens are not known
         on the host yet -- they are what an earlier step sampled and has not been read back -- and are
@@ -206,17 +207,23 @@ class ModelRunner:
         mbs = tuple((max(len(e.cache.tables[g]) for e in entries) + 31) // 32 * 32
                     for g in range(len(self.cache.pools)))
         uneven = Bp > 16 and uneven_contexts(starts, Bp)      # up to 16 tokens attention has a kernel that does not ask
-        key = (Bp, mbs, sampling is not None, uneven)
+        nucleus = sampling is not None and len(sampling) > 3
+        key = (Bp, mbs, sampling is not None, uneven, nucleus)
         g = self._graphs.get(key)
         if g is None:
-            g = self._graphs[key] = _DecodeGraph(self, Bp, mbs, sampling is not None, uneven)
+            g = self._graphs[key] = _DecodeGraph(self, Bp, mbs, sampling is not None, uneven, nucleus)
         host = g.next_host()
         h = host.numpy()
         fill(h, g.lay, entries, self.cache, lens, starts, slots, self.model.vocab_size)
         o = g.lay.off["extra"]
         if sampling is not None:
-            temps, top_ks, draws = sampling
+            temps, top_ks, draws = sampling[:3]
             hf = h.view(np.float32)
+            if nucleus:
+                h[o:o + 6 * Bp] = 0
+                for i, values in enumerate((*sampling[3:], temps)):
+                    hf[o + (3 + i) * Bp:o + (3 + i) * Bp + R] = values
+                temps = without_nucleus(temps, *sampling[3:])
             hf[o:o + R] = temps
             h[o + Bp:o + Bp + R] = top_ks
             hf[o + 2 * Bp:o + 2 * Bp + R] = draws
@@ -245,13 +252,14 @@ class _NotOnHost:
 class _DecodeGraph:
     """One captured decode step for a padded batch size and block-table widths."""
 
-    def __init__(self, runner: "ModelRunner", Bp: int, mbs, with_sampling: bool, uneven: bool):
+    def __init__(self, runner: "ModelRunner", Bp: int, mbs, with_sampling: bool, uneven: bool, nucleus: bool):
         # no reference back to the runner: a cycle would leave the captured graph to the garbage
         # collector, which might then destroy it in the middle of another capture
         self.model = runner.model
         self.device = runner.device
         self.with_sampling = with_sampling
-        self.lay = MetaLayout(Bp, Bp, Bp, mbs, extra=3 * Bp)
+        self.nucleus = nucleus
+        self.lay = MetaLayout(Bp, Bp, Bp, mbs, extra=(6 if nucleus else 3) * Bp)
         # two pinned staging buffers: one may still be in flight while the next step is written
         self.hosts = [torch.empty(self.lay.total, dtype=torch.int32, pin_memory=True) for _ in range(2)]
         self.events = [None, None]
@@ -268,6 +276,8 @@ class _DecodeGraph:
         self.temps = self.dev[o:o + Bp].view(torch.float32)
         self.top_ks = self.dev[o + Bp:o + 2 * Bp]
         self.draws = self.dev[o + 2 * Bp:o + 3 * Bp].view(torch.float32)
+        # of rows with top-p or min-p, whose temperature above is 0
+        self.top_ps, self.min_ps, self.nucleus_temps = (self.dev[o + i * Bp:o + (i + 1) * Bp].view(torch.float32) if nucleus else None for i in (3, 4, 5))
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.logits = None
         self.tokens = None
@@ -291,6 +301,8 @@ class _DecodeGraph:
             if self.with_sampling:
                 self.tokens = torch.empty(self.lay.T, dtype=torch.int32, device=self.device)
                 kernels.sample(self.logits, self.temps, self.top_ks, self.draws, self.tokens)
+                if self.nucleus:
+                    kernels.sample_nucleus(self.logits, self.nucleus_temps, self.top_ks, self.top_ps, self.min_ps, self.draws, self.tokens, only=True)
 
     def run(self) -> None:
         if self.graph is None:

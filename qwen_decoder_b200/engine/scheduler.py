@@ -34,6 +34,9 @@ class SamplingParams:
     """Defaults follow the reference's main (gpu_main.cu:45-48) except top_k, which is off."""
     temperature: float = 0.0
     top_k: int = 0
+    # of what top_k leaves, the most probable tokens that make up ``top_p`` of its probability, and those of at least ``min_p`` times the largest
+    top_p: float = 1.0
+    min_p: float = 0.0
     max_new_tokens: int = 256
     seed: int = 0
     stop_ids: Sequence[int] = ()

@@ -2106,6 +2106,12 @@ class PromptPlan(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("cg", "bn", "splits")]
 
 
+class PromptCache8(ctypes.Structure):
+    """A cache in 8 bits in the native prompt step (PeCache8 in csrc/prompt_exec.cu)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("write", "decode", "prefill", "q", "scratch")] + \
+        [(n, ctypes.c_int) for n in ("n_pos", "table_rows", "decode_keys", "prefill_keys")]
+
+
 class PromptParams(ctypes.Structure):
     """Arguments of the native prompt step (PeParams in csrc/prompt_exec.cu)."""
     _fields_ = [("fn", PromptFns), ("layers", ctypes.c_void_p), ("n_layers", ctypes.c_int)] + \
@@ -2122,7 +2128,7 @@ class PromptParams(ctypes.Structure):
         [("shares", ctypes.c_void_p), ("n_shares", ctypes.c_int), ("scratch_row", ctypes.c_int)] + \
         [("fn8", PromptFns8), ("layers8", ctypes.c_void_p)] + [(n, PromptRows8) for n in ("h8", "attn8", "act8", "hrows8")] + \
         [(n, PromptPlan) for n in ("qkv_plan8", "wo_plan8", "wgu_plan8", "wd_plan8")] + \
-        [("qkv32", ctypes.c_void_p), ("few8", ctypes.c_int), ("final8", ctypes.c_int)]
+        [("qkv32", ctypes.c_void_p), ("few8", ctypes.c_int), ("final8", ctypes.c_int), ("cache8", PromptCache8)]
 
 
 def prompt_exec_struct_sizes_match() -> bool:
@@ -2184,6 +2190,20 @@ def prompt_fns8() -> PromptFns8:
         fns = _prompt_fns["fp8"] = PromptFns8(addr(library("elementwise").qd_rope_kv_write_partial), addr(rows.qd_rows_fp8), addr(rows.qd_add_rmsnorm_fp8),
                                               addr(library("gemm_fp8").qd_gemm_fp8), addr(library("gemm_fp8_few").qd_gemm_fp8_few))
     return fns
+
+
+def prompt_cache8(R: int, T: int, n_decode: int, H: int, G: int, d: int, window: int, decode_keys: int, prefill_keys: int):
+    """(the launchers of a cache in 8 bits for the native prompt step of R requests and T tokens, the first ``n_decode`` of them single; float32
+    numbers of scratch that their attention takes)."""
+    dec, pre = library("attention_fp8_decode"), library("attention_fp8_chunk")
+    addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+    dec.qd_decode_attention_fp8_scratch.restype = pre.qd_prefill_attention_fp8_scratch.restype = _LL
+    sms = sm_count()
+    floats = max(dec.qd_decode_attention_fp8_scratch(n_decode, H, G, d, window, decode_keys, sms) if n_decode else 0,
+                 pre.qd_prefill_attention_fp8_scratch(T, T - n_decode, R - n_decode, H, G, d, window, prefill_keys, sms))
+    c = PromptCache8(addr(library("cache_fp8").qd_rope_kv_write_fp8), addr(dec.qd_decode_attention_fp8), addr(pre.qd_prefill_attention_fp8))
+    c.table_rows, c.decode_keys, c.prefill_keys = R, decode_keys, prefill_keys
+    return c, floats
 
 
 def decode_scratch(n_tokens: int, H: int, d: int, G: int, splits: int, device):

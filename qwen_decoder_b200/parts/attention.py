@@ -9,6 +9,8 @@ attends keys 0..pos with scores (q.k) / sqrt(d), softmax, weighted sum of v
 bias (gpu_decoder.cu:423).  Prompt portions and decoded tokens run through the same
 kernels: a portion's keys are in the pages before its queries read them.
 ``window`` = w limits a query to the last w keys (the reference has no window).
+``cache_dtype`` = "float8_e4m3" caches keys and values in 8 bits with a scale to each row, rounded where they are written;
+queries, scores and sums stay as they are (the reference caches 16 bits).
 """
 from __future__ import annotations
 
@@ -30,7 +32,8 @@ from .linear import Linear
 class GQAttention(Mixer):
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  qkv_bias: bool = True, out_bias: bool = False, position=None,
-                 window: Optional[int] = None, prefix: str = "self_attn.", scale: Optional[float] = None):
+                 window: Optional[int] = None, prefix: str = "self_attn.", scale: Optional[float] = None,
+                 cache_dtype: Optional[str] = None):
         if num_heads % num_kv_heads:
             raise ValueError(f"num_kv_heads ({num_kv_heads}) must divide num_heads ({num_heads})")
         self.hidden_size = hidden_size
@@ -40,18 +43,27 @@ class GQAttention(Mixer):
         self.window = window
         self.position = position        # a PositionEncoding part (Rotary) or None
         self.scale = float(scale) if scale is not None else 1.0 / math.sqrt(head_dim)
+        self.cache_dtype = cache_dtype
+        if cache_dtype is not None:
+            rot = position.rotary_dim if position is not None else 0
+            if cache_dtype != "float8_e4m3" or not kernels.fp8_cache_supported(num_heads, num_kv_heads, head_dim, 16) or \
+                    rot % (16 if rot and position.pairing_code else 8):
+                raise ValueError(f"cache_dtype: 'float8_e4m3' with head sizes 64 and 128, up to 16 query heads per KV head and rotated widths of a multiple "
+                                 f"of 16 (of 8 where neighbours pair), got {cache_dtype!r} with {num_heads} and {num_kv_heads} heads of {head_dim}, {rot} rotated")
         self.qkv = Linear(hidden_size, [(f"{prefix}q_proj", num_heads * head_dim),
                                         (f"{prefix}k_proj", num_kv_heads * head_dim),
                                         (f"{prefix}v_proj", num_kv_heads * head_dim)], bias=qkv_bias)
         self.out = Linear(num_heads * head_dim, [(f"{prefix}o_proj", hidden_size)], bias=out_bias)
 
     def cache_need(self):
-        return PagedKV(self.num_kv_heads, self.head_dim, self.window)
+        return PagedKV(self.num_kv_heads, self.head_dim, self.window, numbers=self.cache_dtype)
 
     def tensor_specs(self) -> List[TensorSpec]:
         return self.qkv.tensor_specs() + self.out.tensor_specs()
 
     def bind(self, source: TensorSource, dtype: torch.dtype, device: torch.device) -> None:
+        if self.cache_dtype is not None and dtype != torch.bfloat16:
+            raise ValueError(f"a cache in 8 bits belongs to a bfloat16 engine, got {dtype}")
         self.dtype = dtype
         self.qkv.bind(source, dtype, device)
         self.out.bind(source, dtype, device)
@@ -64,7 +76,7 @@ class GQAttention(Mixer):
         return {"kind": "gq_attention", "D": self.hidden_size, "H": self.num_heads, "G": self.num_kv_heads, "d": self.head_dim,
                 "window": self.window, "scale": self.scale, "position": pos,
                 "rotary_dim": pos.rotary_dim if pos is not None else 0,
-                "pairing": pos.pairing_code if pos is not None else 0,
+                "pairing": pos.pairing_code if pos is not None else 0, "cache_dtype": self.cache_dtype,
                 "wqkv": self.qkv.weight, "bqkv": self.qkv.bias, "wo": self.out.weight}
 
     def _few_token_sums(self, x: torch.Tensor) -> Optional[torch.Tensor]:
@@ -78,12 +90,30 @@ class GQAttention(Mixer):
     def _out_product(self, attn: torch.Tensor) -> torch.Tensor:
         return self.out.forward_partial(attn)
 
+    def _attend_in_8_bits(self, x, part: Optional[torch.Tensor], rope, ctx, cache: PagedCacheView) -> torch.Tensor:
+        """Attention over a cache in 8 bits: from the products' sums or rows to the attention output."""
+        H, G, d, group, window = self.num_heads, self.num_kv_heads, self.head_dim, cache.group, self.window or 0
+        rows, bias = (part, self.qkv.bias) if part is not None else (self.qkv.forward(x), None)
+        T, ps = ctx.num_tokens, group.page_size
+        q, attn = (torch.empty((T, H * d), dtype=self.dtype, device=ctx.positions.device) for _ in range(2))
+        kernels.rope_kv_write_fp8(rows, bias, q, H, G, d, *rope, ctx.positions, cache.kv, group.slot_map, ps, cache.write)
+        nd, keys = (T, ctx.max_context) if ctx.all_decode else (ctx.num_decode, ctx.decode_max_context)
+        if nd:
+            kernels.decode_attention_fp8(q[:nd], attn[:nd], cache.kv, group.block_table, ctx.token_request[:nd], ctx.positions[:nd], H, G, d, ps,
+                                         self.scale, window, keys)
+        if nd < T:
+            kernels.prefill_attention_fp8(q, attn, cache.kv, group.block_table[nd:], ctx.cu_tokens[nd:], ctx.start_pos[nd:], H, G, d, ps, self.scale,
+                                          window, ctx.max_context, T - nd)
+        return attn
+
     def forward(self, x: torch.Tensor, ctx, cache: PagedCacheView) -> torch.Tensor:
         H, G, d = self.num_heads, self.num_kv_heads, self.head_dim
         pos, dtype = self.position, self.dtype
         rope = (pos.rotary_dim if pos is not None else 0, pos.pairing_code if pos is not None else 0,
                 pos.cos if pos is not None else None, pos.sin if pos is not None else None)
         part = self._few_token_sums(x)
+        if self.cache_dtype is not None:
+            return self._out_product(self._attend_in_8_bits(x, part, rope, ctx, cache))
         if part is not None:
             # few tokens: the product leaves float32 partial sums; bias, rotation and cache write take them
             ps, window = cache.group.page_size, self.window or 0

@@ -65,7 +65,7 @@ class NativePrompt:
             answer = getattr(model.layers[e.layer], "native_params", lambda: None)()
             if answer is None or answer.get("composition") not in (COMPOSITION, COMPOSITION_8):
                 return None
-            key = {k: answer[k] for k in ("composition", "D", "H", "G", "d", "F", "window", "scale", "rotary_dim", "pairing")}
+            key = {k: answer[k] for k in ("composition", "D", "H", "G", "d", "F", "window", "scale", "rotary_dim", "pairing", "cache_dtype")}
             key["position"] = id(answer["position"])
             if common is None:
                 common = dict(key, position_obj=answer["position"])
@@ -184,10 +184,19 @@ class NativePrompt:
         p = kernels.PromptParams()
         use_tc5 = self.attention_impl(group.page_size)
         # a mixed step: its single tokens (first in the batch) go to the split-KV decode kernel
-        nd = ctx.num_decode if kernels.flash_decode_supported(bf, H, G, d, group.page_size) else 0
-        p.fn = kernels.prompt_fns(bool(use_tc5), nd > 0, nd > 0 and kernels.decode_by_tma(d))
+        cache8 = c["cache_dtype"] is not None
+        nd = ctx.num_decode if cache8 or kernels.flash_decode_supported(bf, H, G, d, group.page_size) else 0
+        flash = nd > 0 and not cache8
+        p.fn = kernels.prompt_fns(bool(use_tc5), flash, flash and kernels.decode_by_tma(d))
         keep = None
-        if nd:
+        if cache8:
+            p.n_decode, p.token_req = nd, ctx.token_request.data_ptr()
+            keys = max(1, ctx.decode_max_context)
+            p.cache8, floats = kernels.prompt_cache8(ctx.num_requests, T, nd, H, G, d, c["window"] or 0, keys, ctx.max_context)
+            keep = torch.empty((T, H * d), dtype=bf, device=dev), torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
+            p.cache8.q, p.cache8.scratch = (t.data_ptr() for t in keep)
+            p.cache8.n_pos = pos.cos.shape[0] if pos is not None and c["rotary_dim"] else 0
+        elif nd:
             from .attention import decode_splits
             window = c["window"] or 0
             p.n_decode = nd

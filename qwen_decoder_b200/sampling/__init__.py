@@ -1,3 +1,3 @@
-from .sampler import Sampler, uniform_draw
+from .sampler import Sampler, uniform_draw, without_nucleus
 
-__all__ = ["Sampler", "uniform_draw"]
+__all__ = ["Sampler", "uniform_draw", "without_nucleus"]
