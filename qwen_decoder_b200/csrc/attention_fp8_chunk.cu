@@ -9,14 +9,19 @@
 //   and nothing is converted.  Both operands have to be of 8 bits then, so a row of q is two of them: e4m3 numbers of q over the row's scale,
 //   and of what their rounding left, over a sixteenth of it.  Together they are the bfloat16 number itself where it is above 2^-14 of the row's
 //   largest, and off by 2^-23 of that below.  Two products of 128 features in 8 bits take the tensor cores as long as one of bfloat16.
-// * Values become bfloat16, scale included, which is exact: four warps take tiles from where the copies leave them to where the product reads
-//   them (P and sums as ever).  P in 8 bits would be two numbers as q is, for every weight; this is 16 KB of values to a tile for all 128 rows.
-//   They also bring the keys' scales to tensor memory.
+// * Values become float16, an e4m3 number's scale over the tile's largest one, E, included, which is exact down to 2^-15 E: four warps take tiles from
+//   where the copies leave them to where the product reads them.  P is float16 too, 2^(z + log E - reference): the product's sums are of
+//   values as they are, a row's sum of weights takes a tile's over E.  P is scaled so that 2^8 stands for the largest weight at the time its
+//   reference was taken, and is off by 2^-12 of itself, or by 2^-33 of that weight where that is more.  Where a tile has a scale below 2^-15 of the
+//   largest one up to it, values and P are bfloat16 from there on as long as that is so, whose exponents take anything.  (P in 8 bits would
+//   be two numbers as q is, for every weight; this is 16 KB of values to a tile for all 128 rows.  Values to bfloat16, for every tile, took
+//   twice the instructions: 2,048 tokens behind 6,144 420 us.)  These warps also bring the keys' scales to tensor memory.
 // * A key or value that is no number has the scale 255.  The value becomes zeros, its key's scale 255, so that the score is none and
 //   every row that sees it, and no other, is none.  Values behind the last row's position, which may be anything, become zeros.
 // * Few tiles of rows (a short portion behind a long history) share their keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
 //
-// Warps: 0..7 softmax (two threads to a row: halves of the keys and of the columns), 8 and 9 copies of keys and values, 10 MMAs, 12..15 values.
+// Warps: 0..7 softmax (two threads to a row: halves of the keys and of the columns), 8 and 9 copies of keys and values, 10 MMAs, 11 scales,
+// 12..15 values.
 // Slot i (i = -2 .. n - 1; stage (i + 2) % 3) holds the keys of tile i + 2 with their scales and the values of tile i: what the MMA warp
 // reads in its step i, behind one barrier.  Every wait on an mbarrier is bounded, as in attention_tc5.cu.
 #include "attention_tc5.cuh"
@@ -27,15 +32,23 @@
 #include <cuda_fp16.h>
 
 #define AC_SOFTMAX 256                 // threads
+#define AC_VALUES 128                  // threads that convert
 #define AC_THREADS 512
 #define AC_STAGES 3
 #define AC_META 256                    // requests whose token ranges are staged in shared memory
 #define AC_ROWS 128
 #define AC_KEYS 128
-#define AC_GROW 8.0f                   // powers of two by which a row's maximum grows before it is followed
-#define AC_REGS_SOFTMAX 184            // 2 x 184 + 56 + 88 = 512: what 4 x 128 at the launch add up to
+#define AC_GROW 7.0f                   // powers of two by which a row's maximum grows before it is followed
+#define AC_TOP 8.0f                    // log2 of what stands for the maximum: below 2^15 in all, within float16
+#define AC_WIDE 256u                   // beside a tile's largest scale: values and weights in bfloat16
+#define AC_HOLES 512u                  // and: some of the values are nobody's or no numbers
+#define AC_AHEAD 8                     // tiles of whose scales something is kept
+#define AC_SPREAD 15                   // powers of two between scales up to which they are float16
+#define AC_REGS 128                    // a thread's at the launch; the host looks that it is so: a split that adds up to more waits for ever
+#define AC_REGS_SOFTMAX 184            // 2 x 184 + 56 + 88 = 4 x 128
 #define AC_REGS_ISSUE 56
 #define AC_REGS_VALUES 88
+static_assert(2 * AC_REGS_SOFTMAX + AC_REGS_ISSUE + AC_REGS_VALUES <= 4 * AC_REGS, "registers of the block's four groups of warps");
 
 struct AcParams {
   const bf16* q; long long ldq;
@@ -43,7 +56,7 @@ struct AcParams {
   const unsigned char* pages; long long page_bytes; int n_pages;
   const int* table; int max_blocks;
   const int *cu, *start;
-  int R, H, G, ps, window, tok_tile, rows;
+  int R, H, G, ps, ps_shift, window, tok_tile, rows;      // ps_shift: log2 of ps, or -1
   float scale_log2e;
   float *part_o, *part_s;              // [share][rows][H][HD]; [share][rows][H][2]: maximum, sum
   int* status;
@@ -66,6 +79,17 @@ __device__ __forceinline__ void ac_mma_scaled(unsigned d, unsigned a, unsigned d
 __device__ __forceinline__ void ac_st4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ unsigned ac_halves(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+// two e4m3 numbers times two float16 numbers
+__device__ __forceinline__ unsigned ac_f16x2(unsigned short two, unsigned f) {
+  unsigned h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+  asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(f));
+  return h;
+}
 // two e4m3 numbers times f as bfloat16
 __device__ __forceinline__ unsigned ac_bf16x2(unsigned short two, float f) {
   unsigned h;
@@ -77,7 +101,7 @@ __device__ __forceinline__ unsigned ac_bf16x2(unsigned short two, float f) {
 template <int HD>
 __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_constant__ CUtensorMap map, const AcParams p) {
   constexpr int KQ = AC_KEYS / 2, DH = HD / 2, NS = AC_STAGES;
-  constexpr int TILE8 = AC_KEYS * HD, TILE16 = 2 * TILE8;           // bytes of a tile in 8 bits, in bfloat16
+  constexpr int TILE8 = AC_KEYS * HD, TILE16 = 2 * TILE8;           // bytes of a tile in 8 bits, in 16
   constexpr int BOX = 16 * HD;
   // tensor memory: two buffers of scores and weights, the sums, q's two operands of HD / 4 columns, their scales, the keys' scales
   constexpr unsigned TMEM_COLS = 512, T_O = 2 * AC_KEYS, T_Q = 3 * AC_KEYS, T_SA = 448, T_SB = 456;
@@ -87,11 +111,14 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   unsigned char* base = smem_raw + ((1024 - (tc_smem(smem_raw) & 1023)) & 1023);
   unsigned char* k_s = base;                        // NS stages of keys
   unsigned char* v8_s = k_s + NS * TILE8;           // NS stages of values as they come
-  unsigned char* v_s = v8_s + NS * TILE8;           // NS stages of values in bfloat16
+  unsigned char* v_s = v8_s + NS * TILE8;           // NS stages of values in 16 bits
   __shared__ unsigned long long full[NS], empty[NS], v8_full[NS], v8_empty[NS], s_full[2], p_full[2], o_done, o_last, q_full;
   __shared__ float mx_s[2][2][AC_ROWS], l_s[2][AC_ROWS];
   __shared__ unsigned sa_s[AC_ROWS];
-  __shared__ unsigned short sc_s[4][AC_KEYS];       // of a tile's keys: both scales
+  // of a tile: its values' largest scale with AC_WIDE and AC_HOLES, its keys' scales, by what its values are multiplied (two float16 numbers; a
+  // float32 number where they become bfloat16; 0: nobody's)
+  __shared__ unsigned tile_s[AC_AHEAD];
+  __shared__ __align__(16) unsigned key_s[AC_AHEAD][AC_KEYS / 4], factor_s[AC_AHEAD][AC_KEYS];
   __shared__ unsigned tmem_slot;
   __shared__ int dead;
   __shared__ int cu_s[AC_META + 1], sp_s[AC_META + 1];
@@ -100,15 +127,16 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   if (threadIdx.x == 0) {
     dead = 0;
     for (int s = 0; s < NS; s++) {
-      tc_bar_init(&full[s], 1 + 128);
+      // (a warp's threads arrive by one of them)
+      tc_bar_init(&full[s], 1 + AC_VALUES / 32);
       tc_bar_init(&empty[s], 1);
-      tc_bar_init(&v8_full[s], 1);
-      tc_bar_init(&v8_empty[s], 128);
+      tc_bar_init(&v8_full[s], 2);
+      tc_bar_init(&v8_empty[s], AC_VALUES / 32);
     }
-    for (int s = 0; s < 2; s++) { tc_bar_init(&s_full[s], 1); tc_bar_init(&p_full[s], AC_SOFTMAX); }
+    for (int s = 0; s < 2; s++) { tc_bar_init(&s_full[s], 1); tc_bar_init(&p_full[s], AC_SOFTMAX / 32); }
     // (o_last: the last product has no scores behind it by which its phase of o_done would be known)
     tc_bar_init(&o_done, 1); tc_bar_init(&o_last, 1);
-    tc_bar_init(&q_full, AC_SOFTMAX);
+    tc_bar_init(&q_full, AC_SOFTMAX / 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 10) tc_alloc(&tmem_slot, TMEM_COLS);
@@ -147,10 +175,13 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   const int t0 = key_lo / AC_KEYS, tn = idle ? 0 : (key_hi + AC_KEYS - 1) / AC_KEYS - t0;
   const int kt_lo = t0 + (int)((long long)tn * blockIdx.z / gridDim.z), n_kt = t0 + (int)((long long)tn * (blockIdx.z + 1) / gridDim.z) - kt_lo;
   const int* table = p.table + (long long)(idle ? 0 : r) * p.max_blocks;
-  auto page_at = [&](int key) {                       // keys that are none: any page will do
-    if (key >= key_hi || key / p.ps >= p.max_blocks) return 0;
-    return min(max(table[key / p.ps], 0), p.n_pages - 1);
+  // of a key: its page's entry in the table, for whoever needs it a tile later (keys that are none: any page will do); the page; the place in it
+  auto entry_at = [&](int key) {
+    const int block = p.ps_shift >= 0 ? key >> p.ps_shift : key / p.ps;
+    return key < key_hi && block < p.max_blocks ? table[block] : 0;
   };
+  auto page_of_entry = [&](int entry) { return min(max(entry, 0), p.n_pages - 1); };
+  auto offset_of = [&](int key) { return p.ps_shift >= 0 ? key & (p.ps - 1) : key % p.ps; };
 
   if (warp < AC_SOFTMAX / 32) {
     // ------------------------------------------------------------------ softmax: two threads to a row
@@ -208,42 +239,69 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       }
       tc_st_wait();
       tc_fence_before();
-      tc_arrive(&q_full);
+      __syncwarp();
+      if (lane == 0) tc_arrive(&q_full);
     }
     float m = -INFINITY, l = 0.f;        // m: the maximum that this row's exponentials, sum and output refer to
     const int free_hi = pos0 + 1, free_lo = ac_key_lo(p, key_hi - 1);       // keys that every row sees need no test
     for (int j = 0; j < n_kt; j++) {
       const int tile_base = (kt_lo + j) * AC_KEYS, key_base = tile_base + h * KQ;
       if (!tc_wait_inline(&s_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 7);
+      __syncwarp();                                  // (here and below: what follows is the whole warp's instruction)
       tc_fence_after();
       float sv[KQ];
       at_tmem_ld<KQ>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * KQ, sv);
       const bool interior = tile_base >= free_lo && tile_base + AC_KEYS <= free_hi && p.scale_log2e > 0.f;
-      float mx = -INFINITY;
-      if (interior) {
-#pragma unroll
-        for (int i = 0; i < KQ; i++) mx = fmaxf(mx, sv[i]);
-        mx *= p.scale_log2e;
-      } else {
+      if (!interior) {
 #pragma unroll
         for (int i = 0; i < KQ; i++) {
           const int key = key_base + i;
           sv[i] = ok && key <= pos && key >= lo ? sv[i] * p.scale_log2e : -INFINITY;
-          mx = fmaxf(mx, sv[i]);
         }
       }
+      float mx4[4] = {sv[0], sv[1], sv[2], sv[3]};   // (one chain of 64 would be four cycles each)
+#pragma unroll
+      for (int i = 4; i < KQ; i++) mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
+      const float mul = interior ? p.scale_log2e : 1.0f;
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
       mx_s[j & 1][h][row] = mx;
-      asm volatile("bar.sync 1, %0;" ::"n"(AC_SOFTMAX) : "memory");
-      const float m_tile = fmaxf(mx, mx_s[j & 1][h ^ 1][row]);
+      const unsigned tile = tile_s[j % AC_AHEAD];
+      const float top = (float)((int)(tile & 255u) - 127);
+      unsigned pk[KQ / 2];
+      float sum;
+      auto weigh = [&]() {                           // against the row's reference
+        const float ref = (m == -INFINITY ? 0.f : m) - top - AC_TOP;
+        sum = 0.f;
+        if (tile & AC_WIDE) {
+#pragma unroll
+          for (int i = 0; i < KQ / 2; i++) {
+            const float p0 = at_exp2(fmaf(sv[2 * i], mul, -ref)), p1 = at_exp2(fmaf(sv[2 * i + 1], mul, -ref));
+            sum += p0 + p1;
+            pk[i] = at_pack(p0, p1);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < KQ / 2; i++) {
+            const float p0 = at_exp2(fmaf(sv[2 * i], mul, -ref)), p1 = at_exp2(fmaf(sv[2 * i + 1], mul, -ref));
+            sum += p0 + p1;
+            pk[i] = ac_halves(p0, p1);
+          }
+        }
+      };
+      // Weights first, against the reference as it is; the other thread's maximum then seldom says that it has to move (the first tile's always).
+      if (j > 0) weigh();
+      asm volatile("bar.sync %0, 64;" ::"r"(3 + (warp & 3)) : "memory");       // the two warps of these rows
+      const float m_tile = fmaxf(mx, mx_s[j & 1][h ^ 1][row]) + top;           // of weights with the largest of the tile's scales
       // the row moves to a new reference only when its maximum has grown by more than AC_GROW (always from "no key yet"); both threads of a
       // row decide alike, and the warp acts together
       const bool grow = m_tile > m + AC_GROW;
-      if (__any_sync(0xffffffffu, grow)) {
+      if (__any_sync(0xffffffffu, grow) || j == 0) {
         const float alpha = grow ? at_exp2(m - m_tile) : 1.0f;
         if (grow) m = m_tile;
         l *= alpha;
         if (j > 0) {
           if (!tc_wait_inline(&o_done, (j - 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 8);
+          __syncwarp();
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < DH; c += 32) {
@@ -255,25 +313,18 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
             at_tmem_st<32>(t_lane + T_O + h * DH + c, ob);
           }
         }
+        weigh();
       }
-      const float ref = m == -INFINITY ? 0.f : m;
-      unsigned pk[KQ / 2];
-      float sum = 0.f;
-      const float mul = interior ? p.scale_log2e : 1.0f;
-#pragma unroll
-      for (int i = 0; i < KQ / 2; i++) {
-        const float p0 = at_exp2(fmaf(sv[2 * i], mul, -ref)), p1 = at_exp2(fmaf(sv[2 * i + 1], mul, -ref));
-        sum += p0 + p1;
-        pk[i] = at_pack(p0, p1);
-      }
-      l += sum;
+      l = fmaf(sum, __uint_as_float((254u - (tile & 255u)) << 23), l);
       // over the first half of this tile's own scores, which every thread of the row has in registers since the barrier above
       at_tmem_st<KQ / 2>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * (KQ / 2), pk);
       tc_fence_before();
-      tc_arrive(&p_full[j & 1]);
+      __syncwarp();
+      if (lane == 0) tc_arrive(&p_full[j & 1]);
     }
     if (n_kt > 0) {
       if (!tc_wait_inline(&o_last, 0, &dead) && lane == 0) atomicCAS(p.status, 0, 9);
+      __syncwarp();
       tc_fence_after();
     }
     l_s[h][row] = l;
@@ -315,103 +366,170 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       }
     }
   } else if (warp >= 12) {
-    // ------------------------------------------------------------------ the keys' scales, and values to bfloat16
+    // ------------------------------------------------------------------ the keys' scales, and values to 16 bits
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AC_REGS_VALUES));
-    const int ct = threadIdx.x - 384;
+    // A warp's threads take 8 rows of 64 features at a time, four threads to a row: row r's 16 features in a block are where the swizzles put them,
+    // and with the rows in this order (r and r ^ 5 side by side) neither the 16 bytes read nor the two times 16 written meet a conflict.
+    const int q = lane >> 2, c = lane & 3, x = q & 1 ? (q >> 1) ^ 5 : q >> 1;
     const unsigned t_sb = tmem + ((unsigned)((warp & 3) * 32) << 16) + T_SB;
-    auto key_of = [&](int j) { return (kt_lo + j) * AC_KEYS + ct; };
-    auto scales_at = [&](int j, int page) {           // of this thread's key of tile j
-      const int key = key_of(j);
-      if (j >= n_kt || key >= key_hi) return (unsigned short)0x7f7f;
-      const unsigned char* s = p.pages + page * p.page_bytes + (long long)2 * p.G * p.ps * HD + ((long long)g * p.ps + key % p.ps) * 2;
-      return *reinterpret_cast<const volatile unsigned short*>(s);
-    };
-    unsigned short sc = n_kt > 0 ? scales_at(0, page_at(key_of(0))) : 0;
-    int page = n_kt > 1 ? page_at(key_of(1)) : 0;
+    constexpr int STEPS = AC_KEYS / 8 / 4 * (HD / 64);       // of a warp: 8 rows each, four groups of rows apart, one block of features after the other
     for (int i = -2; i < n_kt; i++) {
       const int s = (i + 2) % NS, j = i + 2;
-      if (j < n_kt) {
-        sc_s[j & 3][ct] = sc;
-        sc = scales_at(j + 1, page);
-        page = j + 2 < n_kt ? page_at(key_of(j + 2)) : 0;
-      }
-      if (!tc_wait_inline(&empty[s], ((i + 2) / NS & 1) ^ 1, &dead)) atomicCAS(p.status, 0, 5);
+      if (!tc_wait_inline(&empty[s], ((i + 2) / NS & 1) ^ 1, &dead) && lane == 0) atomicCAS(p.status, 0, 5);
+      if (!tc_wait_inline(&v8_full[s], (i + 2) / NS & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 6);
+      __syncwarp();
       tc_fence_after();
-      asm volatile("bar.sync 2, 128;" ::: "memory");
-      if (j < n_kt) {
-        unsigned w[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const unsigned both = sc_s[j & 3][32 * c + lane];
-          w[c] = both >> 8 == 255u ? 255u : both & 255u;
-        }
-        ac_st4(t_sb + 4 * s, w[0], w[1], w[2], w[3]);
+      if (j < n_kt) {                                 // the keys' scales: lane l, column c has row 32 c + l's
+        const unsigned char* k = reinterpret_cast<const unsigned char*>(key_s[j % AC_AHEAD]) + lane;
+        ac_st4(t_sb + 4 * s, k[0], k[32], k[64], k[96]);
       }
       if (i >= 0) {
-        if (!tc_wait_inline(&v8_full[i % NS], i / NS & 1, &dead)) atomicCAS(p.status, 0, 6);
-        const unsigned char* from = v8_s + (i % NS) * TILE8;
-        unsigned char* to = v_s + s * TILE16;
-        constexpr int PIECES = HD / 16;               // of 16 features
+        const unsigned tile = tile_s[i % AC_AHEAD];
+        const unsigned* factor = factor_s[i % AC_AHEAD] + (warp & 3) * 8 + x;
+        const unsigned char* from = v8_s + s * TILE8 + ((warp & 3) * 8 + x) * HD;
+        unsigned char* to = v_s + s * TILE16 + ((warp & 3) * 8 + x) * 128;
+        const int a_at = ((2 * c) ^ x) << 4, b_at = ((2 * c + 1) ^ x) << 4;
 #pragma unroll
-        for (int e = 0; e < PIECES; e++) {
-          const int at = ct + 128 * e, key = at / PIECES, c = at % PIECES, k = (kt_lo + i) * AC_KEYS + key;
-          const int place = HD == 128 ? c ^ (key & 7) : c ^ (key >> 1 & 3);
-          uint4 v = *reinterpret_cast<const uint4*>(from + key * HD + 16 * place);
-          const unsigned byte = sc_s[i & 3][key] >> 8;
-          const bool none = byte == 255u || k >= key_hi || k < key_lo;
-          if (none) v = make_uint4(0, 0, 0, 0);
-          const float f = none ? 0.f : c8_power(byte);
-          const uint4 a = make_uint4(ac_bf16x2((unsigned short)v.x, f), ac_bf16x2((unsigned short)(v.x >> 16), f),
-                                     ac_bf16x2((unsigned short)v.y, f), ac_bf16x2((unsigned short)(v.y >> 16), f));
-          const uint4 b = make_uint4(ac_bf16x2((unsigned short)v.z, f), ac_bf16x2((unsigned short)(v.z >> 16), f),
-                                     ac_bf16x2((unsigned short)v.w, f), ac_bf16x2((unsigned short)(v.w >> 16), f));
-          // chunks 2 c and 2 c + 1 of 8 features, in blocks of 64; the second half of a row's threads begins with the other one, against conflicts
-          unsigned char* block = to + (c >> 2) * (AC_KEYS * 128) + key * 128;
-          const int chunk = 2 * (c & 3), x = key & 7;
-          const bool swap = HD == 128 && c >= 4;
-          *reinterpret_cast<uint4*>(block + (((chunk + swap) ^ x) << 4)) = swap ? b : a;
-          *reinterpret_cast<uint4*>(block + (((chunk + !swap) ^ x) << 4)) = swap ? a : b;
+        for (int e0 = 0; e0 < STEPS; e0 += 4) {
+          const int block = e0 / 4;
+          uint4 v[4];
+          unsigned f[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            v[e] = *reinterpret_cast<const uint4*>(from + e * 32 * HD + 16 * (HD == 128 ? (4 * block + c) ^ x : c ^ (x >> 1 & 3)));
+            f[e] = factor[e * 32];
+          }
+          if (tile & (AC_WIDE | AC_HOLES)) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (f[e] == 0) v[e] = make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const unsigned* w = &v[e].x;
+            unsigned o[8];
+            if (tile & AC_WIDE) {
+#pragma unroll
+              for (int y = 0; y < 4; y++) {
+                o[2 * y] = ac_bf16x2((unsigned short)w[y], __uint_as_float(f[e]));
+                o[2 * y + 1] = ac_bf16x2((unsigned short)(w[y] >> 16), __uint_as_float(f[e]));
+              }
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; y++) {
+                o[2 * y] = ac_f16x2((unsigned short)w[y], f[e]);
+                o[2 * y + 1] = ac_f16x2((unsigned short)(w[y] >> 16), f[e]);
+              }
+            }
+            unsigned char* row = to + block * (AC_KEYS * 128) + e * 32 * 128;
+            *reinterpret_cast<uint4*>(row + a_at) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(row + b_at) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
         }
-        tc_arrive(&v8_empty[i % NS]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       tc_st_wait();
       tc_fence_before();
-      tc_arrive(&full[s]);
+      __syncwarp();
+      if (lane == 0) {
+        tc_arrive(&v8_empty[s]);
+        tc_arrive(&full[s]);
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AC_REGS_ISSUE));
     if (warp < 10) {
       // ---------------------------------------------------------------- copies: a tile is eight boxes of 16 keys, each from its page
       const int which = warp - 8;                     // 0 keys, 1 values
-      auto page_of = [&](int j) { return lane < 8 && j < n_kt ? page_at((kt_lo + j) * AC_KEYS + 16 * lane) : 0; };
-      int page_next = page_of(0);
-      for (int j = 0; j < n_kt + (which ? 0 : 2); j++) {       // (the last two slots have no keys)
-        const int page = page_next, s = j % NS;
-        page_next = page_of(j + 1);
+      auto entry_of = [&](int j) { return lane < 8 && j < n_kt ? entry_at((kt_lo + j) * AC_KEYS + 16 * lane) : 0; };
+      int next = entry_of(0);
+      // slot i = u - 2 has the keys of tile u and the values of tile u - 2; a slot without is told without
+      for (int u = 0; u < n_kt + 2; u++) {
+        const int s = u % NS, j = which ? u - 2 : u;
+        const bool have = j >= 0 && j < n_kt;
         unsigned long long* bar = which ? &v8_full[s] : &full[s];
-        if (!tc_wait_inline(which ? &v8_empty[s] : &empty[s], (j / NS & 1) ^ 1, &dead)) {
+        if (!tc_wait_inline(which ? &v8_empty[s] : &empty[s], (u / NS & 1) ^ 1, &dead)) {
           if (lane == 0) atomicCAS(p.status, 0, 1);
           break;                                      // (nobody waits any more, and no more copies are to arrive)
         }
         if (lane == 0) {
-          if (j < n_kt) tc_expect_tx(bar, TILE8);
+          if (have) tc_expect_tx(bar, TILE8);
           else tc_arrive(bar);
         }
         __syncwarp();
-        if (j < n_kt && lane < 8) {
-          const int key = (kt_lo + j) * AC_KEYS + 16 * lane;
-          ac_load_3d((which ? v8_s : k_s) + s * TILE8 + lane * BOX, &map, (which * p.G + g) * p.ps + key % p.ps, page, bar);
+        if (have) {
+          const int page = page_of_entry(next);
+          next = entry_of(j + 1);
+          if (lane < 8) {
+            const int key = (kt_lo + j) * AC_KEYS + 16 * lane;
+            ac_load_3d((which ? v8_s : k_s) + s * TILE8 + lane * BOX, &map, (which * p.G + g) * p.ps + offset_of(key), page, bar);
+          }
         }
+      }
+    } else if (warp == 11) {
+      // ---------------------------------------------------------------- scales, two tiles ahead of the values: a thread has four neighbouring keys'
+      const unsigned char* scales = p.pages + (long long)2 * p.G * p.ps * HD + (long long)g * p.ps * 2;
+      auto key_of = [&](int j) { return (kt_lo + j) * AC_KEYS + 4 * lane; };
+      auto scales_at = [&](int j, int entry) {
+        const int key = key_of(j);
+        if (j >= n_kt || key >= key_hi) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+        return __ldcg(reinterpret_cast<const uint2*>(scales + page_of_entry(entry) * p.page_bytes + 2 * offset_of(key)));
+      };
+      uint2 sc = n_kt > 0 ? scales_at(0, entry_at(key_of(0))) : make_uint2(0, 0);
+      int entry = n_kt > 1 ? entry_at(key_of(1)) : 0;
+      unsigned largest = 0;                           // of the values' scales so far
+      for (int u = 0; u < n_kt + 2; u++) {
+        const int s = u % NS;
+        if (!tc_wait_inline(&v8_empty[s], (u / NS & 1) ^ 1, &dead) && lane == 0) atomicCAS(p.status, 0, 11);
+        __syncwarp();
+        if (u < n_kt) {
+          const uint2 now = sc;
+          sc = scales_at(u + 1, entry);
+          entry = u + 2 < n_kt ? entry_at(key_of(u + 2)) : 0;
+          unsigned bk[4], bv[4], most = 0, least = 255;
+          bool all = true;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const unsigned both = (e < 2 ? now.x : now.y) >> 16 * (e & 1) & 0xffffu;
+            bv[e] = both >> 8;
+            bk[e] = bv[e] == 255u ? 255u : both & 255u;      // (a value without a number: its key's score is none)
+            const int key = key_of(u) + e;
+            if (key >= key_hi || key < key_lo) bv[e] = 255u;
+            all &= bv[e] != 255u;
+            if (bv[e] != 255u) { most = max(most, bv[e] + 1); least = min(least, bv[e]); }
+          }
+          most = __reduce_max_sync(0xffffffffu, most);
+          least = __reduce_min_sync(0xffffffffu, least);
+          all = __all_sync(0xffffffffu, all);
+          if (most == 0) least = 127;                 // (no value that is seen)
+          most = most ? most - 1 : 127u;
+          largest = max(largest, most);
+          const bool wide = largest - least > AC_SPREAD;
+          unsigned f[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const unsigned down = most - min(bv[e], most);
+            if (bv[e] == 255u) f[e] = 0;
+            else if (wide) f[e] = __float_as_uint(scalbnf(1.f, -(int)down));
+            else f[e] = (down < 15 ? (15u - down) << 10 : 0x200u) * 0x10001u;
+          }
+          const int at = u % AC_AHEAD;
+          key_s[at][lane] = bk[0] | bk[1] << 8 | bk[2] << 16 | bk[3] << 24;
+          *reinterpret_cast<uint4*>(&factor_s[at][4 * lane]) = make_uint4(f[0], f[1], f[2], f[3]);
+          if (lane == 0) tile_s[at] = most | (wide ? AC_WIDE : 0u) | (all ? 0u : AC_HOLES);
+        }
+        __syncwarp();
+        if (lane == 0) tc_arrive(&v8_full[s]);
       }
     } else if (warp == 10 && !idle) {
       // ---------------------------------------------------------------- MMAs: the whole warp goes through the tiles, one lane issues
       const bool one = tc_elect();
       const unsigned idesc_qk = (unsigned)(AC_KEYS >> 3) << 17 | 1u << 23 | (unsigned)(AC_ROWS >> 4) << 24;
-      const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(HD >> 3) << 17) | ((unsigned)(AC_ROWS >> 4) << 24);
+      const unsigned idesc_f16 = (1u << 4) | (1u << 16) | ((unsigned)(HD >> 3) << 17) | ((unsigned)(AC_ROWS >> 4) << 24);
       const unsigned k_lo0 = at_desc_lo(tc_smem(k_s), 0), v_lo0 = at_desc_lo(tc_smem(v_s), AC_KEYS * 128);
       auto slot_ready = [&](int i) {
         if (!tc_wait_inline(&full[(i + 2) % NS], ((i + 2) / NS) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 2);
+        __syncwarp();
       };
       auto scores = [&](int j) {
         const unsigned k_lo = k_lo0 + (unsigned)(j % NS) * (TILE8 >> 4);
@@ -438,7 +556,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           if (!tc_wait_inline(&p_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 4);
           slot_ready(j);
           tc_fence_after();
-          const unsigned v_lo = v_lo0 + (unsigned)s * (TILE16 >> 4);
+          const unsigned v_lo = v_lo0 + (unsigned)s * (TILE16 >> 4), idesc_pv = idesc_f16 | (tile_s[j % AC_AHEAD] & AC_WIDE ? 1u << 7 | 1u << 10 : 0u);
           if (one) {
 #pragma unroll
             for (int k = 0; k < AC_KEYS / 16; k++)
@@ -528,9 +646,17 @@ extern "C" long long qd_prefill_attention_fp8_scratch(int rows, int T, int R, in
 template <int HD>
 static int ac_launch(const CUtensorMap& map, const AcParams& p, int tiles, int shares, cudaStream_t stream) {
   const size_t smem = 1024 + (size_t)AC_STAGES * 4 * AC_KEYS * HD;
-  if (cudaFuncSetAttribute(chunk_fp8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return QD_ERR_UNSUPPORTED;
+  static bool allowed[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QD_ERR_UNSUPPORTED;
+  if (!allowed[dev]) {
+    cudaFuncAttributes of;
+    if (cudaFuncGetAttributes(&of, chunk_fp8_kernel<HD>) != cudaSuccess || of.numRegs != AC_REGS ||
+        cudaFuncSetAttribute(chunk_fp8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+      cudaGetLastError();
+      return QD_ERR_UNSUPPORTED;
+    }
+    allowed[dev] = true;
   }
   qd_launch(chunk_fp8_kernel<HD>, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)shares), dim3(AC_THREADS), smem, stream, map, p);
   if (shares > 1) {
@@ -551,23 +677,12 @@ extern "C" int qd_prefill_attention_fp8(const void* q, long long ldq, void* out,
       window < 0 || T > rows || G > 65535)
     return QD_ERR_UNSUPPORTED;
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages) & 15) || ldq % 8 || ldo % 8) return QD_ERR_UNSUPPORTED;
-  TcEncodeFn fn = tc_encode_fn();
   int* status = ac_status_word();
-  if (!fn || !status) return QD_ERR_UNSUPPORTED;
-  const long long page_bytes = c8_page_bytes(G, ps, d);
-  // pages of rows of d bytes (the scales behind a page's rows are no part of it); a box is 16 rows
   CUtensorMap map;
-  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)2 * G * ps, (cuuint64_t)n_pages};
-  cuuint64_t strides[2] = {(cuuint64_t)d, (cuuint64_t)page_bytes};
-  cuuint32_t box[3] = {(cuuint32_t)d, 16, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  if (fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pages), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return QD_ERR_UNSUPPORTED;
+  if (!status || !c8_make_map(&map, pages, n_pages, G, ps, d)) return QD_ERR_UNSUPPORTED;
   const int shares = ac_shares(T, R, H, G, window, max_keys, sms), tok_tile = AC_ROWS / (H / G);
-  AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, page_bytes, (int)n_pages, table, max_blocks, cu, start, R, H, G, ps,
-                window, tok_tile, rows, scale * 1.4426950408889634f, scratch, scratch + (long long)shares * rows * H * d, status};
+  AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, c8_page_bytes(G, ps, d), (int)n_pages, table, max_blocks, cu, start, R, H, G, ps,
+                ps & (ps - 1) ? -1 : __builtin_ctz(ps), window, tok_tile, rows, scale * 1.4426950408889634f, scratch, scratch + (long long)shares * rows * H * d, status};
   const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0);      // of R requests at most
   if (tiles > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   return d == 64 ? ac_launch<64>(map, p, (int)tiles, shares, stream) : ac_launch<128>(map, p, (int)tiles, shares, stream);

@@ -4,11 +4,12 @@
 //
 // Bound by the cache's bytes; what a design has to do is keep them coming and turn them into operands cheaply.
 //
-// * A warp takes 16 keys at a time, straight from memory into registers: keys as the rows of m16n8k16 products, the query heads of the KV
-//   head as their 8 columns (two such for groups of 9 to 16).  Both contractions leave the order of their index free, so each thread loads 16
-//   contiguous bytes: of the keys, features 16 c.. of rows lane / 4 (and 8 more), with q's fragments in the same order; of the values, 16
-//   features of four keys, whose bytes it interleaves by pairs of keys.  Nothing passes through shared memory, and the weights go from the
-//   first product's result to the second's operand by one 8x8 transposition of a register.
+// * A warp takes 16 keys at a time, keys as the rows of m16n8k16 products and the query heads of the KV head as their 8 columns (two such for
+//   groups of 9 to 16).  Each warp has a ring of its own of two stages, filled by TMA copies of 16 rows (swizzled, so that what the threads read
+//   of the values meets no conflict) and one of their scales; no warp waits for another.  Both contractions leave the order of their
+//   index free, so each thread reads 16 contiguous bytes: of the keys, features 16 c.. of rows lane / 4 (and 8 more), with q's fragments in
+//   the same order; of the values, 16 features of four keys, whose bytes it interleaves by pairs of keys.  The weights go from the first
+//   product's result to the second's operand by one 8x8 transposition of a register.
 // * Operands are float16, which an e4m3 number becomes in one instruction and without a rounding.  q is divided by a power of two that
 //   brings its largest magnitude below 2^15: of a bfloat16 number down to 2^-25 of that nothing is lost, and what is lost below is 2^-40 of it.
 //   A key's scale multiplies its score.
@@ -16,19 +17,28 @@
 //   scores'.  So they are numbers up to 2^8 (both maxima are followed when they grow by more than 2^8), rounded to float16 by 2^-12
 //   of themselves, and by 2^-25 of the largest where that is more: 2^-17 of a float16's distance from bfloat16, whatever the scales.  Sums are
 //   float32.
-// * Work: the keys of all (token, KV head) pairs, in units of 128 (a CTA's eight warps, 16 each), are one list; every CTA takes an equal,
-//   contiguous share of it, found from the tokens' positions alone, so that the lengths may differ as they like and a graph's replay needs
-//   nothing of the host.  A pair whose keys are one CTA's is finished by it; the others leave their sums in float32, at most two pieces
-//   to a CTA, for ``decode_fp8_join``.  No counters are shared between launches.
+// * Work, where there is much: the keys of all (token, KV head) pairs, in units of 128 (a CTA's eight warps, 16 each), are one list; every CTA
+//   takes an equal, contiguous share of it, found from the tokens' positions alone, so that the lengths may differ as they like and a
+//   graph's replay needs nothing of the host.  A pair whose keys are one CTA's is finished by it; the others leave their sums in float32, at
+//   most two pieces to a CTA, for ``decode_fp8_join``.  No counters are shared between launches.
+// * Where there is little, a pair is a cluster's, whose CTAs have equal shares of its units and join over their shared memories.
 #include "cache_fp8.cuh"
+#include "entry_points.h"
+#include "tc5_ops.cuh"
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
+
+namespace cg = cooperative_groups;
 
 #define DA_WARPS 8
 #define DA_THREADS (32 * DA_WARPS)
 #define DA_UNIT (16 * DA_WARPS)            // keys
-#define DA_TOKENS 1024                     // of a launch
+#define DA_STAGES 2                        // of a warp's ring
+#define DA_MAX_CLUSTER 16
+#define DA_TOKENS 1024                     // of a launch that deals its units out
 #define DA_GROW 8.0f                       // powers of two by which a maximum grows before it is followed
+#define DA_NONE (-1e30f)                   // the maximum of no scores (a difference to it is a number, as one to minus infinity is not)
 
 struct DaArgs {
   const bf16* q; long long ldq;
@@ -40,6 +50,9 @@ struct DaArgs {
   int T, H, gs, window, max_keys;
   float scale_log2e;
   float *part_o, *part_s;                  // [CTA][2][gs][d]; [CTA][2][gs][4]: sum, maximum of scores, of weights
+  int cluster;                             // CTAs to a pair; 0: units dealt out
+  int ps_shift;                            // log2 of a page's tokens, or -1
+  int* status;
 };
 
 __device__ __forceinline__ float da_exp2(float x) {
@@ -68,21 +81,14 @@ __device__ __forceinline__ unsigned da_transpose(unsigned v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
   return t;
 }
-// the cache is written by launches before: no read-only path
-__device__ __forceinline__ uint4 da_load16(const unsigned char* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
+// x: byte of a row, y: row of a page, z: page
+__device__ __forceinline__ void da_copy_rows(void* dst, const CUtensorMap* map, int y, int z, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(tc_smem(dst)), "l"(map), "r"(tc_smem(bar)), "r"(0), "r"(y), "r"(z) : "memory");
 }
-__device__ __forceinline__ uint2 da_load8(const unsigned char* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ unsigned da_load2(const unsigned char* p) {
-  unsigned short v;
-  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ void da_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(tc_smem(dst)), "l"(src), "r"(bytes), "r"(tc_smem(bar)) : "memory");
 }
 
 // The keys of a token: [lo, hi), and the units that hold them, from the 16 keys on in which lo lies
@@ -97,19 +103,50 @@ __device__ __forceinline__ int da_taking(long long U, int ctas) { return (int)(U
 __device__ __forceinline__ int da_first(long long U, int n, int i) { return (int)(U * i / n); }
 __device__ __forceinline__ int da_cta_of(long long U, int n, int unit) { return (int)((((long long)unit + 1) * n - 1) / U); }
 
-// units of the tokens before each token (and of all of them) to ``sums``, by the whole block
-__device__ __forceinline__ void da_sum_units(const DaArgs& a, int* sums, int* scratch) {
+// The list of all tokens' units.  Up to 32 tokens: in the registers of every warp, a lane to a token; more: in shared memory, made by the
+// whole block.
+struct DaList {
+  int few, T, before, units, pos;              // of this lane's token: units of those before it, its own, its position
+  const int *sums, *positions;
+  __device__ __forceinline__ int all() const { return few ? __shfl_sync(0xffffffffu, before + units, T - 1) : sums[T]; }
+  // the token that unit ``u`` of ``G`` times the list is of
+  __device__ __forceinline__ int token(int u, int G) const {
+    if (few) return __popc(__ballot_sync(0xffffffffu, (threadIdx.x & 31) < T && before * G <= u)) - 1;
+    int t = 0;
+    for (int step = DA_TOKENS / 2; step > 0; step >>= 1)
+      if (t + step < T && (long long)sums[t + step] * G <= u) t += step;
+    return t;
+  }
+  __device__ __forceinline__ int units_before(int t) const { return few ? __shfl_sync(0xffffffffu, before, t) : sums[t]; }
+  __device__ __forceinline__ int units_of(int t) const { return few ? __shfl_sync(0xffffffffu, units, t) : sums[t + 1] - sums[t]; }
+  __device__ __forceinline__ int position(int t) const { return few ? __shfl_sync(0xffffffffu, pos, t) : positions[t]; }
+};
+__device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = 0;
-  for (int t0 = 0; t0 < a.T; t0 += DA_THREADS) {
-    const int t = t0 + threadIdx.x;
-    const int u = t < a.T ? da_units(a, a.positions[t]) : 0;
-    int s = u;
+  auto scan = [&](int s) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += v;
     }
+    return s;
+  };
+  DaList list;
+  list.few = a.T <= 32;
+  list.T = a.T;
+  list.sums = sums;
+  list.positions = a.positions;
+  if (list.few) {
+    list.pos = lane < a.T ? a.positions[lane] : -1;
+    list.units = lane < a.T ? da_units(a, list.pos) : 0;
+    list.before = scan(list.units) - list.units;
+    return list;
+  }
+  int before = 0;
+  for (int t0 = 0; t0 < a.T; t0 += DA_THREADS) {
+    const int t = t0 + threadIdx.x;
+    const int u = t < a.T ? da_units(a, a.positions[t]) : 0;
+    const int s = scan(u);
     if (lane == 31) scratch[warp] = s;
     __syncthreads();
     int base = before, all = before;
@@ -124,38 +161,130 @@ __device__ __forceinline__ void da_sum_units(const DaArgs& a, int* sums, int* sc
   }
   if (threadIdx.x == 0) sums[a.T] = before;
   __syncthreads();
+  return list;
 }
 
-template <int HD, int NT>
-__global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel(const DaArgs a) {
+// What the sum of weighted values is multiplied by
+__device__ __forceinline__ float da_inverse(float sum, float mz, float mw) { return sum == 0.f ? 0.f : da_exp2(mw - mz) / sum; }
+
+// Sums of pieces of a pair together: of the exponentials (their sum and maximum), of the weighted values (and their maximum).
+struct DaJoin {
+  float sum, mz, mw;
+  float4 s;
+  __device__ __forceinline__ void none() { sum = 0.f; mz = mw = DA_NONE; s = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void add(float l, float m, float W, float4 v) {
+    const float z = fmaxf(mz, m), w = fmaxf(mw, W), a = da_exp2(mw - w), b = da_exp2(W - w);
+    sum = sum * da_exp2(mz - z) + l * da_exp2(m - z);
+    s.x = fmaf(v.x, b, s.x * a); s.y = fmaf(v.y, b, s.y * a); s.z = fmaf(v.z, b, s.z * a); s.w = fmaf(v.w, b, s.w * a);
+    mz = z;
+    mw = w;
+  }
+  __device__ __forceinline__ float inverse() const { return da_inverse(sum, mz, mw); }
+};
+__device__ __forceinline__ void da_store(bf16* to, float4 s, float inv) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(s.x * inv, s.y * inv), y = __floats2bfloat162_rn(s.z * inv, s.w * inv);
+  *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+}
+
+// a CTA's part of a pair's keys
+struct DaPiece {
+  int t, kvh, per, u0, n;                      // token, KV head, units of the pair, the first and how many
+  int pos, lo, base;                           // keys [lo, pos]; units from ``base`` on
+  const int* table;
+};
+__device__ __forceinline__ void da_piece_keys(const DaArgs& a, DaPiece& p, int pos) {
+  p.pos = min(pos, a.max_keys - 1);
+  p.lo = da_lo_key(a, p.pos);
+  p.base = p.lo & ~15;
+  p.table = a.table + (long long)min(max(a.token_req[p.t], 0), a.table_rows - 1) * a.max_blocks;
+}
+
+template <int HD, int NT, bool CLUSTER>
+__global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel(const __grid_constant__ CUtensorMap map, const DaArgs a) {
   constexpr int KB = HD / 64;                  // 16-byte pieces of a key's row to a thread
   constexpr int MT = HD / 16;                  // products of 16 features
   constexpr int VW = HD / 32;                  // words of a value's row to a thread
   constexpr int OG = HD / 8 + 4;               // of the sums in shared memory: a thread row's features, and four more against conflicts
-  __shared__ int sums[DA_TOKENS + 1], scratch[DA_WARPS];
-  __shared__ __align__(16) float o_s[DA_WARPS][8][8 * OG];
-  __shared__ float st_s[DA_WARPS][8 * NT][3], f_s[DA_WARPS][8 * NT], fin_s[8 * NT][3];
-  pdl_wait();
-  pdl_launch_dependents();                     // (after the wait: the join reads positions before its own)
+  constexpr int ROWS = 16 * HD, STAGE = 2 * ROWS;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  unsigned char* ring = smem_raw + ((1024 - (tc_smem(smem_raw) & 1023)) & 1023);           // [warp][stage][key, value][16][HD]
+  float* o_s = reinterpret_cast<float*>(ring + DA_WARPS * DA_STAGES * STAGE);              // [warp][8][8 OG]
+  __shared__ __align__(16) unsigned char scales_s[DA_WARPS][DA_STAGES][32];
+  __shared__ unsigned long long full[DA_WARPS][DA_STAGES];
+  __shared__ int sums[CLUSTER ? 1 : DA_TOKENS + 1], scratch[DA_WARPS], dead;
+  __shared__ float st_s[DA_WARPS][8 * NT][3], f_s[DA_WARPS][8 * NT], fin_s[8 * NT][4];
+  __shared__ __align__(16) float res_s[CLUSTER ? 8 * NT * HD : 4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int G = a.pages.G, ps = a.pages.ps;
-  da_sum_units(a, sums, scratch);
-  const long long U = (long long)sums[a.T] * G;
-  const int n = da_taking(U, gridDim.x);
-  if ((int)blockIdx.x >= n) return;
-  int unit = da_first(U, n, blockIdx.x);
-  const int end = da_first(U, n, blockIdx.x + 1);
-  for (int piece = 0; unit < end; piece++) {
-    // ---- the pair this unit belongs to, and how many of its units are this CTA's
-    int t = 0;
-    for (int step = DA_TOKENS / 2; step > 0; step >>= 1)
-      if (t + step < a.T && (long long)sums[t + step] * G <= unit) t += step;
-    const int per = sums[t + 1] - sums[t], of_token = unit - sums[t] * G, kvh = of_token / per, u0 = of_token - kvh * per;
-    const int n_units = min(per - u0, end - unit);
-    const int pos = min(a.positions[t], a.max_keys - 1), lo = da_lo_key(a, pos), base = lo & ~15;
-    const int req = a.token_req[t];
-    const int* table = a.table + (long long)min(max(req, 0), a.table_rows - 1) * a.max_blocks;
+  if (threadIdx.x == 0) dead = 0;
+  if (lane == 0) {
+    for (int s = 0; s < DA_STAGES; s++) tc_bar_init(&full[warp][s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch_dependents();                     // (after the wait: the join reads positions before its own)
 
+  // ---- this CTA's first piece
+  DaPiece p;
+  DaList list;
+  int unit = 0, end = 0;
+  if constexpr (CLUSTER) {
+    const int pair = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;
+    p.t = pair / G;
+    p.kvh = pair % G;
+    da_piece_keys(a, p, a.positions[p.t]);
+    p.per = da_units(a, p.pos);
+    p.u0 = p.per * rank / a.cluster;
+    p.n = p.per * (rank + 1) / a.cluster - p.u0;
+  } else {
+    list = da_list(a, sums, scratch);
+    const long long U = (long long)list.all() * G;
+    const int n = da_taking(U, gridDim.x);
+    if ((int)blockIdx.x >= n) return;
+    unit = da_first(U, n, blockIdx.x);
+    end = da_first(U, n, blockIdx.x + 1);
+  }
+  __syncthreads();                             // (``dead`` and the barriers are there)
+  auto piece_at = [&](int unit) {
+    DaPiece q;
+    q.t = list.token(unit, G);
+    q.per = list.units_of(q.t);
+    const int of_token = unit - list.units_before(q.t) * G;
+    q.kvh = of_token / q.per;
+    q.u0 = of_token - q.kvh * q.per;
+    q.n = min(q.per - q.u0, end - unit);
+    da_piece_keys(a, q, list.position(q.t));
+    return q;
+  };
+  if constexpr (!CLUSTER) p = piece_at(unit);
+  // this warp's 16 keys of unit u: base + 128 u + 16 warp ..
+  auto first_key = [&](const DaPiece& p, int u) { return p.base + u * DA_UNIT + 16 * warp; };
+  auto chunks_of = [&](const DaPiece& p) {
+    const int left = p.pos - first_key(p, p.u0);
+    return left < 0 ? 0 : min(p.n, left / DA_UNIT + 1);
+  };
+  int done = 0;                                // chunks that this warp has taken: the ring's turn
+  auto page_of = [&](const DaPiece& p, int i) {
+    const int key = first_key(p, p.u0 + i);
+    return p.table[a.ps_shift >= 0 ? key >> a.ps_shift : key / ps];
+  };
+  // chunk i of the piece into the stage of turn ``done + ahead``
+  auto request = [&](const DaPiece& p, int i, int ahead, int page) {
+    if (lane == 0) {
+      page = min(max(page, 0), a.n_pages - 1);
+      const int s = (done + ahead) % DA_STAGES, key = first_key(p, p.u0 + i), offset = a.ps_shift >= 0 ? key & (ps - 1) : key % ps;
+      unsigned char* to = ring + (warp * DA_STAGES + s) * STAGE;
+      unsigned long long* bar = &full[warp][s];
+      tc_expect_tx(bar, STAGE + 32);
+      da_copy_rows(to, &map, p.kvh * ps + offset, page, bar);
+      da_copy_rows(to + ROWS, &map, (G + p.kvh) * ps + offset, page, bar);
+      da_copy(scales_s[warp][s], c8_scale(a.pages, page, p.kvh, offset), 32, bar);
+    }
+  };
+  int chunks = chunks_of(p);
+  for (int i = 0; i < min(chunks, DA_STAGES); i++) request(p, i, i, page_of(p, i));
+
+  for (int piece = 0;; piece++) {
     // ---- q: columns of both halves of a product's k in the order of the keys' bytes; a thread's column is head g
     unsigned qf[NT][KB][4][2];
     float qs[NT][2];                           // of heads 2 c and 2 c + 1: what a score is multiplied by
@@ -167,7 +296,7 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
       for (int b = 0; b < KB; b++) {
         uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (h < a.gs) {
-          const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)t * a.ldq + (long long)(kvh * a.gs + h) * HD + 64 * b + 16 * c);
+          const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)p.t * a.ldq + (long long)(p.kvh * a.gs + h) * HD + 64 * b + 16 * c);
           w[0] = src[0]; w[1] = src[1];
         }
         const unsigned x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
@@ -202,101 +331,86 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
       for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) o[n][i][j] = 0.f;
-      m[n][0] = m[n][1] = W[n][0] = W[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = W[n][0] = W[n][1] = DA_NONE;
       l[n][0] = l[n][1] = 0.f;
     }
-    // this warp's 16 keys of unit u: base + 128 u + 16 warp ..; keys that are none read the token's first page
-    auto first_key = [&](int u) { return base + u * DA_UNIT + 16 * warp; };
-    auto page_of = [&](int key) {
-      const int p = key <= pos ? table[key / ps] : 0;
-      return min(max(p, 0), a.n_pages - 1);
-    };
-    uint4 kq[2][KB];
-    unsigned vq[4][VW], sc[2];
-    auto load_keys = [&](int page, int key) {
-      const unsigned char* row = c8_row(a.pages, page, 0, kvh, key % ps);
-#pragma unroll
-      for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int b = 0; b < KB; b++) kq[r][b] = da_load16(row + (g + 8 * r) * HD + 64 * b + 16 * c);
-      const unsigned char* scales = c8_scale(a.pages, page, kvh, key % ps);
-#pragma unroll
-      for (int r = 0; r < 2; r++) sc[r] = da_load2(scales + 2 * (g + 8 * r));
-    };
-    auto load_values = [&](int page, int key) {
-      const unsigned char* row = c8_row(a.pages, page, 1, kvh, key % ps);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const unsigned char* from = row + (2 * c + (j & 1) + 8 * (j >> 1)) * HD + HD / 8 * g;
-        if constexpr (HD == 128) {
-          const uint4 v = da_load16(from);
-          vq[j][0] = v.x; vq[j][1] = v.y; vq[j][2] = v.z; vq[j][3] = v.w;
-        } else {
-          const uint2 v = da_load8(from);
-          vq[j][0] = v.x; vq[j][1] = v.y;
-        }
-      }
-    };
-    const int last = u0 + n_units;
-    int page = 0;
-    if (first_key(u0) <= pos) {
-      page = page_of(first_key(u0));
-      load_keys(page, first_key(u0));
-      load_values(page, first_key(u0));
-    }
-    for (int u = u0; u < last && first_key(u) <= pos; u++) {
-      const int key0 = first_key(u), next = first_key(u + 1);
-      const bool more = u + 1 < last && next <= pos;
-      const int next_page = more ? page_of(next) : 0;
-      // ---- scores
-      float z[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; n++) z[n][0] = z[n][1] = z[n][2] = z[n][3] = 0.f;
+    int page_next = chunks > DA_STAGES ? page_of(p, DA_STAGES) : 0;
+    for (int i = 0; i < chunks; i++, done++) {
+      const int s = done % DA_STAGES, key0 = first_key(p, p.u0 + i);
+      if (!tc_wait(&full[warp][s], done / DA_STAGES & 1, &dead) && lane == 0) atomicCAS(a.status, 0, 1);
+      const unsigned char* ks = ring + (warp * DA_STAGES + s) * STAGE;
+      const unsigned char* vs = ks + ROWS;
+      // ---- scores, of the two halves of the features apart
+      float z[KB][NT][4];
 #pragma unroll
       for (int b = 0; b < KB; b++) {
-        const unsigned *k0 = &kq[0][b].x, *k1 = &kq[1][b].x;
+        uint4 kq[2];
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-          const unsigned a0 = da_lo(k0[s]), a1 = da_lo(k1[s]), a2 = da_hi(k0[s]), a3 = da_hi(k1[s]);
+        for (int r = 0; r < 2; r++) {
+          const int row = g + 8 * r, place = HD == 128 ? (4 * b + c) ^ g : c ^ (g >> 1 & 3);
+          kq[r] = *reinterpret_cast<const uint4*>(ks + row * HD + 16 * place);
+        }
+        const unsigned *k0 = &kq[0].x, *k1 = &kq[1].x;
 #pragma unroll
-          for (int n = 0; n < NT; n++) da_mma(z[n], a0, a1, a2, a3, qf[n][b][s][0], qf[n][b][s][1]);
+        for (int n = 0; n < NT; n++) z[b][n][0] = z[b][n][1] = z[b][n][2] = z[b][n][3] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const unsigned a0 = da_lo(k0[x]), a1 = da_lo(k1[x]), a2 = da_hi(k0[x]), a3 = da_hi(k1[x]);
+#pragma unroll
+          for (int n = 0; n < NT; n++) da_mma(z[b][n], a0, a1, a2, a3, qf[n][b][x][0], qf[n][b][x][1]);
         }
       }
+      const bool border = key0 < p.lo || key0 + 15 > p.pos;     // some of the keys may be seen by nobody
       float fk[2], ev[2];
-      bool seen[2];
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const int key = key0 + g + 8 * r;
-        seen[r] = key <= pos && key >= lo;
-        const unsigned bk = sc[r] & 255u, bv = sc[r] >> 8;
-        fk[r] = bv == 255u ? __uint_as_float(0x7fc00000u) : c8_power(bk);       // (a value without a number: its keys' weight is none either)
-        ev[r] = (float)((int)bv - 127);
+      {
+        const unsigned b0 = *reinterpret_cast<const unsigned short*>(scales_s[warp][s] + 2 * g);
+        const unsigned b1 = *reinterpret_cast<const unsigned short*>(scales_s[warp][s] + 2 * g + 16);
+        fk[0] = __uint_as_float(b0 << 23 & 0x7f800000u);        // (as c8_power but for the bytes 0 and 255)
+        fk[1] = __uint_as_float(b1 << 23 & 0x7f800000u);
+        ev[0] = (float)((int)(b0 >> 8) - 127);
+        ev[1] = (float)((int)(b1 >> 8) - 127);
+        const unsigned two = b0 | b1 << 16;                     // a byte of 0 or 255: (byte + 1) & 254 is 0
+        const unsigned odd = __vadd4(two, 0x01010101u) & 0xfefefefeu;
+        if (__any_sync(0xffffffffu, __vcmpeq4(odd, 0u))) {
+          fk[0] = b0 >> 8 == 255u ? c8_power(255u) : c8_power(b0 & 255u);      // (a value without a number: its key's weight is none either)
+          fk[1] = b1 >> 8 == 255u ? c8_power(255u) : c8_power(b1 & 255u);
+        }
       }
-      if (more) load_keys(next_page, next);
-      // ---- weights
-      float w[NT][4];
+      // ---- weights: scores, and with the values' exponents; d and w: above the references of their maxima
+      float d[NT][4], w[NT][4];
       bool grows = false;
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          z[n][i] = seen[i >> 1] ? z[n][i] * fk[i >> 1] * qs[n][i & 1] : -INFINITY;
-          w[n][i] = z[n][i] + ev[i >> 1];
-          grows |= z[n][i] > m[n][i & 1] + DA_GROW || w[n][i] > W[n][i & 1] + DA_GROW;
+        for (int j = 0; j < 4; j++) z[0][n][j] = (KB == 2 ? z[0][n][j] + z[KB - 1][n][j] : z[0][n][j]) * fk[j >> 1] * qs[n][j & 1];
+      if (border) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int key = key0 + g + 8 * (j >> 1);
+            if (key > p.pos || key < p.lo) z[0][n][j] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          d[n][j] = z[0][n][j] - m[n][j & 1];
+          w[n][j] = z[0][n][j] + ev[j >> 1] - W[n][j & 1];
+          grows |= fmaxf(d[n][j], w[n][j]) > DA_GROW;
         }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int j = 0; j < 2; j++) {
-            float mz = fmaxf(z[n][j], z[n][2 + j]), mw = fmaxf(w[n][j], w[n][2 + j]);
+            float mz = fmaxf(z[0][n][j], z[0][n][2 + j]), mw = fmaxf(z[0][n][j] + ev[0], z[0][n][2 + j] + ev[1]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
               mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, x));
               mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, x));
             }
-            mz = fmaxf(mz, m[n][j]);
-            mw = fmaxf(mw, W[n][j]);
             if (mz > m[n][j]) { l[n][j] *= da_exp2(m[n][j] - mz); m[n][j] = mz; }
             if (mw > W[n][j]) {
               const float f = da_exp2(W[n][j] - mw);
@@ -304,30 +418,51 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
 #pragma unroll
               for (int i = 0; i < MT; i++) { o[n][i][j] *= f; o[n][i][2 + j] *= f; }
             }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              d[n][2 * x + j] = z[0][n][2 * x + j] - m[n][j];
+              w[n][2 * x + j] = z[0][n][2 * x + j] + ev[x] - W[n][j];
+            }
           }
       }
       unsigned pb[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float p[4];
+        float q[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          // (no key seen yet: both maxima are minus infinity, and so is what they are taken from)
-          l[n][i & 1] += m[n][i & 1] == -INFINITY && !(z[n][i] != z[n][i]) ? 0.f : da_exp2(z[n][i] - m[n][i & 1]);
-          p[i] = W[n][i & 1] == -INFINITY && !(w[n][i] != w[n][i]) ? 0.f : da_exp2(w[n][i] - W[n][i & 1]);
+        for (int j = 0; j < 4; j++) {
+          l[n][j & 1] += da_exp2(d[n][j]);
+          q[j] = da_exp2(w[n][j]);
         }
-        pb[n][0] = da_transpose(da_pack(p[0], p[1]));
-        pb[n][1] = da_transpose(da_pack(p[2], p[3]));
+        pb[n][0] = da_transpose(da_pack(q[0], q[1]));
+        pb[n][1] = da_transpose(da_pack(q[2], q[3]));
       }
-      if (key0 < lo || key0 + 15 > pos) {      // values that nobody may see have the weight zero, and may be no numbers
+      // ---- values: of a pair of features, the bytes of two keys side by side
+      unsigned vq[4][VW];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int row = 2 * c + (j & 1) + 8 * (j >> 1);
+        if constexpr (HD == 128) {
+          const uint4 v = *reinterpret_cast<const uint4*>(vs + row * HD + 16 * (g ^ (row & 7)));
+          vq[j][0] = v.x; vq[j][1] = v.y; vq[j][2] = v.z; vq[j][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(vs + row * HD + 16 * ((g >> 1) ^ (row >> 1 & 3)) + 8 * (g & 1));
+          vq[j][0] = v.x; vq[j][1] = v.y;
+        }
+      }
+      __syncwarp();                            // the stage has been read
+      if (i + DA_STAGES < chunks) {
+        request(p, i + DA_STAGES, DA_STAGES, page_next);
+        if (i + DA_STAGES + 1 < chunks) page_next = page_of(p, i + DA_STAGES + 1);
+      }
+      if (border) {                            // values that nobody may see have the weight zero, and may be no numbers
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int key = key0 + 2 * c + (j & 1) + 8 * (j >> 1);
 #pragma unroll
-          for (int x = 0; x < VW; x++) vq[j][x] = key < lo || key > pos ? 0u : vq[j][x];
+          for (int x = 0; x < VW; x++) vq[j][x] = key < p.lo || key > p.pos ? 0u : vq[j][x];
         }
       }
-      // ---- values: of a pair of features, the bytes of two keys side by side
 #pragma unroll
       for (int x = 0; x < VW; x++)
 #pragma unroll
@@ -338,10 +473,20 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
 #pragma unroll
           for (int n = 0; n < NT; n++) da_mma(o[n][2 * x + y], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
-      if (more) load_values(next_page, next);
     }
 
-    // ---- the warps' sums together
+    // ---- the next piece's first keys are on their way while this one's sums come together
+    bool more = false;
+    DaPiece next = p;
+    if constexpr (!CLUSTER) {
+      unit += p.n;
+      more = unit < end;
+      if (more) {
+        next = piece_at(unit);
+        chunks = chunks_of(next);
+        for (int i = 0; i < min(chunks, DA_STAGES); i++) request(next, i, i, page_of(next, i));
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -353,24 +498,7 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
           s[0] = l[n][j]; s[1] = m[n][j]; s[2] = W[n][j];
         }
       }
-    __syncthreads();
-    if (threadIdx.x < 8 * NT) {
-      const int h = threadIdx.x;
-      float mz = -INFINITY, mw = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < DA_WARPS; w++) {
-        mz = fmaxf(mz, st_s[w][h][1]);
-        mw = fmaxf(mw, st_s[w][h][2]);
-      }
-#pragma unroll
-      for (int w = 0; w < DA_WARPS; w++) {
-        // (a warp without a key has sums of zero; one whose scores are no numbers has a sum that is none and no maximum)
-        sum += st_s[w][h][1] == -INFINITY ? st_s[w][h][0] : st_s[w][h][0] * da_exp2(st_s[w][h][1] - mz);
-        f_s[w][h] = st_s[w][h][2] == -INFINITY ? 1.f : da_exp2(st_s[w][h][2] - mw);
-      }
-      fin_s[h][0] = sum; fin_s[h][1] = mz; fin_s[h][2] = mw;
-    }
-    const bool whole = n_units == per;
+    const bool whole = p.n == p.per;
     const long long slot = 2ll * blockIdx.x + (piece ? 1 : 0);      // pieces between a CTA's first and last are whole
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -379,8 +507,28 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
       for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int i = 0; i < MT; i += 2)
-          *reinterpret_cast<float4*>(&o_s[warp][2 * c + j][g * OG + 2 * i]) = make_float4(o[n][i][j], o[n][i][2 + j], o[n][i + 1][j], o[n][i + 1][2 + j]);
+          *reinterpret_cast<float4*>(o_s + (warp * 8 + 2 * c + j) * (8 * OG) + g * OG + 2 * i) =
+              make_float4(o[n][i][j], o[n][i][2 + j], o[n][i + 1][j], o[n][i + 1][2 + j]);
       __syncthreads();
+      if (n == 0) {
+        if (threadIdx.x < 8 * NT) {
+          const int h = threadIdx.x;
+          float mz = DA_NONE, mw = DA_NONE, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < DA_WARPS; w++) {
+            mz = fmaxf(mz, st_s[w][h][1]);
+            mw = fmaxf(mw, st_s[w][h][2]);
+          }
+#pragma unroll
+          for (int w = 0; w < DA_WARPS; w++) {
+            // (a warp without a key has sums of zero; one whose scores are no numbers has a sum that is none)
+            sum += st_s[w][h][0] * da_exp2(st_s[w][h][1] - mz);
+            f_s[w][h] = da_exp2(st_s[w][h][2] - mw);
+          }
+          fin_s[h][0] = sum; fin_s[h][1] = mz; fin_s[h][2] = mw;
+        }
+        __syncthreads();
+      }
       for (int e = threadIdx.x; e < 8 * HD / 4; e += DA_THREADS) {
         const int h = e / (HD / 4), f = e % (HD / 4) * 4, head = 8 * n + h;
         if (head >= a.gs) continue;
@@ -388,80 +536,149 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < DA_WARPS; w++) {
-          const float4 v = *reinterpret_cast<const float4*>(&o_s[w][h][at]);
+          const float4 v = *reinterpret_cast<const float4*>(o_s + (w * 8 + h) * (8 * OG) + at);
           const float x = f_s[w][head];
           s.x = fmaf(v.x, x, s.x); s.y = fmaf(v.y, x, s.y); s.z = fmaf(v.z, x, s.z); s.w = fmaf(v.w, x, s.w);
         }
-        if (whole) {
-          const float sum = fin_s[head][0];
-          const float inv = sum == 0.f ? 0.f : da_exp2(fin_s[head][2] - fin_s[head][1]) / sum;
-          const __nv_bfloat162 x = __floats2bfloat162_rn(s.x * inv, s.y * inv), y = __floats2bfloat162_rn(s.z * inv, s.w * inv);
-          *reinterpret_cast<uint2*>(a.out + (long long)t * a.ldo + (long long)(kvh * a.gs + head) * HD + f) =
-              make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+        if (CLUSTER) {
+          *reinterpret_cast<float4*>(res_s + head * HD + f) = s;
+        } else if (whole) {
+          da_store(a.out + (long long)p.t * a.ldo + (long long)(p.kvh * a.gs + head) * HD + f, s, da_inverse(fin_s[head][0], fin_s[head][1], fin_s[head][2]));
         } else {
           *reinterpret_cast<float4*>(a.part_o + (slot * a.gs + head) * HD + f) = s;
           if (f == 0) *reinterpret_cast<float4*>(a.part_s + (slot * a.gs + head) * 4) = make_float4(fin_s[head][0], fin_s[head][1], fin_s[head][2], 0.f);
         }
       }
     }
+    if (!more) break;
     __syncthreads();                           // shared memory is the next piece's
-    unit += n_units;
+    p = next;
   }
+  if constexpr (CLUSTER) {
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    const int rank = (int)cl.block_rank();
+    for (int e = rank * DA_THREADS + threadIdx.x; e < a.gs * (HD / 4); e += a.cluster * DA_THREADS) {
+      const int head = e / (HD / 4), f = e % (HD / 4) * 4;
+      DaJoin j;
+      j.none();
+      for (int r = 0; r < a.cluster; r++) {
+        const float* st = cl.map_shared_rank(&fin_s[head][0], r);
+        j.add(st[0], st[1], st[2], *reinterpret_cast<const float4*>(cl.map_shared_rank(res_s + head * HD + f, r)));
+      }
+      da_store(a.out + (long long)p.t * a.ldo + (long long)(p.kvh * a.gs + head) * HD + f, j.s, j.inverse());
+    }
+    cl.sync();                                 // (nobody leaves whose shared memory is read)
+  }
+  if (dead)
+    for (int i = 0; i < 1000; i++) __nanosleep(1000);          // copies on their way land in what is still this CTA's
 }
 
-// The pieces of pairs that several CTAs of the launch before (of n_ctas) had: a block to a pair.
+// The pieces of pairs that several CTAs of the launch before (of n_ctas) had: a block to a head, its threads' groups with every so many'th piece
+// each.  (One token of 100,001 keys has 74 pieces to a pair: one after the other in a block to a pair they took 25 us.)
 template <int HD>
 __global__ void __launch_bounds__(DA_THREADS) decode_fp8_join_kernel(const DaArgs a, int n_ctas) {
+  constexpr int LANES = HD / 4, GROUPS = DA_THREADS / LANES;
   __shared__ int sums[DA_TOKENS + 1], scratch[DA_WARPS];
+  __shared__ DaJoin got[DA_THREADS];
   pdl_launch_dependents();
-  da_sum_units(a, sums, scratch);
-  const int t = blockIdx.x / a.pages.G, kvh = blockIdx.x % a.pages.G, per = sums[t + 1] - sums[t];
-  const long long U = (long long)sums[a.T] * a.pages.G;
+  const DaList list = da_list(a, sums, scratch);
+  const int pair = blockIdx.x / a.gs, h = blockIdx.x % a.gs, t = pair / a.pages.G, kvh = pair % a.pages.G, per = list.units_of(t);
+  const long long U = (long long)list.all() * a.pages.G;
   n_ctas = da_taking(U, n_ctas);
-  const int from = sums[t] * a.pages.G + kvh * per, c0 = da_cta_of(U, n_ctas, from), c1 = da_cta_of(U, n_ctas, from + per - 1);
+  const int from = list.units_before(t) * a.pages.G + kvh * per, c0 = da_cta_of(U, n_ctas, from), c1 = da_cta_of(U, n_ctas, from + per - 1);
   if (c0 == c1) return;
   pdl_wait();
-  for (int e = threadIdx.x; e < a.gs * (HD / 4); e += DA_THREADS) {
-    const int h = e / (HD / 4), f = e % (HD / 4) * 4;
-    float mz = -INFINITY, mw = -INFINITY, sum = 0.f;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int f = threadIdx.x % LANES * 4, group = threadIdx.x / LANES;
+  DaJoin j;
+  j.none();
 #pragma unroll 4
-    for (int i = c0; i <= c1; i++) {
-      const long long slot = 2ll * i + (da_first(U, n_ctas, i) < from ? 1 : 0);        // (the CTA's first piece, if it begins here)
-      const float4 st = __ldcg(reinterpret_cast<const float4*>(a.part_s + (slot * a.gs + h) * 4));
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot * a.gs + h) * HD + f));
-      if (st.y > mz) { sum *= da_exp2(mz - st.y); mz = st.y; }
-      sum += st.y == -INFINITY ? st.x : st.x * da_exp2(st.y - mz);
-      float x = 1.f;
-      if (st.z > mw) {
-        const float y = da_exp2(mw - st.z);
-        s.x *= y; s.y *= y; s.z *= y; s.w *= y;
-        mw = st.z;
-      } else if (st.z != -INFINITY) {
-        x = da_exp2(st.z - mw);
-      }
-      s.x = fmaf(v.x, x, s.x); s.y = fmaf(v.y, x, s.y); s.z = fmaf(v.z, x, s.z); s.w = fmaf(v.w, x, s.w);
-    }
-    const float inv = sum == 0.f ? 0.f : da_exp2(mw - mz) / sum;
-    const __nv_bfloat162 x = __floats2bfloat162_rn(s.x * inv, s.y * inv), y = __floats2bfloat162_rn(s.z * inv, s.w * inv);
-    *reinterpret_cast<uint2*>(a.out + (long long)t * a.ldo + (long long)(kvh * a.gs + h) * HD + f) =
-        make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+  for (int i = c0 + group; i <= c1; i += GROUPS) {
+    const long long slot = 2ll * i + (da_first(U, n_ctas, i) < from ? 1 : 0);          // (the CTA's first piece, if it begins here)
+    const float4 st = __ldcg(reinterpret_cast<const float4*>(a.part_s + (slot * a.gs + h) * 4));
+    j.add(st.x, st.y, st.z, __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot * a.gs + h) * HD + f)));
   }
+  got[threadIdx.x] = j;
+  __syncthreads();
+  if (group) return;
+  for (int i = 1; i < GROUPS && c0 + i <= c1; i++) {
+    const DaJoin& k = got[i * LANES + threadIdx.x];
+    j.add(k.sum, k.mz, k.mw, k.s);
+  }
+  da_store(a.out + (long long)t * a.ldo + (long long)(kvh * a.gs + h) * HD + f, j.s, j.inverse());
 }
 
-// CTAs of a launch over T tokens of up to max_keys keys: as many as run at a time, one to a unit at most
-static int da_ctas(int T, int G, int gs, int window, int max_keys, int sms) {
+static int* da_status_word() {
+  static int* words[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!words[dev]) {
+    int* w = nullptr;
+    if (cudaMalloc(&w, sizeof(int)) != cudaSuccess) return nullptr;
+    cudaMemset(w, 0, sizeof(int));
+    words[dev] = w;
+  }
+  return words[dev];
+}
+
+// How a launch over T tokens of up to max_keys keys is cut: CTAs, and how many of them are a pair's cluster (0: units are dealt out)
+struct DaPlan { int ctas, cluster; };
+static DaPlan da_plan(int T, int G, int gs, int window, int max_keys, int sms) {
   const long long keys = window > 0 && window < max_keys ? window + 15 : max_keys;
-  const long long units = (long long)T * G * ((keys + DA_UNIT - 1) / DA_UNIT);
-  const long long at_a_time = (long long)(gs > 8 ? 1 : 2) * sms;
-  return (int)(units < at_a_time ? units : at_a_time);
+  const long long per = (keys + DA_UNIT - 1) / DA_UNIT, pairs = (long long)T * G, at_a_time = (long long)(gs > 8 ? 1 : 2) * sms;
+  int n = 1;
+  while (n < DA_MAX_CLUSTER && n < per && 2 * n * pairs <= at_a_time) n *= 2;
+  if (n * pairs <= at_a_time && per <= 4 * n) return {(int)(n * pairs), n};
+  return {(int)(pairs * per < at_a_time ? pairs * per : at_a_time), 0};
 }
 
 // float32 numbers of scratch memory that a launch takes
 extern "C" long long qd_decode_attention_fp8_scratch(int T, int H, int G, int d, int window, int max_keys, int sms) {
   if (T < 1 || G < 1 || H < 1) return 0;
-  const int n = da_ctas(T < DA_TOKENS ? T : DA_TOKENS, G, H / G, window, max_keys, sms);
-  return 2ll * n * (H / G) * (d + 4);
+  const DaPlan plan = da_plan(T < DA_TOKENS ? T : DA_TOKENS, G, H / G, window, max_keys, sms);
+  return plan.cluster ? 0 : 2ll * plan.ctas * (H / G) * (d + 4);
+}
+
+template <int HD, int NT, bool CLUSTER>
+static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, cudaStream_t stream) {
+  const int smem = 1024 + DA_WARPS * (DA_STAGES * 32 * HD + 8 * 8 * (HD / 8 + 4) * 4);
+  auto kernel = decode_fp8_kernel<HD, NT, CLUSTER>;
+  static bool allowed[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QD_ERR_UNSUPPORTED;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        (CLUSTER && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+      cudaGetLastError();
+      return QD_ERR_UNSUPPORTED;
+    }
+    allowed[dev] = true;
+  }
+  if (!CLUSTER) {
+    qd_launch(kernel, dim3(ctas), dim3(DA_THREADS), smem, stream, map, a);
+    qd_launch(decode_fp8_join_kernel<HD>, dim3(a.T * a.H), dim3(DA_THREADS), 0, stream, a, ctas);
+    return qd_last_error();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(DA_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = qd_pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, map, a);
+  return qd_last_error();
+}
+template <int HD>
+static int da_launch_of(const CUtensorMap& map, const DaArgs& a, int ctas, cudaStream_t stream) {
+  if (a.cluster) return a.gs <= 8 ? da_launch<HD, 1, true>(map, a, ctas, stream) : da_launch<HD, 2, true>(map, a, ctas, stream);
+  return a.gs <= 8 ? da_launch<HD, 1, false>(map, a, ctas, stream) : da_launch<HD, 2, false>(map, a, ctas, stream);
 }
 
 // q, out: bfloat16 rows [T, H d], ``ldq`` and ``ldo`` apart; table [table_rows, max_blocks] of pages of ps tokens (a multiple of 16), its row of token t is
@@ -478,22 +695,29 @@ extern "C" int qd_decode_attention_fp8(const void* q, long long ldq, void* out, 
   const int gs = H / G;
   // the units of a launch fit 31 bits
   if ((long long)(T < DA_TOKENS ? T : DA_TOKENS) * G * (max_keys / DA_UNIT + 2) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
+  int* status = da_status_word();
+  CUtensorMap map;
+  if (!status || !c8_make_map(&map, pages, n_pages, G, ps, d)) return QD_ERR_UNSUPPORTED;
   for (int t = 0; t < T; t += DA_TOKENS) {
-    const int n = T - t < DA_TOKENS ? T - t : DA_TOKENS, ctas = da_ctas(n, G, gs, window, max_keys, sms);
-    DaArgs a = {(const bf16*)q + t * ldq, ldq, (bf16*)out + t * ldo, ldo, {(unsigned char*)pages, c8_page_bytes(G, ps, d), G, ps, d}, (int)n_pages,
-                table, max_blocks, table_rows, token_req + t, positions + t, n, H, gs, window, max_keys, scale * 1.4426950408889634f,
-                scratch, scratch + 2ll * ctas * gs * d};
-    if (d == 128) {
-      if (gs <= 8) qd_launch(decode_fp8_kernel<128, 1>, dim3(ctas), dim3(DA_THREADS), 0, stream, a);
-      else qd_launch(decode_fp8_kernel<128, 2>, dim3(ctas), dim3(DA_THREADS), 0, stream, a);
-    } else {
-      if (gs <= 8) qd_launch(decode_fp8_kernel<64, 1>, dim3(ctas), dim3(DA_THREADS), 0, stream, a);
-      else qd_launch(decode_fp8_kernel<64, 2>, dim3(ctas), dim3(DA_THREADS), 0, stream, a);
-    }
-    if (max_keys > 1) {
-      if (d == 128) qd_launch(decode_fp8_join_kernel<128>, dim3(n * G), dim3(DA_THREADS), 0, stream, a, ctas);
-      else qd_launch(decode_fp8_join_kernel<64>, dim3(n * G), dim3(DA_THREADS), 0, stream, a, ctas);
-    }
+    const int n = T - t < DA_TOKENS ? T - t : DA_TOKENS;
+    const DaPlan plan = da_plan(n, G, gs, window, max_keys, sms);
+    const DaArgs a = {(const bf16*)q + t * ldq, ldq, (bf16*)out + t * ldo, ldo, {(unsigned char*)pages, c8_page_bytes(G, ps, d), G, ps, d}, (int)n_pages,
+                      table, max_blocks, table_rows, token_req + t, positions + t, n, H, gs, window, max_keys, scale * 1.4426950408889634f,
+                      scratch, scratch + 2ll * plan.ctas * gs * d, plan.cluster, ps & (ps - 1) ? -1 : __builtin_ctz(ps), status};
+    const int rc = d == 128 ? da_launch_of<128>(map, a, plan.ctas, stream) : da_launch_of<64>(map, a, plan.ctas, stream);
+    if (rc) return rc;
   }
-  return qd_last_error();
+  return 0;
+}
+
+QD_DEFINE_WAIT_PROBE(qd_decode_attention_fp8_wait_probe, tc_wait(bar, 0, dead, 0, poll_limit), da_status_word, 99)
+
+// 0 if no kernel of this library has recorded a wait that ran out on the current device.  Synchronises.
+extern "C" int qd_decode_attention_fp8_status() {
+  int* status = da_status_word();
+  if (!status) return -1;
+  int v = 0;
+  if (cudaMemcpy(&v, status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
+  if (v) cudaMemset(status, 0, sizeof(int));
+  return v;
 }

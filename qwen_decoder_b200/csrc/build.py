@@ -78,8 +78,8 @@ EXTRA_DEPS: Dict[str, List[str]] = {
     "gemm_fp8": ["tc5_ops.cuh", "fp8.cuh"],
     "gemm_fp8_few": ["fp8.cuh"],
     "rows_fp8": ["fp8.cuh"],
-    "cache_fp8": ["fp8.cuh", "cache_fp8.cuh"],
-    "attention_fp8_decode": ["fp8.cuh", "cache_fp8.cuh"],
+    "cache_fp8": ["fp8.cuh", "cache_fp8.cuh", "tc5_ops.cuh"],
+    "attention_fp8_decode": ["fp8.cuh", "cache_fp8.cuh", "tc5_ops.cuh"],
     "gated_block": ["short_conv.cuh"],
     "attention_diff": ["short_conv.cuh", "mma_sync.cuh"],
     "qkv_prep": ["short_conv.cuh"],

@@ -4,6 +4,7 @@
 // A key or value with an infinity or a NaN has the scale 255 ("no number"), and whoever sees it gets none.
 #pragma once
 #include "fp8.cuh"
+#include "tc5_ops.cuh"
 
 __host__ __device__ __forceinline__ long long c8_page_bytes(int G, int ps, int d) { return (long long)G * ps * (2 * d + 2); }
 
@@ -23,4 +24,17 @@ __device__ __forceinline__ unsigned char* c8_scale(const C8Pages& p, long long p
 // 2^(byte - 127) as float32: byte 0 is 2^-127, no normal number; 255 no number
 __device__ __forceinline__ float c8_power(unsigned byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+// Pages as rows of d bytes, [n_pages][2 G ps] of them (the scales behind a page's rows are no part of it), by boxes of 16 rows, swizzled by as
+// many bytes as a row has
+static bool c8_make_map(CUtensorMap* map, const void* pages, long long n_pages, int G, int ps, int d) {
+  TcEncodeFn fn = tc_encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)2 * G * ps, (cuuint64_t)n_pages};
+  cuuint64_t strides[2] = {(cuuint64_t)d, (cuuint64_t)c8_page_bytes(G, ps, d)};
+  cuuint32_t box[3] = {(cuuint32_t)d, 16, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pages), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

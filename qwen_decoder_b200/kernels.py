@@ -903,6 +903,7 @@ _STATUS = {"gemm_stream": ("qd_gemm_stream_status", "qd_gemm_stream_wait_probe")
            "gemm_fp8": ("qd_gemm_fp8_status", "qd_gemm_fp8_wait_probe"),
            "gemm_f32": ("qd_gemm_f32_status", "qd_gemm_f32_wait_probe"),
            "attention_tc5": ("qd_prefill_attention_tc5_status", "qd_prefill_attention_tc5_wait_probe"),
+           "attention_fp8_decode": ("qd_decode_attention_fp8_status", "qd_decode_attention_fp8_wait_probe"),
            "attention_fp8_chunk": ("qd_prefill_attention_fp8_status", "qd_prefill_attention_fp8_wait_probe"),
            "attention_flash": ("qd_decode_attention_tma_status", "qd_decode_attention_tma_wait_probe")}
 
