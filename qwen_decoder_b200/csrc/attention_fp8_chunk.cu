@@ -18,7 +18,8 @@
 //   twice the instructions: 2,048 tokens behind 6,144 420 us.)  These warps also bring the keys' scales to tensor memory.
 // * A key or value that is no number has the scale 255.  The value becomes zeros, its key's scale 255, so that the score is none and
 //   every row that sees it, and no other, is none.  Values behind the last row's position, which may be anything, become zeros.
-// * Few tiles of rows (a short portion behind a long history) share their keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
+// * Tiles of rows that would leave multiprocessors without work (a short portion behind a long history, the last round of a long one) share their
+//   keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
 //
 // Warps: 0..7 softmax (two threads to a row: halves of the keys and of the columns), 8 and 9 copies of keys and values, 10 MMAs, 11 scales,
 // 12..15 values.
@@ -39,6 +40,7 @@
 #define AC_ROWS 128
 #define AC_KEYS 128
 #define AC_GROW 7.0f                   // powers of two by which a row's maximum grows before it is followed
+#define AC_IDLE 60                     // nanoseconds between two looks of a warp that is ahead, which the others' issue slots are better for
 #define AC_TOP 8.0f                    // log2 of what stands for the maximum: below 2^15 in all, within float16
 #define AC_WIDE 256u                   // beside a tile's largest scale: values and weights in bfloat16
 #define AC_HOLES 512u                  // and: some of the values are nobody's or no numbers
@@ -56,11 +58,33 @@ struct AcParams {
   const unsigned char* pages; long long page_bytes; int n_pages;
   const int* table; int max_blocks;
   const int *cu, *start;
-  int R, H, G, ps, ps_shift, window, tok_tile, rows;      // ps_shift: log2 of ps, or -1
+  int R, H, G, ps, ps_shift, window, tok_tile;      // ps_shift: log2 of ps, or -1
   float scale_log2e;
-  float *part_o, *part_s;              // [share][rows][H][HD]; [share][rows][H][2]: maximum, sum
+  // Pairs of a tile of rows and a KV head, the longest first; the ones before ``whole`` are a CTA's each, those behind it ``shares`` CTAs', which
+  // leave their sums: [pair][share][128][HD], [pair][share][128][2]: reference, sum of weights
+  int tiles, whole, shares;
+  float *part_o, *part_s;
   int* status;
 };
+
+// A pair's rows: which request, which of its tokens (tiles numbered request by request)
+struct AcRows { int r, tok0, n_tok, pos0; };
+__device__ __forceinline__ AcRows ac_rows(const AcParams& p, const int* cu, const int* sp, int pair) {
+  const int b = p.tiles - 1 - pair / p.G;
+  AcRows a = {0, 0, 0, 0};
+  int before = 0;
+  for (; a.r < p.R; a.r++) {
+    const int nt = (cu[a.r + 1] - cu[a.r] + p.tok_tile - 1) / p.tok_tile;
+    if (b < before + nt) break;
+    before += nt;
+  }
+  if (a.r < p.R) {                     // (else: no rows)
+    a.tok0 = cu[a.r] + (b - before) * p.tok_tile;
+    a.n_tok = min(p.tok_tile, cu[a.r + 1] - a.tok0);
+    a.pos0 = sp[a.r] + (a.tok0 - cu[a.r]);
+  }
+  return a;
+}
 
 __device__ __forceinline__ int ac_key_lo(const AcParams& p, int pos) { return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0; }
 // x: byte of a row, y: row of a page, z: page
@@ -78,6 +102,13 @@ __device__ __forceinline__ void ac_mma_scaled(unsigned d, unsigned a, unsigned d
 }
 __device__ __forceinline__ void ac_st4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// whether the phase with this parity has completed, by one look
+__device__ __forceinline__ bool ac_done(unsigned long long* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok) : "r"(tc_smem(bar)), "r"(parity) : "memory");
+  return ok;
 }
 __device__ __forceinline__ unsigned ac_halves(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -152,28 +183,17 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   tc_fence_after();
   const unsigned tmem = tmem_slot;
 
-  // ---- which request and which tokens (tiles numbered request by request, the longest histories first)
-  const int g = blockIdx.y, gs = p.H / p.G;
-  const int* cu = staged ? cu_s : p.cu;
-  const int* sp = staged ? sp_s : p.start;
-  const int b = gridDim.x - 1 - blockIdx.x;
-  int r = 0, before = 0;
-  for (; r < p.R; r++) {
-    const int nt = (cu[r + 1] - cu[r] + p.tok_tile - 1) / p.tok_tile;
-    if (b < before + nt) break;
-    before += nt;
-  }
-  const bool idle = r == p.R;
-  int tok0 = 0, n_tok = 0, pos0 = 0;
-  if (!idle) {
-    tok0 = cu[r] + (b - before) * p.tok_tile;
-    n_tok = min(p.tok_tile, cu[r + 1] - tok0);
-    pos0 = sp[r] + (tok0 - cu[r]);
-  }
+  // ---- which rows, and which share of their keys
+  const int behind = (int)blockIdx.x - p.whole, pair = behind < 0 ? blockIdx.x : p.whole + behind / p.shares, share = behind < 0 ? 0 : behind % p.shares;
+  const int shares = behind < 0 ? 1 : p.shares;
+  const int g = pair % p.G, gs = p.H / p.G;
+  const AcRows rows = ac_rows(p, staged ? cu_s : p.cu, staged ? sp_s : p.start, pair);
+  const bool idle = rows.r == p.R;
+  const int r = rows.r, tok0 = rows.tok0, n_tok = rows.n_tok, pos0 = rows.pos0;
   const int key_hi = pos0 + n_tok, key_lo = ac_key_lo(p, pos0);
   // of the tiles from the first row's first key to the last row's last, this share's
   const int t0 = key_lo / AC_KEYS, tn = idle ? 0 : (key_hi + AC_KEYS - 1) / AC_KEYS - t0;
-  const int kt_lo = t0 + (int)((long long)tn * blockIdx.z / gridDim.z), n_kt = t0 + (int)((long long)tn * (blockIdx.z + 1) / gridDim.z) - kt_lo;
+  const int kt_lo = t0 + (int)((long long)tn * share / shares), n_kt = t0 + (int)((long long)tn * (share + 1) / shares) - kt_lo;
   const int* table = p.table + (long long)(idle ? 0 : r) * p.max_blocks;
   // of a key: its page's entry in the table, for whoever needs it a tile later (keys that are none: any page will do); the page; the place in it
   auto entry_at = [&](int key) {
@@ -244,9 +264,10 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
     }
     float m = -INFINITY, l = 0.f;        // m: the maximum that this row's exponentials, sum and output refer to
     const int free_hi = pos0 + 1, free_lo = ac_key_lo(p, key_hi - 1);       // keys that every row sees need no test
+    bool ready = false;                  // the next tile's scores are there: looked at ahead, since the answer takes 200 to 300 cycles
     for (int j = 0; j < n_kt; j++) {
       const int tile_base = (kt_lo + j) * AC_KEYS, key_base = tile_base + h * KQ;
-      if (!tc_wait_inline(&s_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 7);
+      if (!ready && !tc_wait_inline(&s_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 7);
       __syncwarp();                                  // (here and below: what follows is the whole warp's instruction)
       tc_fence_after();
       float sv[KQ];
@@ -261,7 +282,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       }
       float mx4[4] = {sv[0], sv[1], sv[2], sv[3]};   // (one chain of 64 would be four cycles each)
 #pragma unroll
-      for (int i = 4; i < KQ; i++) mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
+      for (int i = 4; i < KQ; i += 2) mx4[i / 2 & 3] = fmaxf(fmaxf(mx4[i / 2 & 3], sv[i]), sv[i + 1]);
       const float mul = interior ? p.scale_log2e : 1.0f;
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
       mx_s[j & 1][h][row] = mx;
@@ -288,6 +309,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           }
         }
       };
+      ready = __all_sync(0xffffffffu, ac_done(&s_full[j & 1 ^ 1], (j + 1) >> 1 & 1));
       // Weights first, against the reference as it is; the other thread's maximum then seldom says that it has to move (the first tile's always).
       if (j > 0) weigh();
       asm volatile("bar.sync %0, 64;" ::"r"(3 + (warp & 3)) : "memory");       // the two warps of these rows
@@ -316,8 +338,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         weigh();
       }
       l = fmaf(sum, __uint_as_float((254u - (tile & 255u)) << 23), l);
-      // over the first half of this tile's own scores, which every thread of the row has in registers since the barrier above
-      at_tmem_st<KQ / 2>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * (KQ / 2), pk);
+      at_tmem_st<KQ / 2>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * KQ, pk);      // over the first half of this thread's own scores
       tc_fence_before();
       __syncwarp();
       if (lane == 0) tc_arrive(&p_full[j & 1]);
@@ -330,8 +351,8 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
     l_s[h][row] = l;
     asm volatile("bar.sync 1, %0;" ::"n"(AC_SOFTMAX) : "memory");
     const float l_all = l + l_s[h ^ 1][row];
-    if (gridDim.z > 1) {
-      const long long at = ((long long)blockIdx.z * p.rows + tok0 + t) * p.H + g * gs + hh;
+    if (shares > 1) {
+      const long long at = (long long)behind * AC_ROWS + row;
       if (ok && h == 0) *reinterpret_cast<float2*>(p.part_s + 2 * at) = make_float2(m, l_all);
       if (n_kt > 0) {
 #pragma unroll
@@ -375,7 +396,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
     constexpr int STEPS = AC_KEYS / 8 / 4 * (HD / 64);       // of a warp: 8 rows each, four groups of rows apart, one block of features after the other
     for (int i = -2; i < n_kt; i++) {
       const int s = (i + 2) % NS, j = i + 2;
-      if (!tc_wait_inline(&empty[s], ((i + 2) / NS & 1) ^ 1, &dead) && lane == 0) atomicCAS(p.status, 0, 5);
+      if (!tc_wait_inline(&empty[s], ((i + 2) / NS & 1) ^ 1, &dead, AC_IDLE) && lane == 0) atomicCAS(p.status, 0, 5);
       if (!tc_wait_inline(&v8_full[s], (i + 2) / NS & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 6);
       __syncwarp();
       tc_fence_after();
@@ -448,7 +469,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         const int s = u % NS, j = which ? u - 2 : u;
         const bool have = j >= 0 && j < n_kt;
         unsigned long long* bar = which ? &v8_full[s] : &full[s];
-        if (!tc_wait_inline(which ? &v8_empty[s] : &empty[s], (u / NS & 1) ^ 1, &dead)) {
+        if (!tc_wait_inline(which ? &v8_empty[s] : &empty[s], (u / NS & 1) ^ 1, &dead, AC_IDLE)) {
           if (lane == 0) atomicCAS(p.status, 0, 1);
           break;                                      // (nobody waits any more, and no more copies are to arrive)
         }
@@ -480,7 +501,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       unsigned largest = 0;                           // of the values' scales so far
       for (int u = 0; u < n_kt + 2; u++) {
         const int s = u % NS;
-        if (!tc_wait_inline(&v8_empty[s], (u / NS & 1) ^ 1, &dead) && lane == 0) atomicCAS(p.status, 0, 11);
+        if (!tc_wait_inline(&v8_empty[s], (u / NS & 1) ^ 1, &dead, AC_IDLE) && lane == 0) atomicCAS(p.status, 0, 11);
         __syncwarp();
         if (u < n_kt) {
           const uint2 now = sc;
@@ -553,14 +574,15 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         }
         for (int j = 0; j < n_kt; j++) {
           const int s = (j + 2) % NS;
-          if (!tc_wait_inline(&p_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 4);
           slot_ready(j);
+          if (!tc_wait_inline(&p_full[j & 1], (j >> 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 4);
+          __syncwarp();
           tc_fence_after();
           const unsigned v_lo = v_lo0 + (unsigned)s * (TILE16 >> 4), idesc_pv = idesc_f16 | (tile_s[j % AC_AHEAD] & AC_WIDE ? 1u << 7 | 1u << 10 : 0u);
           if (one) {
 #pragma unroll
             for (int k = 0; k < AC_KEYS / 16; k++)
-              at_umma_ta(tmem + T_O, tmem + (unsigned)(j & 1) * AC_KEYS + (unsigned)k * 8, v_lo + (unsigned)k * (2048 >> 4), AT_DESC_HI, idesc_pv,
+              at_umma_ta(tmem + T_O, tmem + (unsigned)(j & 1) * AC_KEYS + (unsigned)(k + (k & 4)) * 8, v_lo + (unsigned)k * (2048 >> 4), AT_DESC_HI, idesc_pv,
                          (j > 0 || k > 0) ? 1u : 0u);
             tc_commit(j + 1 < n_kt ? &o_done : &o_last);
             if (j + 2 < n_kt) scores(j + 2);
@@ -585,31 +607,32 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   }
 }
 
-// The shares of every row together: a thread takes four features of a head.
+// The shares of the pairs behind ``whole``: a block to one's four rows, a thread to four features of one.
+#define AC_JOIN_ROWS 4
 template <int HD>
-__global__ void __launch_bounds__(256) chunk_fp8_join_kernel(const AcParams p, int shares) {
+__global__ void __launch_bounds__(AC_JOIN_ROWS * HD / 4) chunk_fp8_join_kernel(const AcParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int f = (int)(i % (HD / 4)) * 4;
-  const long long at = i / (HD / 4), per = (long long)p.rows * p.H;
-  if (at >= per) return;
-  const int row = (int)(at / p.H), head = (int)(at % p.H);
-  if (row < p.cu[0] || row >= p.cu[p.R]) return;
+  const int behind = blockIdx.x / (AC_ROWS / AC_JOIN_ROWS), pair = p.whole + behind, g = pair % p.G, gs = p.H / p.G;
+  const int row = blockIdx.x % (AC_ROWS / AC_JOIN_ROWS) * AC_JOIN_ROWS + threadIdx.x / (HD / 4), f = threadIdx.x % (HD / 4) * 4;
+  const AcRows rows = ac_rows(p, p.cu, p.start, pair);
+  const int t = row / gs, hh = row - t * gs;
+  if (rows.r == p.R || t >= rows.n_tok) return;
+  const long long first = (long long)behind * p.shares * AC_ROWS + row;
   float m = -INFINITY, l = 0.f;
-  for (int s = 0; s < shares; s++) m = fmaxf(m, __ldcg(p.part_s + 2 * (s * per + at)));
+  for (int s = 0; s < p.shares; s++) m = fmaxf(m, __ldcg(p.part_s + 2 * (first + s * AC_ROWS)));
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int s = 0; s < shares; s++) {
-    const float2 st = __ldcg(reinterpret_cast<const float2*>(p.part_s + 2 * (s * per + at)));
+  for (int s = 0; s < p.shares; s++) {
+    const float2 st = __ldcg(reinterpret_cast<const float2*>(p.part_s + 2 * (first + s * AC_ROWS)));
     if (st.x == -INFINITY) { l += st.y; continue; }           // (no key, whose sums were not written, or no numbers)
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * per + at) * HD + f));
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (first + s * AC_ROWS) * HD + f));
     const float x = at_exp2(st.x - m);
     l = fmaf(st.y, x, l);
     o.x = fmaf(v.x, x, o.x); o.y = fmaf(v.y, x, o.y); o.z = fmaf(v.z, x, o.z); o.w = fmaf(v.w, x, o.w);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + row * p.ldo + (long long)head * HD + f) = make_uint2(at_pack(o.x * inv, o.y * inv), at_pack(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(p.out + (rows.tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + f) = make_uint2(at_pack(o.x * inv, o.y * inv), at_pack(o.z * inv, o.w * inv));
 }
 
 // ------------------------------------------------------------------------------------ host
@@ -626,25 +649,36 @@ static int* ac_status_word() {
   return words[dev];
 }
 
-// Shares of the keys: as many as fill the multiprocessors, and none of fewer than four tiles
-static int ac_shares(int T, int R, int H, int G, int window, int max_keys, int sms) {
+// How a launch is cut: pairs in all, those that are a CTA's each, the shares of the others
+struct AcPlan { long long tiles, whole; int shares; };
+// A CTA holds a multiprocessor.  What does not fill one round of them is shared out: all pairs where there are few, else those of the last
+// round (the shortest), by as many shares as make its time least: rounds of them over their number, each with AC_SHARE tiles of its own on top for
+// what a CTA costs besides its keys.
+#define AC_SHARE 4
+static AcPlan ac_plan(int T, int R, int H, int G, int window, int max_keys, int sms) {
   const int tok_tile = AC_ROWS / (H / G);
-  const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0);
+  const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0), pairs = tiles * G;       // (of R requests at most)
   const long long keys = window > 0 && window + tok_tile < max_keys ? window + tok_tile : max_keys;
-  const long long by_fill = sms / (tiles * G), by_work = keys / (4 * AC_KEYS);
-  const long long n = by_fill < by_work ? by_fill : by_work;
-  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  const double length = (double)keys / AC_KEYS;
+  const long long rest = pairs % sms;
+  AcPlan plan = {tiles, pairs, 1};
+  double best = length + AC_SHARE;
+  for (int s = 2; s <= 64 && rest && s * 4 <= length; s++) {
+    const double time = (double)((rest * s + sms - 1) / sms) * (length / s + AC_SHARE) + 2;             // (2: the launch that joins)
+    if (time < best) { best = time; plan.shares = s; plan.whole = pairs - rest; }
+  }
+  return plan;
 }
 
-// float32 numbers of scratch memory that a launch over ``rows`` rows of q takes
-extern "C" long long qd_prefill_attention_fp8_scratch(int rows, int T, int R, int H, int G, int d, int window, int max_keys, int sms) {
+// float32 numbers of scratch memory that a launch takes
+extern "C" long long qd_prefill_attention_fp8_scratch(int T, int R, int H, int G, int d, int window, int max_keys, int sms) {
   if (T < 1 || R < 1 || G < 1 || H < G) return 0;
-  const int n = ac_shares(T, R, H, G, window, max_keys, sms);
-  return n > 1 ? (long long)n * rows * H * (d + 2) : 0;
+  const AcPlan plan = ac_plan(T, R, H, G, window, max_keys, sms);
+  return (plan.tiles * G - plan.whole) * plan.shares * AC_ROWS * (d + 2);
 }
 
 template <int HD>
-static int ac_launch(const CUtensorMap& map, const AcParams& p, int tiles, int shares, cudaStream_t stream) {
+static int ac_launch(const CUtensorMap& map, const AcParams& p, cudaStream_t stream) {
   const size_t smem = 1024 + (size_t)AC_STAGES * 4 * AC_KEYS * HD;
   static bool allowed[64];
   int dev = 0;
@@ -658,11 +692,9 @@ static int ac_launch(const CUtensorMap& map, const AcParams& p, int tiles, int s
     }
     allowed[dev] = true;
   }
-  qd_launch(chunk_fp8_kernel<HD>, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)shares), dim3(AC_THREADS), smem, stream, map, p);
-  if (shares > 1) {
-    const long long threads = (long long)p.rows * p.H * (HD / 4);
-    qd_launch(chunk_fp8_join_kernel<HD>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p, shares);
-  }
+  const unsigned behind = (unsigned)(p.tiles * p.G - p.whole);
+  qd_launch(chunk_fp8_kernel<HD>, dim3(p.whole + behind * p.shares), dim3(AC_THREADS), smem, stream, map, p);
+  if (behind) qd_launch(chunk_fp8_join_kernel<HD>, dim3(behind * (AC_ROWS / AC_JOIN_ROWS)), dim3(AC_JOIN_ROWS * HD / 4), 0, stream, p);
   return qd_last_error();
 }
 
@@ -680,12 +712,13 @@ extern "C" int qd_prefill_attention_fp8(const void* q, long long ldq, void* out,
   int* status = ac_status_word();
   CUtensorMap map;
   if (!status || !c8_make_map(&map, pages, n_pages, G, ps, d)) return QD_ERR_UNSUPPORTED;
-  const int shares = ac_shares(T, R, H, G, window, max_keys, sms), tok_tile = AC_ROWS / (H / G);
-  AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, c8_page_bytes(G, ps, d), (int)n_pages, table, max_blocks, cu, start, R, H, G, ps,
-                ps & (ps - 1) ? -1 : __builtin_ctz(ps), window, tok_tile, rows, scale * 1.4426950408889634f, scratch, scratch + (long long)shares * rows * H * d, status};
-  const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0);      // of R requests at most
-  if (tiles > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
-  return d == 64 ? ac_launch<64>(map, p, (int)tiles, shares, stream) : ac_launch<128>(map, p, (int)tiles, shares, stream);
+  const AcPlan plan = ac_plan(T, R, H, G, window, max_keys, sms);
+  const long long behind = plan.tiles * G - plan.whole, ctas = plan.whole + behind * plan.shares;
+  if (ctas > 0x7fffffffll || behind * (AC_ROWS / AC_JOIN_ROWS) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
+  const AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, c8_page_bytes(G, ps, d), (int)n_pages, table, max_blocks, cu,
+                      start, R, H, G, ps, ps & (ps - 1) ? -1 : __builtin_ctz(ps), window, AC_ROWS / (H / G), scale * 1.4426950408889634f,
+                      (int)plan.tiles, (int)plan.whole, plan.shares, scratch, scratch + behind * plan.shares * AC_ROWS * d, status};
+  return d == 64 ? ac_launch<64>(map, p, stream) : ac_launch<128>(map, p, stream);
 }
 
 QD_DEFINE_WAIT_PROBE(qd_prefill_attention_fp8_wait_probe, tc_wait(bar, 0, dead, 0, poll_limit), ac_status_word, 99)

@@ -518,7 +518,7 @@ CALL(prefill_attention_fp8, 14)
   if (T == 0 || R == 0) Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   const int sms = multiprocessors(device);
-  const int64_t floats = entry(g_prefill_scratch, "attention_fp8_chunk", "qd_prefill_attention_fp8_scratch")((int)rows, (int)T, (int)R, h.H, h.G, h.d, window,
+  const int64_t floats = entry(g_prefill_scratch, "attention_fp8_chunk", "qd_prefill_attention_fp8_scratch")((int)T, (int)R, h.H, h.G, h.d, window,
                                                                                                          (int)max_keys, sms);
   const at::Tensor scratch = at::empty_strided({floats}, {1}, q.options().dtype(at::kFloat));
   done(entry(g_prefill, "attention_fp8_chunk", "qd_prefill_attention_fp8")(address(q), q.stride(0), address(out), out.stride(0), pages_at, n_pages,

@@ -2201,7 +2201,7 @@ def prompt_cache8(R: int, T: int, n_decode: int, H: int, G: int, d: int, window:
     dec.qd_decode_attention_fp8_scratch.restype = pre.qd_prefill_attention_fp8_scratch.restype = _LL
     sms = sm_count()
     floats = max(dec.qd_decode_attention_fp8_scratch(n_decode, H, G, d, window, decode_keys, sms) if n_decode else 0,
-                 pre.qd_prefill_attention_fp8_scratch(T, T - n_decode, R - n_decode, H, G, d, window, prefill_keys, sms))
+                 pre.qd_prefill_attention_fp8_scratch(T - n_decode, R - n_decode, H, G, d, window, prefill_keys, sms))
     c = PromptCache8(addr(library("cache_fp8").qd_rope_kv_write_fp8), addr(dec.qd_decode_attention_fp8), addr(pre.qd_prefill_attention_fp8))
     c.table_rows, c.decode_keys, c.prefill_keys = R, decode_keys, prefill_keys
     return c, floats
