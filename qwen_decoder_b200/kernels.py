@@ -849,8 +849,8 @@ def sample_nucleus(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch
     the number ``draws`` in [0, 1) (float32 [R], top_k int32).  With w_i = exp((z_i - max z) / temperature): the top_k largest logits stay
     (0: all), of those the most probable that make up ``top_p`` of their weight together (1: all), of those the ones of w_i >= ``min_p``
     (0: all; the largest always), logits that are equal in or out together; the token is the first of them whose running sum of weights reaches draws times
-    their sum.  Temperature 0 is argmax, the lowest index first.  Weights below 2^-45 (of rows of more than 2^18 logits 2^-41) count for
-    nothing; a logit that is no number is none.  ``only``: rows with neither top_p below 1 nor min_p above 0 keep what out holds."""
+    their sum.  Temperature 0 is argmax, the lowest index first.  Weights are held to 2^-42 of the largest (of rows of more than 2^18
+    logits to 2^-38), and smaller ones count for nothing; a logit that is no number is none.  ``only``: rows with neither top_p below 1 nor min_p above 0 keep what out holds."""
     _launch_count[0] += 1
     (_host or _host_calls()).sample_nucleus(logits, temperature, top_k, top_p, min_p, draws, out, only)
 
