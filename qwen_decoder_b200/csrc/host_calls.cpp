@@ -370,6 +370,7 @@ CALL(token_logprobs, 3)
 END
 
 // ---- a cache in 8 bits
+constexpr int64_t MOST_OF_PAGE = 1 << 14;            // (heads or tokens of a page: a page's rows are counted in 32 bits)
 int whole(PyObject* o, const char* what) {
   const long v = PyLong_AsLong(o);
   if (PyErr_Occurred()) throw PythonError{};
@@ -387,7 +388,7 @@ void* plain(const at::Tensor& t, at::ScalarType dt, int64_t n, int device, const
 struct Heads { int H, G, d, ps; };
 Heads heads_of(PyObject* const* a, int at_ps, const char* what) {
   const Heads h = {whole(a[0], what), whole(a[1], what), whole(a[2], what), whole(a[at_ps], what)};
-  if (h.G < 1 || h.H < 1 || h.H % h.G || h.H / h.G > 16 || (h.d != 64 && h.d != 128) || h.ps < 16 || h.ps % 16)
+  if (h.G < 1 || h.G > MOST_OF_PAGE || h.ps > MOST_OF_PAGE || h.H < 1 || h.H % h.G || h.H / h.G > 16 || (h.d != 64 && h.d != 128) || h.ps < 16 || h.ps % 16)
     refuse(what, ": up to 16 query heads to each of ", h.G, " kv heads of 64 or 128 features and pages of a multiple of 16 tokens, got ", h.H, " heads of ",
            h.d, ", pages of ", h.ps);
   return h;
@@ -407,6 +408,24 @@ int64_t heads_rows(const at::Tensor& t, int64_t n, const char* what) {
     refuse(what, " must be bfloat16 [T, ", n, "], rows contiguous, on 16 bytes and a multiple of 16 bytes apart, got ", toString(t.scalar_type()), " ", sizes(t));
   return t.size(0);
 }
+
+// (pages, G, page_size, d): numbers [n, 2, G, page_size, d] and scales [n, G, page_size, 2]
+CALL(fp8_page_views, 4)
+  const char* what = "fp8_page_views";
+  const at::Tensor& pages = tensor(a[0], "fp8_page_views: pages");
+  const int64_t G = whole(a[1], what), ps = whole(a[2], what), d = whole(a[3], what);
+  const int64_t bytes = G * ps * (2 * d + 2), n = 2 * G * ps * d;
+  if (G < 1 || ps < 1 || d < 1 || G > MOST_OF_PAGE || ps > MOST_OF_PAGE || d > MOST_OF_PAGE || pages.scalar_type() != at::kByte || pages.dim() != 2 || pages.size(1) != bytes || pages.stride(1) != 1)
+    refuse(what, ": pages must be uint8 [n, ", bytes, "], rows contiguous, got ", toString(pages.scalar_type()), " ", sizes(pages));
+  const int64_t at = pages.storage_offset(), row = pages.stride(0);
+  const at::Tensor numbers = pages.view(at::kFloat8_e4m3fn).as_strided({pages.size(0), 2, G, ps, d}, {row, n / 2, ps * d, d, 1}, at);
+  const at::Tensor scales = pages.view(at::kFloat8_e8m0fnu).as_strided({pages.size(0), G, ps, 2}, {row, 2 * ps, 2, 1}, at + n);
+  PyObject* out = PyTuple_New(2);
+  if (!out) throw PythonError{};
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(numbers));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(scales));
+  return out;
+END
 
 // (qkv, bias, q_out, H, G, d, rotary_dim, pairing, cos, sin, positions, pages, slot_map, page_size, write_kv)
 CALL(rope_kv_write_fp8, 15)
@@ -566,7 +585,7 @@ END
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(start), ENTRY(fp8_rows), ENTRY(check_rows), ENTRY(quantize_fp8), ENTRY(gate_fp8), ENTRY(add_rmsnorm_fp8), ENTRY(gemm_fp8),
-                         ENTRY(gemm_fp8_gated), ENTRY(gemm_fp8_plan), ENTRY(token_logprobs), ENTRY(rope_kv_write_fp8),
+                         ENTRY(gemm_fp8_gated), ENTRY(gemm_fp8_plan), ENTRY(token_logprobs), ENTRY(fp8_page_views), ENTRY(rope_kv_write_fp8),
                          ENTRY(decode_attention_fp8), ENTRY(prefill_attention_fp8), ENTRY(sample_nucleus), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qd_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

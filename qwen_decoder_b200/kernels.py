@@ -1027,8 +1027,8 @@ def gemm_fp8_gated(x: Fp8Rows, w: Fp8Rows, bias: Optional[torch.Tensor], out: Fp
 # ------------------------------------------------------------------ a paged cache in 8 bits
 def fp8_cache_supported(H: int, G: int, d: int, page_size: int) -> bool:
     """What the attention over a cache in 8 bits takes: heads of 64 or 128 features, up to 16 query heads per KV head, pages of a multiple
-    of 16 tokens."""
-    return d in (64, 128) and G >= 1 and H % G == 0 and 1 <= H // G <= 16 and page_size % 16 == 0 and page_size > 0
+    of 16 tokens (16,384 at most, like KV heads)."""
+    return d in (64, 128) and 1 <= G <= 1 << 14 and H % G == 0 and 1 <= H // G <= 16 and page_size % 16 == 0 and 0 < page_size <= 1 << 14
 
 
 def fp8_page_bytes(G: int, page_size: int, d: int) -> int:
@@ -1045,9 +1045,7 @@ def fp8_pages(n_pages: int, G: int, page_size: int, d: int, device) -> torch.Ten
 def fp8_page_views(pages: torch.Tensor, G: int, page_size: int, d: int):
     """(numbers float8_e4m3fn [n_pages, 2, G, page_size, d], scales float8_e8m0fnu [n_pages, G, page_size, 2]) of such a cache: key and
     value are numbers[:, 0] * scales[..., 0] and numbers[:, 1] * scales[..., 1]."""
-    n = 2 * G * page_size * d
-    return (pages[:, :n].view(torch.float8_e4m3fn).view(-1, 2, G, page_size, d),
-            pages[:, n:].view(torch.float8_e8m0fnu).view(-1, G, page_size, 2))
+    return (_host or _host_calls()).fp8_page_views(pages, G, page_size, d)
 
 
 def rope_kv_write_fp8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tensor, H: int, G: int, d: int, rotary_dim: int,

@@ -19,8 +19,22 @@ def test_pages():
     assert int(pages[1, 2 * 16 * 64 + 3 * 64 + 5]) == 9 and int(pages[1, 4 * 16 * 64 + 16 * 2 + 4 * 2 + 1]) == 8
 
 
+@pytest.mark.parametrize("bad", [(torch.zeros(3, 4160), 2, 16, 64), (torch.zeros(4160, dtype=torch.uint8), 2, 16, 64), (torch.zeros(3, 4161, dtype=torch.uint8), 2, 16, 64),
+                                 (torch.zeros(3, 8320, dtype=torch.uint8)[:, ::2], 2, 16, 64), (torch.zeros(3, 4160, dtype=torch.uint8), -2, -16, 64),
+                                 (torch.zeros(3, 0, dtype=torch.uint8), 0, 16, 64), (torch.zeros(3, 4160, dtype=torch.uint8), 2, 1 << 31, 64), (None, 2, 16, 64)])
+def test_page_views(bad):
+    with pytest.raises((KernelError, TypeError)):
+        kernels.fp8_page_views(*bad)
+
+
+def test_page_views_of_rows_apart():
+    whole = torch.arange(6 * 4160, dtype=torch.int64).remainder(251).to(torch.uint8).view(6, 4160)
+    numbers, scales = kernels.fp8_page_views(whole[1::2], 2, 16, 64)
+    assert torch.equal(numbers.view(torch.uint8).flatten(1), whole[1::2, :4096]) and torch.equal(scales.view(torch.uint8).flatten(1), whole[1::2, 4096:])
+
+
 @pytest.mark.parametrize("H,G,d,ps,ok", [(16, 2, 128, 16, True), (14, 2, 64, 48, True), (17, 1, 128, 16, False), (16, 2, 96, 16, False), (16, 3, 64, 16, False),
-                                         (16, 2, 64, 8, False), (16, 2, 64, 0, False), (16, 1, 64, 16, True)])
+                                         (16, 2, 64, 8, False), (16, 2, 64, 0, False), (16, 1, 64, 16, True), (16, 2, 64, 1 << 15, False)])
 def test_supported(H, G, d, ps, ok):
     assert kernels.fp8_cache_supported(H, G, d, ps) == ok
 
