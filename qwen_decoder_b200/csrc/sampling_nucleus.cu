@@ -37,9 +37,8 @@ namespace cg = cooperative_groups;
 #define SN_STEP 7                                // log2 of the powers to a step of the first histogram
 static_assert((SN_OCTAVES * SN_POWERS >> SN_STEP) + 1 < SN_BINS, "steps of the first histogram");
 #define SN_FEW 256                               // a top-k up to here goes by the list
-#define SN_LIST 2048
+#define SN_LIST 1024
 #define SN_AHEAD 4                               // 16 bytes each that a thread has on their way
-#define SN_NEAR 1024                             // logits next to a border that are put in order
 
 struct SnArgs {
   const float* logits;
@@ -47,7 +46,7 @@ struct SnArgs {
   const float *temperature, *top_p, *min_p, *draws;
   const int* top_k;
   int* out;
-  int V, shares, vec, keep, weights, bits, only;          // keep, weights: a CTA's logits and their weights are in shared memory
+  int V, shares, vec, keep, maxima, bits, only;           // in shared memory: a CTA's logits; the maxima of a thread's 16 of them
 };
 // 2^(-k / 4096) over 2^44: powers of the twelfth root of a half, each root the whole root of the one before, over 2^63
 struct SnPowers {
@@ -77,16 +76,17 @@ struct SnShared {
       uint2 mine[SN_BINS];                       // a 64-bit sum each, the low half in x
       unsigned long long all[SN_BINS];           // of the cluster
     };
-    struct {                                     // with a small top-k, of the cluster's first CTA: logits as keys above the complement of their
-      unsigned long long list[SN_LIST], mass[SN_LIST];       // index, the largest first; sums of weights up to each
+    struct {                                     // logits that go to the cluster's first CTA, of a small top-k or of the step that a border lies in: keys (of a
+      unsigned long long list[SN_LIST], mass[SN_LIST];       // top-k above the complement of their index); their weights
     };
   };
   __align__(16) unsigned long long powers[SN_POWERS];
-  unsigned long long near[SN_NEAR];              // of the cluster's first CTA: keys
+  unsigned near[SN_LIST];                        // (the step's keys: they come while the histogram is still there)
   int listed;
   unsigned long long got[2][SN_MAX_SHARES];      // a word of each CTA
   unsigned long long warps[SN_WARPS], above;
-  unsigned bin, ends[2], key, last_step[2], counts[SN_WARPS];
+  unsigned bin, ends[2], key, token, last_step[2], counts[SN_WARPS];
+  float kept[SN_WARPS][160];                     // what a warp has found, up to 31 of before and 128
 };
 
 __device__ __forceinline__ unsigned sn_order(float z) {             // ascending; no number: 0
@@ -103,7 +103,6 @@ struct SnRow {
   float c, c2;                                   // 1 / (T log 2)
   int bits;
   const unsigned long long* powers;              // in shared memory
-  unsigned long long* weight;                    // of this CTA's part, where they are kept (else null)
 };
 // four neighbouring logits, minus infinity behind the end
 __device__ __forceinline__ void sn_four(const SnRow& r, int i, float (&v)[4]) {
@@ -113,6 +112,14 @@ __device__ __forceinline__ void sn_four(const SnRow& r, int i, float (&v)[4]) {
   } else {
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = i + j < r.n ? r.z[i + j] : -INFINITY;
+  }
+}
+// SN_AHEAD times four, 128 apart
+__device__ __forceinline__ void sn_ahead(const SnRow& r, int i, float (&v)[SN_AHEAD][4]) {
+#pragma unroll
+  for (int u = 0; u < SN_AHEAD; u++) {
+    v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
+    if (i + 128 * u < r.warp_to) sn_four(r, i + 128 * u, v[u]);
   }
 }
 // y = (max - z) / (T log 2) in 4,096ths, of which the first histogram's steps are 128; SN_OCTAVES of them, and what is no number, are far
@@ -128,7 +135,7 @@ __device__ __forceinline__ unsigned long long sn_weight(const SnRow& r, float z,
   const float d = r.top - z, back = d - r.top, d2 = (r.top - (d - back)) - (z + back);       // (what the difference lost)
   const float p = d * r.c;
   const float e = fmaf(d2, r.c, fmaf(d, r.c2, fmaf(d, r.c, -p)));
-  const float f = fmaf((float)k, -1.f / SN_POWERS, p), y = f + e, y2 = e - (y - f);
+  const float f = fmaf(__int_as_float(k + 0x4b400000) - 12582912.f, -1.f / SN_POWERS, p), y = f + e, y2 = e - (y - f);
   const float x = y * 0.693147182f, x2 = fmaf(y2, 0.693147182f, fmaf(y, -1.90465421e-9f, fmaf(y, 0.693147182f, -x)));
   const float rest = fmaf(x * x, fmaf(x, 1.f / 6, -0.5f), x2);
   const int less = __float2int_rn(x * 17592186044416.f) + (__float_as_int(fmaf(rest, 17592186044416.f, 12582912.f)) - 0x4b400000);       // over 2^-44
@@ -139,21 +146,14 @@ __device__ __forceinline__ unsigned long long sn_weight(const SnRow& r, float z,
 }
 // (one copy of the code for what is asked for seldom: a launch goes through most of its code once, and waits for it where it is long)
 __device__ __noinline__ unsigned long long sn_weight_once(const SnRow& r, float z) { return sn_weight(r, z, sn_place(r, z)); }
-// of this CTA's four logits from i on, z; none of those below ``least``
-__device__ __forceinline__ void sn_weights_at(const SnRow& r, int i, const float (&z)[4], float least, unsigned long long (&w)[4]) {
-  if (r.weight) {
-    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(r.weight + i), b = *reinterpret_cast<const ulonglong2*>(r.weight + i + 2);
-    w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
-#pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = z[j] >= least ? w[j] : 0;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = z[j] >= least ? sn_weight_once(r, z[j]) : 0;
-  }
-}
 // the least weight that min_p leaves
 __device__ __forceinline__ unsigned long long sn_least(const SnRow& r, float min_p) {
   return (unsigned long long)ceil(fmin((double)min_p, 1.0) * (double)(1ull << r.bits));
+}
+
+// a share of a sum, in whole weights, ``least`` or more
+__device__ __forceinline__ unsigned long long sn_part(unsigned long long total, float share, unsigned long long least) {
+  return max(__double2ull_ru(fmax((double)share, 0.0) * (double)total), least);
 }
 
 // every CTA's word, in every CTA.  Calls in turn use two places, so that a fast CTA's next word does not meet a slow one's reading.
@@ -198,76 +198,45 @@ __device__ __forceinline__ unsigned sn_first_key(unsigned lo, unsigned hi, F hol
   return hi;
 }
 
-// n 64-bit numbers in order, the largest first, in room for the next power of two.  Up to 384 by counting for each how many come before it (200:
-// 2,000 cycles), more by bitonic steps (36 of them for 200, 150 cycles each with the barrier).
-__device__ void sn_sort(unsigned long long* list, int n) {
-  if (n <= 384) {
-    __syncthreads();
-    const unsigned long long own = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
-    int before = 0;
+// Threads to each of n numbers of a list, neighbours, so that the block has them all in one or two turns
+__device__ __forceinline__ int sn_threads(int n) { return n <= SN_THREADS / 8 ? 8 : n <= SN_THREADS / 4 ? 4 : n <= SN_THREADS / 2 ? 2 : 1; }
+// the sum of the words of those of a list's n that ``with`` holds for, by the ``each`` threads of a number (n^2 additions, n being some hundred: less
+// than putting them in order, whose steps wait for one another)
+template <typename W, typename F>
+__device__ __forceinline__ W sn_sum_with(int n, int each, F word) {
+  W sum = 0;
 #pragma unroll 4
-    for (int i = 0; i < n; i++) before += list[i] > own || list[i] == own && i < (int)threadIdx.x;
-    __syncthreads();
-    if ((int)threadIdx.x < n) list[before] = own;
-    __syncthreads();
-    return;
-  }
-  int size = 32;
-  while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += SN_THREADS) list[i] = 0;
-  for (int span = 2; span <= size; span *= 2)
-    for (int step = span / 2; step > 0; step /= 2) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < size / 2; i += SN_THREADS) {
-        const int x = 2 * i - (i & (step - 1)), y = x + step;
-        const unsigned long long p = list[x], q = list[y];
-        if ((p < q) == !(x & span)) { list[x] = q; list[y] = p; }
-      }
-    }
-  __syncthreads();
+  for (int j = threadIdx.x & (each - 1); j < n; j += each) sum += word(j);
+  for (int o = each / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
 }
-// sums up to each of n words, by the whole block; all of them
-template <typename F>
-__device__ unsigned long long sn_sums(SnShared& s, int n, F word) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long carry = 0;
-  for (int i0 = 0; i0 < n; i0 += SN_THREADS) {
-    const int i = i0 + threadIdx.x;
-    unsigned long long sum = i < n ? word(i) : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    if (lane == 31) s.warps[warp] = sum;
-    __syncthreads();
-    unsigned long long ahead = carry;
-    for (int w = 0; w < SN_WARPS; w++) {
-      if (w < warp) ahead += s.warps[w];
-      carry += s.warps[w];
-    }
-    if (i < n) s.mass[i] = ahead + sum;
-    __syncthreads();
-  }
-  return carry;
+// a logit of the step that a border lies in, to the list
+__device__ __noinline__ void sn_put(const SnRow& r, float z, unsigned bin, int* count, unsigned* near) {
+  if (sn_step(r, z) != bin) return;
+  const int at = atomicAdd(count, 1);
+  if (at < SN_LIST) near[at] = sn_order(z);
 }
 // The border among the n keys of ``near``, above all of which lies ``above``.
 template <bool MASS>
-__device__ unsigned sn_among(SnShared& s, const SnRow& r, int n, unsigned long long above, double want) {
-  sn_sort(s.near, n);
-  sn_sums(s, n, [&](int i) { return MASS ? sn_weight_once(r, sn_value((unsigned)s.near[i])) : 1ull; });
-  if (threadIdx.x == 0) s.bin = n - 1;
+__device__ unsigned sn_among(SnShared& s, const SnRow& r, int n, unsigned long long above, unsigned long long want) {
+  for (int i = threadIdx.x; i < n; i += SN_THREADS) s.mass[i] = MASS ? sn_weight_once(r, sn_value(s.near[i])) : 1ull;
+  if (threadIdx.x == 0) s.token = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += SN_THREADS)
-    if ((double)(above + s.mass[i]) >= want && (i == 0 || !((double)(above + s.mass[i - 1]) >= want))) s.bin = i;
+  const int each = sn_threads(n);
+  for (int i0 = 0; i0 < n; i0 += SN_THREADS / each) {
+    const int i = i0 + threadIdx.x / each;
+    const unsigned own = s.near[min(i, n - 1)];
+    const unsigned long long sum = sn_sum_with<unsigned long long>(n, each, [&](int j) { return s.near[j] >= own ? s.mass[j] : 0ull; });
+    if (i < n && above + sum >= want) atomicMax(&s.token, own);
+  }
   __syncthreads();
-  return (unsigned)s.near[s.bin];
+  return s.token;
 }
 
-// The largest key t so that the logits of keys from t on, none below ``floor`` among them, hold ``want`` or more: counts, or of weights the
-// share ``want`` of them all.  ``floor`` where there is less than that down to where weights end.
+// The largest key t so that the logits of keys from t on, none below ``floor`` among them, hold ``want`` or more: counts, or of weights
+// ``share`` of them all.  ``floor`` where there is less than that down to where weights end.
 template <bool MASS>
-__device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned floor, double want) {
+__device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned floor, float share, unsigned long long want) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned top = sn_order(r.top);
   unsigned k_lo = floor, k_hi = top;             // the border is one of these
@@ -278,35 +247,29 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
     for (int b = threadIdx.x; b < SN_BINS; b += SN_THREADS) s.mine[b] = make_uint2(0, 0);
     __syncthreads();
     const float from_z = sn_value(k_lo), to_z = sn_value(k_hi);
+    float next[4];
+    if (r.warp_from + 4 * lane < r.warp_to) sn_four(r, r.warp_from + 4 * lane, next);
 #pragma unroll 1
     for (int i = r.warp_from + 4 * lane; i < r.warp_to; i += 128) {
       float v[4];
       unsigned bin[4];
       unsigned long long w[4] = {1, 1, 1, 1};
-      sn_four(r, i, v);
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = next[j];
+      if (i + 128 < r.warp_to) sn_four(r, i + 128, next);
       if (level == 0) {
-        int k[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          k[j] = v[j] >= from_z ? sn_place(r, v[j]) : SN_OCTAVES * SN_POWERS;
-          bin[j] = k[j] < SN_OCTAVES * SN_POWERS ? (unsigned)k[j] >> SN_STEP : SN_BINS;
-        }
-        if (MASS) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) w[j] = sn_weight(r, v[j], k[j]);
-          if (r.weight) {
-            *reinterpret_cast<ulonglong2*>(r.weight + i) = make_ulonglong2(w[0], w[1]);
-            *reinterpret_cast<ulonglong2*>(r.weight + i + 2) = make_ulonglong2(w[2], w[3]);
-          }
+          const int k = v[j] >= from_z ? sn_place(r, v[j]) : SN_OCTAVES * SN_POWERS;
+          bin[j] = k < SN_OCTAVES * SN_POWERS ? (unsigned)k >> SN_STEP : SN_BINS;
+          if (MASS) w[j] = sn_weight(r, v[j], k);
         }
       } else {
-        bool any = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           bin[j] = v[j] >= from_z && v[j] <= to_z ? (k_hi - sn_order(v[j])) >> shift : SN_BINS;
-          any |= bin[j] < SN_BINS;
+          if (MASS && bin[j] < SN_BINS) w[j] = sn_weight_once(r, v[j]);
         }
-        if (MASS && any) sn_weights_at(r, i, v, from_z, w);
       }
 #pragma unroll
       for (int j = 0; j < 4; j++)
@@ -360,10 +323,10 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
       run += w < warp ? s.warps[w] : 0;
       total += s.warps[w];
     }
-    if (MASS && level == 0) want = fmax(want * (double)total, 1.0);
-    if (!((double)run >= want) && (double)(run + sum) >= want) {
+    if (MASS && level == 0) want = sn_part(total, share, 1);
+    if (run < want && run + sum >= want) {
       int u = 0;
-      while (u < SN_EACH - 1 && !((double)(run + own[u]) >= want)) run += own[u++];
+      while (u < SN_EACH - 1 && run + own[u] < want) run += own[u++];
       s.bin = threadIdx.x * SN_EACH + u;
       s.above = run;
     }
@@ -374,22 +337,23 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
     if (level == 0) {
       // the step's logits to the first CTA, in any order
       int* count = shares > 1 ? cg::this_cluster().map_shared_rank(&s.listed, 0) : &s.listed;
-      unsigned long long* near = shares > 1 ? cg::this_cluster().map_shared_rank(s.near, 0) : s.near;
-#pragma unroll 1
-      for (int i = r.warp_from + 4 * lane; i < r.warp_to; i += 128) {
-        float v[4];
-        sn_four(r, i, v);
+      unsigned* near = shares > 1 ? cg::this_cluster().map_shared_rank(s.near, 0) : s.near;
+      // (about where the step lies, its ends a 256th of it further out and by what the terms of y can have lost: few are looked at closely)
+      const float wide = (float)(1 << SN_STEP) / SN_POWERS / r.c, out = wide * (1.f / 256) + fabsf(r.top) * 2.4e-7f + ((float)bin + 1.f) * wide * 2.4e-7f;
+      const float lo_z = fmaxf(from_z, r.top - ((float)bin + 1.f) * wide - out), hi_z = fminf(to_z, r.top - ((float)bin - 1.f / 256) * wide + out);
+      for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD) {
+        float v[SN_AHEAD][4];
+        sn_ahead(r, i0, v);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (v[j] >= from_z && v[j] <= to_z && sn_step(r, v[j]) == bin) {
-            const int at = atomicAdd(count, 1);
-            if (at < SN_NEAR) near[at] = sn_order(v[j]);
-          }
+        for (int u = 0; u < SN_AHEAD; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (v[u][j] >= lo_z && v[u][j] <= hi_z) sn_put(r, v[u][j], bin, count, near);
       }
       if (shares > 1) cg::this_cluster().sync();
       else __syncthreads();
       const int n = *count;
-      if (n <= SN_NEAR && (shares == 1 || cg::this_cluster().block_rank() == 0)) {
+      if (n <= SN_LIST && (shares == 1 || cg::this_cluster().block_rank() == 0)) {
         const unsigned key = sn_among<MASS>(s, r, n, above, want);
         if ((int)threadIdx.x < shares) *(shares > 1 ? cg::this_cluster().map_shared_rank(&s.key, threadIdx.x) : &s.key) = key;
         __syncthreads();
@@ -397,7 +361,7 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
       if (shares > 1) cg::this_cluster().sync();           // (the first CTA's list has been counted, too)
       else __syncthreads();
       if (threadIdx.x == 0) s.listed = 0;
-      if (n <= SN_NEAR) return s.key;
+      if (n <= SN_LIST) return s.key;
     }
     if (level) {
       k_hi -= bin << shift;
@@ -423,7 +387,7 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
 
 // A token by the list of a small top-k, or -1 where more logits reach the bound than it holds.  ``best``: this thread's maximum.  The cluster's first CTA
 // knows the token, the others -1 or 0.
-__device__ int sn_by_list(SnShared& s, const SnRow& r, int shares, int rank, int first, int k, unsigned best, float top_p, float min_p, float draw,
+__device__ int sn_by_list(SnShared& s, const SnRow& r, int shares, int rank, int first, int k, unsigned best, const float* maxima, float top_p, float min_p, float draw,
                           int likeliest, int& turn) {
   const int lane = threadIdx.x & 31;
   // the bound: of the threads' maxima the least of those in the steps between the row's maximum and the least of them that hold k, or ceil(k / S)
@@ -476,13 +440,11 @@ __device__ int sn_by_list(SnShared& s, const SnRow& r, int shares, int rank, int
   int* count = shares > 1 ? cl.map_shared_rank(&s.listed, 0) : &s.listed;
   unsigned long long* list = shares > 1 ? cl.map_shared_rank(s.list, 0) : s.list;
   const float bound_z = sn_value(bound);
-  for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD) {
+  const float* mine = maxima + threadIdx.x;
+  for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD, mine += SN_THREADS) {
+    if (maxima && !(*mine >= bound_z)) continue;
     float v[SN_AHEAD][4];
-#pragma unroll
-    for (int u = 0; u < SN_AHEAD; u++) {
-      v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
-      if (i0 + 128 * u < r.warp_to) sn_four(r, i0 + 128 * u, v[u]);
-    }
+    sn_ahead(r, i0, v);
 #pragma unroll
     for (int u = 0; u < SN_AHEAD; u++)
       if (fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3])) >= bound_z) {
@@ -506,40 +468,43 @@ __device__ int sn_by_list(SnShared& s, const SnRow& r, int shares, int rank, int
   if (shares > 1) cl.sync();
   if (threadIdx.x == 0) s.listed = 0;
   if (rank) return 0;
-  sn_sort(s.list, n);
-  // the k-th largest and its equals, sums of weights
+  // weights of those with less than k larger ones
   auto key_at = [&](int i) { return (unsigned)(s.list[i] >> 32); };
-  const unsigned kth = key_at(min(k, n) - 1);
-  const unsigned long long carry = sn_sums(s, n, [&](int i) { return key_at(i) >= kth ? sn_weight_once(r, sn_value(key_at(i))) : 0ull; });
-  // the last key that stays: the k-th largest, or of the nucleus, or of those with enough probability
-  if (threadIdx.x == 0) { s.ends[0] = kth; s.key = 0xffffffffu; s.ends[1] = kth; }
+  if (threadIdx.x == 0) { s.key = 0; s.token = 0xffffffffu; }
   __syncthreads();
-  const double want = top_p < 1.f ? fmax(fmax((double)top_p, 0.0) * (double)carry, 1.0) : 0.0;
-  const unsigned long long enough = sn_least(r, min_p);
-  for (int i = threadIdx.x; i < n; i += SN_THREADS) {
-    if (top_p < 1.f && (double)s.mass[i] >= want && (i == 0 || !((double)s.mass[i - 1] >= want))) s.ends[0] = key_at(i);
-    if (min_p > 0.f) {
-      const bool here = i == 0 || sn_weight_once(r, sn_value(key_at(i))) >= enough;
-      const bool next = i + 1 < n && sn_weight_once(r, sn_value(key_at(i + 1))) >= enough;
-      if (here && !next) s.ends[1] = key_at(i);
+  const int each = sn_threads(n), turns = SN_THREADS / each, part = threadIdx.x & (each - 1);
+  for (int i0 = 0; i0 < n; i0 += turns) {
+    const int i = i0 + threadIdx.x / each;
+    const unsigned own = key_at(min(i, n - 1));
+    const int larger = sn_sum_with<int>(n, each, [&](int j) { return key_at(j) > own ? 1 : 0; });
+    if (i < n && part == 0) s.mass[i] = larger < k ? sn_weight_once(r, sn_value(own)) : 0ull;
+  }
+  __syncthreads();
+  // the last key of the nucleus: the largest with enough of the weights at it and above
+  if (top_p < 1.f) {
+    const unsigned long long want = sn_part(sn_sum_with<unsigned long long>(n, 32, [&](int j) { return s.mass[j]; }), top_p, 1);
+    for (int i0 = 0; i0 < n; i0 += turns) {
+      const int i = i0 + threadIdx.x / each;
+      const unsigned own = key_at(min(i, n - 1));
+      const unsigned long long sum = sn_sum_with<unsigned long long>(n, each, [&](int j) { return key_at(j) >= own ? s.mass[j] : 0ull; });
+      if (i < n && sum >= want) atomicMax(&s.key, own);
     }
+    __syncthreads();
   }
+  const unsigned long long enough = min_p > 0.f ? sn_least(r, min_p) : 0ull;
+  for (int i = threadIdx.x; i < n; i += SN_THREADS)
+    if (key_at(i) < s.key || s.mass[i] < enough) s.mass[i] = 0;
   __syncthreads();
-  const unsigned last = max(kth, max(s.ends[0], s.ends[1]));
-  int stay = 0;
-  for (int i0 = 0; i0 < n; i0 += SN_THREADS) stay += __syncthreads_count(i0 + (int)threadIdx.x < n && key_at(i0 + threadIdx.x) >= last);
   // the first of them, by index, whose sum of weights up to it reaches the draw's share
-  const unsigned long long total = s.mass[stay - 1];
-  const double target = (double)total * (double)draw;
-  for (int i = threadIdx.x; i < stay; i += SN_THREADS) {
-    const unsigned low = (unsigned)s.list[i];    // (larger: an index before)
-    unsigned long long sum = 0;
-    for (int j = 0; j < stay; j++) sum += (unsigned)s.list[j] >= low ? s.mass[j] - (j ? s.mass[j - 1] : 0) : 0;
-    const unsigned long long own = s.mass[i] - (i ? s.mass[i - 1] : 0);
-    if (own && (double)sum >= target) atomicMin(&s.key, 0xffffffffu - low);
+  const unsigned long long want = sn_part(sn_sum_with<unsigned long long>(n, 32, [&](int j) { return s.mass[j]; }), draw, 1);
+  for (int i0 = 0; i0 < n; i0 += turns) {
+    const int i = i0 + threadIdx.x / each;
+    const unsigned low = (unsigned)s.list[min(i, n - 1)];            // (larger: an index before)
+    const unsigned long long sum = sn_sum_with<unsigned long long>(n, each, [&](int j) { return (unsigned)s.list[j] >= low ? s.mass[j] : 0ull; });
+    if (i < n && s.mass[i] && sum >= want) atomicMin(&s.token, 0xffffffffu - low);
   }
   __syncthreads();
-  return s.key == 0xffffffffu ? likeliest : (int)s.key;
+  return s.token == 0xffffffffu ? likeliest : (int)s.token;
 }
 
 __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnArgs a) {
@@ -563,7 +528,6 @@ __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnA
   const int per_warp = ((r.n + SN_WARPS - 1) / SN_WARPS + 127) / 128 * 128;
   r.warp_from = min(warp * per_warp, r.n);
   r.warp_to = min(r.warp_from + per_warp, r.n);
-  r.weight = nullptr;
   r.powers = s.powers;
   r.bits = a.bits;
   if (threadIdx.x == 0) s.listed = 0;
@@ -574,21 +538,21 @@ __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnA
   // ---- the maximum, of equal ones the first
   float top = -INFINITY;
   int top_at = -1;                               // (none but minus infinity and no numbers)
-  for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD) {
-    float v[SN_AHEAD][4];
-#pragma unroll
-    for (int u = 0; u < SN_AHEAD; u++) {
-      v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
-      if (i0 + 128 * u < r.warp_to) sn_four(r, i0 + 128 * u, v[u]);
-    }
+  float* most = kept + threadIdx.x;
+  for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD, most += SN_THREADS) {
+    float v[SN_AHEAD][4], here = -INFINITY;
+    int here_at = -1;
+    sn_ahead(r, i0, v);
 #pragma unroll
     for (int u = 0; u < SN_AHEAD; u++) {
       const int i = i0 + 128 * u;
       if (a.keep && i < r.warp_to) *reinterpret_cast<float4*>(kept + i) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        if (v[u][j] > top) { top = v[u][j]; top_at = i + j; }
+        if (v[u][j] > here) { here = v[u][j]; here_at = i + j; }
     }
+    if (a.maxima) *most = here;
+    if (here > top) { top = here; top_at = here_at; }
   }
   // key above the complement of the index
   unsigned long long best = top_at < 0 ? 0ull : (unsigned long long)sn_order(top) << 32 | (0xffffffffu - (unsigned)(first + top_at));
@@ -607,26 +571,26 @@ __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnA
     return;
   }
   // (a temperature of 2^-120 and below is this one: all but the largest are out of sight)
-  const double c = 1.0 / (fmax((double)temperature, 7.5e-37) * 0.69314718055994530942);
-  r.c = (float)c;
-  r.c2 = (float)(c - (double)r.c);
+  // 1 / (T log 2) as a pair: the quotient of one of 32 bits, and what it lacks
+  const float up = temperature < 8.7e-19f ? 1.15292150e18f : 1.f, t = fmaxf(temperature, 7.5e-37f) * up;               // (2^60)
+  const float t1 = t * 0.693147182f, t2 = fmaf(t, 0.693147182f, -t1) + t * -1.90465421e-9f;
+  const float c1 = 1.f / t1;
+  r.c = c1 * up;
+  r.c2 = c1 * fmaf(-c1, t2, fmaf(-c1, t1, 1.f)) * up;
 
   // ---- which logits stay
   unsigned floor = SN_LOWEST;
   const int k = a.top_k[row];
   if (k > 0 && k <= SN_FEW && k < a.V) {
-    const int token = sn_by_list(s, r, a.shares, rank, first, k, own, top_p, min_p, a.draws[row], likeliest, turn);
+    const int token = sn_by_list(s, r, a.shares, rank, first, k, own, a.maxima ? kept : nullptr, top_p, min_p, a.draws[row], likeliest, turn);
     if (token >= 0) {
       if (rank == 0 && threadIdx.x == 0) a.out[row] = token;
       return;
     }
   }
-  if (k > 0 && k < a.V) floor = sn_border<false>(s, r, a.shares, floor, (double)k);
+  if (k > 0 && k < a.V) floor = sn_border<false>(s, r, a.shares, floor, 0.f, k);
   unsigned last = floor;
-  if (top_p < 1.f) {
-    if (a.weights) r.weight = reinterpret_cast<unsigned long long*>(kept + part);
-    last = max(last, sn_border<true>(s, r, a.shares, floor, fmax((double)top_p, 0.0)));
-  }
+  if (top_p < 1.f) last = max(last, sn_border<true>(s, r, a.shares, floor, top_p, 0));
   if (min_p > 0.f) {
     const unsigned long long enough = sn_least(r, min_p);
     __syncthreads();
@@ -639,52 +603,79 @@ __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnA
     last = max(last, s.key);
   }
 
-  // ---- the first of them whose running sum reaches the draw's share
+  // ---- the first of them whose running sum reaches the draw's share: the CTA that it falls to, a sixteenth of its part, of that, ..., 128 logits
   const float last_z = sn_value(last);
-  auto weights = [&](int i, unsigned long long (&w)[4]) {
-    float v[4];
-    sn_four(r, i, v);
-    w[0] = w[1] = w[2] = w[3] = 0;
-    if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= last_z) sn_weights_at(r, i, v, last_z, w);
-    return w[0] + w[1] + w[2] + w[3];
-  };
-  unsigned long long sum = 0, w[4];
+  unsigned long long before = 0, want = 0;
+  int lo = 0, hi = r.n;
+  float* found = s.kept[warp];
+  for (bool whole = true;; whole = false) {
+    const int per = ((hi - lo + SN_WARPS - 1) / SN_WARPS + 127) / 128 * 128, from = min(lo + warp * per, hi), to = min(from + per, hi);
+    // weights of what stays, 32 at a time: few do, and those lie apart
+    unsigned long long sum = 0;
+    int held = 0;
 #pragma unroll 1
-  for (int i = r.warp_from + 4 * lane; i < r.warp_to; i += 128) sum += weights(i, w);
-  sum = sn_block(s, sum, [](unsigned long long x, unsigned long long y) { return x + y; });
-  words = sn_exchange(s, a.shares, sum, turn);
-  unsigned long long total = 0, before = 0;
-  for (int c = 0; c < a.shares; c++) total += words[c];
-  const double target = (double)total * (double)a.draws[row];
-  int owner = -1;
-  for (int c = 0; c < a.shares && owner < 0; c++) {
-    if (words[c] && (double)(before + words[c]) >= target) owner = c;
-    else before += words[c];
-  }
-  if (owner < 0 && rank == 0 && threadIdx.x == 0) a.out[row] = likeliest;      // (a draw beyond its range)
-  if (owner != rank) return;
-  int at = 0;
-  for (; at < SN_WARPS - 1 && !(s.warps[at] && (double)(before + s.warps[at]) >= target); at++) before += s.warps[at];
-  if (warp != at) return;
-  for (int i = r.warp_from + 4 * lane; i - 4 * lane < r.warp_to; i += 128) {
-    const unsigned long long own = i < r.warp_to ? weights(i, w) : 0;
-    unsigned long long incl = own;
+    for (int i = from; i < to || held; i += 128) {
+      if (i < to) {
+        float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i + 4 * lane < to) sn_four(r, i + 4 * lane, v);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, own && (double)(before + incl) >= target);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        unsigned long long run = before + incl - own;
-        int j = 0;
-        while (j < 3 && !(w[j] && (double)(run + w[j]) >= target)) run += w[j++];
-        a.out[row] = first + i + j;
+        for (int j = 0; j < 4; j++) {
+          const bool stays = i + 4 * lane + j < to && v[j] >= last_z;
+          const unsigned all = __ballot_sync(0xffffffffu, stays);
+          if (stays) found[held + __popc(all & ((1u << lane) - 1))] = v[j];
+          held += __popc(all);
+        }
+        __syncwarp();
       }
-      return;
+      while (held >= 32 || (held && i + 128 >= to)) {
+        const int n = min(held, 32);
+        held -= n;
+        const float z = found[held + min(lane, n - 1)];
+        if (lane < n) sum += sn_weight(r, z, sn_place(r, z));
+      }
+      __syncwarp();
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    sum = sn_block(s, sum, [](unsigned long long x, unsigned long long y) { return x + y; });
+    if (whole) {
+      words = sn_exchange(s, a.shares, sum, turn);
+      unsigned long long total = 0;
+      for (int c = 0; c < a.shares; c++) total += words[c];
+      want = sn_part(total, a.draws[row], 1);
+      int owner = -1;
+      for (int c = 0; c < a.shares && owner < 0; c++) {
+        if (before + words[c] >= want) owner = c;
+        else before += words[c];
+      }
+      if (owner < 0 && rank == 0 && threadIdx.x == 0) a.out[row] = likeliest;  // (a draw beyond its range)
+      if (owner != rank) return;
+    }
+    int at = 0;
+    for (; at < SN_WARPS - 1 && before + s.warps[at] < want; at++) before += s.warps[at];
+    lo = min(lo + at * per, hi);
+    hi = min(lo + per, hi);
+    if (hi - lo <= 128) break;
+  }
+  if (warp) return;
+  float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  unsigned long long w[4], own_sum = 0;
+  if (lo + 4 * lane < hi) sn_four(r, lo + 4 * lane, v);
+#pragma unroll 1
+  for (int j = 0; j < 4; j++) {
+    w[j] = lo + 4 * lane + j < hi && v[j] >= last_z ? sn_weight_once(r, v[j]) : 0;
+    own_sum += w[j];
+  }
+  unsigned long long incl = own_sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  const unsigned hit = __ballot_sync(0xffffffffu, before + incl >= want);
+  if (hit && lane == __ffs(hit) - 1) {
+    unsigned long long run = before + incl - own_sum;
+    int j = 0;
+    while (j < 3 && run + w[j] < want) run += w[j++];
+    a.out[row] = first + lo + 4 * lane + j;
   }
 }
 
@@ -732,12 +723,13 @@ extern "C" int qd_sample_nucleus(const float* logits, long long ld, int R, int V
   for (int n = 2; n <= SN_MAX_SHARES && V / n >= 4096 && R <= sn_clusters(n, most, sms, dev); n *= 2) a.shares = n;
   const int part = ((V + a.shares - 1) / a.shares + 3) & ~3;
   a.keep = part <= SN_KEEP;
-  a.weights = part <= SN_KEEP / 3;                  // (8 bytes each beside 4)
+  const size_t per_warp = ((size_t)(part + SN_WARPS - 1) / SN_WARPS + 127) / 128 * 128, turns = (per_warp + 128 * SN_AHEAD - 1) / (128 * SN_AHEAD);
+  a.maxima = !a.keep && turns * SN_THREADS <= SN_KEEP;
   if ((long long)R * a.shares > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(R * a.shares));
   cfg.blockDim = dim3(SN_THREADS);
-  cfg.dynamicSmemBytes = fixed + (a.keep ? (size_t)part * (a.weights ? 12 : 4) : 0);
+  cfg.dynamicSmemBytes = fixed + (a.keep ? part : a.maxima ? turns * SN_THREADS : 0) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
