@@ -7,11 +7,11 @@
 // temperature and top-k (common.cpp:576-629).
 //
 // Which token a number falls to, and which logit is the last of a nucleus, changes where sums are next to a border, and rows have a hundred
-// thousand borders.  So weights are whole numbers, w 2^44 to within three (2^40 for rows of more than 2^18 logits): their sums are exact, in whatever
+// thousand borders.  So weights are whole numbers, w 2^45 to within six (2^41 for rows of more than 2^18 logits): their sums are exact, in whatever
 // order, and a row's token does not depend on how its work is shared.  What is lost is 3 2^-44 of the largest weight for each at most.
 //
 // A cluster of S CTAs shares a row, contiguous parts of it (in shared memory where they fit).  The k-th largest logit and t are found
-// alike, by histograms (counts, or counts and weights) over the cluster: first over 1,472 equal steps of z below the maximum, down to 46 ln 2 T,
+// alike, by histograms (counts, or counts and weights) over the cluster: first over 1,409 equal steps of z below the maximum, down to 44 ln 2 T,
 // where weights end (the logits of a row are spread over many of these, so that few additions meet; in steps of the number's leading bits
 // they would not be); then the logits of the step that the border lies in go to one CTA, which puts them in order.  Where they are more than
 // SN_NEAR (a thousand equal logits), histograms over steps of the logit's bits follow, until a step is one number.
@@ -33,8 +33,9 @@ namespace cg = cooperative_groups;
 #define SN_MAX_SHARES 16
 #define SN_KEEP 36864                            // logits that a CTA holds in shared memory
 #define SN_POWERS 4096                           // to an octave
-#define SN_OCTAVES 46                            // below the maximum a weight is 0
+#define SN_OCTAVES 44                            // below the maximum a weight is 0
 #define SN_STEP 7                                // log2 of the powers to a step of the first histogram
+#define SN_DOWN 18                               // what a power is shifted by at the maximum: 2^63 over 2^45
 static_assert((SN_OCTAVES * SN_POWERS >> SN_STEP) + 1 < SN_BINS, "steps of the first histogram");
 #define SN_FEW 256                               // a top-k up to here goes by the list
 #define SN_LIST 1024
@@ -46,9 +47,9 @@ struct SnArgs {
   const float *temperature, *top_p, *min_p, *draws;
   const int* top_k;
   int* out;
-  int V, shares, vec, keep, maxima, bits, only;           // in shared memory: a CTA's logits; the maxima of a thread's 16 of them
+  int V, shares, vec, keep, maxima, wide, only;           // in shared memory: a CTA's logits, the maxima of a thread's 16; wide: octaves that weights are smaller by
 };
-// 2^(-k / 4096) over 2^44: powers of the twelfth root of a half, each root the whole root of the one before, over 2^63
+// 2^(-k / 4096) over 2^63: powers of the twelfth root of a half, each root the whole root of the one before, over 2^63
 struct SnPowers {
   unsigned long long of[SN_POWERS];
   static constexpr unsigned long long root(unsigned __int128 v) {            // whole part, bit by bit
@@ -63,7 +64,7 @@ struct SnPowers {
     unsigned long long s = 1ull << 62, p = 1ull << 63;
     for (int i = 0; i < 12; i++) s = root((unsigned __int128)s << 63);
     for (int k = 0; k < SN_POWERS; k++) {
-      of[k] = (p + (1 << 18)) >> 19;
+      of[k] = p;
       p = (unsigned long long)((unsigned __int128)p * s >> 63);
     }
   }
@@ -101,7 +102,8 @@ struct SnRow {
   int n, vec, warp_from, warp_to;                // how many, 16 bytes at a time; of this warp
   float top;                                     // the maximum
   float c, c2;                                   // 1 / (T log 2)
-  int bits;
+  float base, octaves;                           // what is added to z's distance in 8 SN_POWERS-ths of an octave; of them until weights end
+  unsigned first_step;
   const unsigned long long* powers;              // in shared memory
 };
 // four neighbouring logits, minus infinity behind the end
@@ -122,38 +124,42 @@ __device__ __forceinline__ void sn_ahead(const SnRow& r, int i, float (&v)[SN_AH
     if (i + 128 * u < r.warp_to) sn_four(r, i + 128 * u, v[u]);
   }
 }
-// y = (max - z) / (T log 2) in 4,096ths, of which the first histogram's steps are 128; SN_OCTAVES of them, and what is no number, are far
-__device__ __forceinline__ int sn_place(const SnRow& r, float z) {
+// z's place: eight times the whole number j of 4,096ths next above y = (max - z) / (T log 2) (or the one behind that), as the bits of a float32 number of
+// 2^23 and more that has ``base`` for 0, whose octaves are SN_DOWN and more.  0 where weights have ended, and for what is no number.
+__device__ __forceinline__ unsigned sn_place(const SnRow& r, float z) {
   const float p = (r.top - z) * r.c;
-  return p < SN_OCTAVES ? __float_as_int(fmaf(p, (float)SN_POWERS, 12582912.f)) - 0x4b400000 : SN_OCTAVES * SN_POWERS;
+  return p < r.octaves ? __float_as_uint(fmaf(p, 8.f * SN_POWERS, r.base + 8.f)) & ~7u : 0u;
 }
-__device__ __forceinline__ unsigned sn_step(const SnRow& r, float z) { return (unsigned)sn_place(r, z) >> SN_STEP; }
-// e^((z - max) / T) over 2^-44 (2^-bits) as a whole number, within three of it (2.6 of 6 million, without a bias), in 32-bit arithmetic (an instruction of 64-bit floating point is some
-// 20 cycles of a scheduler).  With d = max - z and c = 1 / (T log 2), each a sum of two float32 numbers, y = c d is one to 2^-47 of itself; with
-// ``place`` k of it taken away x / log 2 is left, and the result is 2^(-k / 4096) (1 - x + x^2 / 2 - x^3 / 6), |x| < 2^-13.
-__device__ __forceinline__ unsigned long long sn_weight(const SnRow& r, float z, int k) {
+// steps of the first histogram: 128 of them; none (SN_BINS and more) for what has no place
+__device__ __forceinline__ unsigned sn_step(const SnRow& r, unsigned place) { return (place >> (SN_STEP + 3)) - r.first_step; }
+// e^((z - max) / T) over 2^-45 (2^-41 for long rows) as a whole number, -5.2 to 1.2 of it off, in 32-bit arithmetic (an instruction of 64-bit
+// floating point is some 20 cycles of a scheduler; whole numbers go through at half of floating point's rate).  With d = max - z and
+// c = 1 / (T log 2), each a sum of two float32 numbers, y = c d is one to 2^-47 of itself; x / log 2 = j / 4096 - y is what the place lies behind it,
+// up to 8.7 / 32768, and the result is 2^(-j / 4096) (1 + x + x^2 / 2 + x^3 / 6), of a power with 31 bits beside x.
+__device__ __forceinline__ unsigned long long sn_weight(const SnRow& r, float z, unsigned place) {
   const float d = r.top - z, back = d - r.top, d2 = (r.top - (d - back)) - (z + back);       // (what the difference lost)
   const float p = d * r.c;
   const float e = fmaf(d2, r.c, fmaf(d, r.c2, fmaf(d, r.c, -p)));
-  const float f = fmaf(__int_as_float(k + 0x4b400000) - 12582912.f, -1.f / SN_POWERS, p), y = f + e, y2 = e - (y - f);
+  const float j = (__uint_as_float(place) - r.base) * (1.f / (8 * SN_POWERS)), f = j - p, y = f - e, y2 = ((f - y) - e) + ((j - f) - p);
   const float x = y * 0.693147182f, x2 = fmaf(y2, 0.693147182f, fmaf(y, -1.90465421e-9f, fmaf(y, 0.693147182f, -x)));
-  const float rest = fmaf(x * x, fmaf(x, 1.f / 6, -0.5f), x2);
-  const int less = __float2int_rn(x * 17592186044416.f) + (__float_as_int(fmaf(rest, 17592186044416.f, 12582912.f)) - 0x4b400000);       // over 2^-44
-  const unsigned long long w = r.powers[k & (SN_POWERS - 1)];
-  const unsigned long long whole = w - (long long)(int)(((long long)(int)(w >> 14) * less + (1 << 29)) >> 30);
-  const int down = 44 - r.bits + (k / SN_POWERS);
-  return k < SN_OCTAVES * SN_POWERS ? whole + (1ull << down >> 1) >> down : 0ull;
+  const float a = fmaf(x, 2147483648.f, 12582912.f), left = fmaf(a - 12582912.f, -1.f / 2147483648.f, x);
+  const float b = fmaf(left + fmaf(x * x, fmaf(x, 1.f / 6, 0.5f), x2), 17592186044416.f, 12582912.f);
+  const unsigned more = (__float_as_uint(a) << 13) + __float_as_uint(b) - ((0x4b400000u << 13) + 0x4b400000u);               // e^x - 1 over 2^-44
+  const unsigned long long w = *reinterpret_cast<const unsigned long long*>(reinterpret_cast<const unsigned char*>(r.powers) + (place & 8 * (SN_POWERS - 1)));
+  return (w + ((w >> 32) * more >> 12)) >> (place >> 15 & 63);
 }
 // (one copy of the code for what is asked for seldom: a launch goes through most of its code once, and waits for it where it is long)
-__device__ __noinline__ unsigned long long sn_weight_once(const SnRow& r, float z) { return sn_weight(r, z, sn_place(r, z)); }
-// the least weight that min_p leaves
-__device__ __forceinline__ unsigned long long sn_least(const SnRow& r, float min_p) {
-  return (unsigned long long)ceil(fmin((double)min_p, 1.0) * (double)(1ull << r.bits));
+__device__ __noinline__ unsigned long long sn_weight_once(const SnRow& r, float z) {
+  const unsigned place = sn_place(r, z);
+  return place ? sn_weight(r, z, place) : 0;
 }
-
 // a share of a sum, in whole weights, ``least`` or more
 __device__ __forceinline__ unsigned long long sn_part(unsigned long long total, float share, unsigned long long least) {
   return max(__double2ull_ru(fmax((double)share, 0.0) * (double)total), least);
+}
+// the least weight that min_p leaves
+__device__ __forceinline__ unsigned long long sn_least(const SnRow& r, float min_p) {
+  return sn_part(sn_weight_once(r, r.top), fminf(min_p, 1.f), 0);
 }
 
 // every CTA's word, in every CTA.  Calls in turn use two places, so that a fast CTA's next word does not meet a slow one's reading.
@@ -212,7 +218,7 @@ __device__ __forceinline__ W sn_sum_with(int n, int each, F word) {
 }
 // a logit of the step that a border lies in, to the list
 __device__ __noinline__ void sn_put(const SnRow& r, float z, unsigned bin, int* count, unsigned* near) {
-  if (sn_step(r, z) != bin) return;
+  if (sn_step(r, sn_place(r, z)) != bin) return;
   const int at = atomicAdd(count, 1);
   if (at < SN_LIST) near[at] = sn_order(z);
 }
@@ -260,9 +266,9 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
       if (level == 0) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const int k = v[j] >= from_z ? sn_place(r, v[j]) : SN_OCTAVES * SN_POWERS;
-          bin[j] = k < SN_OCTAVES * SN_POWERS ? (unsigned)k >> SN_STEP : SN_BINS;
-          if (MASS) w[j] = sn_weight(r, v[j], k);
+          const unsigned place = v[j] >= from_z ? sn_place(r, v[j]) : 0u;
+          bin[j] = sn_step(r, place);
+          if (MASS) w[j] = sn_weight(r, v[j], place);      // (of no use without a place)
         }
       } else {
 #pragma unroll
@@ -338,9 +344,9 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
       // the step's logits to the first CTA, in any order
       int* count = shares > 1 ? cg::this_cluster().map_shared_rank(&s.listed, 0) : &s.listed;
       unsigned* near = shares > 1 ? cg::this_cluster().map_shared_rank(s.near, 0) : s.near;
-      // (about where the step lies, its ends a 256th of it further out and by what the terms of y can have lost: few are looked at closely)
-      const float wide = (float)(1 << SN_STEP) / SN_POWERS / r.c, out = wide * (1.f / 256) + fabsf(r.top) * 2.4e-7f + ((float)bin + 1.f) * wide * 2.4e-7f;
-      const float lo_z = fmaxf(from_z, r.top - ((float)bin + 1.f) * wide - out), hi_z = fminf(to_z, r.top - ((float)bin - 1.f / 256) * wide + out);
+      // (about where the step lies, its ends a 64th of it further out and by what the terms of y can have lost: few are looked at closely)
+      const float wide = (float)(1 << SN_STEP) / SN_POWERS / r.c, out = wide * (1.f / 64) + fabsf(r.top) * 2.4e-7f + ((float)bin + 1.f) * wide * 2.4e-7f;
+      const float lo_z = fmaxf(from_z, r.top - ((float)bin + 1.f) * wide - out), hi_z = fminf(to_z, r.top - (float)bin * wide + out);
       for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD) {
         float v[SN_AHEAD][4];
         sn_ahead(r, i0, v);
@@ -372,7 +378,8 @@ __device__ unsigned sn_border(SnShared& s, const SnRow& r, int shares, unsigned 
       // the keys of this step of z, by bisection of the very expression: the first of the step, the first behind it
       if (warp < 2) {
         const unsigned end = sn_first_key(k_lo - 1, top + 1, [&](unsigned key) {
-          return key > top || (warp ? sn_step(r, sn_value(key)) < bin : sn_step(r, sn_value(key)) <= bin);
+          const unsigned step = sn_step(r, sn_place(r, sn_value(key)));
+          return key > top || (warp ? step < bin : step <= bin);
         });
         if (lane == 0) s.ends[warp] = end;
       }
@@ -529,7 +536,9 @@ __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnA
   r.warp_from = min(warp * per_warp, r.n);
   r.warp_to = min(r.warp_from + per_warp, r.n);
   r.powers = s.powers;
-  r.bits = a.bits;
+  r.base = 12582912.f + (float)(SN_DOWN + a.wide) * 8 * SN_POWERS;
+  r.octaves = (float)(SN_OCTAVES - a.wide);
+  r.first_step = __float_as_uint(r.base) >> (SN_STEP + 3);
   if (threadIdx.x == 0) s.listed = 0;
 #pragma unroll
   for (int i = threadIdx.x; i < SN_POWERS / 2; i += SN_THREADS) reinterpret_cast<ulonglong2*>(s.powers)[i] = reinterpret_cast<const ulonglong2*>(sn_powers.of)[i];
@@ -631,7 +640,8 @@ __global__ void __launch_bounds__(SN_THREADS, 1) sample_nucleus_kernel(const SnA
         const int n = min(held, 32);
         held -= n;
         const float z = found[held + min(lane, n - 1)];
-        if (lane < n) sum += sn_weight(r, z, sn_place(r, z));
+        const unsigned place = sn_place(r, z);
+        if (lane < n && place) sum += sn_weight(r, z, place);
       }
       __syncwarp();
     }
@@ -707,7 +717,7 @@ extern "C" int qd_sample_nucleus(const float* logits, long long ld, int R, int V
                                  const float* min_p, const float* draws, int* out, int only, int sms, cudaStream_t stream) {
   if (R <= 0) return 0;
   if (V <= 0 || V > QD_NUCLEUS_MAX_VOCABULARY || sms < 1) return QD_ERR_UNSUPPORTED;
-  SnArgs a = {logits, ld, temperature, top_p, min_p, draws, top_k, out, V, 1, 0, 0, 0, V > 1 << 18 ? 40 : 44, only};
+  SnArgs a = {logits, ld, temperature, top_p, min_p, draws, top_k, out, V, 1, 0, 0, 0, V > 1 << 18 ? 4 : 0, only};
   a.vec = !((uintptr_t)logits & 15) && ld % 4 == 0;
   const size_t fixed = (sizeof(SnShared) + 15) / 16 * 16, most = fixed + SN_KEEP * 4;
   static bool allowed[64];
