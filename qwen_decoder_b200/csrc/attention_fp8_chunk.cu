@@ -11,9 +11,10 @@
 //   largest, and off by 2^-23 of that below.  Two products of 128 features in 8 bits take the tensor cores as long as one of bfloat16.
 // * Values become float16, an e4m3 number's scale over the tile's largest one, E, included, which is exact down to 2^-15 E: four warps take tiles from
 //   where the copies leave them to where the product reads them.  P is float16 too, 2^(z + log E - reference): the product's sums are of
-//   values as they are, a row's sum of weights takes a tile's over E.  P is scaled so that 2^8 stands for the largest weight at the time its
+//   values as they are, and a row's sum of exponentials has a maximum of its own.  P is scaled so that 2^8 stands for the largest weight at the time its
 //   reference was taken, and is off by 2^-12 of itself, or by 2^-33 of that weight where that is more.  Where a tile has a scale below 2^-15 of the
-//   largest one up to it, values and P are bfloat16 from there on as long as that is so, whose exponents take anything.  (P in 8 bits would
+//   largest one up to it, values and P are bfloat16 as long as that is so, whose exponents take anything (E is 2^-60 of that largest one or more
+//   then, so that no exponential is lost that a row's sum has).  (P in 8 bits would
 //   be two numbers as q is, for every weight; this is 16 KB of values to a tile for all 128 rows.  Values to bfloat16, for every tile, took
 //   twice the instructions: 2,048 tokens behind 6,144 420 us.)  These warps also bring the keys' scales to tensor memory.
 // * A key or value that is no number has the scale 255.  The value becomes zeros, its key's scale 255, so that the score is none and
@@ -46,6 +47,8 @@
 #define AC_HOLES 512u                  // and: some of the values are nobody's or no numbers
 #define AC_AHEAD 8                     // tiles of whose scales something is kept
 #define AC_SPREAD 15                   // powers of two between scales up to which they are float16
+#define AC_DEEP 60                     // and what a tile's largest one is taken to be below the largest of all at most
+#define AC_NONE (-1e30f)               // the maximum of no scores
 #define AC_REGS 128                    // a thread's at the launch; the host looks that it is so: a split that adds up to more waits for ever
 #define AC_REGS_SOFTMAX 184            // 2 x 184 + 56 + 88 = 4 x 128
 #define AC_REGS_ISSUE 56
@@ -58,10 +61,10 @@ struct AcParams {
   const unsigned char* pages; long long page_bytes; int n_pages;
   const int* table; int max_blocks;
   const int *cu, *start;
-  int R, H, G, ps, ps_shift, window, tok_tile;      // ps_shift: log2 of ps, or -1
+  int R, rows, H, G, ps, ps_shift, window, tok_tile;      // ps_shift: log2 of ps, or -1
   float scale_log2e;
   // Pairs of a tile of rows and a KV head, the longest first; the ones before ``whole`` are a CTA's each, those behind it ``shares`` CTAs', which
-  // leave their sums: [pair][share][128][HD], [pair][share][128][2]: reference, sum of weights
+  // leave their sums: [pair][share][128][HD], [pair][share][128][4]: reference, maximum of scores, sum of exponentials
   int tiles, whole, shares;
   float *part_o, *part_s;
   int* status;
@@ -70,18 +73,19 @@ struct AcParams {
 // A pair's rows: which request, which of its tokens (tiles numbered request by request)
 struct AcRows { int r, tok0, n_tok, pos0; };
 __device__ __forceinline__ AcRows ac_rows(const AcParams& p, const int* cu, const int* sp, int pair) {
+  auto row_at = [&](int r) { return min(max(cu[r], 0), p.rows); };      // (no row is touched that is none, whatever the list says)
   const int b = p.tiles - 1 - pair / p.G;
   AcRows a = {0, 0, 0, 0};
   int before = 0;
   for (; a.r < p.R; a.r++) {
-    const int nt = (cu[a.r + 1] - cu[a.r] + p.tok_tile - 1) / p.tok_tile;
+    const int nt = (row_at(a.r + 1) - row_at(a.r) + p.tok_tile - 1) / p.tok_tile;
     if (b < before + nt) break;
     before += nt;
   }
   if (a.r < p.R) {                     // (else: no rows)
-    a.tok0 = cu[a.r] + (b - before) * p.tok_tile;
-    a.n_tok = min(p.tok_tile, cu[a.r + 1] - a.tok0);
-    a.pos0 = sp[a.r] + (a.tok0 - cu[a.r]);
+    a.tok0 = row_at(a.r) + (b - before) * p.tok_tile;
+    a.n_tok = min(p.tok_tile, row_at(a.r + 1) - a.tok0);
+    a.pos0 = sp[a.r] + (b - before) * p.tok_tile;
   }
   return a;
 }
@@ -113,6 +117,12 @@ __device__ __forceinline__ bool ac_done(unsigned long long* bar, unsigned parity
 __device__ __forceinline__ unsigned ac_halves(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const unsigned*>(&h);
+}
+// 2^x, subnormal numbers included
+__device__ __forceinline__ float ac_power(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // two e4m3 numbers times two float16 numbers
 __device__ __forceinline__ unsigned ac_f16x2(unsigned short two, unsigned f) {
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   const int r = rows.r, tok0 = rows.tok0, n_tok = rows.n_tok, pos0 = rows.pos0;
   const int key_hi = pos0 + n_tok, key_lo = ac_key_lo(p, pos0);
   // of the tiles from the first row's first key to the last row's last, this share's
-  const int t0 = key_lo / AC_KEYS, tn = idle ? 0 : (key_hi + AC_KEYS - 1) / AC_KEYS - t0;
+  const int t0 = key_lo / AC_KEYS, tn = idle ? 0 : max((key_hi + AC_KEYS - 1) / AC_KEYS - t0, 0);
   const int kt_lo = t0 + (int)((long long)tn * share / shares), n_kt = t0 + (int)((long long)tn * (share + 1) / shares) - kt_lo;
   const int* table = p.table + (long long)(idle ? 0 : r) * p.max_blocks;
   // of a key: its page's entry in the table, for whoever needs it a tile later (keys that are none: any page will do); the page; the place in it
@@ -262,7 +272,8 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) tc_arrive(&q_full);
     }
-    float m = -INFINITY, l = 0.f;        // m: the maximum that this row's exponentials, sum and output refer to
+    // m: the maximum that this row's weights and output refer to; z: of its scores so far, which the sum of its exponentials refers to
+    float m = -INFINITY, z = AC_NONE, l = 0.f;
     const int free_hi = pos0 + 1, free_lo = ac_key_lo(p, key_hi - 1);       // keys that every row sees need no test
     bool ready = false;                  // the next tile's scores are there: looked at ahead, since the answer takes 200 to 300 cycles
     for (int j = 0; j < n_kt; j++) {
@@ -313,14 +324,13 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       // Weights first, against the reference as it is; the other thread's maximum then seldom says that it has to move (the first tile's always).
       if (j > 0) weigh();
       asm volatile("bar.sync %0, 64;" ::"r"(3 + (warp & 3)) : "memory");       // the two warps of these rows
-      const float m_tile = fmaxf(mx, mx_s[j & 1][h ^ 1][row]) + top;           // of weights with the largest of the tile's scales
+      const float z_tile = fmaxf(mx, mx_s[j & 1][h ^ 1][row]), m_tile = z_tile + top;       // of weights with the largest of the tile's scales
       // the row moves to a new reference only when its maximum has grown by more than AC_GROW (always from "no key yet"); both threads of a
       // row decide alike, and the warp acts together
       const bool grow = m_tile > m + AC_GROW;
       if (__any_sync(0xffffffffu, grow) || j == 0) {
         const float alpha = grow ? at_exp2(m - m_tile) : 1.0f;
         if (grow) m = m_tile;
-        l *= alpha;
         if (j > 0) {
           if (!tc_wait_inline(&o_done, (j - 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 8);
           __syncwarp();
@@ -337,7 +347,9 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         }
         weigh();
       }
-      l = fmaf(sum, __uint_as_float((254u - (tile & 255u)) << 23), l);
+      const float z_new = fmaxf(z, z_tile);          // (the difference is bounded where there is a sum)
+      l = fmaf(sum, at_exp2(fminf((m == -INFINITY ? 0.f : m) - top - z_new, 100.f)), l * at_exp2(z - z_new));
+      z = z_new;
       at_tmem_st<KQ / 2>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * KQ, pk);      // over the first half of this thread's own scores
       tc_fence_before();
       __syncwarp();
@@ -353,7 +365,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
     const float l_all = l + l_s[h ^ 1][row];
     if (shares > 1) {
       const long long at = (long long)behind * AC_ROWS + row;
-      if (ok && h == 0) *reinterpret_cast<float2*>(p.part_s + 2 * at) = make_float2(m, l_all);
+      if (ok && h == 0) *reinterpret_cast<float4*>(p.part_s + 4 * at) = make_float4(m, z, l_all, 0.f);
       if (n_kt > 0) {
 #pragma unroll
         for (int c = 0; c < DH; c += 32) {
@@ -366,21 +378,26 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           }
         }
       }
-    } else if (n_kt > 0) {
-      const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+    } else {
+      const float inv = l_all == 0.f ? 0.f : 1.f / l_all, up = ac_power(m - z);
       bf16* d = p.out + (long long)(tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + h * DH;
 #pragma unroll
       for (int c = 0; c < DH; c += 32) {
         float ov[32];
-        at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);
+        if (n_kt > 0) {
+          at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);
+        } else {                                     // (rows in front of the first position)
+#pragma unroll
+          for (int i = 0; i < 32; i++) ov[i] = 0.f;
+        }
         if (ok) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint4 v;
-            v.x = at_pack(ov[i] * inv, ov[i + 1] * inv);
-            v.y = at_pack(ov[i + 2] * inv, ov[i + 3] * inv);
-            v.z = at_pack(ov[i + 4] * inv, ov[i + 5] * inv);
-            v.w = at_pack(ov[i + 6] * inv, ov[i + 7] * inv);
+            v.x = at_pack(ov[i] * inv * up, ov[i + 1] * inv * up);
+            v.y = at_pack(ov[i + 2] * inv * up, ov[i + 3] * inv * up);
+            v.z = at_pack(ov[i + 4] * inv * up, ov[i + 5] * inv * up);
+            v.w = at_pack(ov[i + 6] * inv * up, ov[i + 7] * inv * up);
             *reinterpret_cast<uint4*>(d + c + i) = v;
           }
         }
@@ -522,9 +539,10 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           most = __reduce_max_sync(0xffffffffu, most);
           least = __reduce_min_sync(0xffffffffu, least);
           all = __all_sync(0xffffffffu, all);
-          if (most == 0) least = 127;                 // (no value that is seen)
-          most = most ? most - 1 : 127u;
+          if (most == 0) least = most = largest ? largest : 127u;            // (no value that is seen)
+          else most--;
           largest = max(largest, most);
+          most = max(most, largest - min(largest, (unsigned)AC_DEEP));
           const bool wide = largest - least > AC_SPREAD;
           unsigned f[4];
 #pragma unroll
@@ -619,20 +637,25 @@ __global__ void __launch_bounds__(AC_JOIN_ROWS * HD / 4) chunk_fp8_join_kernel(c
   const int t = row / gs, hh = row - t * gs;
   if (rows.r == p.R || t >= rows.n_tok) return;
   const long long first = (long long)behind * p.shares * AC_ROWS + row;
-  float m = -INFINITY, l = 0.f;
-  for (int s = 0; s < p.shares; s++) m = fmaxf(m, __ldcg(p.part_s + 2 * (first + s * AC_ROWS)));
+  float m = -INFINITY, z = AC_NONE, l = 0.f;
+  for (int s = 0; s < p.shares; s++) {
+    const float2 st = __ldcg(reinterpret_cast<const float2*>(p.part_s + 4 * (first + s * AC_ROWS)));
+    m = fmaxf(m, st.x);
+    z = fmaxf(z, st.y);
+  }
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int s = 0; s < p.shares; s++) {
-    const float2 st = __ldcg(reinterpret_cast<const float2*>(p.part_s + 2 * (first + s * AC_ROWS)));
-    if (st.x == -INFINITY) { l += st.y; continue; }           // (no key, whose sums were not written, or no numbers)
+    const float4 st = __ldcg(reinterpret_cast<const float4*>(p.part_s + 4 * (first + s * AC_ROWS)));
+    l = fmaf(st.z, at_exp2(st.y - z), l);
+    if (st.x == -INFINITY) continue;             // (no key, whose sums were not written, or no numbers)
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (first + s * AC_ROWS) * HD + f));
     const float x = at_exp2(st.x - m);
-    l = fmaf(st.y, x, l);
     o.x = fmaf(v.x, x, o.x); o.y = fmaf(v.y, x, o.y); o.z = fmaf(v.z, x, o.z); o.w = fmaf(v.w, x, o.w);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + (rows.tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + f) = make_uint2(at_pack(o.x * inv, o.y * inv), at_pack(o.z * inv, o.w * inv));
+  const float inv = l == 0.f ? 0.f : 1.f / l, up = ac_power(m - z);
+  *reinterpret_cast<uint2*>(p.out + (rows.tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + f) =
+      make_uint2(at_pack(o.x * inv * up, o.y * inv * up), at_pack(o.z * inv * up, o.w * inv * up));
 }
 
 // ------------------------------------------------------------------------------------ host
@@ -674,7 +697,7 @@ static AcPlan ac_plan(int T, int R, int H, int G, int window, int max_keys, int 
 extern "C" long long qd_prefill_attention_fp8_scratch(int T, int R, int H, int G, int d, int window, int max_keys, int sms) {
   if (T < 1 || R < 1 || G < 1 || H < G) return 0;
   const AcPlan plan = ac_plan(T, R, H, G, window, max_keys, sms);
-  return (plan.tiles * G - plan.whole) * plan.shares * AC_ROWS * (d + 2);
+  return (plan.tiles * G - plan.whole) * plan.shares * AC_ROWS * (d + 4);
 }
 
 template <int HD>
@@ -716,7 +739,7 @@ extern "C" int qd_prefill_attention_fp8(const void* q, long long ldq, void* out,
   const long long behind = plan.tiles * G - plan.whole, ctas = plan.whole + behind * plan.shares;
   if (ctas > 0x7fffffffll || behind * (AC_ROWS / AC_JOIN_ROWS) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   const AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, c8_page_bytes(G, ps, d), (int)n_pages, table, max_blocks, cu,
-                      start, R, H, G, ps, ps & (ps - 1) ? -1 : __builtin_ctz(ps), window, AC_ROWS / (H / G), scale * 1.4426950408889634f,
+                      start, R, rows, H, G, ps, ps & (ps - 1) ? -1 : __builtin_ctz(ps), window, AC_ROWS / (H / G), scale * 1.4426950408889634f,
                       (int)plan.tiles, (int)plan.whole, plan.shares, scratch, scratch + behind * plan.shares * AC_ROWS * d, status};
   return d == 64 ? ac_launch<64>(map, p, stream) : ac_launch<128>(map, p, stream);
 }

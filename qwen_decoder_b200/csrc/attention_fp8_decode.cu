@@ -15,8 +15,7 @@
 //   A key's scale multiplies its score.
 // * A value's scale joins its weight: with w_k = z_k / log 2 + s_v, the weights are 2^(w_k - W), W their own running maximum beside the
 //   scores'.  So they are numbers up to 2^8 (both maxima are followed when they grow by more than 2^8), rounded to float16 by 2^-12
-//   of themselves, and by 2^-25 of the largest where that is more: 2^-17 of a float16's distance from bfloat16, whatever the scales.  Sums are
-//   float32.
+//   of themselves, and by 2^-25 of one where that is more (weights below 2^-13), whatever the scales.  Sums are float32.
 // * Work, where there is much: the keys of all (token, KV head) pairs, in units of 128 (a CTA's eight warps, 16 each), are one list; every CTA
 //   takes an equal, contiguous share of it, found from the tokens' positions alone, so that the lengths may differ as they like and a
 //   graph's replay needs nothing of the host.  A pair whose keys are one CTA's is finished by it; the others leave their sums in float32, at
@@ -164,8 +163,12 @@ __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scrat
   return list;
 }
 
-// What the sum of weighted values is multiplied by
-__device__ __forceinline__ float da_inverse(float sum, float mz, float mw) { return sum == 0.f ? 0.f : da_exp2(mw - mz) / sum; }
+// What the sum of weighted values is multiplied by, one after the other (together they may be no normal number): 1 / sum, 2^(mw - mz)
+__device__ __forceinline__ float2 da_inverse(float sum, float mz, float mw) {
+  float up;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(up) : "f"(mw - mz));
+  return make_float2(sum == 0.f ? 0.f : 1.f / sum, up);
+}
 
 // Sums of pieces of a pair together: of the exponentials (their sum and maximum), of the weighted values (and their maximum).
 struct DaJoin {
@@ -179,10 +182,10 @@ struct DaJoin {
     mz = z;
     mw = w;
   }
-  __device__ __forceinline__ float inverse() const { return da_inverse(sum, mz, mw); }
+  __device__ __forceinline__ float2 inverse() const { return da_inverse(sum, mz, mw); }
 };
-__device__ __forceinline__ void da_store(bf16* to, float4 s, float inv) {
-  const __nv_bfloat162 x = __floats2bfloat162_rn(s.x * inv, s.y * inv), y = __floats2bfloat162_rn(s.z * inv, s.w * inv);
+__device__ __forceinline__ void da_store(bf16* to, float4 s, float2 by) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(s.x * by.x * by.y, s.y * by.x * by.y), y = __floats2bfloat162_rn(s.z * by.x * by.y, s.w * by.x * by.y);
   *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
 }
 
@@ -587,8 +590,8 @@ __global__ void __launch_bounds__(DA_THREADS) decode_fp8_join_kernel(const DaArg
   const long long U = (long long)list.all() * a.pages.G;
   n_ctas = da_taking(U, n_ctas);
   const int from = list.units_before(t) * a.pages.G + kvh * per, c0 = da_cta_of(U, n_ctas, from), c1 = da_cta_of(U, n_ctas, from + per - 1);
+  pdl_wait();                                  // (also where there is nothing to join: the next launch waits for this one alone)
   if (c0 == c1) return;
-  pdl_wait();
   const int f = threadIdx.x % LANES * 4, group = threadIdx.x / LANES;
   DaJoin j;
   j.none();

@@ -431,3 +431,76 @@ def test_prefill_wait_that_runs_out():
     with pytest.raises(kernels.KernelError, match="attention_fp8_chunk"):
         kernels.check_status()
     check_prefill([5], [0], 2, 1, 64)
+
+
+# ---- scales of values anywhere -----------------------------------------------------------------------------------
+
+def moved(pages, table, lengths, G, d, ps, by):
+    """The values' scales of keys [128 i, 128 (i + 1)) times 2^by[i], the last entry for all behind."""
+    pages = pages.clone()
+    scales = kernels.fp8_page_views(pages, G, ps, d)[1].view(torch.uint8)
+    for r, n in enumerate(lengths):
+        for key in range(n):
+            at = scales[int(table[r, key // ps]), :, key % ps, 1]
+            new = at.int() + by[min(key // 128, len(by) - 1)]
+            assert 1 <= int(new.min()) and int(new.max()) <= 254
+            at.copy_(new.to(torch.uint8))
+    return pages
+
+
+def both_kernels(q, pages, table, tokens, before, H, G, d, ps):
+    """Rows of the portions' kernel, and of the single tokens' one."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    reqs = [r for r, t in enumerate(tokens) for _ in range(t)]
+    positions = [b + i for b, t in zip(before, tokens) for i in range(t)]
+    q, pages, table = q.to(DEV), pages.to(DEV), table.to(DEV)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    kernels.prefill_attention_fp8(q, a, pages, table, i32([0] + tokens).cumsum(0).to(torch.int32), i32(before), H, G, d, ps, d ** -0.5)
+    kernels.decode_attention_fp8(q, b, pages, table, i32(reqs), i32(positions), H, G, d, ps, d ** -0.5)
+    kernels.check_status()
+    return reqs, positions, a.cpu().double(), b.cpu().double()
+
+
+@pytest.mark.parametrize("tokens,before", [([20, 3], [300, 0]), ([3], [4000])])
+@pytest.mark.parametrize("by", [-110, 60, 120])
+@pytest.mark.parametrize("H,G,d", [(8, 2, 128), (4, 2, 64)])
+def test_values_times_a_power_of_two(guard_regions, H, G, d, by, tokens, before):
+    gen, ps = torch.Generator().manual_seed(21), 16
+    lengths = [b + t for b, t in zip(before, tokens)]
+    pages, table = a_cache(gen, lengths, G, ps, d)
+    q = torch.randn((sum(tokens), H * d), generator=gen).bfloat16()
+    reqs, positions, *got = both_kernels(q, moved(pages, table, lengths, G, d, ps, [by]), table, tokens, before, H, G, d, ps)
+    for out, step in zip(got, (plain.BF16_HALF_STEP, plain.FP16_HALF_STEP)):
+        want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, 0, step)
+        # a score and its value's scale add up to numbers below 256, three roundings of 2^-17 each: 3% of a weight's own 2^-11; bfloat16's least step
+        assert bool(((out - want * 2.0 ** by).abs() <= bound * 2.0 ** by * (1 + 2.0 ** -4) + 2.0 ** -133).all())
+
+
+@pytest.mark.parametrize("by", [[0, -110, 0], [-110, 0], [0, 0, -110], [-110, 100, -60], [100, -110], [20, -20, 0, 20]])
+@pytest.mark.parametrize("tokens,before", [([20, 3], [500, 90]), ([3], [4000])])
+def test_values_of_keys_far_apart(guard_regions, tokens, before, by):
+    """Values that are next to nothing beside others take their share of the softmax all the same."""
+    gen, H, G, d, ps = torch.Generator().manual_seed(22), 8, 2, 128, 16
+    lengths = [b + t for b, t in zip(before, tokens)]
+    pages, table = a_cache(gen, lengths, G, ps, d)
+    pages = moved(pages, table, lengths, G, d, ps, by)
+    q = torch.randn((sum(tokens), H * d), generator=gen).bfloat16()
+    reqs, positions, *got = both_kernels(q, pages, table, tokens, before, H, G, d, ps)
+    for out, step in zip(got, (plain.BF16_HALF_STEP, plain.FP16_HALF_STEP)):
+        want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, 0, step)
+        assert bool(((out - want).abs() <= bound * (1 + 2.0 ** -4)).all()), float(((out - want).abs() / bound).max())
+
+
+def test_prefill_rows_before_the_first_position(guard_regions):
+    """Rows at positions below zero see nothing: zeros; a list of rows that ends behind q's is cut."""
+    gen, H, G, d, ps = torch.Generator().manual_seed(23), 4, 2, 64, 16
+    pages, table = a_cache(gen, [40, 30], G, ps, d)
+    q = torch.randn((60, H * d), generator=gen).bfloat16()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    for cu, start, tokens in (([0, 40, 60], [-7, 5], (40, 20)), ([0, 45, 60], [-200, 0], (45, 15)), ([0, 40, 90], [0, 5], (40, 20))):
+        out = torch.full_like(q, 7.0).to(DEV)
+        kernels.prefill_attention_fp8(q.to(DEV), out, pages.to(DEV), table.to(DEV), i32(cu), i32(start), H, G, d, ps, d ** -0.5)
+        kernels.check_status()
+        reqs, positions = [0] * tokens[0] + [1] * tokens[1], [start[r] + i for r, t in enumerate(tokens) for i in range(t)]
+        want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, 0, plain.BF16_HALF_STEP)
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
