@@ -74,11 +74,11 @@ struct AcParams {
 struct AcRows { int r, tok0, n_tok, pos0; };
 __device__ __forceinline__ AcRows ac_rows(const AcParams& p, const int* cu, const int* sp, int pair) {
   auto row_at = [&](int r) { return min(max(cu[r], 0), p.rows); };      // (no row is touched that is none, whatever the list says)
-  const int b = p.tiles - 1 - pair / p.G;
+  const int b = p.tiles - 1 - (int)((unsigned)pair / (unsigned)p.G);
   AcRows a = {0, 0, 0, 0};
   int before = 0;
   for (; a.r < p.R; a.r++) {
-    const int nt = (row_at(a.r + 1) - row_at(a.r) + p.tok_tile - 1) / p.tok_tile;
+    const int nt = (int)((unsigned)(max(row_at(a.r + 1) - row_at(a.r), 0) + p.tok_tile - 1) / (unsigned)p.tok_tile);
     if (b < before + nt) break;
     before += nt;
   }
@@ -194,16 +194,18 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
   const unsigned tmem = tmem_slot;
 
   // ---- which rows, and which share of their keys
-  const int behind = (int)blockIdx.x - p.whole, pair = behind < 0 ? blockIdx.x : p.whole + behind / p.shares, share = behind < 0 ? 0 : behind % p.shares;
+  const int behind = (int)blockIdx.x - p.whole, pair = behind < 0 ? blockIdx.x : p.whole + (unsigned)behind / (unsigned)p.shares;
+  const int share = behind < 0 ? 0 : (unsigned)behind % (unsigned)p.shares;
   const int shares = behind < 0 ? 1 : p.shares;
-  const int g = pair % p.G, gs = p.H / p.G;
+  const int g = (unsigned)pair % (unsigned)p.G, gs = (unsigned)p.H / (unsigned)p.G;
   const AcRows rows = ac_rows(p, staged ? cu_s : p.cu, staged ? sp_s : p.start, pair);
   const bool idle = rows.r == p.R;
   const int r = rows.r, tok0 = rows.tok0, n_tok = rows.n_tok, pos0 = rows.pos0;
   const int key_hi = pos0 + n_tok, key_lo = ac_key_lo(p, pos0);
   // of the tiles from the first row's first key to the last row's last, this share's
   const int t0 = key_lo / AC_KEYS, tn = idle ? 0 : max((key_hi + AC_KEYS - 1) / AC_KEYS - t0, 0);
-  const int kt_lo = t0 + (int)((long long)tn * share / shares), n_kt = t0 + (int)((long long)tn * (share + 1) / shares) - kt_lo;
+  // (2^24 tiles and 64 shares at most: 32 bits, whose quotients are a third of the way)
+  const int kt_lo = t0 + (int)((unsigned)(tn * share) / (unsigned)shares), n_kt = t0 + (int)((unsigned)(tn * (share + 1)) / (unsigned)shares) - kt_lo;
   const int* table = p.table + (long long)(idle ? 0 : r) * p.max_blocks;
   // of a key: its page's entry in the table, for whoever needs it a tile later (keys that are none: any page will do); the page; the place in it
   auto entry_at = [&](int key) {
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
     // ------------------------------------------------------------------ softmax: two threads to a row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AC_REGS_SOFTMAX));
     const int row = (warp & 3) * 32 + lane, h = warp >> 2;          // row: also the lane of tensor memory
-    const int t = row / gs, hh = row - t * gs;
+    const int t = (unsigned)row / (unsigned)gs, hh = row - t * gs;
     const bool ok = !idle && t < n_tok;
     const int pos = pos0 + t, lo = ac_key_lo(p, pos);
     const unsigned t_lane = tmem + ((unsigned)((warp & 3) * 32) << 16);
@@ -638,20 +640,18 @@ __global__ void __launch_bounds__(AC_JOIN_ROWS * HD / 4) chunk_fp8_join_kernel(c
   if (rows.r == p.R || t >= rows.n_tok) return;
   const long long first = (long long)behind * p.shares * AC_ROWS + row;
   float m = -INFINITY, z = AC_NONE, l = 0.f;
-  for (int s = 0; s < p.shares; s++) {
-    const float2 st = __ldcg(reinterpret_cast<const float2*>(p.part_s + 4 * (first + s * AC_ROWS)));
-    m = fmaxf(m, st.x);
-    z = fmaxf(z, st.y);
-  }
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < p.shares; s++) {
     const float4 st = __ldcg(reinterpret_cast<const float4*>(p.part_s + 4 * (first + s * AC_ROWS)));
-    l = fmaf(st.z, at_exp2(st.y - z), l);
-    if (st.x == -INFINITY) continue;             // (no key, whose sums were not written, or no numbers)
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (first + s * AC_ROWS) * HD + f));
-    const float x = at_exp2(st.x - m);
-    o.x = fmaf(v.x, x, o.x); o.y = fmaf(v.y, x, o.y); o.z = fmaf(v.z, x, o.z); o.w = fmaf(v.w, x, o.w);
+    const float z_new = fmaxf(z, st.y);
+    l = fmaf(st.z, at_exp2(st.y - z_new), l * at_exp2(z - z_new));
+    z = z_new;
+    if (st.x == -INFINITY) continue;             // (no key, whose sums were not written, or no numbers)
+    const float m_new = fmaxf(m, st.x), x = at_exp2(st.x - m_new), y = at_exp2(m - m_new);
+    o.x = fmaf(v.x, x, o.x * y); o.y = fmaf(v.y, x, o.y * y); o.z = fmaf(v.z, x, o.z * y); o.w = fmaf(v.w, x, o.w * y);
+    m = m_new;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l, up = ac_power(m - z);
   *reinterpret_cast<uint2*>(p.out + (rows.tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + f) =
