@@ -32,6 +32,7 @@
 #include "tc5_ops.cuh"
 
 #include <cuda_fp16.h>
+#include <math.h>
 
 #define AC_SOFTMAX 256                 // threads
 #define AC_VALUES 128                  // threads that convert
@@ -641,17 +642,29 @@ __global__ void __launch_bounds__(AC_JOIN_ROWS * HD / 4) chunk_fp8_join_kernel(c
   const long long first = (long long)behind * p.shares * AC_ROWS + row;
   float m = -INFINITY, z = AC_NONE, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int s = 0; s < p.shares; s++) {
-    const float4 st = __ldcg(reinterpret_cast<const float4*>(p.part_s + 4 * (first + s * AC_ROWS)));
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (first + s * AC_ROWS) * HD + f));
-    const float z_new = fmaxf(z, st.y);
-    l = fmaf(st.z, at_exp2(st.y - z_new), l * at_exp2(z - z_new));
-    z = z_new;
-    if (st.x == -INFINITY) continue;             // (no key, whose sums were not written, or no numbers)
-    const float m_new = fmaxf(m, st.x), x = at_exp2(st.x - m_new), y = at_exp2(m - m_new);
-    o.x = fmaf(v.x, x, o.x * y); o.y = fmaf(v.y, x, o.y * y); o.z = fmaf(v.z, x, o.z * y); o.w = fmaf(v.w, x, o.w * y);
-    m = m_new;
+  // (eight at a time are on their way: one after the other each is a trip to memory)
+  for (int s0 = 0; s0 < p.shares; s0 += 8) {
+    float4 st[8], v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const long long at = first + (s0 + u) * AC_ROWS;
+      st[u] = v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + u < p.shares) {
+        st[u] = __ldcg(reinterpret_cast<const float4*>(p.part_s + 4 * at));
+        v[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + f));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      if (s0 + u >= p.shares) break;
+      const float z_new = fmaxf(z, st[u].y);
+      l = fmaf(st[u].z, at_exp2(st[u].y - z_new), l * at_exp2(z - z_new));
+      z = z_new;
+      if (st[u].x == -INFINITY) continue;        // (no key, whose sums were not written, or no numbers)
+      const float m_new = fmaxf(m, st[u].x), x = at_exp2(st[u].x - m_new), y = at_exp2(m - m_new);
+      o.x = fmaf(v[u].x, x, o.x * y); o.y = fmaf(v[u].y, x, o.y * y); o.z = fmaf(v[u].z, x, o.z * y); o.w = fmaf(v[u].w, x, o.w * y);
+      m = m_new;
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l, up = ac_power(m - z);
   *reinterpret_cast<uint2*>(p.out + (rows.tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + f) =
@@ -675,9 +688,13 @@ static int* ac_status_word() {
 // How a launch is cut: pairs in all, those that are a CTA's each, the shares of the others
 struct AcPlan { long long tiles, whole; int shares; };
 // A CTA holds a multiprocessor.  What does not fill one round of them is shared out: all pairs where there are few, else those of the last
-// round (the shortest), by as many shares as make its time least: rounds of them over their number, each with AC_SHARE tiles of its own on top for
-// what a CTA costs besides its keys.
-#define AC_SHARE 4
+// round (the shortest), by as many shares as make its time least.  In tiles of keys (1.2 us each): rounds of what a share has, each with what a CTA
+// costs besides, and with shares the launch that joins them and their sums' way through memory.  (With 28 + 4 heads: 18 tokens behind 4,000, 4 pairs
+// of 32 tiles: 48.9 us whole, 22.7, 18.1, 16.7, 18.2 in 4, 8, 16, 24 shares; 37 behind 1,000, 12 of 9 tiles: 20.9, 17.5, 16.4, 16.9 in 1, 3, 5, 9;
+// 512 behind 300 with 16 + 2 heads, 64 of 7: 18.5, 22.7 in 1, 2; behind 1,500, 64 of 16: 29.6, 28.4.)
+#define AC_CTA 5.0
+#define AC_JOIN 2.5
+#define AC_SUMS (1.0 / 30)             // for each share
 static AcPlan ac_plan(int T, int R, int H, int G, int window, int max_keys, int sms) {
   const int tok_tile = AC_ROWS / (H / G);
   const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0), pairs = tiles * G;       // (of R requests at most)
@@ -685,9 +702,9 @@ static AcPlan ac_plan(int T, int R, int H, int G, int window, int max_keys, int 
   const double length = (double)keys / AC_KEYS;
   const long long rest = pairs % sms;
   AcPlan plan = {tiles, pairs, 1};
-  double best = length + AC_SHARE;
-  for (int s = 2; s <= 64 && rest && s * 4 <= length; s++) {
-    const double time = (double)((rest * s + sms - 1) / sms) * (length / s + AC_SHARE) + 2;             // (2: the launch that joins)
+  double best = ceil(length) + AC_CTA;
+  for (int s = 2; s <= 64 && rest && s <= length; s++) {
+    const double time = (double)((rest * s + sms - 1) / sms) * (ceil(length / s) + AC_CTA) + AC_JOIN + (double)(rest * s) * AC_SUMS;
     if (time < best) { best = time; plan.shares = s; plan.whole = pairs - rest; }
   }
   return plan;
