@@ -17,8 +17,8 @@
 //   scores'.  So they are numbers up to 2^8 (both maxima are followed when they grow by more than 2^8), rounded to float16 by 2^-12
 //   of themselves, and by 2^-25 of one where that is more (weights below 2^-13), whatever the scales.  Sums are float32.
 // * Work, where there is much: the keys of all (token, KV head) pairs, in units of 128 (a CTA's eight warps, 16 each), are one list; every CTA
-//   takes an equal, contiguous share of it, found from the tokens' positions alone, so that the lengths may differ as they like and a
-//   graph's replay needs nothing of the host.  A pair whose keys are one CTA's is finished by it; the others leave their sums in float32, at
+//   takes a contiguous share of it that takes as long as the others', found from the tokens' positions alone, so that the lengths may differ as they
+//   like and a graph's replay needs nothing of the host.  A pair whose keys are one CTA's is finished by it; the others leave their sums in float32, at
 //   most two pieces to a CTA, for ``decode_fp8_join``.  No counters are shared between launches.
 // * Where there is little, a pair is a cluster's, whose CTAs have equal shares of its units and join over their shared memories.
 #include "cache_fp8.cuh"
@@ -35,6 +35,8 @@ namespace cg = cooperative_groups;
 #define DA_UNIT (16 * DA_WARPS)            // keys
 #define DA_STAGES 2                        // of a warp's ring
 #define DA_MAX_CLUSTER 16
+#define DA_PIECE 3                         // units that a pair costs besides its own (128 tokens of up to 2,000 keys: 48 us without, 39 with 2 or 3, 41 with 4)
+#define DA_SNAP 1                          // units next to a pair's ends where it is not cut (64 of up to 300: 14.5 us without)
 #define DA_TOKENS 1024                     // of a launch that deals its units out
 #define DA_GROW 8.0f                       // powers of two by which a maximum grows before it is followed
 #define DA_NONE (-1e30f)                   // the maximum of no scores (a difference to it is a number, as one to minus infinity is not)
@@ -97,10 +99,23 @@ __device__ __forceinline__ int da_units(const DaArgs& a, int pos) {
   pos = min(pos, a.max_keys - 1);
   return (pos - (da_lo_key(a, pos) & ~15)) / DA_UNIT + 1;
 }
-// CTAs that take units, of those there are; CTA i of n takes units [i U / n, (i + 1) U / n)
+// What is dealt out are the keys' units and DA_PIECE more in front of them for each pair, which stand for what a pair costs besides.  CTAs that take
+// units, of those there are: CTA i of n takes those from i U / n on, or from where the pair begins or ends that lies near: a part of a pair costs its sums' way
+// through memory
 __device__ __forceinline__ int da_taking(long long U, int ctas) { return (int)(U < ctas ? U : ctas); }
-__device__ __forceinline__ int da_first(long long U, int n, int i) { return (int)(U * i / n); }
-__device__ __forceinline__ int da_cta_of(long long U, int n, int unit) { return (int)((((long long)unit + 1) * n - 1) / U); }
+__device__ __forceinline__ int da_cut(long long U, int n, int i) { return (int)(U * i / n); }
+// (``per``: units of the pair with those in front, ``of_pair``: of them before the cut)
+__device__ __forceinline__ int da_snap(int cut, int of_pair, int per) {
+  const bool start = per <= DA_PIECE + 2 * DA_SNAP + 1 ? 2 * of_pair <= per : of_pair <= DA_PIECE + DA_SNAP;
+  if (start) return cut - of_pair;
+  return per <= DA_PIECE + 2 * DA_SNAP + 1 || per - of_pair <= DA_SNAP ? cut + per - of_pair : cut;
+}
+// The CTAs that units [from, from + per) of a pair are cut between: the first of them and the last (none: not less)
+__device__ __forceinline__ int2 da_cut_by(long long U, int n, int from, int per) {
+  const long long a = (long long)from + DA_PIECE + DA_SNAP + 1, b = (long long)from + per - DA_SNAP;            // cuts in [a, b)
+  if (a >= b) return make_int2(0, 0);
+  return make_int2((int)((a * n + U - 1) / U) - 1, (int)((b * n + U - 1) / U) - 1);
+}
 
 // The list of all tokens' units.  Up to 32 tokens: in the registers of every warp, a lane to a token; more: in shared memory, made by the
 // whole block.
@@ -108,13 +123,13 @@ struct DaList {
   int few, T, before, units, pos;              // of this lane's token: units of those before it, its own, its position
   const int *sums, *positions;
   __device__ __forceinline__ int all() const { return few ? __shfl_sync(0xffffffffu, before + units, T - 1) : sums[T]; }
-  // the token that unit ``u`` of ``G`` times the list is of
+  // the token that unit ``u`` of ``G`` times the list is of: a whole warp looks, at every 32nd of them and then at 32 (one after the other by halves it
+  // was 900 cycles, at the beginning of every CTA)
   __device__ __forceinline__ int token(int u, int G) const {
-    if (few) return __popc(__ballot_sync(0xffffffffu, (threadIdx.x & 31) < T && before * G <= u)) - 1;
-    int t = 0;
-    for (int step = DA_TOKENS / 2; step > 0; step >>= 1)
-      if (t + step < T && (long long)sums[t + step] * G <= u) t += step;
-    return t;
+    const int lane = threadIdx.x & 31;
+    if (few) return __popc(__ballot_sync(0xffffffffu, lane < T && before * G <= u)) - 1;
+    const int from = 32 * (__popc(__ballot_sync(0xffffffffu, 32 * lane < T && sums[min(32 * lane, T)] * G <= u)) - 1);
+    return from + __popc(__ballot_sync(0xffffffffu, from + lane < T && sums[min(from + lane, T)] * G <= u)) - 1;
   }
   __device__ __forceinline__ int units_before(int t) const { return few ? __shfl_sync(0xffffffffu, before, t) : sums[t]; }
   __device__ __forceinline__ int units_of(int t) const { return few ? __shfl_sync(0xffffffffu, units, t) : sums[t + 1] - sums[t]; }
@@ -137,14 +152,14 @@ __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scrat
   list.positions = a.positions;
   if (list.few) {
     list.pos = lane < a.T ? a.positions[lane] : -1;
-    list.units = lane < a.T ? da_units(a, list.pos) : 0;
+    list.units = lane < a.T ? da_units(a, list.pos) + DA_PIECE : 0;
     list.before = scan(list.units) - list.units;
     return list;
   }
   int before = 0;
   for (int t0 = 0; t0 < a.T; t0 += DA_THREADS) {
     const int t = t0 + threadIdx.x;
-    const int u = t < a.T ? da_units(a, a.positions[t]) : 0;
+    const int u = t < a.T ? da_units(a, a.positions[t]) + DA_PIECE : 0;
     const int s = scan(u);
     if (lane == 31) scratch[warp] = s;
     __syncthreads();
@@ -192,14 +207,13 @@ __device__ __forceinline__ void da_store(bf16* to, float4 s, float2 by) {
 // a CTA's part of a pair's keys
 struct DaPiece {
   int t, kvh, per, u0, n;                      // token, KV head, units of the pair, the first and how many
-  int pos, lo, base;                           // keys [lo, pos]; units from ``base`` on
+  int pos, lo;                                 // keys [lo, pos]; units from the 16 keys on in which lo lies
   const int* table;
 };
-__device__ __forceinline__ void da_piece_keys(const DaArgs& a, DaPiece& p, int pos) {
+__device__ __forceinline__ void da_piece_keys(const DaArgs& a, DaPiece& p, int pos, int request) {
   p.pos = min(pos, a.max_keys - 1);
   p.lo = da_lo_key(a, p.pos);
-  p.base = p.lo & ~15;
-  p.table = a.table + (long long)min(max(a.token_req[p.t], 0), a.table_rows - 1) * a.max_blocks;
+  p.table = a.table + (long long)min(max(request, 0), a.table_rows - 1) * a.max_blocks;
 }
 
 template <int HD, int NT, bool CLUSTER>
@@ -235,7 +249,7 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
     const int pair = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;
     p.t = pair / G;
     p.kvh = pair % G;
-    da_piece_keys(a, p, a.positions[p.t]);
+    da_piece_keys(a, p, a.positions[p.t], a.token_req[p.t]);
     p.per = da_units(a, p.pos);
     p.u0 = p.per * rank / a.cluster;
     p.n = p.per * (rank + 1) / a.cluster - p.u0;
@@ -244,24 +258,49 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
     const long long U = (long long)list.all() * G;
     const int n = da_taking(U, gridDim.x);
     if ((int)blockIdx.x >= n) return;
-    unit = da_first(U, n, blockIdx.x);
-    end = da_first(U, n, blockIdx.x + 1);
+    auto first_of = [&](int i) {
+      const int cut = da_cut(U, n, i);
+      if (i == n) return cut;
+      const int t = list.token(cut, G), per = list.units_of(t);
+      return da_snap(cut, (cut - list.units_before(t) * G) % per, per);
+    };
+    unit = first_of(blockIdx.x);
+    end = first_of(blockIdx.x + 1);
+    if (unit == end) return;
   }
   __syncthreads();                             // (``dead`` and the barriers are there)
-  auto piece_at = [&](int unit) {
+  // the piece that begins at ``unit``, but for its keys; ``unit`` moves on behind it
+  auto piece_to = [&](DaPiece& q, int of_pair) {
+    const int n = min(q.per + DA_PIECE - of_pair, end - unit);
+    q.u0 = max(of_pair - DA_PIECE, 0);
+    q.n = of_pair + n - DA_PIECE - q.u0;
+    unit += n;
+  };
+  auto piece_at = [&]() {
     DaPiece q;
     q.t = list.token(unit, G);
-    q.per = list.units_of(q.t);
+    q.per = list.units_of(q.t) - DA_PIECE;
     const int of_token = unit - list.units_before(q.t) * G;
-    q.kvh = of_token / q.per;
-    q.u0 = of_token - q.kvh * q.per;
-    q.n = min(q.per - q.u0, end - unit);
-    da_piece_keys(a, q, list.position(q.t));
+    q.kvh = of_token / (q.per + DA_PIECE);
+    piece_to(q, of_token - q.kvh * (q.per + DA_PIECE));
     return q;
   };
-  if constexpr (!CLUSTER) p = piece_at(unit);
+  auto piece_after = [&](const DaPiece& p) {   // (of the same token: with its keys)
+    DaPiece q = p;
+    if (++q.kvh == G) {
+      q.kvh = 0;
+      q.t++;
+      q.per = list.units_of(q.t) - DA_PIECE;
+    }
+    piece_to(q, 0);
+    return q;
+  };
+  if constexpr (!CLUSTER) {
+    p = piece_at();
+    da_piece_keys(a, p, list.position(p.t), a.token_req[p.t]);
+  }
   // this warp's 16 keys of unit u: base + 128 u + 16 warp ..
-  auto first_key = [&](const DaPiece& p, int u) { return p.base + u * DA_UNIT + 16 * warp; };
+  auto first_key = [&](const DaPiece& p, int u) { return (p.lo & ~15) + u * DA_UNIT + 16 * warp; };
   auto chunks_of = [&](const DaPiece& p) {
     const int left = p.pos - first_key(p, p.u0);
     return left < 0 ? 0 : min(p.n, left / DA_UNIT + 1);
@@ -338,6 +377,28 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
       l[n][0] = l[n][1] = 0.f;
     }
     int page_next = chunks > DA_STAGES ? page_of(p, DA_STAGES) : 0;
+    // What the next piece's first requests need, each a trip to memory that would otherwise begin with this one's end: its token's position
+    // and request now, its first pages after this piece's first keys
+    bool more = false;
+    DaPiece next = p;
+    int next_pages[DA_STAGES] = {0, 0};
+    if constexpr (!CLUSTER) {
+      more = unit < end;
+      if (more) {
+        next = piece_after(p);
+        if (next.t != p.t) {
+          next.pos = list.position(next.t);
+          next.lo = a.token_req[next.t];       // (until its pages are looked up)
+        }
+      }
+    }
+    auto next_pages_of = [&]() {
+      if (next.t != p.t) da_piece_keys(a, next, next.pos, next.lo);
+      const int n = chunks_of(next);
+#pragma unroll
+      for (int i = 0; i < DA_STAGES; i++) next_pages[i] = i < n ? page_of(next, i) : 0;
+    };
+    if (more && chunks == 0) next_pages_of();
     for (int i = 0; i < chunks; i++, done++) {
       const int s = done % DA_STAGES, key0 = first_key(p, p.u0 + i);
       if (!tc_wait(&full[warp][s], done / DA_STAGES & 1, &dead) && lane == 0) atomicCAS(a.status, 0, 1);
@@ -458,6 +519,7 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
         request(p, i + DA_STAGES, DA_STAGES, page_next);
         if (i + DA_STAGES + 1 < chunks) page_next = page_of(p, i + DA_STAGES + 1);
       }
+      if (!CLUSTER && i == 0 && more) next_pages_of();
       if (border) {                            // values that nobody may see have the weight zero, and may be no numbers
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -479,15 +541,12 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
     }
 
     // ---- the next piece's first keys are on their way while this one's sums come together
-    bool more = false;
-    DaPiece next = p;
     if constexpr (!CLUSTER) {
-      unit += p.n;
-      more = unit < end;
       if (more) {
-        next = piece_at(unit);
         chunks = chunks_of(next);
-        for (int i = 0; i < min(chunks, DA_STAGES); i++) request(next, i, i, page_of(next, i));
+#pragma unroll
+        for (int i = 0; i < DA_STAGES; i++)
+          if (i < chunks) request(next, i, i, next_pages[i]);
       }
     }
 #pragma unroll
@@ -577,35 +636,51 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
     for (int i = 0; i < 1000; i++) __nanosleep(1000);          // copies on their way land in what is still this CTA's
 }
 
-// The pieces of pairs that several CTAs of the launch before (of n_ctas) had: a block to a head, its threads' groups with every so many'th piece
-// each.  (One token of 100,001 keys has 74 pieces to a pair: one after the other in a block to a pair they took 25 us.)
+// The pieces of pairs that several CTAs of the launch before (of n_ctas) had: a block to ``heads`` of a pair's heads (a power of two), whose threads'
+// groups have every so many'th piece of one each.  (One token of 100,001 keys has 74 pieces to a pair: one after the other in a block to a pair
+// they took 25 us.  64 tokens of 28 heads in blocks to a head each: 1,792, twice what fits beside the launch before and finds out what it
+// has to join meanwhile, 10 us; ``heads`` is as many as bring the blocks to four a multiprocessor.)
 template <int HD>
-__global__ void __launch_bounds__(DA_THREADS) decode_fp8_join_kernel(const DaArgs a, int n_ctas) {
-  constexpr int LANES = HD / 4, GROUPS = DA_THREADS / LANES;
+__global__ void __launch_bounds__(DA_THREADS) decode_fp8_join_kernel(const DaArgs a, int n_ctas, int heads) {
+  constexpr int LANES = HD / 4;
   __shared__ int sums[DA_TOKENS + 1], scratch[DA_WARPS];
   __shared__ DaJoin got[DA_THREADS];
   pdl_launch_dependents();
   const DaList list = da_list(a, sums, scratch);
-  const int pair = blockIdx.x / a.gs, h = blockIdx.x % a.gs, t = pair / a.pages.G, kvh = pair % a.pages.G, per = list.units_of(t);
+  const int sets = (a.gs + heads - 1) / heads, pair = blockIdx.x / sets, t = pair / a.pages.G, kvh = pair % a.pages.G, per = list.units_of(t);
   const long long U = (long long)list.all() * a.pages.G;
   n_ctas = da_taking(U, n_ctas);
-  const int from = list.units_before(t) * a.pages.G + kvh * per, c0 = da_cta_of(U, n_ctas, from), c1 = da_cta_of(U, n_ctas, from + per - 1);
+  const int from = list.units_before(t) * a.pages.G + kvh * per;
+  const int2 cut = da_cut_by(U, n_ctas, from, per);
+  const int c0 = cut.x, c1 = cut.y;
+  // whether CTA c0 has something before this pair: then this is its second piece
+  bool second = false;
+  if (c0 < c1) {
+    const int at = da_cut(U, n_ctas, c0);
+    if (at < from) {
+      const int u = list.token(at, a.pages.G), of = list.units_of(u);
+      second = da_snap(at, (at - list.units_before(u) * a.pages.G) % of, of) < from;
+    }
+  }
   pdl_wait();                                  // (also where there is nothing to join: the next launch waits for this one alone)
-  if (c0 == c1) return;
-  const int f = threadIdx.x % LANES * 4, group = threadIdx.x / LANES;
+  if (c0 >= c1) return;
+  const int f = threadIdx.x % LANES * 4, slot = threadIdx.x / LANES, h = blockIdx.x % sets * heads + (slot & (heads - 1));
+  const int group = slot / heads, groups = DA_THREADS / LANES / heads;
   DaJoin j;
   j.none();
+  if (h < a.gs) {
 #pragma unroll 4
-  for (int i = c0 + group; i <= c1; i += GROUPS) {
-    const long long slot = 2ll * i + (da_first(U, n_ctas, i) < from ? 1 : 0);          // (the CTA's first piece, if it begins here)
-    const float4 st = __ldcg(reinterpret_cast<const float4*>(a.part_s + (slot * a.gs + h) * 4));
-    j.add(st.x, st.y, st.z, __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot * a.gs + h) * HD + f)));
+    for (int i = c0 + group; i <= c1; i += groups) {
+      const long long at = (2ll * i + (i == c0 && second ? 1 : 0)) * a.gs + h;
+      const float4 st = __ldcg(reinterpret_cast<const float4*>(a.part_s + at * 4));
+      j.add(st.x, st.y, st.z, __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + f)));
+    }
   }
   got[threadIdx.x] = j;
   __syncthreads();
-  if (group) return;
-  for (int i = 1; i < GROUPS && c0 + i <= c1; i++) {
-    const DaJoin& k = got[i * LANES + threadIdx.x];
+  if (group || h >= a.gs) return;
+  for (int i = 1; i < groups && c0 + i <= c1; i++) {
+    const DaJoin& k = got[i * heads * LANES + threadIdx.x];
     j.add(k.sum, k.mz, k.mw, k.s);
   }
   da_store(a.out + (long long)t * a.ldo + (long long)(kvh * a.gs + h) * HD + f, j.s, j.inverse());
@@ -624,14 +699,20 @@ static int* da_status_word() {
   return words[dev];
 }
 
-// How a launch over T tokens of up to max_keys keys is cut: CTAs, and how many of them are a pair's cluster (0: units are dealt out)
+// How a launch over T tokens of up to max_keys keys is cut: CTAs, and how many of them are a pair's cluster (0: units are dealt out).  A cluster costs 5 us
+// and 0.85 for each of its CTAs' units, however short the other tokens are; dealing out costs 13 and more with the tokens (a list of them in every CTA,
+// pieces, the launch that joins them), and takes no longer for one long token among short ones.  With 28 + 4 heads, dealt out and in clusters: 1 token of
+// 12,000 keys 14.3 and 11.2 us, of 24,000 15.4 and 16.3; 8 of 500 8.1 and 6.6, of up to 4,000 13.6 and 12.9; 16 of up to 4,000 16.0 and 18.4; 32 of 1,000
+// 17.7 and 11.3, of up to 4,000 22.2 and 30.7; 64 of up to 300 12.2 and 8.8, of up to 2,000 23.1 and 23.3, of up to 8,000 55.6 and 76.2; 256 of up to 500
+// 34.5 and 30.5, of up to 2,000 64.1 and 64.4.
 struct DaPlan { int ctas, cluster; };
 static DaPlan da_plan(int T, int G, int gs, int window, int max_keys, int sms) {
   const long long keys = window > 0 && window < max_keys ? window + 15 : max_keys;
   const long long per = (keys + DA_UNIT - 1) / DA_UNIT, pairs = (long long)T * G, at_a_time = (long long)(gs > 8 ? 1 : 2) * sms;
+  // a CTA to a multiprocessor, at most
   int n = 1;
-  while (n < DA_MAX_CLUSTER && n < per && 2 * n * pairs <= at_a_time) n *= 2;
-  if (n * pairs <= at_a_time && per <= 4 * n) return {(int)(n * pairs), n};
+  while (n < DA_MAX_CLUSTER && n < per && 2 * n * pairs <= sms) n *= 2;
+  if (per <= (pairs > sms ? 16 : 8) * n && n * pairs <= 0x7fffffffll) return {(int)(n * pairs), n};
   return {(int)(pairs * per < at_a_time ? pairs * per : at_a_time), 0};
 }
 
@@ -643,7 +724,7 @@ extern "C" long long qd_decode_attention_fp8_scratch(int T, int H, int G, int d,
 }
 
 template <int HD, int NT, bool CLUSTER>
-static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, cudaStream_t stream) {
+static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, int sms, cudaStream_t stream) {
   const int smem = 1024 + DA_WARPS * (DA_STAGES * 32 * HD + 8 * 8 * (HD / 8 + 4) * 4);
   auto kernel = decode_fp8_kernel<HD, NT, CLUSTER>;
   static bool allowed[64];
@@ -659,7 +740,9 @@ static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, cudaStre
   }
   if (!CLUSTER) {
     qd_launch(kernel, dim3(ctas), dim3(DA_THREADS), smem, stream, map, a);
-    qd_launch(decode_fp8_join_kernel<HD>, dim3(a.T * a.H), dim3(DA_THREADS), 0, stream, a, ctas);
+    int heads = 1;
+    while (heads < 8 && heads < a.gs && (long long)a.T * a.pages.G * ((a.gs + heads - 1) / heads) > 4ll * sms) heads *= 2;
+    qd_launch(decode_fp8_join_kernel<HD>, dim3(a.T * a.pages.G * ((a.gs + heads - 1) / heads)), dim3(DA_THREADS), 0, stream, a, ctas, heads);
     return qd_last_error();
   }
   cudaLaunchConfig_t cfg = {};
@@ -679,9 +762,9 @@ static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, cudaStre
   return qd_last_error();
 }
 template <int HD>
-static int da_launch_of(const CUtensorMap& map, const DaArgs& a, int ctas, cudaStream_t stream) {
-  if (a.cluster) return a.gs <= 8 ? da_launch<HD, 1, true>(map, a, ctas, stream) : da_launch<HD, 2, true>(map, a, ctas, stream);
-  return a.gs <= 8 ? da_launch<HD, 1, false>(map, a, ctas, stream) : da_launch<HD, 2, false>(map, a, ctas, stream);
+static int da_launch_of(const CUtensorMap& map, const DaArgs& a, int ctas, int sms, cudaStream_t stream) {
+  if (a.cluster) return a.gs <= 8 ? da_launch<HD, 1, true>(map, a, ctas, sms, stream) : da_launch<HD, 2, true>(map, a, ctas, sms, stream);
+  return a.gs <= 8 ? da_launch<HD, 1, false>(map, a, ctas, sms, stream) : da_launch<HD, 2, false>(map, a, ctas, sms, stream);
 }
 
 // q, out: bfloat16 rows [T, H d], ``ldq`` and ``ldo`` apart; table [table_rows, max_blocks] of pages of ps tokens (a multiple of 16), its row of token t is
@@ -697,7 +780,7 @@ extern "C" int qd_decode_attention_fp8(const void* q, long long ldq, void* out, 
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages) & 15) || ldq % 8 || ldo % 8) return QD_ERR_UNSUPPORTED;
   const int gs = H / G;
   // the units of a launch fit 31 bits
-  if ((long long)(T < DA_TOKENS ? T : DA_TOKENS) * G * (max_keys / DA_UNIT + 2) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
+  if ((long long)(T < DA_TOKENS ? T : DA_TOKENS) * G * (max_keys / DA_UNIT + 2 + DA_PIECE) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   int* status = da_status_word();
   CUtensorMap map;
   if (!status || !c8_make_map(&map, pages, n_pages, G, ps, d)) return QD_ERR_UNSUPPORTED;
@@ -707,7 +790,7 @@ extern "C" int qd_decode_attention_fp8(const void* q, long long ldq, void* out, 
     const DaArgs a = {(const bf16*)q + t * ldq, ldq, (bf16*)out + t * ldo, ldo, {(unsigned char*)pages, c8_page_bytes(G, ps, d), G, ps, d}, (int)n_pages,
                       table, max_blocks, table_rows, token_req + t, positions + t, n, H, gs, window, max_keys, scale * 1.4426950408889634f,
                       scratch, scratch + 2ll * plan.ctas * gs * d, plan.cluster, ps & (ps - 1) ? -1 : __builtin_ctz(ps), status};
-    const int rc = d == 128 ? da_launch_of<128>(map, a, plan.ctas, stream) : da_launch_of<64>(map, a, plan.ctas, stream);
+    const int rc = d == 128 ? da_launch_of<128>(map, a, plan.ctas, sms, stream) : da_launch_of<64>(map, a, plan.ctas, sms, stream);
     if (rc) return rc;
   }
   return 0;

@@ -174,6 +174,22 @@ def test_decode_long(guard_regions):
     check_decode([9000] * 3, 8, 4, 64)
 
 
+@pytest.mark.parametrize("T", [5, 31, 33, 64, 130, 400, 1100])
+@pytest.mark.parametrize("H,G,d", [(8, 2, 128), (3, 3, 64), (9, 1, 64)])
+def test_decode_ragged(guard_regions, T, H, G, d):
+    """Tokens of lengths from nothing on beside a few long ones, whose keys several CTAs have."""
+    gen = torch.Generator().manual_seed(T)
+    lengths = [5000, 700, 129, 1]
+    reqs = [0, 3] + torch.randint(0, 4, (T - 2,), generator=gen).tolist()
+    short = torch.rand((T,), generator=gen) < 0.7
+    positions = [4999, 0] + [int(torch.randint(-1, min(lengths[r], 300) if short[t + 2] else lengths[r], (1,), generator=gen)) for t, r in enumerate(reqs[2:])]
+    check_decode(lengths, H, G, d, reqs=reqs, positions=positions)
+    if T in (33, 130):
+        check_decode(lengths, H, G, d, reqs=reqs, positions=positions, window=1500)
+        check_decode(lengths, H, G, d, reqs=reqs[:-1] + [0], positions=[-1] * (T - 1) + [4999])
+        check_decode(lengths, H, G, d, reqs=[0] * T, positions=[4999 - t % 7 for t in range(T)])
+
+
 def test_decode_scales_far_apart(guard_regions):
     """Values whose scales lie 2^20 and more apart, scores that leave one key nearly alone."""
     check_decode([300, 40, 1000], 8, 2, 128, spread=8.0, q_scale=0.01)
