@@ -125,6 +125,27 @@ __device__ __forceinline__ float ac_power(float x) {
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two float32 numbers in one register pair
+__device__ __forceinline__ unsigned long long ac_two(float a, float b) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 ac_both(unsigned long long v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ unsigned long long ac_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ unsigned long long ac_add(unsigned long long a, unsigned long long b) {
+  unsigned long long v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
 // two e4m3 numbers times two float16 numbers
 __device__ __forceinline__ unsigned ac_f16x2(unsigned short two, unsigned f) {
   unsigned h;
@@ -314,13 +335,18 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
             sum += p0 + p1;
             pk[i] = at_pack(p0, p1);
           }
-        } else {
+        } else {                                     // (two numbers to an instruction: 2,048 tokens behind 6,144 283 -> 276 us)
+          const unsigned long long by = ac_two(mul, mul), from = ac_two(-ref, -ref);
+          unsigned long long two = 0;
 #pragma unroll
           for (int i = 0; i < KQ / 2; i++) {
-            const float p0 = at_exp2(fmaf(sv[2 * i], mul, -ref)), p1 = at_exp2(fmaf(sv[2 * i + 1], mul, -ref));
-            sum += p0 + p1;
+            const float2 x = ac_both(ac_fma(ac_two(sv[2 * i], sv[2 * i + 1]), by, from));
+            const float p0 = at_exp2(x.x), p1 = at_exp2(x.y);
+            two = ac_add(two, ac_two(p0, p1));
             pk[i] = ac_halves(p0, p1);
           }
+          const float2 sums = ac_both(two);
+          sum = sums.x + sums.y;
         }
       };
       ready = __all_sync(0xffffffffu, ac_done(&s_full[j & 1 ^ 1], (j + 1) >> 1 & 1));
