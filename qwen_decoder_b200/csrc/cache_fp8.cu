@@ -12,7 +12,7 @@
 // A thread has eight neighbouring features (16 bytes of a bfloat16 row) of four heads of a token's q, so that the tables' rows, four times
 // a head's bytes, are read once for all of them, or of one head of its k or v, whose work is the longest; rows of few tokens, which wait for
 // their loads alone, have q's heads one by one, too.  The pair's other half is a shuffle away.  Blocks of the same tokens lie together: a row of
-// x is read from one end to the other (2,048 tokens out of the caches' reach 18.4 us, a head of all tokens at a time 20.4).
+// x is read from one end to the other (2,048 tokens, with x out of the caches, 18.4 us, a set of heads of all tokens at a time 20.4).
 //
 // One token of 16 + 2 heads, four parts: 3.0 us, which are a launch and three trips to memory behind one another (position, table,
 // nothing to overlap them with).  2,048 of 28 + 4: 12.2 us, of which 6 are its 37 MB at the rate of device memory; the rest is the
@@ -240,7 +240,8 @@ extern "C" int qd_rope_kv_write_fp8(const void* x, int dtype, long long ld, int 
   CwArgs a = {x, ld, part_step, parts, bias, (bf16*)q, T, H, rot, n_pos, 0, 0, cos_t, sin_t, positions, slots, (int)(n_pages * ps),
               {(unsigned char*)pages, c8_page_bytes(G, ps, d), G, ps, d}};
   const int rows = CW_THREADS / (d / 8);
-  // four heads to a thread where that still leaves every multiprocessor two blocks' worth of them
+  // four heads to a thread where that still leaves every multiprocessor two blocks' worth of them (of 28 + 4 heads, four and one: 64 tokens 3.1 and 2.7 us,
+  // 256 3.9 and 3.7, 512 4.6 and 5.8, 2,048 12.1 and 16.4)
   const int nh = (long long)T * (H + 2 * G) >= 4ll * 2 * sms * rows ? 4 : 1;
   a.kv_sets = write ? G : 0;
   a.sets = (H + nh - 1) / nh + 2 * a.kv_sets;

@@ -13,13 +13,19 @@
 // A cluster of S CTAs shares a row, contiguous parts of it (in shared memory where they fit).  The k-th largest logit and t are found
 // alike, by histograms (counts, or counts and weights) over the cluster: first over 1,409 equal steps of z below the maximum, down to 44 ln 2 T,
 // where weights end (the logits of a row are spread over many of these, so that few additions meet; in steps of the number's leading bits
-// they would not be); then the logits of the step that the border lies in go to one CTA, which puts them in order.  Where they are more than
-// SN_NEAR (a thousand equal logits), histograms over steps of the logit's bits follow, until a step is one number.
-// Bound by the row's reading for the rest and by the trips over the cluster, two to a histogram.
+// they would not be); then the logits of the step that the border lies in go to one CTA, which adds up for each of them what it and those above it
+// have.  Where they are more than SN_LIST (a thousand equal logits), histograms over steps of the logit's bits follow, until a step is one number.
+// The draw's token is looked for in the CTA that it falls to, a sixteenth of its part, a sixteenth of that, 128 logits.
 //
 // A top-k of up to 256 needs none of that: the k-th largest of a CTA's threads' own maxima has k logits that reach it, as the least of the
-// CTAs' ceil(k / S)-th ones has; what reaches the larger of these bounds is little more than k logits, which go to one CTA's list, are put in order
-// there and decide the rest.
+// CTAs' ceil(k / S)-th ones has; what reaches the larger of these bounds is little more than k logits, which go to one CTA's list and decide the rest
+// there.  (Rows of 152,064 with top-p 0.95, by the list and by histograms: one with k = 20 13.4 and 32.1 us, with 250 32.1 and 32.4, with 500 98
+// and 33; 64 with k = 20 17.5 and 92, with 250 43 and 93, with 500 122 and 94.)
+//
+// 64 rows of 152,064 take 23 us with k of up to 100, top-p and min-p, of which 6 are their 39 MB at the rate of device memory; then bound by trips over
+// the cluster (1.5 to 3 thousand cycles each) and the list's sums.  By top-p alone 82: bound by the weights' arithmetic, 55 instructions for each logit,
+// a third of them on whole numbers at half the rate, and their two additions in shared memory (40 us with the rows and no weights).  One row of
+// 151,936 by top-p 25, S = 16: seven trips over the cluster and code that runs once, out of the reach of the instructions' caches.
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <math.h>
@@ -729,7 +735,8 @@ extern "C" int qd_sample_nucleus(const float* logits, long long ld, int R, int V
       return (int)cudaGetLastError();
     allowed[dev] = true;
   }
-  // as many CTAs to a row as run at a time, with two tiles of 2,048 to each
+  // as many CTAs to a row as run at a time, with 4,096 logits or more to each (by top-p, S = 1, 2, 4, 8, 16: one row of 151,936 134, 79, 48, 30, 25 us, 16 of
+  // them 138, 80, 49, where no more than 4 run at a time; one of 32,000 34, 24, 18.3, 17.2, 17.7; of 8,000 16.0, 16.1, 14.4, and with k = 50 9.1, 10.7, 11.1)
   for (int n = 2; n <= SN_MAX_SHARES && V / n >= 4096 && R <= sn_clusters(n, most, sms, dev); n *= 2) a.shares = n;
   const int part = ((V + a.shares - 1) / a.shares + 3) & ~3;
   a.keep = part <= SN_KEEP;
