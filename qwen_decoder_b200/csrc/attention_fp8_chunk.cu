@@ -22,9 +22,9 @@
 // * Tiles of rows that would leave multiprocessors without work (a short portion behind a long history, the last round of a long one) share their
 //   keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
 //
-// With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 274 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
-// 2,300 cycles, in which the softmax warps never wait: 1,024 are the exponentials' (16 a cycle), the rest what comes before and behind them (scores
-// from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 44 us, of which 10 are their products': three tiles of rows,
+// With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 259 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
+// 2,200 cycles, in which the softmax warps never wait: 1,024 are the exponentials' (16 a cycle), the rest what comes before and behind them (scores
+// from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 43 us, of which 10 are their products': three tiles of rows,
 // the last of them one token's, in 12 shares each.  512 tokens of three requests behind 655 at most, 16 + 2 heads: 17.5 us, of which the launch and the way to
 // the first scores (rows, q's operands) are 6.
 //
@@ -159,11 +159,15 @@ __device__ __forceinline__ unsigned ac_f16x2(unsigned short two, unsigned f) {
   asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(f));
   return h;
 }
-// two e4m3 numbers times f as bfloat16
-__device__ __forceinline__ unsigned ac_bf16x2(unsigned short two, float f) {
+// two e4m3 numbers
+__device__ __forceinline__ float2 ac_values(unsigned short two) {
   unsigned h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// two e4m3 numbers times f as bfloat16
+__device__ __forceinline__ unsigned ac_bf16x2(unsigned short two, float f) {
+  const float2 v = ac_values(two);
   return at_pack(v.x * f, v.y * f);
 }
 
@@ -275,8 +279,8 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         const float v0 = __uint_as_float(x[0] << 16) * inv, v1 = __uint_as_float(x[0] & 0xffff0000u) * inv;
         const float v2 = __uint_as_float(x[1] << 16) * inv, v3 = __uint_as_float(x[1] & 0xffff0000u) * inv;
         big[i] = fp8_pack4(v0, v1, v2, v3);
-        small[i] = fp8_pack4((v0 - fp8_value(big[i] & 255u)) * 16.f, (v1 - fp8_value(big[i] >> 8 & 255u)) * 16.f,
-                             (v2 - fp8_value(big[i] >> 16 & 255u)) * 16.f, (v3 - fp8_value(big[i] >> 24)) * 16.f);
+        const float2 b01 = ac_values((unsigned short)big[i]), b23 = ac_values((unsigned short)(big[i] >> 16));
+        small[i] = fp8_pack4((v0 - b01.x) * 16.f, (v1 - b01.y) * 16.f, (v2 - b23.x) * 16.f, (v3 - b23.y) * 16.f);
       }
 #pragma unroll
       for (int i = 0; i < DH / 4; i += 8) {
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           if (!tc_wait_inline(&o_done, (j - 1) & 1, &dead) && lane == 0) atomicCAS(p.status, 0, 8);
           __syncwarp();
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < DH; c += 32) {
             float ov[32];
             at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       const long long at = (long long)behind * AC_ROWS + row;
       if (ok && h == 0) *reinterpret_cast<float4*>(p.part_s + 4 * at) = make_float4(m, z, l_all, 0.f);
       if (n_kt > 0) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DH; c += 32) {
           float ov[32];
           at_tmem_ld<32>(t_lane + T_O + h * DH + c, ov);      // the warp's access: rows without a token take part too
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
     } else {
       const float inv = l_all == 0.f ? 0.f : 1.f / l_all, up = ac_power(m - z);
       bf16* d = p.out + (long long)(tok0 + t) * p.ldo + (long long)(g * gs + hh) * HD + h * DH;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < DH; c += 32) {
         float ov[32];
         if (n_kt > 0) {
@@ -462,7 +466,8 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         const unsigned char* from = v8_s + s * TILE8 + ((warp & 3) * 8 + x) * HD;
         unsigned char* to = v_s + s * TILE16 + ((warp & 3) * 8 + x) * 128;
         const int a_at = ((2 * c) ^ x) << 4, b_at = ((2 * c + 1) ^ x) << 4;
-#pragma unroll
+        // (rolled: 2,048 tokens behind 6,144 276 -> 259 us, with the code of both kinds of tile in one body; in two 274 to 294, with waits between the turns 267)
+#pragma unroll 1
         for (int e0 = 0; e0 < STEPS; e0 += 4) {
           const int block = e0 / 4;
           uint4 v[4];
