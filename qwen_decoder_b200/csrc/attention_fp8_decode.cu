@@ -23,7 +23,7 @@
 // * Where there is little, a pair is a cluster's, whose CTAs have equal shares of its units and join over their shared memories.
 //
 // With 28 + 4 heads of 128: 64 tokens of 8,192 keys 98.6 us, where their 545 MB take 83 at the rate of device memory (88 in a CTA to each pair, which one
-// long token among short ones would have wait for one); 23 of 500 to 4,000 18.3, of which 8.3; one of 100,001 27.7, of which 15.8 (the rest: the launches, the way to the
+// long token among short ones would have wait for one); 23 of 500 to 4,000 18.3, of which 8.3; one of 100,001 26.2, of which 15.8 (the rest: the launches, the way to the
 // first keys, 74 pieces to a pair).  16 + 2 heads, one token of 2,048: 6.9, nothing but latencies (position, page, keys, 16 CTAs' join).
 #include "cache_fp8.cuh"
 #include "entry_points.h"
@@ -139,6 +139,7 @@ struct DaList {
   __device__ __forceinline__ int units_of(int t) const { return few ? __shfl_sync(0xffffffffu, units, t) : sums[t + 1] - sums[t]; }
   __device__ __forceinline__ int position(int t) const { return few ? __shfl_sync(0xffffffffu, pos, t) : positions[t]; }
 };
+template <int THREADS>
 __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto scan = [&](int s) {
@@ -161,7 +162,7 @@ __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scrat
     return list;
   }
   int before = 0;
-  for (int t0 = 0; t0 < a.T; t0 += DA_THREADS) {
+  for (int t0 = 0; t0 < a.T; t0 += THREADS) {
     const int t = t0 + threadIdx.x;
     const int u = t < a.T ? da_units(a, a.positions[t]) + DA_PIECE : 0;
     const int s = scan(u);
@@ -169,7 +170,7 @@ __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scrat
     __syncthreads();
     int base = before, all = before;
 #pragma unroll
-    for (int w = 0; w < DA_WARPS; w++) {
+    for (int w = 0; w < THREADS / 32; w++) {
       if (w < warp) base += scratch[w];
       all += scratch[w];
     }
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
     p.u0 = p.per * rank / a.cluster;
     p.n = p.per * (rank + 1) / a.cluster - p.u0;
   } else {
-    list = da_list(a, sums, scratch);
+    list = da_list<DA_THREADS>(a, sums, scratch);
     const long long U = (long long)list.all() * G;
     const int n = da_taking(U, gridDim.x);
     if ((int)blockIdx.x >= n) return;
@@ -644,13 +645,13 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
 // groups have every so many'th piece of one each.  (One token of 100,001 keys has 74 pieces to a pair: one after the other in a block to a pair
 // they took 25 us.  64 tokens of 28 heads in blocks to a head each: 1,792, twice what fits beside the launch before and finds out what it
 // has to join meanwhile, 10 us; ``heads`` is as many as bring the blocks to four a multiprocessor.)
-template <int HD>
-__global__ void __launch_bounds__(DA_THREADS) decode_fp8_join_kernel(const DaArgs a, int n_ctas, int heads) {
+template <int HD, int THREADS>
+__global__ void __launch_bounds__(THREADS) decode_fp8_join_kernel(const DaArgs a, int n_ctas, int heads) {
   constexpr int LANES = HD / 4;
-  __shared__ int sums[DA_TOKENS + 1], scratch[DA_WARPS];
-  __shared__ DaJoin got[DA_THREADS];
+  __shared__ int sums[DA_TOKENS + 1], scratch[THREADS / 32];
+  __shared__ DaJoin got[THREADS];
   pdl_launch_dependents();
-  const DaList list = da_list(a, sums, scratch);
+  const DaList list = da_list<THREADS>(a, sums, scratch);
   const int sets = (a.gs + heads - 1) / heads, pair = blockIdx.x / sets, t = pair / a.pages.G, kvh = pair % a.pages.G, per = list.units_of(t);
   const long long U = (long long)list.all() * a.pages.G;
   n_ctas = da_taking(U, n_ctas);
@@ -669,7 +670,7 @@ __global__ void __launch_bounds__(DA_THREADS) decode_fp8_join_kernel(const DaArg
   pdl_wait();                                  // (also where there is nothing to join: the next launch waits for this one alone)
   if (c0 >= c1) return;
   const int f = threadIdx.x % LANES * 4, slot = threadIdx.x / LANES, h = blockIdx.x % sets * heads + (slot & (heads - 1));
-  const int group = slot / heads, groups = DA_THREADS / LANES / heads;
+  const int group = slot / heads, groups = THREADS / LANES / heads;
   DaJoin j;
   j.none();
   if (h < a.gs) {
@@ -746,7 +747,11 @@ static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, int sms,
     qd_launch(kernel, dim3(ctas), dim3(DA_THREADS), smem, stream, map, a);
     int heads = 1;
     while (heads < 8 && heads < a.gs && (long long)a.T * a.pages.G * ((a.gs + heads - 1) / heads) > 4ll * sms) heads *= 2;
-    qd_launch(decode_fp8_join_kernel<HD>, dim3(a.T * a.pages.G * ((a.gs + heads - 1) / heads)), dim3(DA_THREADS), 0, stream, a, ctas, heads);
+    // few blocks have many threads, for as many pieces at a time (one token, 28 + 4 heads, 24,000 keys 14.7 us, with 256 threads 16.1, 100,000 26.2 and 27.9;
+    // two of 32,000 19.9 and 19.0: past some thirty blocks the wait for room beside the launch before is longer)
+    const dim3 blocks(a.T * a.pages.G * ((a.gs + heads - 1) / heads));
+    if (4 * (int)blocks.x <= sms) qd_launch(decode_fp8_join_kernel<HD, 1024>, blocks, dim3(1024), 0, stream, a, ctas, heads);
+    else qd_launch(decode_fp8_join_kernel<HD, DA_THREADS>, blocks, dim3(DA_THREADS), 0, stream, a, ctas, heads);
     return qd_last_error();
   }
   cudaLaunchConfig_t cfg = {};
