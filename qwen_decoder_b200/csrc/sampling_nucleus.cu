@@ -22,7 +22,7 @@
 // there.  (Rows of 152,064 with top-p 0.95, by the list and by histograms: one with k = 20 13.4 and 32.1 us, with 250 32.1 and 32.4, with 500 98
 // and 33; 64 with k = 20 17.5 and 92, with 250 43 and 93, with 500 122 and 94.)
 //
-// 64 rows of 152,064 take 23 us with k of up to 100, top-p and min-p, of which 6 are their 39 MB at the rate of device memory; then bound by trips over
+// 64 rows of 152,064 take 20 us with k of up to 100, top-p and min-p, of which 6 are their 39 MB at the rate of device memory; then bound by trips over
 // the cluster (1.5 to 3 thousand cycles each) and the list's sums.  By top-p alone 82: bound by the weights' arithmetic, 55 instructions for each logit,
 // a third of them on whole numbers at half the rate, and their two additions in shared memory (40 us with the rows and no weights).  One row of
 // 151,936 by top-p 25, S = 16: seven trips over the cluster and code that runs once, out of the reach of the instructions' caches.
@@ -453,21 +453,27 @@ __device__ int sn_by_list(SnShared& s, const SnRow& r, int shares, int rank, int
   int* count = shares > 1 ? cl.map_shared_rank(&s.listed, 0) : &s.listed;
   unsigned long long* list = shares > 1 ? cl.map_shared_rank(s.list, 0) : s.list;
   const float bound_z = sn_value(bound);
-  const float* mine = maxima + threadIdx.x;
-  for (int i0 = r.warp_from + 4 * lane; i0 < r.warp_to; i0 += 128 * SN_AHEAD, mine += SN_THREADS) {
-    if (maxima && !(*mine >= bound_z)) continue;
-    float v[SN_AHEAD][4];
-    sn_ahead(r, i0, v);
+  // (first which of a thread's sixteens have some, then those: few have, and a turn of the whole warp for each is a trip to memory)
+  const int mine = r.warp_from + 4 * lane, runs = (r.warp_to - mine + 128 * SN_AHEAD - 1) / (128 * SN_AHEAD);
+  for (int t0 = 0; t0 < runs; t0 += 32) {
+    unsigned has = 0;
+    for (int t = t0; t < min(t0 + 32, runs); t++)
+      if (!maxima || maxima[t * SN_THREADS + threadIdx.x] >= bound_z) has |= 1u << (t - t0);
+    for (; has; has &= has - 1) {
+      const int i0 = mine + (t0 + __ffs(has) - 1) * 128 * SN_AHEAD;
+      float v[SN_AHEAD][4];
+      sn_ahead(r, i0, v);
 #pragma unroll
-    for (int u = 0; u < SN_AHEAD; u++)
-      if (fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3])) >= bound_z) {
+      for (int u = 0; u < SN_AHEAD; u++)
+        if (fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3])) >= bound_z) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (v[u][j] >= bound_z) {
-            const int at = atomicAdd(count, 1);
-            if (at < SN_LIST) list[at] = (unsigned long long)sn_order(v[u][j]) << 32 | (0xffffffffu - (unsigned)(first + i0 + 128 * u + j));
-          }
-      }
+          for (int j = 0; j < 4; j++)
+            if (v[u][j] >= bound_z) {
+              const int at = atomicAdd(count, 1);
+              if (at < SN_LIST) list[at] = (unsigned long long)sn_order(v[u][j]) << 32 | (0xffffffffu - (unsigned)(first + i0 + 128 * u + j));
+            }
+        }
+    }
   }
   if (shares > 1) cl.sync();
   else __syncthreads();
