@@ -22,7 +22,7 @@
 // * Tiles of rows that would leave multiprocessors without work (a short portion behind a long history, the last round of a long one) share their
 //   keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
 //
-// With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 259 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
+// With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 255 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
 // 2,200 cycles, in which the softmax warps never wait: 1,024 are the exponentials' (16 a cycle), the rest what comes before and behind them (scores
 // from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 43 us, of which 10 are their products': three tiles of rows,
 // the last of them one token's, in 12 shares each.  512 tokens of three requests behind 655 at most, 16 + 2 heads: 17.5 us, of which the launch and the way to
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
         const unsigned char* from = v8_s + s * TILE8 + ((warp & 3) * 8 + x) * HD;
         unsigned char* to = v_s + s * TILE16 + ((warp & 3) * 8 + x) * 128;
         const int a_at = ((2 * c) ^ x) << 4, b_at = ((2 * c + 1) ^ x) << 4;
-        // (rolled: 2,048 tokens behind 6,144 276 -> 259 us, with the code of both kinds of tile in one body; in two 274 to 294, with waits between the turns 267)
+        // (rolled: 2,048 tokens behind 6,144 276 -> 259 us at the time, with the code of both kinds of tile in one body; in two 274 to 294, with waits between the turns 267)
 #pragma unroll 1
         for (int e0 = 0; e0 < STEPS; e0 += 4) {
           const int block = e0 / 4;
@@ -564,21 +564,20 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           const uint2 now = sc;
           sc = scales_at(u + 1, entry);
           entry = u + 2 < n_kt ? entry_at(key_of(u + 2)) : 0;
-          unsigned bk[4], bv[4], most = 0, least = 255;
-          bool all = true;
+          // (four keys' bytes at a time, in little code: one warp goes through it, and the first scores of a launch wait for it)
+          const unsigned values = __byte_perm(now.x, now.y, 0x7531), none = __vcmpeq4(values, ~0u);
+          const int first = key_lo - key_of(u), last = key_hi - key_of(u);      // of the four, the ones that are somebody's
+          const unsigned seen = values | (first <= 0 ? 0u : first >= 4 ? ~0u : ~(~0u << 8 * first)) | (last >= 4 ? 0u : last <= 0 ? ~0u : ~0u << 8 * last);
+          const bool all = __all_sync(0xffffffffu, __vcmpeq4(seen, ~0u) == 0u);
+          unsigned most = 0, least = 255;
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const unsigned both = (e < 2 ? now.x : now.y) >> 16 * (e & 1) & 0xffffu;
-            bv[e] = both >> 8;
-            bk[e] = bv[e] == 255u ? 255u : both & 255u;      // (a value without a number: its key's score is none)
-            const int key = key_of(u) + e;
-            if (key >= key_hi || key < key_lo) bv[e] = 255u;
-            all &= bv[e] != 255u;
-            if (bv[e] != 255u) { most = max(most, bv[e] + 1); least = min(least, bv[e]); }
+            const unsigned b = seen >> 8 * e & 255u;
+            most = max(most, b + 1 & 255u);
+            least = min(least, b);
           }
           most = __reduce_max_sync(0xffffffffu, most);
           least = __reduce_min_sync(0xffffffffu, least);
-          all = __all_sync(0xffffffffu, all);
           if (most == 0) least = most = largest ? largest : 127u;            // (no value that is seen)
           else most--;
           largest = max(largest, most);
@@ -587,13 +586,12 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           unsigned f[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const unsigned down = most - min(bv[e], most);
-            if (bv[e] == 255u) f[e] = 0;
-            else if (wide) f[e] = __float_as_uint(scalbnf(1.f, -(int)down));
-            else f[e] = (down < 15 ? (15u - down) << 10 : 0x200u) * 0x10001u;
+            const unsigned b = seen >> 8 * e & 255u, down = most - min(b, most);
+            f[e] = wide ? (127u - min(down, 127u)) << 23 : (down < 15 ? (15u - down) << 10 : 0x200u) * 0x10001u;
+            if (b == 255u) f[e] = 0;
           }
           const int at = u % AC_AHEAD;
-          key_s[at][lane] = bk[0] | bk[1] << 8 | bk[2] << 16 | bk[3] << 24;
+          key_s[at][lane] = __byte_perm(now.x, now.y, 0x6420) | none;          // (a value without a number: its key's score is none)
           *reinterpret_cast<uint4*>(&factor_s[at][4 * lane]) = make_uint4(f[0], f[1], f[2], f[3]);
           if (lane == 0) tile_s[at] = most | (wide ? AC_WIDE : 0u) | (all ? 0u : AC_HOLES);
         }
