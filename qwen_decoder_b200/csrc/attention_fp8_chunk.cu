@@ -22,9 +22,9 @@
 // * Tiles of rows that would leave multiprocessors without work (a short portion behind a long history, the last round of a long one) share their
 //   keys among CTAs, whose sums chunk_fp8_join_kernel adds up.
 //
-// With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 255 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
+// With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 252 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
 // 2,200 cycles, in which the softmax warps never wait: 1,024 are the exponentials' (16 a cycle), the rest what comes before and behind them (scores
-// from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 43 us, of which 10 are their products': three tiles of rows,
+// from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 42 us, of which 10 are their products': three tiles of rows,
 // the last of them one token's, in 12 shares each.  512 tokens of three requests behind 655 at most, 16 + 2 heads: 17.5 us, of which the launch and the way to
 // the first scores (rows, q's operands) are 6.
 //
@@ -319,11 +319,10 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       at_tmem_ld<KQ>(t_lane + (unsigned)(j & 1) * AC_KEYS + h * KQ, sv);
       const bool interior = tile_base >= free_lo && tile_base + AC_KEYS <= free_hi && p.scale_log2e > 0.f;
       if (!interior) {
+        // of this thread's keys the first that the row sees, and how many
+        const int from = max(lo - key_base, 0), many = ok ? max(pos - key_base - from + 1, 0) : 0;
 #pragma unroll
-        for (int i = 0; i < KQ; i++) {
-          const int key = key_base + i;
-          sv[i] = ok && key <= pos && key >= lo ? sv[i] * p.scale_log2e : -INFINITY;
-        }
+        for (int i = 0; i < KQ; i++) sv[i] = (unsigned)(i - from) < (unsigned)many ? sv[i] * p.scale_log2e : -INFINITY;
       }
       float mx4[4] = {sv[0], sv[1], sv[2], sv[3]};   // (one chain of 64 would be four cycles each)
 #pragma unroll
@@ -610,7 +609,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       };
       auto scores = [&](int j) {
         const unsigned k_lo = k_lo0 + (unsigned)(j % NS) * (TILE8 >> 4);
-#pragma unroll
+#pragma unroll 1
         for (int part = 0; part < 2; part++)
 #pragma unroll
           for (int k = 0; k < HD / 32; k++)
@@ -619,6 +618,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
       };
       if (n_kt > 0) {
         if (!tc_wait_inline(&q_full, 0, &dead) && lane == 0) atomicCAS(p.status, 0, 3);
+#pragma unroll 1
         for (int j = 0; j < 2; j++) {                   // slots -2 and -1: the first two tiles' scores
           slot_ready(j - 2);
           tc_fence_after();
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
           tc_fence_after();
           const unsigned v_lo = v_lo0 + (unsigned)s * (TILE16 >> 4), idesc_pv = idesc_f16 | (tile_s[j % AC_AHEAD] & AC_WIDE ? 1u << 7 | 1u << 10 : 0u);
           if (one) {
-#pragma unroll
+#pragma unroll 2
             for (int k = 0; k < AC_KEYS / 16; k++)
               at_umma_ta(tmem + T_O, tmem + (unsigned)(j & 1) * AC_KEYS + (unsigned)(k + (k & 4)) * 8, v_lo + (unsigned)k * (2048 >> 4), AT_DESC_HI, idesc_pv,
                          (j > 0 || k > 0) ? 1u : 0u);
