@@ -22,7 +22,7 @@
 //   most two pieces to a CTA, for ``decode_fp8_join``.  No counters are shared between launches.
 // * Where there is little, a pair is a cluster's, whose CTAs have equal shares of its units and join over their shared memories.
 //
-// With 28 + 4 heads of 128: 64 tokens of 8,192 keys 98.6 us, where their 545 MB take 83 at the rate of device memory (88 in a CTA to each pair, which one
+// With 28 + 4 heads of 128: 64 tokens of 8,192 keys 95.5 us, where their 545 MB take 83 at the rate of device memory (88 in a CTA to each pair, which one
 // long token among short ones would have wait for one); 23 of 500 to 4,000 18.3, of which 8.3; one of 100,001 26.2, of which 15.8 (the rest: the launches, the way to the
 // first keys, 74 pieces to a pair).  16 + 2 heads, one token of 2,048: 6.9, nothing but latencies (position, page, keys, 16 CTAs' join).
 #include "cache_fp8.cuh"
@@ -106,7 +106,13 @@ __device__ __forceinline__ int da_units(const DaArgs& a, int pos) {
 // What is dealt out are the keys' units and DA_PIECE more in front of them for each pair, which stand for what a pair costs besides.  CTAs that take
 // units, of those there are: CTA i of n takes those from i U / n on, or from where the pair begins or ends that lies near: a part of a pair costs its sums' way
 // through memory
-__device__ __forceinline__ int da_taking(long long U, int ctas) { return (int)(U < ctas ? U : ctas); }
+__device__ __forceinline__ int da_taking(long long U, int ctas, int pairs, int most) {
+  // Pairs of as many units each, ``most``: a whole number of CTAs to a pair, so that no cut leaves a little of one (64 tokens of 8,192 keys, 28 + 4 heads,
+  // 256 CTAs and 296: 95.5 and 99 us, of 4,000 51.4 and 56.2; of lengths that differ there is no such number, and fewer CTAs take longer: up to 8,000 keys 59.8 and 55.6)
+  const int alike = ctas / pairs * pairs;
+  if ((long long)most * pairs == U && 5 * alike >= 4 * ctas) return alike;
+  return (int)(U < ctas ? U : ctas);
+}
 __device__ __forceinline__ int da_cut(long long U, int n, int i) { return (int)(U * i / n); }
 // (``per``: units of the pair with those in front, ``of_pair``: of them before the cut)
 __device__ __forceinline__ int da_snap(int cut, int of_pair, int per) {
@@ -124,7 +130,7 @@ __device__ __forceinline__ int2 da_cut_by(long long U, int n, int from, int per)
 // The list of all tokens' units.  Up to 32 tokens: in the registers of every warp, a lane to a token; more: in shared memory, made by the
 // whole block.
 struct DaList {
-  int few, T, before, units, pos;              // of this lane's token: units of those before it, its own, its position
+  int few, T, most, before, units, pos;        // most: units that a token has; of this lane's token: units of those before it, its own, its position
   const int *sums, *positions;
   __device__ __forceinline__ int all() const { return few ? __shfl_sync(0xffffffffu, before + units, T - 1) : sums[T]; }
   // the token that unit ``u`` of ``G`` times the list is of: a whole warp looks, at every 32nd of them and then at 32 (one after the other by halves it
@@ -159,13 +165,16 @@ __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scrat
     list.pos = lane < a.T ? a.positions[lane] : -1;
     list.units = lane < a.T ? da_units(a, list.pos) + DA_PIECE : 0;
     list.before = scan(list.units) - list.units;
+    list.most = (int)__reduce_max_sync(0xffffffffu, (unsigned)list.units);
     return list;
   }
   int before = 0;
+  unsigned most = 0;
   for (int t0 = 0; t0 < a.T; t0 += THREADS) {
     const int t = t0 + threadIdx.x;
     const int u = t < a.T ? da_units(a, a.positions[t]) + DA_PIECE : 0;
     const int s = scan(u);
+    most = max(most, __reduce_max_sync(0xffffffffu, (unsigned)u));
     if (lane == 31) scratch[warp] = s;
     __syncthreads();
     int base = before, all = before;
@@ -179,7 +188,11 @@ __device__ __forceinline__ DaList da_list(const DaArgs& a, int* sums, int* scrat
     __syncthreads();
   }
   if (threadIdx.x == 0) sums[a.T] = before;
+  if (lane == 0) scratch[warp] = (int)most;
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; w++) most = max(most, (unsigned)scratch[w]);
+  list.most = (int)most;
   return list;
 }
 
@@ -261,7 +274,7 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
   } else {
     list = da_list<DA_THREADS>(a, sums, scratch);
     const long long U = (long long)list.all() * G;
-    const int n = da_taking(U, gridDim.x);
+    const int n = da_taking(U, gridDim.x, a.T * G, list.most);
     if ((int)blockIdx.x >= n) return;
     auto first_of = [&](int i) {
       const int cut = da_cut(U, n, i);
@@ -654,7 +667,7 @@ __global__ void __launch_bounds__(THREADS) decode_fp8_join_kernel(const DaArgs a
   const DaList list = da_list<THREADS>(a, sums, scratch);
   const int sets = (a.gs + heads - 1) / heads, pair = blockIdx.x / sets, t = pair / a.pages.G, kvh = pair % a.pages.G, per = list.units_of(t);
   const long long U = (long long)list.all() * a.pages.G;
-  n_ctas = da_taking(U, n_ctas);
+  n_ctas = da_taking(U, n_ctas, a.T * a.pages.G, list.most);
   const int from = list.units_before(t) * a.pages.G + kvh * per;
   const int2 cut = da_cut_by(U, n_ctas, from, per);
   const int c0 = cut.x, c1 = cut.y;
