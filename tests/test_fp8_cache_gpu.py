@@ -520,3 +520,40 @@ def test_prefill_rows_before_the_first_position(guard_regions):
         reqs, positions = [0] * tokens[0] + [1] * tokens[1], [start[r] + i for r, t in enumerate(tokens) for i in range(t)]
         want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, 0, plain.BF16_HALF_STEP)
         assert bool(((out.cpu().double() - want).abs() <= bound).all())
+
+
+# ---- large sizes -------------------------------------------------------------------------------------------------
+
+def test_pages_past_32_bits():
+    """Written, and attended to by both kernels, at the end of a pool of more than 2^32 bytes as at its beginning."""
+    gen, H, G, d, ps = torch.Generator().manual_seed(31), 8, 4, 128, 16
+    n = (1 << 32) // kernels.fp8_page_bytes(G, ps, d) + 1000
+    pool = torch.empty((n, kernels.fp8_page_bytes(G, ps, d)), dtype=torch.uint8, device=DEV)
+    T, before, lengths = 40, [260, 0], [290, 10]
+    pages, table = a_cache(gen, lengths, G, ps, d, extra=0)
+    blocks = len(pages)
+    x = torch.randn((T, (H + 2 * G) * d), generator=gen).bfloat16().to(DEV)
+    reqs = torch.tensor([0] * 30 + [1] * 10, dtype=torch.int32, device=DEV)
+    positions = torch.tensor([260 + i for i in range(30)] + list(range(10)), dtype=torch.int32, device=DEV)
+    cu, start = torch.tensor([0, 30, 40], dtype=torch.int32, device=DEV), torch.tensor(before, dtype=torch.int32, device=DEV)
+    got = []
+    for first in (0, n - blocks):
+        pool[first:first + blocks] = pages.to(DEV)
+        at = torch.where(table >= 0, table + first, table).to(DEV)
+        slots = (at[reqs.long(), positions.long() // ps] * ps + positions % ps).to(torch.int32)
+        q, a, b = (torch.empty((T, H * d), dtype=torch.bfloat16, device=DEV) for _ in range(3))
+        kernels.rope_kv_write_fp8(x, None, q, H, G, d, 0, 1, None, None, positions, pool, slots, ps)
+        kernels.prefill_attention_fp8(q, a, pool, at, cu, start, H, G, d, ps, d ** -0.5)
+        kernels.decode_attention_fp8(q, b, pool, at, reqs, positions, H, G, d, ps, d ** -0.5)
+        kernels.check_status()
+        got.append((q, a, b, pool[first:first + blocks].clone()))
+        pool[first:first + blocks] = 255
+    assert all(torch.equal(x, y) for x, y in zip(*got)) and not bool(got[0][1].isnan().any())
+    want, bound = plain.attention(got[0][0].cpu(), got[0][3].cpu(), table, reqs.tolist(), positions.tolist(), H, G, d, ps, d ** -0.5, 0, plain.BF16_HALF_STEP)
+    assert bool(((got[0][1].cpu().double() - want).abs() <= bound).all())
+
+
+def test_prefill_many_rows(guard_regions):
+    """More rows than one round of multiprocessors has room for, in one request and in several."""
+    check_prefill([1500, 700], [100, 0], 2, 2, 64)
+    check_prefill([1200], [0], 16, 2, 64, window=300)
