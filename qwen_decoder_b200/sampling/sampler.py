@@ -34,8 +34,9 @@ def uniform_draw(seed: int, key: int, index: int) -> float:
 
 
 def without_nucleus(temperatures: Sequence[float], top_ps: Sequence[float], min_ps: Sequence[float]) -> List[float]:
-    """The temperatures with 0 for the rows that have top-p or min-p: the kernel of temperature and top-k passes over those."""
-    return [0.0 if p < 1.0 or m > 0.0 else t for t, p, m in zip(temperatures, top_ps, min_ps)]
+    """The temperatures with 0 for the rows that have top-p or min-p, as the float32 numbers that the kernels read: the kernel of temperature and
+    top-k passes over those."""
+    return [0.0 if np.float32(p) < 1.0 or np.float32(m) > 0.0 else t for t, p, m in zip(temperatures, top_ps, min_ps)]
 
 
 class Sampler:

@@ -57,3 +57,13 @@ def test_manager():
         PagedKV(2, 64, numbers="int8")
     with pytest.raises(ValueError):
         PagedKV(2, 64, v_dim=32, numbers="float8_e4m3")
+
+
+def test_rows_that_top_p_and_min_p_leave_alone():
+    """What rounds to 1 (0) where the kernels read it is no top-p (min-p) for anybody: one of the two kernels has each row."""
+    from qwen_decoder_b200.sampling import without_nucleus
+    top_p, min_p = [1.0, 1.0 - 1e-12, 0.99999999, 0.9999999, 1.0, 1.0, 0.5], [0.0, 0.0, 0.0, 0.0, 1e-60, 1e-30, 0.0]
+    assert without_nucleus([0.8] * 7, top_p, min_p) == [0.8, 0.8, 0.8, 0.0, 0.8, 0.0, 0.0]
+    for p, m, t in zip(top_p, min_p, without_nucleus([0.8] * 7, top_p, min_p)):
+        on_device = torch.tensor([p, m], dtype=torch.float32)
+        assert (t == 0.0) == bool(on_device[0] < 1 or on_device[1] > 0)
