@@ -789,7 +789,7 @@ extern "C" int qd_prefill_attention_fp8(const void* q, long long ldq, void* out,
   if (!status || !c8_make_map(&map, pages, n_pages, G, ps, d)) return QD_ERR_UNSUPPORTED;
   const AcPlan plan = ac_plan(T, R, H, G, window, max_keys, sms);
   const long long behind = plan.tiles * G - plan.whole, ctas = plan.whole + behind * plan.shares;
-  if (ctas > 0x7fffffffll || behind * (AC_ROWS / AC_JOIN_ROWS) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
+  if (ctas > 0x7fffffffll || behind * (AC_ROWS / AC_JOIN_ROWS) > 0x7fffffffll || (behind && !scratch)) return QD_ERR_UNSUPPORTED;
   const AcParams p = {(const bf16*)q, ldq, (bf16*)out, ldo, (const unsigned char*)pages, c8_page_bytes(G, ps, d), (int)n_pages, table, max_blocks, cu,
                       start, R, rows, H, G, ps, ps & (ps - 1) ? -1 : __builtin_ctz(ps), window, AC_ROWS / (H / G), scale * 1.4426950408889634f,
                       (int)plan.tiles, (int)plan.whole, plan.shares, scratch, scratch + behind * plan.shares * AC_ROWS * d, status};

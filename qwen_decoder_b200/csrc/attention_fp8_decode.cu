@@ -734,11 +734,18 @@ static DaPlan da_plan(int T, int G, int gs, int window, int max_keys, int sms) {
   return {(int)(pairs * per < at_a_time ? pairs * per : at_a_time), 0};
 }
 
-// float32 numbers of scratch memory that a launch takes
+// float32 numbers of scratch memory that a call takes: the most that a round of it does.  Rounds are DA_TOKENS and what is left, each with a plan of its own:
+// the rest may be dealt out where a full round goes in clusters
 extern "C" long long qd_decode_attention_fp8_scratch(int T, int H, int G, int d, int window, int max_keys, int sms) {
   if (T < 1 || G < 1 || H < 1) return 0;
-  const DaPlan plan = da_plan(T < DA_TOKENS ? T : DA_TOKENS, G, H / G, window, max_keys, sms);
-  return plan.cluster ? 0 : 2ll * plan.ctas * (H / G) * (d + 4);
+  long long most = 0;
+  for (const int n : {T < DA_TOKENS ? T : DA_TOKENS, T % DA_TOKENS}) {
+    if (!n) continue;
+    const DaPlan plan = da_plan(n, G, H / G, window, max_keys, sms);
+    const long long floats = plan.cluster ? 0 : 2ll * plan.ctas * (H / G) * (d + 4);
+    if (floats > most) most = floats;
+  }
+  return most;
 }
 
 template <int HD, int NT, bool CLUSTER>
@@ -791,7 +798,7 @@ static int da_launch_of(const CUtensorMap& map, const DaArgs& a, int ctas, int s
 
 // q, out: bfloat16 rows [T, H d], ``ldq`` and ``ldo`` apart; table [table_rows, max_blocks] of pages of ps tokens (a multiple of 16), its row of token t is
 // token_req[t]; the token sees the keys up to positions[t] (none below zero), the last ``window`` of them if that is positive.  No position may be
-// beyond max_keys - 1 (later keys are not seen).
+// beyond max_keys - 1 (later keys are not seen).  scratch: qd_decode_attention_fp8_scratch of the same sizes, on 16 bytes; null where that is 0.
 extern "C" int qd_decode_attention_fp8(const void* q, long long ldq, void* out, long long ldo, const void* pages, long long n_pages, const int* table,
                                        int max_blocks, int table_rows, const int* token_req, const int* positions, int T, int H, int G, int d, int ps,
                                        float scale, int window, int max_keys, float* scratch, int sms, cudaStream_t stream) {
@@ -801,6 +808,7 @@ extern "C" int qd_decode_attention_fp8(const void* q, long long ldq, void* out, 
     return QD_ERR_UNSUPPORTED;
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages) & 15) || ldq % 8 || ldo % 8) return QD_ERR_UNSUPPORTED;
   const int gs = H / G;
+  if (!scratch && qd_decode_attention_fp8_scratch(T, H, G, d, window, max_keys, sms)) return QD_ERR_UNSUPPORTED;
   // the units of a launch fit 31 bits
   if ((long long)(T < DA_TOKENS ? T : DA_TOKENS) * G * (max_keys / DA_UNIT + 2 + DA_PIECE) > 0x7fffffffll) return QD_ERR_UNSUPPORTED;
   int* status = da_status_word();
