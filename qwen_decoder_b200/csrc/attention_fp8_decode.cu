@@ -105,12 +105,12 @@ __device__ __forceinline__ int da_units(const DaArgs& a, int pos) {
 }
 // What is dealt out are the keys' units and DA_PIECE more in front of them for each pair, which stand for what a pair costs besides.  CTAs that take
 // units, of those there are: CTA i of n takes those from i U / n on, or from where the pair begins or ends that lies near: a part of a pair costs its sums' way
-// through memory
+// through memory.  n is U at most: no two cuts are the same, so every CTA that the join asks for a part of a pair has had one
 __device__ __forceinline__ int da_taking(long long U, int ctas, int pairs, int most) {
   // Pairs of as many units each, ``most``: a whole number of CTAs to a pair, so that no cut leaves a little of one (64 tokens of 8,192 keys, 28 + 4 heads,
   // 256 CTAs and 296: 95.5 and 99 us, of 4,000 51.4 and 56.2; of lengths that differ there is no such number, and fewer CTAs take longer: up to 8,000 keys 59.8 and 55.6)
   const int alike = ctas / pairs * pairs;
-  if ((long long)most * pairs == U && 5 * alike >= 4 * ctas) return alike;
+  if ((long long)most * pairs == U && 5 * alike >= 4 * ctas && alike <= U) return alike;
   return (int)(U < ctas ? U : ctas);
 }
 __device__ __forceinline__ int da_cut(long long U, int n, int i) { return (int)(U * i / n); }

@@ -78,3 +78,33 @@ def test_scratch_that_is_missing():
                                         64000, None, kernels.sm_count(), None)
     assert code == kernels.ERR_UNSUPPORTED
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lengths,H,G,d,keys", [([1001], 28, 4, 128, 100001), ([8001], 28, 4, 128, 32768), ([5001, 5001], 14, 2, 64, 65536), ([16385], 16, 2, 128, 17408),
+                                                ([200] * 3, 7, 1, 128, 40000), ([1], 28, 4, 128, 100001), ([300] * 40, 8, 2, 64, 30000)])
+def test_tokens_alike_far_below_the_most(guard_regions, lengths, H, G, d, keys):
+    """More CTAs than the keys have units, since the call allows for more keys than there are."""
+    check(lengths, H, G, d, columns=-(-keys // 16), dealt=True)
+    check(lengths, H, G, d, columns=-(-keys // 16), max_keys=keys - 5, window=700 if keys > 50000 else 0, dealt=None)
+
+
+def test_replays_of_other_lengths(guard_regions):
+    """One captured call that is dealt out, replayed with lengths short, long, alike and not."""
+    gen, H, G, d, ps = torch.Generator().manual_seed(12), 14, 2, 64, 16
+    pages, table = a_cache(gen, [9000, 9000, 9000], G, ps, d)
+    q = torch.randn((3, H * d), generator=gen).bfloat16()
+    args = pages.to(DEV), table.to(DEV), torch.arange(3, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    qd, out = q.to(DEV), torch.empty((3, H * d), dtype=torch.bfloat16, device=DEV)
+    call = lambda: kernels.decode_attention_fp8(qd, out, *args, H, G, d, ps, d ** -0.5, 0, 9000)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for positions in ([8999, 8999, 8999], [3, 3, 3], [0, 8000, 17], [500, 500, 500], [-1, -1, -1], [2500, 2500, -1], [100, 100, 100], [8999, 1, 1]):
+        args[3].copy_(torch.tensor(positions, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        want, bound = plain.attention(q, pages, table, [0, 1, 2], positions, H, G, d, ps, d ** -0.5, 0, plain.FP16_HALF_STEP)
+        off = (out.cpu().double() - want).abs()
+        assert bool((off <= bound).all()), (positions, float((off / bound).max()))
