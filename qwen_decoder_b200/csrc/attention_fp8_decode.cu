@@ -229,7 +229,7 @@ struct DaPiece {
   const int* table;
 };
 __device__ __forceinline__ void da_piece_keys(const DaArgs& a, DaPiece& p, int pos, int request) {
-  p.pos = min(pos, a.max_keys - 1);
+  p.pos = max(min(pos, a.max_keys - 1), -1);     // (what is far below zero as well: differences to it fit 32 bits)
   p.lo = da_lo_key(a, p.pos);
   p.table = a.table + (long long)min(max(request, 0), a.table_rows - 1) * a.max_blocks;
 }

@@ -108,3 +108,11 @@ def test_replays_of_other_lengths(guard_regions):
         want, bound = plain.attention(q, pages, table, [0, 1, 2], positions, H, G, d, ps, d ** -0.5, 0, plain.FP16_HALF_STEP)
         off = (out.cpu().double() - want).abs()
         assert bool((off <= bound).all()), (positions, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("keys,dealt", [(16, False), (3000, False), (9000, True)])
+def test_positions_far_below_zero(guard_regions, keys, dealt):
+    """Any position below zero is a token that sees nothing."""
+    positions = [-1, -2 ** 31, keys - 1, -2 ** 31 + 100, -200, 3, -2 ** 31 + 15]
+    check([keys], 14, 2, 64, reqs=[0] * 7, positions=positions, dealt=dealt)
+    check([keys], 14, 2, 64, reqs=[0] * 7, positions=positions, window=5)
