@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(DA_THREADS, NT == 1 ? 2 : 1) decode_fp8_kernel
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) z[0][n][j] = (KB == 2 ? z[0][n][j] + z[KB - 1][n][j] : z[0][n][j]) * fk[j >> 1] * qs[n][j & 1];
+        for (int j = 0; j < 4; j++)            // (the scales first: a large one times a score before the query's small one may leave float32)
+          z[0][n][j] = (KB == 2 ? z[0][n][j] + z[KB - 1][n][j] : z[0][n][j]) * (fk[j >> 1] * qs[n][j & 1]);
       if (border) {
 #pragma unroll
         for (int n = 0; n < NT; n++)

@@ -8,7 +8,7 @@ import torch
 
 import plain_fp8_cache as plain
 from qwen_decoder_b200 import kernels
-from test_fp8_cache_gpu import a_cache
+from test_fp8_cache_gpu import a_cache, both_kernels
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -116,3 +116,18 @@ def test_positions_far_below_zero(guard_regions, keys, dealt):
     positions = [-1, -2 ** 31, keys - 1, -2 ** 31 + 100, -200, 3, -2 ** 31 + 15]
     check([keys], 14, 2, 64, reqs=[0] * 7, positions=positions, dealt=dealt)
     check([keys], 14, 2, 64, reqs=[0] * 7, positions=positions, window=5)
+
+
+@pytest.mark.parametrize("by", [110, -60])
+@pytest.mark.parametrize("H,G,d", [(8, 2, 128), (4, 2, 64), (12, 1, 64)])
+def test_keys_times_a_power_of_two_and_queries_over_it(guard_regions, H, G, d, by):
+    """Scores are what they are however large or small keys alone are."""
+    gen, ps, lengths = torch.Generator().manual_seed(24), 16, [300, 23]
+    pages, table = a_cache(gen, lengths, G, ps, d)
+    scales = kernels.fp8_page_views(pages, G, ps, d)[1].view(torch.uint8)
+    scales[..., 0] = (scales[..., 0].int() + by).to(torch.uint8)
+    q = (torch.randn((23, H * d), generator=gen) * 2.0 ** -by).bfloat16()
+    reqs, positions, *got = both_kernels(q, pages, table, [20, 3], [280, 20], H, G, d, ps)
+    want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, 0, plain.FP16_HALF_STEP)
+    for out in got:
+        assert bool(((out - want).abs() <= bound).all())
