@@ -733,7 +733,7 @@ struct AcPlan { long long tiles, whole; int shares; };
 static AcPlan ac_plan(int T, int R, int H, int G, int window, int max_keys, int sms) {
   const int tok_tile = AC_ROWS / (H / G);
   const long long tiles = (T + tok_tile - 1) / tok_tile + (R > 1 ? R - 1 : 0), pairs = tiles * G;       // (of R requests at most)
-  const long long keys = window > 0 && window + tok_tile < max_keys ? window + tok_tile : max_keys;
+  const long long seen = (long long)window + tok_tile, keys = window > 0 && seen < max_keys ? seen : max_keys;
   const double length = (double)keys / AC_KEYS;
   const long long rest = pairs % sms;
   AcPlan plan = {tiles, pairs, 1};

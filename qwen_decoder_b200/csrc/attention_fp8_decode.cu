@@ -726,7 +726,7 @@ static int* da_status_word() {
 // 34.5 and 30.5, of up to 2,000 64.1 and 64.4.
 struct DaPlan { int ctas, cluster; };
 static DaPlan da_plan(int T, int G, int gs, int window, int max_keys, int sms) {
-  const long long keys = window > 0 && window < max_keys ? window + 15 : max_keys;
+  const long long keys = window > 0 && window < max_keys ? window + 15ll : max_keys;
   const long long per = (keys + DA_UNIT - 1) / DA_UNIT, pairs = (long long)T * G, at_a_time = (long long)(gs > 8 ? 1 : 2) * sms;
   // a CTA to a multiprocessor, at most
   int n = 1;

@@ -34,3 +34,11 @@ def test_scratch_of_single_tokens_holds_every_round(H, G, d, window):
             assert asked >= max(of_round[n] for n in rounds), (T, keys)
             more += T > 1024 and of_round[T % 1024] > of_round[1024]
     assert more                                            # (such calls are among these)
+
+
+@pytest.mark.parametrize("H,G,d", HEADS)
+def test_a_window_past_all_keys_is_none(H, G, d):
+    for window in (40000, 1 << 30, 2 ** 31 - 1):
+        for T, keys in ((1, 32000), (18, 2000), (37, 32037), (300, 700)):
+            assert prefill_scratch(T, 1, H, G, d, window, keys, SMS) == prefill_scratch(T, 1, H, G, d, 0, keys, SMS)
+            assert decode_scratch(T, H, G, d, window, keys, SMS) == decode_scratch(T, H, G, d, 0, keys, SMS)
