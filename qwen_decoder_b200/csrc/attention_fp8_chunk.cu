@@ -56,7 +56,7 @@
 #define AC_SPREAD 15                   // powers of two between scales up to which they are float16
 #define AC_DEEP 60                     // and what a tile's largest one is taken to be below the largest of all at most
 #define AC_NONE (-1e30f)               // the maximum of no scores
-#define AC_REGS 128                    // a thread's at the launch; the host looks that it is so: a split that adds up to more waits for ever
+#define AC_REGS 128                    // a thread's at the launch; the host looks that it is so
 #define AC_REGS_SOFTMAX 184            // 2 x 184 + 56 + 88 = 4 x 128
 #define AC_REGS_ISSUE 56
 #define AC_REGS_VALUES 88
@@ -760,11 +760,12 @@ static int ac_launch(const CUtensorMap& map, const AcParams& p, cudaStream_t str
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QD_ERR_UNSUPPORTED;
   if (!allowed[dev]) {
     cudaFuncAttributes of;
-    if (cudaFuncGetAttributes(&of, chunk_fp8_kernel<HD>) != cudaSuccess || of.numRegs != AC_REGS ||
+    if (cudaFuncGetAttributes(&of, chunk_fp8_kernel<HD>) != cudaSuccess ||
         cudaFuncSetAttribute(chunk_fp8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
       cudaGetLastError();
       return QD_ERR_UNSUPPORTED;
     }
+    if (of.numRegs != AC_REGS) return QD_ERR_BUILD;            // (a split that adds up to more than the launch's waits for ever)
     allowed[dev] = true;
   }
   const unsigned behind = (unsigned)(p.tiles * p.G - p.whole);

@@ -9,6 +9,8 @@
 #define QD_BF16 1
 // returned by launchers for arguments a kernel refuses (never a wrong result)
 #define QD_ERR_UNSUPPORTED 10001
+// and where a kernel, whatever the arguments, was not built as its launch has to have it
+#define QD_ERR_BUILD 10002
 // gated activations
 #define QD_ACT_SILU 0
 #define QD_ACT_GELU_TANH 2

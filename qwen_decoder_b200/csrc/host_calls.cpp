@@ -82,6 +82,7 @@ std::string sizes(const at::Tensor& t) {
 void done(int code, const char* what) {
   if (code == 0) return;
   if (code == QD_ERR_UNSUPPORTED) refuse(what, ": the kernel refuses these sizes or types");
+  if (code == QD_ERR_BUILD) refuse(what, ": the kernel was built with other registers to a thread than its warps share out");
   refuse(what, ": CUDA error ", code);
 }
 

@@ -16,7 +16,7 @@ import torch
 from .csrc.build import extension, library, loaded as _library_loaded
 
 F32, BF16 = 0, 1
-ERR_UNSUPPORTED = 10001
+ERR_UNSUPPORTED, ERR_BUILD = 10001, 10002
 
 
 class KernelError(RuntimeError):
@@ -81,6 +81,8 @@ def _check(code: int, what: str) -> None:
         return
     if code == ERR_UNSUPPORTED:
         raise KernelError(f"{what}: the kernel refuses these sizes or types")
+    if code == ERR_BUILD:
+        raise KernelError(f"{what}: the kernel was built with other registers to a thread than its warps share out")
     raise KernelError(f"{what}: CUDA error {code}")
 
 

@@ -42,3 +42,10 @@ def test_a_window_past_all_keys_is_none(H, G, d):
         for T, keys in ((1, 32000), (18, 2000), (37, 32037), (300, 700)):
             assert prefill_scratch(T, 1, H, G, d, window, keys, SMS) == prefill_scratch(T, 1, H, G, d, 0, keys, SMS)
             assert decode_scratch(T, H, G, d, window, keys, SMS) == decode_scratch(T, H, G, d, 0, keys, SMS)
+
+
+def test_a_kernel_built_otherwise_is_no_refusal_of_sizes():
+    with pytest.raises(kernels.KernelError, match="built with other registers"):
+        kernels._check(kernels.ERR_BUILD, "prefill_attention_fp8")
+    with pytest.raises(kernels.KernelError, match="sizes or types"):
+        kernels._check(kernels.ERR_UNSUPPORTED, "prefill_attention_fp8")
