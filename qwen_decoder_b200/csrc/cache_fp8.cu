@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(CW_THREADS) rope_kv_write_fp8_kernel(const CwA
     more = __any_sync(mask, more);
   }
   const unsigned byte = cw_scale_byte(m, more);
-  // 2^(127 - byte), a subnormal number for the largest byte; the product is exact
-  const float inv = byte == 255u ? __uint_as_float(0x7fc00000u) : byte == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - byte) << 23);
+  // 2^(127 - byte), of a byte up to 247 (that of the largest float32 number); the product is exact
+  const float inv = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - byte) << 23);
   float n[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) n[i] = v[i].hi * inv;
