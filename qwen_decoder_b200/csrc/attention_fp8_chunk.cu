@@ -751,6 +751,12 @@ extern "C" long long qd_prefill_attention_fp8_scratch(int T, int R, int H, int G
   const AcPlan plan = ac_plan(T, R, H, G, window, max_keys, sms);
   return (plan.tiles * G - plan.whole) * plan.shares * AC_ROWS * (d + 4);
 }
+// and the kernels of it: where some of the pairs are shared out, the one that joins their shares, too
+extern "C" int qd_prefill_attention_fp8_launches(int T, int R, int H, int G, int window, int max_keys, int sms) {
+  if (T < 1 || R < 1 || G < 1 || H < G) return 0;
+  const AcPlan plan = ac_plan(T, R, H, G, window, max_keys, sms);
+  return plan.tiles * G > plan.whole ? 2 : 1;
+}
 
 template <int HD>
 static int ac_launch(const CUtensorMap& map, const AcParams& p, cudaStream_t stream) {

@@ -748,6 +748,12 @@ extern "C" long long qd_decode_attention_fp8_scratch(int T, int H, int G, int d,
   }
   return most;
 }
+// and the kernels that it launches: a round's, and where that is dealt out the one that joins its pieces
+extern "C" int qd_decode_attention_fp8_launches(int T, int H, int G, int window, int max_keys, int sms) {
+  if (T < 1 || G < 1 || H < 1) return 0;
+  auto of_round = [&](int n) { return da_plan(n, G, H / G, window, max_keys, sms).cluster ? 1 : 2; };
+  return (T >= DA_TOKENS ? T / DA_TOKENS * of_round(DA_TOKENS) : 0) + (T % DA_TOKENS ? of_round(T % DA_TOKENS) : 0);
+}
 
 template <int HD, int NT, bool CLUSTER>
 static int da_launch(const CUtensorMap& map, const DaArgs& a, int ctas, int sms, cudaStream_t stream) {

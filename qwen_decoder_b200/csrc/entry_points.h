@@ -53,10 +53,12 @@ int qd_rope_kv_write_fp8(const void* x, int dtype, long long ld, int parts, long
                          int d, int rot, int half, const float* cos_t, const float* sin_t, int n_pos, const int* positions, void* pages,
                          long long n_pages, const int* slots, int ps, int write, int sms, cudaStream_t stream);
 long long qd_decode_attention_fp8_scratch(int T, int H, int G, int d, int window, int max_keys, int sms);
+int qd_decode_attention_fp8_launches(int T, int H, int G, int window, int max_keys, int sms);
 int qd_decode_attention_fp8(const void* q, long long ldq, void* out, long long ldo, const void* pages, long long n_pages, const int* table,
                             int max_blocks, int table_rows, const int* token_req, const int* positions, int T, int H, int G, int d, int ps, float scale,
                             int window, int max_keys, float* scratch, int sms, cudaStream_t stream);
 long long qd_prefill_attention_fp8_scratch(int T, int R, int H, int G, int d, int window, int max_keys, int sms);
+int qd_prefill_attention_fp8_launches(int T, int R, int H, int G, int window, int max_keys, int sms);
 int qd_prefill_attention_fp8(const void* q, long long ldq, void* out, long long ldo, const void* pages, long long n_pages, const int* table,
                              int max_blocks, const int* cu, const int* start, int R, int T, int rows, int H, int G, int d, int ps, float scale,
                              int window, int max_keys, float* scratch, int sms, cudaStream_t stream);

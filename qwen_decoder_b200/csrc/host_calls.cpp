@@ -155,8 +155,10 @@ decltype(qd_sample_nucleus)* g_nucleus;
 decltype(qd_rope_kv_write_fp8)* g_write;
 decltype(qd_decode_attention_fp8)* g_decode;
 decltype(qd_decode_attention_fp8_scratch)* g_decode_scratch;
+decltype(qd_decode_attention_fp8_launches)* g_decode_launches;
 decltype(qd_prefill_attention_fp8)* g_prefill;
 decltype(qd_prefill_attention_fp8_scratch)* g_prefill_scratch;
+decltype(qd_prefill_attention_fp8_launches)* g_prefill_launches;
 
 struct Plan { int cg, bn, splits; };
 // (kept by sizes and device: a few microseconds of estimates)
@@ -473,7 +475,7 @@ CALL(rope_kv_write_fp8, 15)
   Py_RETURN_NONE;
 END
 
-// (q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys)
+// (q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys) -> kernels launched
 CALL(decode_attention_fp8, 13)
   const char* what = "decode_attention_fp8";
   const at::Tensor &q = tensor(a[0], "decode_attention_fp8: q"), &out = tensor(a[1], "decode_attention_fp8: out"), &pages = tensor(a[2], "decode_attention_fp8: pages");
@@ -496,7 +498,7 @@ CALL(decode_attention_fp8, 13)
   if (!out.is_cuda() || out.get_device() != device) refuse(what, ": out is on another device");
   void *pages_at = plain(pages, at::kByte, -1, device, "decode_attention_fp8: pages"), *table_at = plain(table, at::kInt, -1, device, "decode_attention_fp8: block_table");
   void *req_at = plain(req, at::kInt, T, device, "decode_attention_fp8: token_req"), *pos_at = plain(pos, at::kInt, T, device, "decode_attention_fp8: positions");
-  if (T == 0) Py_RETURN_NONE;
+  if (T == 0) return PyLong_FromLong(0);
   if (max_keys == 0) max_keys = 1;
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   const int sms = multiprocessors(device);
@@ -506,10 +508,10 @@ CALL(decode_attention_fp8, 13)
                                                                          (const int*)table_at, (int)table.size(1), (int)table.size(0), (const int*)req_at,
                                                                          (const int*)pos_at, (int)T, h.H, h.G, h.d, h.ps, (float)scale, window, (int)max_keys,
                                                                          address(scratch), sms, stream_of(q)), what);
-  Py_RETURN_NONE;
+  return PyLong_FromLong(entry(g_decode_launches, "attention_fp8_decode", "qd_decode_attention_fp8_launches")((int)T, h.H, h.G, window, (int)max_keys, sms));
 END
 
-// (q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window, max_keys, n_tokens)
+// (q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window, max_keys, n_tokens) -> kernels launched
 CALL(prefill_attention_fp8, 14)
   const char* what = "prefill_attention_fp8";
   const at::Tensor &q = tensor(a[0], "prefill_attention_fp8: q"), &out = tensor(a[1], "prefill_attention_fp8: out"), &pages = tensor(a[2], "prefill_attention_fp8: pages");
@@ -535,7 +537,7 @@ CALL(prefill_attention_fp8, 14)
   if (!out.is_cuda() || out.get_device() != device) refuse(what, ": out is on another device");
   void *pages_at = plain(pages, at::kByte, -1, device, "prefill_attention_fp8: pages"), *table_at = plain(table, at::kInt, -1, device, "prefill_attention_fp8: block_table");
   void *cu_at = plain(cu, at::kInt, R + 1, device, "prefill_attention_fp8: cu_tokens"), *start_at = plain(start, at::kInt, R, device, "prefill_attention_fp8: start_pos");
-  if (T == 0 || R == 0) Py_RETURN_NONE;
+  if (T == 0 || R == 0) return PyLong_FromLong(0);
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   const int sms = multiprocessors(device);
   const int64_t floats = entry(g_prefill_scratch, "attention_fp8_chunk", "qd_prefill_attention_fp8_scratch")((int)T, (int)R, h.H, h.G, h.d, window,
@@ -545,7 +547,7 @@ CALL(prefill_attention_fp8, 14)
                                                                           (const int*)table_at, (int)table.size(1), (const int*)cu_at, (const int*)start_at,
                                                                           (int)R, (int)T, (int)rows, h.H, h.G, h.d, h.ps, (float)scale, window, (int)max_keys,
                                                                           address(scratch), sms, stream_of(q)), what);
-  return PyBool_FromLong(floats > 0);
+  return PyLong_FromLong(entry(g_prefill_launches, "attention_fp8_chunk", "qd_prefill_attention_fp8_launches")((int)T, (int)R, h.H, h.G, window, (int)max_keys, sms));
 END
 
 // (logits, temperature, top_k, top_p, min_p, draws, out, only)

@@ -1069,8 +1069,7 @@ def decode_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor
     positions[t] of the request whose pages are row token_req[t] of ``block_table``, the last ``window`` of them if that is not 0; with a
     negative position none, and its row of out is zeros.  ``max_keys``: no position lies beyond max_keys - 1 (None: what the table
     holds); the launch is cut by it."""
-    _launch_count[0] += 2
-    (_host or _host_calls()).decode_attention_fp8(q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys)
+    _launch_count[0] += (_host or _host_calls()).decode_attention_fp8(q, out, pages, block_table, token_req, positions, H, G, d, page_size, scale, window, max_keys)
 
 
 def prefill_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Tensor,
@@ -1080,9 +1079,8 @@ def prefill_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tenso
     (bfloat16 [T, H d], rows may lie apart; rows of no request stay as they are), at the positions from start_pos[r] on, and its pages are
     row r of ``block_table``; a token sees the keys up to its own, the last ``window`` of them if that is not 0.  ``max_keys``: no request
     has more (None: what the table holds), ``n_tokens``: nor all of them together more tokens (None: T); the launch is cut by both."""
-    joined = (_host or _host_calls()).prefill_attention_fp8(q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window, max_keys,
-                                                            n_tokens)
-    _launch_count[0] += 2 if joined else 1
+    _launch_count[0] += (_host or _host_calls()).prefill_attention_fp8(q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window,
+                                                                       max_keys, n_tokens)
 
 
 # ------------------------------------------------------------------ latent attention
@@ -2195,16 +2193,18 @@ def prompt_fns8() -> PromptFns8:
 
 def prompt_cache8(R: int, T: int, n_decode: int, H: int, G: int, d: int, window: int, decode_keys: int, prefill_keys: int):
     """(the launchers of a cache in 8 bits for the native prompt step of R requests and T tokens, the first ``n_decode`` of them single; float32
-    numbers of scratch that their attention takes)."""
+    numbers of scratch that their attention takes; kernels that it launches)."""
     dec, pre = library("attention_fp8_decode"), library("attention_fp8_chunk")
     addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value
     dec.qd_decode_attention_fp8_scratch.restype = pre.qd_prefill_attention_fp8_scratch.restype = _LL
     sms = sm_count()
     floats = max(dec.qd_decode_attention_fp8_scratch(n_decode, H, G, d, window, decode_keys, sms) if n_decode else 0,
                  pre.qd_prefill_attention_fp8_scratch(T - n_decode, R - n_decode, H, G, d, window, prefill_keys, sms))
+    launches = (dec.qd_decode_attention_fp8_launches(n_decode, H, G, window, decode_keys, sms) if n_decode else 0) + \
+        pre.qd_prefill_attention_fp8_launches(T - n_decode, R - n_decode, H, G, window, prefill_keys, sms)
     c = PromptCache8(addr(library("cache_fp8").qd_rope_kv_write_fp8), addr(dec.qd_decode_attention_fp8), addr(pre.qd_prefill_attention_fp8))
     c.table_rows, c.decode_keys, c.prefill_keys = R, decode_keys, prefill_keys
-    return c, floats
+    return c, floats, launches
 
 
 def decode_scratch(n_tokens: int, H: int, d: int, G: int, splits: int, device):

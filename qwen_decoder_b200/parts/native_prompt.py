@@ -192,7 +192,7 @@ class NativePrompt:
         if cache8:
             p.n_decode, p.token_req = nd, ctx.token_request.data_ptr()
             keys = max(1, ctx.decode_max_context)
-            p.cache8, floats = kernels.prompt_cache8(ctx.num_requests, T, nd, H, G, d, c["window"] or 0, keys, ctx.max_context)
+            p.cache8, floats, attention_launches = kernels.prompt_cache8(ctx.num_requests, T, nd, H, G, d, c["window"] or 0, keys, ctx.max_context)
             keep = torch.empty((T, H * d), dtype=bf, device=dev), torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
             p.cache8.q, p.cache8.scratch = (t.data_ptr() for t in keep)
             p.cache8.n_pos = pos.cos.shape[0] if pos is not None and c["rotary_dim"] else 0
@@ -249,7 +249,8 @@ class NativePrompt:
         p.o_part = o_part.data_ptr() if o_part is not None else None
         own = 4 if self.in_8_bits else sum(1 for plan in plans if plan)
         per_layer = LAUNCHES_PER_LAYER_8 if self.in_8_bits else OWN_LAUNCHES_PER_LAYER + own + (0 if wgu_plan else 1)
-        n_launches = len(self.entries) * (per_layer + (1 if nd else 0)) + (1 if ctx.num_wanted else 0)
+        more = attention_launches - 1 if cache8 else 1 if nd else 0         # than one launch of attention
+        n_launches = len(self.entries) * (per_layer + more) + (1 if ctx.num_wanted else 0)
         kernels.prompt_exec(p, n_launches)
         self.steps += 1
         matmul_backend.counters["library"] += (4 - own) * len(self.entries)

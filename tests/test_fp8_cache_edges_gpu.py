@@ -7,6 +7,7 @@ import torch
 
 import plain_fp8_cache as plain
 from qwen_decoder_b200 import kernels
+from test_fp8_cache_engine_gpu import folder, runner_of
 from test_fp8_cache_gpu import a_cache, check_prefill, check_write
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,41 @@ def test_write_of_the_largest_and_the_smallest_numbers(guard_regions):
     x[:, d + 7] = x[:, 2 * d + 9] = sizes.float()
     x[-1, 2 * d + 9] = -torch.finfo(torch.float32).max
     check_write(x, None, H, G, d, 0, True, ps, torch.randperm(255, generator=gen).to(torch.int32), 16)
+
+
+def test_launches_are_counted():
+    """As the kernels are: in clusters one, dealt out with the one that joins, a round of 1,024 tokens after the other."""
+    gen, H, G, d, ps = torch.Generator().manual_seed(42), 7, 1, 128, 16
+    pages, table = (t.to(DEV) for t in a_cache(gen, [2048, 40], G, ps, d))
+    wide = torch.cat([table, torch.full((2, 2000), -1, dtype=torch.int32, device=DEV)], 1)
+    q, out = (torch.zeros((1200, H * d), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    zeros = torch.zeros(1200, dtype=torch.int32, device=DEV)
+
+    def launched(call):
+        count = kernels.launches()
+        call()
+        return kernels.launches() - count
+
+    decode = lambda T, table, keys: launched(lambda: kernels.decode_attention_fp8(q[:T], out[:T], pages, table, zeros[:T], zeros[:T], H, G, d, ps, 0.1, 0, keys))
+    assert [decode(1, table, 2048), decode(1, wide, None), decode(1150, table, 2048), decode(1024, table, 2048)] == [1, 2, 3, 1]
+    prefill = lambda T, table: launched(lambda: kernels.prefill_attention_fp8(q[:T], out[:T], pages, table[:1], int32([0, T]), zeros[:1], H, G, d, ps, 0.1))
+    assert [prefill(300, table[:, :20]), prefill(3, wide)] == [1, 2]
+    assert launched(lambda: kernels.rope_kv_write_fp8(torch.zeros((4, 9 * d), device=DEV), None, q[:4], H, G, d, 0, 1, None, None, zeros[:4], pages, zeros[:4] - 1, ps)) == 1
+
+
+@pytest.mark.parametrize("size", ["64", "128"])
+def test_native_prompt_steps_count_what_the_parts_do(size, tmp_path):
+    """Both launch the same kernels: prompts alone, behind cached tokens (shares of keys and their join) and beside single tokens."""
+    from qwen_decoder_b200.engine import StepEntry
+    path, got = folder(size, tmp_path, projection_dtype="float8_e4m3", max_position_embeddings=8192), []
+    for native in (True, False):
+        runner = runner_of(path, num_pages=600)
+        if not native:
+            runner.model.native_prompt = None
+        a, b, counts = runner.open("a"), runner.open("b"), []
+        for entries in ([(a, 4000)], [(a, 3)], [(a, 1), (b, 300)], [(a, 5), (b, 1)]):
+            count = kernels.launches()
+            runner.step([StepEntry(c, [7] * n, [n - 1]) for c, n in entries])
+            counts.append(kernels.launches() - count)
+        got.append(counts)
+    assert got[0] == got[1]
