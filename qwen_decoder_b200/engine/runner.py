@@ -221,6 +221,7 @@ class ModelRunner:
             hf = h.view(np.float32)
             if nucleus:
                 h[o:o + 6 * Bp] = 0
+                hf[o + 3 * Bp:o + 4 * Bp] = 1.0          # (padding has no top-p: its rows are left alone)
                 for i, values in enumerate((*sampling[3:], temps)):
                     hf[o + (3 + i) * Bp:o + (3 + i) * Bp + R] = values
                 temps = without_nucleus(temps, *sampling[3:])

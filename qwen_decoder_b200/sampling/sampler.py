@@ -35,7 +35,7 @@ def uniform_draw(seed: int, key: int, index: int) -> float:
 
 def without_nucleus(temperatures: Sequence[float], top_ps: Sequence[float], min_ps: Sequence[float]) -> List[float]:
     """The temperatures with 0 for the rows that have top-p or min-p, as the float32 numbers that the kernels read: the kernel of temperature and
-    top-k passes over those."""
+    top-k looks for the largest logit alone in those, and ``kernels.sample_nucleus`` behind it writes their tokens over that."""
     return [0.0 if np.float32(p) < 1.0 or np.float32(m) > 0.0 else t for t, p, m in zip(temperatures, top_ps, min_ps)]
 
 

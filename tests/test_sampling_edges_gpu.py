@@ -16,3 +16,16 @@ def test_high_temperatures(guard_regions, temperature):
     z = torch.randn((4, 5000), generator=gen) * 2.5
     for k in (0, 50, 300):
         check(z, [temperature] * 4, [k] * 4, [0.999, 0.7, 1.0, 0.5], [0.0, 0.0, 0.5, 0.9], torch.rand(4, generator=gen).tolist())
+
+
+def test_padding_of_a_captured_step_has_no_top_p(tmp_path):
+    """Rows that pad a batch are nobody's: neither top-p nor min-p, so that their logits are not gone through for them."""
+    from qwen_decoder_b200.engine import StepEntry
+    from test_fp8_cache_engine_gpu import folder, runner_of
+    runner = runner_of(folder("64", tmp_path), projections=None)
+    opened = [runner.open(c) for c in "abc"]
+    runner.step([StepEntry(c, [5, 6, 7], [2]) for c in opened])
+    for top_ps, min_ps in (([0.5, 0.9, 1.0], [0.0, 0.1, 0.0]), ([1.0, 1.0, 0.25], [0.0, 0.5, 0.0])):
+        runner.step([StepEntry(c, [9], [0]) for c in opened], sampling=([0.8] * 3, [0, 5, 7], [0.3] * 3, top_ps, min_ps))
+        graph, = (g for g in runner._graphs.values() if g.nucleus)
+        assert torch.equal(graph.top_ps.cpu(), torch.tensor(top_ps + [1.0])) and torch.equal(graph.min_ps.cpu(), torch.tensor(min_ps + [0.0]))
