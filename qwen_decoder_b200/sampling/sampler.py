@@ -50,9 +50,10 @@ class Sampler:
     def sample(self, logits: torch.Tensor, temperatures: Sequence[float], top_ks: Sequence[int],
                draws: Sequence[float], top_ps: Optional[Sequence[float]] = None, min_ps: Optional[Sequence[float]] = None) -> torch.Tensor:
         R = logits.shape[0]
-        nucleus = top_ps is not None
+        nucleus = top_ps is not None or min_ps is not None
         host = torch.empty((6 if nucleus else 3, max(R, 1)), dtype=torch.float32, pin_memory=True)
         if nucleus:
+            top_ps, min_ps = [1.0] * R if top_ps is None else top_ps, [0.0] * R if min_ps is None else min_ps
             for i, values in enumerate((top_ps, min_ps, temperatures)):
                 host[3 + i, :R] = torch.tensor(list(values), dtype=torch.float32)
             temperatures = without_nucleus(temperatures, top_ps, min_ps)

@@ -29,3 +29,15 @@ def test_padding_of_a_captured_step_has_no_top_p(tmp_path):
         runner.step([StepEntry(c, [9], [0]) for c in opened], sampling=([0.8] * 3, [0, 5, 7], [0.3] * 3, top_ps, min_ps))
         graph, = (g for g in runner._graphs.values() if g.nucleus)
         assert torch.equal(graph.top_ps.cpu(), torch.tensor(top_ps + [1.0])) and torch.equal(graph.min_ps.cpu(), torch.tensor(min_ps + [0.0]))
+
+
+def test_top_p_or_min_p_alone():
+    """Either list without the other: the other's rows have none."""
+    from qwen_decoder_b200.sampling import Sampler
+    gen = torch.Generator().manual_seed(14)
+    z, sampler = (torch.randn((3, 4000), generator=gen) * 2.5).cuda(), Sampler("cuda:0")
+    args = z, [0.9, 0.0, 1.3], [0, 0, 40], [0.3, 0.5, 0.99]
+    p, m, ones, zeros = [0.5, 0.5, 1.0], [0.2, 0.1, 0.3], [1.0] * 3, [0.0] * 3
+    assert torch.equal(sampler.sample(*args, min_ps=m), sampler.sample(*args, ones, m))
+    assert torch.equal(sampler.sample(*args, top_ps=p), sampler.sample(*args, p, zeros))
+    assert torch.equal(sampler.sample(*args), sampler.sample(*args, ones, zeros))
