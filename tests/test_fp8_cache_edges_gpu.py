@@ -66,3 +66,36 @@ def test_native_prompt_steps_count_what_the_parts_do(size, tmp_path):
             counts.append(kernels.launches() - count)
         got.append(counts)
     assert got[0] == got[1]
+
+
+@pytest.mark.parametrize("H,G,d", [(16, 2, 128), (28, 4, 128), (14, 2, 64), (11, 1, 64)])
+@pytest.mark.parametrize("tokens,before,window,columns", [([130], [0], 0, 0), ([20, 1, 37], [0, 200, 3], 0, 0), ([300, 2], [100, 511], 100, 0), ([37], [4000], 0, 0),
+                                                          ([3, 40], [9000, 10], 0, 0), ([5, 9], [30, 200], 0, 3000)])
+def test_portions_weights_are_float16(guard_regions, H, G, d, tokens, before, window, columns):
+    """Where scales are near one another weights are off by half a step of float16; on scratch of exactly the size asked for, no numbers before."""
+    gen, ps, T = torch.Generator().manual_seed(43), 16, sum(tokens)
+    pages, table = a_cache(gen, [b + t for b, t in zip(before, tokens)], G, ps, d)
+    if columns:
+        table = torch.cat([table, torch.full((len(tokens), columns), -1, dtype=torch.int32)], 1)
+    q = torch.randn((T, H * d), generator=gen).bfloat16()
+    reqs = [r for r, t in enumerate(tokens) for _ in range(t)]
+    positions = [b + i for b, t in zip(before, tokens) for i in range(t)]
+    want, bound = plain.attention(q, pages, table, reqs, positions, H, G, d, ps, d ** -0.5, window, plain.FP16_HALF_STEP)
+    lib, LL, R, keys = kernels.library("attention_fp8_chunk"), ctypes.c_longlong, len(tokens), table.shape[1] * ps
+    lib.qd_prefill_attention_fp8_scratch.restype = LL
+    floats = lib.qd_prefill_attention_fp8_scratch(T, R, H, G, d, window, keys, kernels.sm_count())
+    assert (floats > 0) == (columns > 0 or keys > 1000)
+    scratch = torch.full((max(floats, 4),), math.nan, device=DEV)
+    args = q.to(DEV), torch.empty((T, H * d), dtype=torch.bfloat16, device=DEV), pages.to(DEV), table.to(DEV), int32([0] + tokens).cumsum(0).to(torch.int32), int32(before)
+    qd, out, pd, td, cu, start = args
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    code = lib.qd_prefill_attention_fp8(at(qd), LL(H * d), at(out), LL(H * d), at(pd), LL(len(pd)), at(td), table.shape[1], at(cu), at(start), R, T, T, H, G, d, ps,
+                                        ctypes.c_float(d ** -0.5), window, keys, at(scratch) if floats else None, kernels.sm_count(),
+                                        ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert code == 0
+    kernels.check_status()
+    off = (out.cpu().double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+    other = torch.empty_like(out)
+    kernels.prefill_attention_fp8(qd, other, *args[2:], H, G, d, ps, d ** -0.5, window)
+    assert torch.equal(out, other)
