@@ -707,15 +707,19 @@ __global__ void __launch_bounds__(AC_JOIN_ROWS * HD / 4) chunk_fp8_join_kernel(c
 }
 
 // ------------------------------------------------------------------------------------ host
+// the number of the first wait that ran out (made with the module, not by the first call, which may be a captured one)
+static __device__ int ac_status;
 static int* ac_status_word() {
   static int* words[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   if (!words[dev]) {
-    int* w = nullptr;
-    if (cudaMalloc(&w, sizeof(int)) != cudaSuccess) return nullptr;
-    cudaMemset(w, 0, sizeof(int));
-    words[dev] = w;
+    void* w = nullptr;
+    if (cudaGetSymbolAddress(&w, ac_status) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    words[dev] = (int*)w;
   }
   return words[dev];
 }

@@ -705,15 +705,19 @@ __global__ void __launch_bounds__(THREADS) decode_fp8_join_kernel(const DaArgs a
   da_store(a.out + (long long)t * a.ldo + (long long)(kvh * a.gs + h) * HD + f, j.s, j.inverse());
 }
 
+// the number of the first wait that ran out (made with the module, not by the first call, which may be a captured one)
+static __device__ int da_status;
 static int* da_status_word() {
   static int* words[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   if (!words[dev]) {
-    int* w = nullptr;
-    if (cudaMalloc(&w, sizeof(int)) != cudaSuccess) return nullptr;
-    cudaMemset(w, 0, sizeof(int));
-    words[dev] = w;
+    void* w = nullptr;
+    if (cudaGetSymbolAddress(&w, da_status) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    words[dev] = (int*)w;
   }
   return words[dev];
 }

@@ -1,6 +1,9 @@
 """The cache in 8 bits at the ends of its ranges: numbers of every size, scratch memory of exactly the size asked for, launches counted."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -99,3 +102,47 @@ def test_portions_weights_are_float16(guard_regions, H, G, d, tokens, before, wi
     other = torch.empty_like(out)
     kernels.prefill_attention_fp8(qd, other, *args[2:], H, G, d, ps, d ** -0.5, window)
     assert torch.equal(out, other)
+
+
+FIRST = """
+import sys, torch
+sys.path[:0] = {paths!r}
+import plain_fp8_cache as plain
+from qwen_decoder_b200 import kernels
+H, G, d, ps, DEV = 4, 2, 64, 16, "cuda:0"
+pages = plain.filled_pages(torch.Generator().manual_seed(0), 400, G, ps, d).to(DEV)
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+table, zeros, positions, slots = torch.arange(400, dtype=torch.int32, device=DEV).view(1, 400), i32([0, 0, 0]), i32([3, 50, 6000]), i32([1, 2, 3])
+x, out = torch.randn((3, 8 * d), device=DEV).bfloat16(), torch.zeros((3, H * d), dtype=torch.bfloat16, device=DEV)
+q, f, z, cu = x[:, :H * d], torch.full((3,), 0.5, device=DEV), torch.randn((3, 5000), device=DEV), i32([0, 3])
+call = {{"write": lambda: kernels.rope_kv_write_fp8(x, None, out, H, G, d, 0, 1, None, None, positions, pages, slots, ps),
+         "decode": lambda: kernels.decode_attention_fp8(q, out, pages, table, zeros, positions, H, G, d, ps, 0.1),
+         "prefill": lambda: kernels.prefill_attention_fp8(q, out, pages, table, cu, positions[2:], H, G, d, ps, 0.1),
+         "sample": lambda: kernels.sample_nucleus(z, f, zeros, f, f, f, out[0, :6].view(torch.int32))}}[sys.argv[1]]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    call()
+out.zero_()
+graph.replay()
+first = out.clone()
+call()
+assert torch.equal(first, out) and (sys.argv[1] == "sample" or float(out.float().abs().sum()) > 0)
+kernels.check_status()
+print("captured first")
+"""
+
+
+@pytest.mark.parametrize("which", ["write", "decode", "prefill", "sample"])
+def test_a_process_first_call_may_be_captured(which):
+    here = os.path.dirname(os.path.abspath(__file__))
+    got = subprocess.run([sys.executable, "-c", FIRST.format(paths=[os.path.dirname(here), here]), which], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "captured first" in got.stdout, got.stderr[-2000:]
+
+
+def test_a_wait_of_single_tokens_that_runs_out():
+    kernels.check_status()
+    kernels.wait_probe("attention_fp8_decode")
+    with pytest.raises(kernels.KernelError, match="attention_fp8_decode"):
+        kernels.check_status()
+    kernels.check_status()
