@@ -12,7 +12,7 @@
 // * Values become float16, an e4m3 number's scale over the tile's largest one, E, included, which is exact down to 2^-15 E: four warps take tiles from
 //   where the copies leave them to where the product reads them.  P is float16 too, 2^(z + log E - reference): the product's sums are of
 //   values as they are, and a row's sum of exponentials has a maximum of its own.  P is scaled so that 2^8 stands for the largest weight at the time its
-//   reference was taken, and is off by 2^-12 of itself, or by 2^-33 of that weight where that is more.  Where a tile has a scale below 2^-15 of the
+//   reference was taken, and is off by 2^-11 of itself, or by 2^-33 of that weight where that is more.  Where a tile has a scale below 2^-15 of the
 //   largest one up to it, values and P are bfloat16 as long as that is so, whose exponents take anything (E is 2^-60 of that largest one or more
 //   then, so that no exponential is lost that a row's sum has).  (P in 8 bits would
 //   be two numbers as q is, for every weight; this is 16 KB of values to a tile for all 128 rows.  Values to bfloat16, for every tile, took
@@ -24,8 +24,8 @@
 //
 // With 28 + 4 heads of 128, 2,048 tokens behind 6,144 take 252 us, of which 125 are the products at the rate of a library's; a tile of 128 x 128 takes some
 // 2,200 cycles, in which the softmax warps never wait: 1,024 are the exponentials' (16 a cycle), the rest what comes before and behind them (scores
-// from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 42 us, of which 10 are their products': three tiles of rows,
-// the last of them one token's, in 12 shares each.  512 tokens of three requests behind 655 at most, 16 + 2 heads: 17.5 us, of which the launch and the way to
+// from tensor memory, maxima, the other half's maximum, weights back).  37 tokens behind 32,000 take 41 us, of which 10 are their products': three tiles of rows,
+// the last of them one token's, in 12 shares each.  512 tokens of three requests behind 655 at most, 16 + 2 heads: 16.7 us, of which the launch and the way to
 // the first scores (rows, q's operands) are 6.
 //
 // Warps: 0..7 softmax (two threads to a row: halves of the keys and of the columns), 8 and 9 copies of keys and values, 10 MMAs, 11 scales,
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) chunk_fp8_kernel(const __grid_c
             sum += p0 + p1;
             pk[i] = at_pack(p0, p1);
           }
-        } else {                                     // (two numbers to an instruction: 2,048 tokens behind 6,144 283 -> 276 us)
+        } else {                                     // (two numbers to an instruction: 2,048 tokens behind 6,144 283 -> 274 us)
           const unsigned long long by = ac_two(mul, mul), from = ac_two(-ref, -ref);
           unsigned long long two = 0;
 #pragma unroll

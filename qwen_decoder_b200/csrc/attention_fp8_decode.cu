@@ -14,17 +14,18 @@
 //   brings its largest magnitude below 2^15: of a bfloat16 number down to 2^-25 of that nothing is lost, and what is lost below is 2^-40 of it.
 //   A key's scale multiplies its score.
 // * A value's scale joins its weight: with w_k = z_k / log 2 + s_v, the weights are 2^(w_k - W), W their own running maximum beside the
-//   scores'.  So they are numbers up to 2^8 (both maxima are followed when they grow by more than 2^8), rounded to float16 by 2^-12
-//   of themselves, and by 2^-25 of one where that is more (weights below 2^-13), whatever the scales.  Sums are float32.
+//   scores'.  So they are numbers up to 2^8 (both maxima are followed when they grow by more than 2^8), rounded to float16 by 2^-11
+//   of themselves, and by 2^-25 of one where that is more (weights below 2^-14), whatever the scales.  Sums are float32.  (w_k is one float32 number: at
+//   scores of 2^13 it costs a weight 2^-12 of itself, less than such scores' own errors.)
 // * Work, where there is much: the keys of all (token, KV head) pairs, in units of 128 (a CTA's eight warps, 16 each), are one list; every CTA
 //   takes a contiguous share of it that takes as long as the others', found from the tokens' positions alone, so that the lengths may differ as they
 //   like and a graph's replay needs nothing of the host.  A pair whose keys are one CTA's is finished by it; the others leave their sums in float32, at
 //   most two pieces to a CTA, for ``decode_fp8_join``.  No counters are shared between launches.
 // * Where there is little, a pair is a cluster's, whose CTAs have equal shares of its units and join over their shared memories.
 //
-// With 28 + 4 heads of 128: 64 tokens of 8,192 keys 95.5 us, where their 545 MB take 83 at the rate of device memory (88 in a CTA to each pair, which one
-// long token among short ones would have wait for one); 23 of 500 to 4,000 18.3, of which 8.3; one of 100,001 26.2, of which 15.8 (the rest: the launches, the way to the
-// first keys, 74 pieces to a pair).  16 + 2 heads, one token of 2,048: 6.9, nothing but latencies (position, page, keys, 16 CTAs' join).
+// With 28 + 4 heads of 128: 64 tokens of 8,192 keys 95 us, where their 545 MB take 83 at the rate of device memory (88 in a CTA to each pair, which one
+// long token among short ones would have wait for one); 23 of 500 to 4,000 18.4, of which 8.3; one of 100,001 26.3, of which 15.8 (the rest: the launches, the way to the
+// first keys, 74 pieces to a pair).  16 + 2 heads, one token of 2,048: 6.8, nothing but latencies (position, page, keys, 16 CTAs' join).
 #include "cache_fp8.cuh"
 #include "entry_points.h"
 #include "tc5_ops.cuh"

@@ -14,8 +14,8 @@
 // their loads alone, have q's heads one by one, too.  The pair's other half is a shuffle away.  Blocks of the same tokens lie together: a row of
 // x is read from one end to the other (2,048 tokens, with x out of the caches, 18.4 us, a set of heads of all tokens at a time 20.4).
 //
-// One token of 16 + 2 heads, four parts: 3.0 us, which are a launch and three trips to memory behind one another (position, table,
-// nothing to overlap them with).  2,048 of 28 + 4: 12.2 us, of which 6 are its 37 MB at the rate of device memory; the rest is the
+// One token of 16 + 2 heads, four parts: 2.8 us, which are a launch and three trips to memory behind one another (position, table,
+// nothing to overlap them with).  2,048 of 28 + 4: 11.8 us, of which 6 are its 37 MB at the rate of device memory; the rest is the
 // wait of each block for its loads, 16 to 20 warps on a multiprocessor.
 #include "cache_fp8.cuh"
 

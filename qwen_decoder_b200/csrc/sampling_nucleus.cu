@@ -23,7 +23,7 @@
 // and 33; 64 with k = 20 17.5 and 92, with 250 43 and 93, with 500 122 and 94.)
 //
 // 64 rows of 152,064 take 20 us with k of up to 100, top-p and min-p, of which 6 are their 39 MB at the rate of device memory; then bound by trips over
-// the cluster (1.5 to 3 thousand cycles each) and the list's sums.  By top-p alone 82: bound by the weights' arithmetic, 55 instructions for each logit,
+// the cluster (1.5 to 3 thousand cycles each) and the list's sums.  By top-p alone 82 (122 with a top-p of 0.925 to 0.975, row by row), by min-p alone 31.  By top-p bound by the weights' arithmetic, 55 instructions for each logit,
 // a third of them on whole numbers at half the rate, and their two additions in shared memory (40 us with the rows and no weights).  One row of
 // 151,936 by top-p 25, S = 16: seven trips over the cluster and code that runs once, out of the reach of the instructions' caches.
 #include "common.cuh"

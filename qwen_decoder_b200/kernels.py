@@ -1057,7 +1057,7 @@ def rope_kv_write_fp8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: to
     ``bias`` (float32 [(H + 2G) d] or None); q and k turned by the table rows of ``positions``, q to q_out bfloat16 [T, H d], k and v to
     their slots of ``pages`` (``fp8_pages``).  A row's scale is the smallest power of two with which its largest magnitude stays within 448,
     of the numbers before any rounding; a row with an infinity or a NaN gets the scale NaN.  A token whose slot is negative is not
-    written."""
+    written; no two tokens have the same slot, unless their rows are the same."""
     _launch_count[0] += 1
     (_host or _host_calls()).rope_kv_write_fp8(qkv, bias, q_out, H, G, d, rotary_dim, pairing, cos, sin, positions, pages, slot_map, page_size, write_kv)
 
@@ -1077,8 +1077,8 @@ def prefill_attention_fp8(q: torch.Tensor, out: torch.Tensor, pages: torch.Tenso
                           max_keys: Optional[int] = None, n_tokens: Optional[int] = None) -> None:
     """Attention of portions over a cache in 8 bits, causal: request r's tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1 of q and out
     (bfloat16 [T, H d], rows may lie apart; rows of no request stay as they are), at the positions from start_pos[r] on, and its pages are
-    row r of ``block_table``; a token sees the keys up to its own, the last ``window`` of them if that is not 0.  ``max_keys``: no request
-    has more (None: what the table holds), ``n_tokens``: nor all of them together more tokens (None: T); the launch is cut by both."""
+    row r of ``block_table``, which hold all of its positions; a token sees the keys up to its own, the last ``window`` of them if that is not 0; one at a
+    position below zero none, and its row of out is zeros.  ``max_keys``: no request has more (None: what the table holds), ``n_tokens``: nor all of them together more tokens (None: T); the launch is cut by both."""
     _launch_count[0] += (_host or _host_calls()).prefill_attention_fp8(q, out, pages, block_table, cu_tokens, start_pos, H, G, d, page_size, scale, window,
                                                                        max_keys, n_tokens)
 
